@@ -5,7 +5,7 @@ package without the built library fails (no CPU or PyTorch fallback exists).
 """
 from ._lib import Ab2Error, check, device_status, lib  # noqa: F401
 from .qlinear import QuantLinear  # noqa: F401
-from .kvcache import KVCache  # noqa: F401
+from .kvcache import KVCache, PagedKVCache, PagedStep  # noqa: F401
 from . import dispatch  # noqa: F401
 from .model import (AarambhModel, AttentionMixer, DecoderModel, InferenceEngine, LatentMixer,  # noqa: F401
                     LightningMixer, ModelConfig, MoeFfn, PolyFfn, StackConfig, StackModel)

@@ -40,6 +40,7 @@ lib = C.CDLL(LIB_PATH)
 _p = C.c_void_p
 _i = C.c_int
 _f = C.c_float
+_ll = C.c_longlong
 _pp = C.POINTER(C.c_void_p)
 
 # name -> (argtypes, restype); every symbol declared in include/aarambh_b200.h.
@@ -96,6 +97,11 @@ SIGNATURES = {
     "ab2_attention_decode_static": ([_p, _i, _p, _p, _i, _i, _f, _i, _p], _i),
     "ab2_attention_cached": ([_p, _i, _p, _p, _i, _i, _i, _f, _i, _p], _i),
     "ab2_attention_causal": ([_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _f, _i, _p], _i),
+    "ab2_rotary_apply": ([_p, _ll, _i, _p, _ll, _i, _i, _p, _i, _i, _p, _i, _i, _f, _p, _ll, _p, _ll, _i, _p], _i),
+    "ab2_paged_append": ([_p, _p, _ll, _p, _ll, _p, _ll, _i, _p, _ll, _p, _i, _i, _f, _i, _p], _i),
+    "ab2_paged_workspace": ([_i, C.POINTER(C.c_size_t)], _i),
+    "ab2_paged_attention": ([_p, _p, _ll, _i, _p, _ll, _i, _f, _p, C.c_size_t, _i, _p], _i),
+    "ab2_adjust_logits": ([_p, _ll, _i, _i, _p, _ll, _i, _p, _p, _p, _p, _i, _p, _p, _i, _p], _i),
     "ab2_model_create": ([_pp, _p, _i, _i], _i),
     "ab2_model_create_stack": ([_pp, _p, _p, _i, _i], _i),
     "ab2_model_set_form": ([_p, _p], _i),
@@ -147,6 +153,16 @@ class LayerSpec(C.Structure):
                 ("rot_dims", _i), ("rot_base", C.c_double), ("qk_norm", _i), ("scale", _f), ("v_mix", _i),
                 ("v_lambda", _f), ("decay", C.POINTER(_f)), ("ffn", _i), ("experts", _i), ("top", _i), ("ff", _i),
                 ("limit", _f), ("kv_rank", _i), ("head_gate", _i), ("glu", _i), ("routing", _i), ("shared_ff", _i), ("poly", _f * 4)]
+
+
+class Paged(C.Structure):
+    """ab2_paged."""
+    _fields_ = [("k_pages", _p), ("v_pages", _p), ("table", _p), ("lens", _p), ("starts", _p), ("pages", _i), ("page_size", _i),
+                ("kv_heads", _i), ("head_dim", _i), ("table_width", _i), ("rows", _i), ("tokens", _i),
+                ("table_stride", _ll)]
+
+
+ROTARY = {"half": 0, "interleaved": 1}
 
 
 class StackForm(C.Structure):

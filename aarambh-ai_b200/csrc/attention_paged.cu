@@ -1,0 +1,318 @@
+// Attention of a ragged batch of new tokens over a paged cache: row b's new tokens are its last ones, and its i-th sees the keys up to its own
+// position, len - new + i.
+//
+//   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(s_j - m),   s_j = scale log2(e) q k_j,   m the running maximum
+//
+// One pass over the keys: each tile of scores moves m, rescales what has been summed, and adds its weights and values.  Scores, weights,
+// their sums and the sums of values are f32.  A query that sees no key answers zeros.
+//
+// A CTA multiplies the queries of a KV head's whole group (tokens x heads of the group, up to QR rows) with a tile of 32 keys on CUDA cores;
+// keys and values come by cp.async, the next tile's while this one's are looked at.
+#include <algorithm>
+
+#include "paged.cuh"
+
+using namespace ab2;
+
+namespace ab2 {
+int paged_check(const ab2_paged *c, ab2_dtype dtype);
+PagedView paged_view(const ab2_paged *c);
+namespace {
+
+struct PagedAttnArgs {
+    PagedPlan plan;
+    const void *q, *k, *v;
+    void *out;
+    long long q_stride, o_stride;
+    int group;
+    float sl;          // scale in powers of two
+    float *acc, *ml;   // pieces: [2 ctas][QR][HD] sums, [2 ctas][QR][2] maximum and sum of weights
+    int *status;
+};
+
+constexpr int PA_THREADS = 128, PA_KEYS = 32;
+
+template <typename T, int HD, int QR> struct SimtShape {
+    static constexpr int TX = QR == 32 ? 8 : 16, RPT = QR * TX / PA_THREADS, KPT = PA_KEYS / TX, DPT = HD / TX;
+    static constexpr int KROW = HD + 16 / (int)sizeof(T);                     // a row's bank moves on by 16 bytes
+    static constexpr int BUF = PA_KEYS * KROW * (int)sizeof(T);
+    static constexpr int SMEM = 4 * BUF + QR * (HD + 4) * 4 + QR * (PA_KEYS + 1) * 4;
+};
+
+__device__ __forceinline__ void cp16(void *dst, const void *src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+__device__ __forceinline__ float4 load4(const __nv_bfloat16 *p) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+
+template <typename T, int HD, int QR>
+__global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_constant__ PagedAttnArgs a) {
+    using S = SimtShape<T, HD, QR>;
+    constexpr int TX = S::TX, RPT = S::RPT, KPT = S::KPT, DPT = S::DPT, KROW = S::KROW, CH = 16 / (int)sizeof(T);
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ long long warp_sums[PA_THREADS / 32];
+    __shared__ PagedRun found;
+    T *kbuf = (T *)smem, *vbuf = kbuf + 2 * PA_KEYS * KROW;
+    float *qs = (float *)(smem + 4 * S::BUF), *ps = qs + QR * (HD + 4);
+    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+    const PagedView &p = a.plan.p;
+    PagedRun run = paged_run<PA_THREADS>(a.plan, blockIdx.x, gridDim.x, warp_sums, &found, a.status);
+    PagedPiece w;
+    while (paged_next(a.plan, run, w)) {
+        const int base = w.r.len - w.r.count, t0 = w.q_tile * a.plan.tq, ntok = min(a.plan.tq, w.r.count - t0);
+        const int last = base + t0 + ntok - 1;   // the last key that a query of the item sees
+        const int lo = a.plan.whole ? 0 : w.k0 << a.plan.key_shift;
+        const int hi = a.plan.whole ? last + 1 : (int)min((long long)last + 1, (long long)w.k1 << a.plan.key_shift);
+        __syncthreads();
+        for (int i = threadIdx.x; i < QR * HD / 4; i += PA_THREADS) {
+            const int r = i / (HD / 4), d = i % (HD / 4) * 4, tok = r / a.group, g = r - tok * a.group;
+            float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (tok < ntok) f = load4((const T *)a.q + (size_t)(w.r.first + t0 + tok) * a.q_stride + (size_t)(w.head * a.group + g) * HD + d);
+            *reinterpret_cast<float4 *>(qs + r * (HD + 4) + d) = make_float4(f.x * a.sl, f.y * a.sl, f.z * a.sl, f.w * a.sl);
+        }
+        // rows past the last key read as zeros
+        auto fetch = [&](int key0, int buf) {
+            for (int i = threadIdx.x; i < PA_KEYS * HD / CH; i += PA_THREADS) {
+                const int j = i / (HD / CH), d = i % (HD / CH) * CH, key = key0 + j;
+                const bool in = key < hi;
+                const int at = in ? key : lo;
+                const size_t row = (((size_t)paged_page(p, w.row, at, a.status) * p.kv_heads + w.head) << p.page_shift) + (at & ((1 << p.page_shift) - 1));
+                cp16(kbuf + (buf * PA_KEYS + j) * KROW + d, (const T *)a.k + row * HD + d, in);
+                cp16(vbuf + (buf * PA_KEYS + j) * KROW + d, (const T *)a.v + row * HD + d, in);
+            }
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        };
+        float top[RPT], sum[RPT], o[RPT][DPT];
+        int lim[RPT];
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            const int tok = (ty * RPT + i) / a.group;
+            lim[i] = tok < ntok ? base + t0 + tok : -1;
+            top[i] = -INFINITY;
+            sum[i] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DPT; ++d) o[i][d] = 0.f;
+        }
+        if (lo < hi) fetch(lo, 0);
+        for (int key0 = lo, buf = 0; key0 < hi; key0 += PA_KEYS, buf ^= 1) {
+            if (key0 + PA_KEYS < hi) {
+                fetch(key0 + PA_KEYS, buf ^ 1);
+                asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+            } else {
+                asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+            }
+            __syncthreads();
+            float s[RPT][KPT];
+#pragma unroll
+            for (int i = 0; i < RPT; ++i)
+#pragma unroll
+                for (int j = 0; j < KPT; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+            for (int d = 0; d < HD; d += 4) {
+                float4 qv[RPT], kv[KPT];
+#pragma unroll
+                for (int i = 0; i < RPT; ++i) qv[i] = *reinterpret_cast<const float4 *>(qs + (ty * RPT + i) * (HD + 4) + d);
+#pragma unroll
+                for (int j = 0; j < KPT; ++j) kv[j] = load4(kbuf + (buf * PA_KEYS + tx + TX * j) * KROW + d);
+#pragma unroll
+                for (int i = 0; i < RPT; ++i)
+#pragma unroll
+                    for (int j = 0; j < KPT; ++j) s[i][j] = fmaf(qv[i].x, kv[j].x, fmaf(qv[i].y, kv[j].y, fmaf(qv[i].z, kv[j].z, fmaf(qv[i].w, kv[j].w, s[i][j]))));
+            }
+#pragma unroll
+            for (int i = 0; i < RPT; ++i) {
+                float best = top[i];
+#pragma unroll
+                for (int j = 0; j < KPT; ++j) {
+                    const int key = key0 + tx + TX * j;
+                    if (key > lim[i] || key >= hi) s[i][j] = -INFINITY;   // out of sight, whatever it holds
+                    best = fmaxf(best, s[i][j]);
+                }
+#pragma unroll
+                for (int m = TX / 2; m > 0; m >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, m));
+                const float m = best == -INFINITY ? 0.f : best, keep = exp2f(top[i] - m);
+                top[i] = best;
+                sum[i] *= keep;
+#pragma unroll
+                for (int d = 0; d < DPT; ++d) o[i][d] *= keep;
+#pragma unroll
+                for (int j = 0; j < KPT; ++j) {
+                    const int key = key0 + tx + TX * j;
+                    const float e = key > lim[i] || key >= hi ? 0.f : exp2f(s[i][j] - m);
+                    sum[i] += e;
+                    ps[(ty * RPT + i) * (PA_KEYS + 1) + tx + TX * j] = e;
+                }
+            }
+            __syncwarp();  // a row's weights come from lanes of one warp
+            // keys that no row of the thread sees may hold anything: their weight is 0, and 0 times Inf is not
+            int seen = -1;
+#pragma unroll
+            for (int i = 0; i < RPT; ++i) seen = max(seen, lim[i]);
+            const int n = min(PA_KEYS, min(hi, seen + 1) - key0);
+            for (int j = 0; j < n; ++j) {
+                float e[RPT];
+#pragma unroll
+                for (int i = 0; i < RPT; ++i) e[i] = ps[(ty * RPT + i) * (PA_KEYS + 1) + j];
+#pragma unroll
+                for (int d = 0; d < DPT; d += 4) {
+                    const float4 v = load4(vbuf + (buf * PA_KEYS + j) * KROW + tx * 4 + d * TX);
+#pragma unroll
+                    for (int i = 0; i < RPT; ++i) {
+                        if (RPT > 1 && key0 + j > lim[i]) continue;
+                        o[i][d] = fmaf(e[i], v.x, o[i][d]);
+                        o[i][d + 1] = fmaf(e[i], v.y, o[i][d + 1]);
+                        o[i][d + 2] = fmaf(e[i], v.z, o[i][d + 2]);
+                        o[i][d + 3] = fmaf(e[i], v.w, o[i][d + 3]);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        const bool all = w.k0 == 0 && w.k1 == w.k_tiles;
+        const size_t slot = 2 * (size_t)blockIdx.x + (w.k0 == 0);
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            const int r = ty * RPT + i, tok = r / a.group, g = r - tok * a.group;
+#pragma unroll
+            for (int m = TX / 2; m > 0; m >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], m);
+            if (tok >= ntok) continue;
+            if (all) {
+                const float f = top[i] == -INFINITY ? 0.f : 1.f / sum[i];
+                T *dst = (T *)a.out + (size_t)(w.r.first + t0 + tok) * a.o_stride + (size_t)(w.head * a.group + g) * HD;
+#pragma unroll
+                for (int d = 0; d < DPT; d += 4)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dst[tx * 4 + d * TX + e] = from_f32<T>(o[i][d + e] * f);
+            } else {
+                float *dst = a.acc + (slot * QR + r) * HD;
+#pragma unroll
+                for (int d = 0; d < DPT; d += 4) *reinterpret_cast<float4 *>(dst + tx * 4 + d * TX) = make_float4(o[i][d], o[i][d + 1], o[i][d + 2], o[i][d + 3]);
+                if (tx == 0) { a.ml[(slot * QR + r) * 2] = top[i]; a.ml[(slot * QR + r) * 2 + 1] = sum[i]; }
+            }
+        }
+    }
+}
+
+// The pieces of cut items: CTA c (from 1 on) finishes the item that CTA c - 1 began and did not end.
+template <typename T, int HD, int QR>
+__global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a, int ctas) {
+    __shared__ long long warp_sums[PA_THREADS / 32];
+    __shared__ PagedRun found;
+    pdl_wait();
+    const int c = blockIdx.x;   // the CTA whose last piece may begin an item
+    PagedRun run = paged_run<PA_THREADS>(a.plan, c, ctas, warp_sums, &found, nullptr);
+    PagedPiece w;
+    bool cut = false;
+    long long end = 0;
+    while (paged_next(a.plan, run, w)) {
+        cut = w.k0 == 0 && w.k1 < w.k_tiles;
+        end = run.u + (w.k_tiles - w.k1);   // the unit behind the item
+    }
+    if (!cut) return;
+    // how many CTAs hold pieces of it: c, c + 1, ... up to the one whose run reaches the item's end
+    __shared__ long long total_units;
+    {
+        long long total = 0, n;
+        for (int r0 = 0; r0 < a.plan.p.rows; r0 += PA_THREADS) {
+            const int r = r0 + threadIdx.x;
+            (void)cta_prefix<PA_THREADS>(r < a.plan.p.rows ? paged_shape(a.plan, paged_row(a.plan.p, r, nullptr)).units : 0, n, warp_sums);
+            total += n;
+        }
+        if (threadIdx.x == 0) total_units = total;
+        __syncthreads();
+    }
+    int last = c + 1;
+    while (last + 1 < ctas && total_units * (last + 1) / ctas < end) ++last;
+    const int t0 = w.q_tile * a.plan.tq, ntok = min(a.plan.tq, w.r.count - t0);
+    auto slot = [&](int i) { return 2 * (size_t)i + (i == c); };
+    auto empty = [&](int i) { return total_units * i / ctas == total_units * (i + 1) / ctas; };  // a CTA without units holds no piece
+    for (int i = threadIdx.x; i < ntok * a.group * (HD / 4); i += PA_THREADS) {
+        const int r = i / (HD / 4), d = i % (HD / 4) * 4, tok = r / a.group, g = r - tok * a.group;
+        float top = -INFINITY;
+        for (int j = c; j <= last; ++j)
+            if (!empty(j)) top = fmaxf(top, a.ml[(slot(j) * QR + r) * 2]);
+        const float m = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = c; j <= last; ++j) {
+            if (empty(j)) continue;
+            const float f = exp2f(a.ml[(slot(j) * QR + r) * 2] - m);
+            const float4 v = *reinterpret_cast<const float4 *>(a.acc + (slot(j) * QR + r) * HD + d);
+            sum = fmaf(f, a.ml[(slot(j) * QR + r) * 2 + 1], sum);
+            o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+        }
+        const float f = top == -INFINITY ? 0.f : 1.f / sum;
+        T *dst = (T *)a.out + (size_t)(w.r.first + t0 + tok) * a.o_stride + (size_t)(w.head * a.group + g) * HD + d;
+        dst[0] = from_f32<T>(o.x * f); dst[1] = from_f32<T>(o.y * f); dst[2] = from_f32<T>(o.z * f); dst[3] = from_f32<T>(o.w * f);
+    }
+}
+
+int simt_ctas() { return 2 * device_sm_count(); }
+
+template <typename T, int HD, int QR>
+int launch_simt(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
+    using S = SimtShape<T, HD, QR>;
+    static bool configured[64] = {false};  // the attribute is per device
+    int dev = 0;
+    AB2_CUDA(cudaGetDevice(&dev));
+    AB2_REQUIRE(dev >= 0 && dev < 64, AB2_ERR_BAD_ARG, "device index %d out of range", dev);
+    if (!configured[dev]) {
+        AB2_CUDA(cudaFuncSetAttribute(paged_simt_kernel<T, HD, QR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+        configured[dev] = true;
+    }
+    const int ctas = simt_ctas();
+    a.plan.tq = std::max(1, QR / a.group);
+    a.plan.key_shift = 6;
+    a.plan.whole = !workspace || bytes < (size_t)2 * ctas * QR * (HD + 2) * 4;
+    a.acc = (float *)workspace;
+    a.ml = a.acc + (size_t)2 * ctas * QR * HD;
+    paged_simt_kernel<T, HD, QR><<<ctas, PA_THREADS, S::SMEM, s>>>(a);
+    AB2_LAUNCH_CHECK();
+    if (a.plan.whole) return AB2_OK;
+    ChainedLaunches chained(true);
+    cudaError_t e = launch_kernel(paged_merge_kernel<T, HD, QR>, dim3(ctas - 1), dim3(PA_THREADS), 0, s, a, ctas);
+    if (e != cudaSuccess) return fail(AB2_ERR_CUDA, "paged attention launch failed: %s", cudaGetErrorString(e));
+    return AB2_OK;
+}
+
+template <typename T>
+int simt_attention(const PagedAttnArgs &a, int hd, int max_new, void *workspace, size_t bytes, cudaStream_t s) {
+    const bool few = max_new * (long long)a.group <= 8;
+    if (hd == 128) return few ? launch_simt<T, 128, 8>(a, workspace, bytes, s) : launch_simt<T, 128, 32>(a, workspace, bytes, s);
+    return few ? launch_simt<T, 64, 8>(a, workspace, bytes, s) : launch_simt<T, 64, 32>(a, workspace, bytes, s);
+}
+
+}  // namespace
+}  // namespace ab2
+
+AB2_API int ab2_paged_workspace(int head_dim, size_t *bytes) {
+    AB2_REQUIRE(bytes, AB2_ERR_BAD_ARG, "null argument");
+    AB2_REQUIRE(head_dim == 64 || head_dim == 128, AB2_ERR_UNSUPPORTED, "paged caches have heads of 64 or 128, not %d", head_dim);
+    *bytes = (size_t)2 * simt_ctas() * 32 * (head_dim + 2) * 4;
+    return AB2_OK;
+}
+
+AB2_API int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long long q_stride, int heads, void *out_dev, long long out_stride, int max_new, float scale,
+                                void *workspace_dev, size_t workspace_bytes, ab2_dtype dtype, ab2_stream stream) {
+    int rc = paged_check(cache, dtype);
+    if (rc != AB2_OK) return rc;
+    AB2_REQUIRE(heads > 0 && heads % cache->kv_heads == 0 && heads / cache->kv_heads <= 32, AB2_ERR_BAD_SHAPE, "%d query heads over %d KV heads: a multiple of them up to 32 is served", heads, cache->kv_heads);
+    AB2_REQUIRE(max_new > 0, AB2_ERR_BAD_SHAPE, "rows of at most %d new tokens", max_new);
+    if (cache->tokens == 0) return AB2_OK;
+    AB2_REQUIRE(q_dev && out_dev, AB2_ERR_BAD_ARG, "null argument");
+    const long long row = (long long)heads * cache->head_dim;
+    AB2_REQUIRE(q_stride >= row && out_stride >= row, AB2_ERR_BAD_SHAPE, "a token's heads lie one after the other, and tokens do not overlap");
+    const size_t esize = dtype_size(dtype);
+    AB2_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev | (uintptr_t)workspace_dev) & 15) == 0 && ((q_stride | out_stride) * esize & 15) == 0, AB2_ERR_BAD_ALIGN, "queries, outputs and their rows must be 16-byte aligned");
+    PagedAttnArgs a = {};
+    a.plan.p = paged_view(cache);
+    a.q = q_dev; a.k = cache->k_pages; a.v = cache->v_pages; a.out = out_dev; a.q_stride = q_stride; a.o_stride = out_stride;
+    a.group = heads / cache->kv_heads; a.sl = scale * 1.44269504088896341f;
+    rc = device_status_word(&a.status);
+    if (rc != AB2_OK) return rc;
+    if (dtype == AB2_F32) return simt_attention<float>(a, cache->head_dim, max_new, workspace_dev, workspace_bytes, (cudaStream_t)stream);
+    return simt_attention<__nv_bfloat16>(a, cache->head_dim, max_new, workspace_dev, workspace_bytes, (cudaStream_t)stream);
+}

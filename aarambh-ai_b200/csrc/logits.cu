@@ -1,0 +1,140 @@
+// Rules of a sampler on the logits of a batch: with c the times token v occurs in the row's history,
+//
+//   z <- z / rho if z > 0 else z rho       where c > 0        (repetition)
+//   z <- z - presence - frequency c        where c > 0
+//   z <- z + bias_v                        where v is biased
+//   z <- -inf                              where the row's mask has v's bit 0
+//
+// in f32, rounded once.  A CTA has a slice of a row's vocabulary: it counts the history's tokens of its slice in shared memory (integer
+// additions, whose order changes nothing), notes which entry of the bias list is each token's last, and then passes over
+// the slice once, 16 bytes a load.  Every CTA of a row reads the row's history, from L2 after the first.  Bound by HBM for large
+// batches, by the launch, the clearing of the counts and the history's latency for small ones.
+#include <algorithm>
+
+#include "common.cuh"
+
+using namespace ab2;
+
+namespace ab2 {
+int device_sm_count();
+namespace {
+
+constexpr int LG_THREADS = 256;
+
+struct LogitArgs {
+    const void *logits;
+    void *out;
+    long long stride;
+    int vocab, slice;
+    const int *history, *lengths;
+    long long history_stride;
+    int history_width;
+    const float *rules;
+    const int *bias_ids;
+    const float *bias_values;
+    int biases;
+    const uint32_t *allowed;
+    int words;
+};
+
+// One token's logit.
+__device__ __forceinline__ float ruled(float z, int count, float rho, float presence, float frequency) {
+    if (count == 0) return z;
+    z = z > 0.f ? z / rho : z * rho;
+    return z - (presence + frequency * (float)count);
+}
+
+template <typename T, int V>  // V elements a load
+__global__ void __launch_bounds__(LG_THREADS) adjust_logits_kernel(const __grid_constant__ LogitArgs a) {
+    extern __shared__ __align__(16) int counts[];  // [slice], then with biases [slice]: the list's entry for the token, + 1
+    const int row = blockIdx.y, first = blockIdx.x * a.slice, n = min(a.slice, a.vocab - first);
+    int *entry = counts + a.slice;
+    const int tables = (a.history ? a.slice : 0) + (a.biases ? a.slice : 0);
+    int *table = a.history ? counts : entry;
+    for (int i = threadIdx.x * 4; i < tables; i += LG_THREADS * 4) *reinterpret_cast<int4 *>(table + i) = make_int4(0, 0, 0, 0);
+    __syncthreads();
+    float rho = 1.f, presence = 0.f, frequency = 0.f;
+    if (a.history) {
+        rho = a.rules[3 * row]; presence = a.rules[3 * row + 1]; frequency = a.rules[3 * row + 2];
+        const int *h = a.history + row * a.history_stride;
+        const int len = min(a.lengths ? a.lengths[row] : a.history_width, a.history_width);
+        for (int i = threadIdx.x; i < len; i += LG_THREADS * 8) {
+            int v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = i + u * LG_THREADS < len ? h[i + u * LG_THREADS] - first : -1;
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if ((unsigned)v[u] < (unsigned)n) atomicAdd(counts + v[u], 1);
+        }
+    }
+    for (int i = threadIdx.x; i < a.biases; i += LG_THREADS) {
+        const int v = a.bias_ids[(size_t)row * a.biases + i] - first;
+        if ((unsigned)v < (unsigned)n) atomicMax(entry + v, i + 1);
+    }
+    __syncthreads();
+    const T *in = (const T *)a.logits + row * a.stride + first;
+    T *out = (T *)a.out + (size_t)row * a.vocab + first;
+    const uint32_t *mask = a.allowed ? a.allowed + (size_t)row * a.words + (first >> 5) : nullptr;
+    const float *bias = a.bias_values + (size_t)row * a.biases;
+    for (int i = threadIdx.x * V; i < n; i += LG_THREADS * V) {
+        alignas(16) T e[V];
+        if constexpr (V > 1) *reinterpret_cast<uint4 *>(e) = *reinterpret_cast<const uint4 *>(in + i);
+        else e[0] = in[i];
+        const uint32_t bits = mask ? mask[i >> 5] >> (i & 31) : 0xffffffffu;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float z = to_f32(e[j]);
+            if (a.history) z = ruled(z, counts[i + j], rho, presence, frequency);
+            if (a.biases) {
+                const int b = entry[i + j];
+                if (b) z += bias[b - 1];
+            }
+            e[j] = from_f32<T>((bits >> j) & 1 ? z : -INFINITY);
+        }
+        if constexpr (V > 1) *reinterpret_cast<uint4 *>(out + i) = *reinterpret_cast<const uint4 *>(e);
+        else out[i] = e[0];
+    }
+}
+
+template <typename T>
+int launch_adjust(LogitArgs a, int rows, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const bool wide = a.vocab % V == 0 && a.stride % V == 0 && (((uintptr_t)a.logits | (uintptr_t)a.out) & 15) == 0;
+    // Slices of 4096 tokens, smaller ones where those are fewer than two CTAs an SM; 512 at least, so that a thread has a load of its own.
+    a.slice = 4096;
+    while (a.slice > 512 && (long long)rows * ((a.vocab + a.slice - 1) / a.slice) < 2 * device_sm_count()) a.slice /= 2;
+    const dim3 grid((a.vocab + a.slice - 1) / a.slice, rows);
+    const size_t smem = (size_t)a.slice * 4 * (a.biases ? 2 : 1);
+    if (wide) adjust_logits_kernel<T, V><<<grid, LG_THREADS, smem, s>>>(a);
+    else adjust_logits_kernel<T, 1><<<grid, LG_THREADS, smem, s>>>(a);
+    AB2_LAUNCH_CHECK();
+    return AB2_OK;
+}
+
+}  // namespace
+}  // namespace ab2
+
+AB2_API int ab2_adjust_logits(const void *logits_dev, long long stride, int rows, int vocab, const int *history_dev, long long history_stride, int history_width,
+                              const int *lengths_dev, const float *rules_dev, const int *bias_ids_dev, const float *bias_values_dev, int biases, const uint32_t *allowed_dev,
+                              void *out_dev, ab2_dtype dtype, ab2_stream stream) {
+    AB2_REQUIRE(rows >= 0 && vocab > 0, AB2_ERR_BAD_SHAPE, "logits of %d rows, %d tokens", rows, vocab);
+    AB2_REQUIRE(rows <= 65535, AB2_ERR_BAD_SHAPE, "%d rows are more than the 65535 of a launch", rows);
+    AB2_REQUIRE(dtype == AB2_F32 || dtype == AB2_F16 || dtype == AB2_BF16, AB2_ERR_BAD_DTYPE, "unsupported dtype %d", (int)dtype);
+    if (rows == 0) return AB2_OK;
+    AB2_REQUIRE(logits_dev && out_dev, AB2_ERR_BAD_ARG, "null argument");
+    AB2_REQUIRE(stride >= vocab, AB2_ERR_BAD_SHAPE, "rows of %d logits lie %lld apart", vocab, stride);
+    AB2_REQUIRE((((uintptr_t)logits_dev | (uintptr_t)out_dev) & (dtype_size(dtype) - 1)) == 0, AB2_ERR_BAD_ALIGN, "logits must lie on their elements");
+    AB2_REQUIRE(history_width >= 0 && biases >= 0, AB2_ERR_BAD_SHAPE, "history of %d, %d biases", history_width, biases);
+    AB2_REQUIRE(history_width == 0 || (history_dev && rules_dev && history_stride >= history_width), AB2_ERR_BAD_ARG, "a history needs its tokens, rows that do not overlap, and rules");
+    AB2_REQUIRE(biases == 0 || (bias_ids_dev && bias_values_dev), AB2_ERR_BAD_ARG, "null bias list");
+    LogitArgs a = {};
+    a.logits = logits_dev; a.out = out_dev; a.stride = stride; a.vocab = vocab;
+    if (history_width > 0) { a.history = history_dev; a.history_stride = history_stride; a.history_width = history_width; a.lengths = lengths_dev; a.rules = rules_dev; }
+    a.bias_ids = bias_ids_dev; a.bias_values = bias_values_dev; a.biases = biases;
+    a.allowed = allowed_dev; a.words = (vocab + 31) / 32;
+    switch (dtype) {
+    case AB2_F32: return launch_adjust<float>(a, rows, (cudaStream_t)stream);
+    case AB2_F16: return launch_adjust<__half>(a, rows, (cudaStream_t)stream);
+    default: return launch_adjust<__nv_bfloat16>(a, rows, (cudaStream_t)stream);
+    }
+}

@@ -6,6 +6,8 @@ allocated, inputs are borrowed, tensors must be CUDA and are made contiguous.
 from __future__ import annotations
 
 import ctypes as C
+import math
+from dataclasses import dataclass
 
 import torch
 
@@ -227,3 +229,278 @@ class MoeExperts:
         check(lib.ab2_moe_forward(C.byref(self.spec), self.router._h, self.gate._h, self.up._h, self.down._h, x.data_ptr(), T,
                                   dtype_code(x.dtype), out.data_ptr(), self._work.data_ptr(), stream_ptr()))
         return out
+
+
+# -- a serving step over a paged cache (``kvcache.PagedKVCache`` keeps the pages) ---------------------
+
+@dataclass
+class RotaryScaling:
+    """How frequencies are changed for contexts longer than the one learnt, ``factor`` times as long.  ``linear``: every
+    frequency divided by it.  ``base``: the base times factor ** (dims / (dims - 2)), so that the fastest pair stays and the slowest is
+    divided by it.  ``ramp``: pairs that turn at least ``high`` times over the ``original`` context stay, those that turn at most
+    ``low`` times are divided, the others lie between, linearly in their turns; magnitude 0.1 ln(factor) + 1."""
+    kind: str
+    factor: float
+    original: int = 0
+    low: float = 1.0
+    high: float = 32.0
+
+    @property
+    def magnitude(self) -> float:
+        return 0.1 * math.log(self.factor) + 1.0 if self.kind == "ramp" and self.factor > 1 else 1.0
+
+
+def rotary_frequencies(dims: int, base: float = 10000.0, scaling: RotaryScaling | None = None, device="cuda") -> torch.Tensor:
+    """[dims / 2] f64: the radians a position turns each pair by, base ** (-2i / dims), scaled."""
+    if dims < 2 or dims % 2:
+        raise _lib.Ab2Error(-1, f"an even number of dimensions is rotated, got {dims}")
+    if not base > 0:
+        raise _lib.Ab2Error(-7, f"the base of the frequencies must be positive, got {base}")
+    if scaling is not None:
+        if scaling.kind not in ("linear", "base", "ramp") or not scaling.factor > 0:
+            raise _lib.Ab2Error(-7, f"unknown scaling {scaling}")
+        if scaling.kind == "base":
+            if dims == 2:
+                raise _lib.Ab2Error(-1, "a single pair has no base to scale")
+            base = base * scaling.factor ** (dims / (dims - 2))
+    f = torch.pow(torch.tensor(float(base), dtype=torch.float64), -2.0 * torch.arange(dims // 2, dtype=torch.float64) / dims)
+    if scaling is not None and scaling.kind == "linear":
+        f = f / scaling.factor
+    elif scaling is not None and scaling.kind == "ramp":
+        if scaling.original <= 0 or not scaling.high > scaling.low:
+            raise _lib.Ab2Error(-7, f"a ramp needs the original context and high > low, got {scaling}")
+        turns = scaling.original * f / (2 * math.pi)
+        keep = ((turns - scaling.low) / (scaling.high - scaling.low)).clamp(0, 1)
+        f = f * keep + f / scaling.factor * (1 - keep)
+    return f.to(device)
+
+
+def _on_device(*tensors) -> None:
+    """Kernels run on the current device's stream: every tensor has to be there."""
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.get_device() != torch.cuda.current_device()):
+            raise _lib.Ab2Error(-7, f"tensors must be on the current CUDA device (this library has no CPU path), got one on {t.device}")
+
+
+def _typed(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str) -> torch.Tensor:
+    if t.dtype != dtype:
+        raise _lib.Ab2Error(-3, f"{what} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise _lib.Ab2Error(-1, f"{what} must have shape {list(shape)}, got {list(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _heads(t: torch.Tensor, what: str):
+    """A [tokens, heads, dim] tensor whose tokens may lie apart (q of a fused projection): itself or a copy, and the elements
+    from one token to the next."""
+    if t.dim() != 3:
+        raise _lib.Ab2Error(-1, f"{what} must be [tokens, heads, head_dim], got {list(t.shape)}")
+    n, h, d = t.shape
+    s0, s1, s2 = t.stride()
+    if (s2 == 1 or d == 1) and (s1 == d or h == 1) and (s0 >= h * d or n < 2):
+        return t, (s0 if n > 1 else h * d)
+    return t.contiguous(), h * d
+
+
+def _rotation(frequencies, layout: str, dim: int):
+    if layout not in _lib.ROTARY:
+        raise _lib.Ab2Error(-7, f"unknown rotary layout {layout!r}")
+    if frequencies is None:
+        return None, 0
+    n = frequencies.numel()
+    if 2 * n > dim:
+        raise _lib.Ab2Error(-1, f"{n} pairs do not fit a head of {dim}")
+    return _typed(frequencies, torch.float64, (n,), "frequencies"), 2 * n
+
+
+def rotary_apply(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, frequencies: torch.Tensor, layout: str = "half",
+                 magnitude: float = 1.0, out=None):
+    """q [tokens, heads, dim] and k [tokens, kv_heads, dim] (or None), each token rotated by its position (``positions`` [tokens],
+    int32 or int64); pairs ``half`` (i, i + n) or ``interleaved`` (2i, 2i + 1), n the count of ``frequencies`` (``rotary_frequencies``).
+    ``out``: a pair of tensors for the results, which may be q and k."""
+    _on_device(q, k, positions, frequencies)
+    q, qs = _heads(q, "q")
+    n, h, d = q.shape
+    ks = kv = 0
+    if k is not None:
+        k, ks = _heads(k, "k")
+        kv = k.shape[1]
+        if k.shape[0] != n or k.shape[2] != d or k.dtype != q.dtype:
+            raise _lib.Ab2Error(-1, f"q {list(q.shape)} {q.dtype} and k {list(k.shape)} {k.dtype} do not match")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise _lib.Ab2Error(-3, f"positions must be int32 or int64, got {positions.dtype}")
+    positions = _typed(positions, positions.dtype, (n,), "positions")
+    frequencies, rot = _rotation(frequencies, layout, d)
+    if out is None:
+        qo, qos, ko, kos = torch.empty((n, h, d), dtype=q.dtype, device=q.device), h * d, None, kv * d
+        if k is not None:
+            ko = torch.empty((n, kv, d), dtype=q.dtype, device=q.device)
+    else:
+        qo, qos = _result(out[0], q, "out[0]")
+        ko, kos = _result(out[1], k, "out[1]") if k is not None else (None, 0)
+    check(lib.ab2_rotary_apply(q.data_ptr(), qs, h, k.data_ptr() if k is not None else None, ks, kv, d, positions.data_ptr(),
+                               positions.dtype == torch.int64, n, frequencies.data_ptr() if frequencies is not None else None, rot, _lib.ROTARY[layout], magnitude,
+                               qo.data_ptr(), qos, ko.data_ptr() if ko is not None else None, kos, dtype_code(q.dtype), stream_ptr()))
+    return qo, ko
+
+
+def _result(out: torch.Tensor, like: torch.Tensor, what: str):
+    """A caller's tensor for a result, and its token stride; it is written in place, so no copy will do."""
+    _on_device(out)
+    if out.shape != like.shape or out.dtype != like.dtype:
+        raise _lib.Ab2Error(-1, f"{what} must be {like.dtype} {list(like.shape)}, got {out.dtype} {list(out.shape)}")
+    same, stride = _heads(out, what)
+    if same is not out:
+        raise _lib.Ab2Error(-1, f"{what}'s heads must lie one after the other")
+    return out, stride
+
+
+def _paged(k_pages, v_pages, table, lens, starts, tokens: int):
+    """ab2_paged of a layer's pages and a batch, and the tensors it points to."""
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+        raise _lib.Ab2Error(-1, f"pages must be two tensors [pages, kv_heads, page_size, head_dim] of one type, got {list(k_pages.shape)} and {list(v_pages.shape)}")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise _lib.Ab2Error(-1, "pages must be contiguous")
+    if table.dim() != 2 or table.dtype != torch.int32:
+        raise _lib.Ab2Error(-1, f"the table must be int32 [rows, pages], got {table.dtype} {list(table.shape)}")
+    rows, width = table.shape
+    if width > 1 and table.stride(1) != 1 or rows > 1 and table.stride(0) < width:
+        table = table.contiguous()
+    lens = _typed(lens, torch.int32, (rows,), "lens")
+    if starts is not None:
+        starts = _typed(starts, torch.int32, (rows + 1,), "starts")
+    pages, kv, page, dim = k_pages.shape
+    c = _lib.Paged(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lens.data_ptr(), starts.data_ptr() if starts is not None else None,
+                   pages, page, kv, dim, width, rows, tokens, table.stride(0) if rows > 1 else width)
+    return c, (table, lens, starts)
+
+
+def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                 starts: torch.Tensor | None = None, q: torch.Tensor | None = None, frequencies: torch.Tensor | None = None, layout: str = "half",
+                 magnitude: float = 1.0, out: torch.Tensor | None = None):
+    """Writes the new tokens' k (rotated at their positions in their rows, as they are without ``frequencies``) and v
+    [tokens, kv_heads, dim] to the pages that ``table`` [rows, pages] names; ``lens`` [rows] are the rows' tokens with the new ones,
+    ``starts`` [rows + 1] where a row's new tokens begin (None: one a row).  Returns the rotated q [tokens, heads, dim], if any."""
+    _on_device(k_pages, v_pages, k, v, table, lens, starts, q, frequencies)
+    k, ks = _heads(k, "k")
+    v, vs = _heads(v, "v")
+    n, kv, d = k.shape
+    if v.shape != k.shape or v.dtype != k.dtype or k.dtype != k_pages.dtype:
+        raise _lib.Ab2Error(-1, f"k {list(k.shape)} {k.dtype} and v {list(v.shape)} {v.dtype} do not match each other and pages of {k_pages.dtype}")
+    c, _keep = _paged(k_pages, v_pages, table, lens, starts, n)
+    if (kv, d) != (c.kv_heads, c.head_dim):
+        raise _lib.Ab2Error(-1, f"k has {kv} heads of {d}, the pages {c.kv_heads} of {c.head_dim}")
+    frequencies, rot = _rotation(frequencies, layout, d)
+    h = qs = qos = 0
+    qo = None
+    if q is not None:
+        q, qs = _heads(q, "q")
+        h = q.shape[1]
+        if q.shape[0] != n or q.shape[2] != d or q.dtype != k.dtype:
+            raise _lib.Ab2Error(-1, f"q {list(q.shape)} {q.dtype} does not match k {list(k.shape)} {k.dtype}")
+        if out is None:
+            qo, qos = torch.empty((n, h, d), dtype=q.dtype, device=q.device), h * d
+        else:
+            qo, qos = _result(out, q, "out")
+    check(lib.ab2_paged_append(C.byref(c), k.data_ptr(), ks, v.data_ptr(), vs, q.data_ptr() if q is not None else None, qs, h,
+                               qo.data_ptr() if qo is not None else None, qos, frequencies.data_ptr() if frequencies is not None else None, rot,
+                               _lib.ROTARY[layout], magnitude, dtype_code(k.dtype), stream_ptr()))
+    return qo
+
+
+_paged_bytes = {}   # head_dim, device -> bytes of a workspace
+
+
+def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float,
+                    starts: torch.Tensor | None = None, max_new: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """q [tokens, heads, dim]: each row's new tokens, whose keys and values have been appended, attend to the row's keys up to their
+    own; table, lens and starts as in ``paged_append``.  ``max_new`` bounds the new tokens of a row (None: not known); it picks
+    kernels and changes no result.  Tokens behind the last row are left as ``out`` holds them."""
+    _on_device(q, k_pages, v_pages, table, lens, starts)
+    q, qs = _heads(q, "q")
+    n, h, d = q.shape
+    if q.dtype != k_pages.dtype:
+        raise _lib.Ab2Error(-3, f"queries of {q.dtype} over pages of {k_pages.dtype}")
+    c, _keep = _paged(k_pages, v_pages, table, lens, starts, n)
+    if d != c.head_dim:
+        raise _lib.Ab2Error(-1, f"queries have heads of {d}, the pages of {c.head_dim}")
+    if (q.data_ptr() | qs * q.element_size()) & 15:
+        q, qs = q.clone(memory_format=torch.contiguous_format), h * d
+    if out is None:
+        out, os = torch.empty((n, h, d), dtype=q.dtype, device=q.device), h * d
+    else:
+        out, os = _result(out, q, "out")
+    if max_new is None:
+        max_new = 1 if starts is None else max(n, 1)
+    key = (d, q.get_device())
+    if key not in _paged_bytes:
+        size = C.c_size_t()
+        check(lib.ab2_paged_workspace(d, C.byref(size)))
+        _paged_bytes[key] = size.value
+    work = torch.empty(_paged_bytes[key], dtype=torch.uint8, device=q.device)
+    check(lib.ab2_paged_attention(C.byref(c), q.data_ptr(), qs, h, out.data_ptr(), os, max_new, scale, work.data_ptr(), work.numel(),
+                                  dtype_code(q.dtype), stream_ptr()))
+    return out
+
+
+def allowed_words(mask: torch.Tensor) -> torch.Tensor:
+    """A truth value for every token [rows, vocab] as the words that ``adjust_logits`` takes: int32 [rows, ceil(vocab / 32)]."""
+    rows, vocab = mask.shape
+    bits = torch.zeros((rows, (vocab + 31) // 32 * 32), dtype=torch.int64, device=mask.device)
+    bits[:, :vocab] = mask
+    words = (bits.view(rows, -1, 32) << torch.arange(32, device=mask.device)).sum(-1)
+    return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+
+
+def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, lengths: torch.Tensor | None = None, rules: torch.Tensor | None = None,
+                  bias_ids: torch.Tensor | None = None, bias_values: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """The rules of a sampler on logits [rows, vocab]; ``argmax`` picks from the result.
+
+    With c the times a token occurs in ``history`` [rows, n] int32 (the first ``lengths`` [rows] of a row, None: all; ids outside the
+    vocabulary are passed over) and ``rules`` [rows, 3] f32 = (repetition > 0, presence, frequency): a token with c > 0 has its logit divided
+    by the repetition where it is positive, else multiplied, then lowered by presence + frequency c.  Then ``bias_values`` [rows, m] f32 are
+    added at ``bias_ids`` [rows, m] int32 (of an id named twice the last counts), and tokens whose bit in ``allowed``
+    [rows, ceil(vocab / 32)] int32 (``allowed_words``) is 0 become -inf.  ``out`` may be the logits."""
+    _on_device(logits, history, lengths, rules, bias_ids, bias_values, allowed, out)
+    if logits.dim() != 2:
+        raise _lib.Ab2Error(-1, f"logits must be [rows, vocab], got {list(logits.shape)}")
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < vocab:
+        logits = logits.contiguous()
+    stride = logits.stride(0) if rows > 1 else vocab
+    hp = lp = rp = bp = vp = ap = None
+    hs = width = biases = 0
+    if history is not None:
+        if rules is None:
+            raise _lib.Ab2Error(-7, "a history needs rules")
+        if history.dim() != 2 or history.shape[0] != rows or history.dtype != torch.int32:
+            raise _lib.Ab2Error(-1, f"history must be int32 [{rows}, tokens], got {history.dtype} {list(history.shape)}")
+        width = history.shape[1]
+        if width > 1 and history.stride(1) != 1 or rows > 1 and history.stride(0) < width:
+            history = history.contiguous()
+        hp, hs = history.data_ptr(), (history.stride(0) if rows > 1 else width)
+        rules = _typed(rules, torch.float32, (rows, 3), "rules")
+        rp = rules.data_ptr()
+        if lengths is not None:
+            lengths = _typed(lengths, torch.int32, (rows,), "lengths")
+            lp = lengths.data_ptr()
+    elif lengths is not None or rules is not None:
+        raise _lib.Ab2Error(-7, "lengths and rules are those of a history")
+    if (bias_ids is None) != (bias_values is None):
+        raise _lib.Ab2Error(-7, "biases need both ids and values")
+    if bias_ids is not None:
+        biases = bias_ids.shape[-1]
+        bias_ids = _typed(bias_ids, torch.int32, (rows, biases), "bias_ids")
+        bias_values = _typed(bias_values, torch.float32, (rows, biases), "bias_values")
+        bp, vp = bias_ids.data_ptr(), bias_values.data_ptr()
+    if allowed is not None:
+        allowed = _typed(allowed, torch.int32, (rows, (vocab + 31) // 32), "allowed")
+        ap = allowed.data_ptr()
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or not out.is_contiguous():
+        raise _lib.Ab2Error(-1, f"out must be contiguous {logits.dtype} {list(logits.shape)}")
+    check(lib.ab2_adjust_logits(logits.data_ptr(), stride, rows, vocab, hp, hs, width, lp, rp, bp, vp, biases, ap, out.data_ptr(),
+                                dtype_code(logits.dtype), stream_ptr()))
+    return out

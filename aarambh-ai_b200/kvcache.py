@@ -9,6 +9,7 @@ layers, snapshot / restore).  Storage is f32, bf16 or per-token-per-head INT8.
 from __future__ import annotations
 
 import ctypes as C
+from dataclasses import dataclass
 
 import torch
 
@@ -118,3 +119,132 @@ class KVCache:
                 self._h = None
         except Exception:
             pass
+
+
+@dataclass
+class PagedStep:
+    """The new tokens of some rows of a paged cache, on the device: what ``paged_append`` and ``attention_paged`` read."""
+    rows: list
+    new: list                     # new tokens of each
+    table: torch.Tensor           # [rows, pages]
+    lens: torch.Tensor            # [rows], new tokens included
+    starts: torch.Tensor          # [rows + 1]
+    tokens: int                   # that q, k and v have room for
+    max_new: int
+    packed: torch.Tensor          # the three above
+
+
+class PagedKVCache:
+    """Keys and values in pages of one pool that the sequences share: a sequence holds as many as its tokens need, in any order, where
+    ``KVCache`` gives each the same capacity for good.  ``k`` and ``v`` are [layers, pages, kv_heads, page_size, head_dim] (f32 or bf16).
+    A pass over some rows: ``step`` takes the pages it needs, then for every layer ``append`` and ``attention``, at its end ``commit``.
+    Calls on a cache go on one stream, or are ordered by the caller."""
+
+    def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, batch: int = 1, n_layers: int = 1, dtype: str = "bf16", device="cuda"):
+        if dtype not in ("f32", "bf16"):
+            raise _lib.Ab2Error(-3, f"paged caches hold f32 or bf16, not {dtype}")
+        if page_size not in (16, 32, 64, 128, 256) or head_dim not in (64, 128):
+            raise _lib.Ab2Error(-8, f"pages of {page_size} tokens, heads of {head_dim}: 16, 32, 64, 128 or 256 tokens and heads of 64 or 128 are served")
+        if min(pages, kv_heads, batch, n_layers) <= 0:
+            raise _lib.Ab2Error(-1, f"paged cache of {pages} pages, {kv_heads} heads, {batch} rows, {n_layers} layers")
+        self.page_size, self.kv_heads, self.head_dim, self.batch, self.n_layers, self.dtype = page_size, kv_heads, head_dim, batch, n_layers, dtype
+        self.k, self.v = (torch.zeros((n_layers, pages, kv_heads, page_size, head_dim), dtype=torch.float32 if dtype == "f32" else torch.bfloat16, device=device)
+                          for _ in range(2))
+        self._free = list(range(pages - 1, -1, -1))
+        self._pages = [[] for _ in range(batch)]
+        self._lens = [0] * batch
+
+    def _row(self, row: int) -> int:
+        if not 0 <= row < self.batch:
+            raise _lib.Ab2Error(-7, f"row {row} of a cache of {self.batch}")
+        return row
+
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def seq_len(self, row: int = 0) -> int:
+        return self._lens[self._row(row)]
+
+    def reserve(self, row: int, tokens: int) -> None:
+        """Takes the pages that ``tokens`` more tokens of a row need (AB2_ERR_CAPACITY, and none taken, where they are not to be had)."""
+        need = -(-(self.seq_len(row) + tokens) // self.page_size) - len(self._pages[row])
+        if need > len(self._free):
+            raise _lib.Ab2Error(-4, f"row {row} needs {need} more pages, {len(self._free)} are free")
+        for _ in range(need):
+            self._pages[row].append(self._free.pop())
+
+    def step(self, rows, new, room: int = 0, into: PagedStep | None = None) -> PagedStep:
+        """The batch of ``new[i]`` new tokens (0 or more) of row ``rows[i]``, with pages for them.  ``room``: the table is wide enough for that many
+        more tokens of each row.  ``into``: an earlier step over as many rows is written anew in place, for passes that were recorded with it."""
+        rows, new = [int(r) for r in rows], [int(n) for n in new]
+        if not rows or len(rows) != len(new) or min(new) < 0 or len(set(rows)) != len(rows):
+            raise _lib.Ab2Error(-1, f"a step takes distinct rows and new tokens of each, got rows {rows}, new {new}")
+        for r in rows:
+            self._row(r)
+        lens = [self._lens[r] + n for r, n in zip(rows, new)]
+        short = sum(max(0, -(-l // self.page_size) - len(self._pages[r])) for r, l in zip(rows, lens))
+        if short > len(self._free):
+            raise _lib.Ab2Error(-4, f"the step needs {short} more pages, {len(self._free)} are free")
+        widest = max(1, max(max(len(self._pages[r]), -(-(l + room) // self.page_size)) for r, l in zip(rows, lens)))
+        n, total, most = len(rows), sum(new), max(max(new), 1)
+        if into is None:
+            width = 1 << (widest - 1).bit_length()
+            packed = torch.empty(2 * n + 1 + n * width, dtype=torch.int32, device=self.k.device)
+            into = PagedStep(rows, new, packed[2 * n + 1:].view(n, width), packed[n + 1:2 * n + 1], packed[:n + 1], total, most, packed)
+        elif into.table.shape[0] != n or into.table.shape[1] < widest or into.tokens < total or into.max_new < most:
+            raise _lib.Ab2Error(-1, f"the step has {into.table.shape[0]} rows of {into.table.shape[1]} pages, {into.tokens} tokens, {into.max_new} a row: "
+                                    f"{n} rows of {widest}, {total}, {most} do not fit")
+        for r, c in zip(rows, new):
+            self.reserve(r, c)
+        width = into.table.shape[1]
+        flat = [0]
+        for c in new:
+            flat.append(flat[-1] + c)
+        flat += lens
+        for r in rows:
+            flat += self._pages[r] + [0] * (width - len(self._pages[r]))
+        into.packed.copy_(torch.tensor(flat, dtype=torch.int32))
+        into.rows, into.new = rows, new
+        return into
+
+    def append(self, step: PagedStep, k: torch.Tensor, v: torch.Tensor, layer: int = 0, q: torch.Tensor | None = None, frequencies=None, layout: str = "half",
+               magnitude: float = 1.0, out: torch.Tensor | None = None):
+        """``dispatch.paged_append`` on a layer: k, v (and q) [step.tokens, heads, dim]."""
+        from .dispatch import paged_append
+        self._fits(step, k)
+        return paged_append(self.k[layer], self.v[layer], k, v, step.table, step.lens, step.starts, q, frequencies, layout, magnitude, out)
+
+    def attention(self, step: PagedStep, q: torch.Tensor, scale: float, layer: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+        """``dispatch.attention_paged`` on a layer: q [step.tokens, heads, dim]."""
+        from .dispatch import attention_paged
+        self._fits(step, q)
+        return attention_paged(q, self.k[layer], self.v[layer], step.table, step.lens, scale, step.starts, step.max_new, out)
+
+    @staticmethod
+    def _fits(step, t):
+        if t.shape[0] < step.tokens:
+            raise _lib.Ab2Error(-1, f"a step of {step.tokens} tokens over a tensor of {t.shape[0]}")
+
+    def commit(self, step: PagedStep) -> None:
+        """The rows' lengths move on by the step's new tokens."""
+        for r, n in zip(step.rows, step.new):
+            self._lens[r] += n
+
+    def truncate(self, new_len: int, row: int = 0) -> None:
+        """Cuts a row back; pages behind its end are free again."""
+        if not 0 <= new_len <= self.seq_len(row):
+            raise _lib.Ab2Error(-4, f"row {row} holds {self.seq_len(row)} tokens and cannot be cut to {new_len}")
+        self._lens[row] = new_len
+        keep = -(-new_len // self.page_size)
+        self._free += self._pages[row][:keep - 1 if keep else None:-1]
+        del self._pages[row][keep:]
+
+    def clear(self) -> None:
+        for row in range(self.batch):
+            self.truncate(0, row)
+
+    def read(self, row: int = 0, layer: int = 0):
+        """The row's keys and values [len, kv_heads, head_dim] in f32."""
+        n = self.seq_len(row)
+        at = torch.tensor(self._pages[row], dtype=torch.int64, device=self.k.device)
+        return tuple(p[layer][at].transpose(1, 2).reshape(-1, self.kv_heads, self.head_dim)[:n].float() for p in (self.k, self.v))

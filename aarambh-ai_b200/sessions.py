@@ -14,13 +14,51 @@ sampler.rs:217-224); text, tools and stochastic samplers stay with the caller.
 """
 from __future__ import annotations
 
+from collections.abc import Callable
 from dataclasses import dataclass, field
 
 import torch
 
 from . import _lib
-from .dispatch import argmax
+from .dispatch import adjust_logits, allowed_words, argmax
 from .model import DecoderModel
+
+
+@dataclass
+class LogitRules:
+    """What a session's logits pass before the greedy choice (``dispatch.adjust_logits``): penalties for tokens that it has seen
+    (``prompt_counts``: those of its prompt too), biases by token id, and the tokens that a grammar allows next - a function of the ids
+    generated so far that returns ids, or a truth value for every token, or None for all."""
+    repetition: float = 1.0
+    presence: float = 0.0
+    frequency: float = 0.0
+    bias: dict | None = None
+    allowed: Callable | None = None
+    prompt_counts: bool = True
+
+    def __post_init__(self):
+        if not self.repetition > 0:
+            raise _lib.Ab2Error(-7, f"a repetition penalty is a positive factor, got {self.repetition}")
+
+    def apply(self, logits: torch.Tensor, prompt_ids, generated_ids) -> torch.Tensor:
+        """logits [1, vocab] -> the same under the rules."""
+        vocab, args = logits.shape[-1], {}
+        seen = (list(prompt_ids) if self.prompt_counts else []) + list(generated_ids)
+        if seen and (self.repetition != 1.0 or self.presence or self.frequency):
+            args["history"] = torch.tensor([seen], dtype=torch.int32, device=logits.device)
+            args["rules"] = torch.tensor([[self.repetition, self.presence, self.frequency]], dtype=torch.float32, device=logits.device)
+        if self.bias:
+            args["bias_ids"] = torch.tensor([list(self.bias)], dtype=torch.int32, device=logits.device)
+            args["bias_values"] = torch.tensor([list(self.bias.values())], dtype=torch.float32, device=logits.device)
+        may = self.allowed(list(generated_ids)) if self.allowed is not None else None
+        if may is not None:
+            may = torch.as_tensor(may, device=logits.device)
+            if may.dtype != torch.bool:
+                if may.numel() and (int(may.min()) < 0 or int(may.max()) >= vocab):
+                    raise _lib.Ab2Error(-1, "an allowed token outside the vocabulary")
+                may = torch.zeros(vocab, dtype=torch.bool, device=logits.device).index_fill_(0, may.long().view(-1), True)
+            args["allowed"] = allowed_words(may.view(1, vocab))
+        return adjust_logits(logits, **args) if args else logits
 
 
 @dataclass
@@ -33,6 +71,8 @@ class GenerationSession:
     pending_token: int | None = None
     eos_token_id: int | None = None
     finished: bool = False
+    rules: LogitRules | None = None
+    prompt_ids: list = field(default_factory=list)
 
     def is_finished(self) -> bool:
         return self.finished
@@ -98,7 +138,7 @@ class SessionEngine:
 
     # -- engine.rs:271-318 ---------------------------------------------------
     def prepare_session_with_chunk_size(self, prompt_ids, max_new_tokens: int, chunk_size: int = 128,
-                                        eos_token_id: int | None = None) -> GenerationSession:
+                                        eos_token_id: int | None = None, rules: LogitRules | None = None) -> GenerationSession:
         if chunk_size <= 0:
             raise _lib.Ab2Error(-1, "prefill chunk size must be greater than zero")
         ids = [int(t) for t in prompt_ids]
@@ -113,15 +153,18 @@ class SessionEngine:
             chunk = torch.tensor([ids[off:off + chunk_size]])
             logits = self.model.forward_with_cache(chunk, off, self.cache, row=row, last_only=True)
         return GenerationSession(row, len(ids), min(max_new_tokens, max_seq - len(ids)), logits.view(-1),
-                                 eos_token_id=eos_token_id)
+                                 eos_token_id=eos_token_id, rules=rules, prompt_ids=ids if rules is not None else [])
 
     # -- GenerationSession::advance, greedy (engine.rs:822-976) ---------------
     def advance(self, session: GenerationSession) -> int | None:
-        """Samples the next token from ``next_logits``; it becomes the pending
-        token of the next decode pass.  Returns it, or None once finished."""
+        """Samples the next token from ``next_logits``, under the session's rules if it has any; it becomes the
+        pending token of the next decode pass.  Returns it, or None once finished."""
         if session.finished:
             return None
-        token = int(argmax(session.next_logits.view(1, -1))[0])
+        logits = session.next_logits.view(1, -1)
+        if session.rules is not None:
+            logits = session.rules.apply(logits, session.prompt_ids, session.generated_ids)
+        token = int(argmax(logits)[0])
         session.generated_ids.append(token)
         if len(session.generated_ids) >= session.max_new_tokens or token == session.eos_token_id:
             session.finished = True

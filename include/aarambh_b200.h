@@ -352,6 +352,57 @@ int ab2_attention_causal(const void *q_dev, const void *k_dev, const void *v_dev
                          int h, int kv_heads, int q_len, int kv_len, int head_dim, float scale,
                          ab2_dtype dtype, ab2_stream stream);
 
+/* ---- a serving step over a paged cache ----------------------------------------
+ * Rotary positions of a batch, the append of its keys and values to pages, its attention over them, and the rules of a
+ * sampler on its logits.  No counterpart in the reference, whose caches are one slab a sequence.
+ *
+ * Rotation: pair i of a head at position p becomes magnitude * R(p * frequencies[i]) (x, y), R(a) (x, y) =
+ * (x cos a - y sin a, x sin a + y cos a); frequencies_dev [rot_dims / 2] f64 are radians a position, angles are exact to the
+ * f64's rounding at any position.  Dimensions from rot_dims on pass as they are. */
+typedef enum {
+    AB2_ROTARY_HALF = 0,       /* pairs (i, i + rot_dims / 2) */
+    AB2_ROTARY_INTERLEAVED = 1 /* pairs (2 i, 2 i + 1) */
+} ab2_rotary_layout;
+/* q [tokens][heads][head_dim] and k [tokens][kv_heads][head_dim] of element type `dtype` (either may have 0 heads), tokens
+ * `*_stride` elements apart, to the same shapes; an output may be its input.  positions_dev [tokens], i32 or (positions_64) i64. */
+int ab2_rotary_apply(const void *q_dev, long long q_stride, int heads, const void *k_dev, long long k_stride, int kv_heads, int head_dim,
+                     const void *positions_dev, int positions_64, int tokens, const double *frequencies_dev, int rot_dims, int layout, float magnitude,
+                     void *q_out_dev, long long q_out_stride, void *k_out_dev, long long k_out_stride, ab2_dtype dtype, ab2_stream stream);
+/* A paged cache of one layer and the batch that goes over it.  k_pages, v_pages [pages][kv_heads][page_size][head_dim] f32 or bf16
+ * (the calls' dtype), 16-byte aligned; page_size 16, 32, 64, 128 or 256; head_dim 64 or 128.  table [rows][table_width] i32: the
+ * pages of a row in order, rows table_stride apart.  lens [rows]: a row's tokens, its new ones included, which are the last of them.  starts [rows + 1]: row
+ * b's new tokens are starts[b] .. starts[b + 1] - 1 of q, k and v; NULL: one new token a row.  `tokens` of q, k and v exist; those
+ * behind the last row are left as they are.  Table, lens and starts are device memory, read when the kernels run: a recorded call
+ * serves what they hold then.  Values out of bounds (a page outside the pool, a row longer than its table, starts that fall or pass
+ * `tokens`) are brought within them, nothing outside the buffers is touched, and ab2_device_status reports AB2_ERR_BAD_ARG; the
+ * outputs are void then.  Rows that write a page must not share it. */
+typedef struct {
+    void *k_pages, *v_pages;
+    const int *table, *lens, *starts;
+    int pages, page_size, kv_heads, head_dim, table_width, rows, tokens;
+    long long table_stride;   /* entries from a row of the table to the next, table_width or more */
+} ab2_paged;
+/* Writes k (rotated at its position in the row; rot_dims 0: as it is) and v of the new tokens to their pages, and with heads > 0 the
+ * rotated q to q_out_dev, in one launch. */
+int ab2_paged_append(const ab2_paged *cache, const void *k_dev, long long k_stride, const void *v_dev, long long v_stride, const void *q_dev, long long q_stride,
+                     int heads, void *q_out_dev, long long q_out_stride, const double *frequencies_dev, int rot_dims, int layout, float magnitude, ab2_dtype dtype, ab2_stream stream);
+/* Attention of the new tokens, whose keys and values have been appended: a token sees its row's keys up to its own position, query head
+ * j reads KV head j / (heads / kv_heads), up to 32 query heads for one KV head; a token that sees no key answers zeros.  Keys and values out of
+ * sight may hold anything.  max_new (at least the most new tokens of a row) picks kernels, results do not rest on it.  workspace_dev
+ * (ab2_paged_workspace bytes, 16-byte aligned, nothing in it is kept between calls) lets long rows be cut between CTAs; NULL: they are not. */
+int ab2_paged_workspace(int head_dim, size_t *bytes);
+int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long long q_stride, int heads, void *out_dev, long long out_stride, int max_new, float scale,
+                        void *workspace_dev, size_t workspace_bytes, ab2_dtype dtype, ab2_stream stream);
+/* Rules of a sampler on logits [rows][vocab] (`stride` elements from row to row) to out_dev [rows][vocab], which may be the logits where
+ * stride = vocab.  With c the times a token occurs in history_dev [rows][history_width] (i32, the first lengths_dev[row] of a row or, NULL, all;
+ * ids outside the vocabulary are passed over) and rules_dev [rows][3] = {repetition > 0, presence, frequency}: where c > 0, z = z > 0 ? z /
+ * repetition : z * repetition, then z -= presence + frequency c.  Then z += bias_values[row][i] at bias_ids[row][i] ([rows][biases]; of an id
+ * named twice the last counts, ids outside the vocabulary are passed over), and z = -inf where bit v % 32 of allowed_dev [rows][ceil(vocab / 32)]
+ * word v / 32 is 0 (NULL: all are allowed).  In f32, rounded once. */
+int ab2_adjust_logits(const void *logits_dev, long long stride, int rows, int vocab, const int *history_dev, long long history_stride, int history_width,
+                      const int *lengths_dev, const float *rules_dev, const int *bias_ids_dev, const float *bias_values_dev, int biases, const uint32_t *allowed_dev,
+                      void *out_dev, ab2_dtype dtype, ab2_stream stream);
+
 /* ---- decoder -----------------------------------------------------------------
  * The dense grouped-query decoder of AarambhModel (crates/aarambh-studio-model/
  * src/model.rs) over packed weights.  Field names follow ModelConfig
