@@ -17,18 +17,10 @@ using namespace ab2;
 namespace ab2 {
 int paged_check(const ab2_paged *c, ab2_dtype dtype);
 PagedView paged_view(const ab2_paged *c);
+size_t paged_tc_bytes(int hd);
+int paged_tc_attention(const PagedAttnArgs &a, int hd, void *workspace, size_t bytes, cudaStream_t s);
+constexpr int PAGED_FEW_ROWS = 32;   // query rows of a KV head up to which the tensor-memory kernel's tiles of 128 would be nearly empty
 namespace {
-
-struct PagedAttnArgs {
-    PagedPlan plan;
-    const void *q, *k, *v;
-    void *out;
-    long long q_stride, o_stride;
-    int group;
-    float sl;          // scale in powers of two
-    float *acc, *ml;   // pieces: [2 ctas][QR][HD] sums, [2 ctas][QR][2] maximum and sum of weights
-    int *status;
-};
 
 constexpr int PA_THREADS = 128, PA_KEYS = 32;
 
@@ -62,15 +54,13 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
     PagedRun run = paged_run<PA_THREADS>(a.plan, blockIdx.x, gridDim.x, warp_sums, &found, a.status);
     PagedPiece w;
     while (paged_next(a.plan, run, w)) {
-        const int base = w.r.len - w.r.count, t0 = w.q_tile * a.plan.tq, ntok = min(a.plan.tq, w.r.count - t0);
-        const int last = base + t0 + ntok - 1;   // the last key that a query of the item sees
-        const int lo = a.plan.whole ? 0 : w.k0 << a.plan.key_shift;
-        const int hi = a.plan.whole ? last + 1 : (int)min((long long)last + 1, (long long)w.k1 << a.plan.key_shift);
+        const PagedSpan sp = paged_span(a.plan, w);
+        const int t0 = sp.t0, ntok = sp.ntok, base = sp.base, lo = sp.lo, hi = sp.hi, group = a.plan.group;
         __syncthreads();
         for (int i = threadIdx.x; i < QR * HD / 4; i += PA_THREADS) {
-            const int r = i / (HD / 4), d = i % (HD / 4) * 4, tok = r / a.group, g = r - tok * a.group;
+            const int r = i / (HD / 4), d = i % (HD / 4) * 4, tok = r / group, g = r - tok * group;
             float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (tok < ntok) f = load4((const T *)a.q + (size_t)(w.r.first + t0 + tok) * a.q_stride + (size_t)(w.head * a.group + g) * HD + d);
+            if (tok < ntok) f = load4((const T *)a.q + (size_t)(w.r.first + t0 + tok) * a.q_stride + (size_t)(w.head * group + g) * HD + d);
             *reinterpret_cast<float4 *>(qs + r * (HD + 4) + d) = make_float4(f.x * a.sl, f.y * a.sl, f.z * a.sl, f.w * a.sl);
         }
         // rows past the last key read as zeros
@@ -89,7 +79,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
         int lim[RPT];
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
-            const int tok = (ty * RPT + i) / a.group;
+            const int tok = (ty * RPT + i) / group;
             lim[i] = tok < ntok ? base + t0 + tok : -1;
             top[i] = -INFINITY;
             sum[i] = 0.f;
@@ -175,13 +165,13 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
         const size_t slot = 2 * (size_t)blockIdx.x + (w.k0 == 0);
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
-            const int r = ty * RPT + i, tok = r / a.group, g = r - tok * a.group;
+            const int r = ty * RPT + i, tok = r / group, g = r - tok * group;
 #pragma unroll
             for (int m = TX / 2; m > 0; m >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], m);
             if (tok >= ntok) continue;
             if (all) {
-                const float f = top[i] == -INFINITY ? 0.f : 1.f / sum[i];
-                T *dst = (T *)a.out + (size_t)(w.r.first + t0 + tok) * a.o_stride + (size_t)(w.head * a.group + g) * HD;
+                const float f = sum[i] == 0.f ? 0.f : 1.f / sum[i];
+                T *dst = (T *)a.out + (size_t)(w.r.first + t0 + tok) * a.o_stride + (size_t)(w.head * group + g) * HD;
 #pragma unroll
                 for (int d = 0; d < DPT; d += 4)
 #pragma unroll
@@ -196,56 +186,39 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
     }
 }
 
-// The pieces of cut items: CTA c (from 1 on) finishes the item that CTA c - 1 began and did not end.
-template <typename T, int HD, int QR>
-__global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a, int ctas) {
+// The pieces of cut items: CTA c finishes the item that CTA c of the launch before began and did not end.
+template <typename T, int HD>
+__global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
     __shared__ long long warp_sums[PA_THREADS / 32];
     __shared__ PagedRun found;
     pdl_wait();
-    const int c = blockIdx.x;   // the CTA whose last piece may begin an item
-    PagedRun run = paged_run<PA_THREADS>(a.plan, c, ctas, warp_sums, &found, nullptr);
+    const int c = blockIdx.x, group = a.plan.group;
+    PagedRun run = paged_run<PA_THREADS>(a.plan, c, a.ctas, warp_sums, &found, nullptr);
     PagedPiece w;
-    bool cut = false;
-    long long end = 0;
-    while (paged_next(a.plan, run, w)) {
-        cut = w.k0 == 0 && w.k1 < w.k_tiles;
-        end = run.u + (w.k_tiles - w.k1);   // the unit behind the item
-    }
-    if (!cut) return;
-    // how many CTAs hold pieces of it: c, c + 1, ... up to the one whose run reaches the item's end
-    __shared__ long long total_units;
-    {
-        long long total = 0, n;
-        for (int r0 = 0; r0 < a.plan.p.rows; r0 += PA_THREADS) {
-            const int r = r0 + threadIdx.x;
-            (void)cta_prefix<PA_THREADS>(r < a.plan.p.rows ? paged_shape(a.plan, paged_row(a.plan.p, r, nullptr)).units : 0, n, warp_sums);
-            total += n;
-        }
-        if (threadIdx.x == 0) total_units = total;
-        __syncthreads();
-    }
-    int last = c + 1;
-    while (last + 1 < ctas && total_units * (last + 1) / ctas < end) ++last;
-    const int t0 = w.q_tile * a.plan.tq, ntok = min(a.plan.tq, w.r.count - t0);
-    auto slot = [&](int i) { return 2 * (size_t)i + (i == c); };
-    auto empty = [&](int i) { return total_units * i / ctas == total_units * (i + 1) / ctas; };  // a CTA without units holds no piece
-    for (int i = threadIdx.x; i < ntok * a.group * (HD / 4); i += PA_THREADS) {
-        const int r = i / (HD / 4), d = i % (HD / 4) * 4, tok = r / a.group, g = r - tok * a.group;
+    w.k1 = w.k_tiles = w.k0 = 0;
+    while (paged_next(a.plan, run, w)) {}
+    if (w.k0 != 0 || w.k1 >= w.k_tiles) return;   // the CTA's last piece
+    const long long end = run.u + (w.k_tiles - w.k1);   // the unit behind the item
+    int last = c + 1;   // the CTA that ends it
+    while (last + 1 < run.ctas && paged_begin(run, last + 1) < end) ++last;
+    const PagedSpan sp = paged_span(a.plan, w);
+    auto slot = [&](int i) { return (2 * (size_t)i + (i == c)) * a.tile_rows; };
+    for (int i = threadIdx.x + blockIdx.y * PA_THREADS; i < sp.ntok * group * (HD / 4); i += PA_THREADS * gridDim.y) {
+        const int r = i / (HD / 4), d = i % (HD / 4) * 4, tok = r / group, g = r - tok * group;
         float top = -INFINITY;
-        for (int j = c; j <= last; ++j)
-            if (!empty(j)) top = fmaxf(top, a.ml[(slot(j) * QR + r) * 2]);
+        for (int j = c; j <= last; ++j) top = fmaxf(top, a.ml[(slot(j) + r) * 2]);
         const float m = top == -INFINITY ? 0.f : top;
         float sum = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int j = c; j <= last; ++j) {
-            if (empty(j)) continue;
-            const float f = exp2f(a.ml[(slot(j) * QR + r) * 2] - m);
-            const float4 v = *reinterpret_cast<const float4 *>(a.acc + (slot(j) * QR + r) * HD + d);
-            sum = fmaf(f, a.ml[(slot(j) * QR + r) * 2 + 1], sum);
+            const float2 ml = *reinterpret_cast<const float2 *>(a.ml + (slot(j) + r) * 2);
+            const float f = exp2f(ml.x - m);
+            const float4 v = *reinterpret_cast<const float4 *>(a.acc + (slot(j) + r) * HD + d);
+            sum = fmaf(f, ml.y, sum);
             o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
         }
-        const float f = top == -INFINITY ? 0.f : 1.f / sum;
-        T *dst = (T *)a.out + (size_t)(w.r.first + t0 + tok) * a.o_stride + (size_t)(w.head * a.group + g) * HD + d;
+        const float f = sum == 0.f ? 0.f : 1.f / sum;
+        T *dst = (T *)a.out + (size_t)(w.r.first + sp.t0 + tok) * a.o_stride + (size_t)(w.head * group + g) * HD + d;
         dst[0] = from_f32<T>(o.x * f); dst[1] = from_f32<T>(o.y * f); dst[2] = from_f32<T>(o.z * f); dst[3] = from_f32<T>(o.w * f);
     }
 }
@@ -263,35 +236,37 @@ int launch_simt(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) 
         AB2_CUDA(cudaFuncSetAttribute(paged_simt_kernel<T, HD, QR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
         configured[dev] = true;
     }
-    const int ctas = simt_ctas();
-    a.plan.tq = std::max(1, QR / a.group);
-    a.plan.key_shift = 6;
-    a.plan.whole = !workspace || bytes < (size_t)2 * ctas * QR * (HD + 2) * 4;
-    a.acc = (float *)workspace;
-    a.ml = a.acc + (size_t)2 * ctas * QR * HD;
-    paged_simt_kernel<T, HD, QR><<<ctas, PA_THREADS, S::SMEM, s>>>(a);
+    paged_deal(a, simt_ctas(), QR, 6, 1, HD, workspace, bytes);
+    paged_simt_kernel<T, HD, QR><<<a.ctas, PA_THREADS, S::SMEM, s>>>(a);
     AB2_LAUNCH_CHECK();
-    if (a.plan.whole) return AB2_OK;
-    ChainedLaunches chained(true);
-    cudaError_t e = launch_kernel(paged_merge_kernel<T, HD, QR>, dim3(ctas - 1), dim3(PA_THREADS), 0, s, a, ctas);
-    if (e != cudaSuccess) return fail(AB2_ERR_CUDA, "paged attention launch failed: %s", cudaGetErrorString(e));
-    return AB2_OK;
+    return a.plan.whole ? AB2_OK : paged_merge(a, HD, ActType<T>::value, s);
 }
 
 template <typename T>
 int simt_attention(const PagedAttnArgs &a, int hd, int max_new, void *workspace, size_t bytes, cudaStream_t s) {
-    const bool few = max_new * (long long)a.group <= 8;
+    const bool few = max_new * (long long)a.plan.group <= 8;
     if (hd == 128) return few ? launch_simt<T, 128, 8>(a, workspace, bytes, s) : launch_simt<T, 128, 32>(a, workspace, bytes, s);
     return few ? launch_simt<T, 64, 8>(a, workspace, bytes, s) : launch_simt<T, 64, 32>(a, workspace, bytes, s);
 }
 
 }  // namespace
+
+int paged_merge(const PagedAttnArgs &a, int hd, ab2_dtype dtype, cudaStream_t s) {
+    ChainedLaunches chained(true);
+    const dim3 grid(a.ctas - 1, std::max(1, a.tile_rows / 32));
+    auto kernel = dtype == AB2_F32 ? (hd == 128 ? paged_merge_kernel<float, 128> : paged_merge_kernel<float, 64>)
+                                   : (hd == 128 ? paged_merge_kernel<__nv_bfloat16, 128> : paged_merge_kernel<__nv_bfloat16, 64>);
+    cudaError_t e = launch_kernel(kernel, grid, dim3(PA_THREADS), 0, s, a);
+    if (e != cudaSuccess) return fail(AB2_ERR_CUDA, "paged attention launch failed: %s", cudaGetErrorString(e));
+    return AB2_OK;
+}
+
 }  // namespace ab2
 
 AB2_API int ab2_paged_workspace(int head_dim, size_t *bytes) {
     AB2_REQUIRE(bytes, AB2_ERR_BAD_ARG, "null argument");
     AB2_REQUIRE(head_dim == 64 || head_dim == 128, AB2_ERR_UNSUPPORTED, "paged caches have heads of 64 or 128, not %d", head_dim);
-    *bytes = (size_t)2 * simt_ctas() * 32 * (head_dim + 2) * 4;
+    *bytes = std::max(paged_piece_bytes(simt_ctas(), 32, head_dim), paged_tc_bytes(head_dim));
     return AB2_OK;
 }
 
@@ -310,9 +285,15 @@ AB2_API int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long 
     PagedAttnArgs a = {};
     a.plan.p = paged_view(cache);
     a.q = q_dev; a.k = cache->k_pages; a.v = cache->v_pages; a.out = out_dev; a.q_stride = q_stride; a.o_stride = out_stride;
-    a.group = heads / cache->kv_heads; a.sl = scale * 1.44269504088896341f;
+    a.plan.group = heads / cache->kv_heads; a.plan.above = 0; a.plan.most = 0x7fffffff; a.sl = scale * 1.44269504088896341f;
     rc = device_status_word(&a.status);
     if (rc != AB2_OK) return rc;
     if (dtype == AB2_F32) return simt_attention<float>(a, cache->head_dim, max_new, workspace_dev, workspace_bytes, (cudaStream_t)stream);
-    return simt_attention<__nv_bfloat16>(a, cache->head_dim, max_new, workspace_dev, workspace_bytes, (cudaStream_t)stream);
+    const bool chunks = cache->starts && (long long)max_new * a.plan.group > PAGED_FEW_ROWS;   // there may be rows for the tensor-memory kernel
+    if (chunks) a.plan.most = PAGED_FEW_ROWS;
+    rc = simt_attention<__nv_bfloat16>(a, cache->head_dim, max_new, workspace_dev, workspace_bytes, (cudaStream_t)stream);
+    if (rc != AB2_OK || !chunks) return rc;
+    a.plan.above = PAGED_FEW_ROWS;
+    a.plan.most = 0x7fffffff;
+    return paged_tc_attention(a, cache->head_dim, workspace_dev, workspace_bytes, (cudaStream_t)stream);
 }

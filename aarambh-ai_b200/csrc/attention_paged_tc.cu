@@ -1,0 +1,418 @@
+// Attention of chunks over a paged bf16 cache on the 5th-generation tensor cores: rows whose new tokens fill more than a warp-level tile.
+// The mathematics is that of attention_paged.cu.  An item is up to 256 query rows, tokens x heads of one KV head's group, in two tiles of 128:
+//
+//   S_g[128 rows][128 keys] = Q_g . K^T          both K-major in shared memory
+//   O_g[128 rows][dim]     += P_g . V            P in tensor memory, where the scores were; V N-major in shared memory
+//
+//   warp 0       TMA producer: pages to tiles of 128 keys, K and V in turn, in a ring
+//   warp 1       MMA issue
+//   warps 4-7    softmax of tile 0, a thread per row;   warps 8-11   of tile 1
+// While one tile's scores become weights the other's products run.  The weights enter rounded to bf16, half a step (2^-8) each and
+// independent, which the sum over the keys averages; their sum is that of the f32 weights.  Scores, maxima, sums and O are f32.
+// The weights are relative to a maximum per row that moves only when a score exceeds it by 2^8; then O is rescaled in tensor memory.
+//
+// An MMA multiplies a hidden value by a weight of 0, so an Inf or a NaN there would reach rows that do not see it.  Rows of a page behind the
+// sequence's end are cleared in shared memory; a row whose sums come out as Inf or NaN (a later token's value may hold them) is computed
+// again on CUDA cores over the keys in its sight.  Every wait on an mbarrier is bounded; on a time-out the CTA records AB2_ERR_TIMEOUT and
+// walks through the rest of its work without waiting.
+#include <algorithm>
+
+#include "paged.cuh"
+#include "tcgen05_util.cuh"
+
+using namespace ab2;
+using namespace ab2::tc;
+
+namespace ab2 {
+namespace {
+
+constexpr int PC_Q = 128, PC_KEYS = 128, PC_THREADS = 384, PC_BOX = 128 * 128;  // a box is 128 rows of 64 elements
+constexpr float PC_SLACK = 8.f;  // powers of two a score may exceed the row's maximum by
+constexpr float PC_NONE = -1e30f;
+
+template <int HD> struct PcShape {
+    static constexpr int BOXES = HD / 64, TILE = BOXES * PC_BOX, SLOTS = HD == 128 ? 5 : 8;
+    static constexpr int SMEM = 1024 + (2 + SLOTS) * TILE;
+};
+
+struct PcShared {
+    uint64_t full[8], empty[8], qfull[2], sfull[2], pfull[2], odone[2];
+    uint32_t tmem_base;
+    int failed;
+    PagedRun found;
+    long long warp_sums[PC_THREADS / 32];
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// What all roles know of a piece.
+struct PcPiece {
+    PagedPiece w;
+    PagedSpan s;
+    int first;      // tile of keys that it begins with
+    int tiles[2];   // of keys that a tile of rows looks at
+    int most;
+};
+__device__ __forceinline__ bool pc_next(const PagedPlan &a, PagedRun &run, PcPiece &x) {
+    if (!paged_next(a, run, x.w)) return false;
+    x.s = paged_span(a, x.w);
+    x.first = x.s.lo / PC_KEYS;
+    const int rows = x.s.ntok * a.group;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        // keys up to those of the last token of the tile of rows
+        const int last = min(x.s.hi, x.s.base + x.s.t0 + (min(rows, (g + 1) * PC_Q) - 1) / a.group + 1);
+        x.tiles[g] = rows > g * PC_Q ? max(0, (last + PC_KEYS - 1) / PC_KEYS - x.first) : 0;
+    }
+    x.most = max(x.tiles[0], x.tiles[1]);
+    return true;
+}
+
+// One tile of keys for the warp's 32 rows, a lane each: scores to weights in tensor memory.  With EDGE keys past `lim` are out of sight.
+template <int HD, bool EDGE>
+__device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, float sl, int lim, bool has_o, float &top, float &sum) {
+    uint32_t v[4][32];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tmem_ld32_start(v[c], s_addr + 32 * c);
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        tmem_ld32_wait(v[c]);
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+            if (EDGE && 32 * c + k > lim) v[c][k] = 0xff800000u;
+#pragma unroll
+        for (int k = 0; k < 32; k += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(v[c][k + e]), __uint_as_float(v[c][k + 4 + e]));
+    }
+    const float best = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sl;  // the scale is not negative
+    const float now = best > top + PC_SLACK ? best : top;
+    if (__any_sync(0xffffffffu, now != top)) {
+        const float corr = ex2(top - now);
+        sum *= corr;
+        top = now;
+        // the scores came after the products of the last tile: the sums stand still
+        if (has_o) {
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(o, o_addr + 32 * c);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
+                tmem_st32(o_addr + 32 * c, o);
+            }
+        }
+    }
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint32_t p[16];
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+            const float e0 = ex2(fmaf(__uint_as_float(v[c][k]), sl, -top)), e1 = ex2(fmaf(__uint_as_float(v[c][k + 1]), sl, -top));
+            part[(k >> 1) & 1] += e0;
+            part[2 + ((k >> 1) & 1)] += e1;
+            const __nv_bfloat162 b = __floats2bfloat162_rn(e0, e1);
+            p[k >> 1] = *reinterpret_cast<const uint32_t *>(&b);
+        }
+        tmem_st16(s_addr + 16 * c, p);
+    }
+    sum += (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// A row of a piece over the keys [lo, to] of it that it sees, by one warp: a lane has every 32nd dimension.
+template <int HD>
+__device__ __forceinline__ void pc_again(const PagedAttnArgs &a, const PcPiece &x, int r, int lane, bool all, size_t slot) {
+    constexpr int N = HD / 32;
+    const int tok = r / a.plan.group, head = x.w.head * a.plan.group + r % a.plan.group;
+    const int to = min(x.s.hi - 1, x.s.base + x.s.t0 + tok);
+    const __nv_bfloat16 *q = (const __nv_bfloat16 *)a.q + (size_t)(x.w.r.first + x.s.t0 + tok) * a.q_stride + (size_t)head * HD;
+    float qv[N], acc[N] = {}, top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) qv[i] = __bfloat162float(q[lane + 32 * i]) * a.sl;
+    for (int key = x.s.lo; key <= to; ++key) {
+        const size_t row = (((size_t)paged_page(a.plan.p, x.w.row, key, a.status) * a.plan.p.kv_heads + x.w.head) << a.plan.p.page_shift) + (key & ((1 << a.plan.p.page_shift) - 1));
+        float s = 0.f, vv[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            s = fmaf(qv[i], __bfloat162float(((const __nv_bfloat16 *)a.k)[row * HD + lane + 32 * i]), s);
+            vv[i] = __bfloat162float(((const __nv_bfloat16 *)a.v)[row * HD + lane + 32 * i]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        const float best = fmaxf(top, s), m = best == -INFINITY ? 0.f : best, keep = exp2f(top - m), w = exp2f(s - m);
+        sum = sum * keep + w;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = fmaf(w, vv[i], acc[i] * keep);
+        top = best;
+    }
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (all) ((__nv_bfloat16 *)a.out)[(size_t)(x.w.r.first + x.s.t0 + tok) * a.o_stride + (size_t)head * HD + lane + 32 * i] = __float2bfloat16_rn(acc[i] * f);
+        else a.acc[(slot + r) * HD + lane + 32 * i] = acc[i];
+    }
+    if (!all && lane == 0) *reinterpret_cast<float2 *>(a.ml + (slot + r) * 2) = make_float2(top, sum);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(PC_THREADS, 1)
+paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PagedAttnArgs a) {
+    using S = PcShape<HD>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ PcShared sh;
+    uint8_t *qbuf = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023), *ring = qbuf + 2 * S::TILE;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int *failed = &sh.failed;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::SLOTS; ++i) { bar_init(&sh.full[i], 1); bar_init(&sh.empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { bar_init(&sh.qfull[i], 4); bar_init(&sh.sfull[i], 1); bar_init(&sh.pfull[i], 4); bar_init(&sh.odone[i], 1); }
+        sh.failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    PagedRun run = paged_run<PC_THREADS>(a.plan, blockIdx.x, a.ctas, sh.warp_sums, &sh.found, a.status);
+    if (run.u >= run.u1) return;   // the whole CTA
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(sptr(&sh.tmem_base)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    const uint32_t tmem = sh.tmem_base, tmem_o = tmem + 2 * PC_KEYS;
+    const PagedView &p = a.plan.p;
+    PcPiece x;
+    // the block's registers: 128 threads of 72 and 256 of 216 are the 384 of 168 that it was launched with
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        if (warp == 0) {
+            // ---------------------------------------------------------- TMA producer: K, V, K, V, ...
+            const int rows = min(PC_KEYS, 1 << p.page_shift), boxes = PC_KEYS / rows;   // of a page in a tile, pages a tile
+            int n = 0;
+            while (pc_next(a.plan, run, x)) {
+                for (int j = 0; j < x.most; ++j) {
+                    const int key = (x.first + j) * PC_KEYS + lane * rows;
+                    const bool mine = lane < boxes && key < x.s.hi;   // pages that hold keys of the piece
+                    const int page = mine ? paged_page(p, x.w.row, key, a.status) : 0;
+                    const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * rows * HD * 2;
+                    for (int kv = 0; kv < 2; ++kv, ++n) {
+                        const int slot = n % S::SLOTS;
+                        warp_wait(&sh.empty[slot], ((n / S::SLOTS) & 1) ^ 1, failed);
+                        if (lane == 0) bar_expect_tx(&sh.full[slot], (uint32_t)bytes);
+                        __syncwarp();
+                        if (mine && !*failed)
+#pragma unroll
+                            for (int b = 0; b < S::BOXES; ++b)
+                                tma_load_3d(ring + slot * S::TILE + b * PC_BOX + lane * rows * 128, kv ? &vmap : &kmap, b * 64, key & ((1 << p.page_shift) - 1), page * p.kv_heads + x.w.head, &sh.full[slot]);
+                    }
+                }
+            }
+        } else if (warp == 1) {
+            // ---------------------------------------------------------- MMA issue
+            constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
+            constexpr uint32_t S_DESC = IDESC | ((uint32_t)(PC_KEYS >> 3) << 17), O_DESC = IDESC | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
+            int n = 0, summed[2] = {0, 0}, asked[2] = {0, 0};   // slots of the ring taken; of either tile of rows the products with V and the pieces
+            // n0: the slot of the piece's first K
+            auto scores = [&](int n0, int g, int j) {
+                const int slot = (n0 + 2 * j) % S::SLOTS;
+                if (elect_one()) {
+#pragma unroll
+                    for (int b = 0; b < S::BOXES; ++b) {
+                        const uint64_t qd = umma_desc(sptr(qbuf + g * S::TILE + b * PC_BOX)), kd = umma_desc(sptr(ring + slot * S::TILE + b * PC_BOX));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)  // descriptors count in 16 bytes
+                            umma_bf16(tmem + (uint32_t)(g * PC_KEYS), qd + (uint64_t)(2 * k), kd + (uint64_t)(2 * k), S_DESC, (b | k) != 0);
+                    }
+                    if (g == 1 || x.tiles[1] <= j) umma_commit(&sh.empty[slot]);
+                    umma_commit(&sh.sfull[g]);
+                }
+                __syncwarp();
+            };
+            while (pc_next(a.plan, run, x)) {
+                const int n0 = n;
+                for (int g = 0; g < 2; ++g)
+                    if (x.s.ntok * a.plan.group > g * PC_Q) warp_wait(&sh.qfull[g], asked[g]++ & 1, failed);
+                if (x.most > 0) {
+                    warp_wait(&sh.full[n % S::SLOTS], (n / S::SLOTS) & 1, failed);
+                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                    for (int g = 0; g < 2; ++g)
+                        if (x.tiles[g] > 0) scores(n0, g, 0);
+                }
+                for (int j = 0; j < x.most; ++j, n += 2) {
+                    const int slot = (n + 1) % S::SLOTS;
+                    warp_wait(&sh.full[slot], ((n + 1) / S::SLOTS) & 1, failed);
+                    bool next = false;   // the next tile of keys has come
+                    for (int g = 0; g < 2; ++g) {
+                        if (j >= x.tiles[g]) continue;
+                        warp_wait(&sh.pfull[g], summed[g] & 1, failed);
+                        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                        if (elect_one()) {
+                            const uint64_t vd = umma_desc_mn(sptr(ring + slot * S::TILE), PC_BOX);
+#pragma unroll
+                            for (int k = 0; k < PC_KEYS / 16; ++k)
+                                umma_bf16_ts(tmem_o + (uint32_t)(g * HD), tmem + (uint32_t)(g * PC_KEYS + 8 * k), vd + (uint64_t)(k * (2048 >> 4)), O_DESC, j > 0 || k > 0);
+                            if (g == 1 || x.tiles[1] <= j) umma_commit(&sh.empty[slot]);
+                            umma_commit(&sh.odone[g]);
+                        }
+                        __syncwarp();
+                        ++summed[g];
+                        if (j + 1 < x.tiles[g]) {
+                            if (!next) warp_wait(&sh.full[(n + 2) % S::SLOTS], ((n + 2) / S::SLOTS) & 1, failed);
+                            next = true;
+                            warp_wait(&sh.odone[g], (summed[g] - 1) & 1, failed);   // the weights lie where the scores will
+                            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                            scores(n0, g, j + 1);
+                        }
+                    }
+                }
+            }
+        }
+    } else {
+        // ---------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
+        const int g = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, group = a.plan.group;
+        const uint32_t quad_addr = (uint32_t)(quad * 32) << 16, s_addr = tmem + quad_addr + (uint32_t)(g * PC_KEYS), o_addr = tmem_o + quad_addr + (uint32_t)(g * HD);
+        const float sl = fabsf(a.sl);
+        const uint32_t flip = a.sl < 0.f ? 0x80008000u : 0u;   // a negative scale's sign goes to the queries
+        int n = 0, scored = 0;
+        while (pc_next(a.plan, run, x)) {
+            const int rows = x.s.ntok * group, n0 = n;
+            n += 2 * x.most;
+            if (rows <= g * PC_Q) continue;
+            // the queries: a quad's warp stores 32 rows of its tile, a row 16 bytes a lane
+            for (int i = threadIdx.x & 127; i < PC_Q * HD / 8; i += 128) {
+                const int row = i / (HD / 8), d = i % (HD / 8), rr = g * PC_Q + row, tok = rr / group;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (rr < rows) v = *reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)a.q + (size_t)(x.w.r.first + x.s.t0 + tok) * a.q_stride + (size_t)(x.w.head * group + rr - tok * group) * HD + d * 8);
+                v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+                *reinterpret_cast<uint4 *>(qbuf + g * S::TILE + (d >> 3) * PC_BOX + row * 128 + (((d & 7) ^ (row & 7)) << 4)) = v;
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.qfull[g]);
+            const int rr = g * PC_Q + r, tok = rr / group, pos = rr < rows ? x.s.base + x.s.t0 + tok : -1;
+            const int least = x.s.base + x.s.t0 + (g * PC_Q) / group;   // the first row sees up to here
+            float top = PC_NONE, sum = 0.f;
+            for (int j = 0; j < x.tiles[g]; ++j, ++scored) {
+                const int at = (x.first + j) * PC_KEYS;
+                warp_wait(&sh.sfull[g], scored & 1, failed);
+                asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                const int lim = min(pos, x.s.hi - 1) - at;
+                if (at + PC_KEYS - 1 > least || at + PC_KEYS > x.s.hi || (g + 1) * PC_Q > rows) pc_softmax<HD, true>(s_addr, o_addr, sl, lim, j > 0, top, sum);
+                else pc_softmax<HD, false>(s_addr, o_addr, sl, lim, j > 0, top, sum);
+                if (at + PC_KEYS > x.s.hi) {   // what lies behind the piece's keys may be anything
+                    const int slot = (n0 + 2 * j + 1) % S::SLOTS;
+                    warp_wait(&sh.full[slot], ((n0 + 2 * j + 1) / S::SLOTS) & 1, failed);
+                    if (at + r >= x.s.hi)
+#pragma unroll
+                        for (int b = 0; b < S::BOXES; ++b)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4 *>(ring + slot * S::TILE + b * PC_BOX + r * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    __syncwarp();
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.pfull[g]);
+            }
+            if (x.tiles[g] > 0) warp_wait(&sh.odone[g], (scored - 1) & 1, failed);
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            const bool all = x.w.k0 == 0 && x.w.k1 == x.w.k_tiles;
+            const size_t slot = (2 * (size_t)blockIdx.x + (x.w.k0 == 0)) * a.tile_rows;
+            const float f = !all ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+            float poison = 0.f;  // stays 0 unless an output is Inf or NaN
+            __nv_bfloat16 *dst = (__nv_bfloat16 *)a.out + (size_t)(x.w.r.first + x.s.t0 + tok) * a.o_stride + (size_t)(x.w.head * group + rr - tok * group) * HD;
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+                uint32_t v[32];
+                __syncwarp();
+                tmem_ld32(v, o_addr + 32 * c);
+                if (x.tiles[g] == 0)
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[k] = 0u;
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                    const float y = __uint_as_float(v[k]) * f;
+                    poison = fmaf(y, 0.f, poison);
+                    v[k] = __float_as_uint(y);
+                }
+                if (all && rr < rows) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) {
+                        uint32_t o[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[k + 2 * e]), __uint_as_float(v[k + 2 * e + 1]));
+                            o[e] = *reinterpret_cast<const uint32_t *>(&b);
+                        }
+                        *reinterpret_cast<uint4 *>(dst + 32 * c + k) = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+                } else if (rr < rows) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4 *>(a.acc + (slot + rr) * HD + 32 * c + k) = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                }
+            }
+            if (!all && rr < rows) *reinterpret_cast<float2 *>(a.ml + (slot + rr) * 2) = make_float2(top, sum);
+            __syncwarp();
+            for (uint32_t left = __ballot_sync(0xffffffffu, rr < rows && poison != 0.f); left; left &= left - 1)  // NaN is not 0
+                pc_again<HD>(a, x, g * PC_Q + quad * 32 + __ffs(left) - 1, lane, all, slot);
+            // the next piece's products may go over what has been read
+            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+        }
+    }
+    // ---- teardown: every warp arrives here (all waits are bounded)
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0 && sh.failed) atomicExch(a.status, (int)AB2_ERR_TIMEOUT);
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
+    }
+}
+
+// The pages of a layer: [pages kv_heads][page_size][dim], in boxes of 64 elements of the rows that a page has in a tile.
+int pages_map(CUtensorMap *map, const void *pages, const PagedView &p, int hd) {
+    const int page = 1 << p.page_shift;
+    return make_mats_map(map, pages, p.pages * p.kv_heads, page, hd, hd, (long long)page * hd, std::min(page, PC_KEYS));
+}
+
+template <int HD>
+int launch_tc(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
+    using S = PcShape<HD>;
+    static bool configured[64] = {false};  // the attribute is per device
+    int dev = 0;
+    AB2_CUDA(cudaGetDevice(&dev));
+    AB2_REQUIRE(dev >= 0 && dev < 64, AB2_ERR_BAD_ARG, "device index %d out of range", dev);
+    if (!configured[dev]) {
+        AB2_CUDA(cudaFuncSetAttribute(paged_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+        configured[dev] = true;
+    }
+    CUtensorMap kmap, vmap;
+    int rc = pages_map(&kmap, a.k, a.plan.p, HD);
+    if (rc == AB2_OK) rc = pages_map(&vmap, a.v, a.plan.p, HD);
+    if (rc != AB2_OK) return rc;
+    paged_deal(a, device_sm_count(), 2 * PC_Q, paged_log2(PC_KEYS), 4, HD, workspace, bytes);
+    paged_tc_kernel<HD><<<a.ctas, PC_THREADS, S::SMEM, s>>>(kmap, vmap, a);
+    AB2_LAUNCH_CHECK();
+    return a.plan.whole ? AB2_OK : paged_merge(a, HD, AB2_BF16, s);
+}
+
+}  // namespace
+
+size_t paged_tc_bytes(int hd) { return paged_piece_bytes(device_sm_count(), 2 * PC_Q, hd); }
+int paged_tc_attention(const PagedAttnArgs &a, int hd, void *workspace, size_t bytes, cudaStream_t s) {
+    return hd == 128 ? launch_tc<128>(a, workspace, bytes, s) : launch_tc<64>(a, workspace, bytes, s);
+}
+
+}  // namespace ab2

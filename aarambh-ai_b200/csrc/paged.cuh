@@ -58,24 +58,40 @@ __device__ __forceinline__ void turn_cos_sin(unsigned long long a, float m, floa
 }
 
 // ---- attention over a paged cache: how the work is dealt out
-// An item is a tile of a row's queries (tq of its new tokens, all heads of one KV head's group) against that row's keys; a unit is `1 << key_shift`
-// of an item's keys.  Every CTA of a launch takes an equal run of the units of all rows, whose lengths only the device knows (so a recorded
+// An item is a tile of 2^tq_shift of a row's new tokens, with all query heads of one KV head, against the keys that they see; a unit is 2^key_shift
+// of those keys.  Every CTA of a launch takes an equal run of the units of all rows, whose lengths only the device knows (so a recorded
 // launch serves other lengths when it runs again).  An item that one CTA has to itself is finished there; the pieces of one that is cut meet in
 // the merge kernel.  A piece that does not begin its item is its CTA's first: slot 2 c; one that begins it and does not end it is its last: slot 2 c + 1.
-// Without room for pieces items are not cut.  Keys that no query of an item sees are counted in, but skipped.
+// Without room for pieces items are not cut.  A launch serves the rows whose new tokens times query heads a KV head are above `above` and
+// at most `most`.
 struct PagedPlan {
     PagedView p;
-    int tq, key_shift, whole;
+    int tq_shift, key_shift, whole, group, above, most;
+    int least;                  // units that are worth a CTA
 };
 struct PagedShape {
-    int q_tiles, k_tiles;       // of the row
+    int q_tiles, base;          // of the row; keys before its new tokens
+    long long per;              // units of a head
     long long units;
 };
+// Units of the first n tiles of a row's queries: the sum over i < n of ceil((base + (i + 1) tq) / keys), both powers of two.
+__device__ __forceinline__ long long paged_units(const PagedPlan &a, int base, long long n) {
+    if (a.whole) return n;
+    const int s = a.key_shift - a.tq_shift;
+    if (s <= 0) return n * (((long long)base + (1 << a.key_shift) - 1) >> a.key_shift) + ((n * (n + 1) / 2) << -s);
+    // ceil((b + i + 1) / 2^s) with b = ceil(base / tq): floors of c + i over 2^s, summed up to c + n and without those up to c
+    const long long c = (((long long)base + (1 << a.tq_shift) - 1) >> a.tq_shift) + (1ll << s);
+    auto floors = [&](long long y) { const long long q = y >> s; return (q * (q - 1) / 2 << s) + q * (y & ((1ll << s) - 1)); };
+    return floors(c + n) - floors(c);
+}
 __device__ __forceinline__ PagedShape paged_shape(const PagedPlan &a, const PagedRow &r) {
-    PagedShape s;
-    s.q_tiles = (r.count + a.tq - 1) / a.tq;
-    s.k_tiles = a.whole ? 1 : max(1, (int)(((long long)r.len + (1 << a.key_shift) - 1) >> a.key_shift));
-    s.units = (long long)s.q_tiles * s.k_tiles * a.p.kv_heads;
+    PagedShape s = {0, 0, 0, 0};
+    const long long rows = (long long)r.count * a.group;
+    if (rows <= a.above || rows > a.most) return s;
+    s.q_tiles = (int)(((long long)r.count + (1 << a.tq_shift) - 1) >> a.tq_shift);
+    s.base = max(r.len - r.count, 0);
+    s.per = paged_units(a, s.base, s.q_tiles);
+    s.units = s.per * a.p.kv_heads;
     return s;
 }
 // Sums over a CTA of THREADS threads: returns the thread's exclusive prefix of v, `total` gets the sum.  Every thread calls it.
@@ -103,39 +119,47 @@ struct PagedRun {
     long long u, u1;       // units left to the CTA
     int row;               // that u lies in
     long long row_first;   // the row's first unit
+    long long total;       // units of the launch
+    int ctas;              // that have any
 };
+// Where the run of CTA c begins.
+__device__ __forceinline__ long long paged_begin(const PagedRun &run, int c) { return run.total * min(c, run.ctas) / run.ctas; }
 // The run of CTA `c` of `ctas`, found by the whole CTA.  `found` is shared.
 template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const PagedPlan &a, int c, int ctas, long long *warp_sums, PagedRun *found, int *status) {
-    long long total = 0, n, first_prefix = 0, first_units = 0;
+    PagedRun run = {0, 0, 0, 0, 0, 0};
+    long long n, prefix = 0, units = 0;
     for (int r0 = 0; r0 < a.p.rows; r0 += THREADS) {
         const int r = r0 + threadIdx.x;
-        const long long units = r < a.p.rows ? paged_shape(a, paged_row(a.p, r, c == 0 ? status : nullptr)).units : 0;
-        const long long at = cta_prefix<THREADS>(units, n, warp_sums);
-        if (r0 == 0) { first_prefix = at; first_units = units; }
-        total += n;
+        const long long here = r < a.p.rows ? paged_shape(a, paged_row(a.p, r, c == 0 ? status : nullptr)).units : 0;
+        const long long at = cta_prefix<THREADS>(here, n, warp_sums);
+        if (r0 == 0) { prefix = at; units = here; }
+        run.total += n;
     }
-    const long long u = total * c / ctas, u1 = total * (c + 1) / ctas;
-    if (threadIdx.x == 0) *found = {u, u, 0, 0};  // nothing to do
-    long long before = 0;
-    for (int r0 = 0; r0 < a.p.rows && before <= u; r0 += THREADS) {
-        const int r = r0 + threadIdx.x;
-        long long units = first_units, at = first_prefix;
+    run.ctas = (int)max(1ll, min((long long)ctas, run.total / a.least));
+    run.u = paged_begin(run, c);
+    run.u1 = paged_begin(run, c + 1);
+    if (run.u >= run.u1) return run;
+    // the row whose units the run's first is among; found by one thread
+    for (int r0 = 0;; r0 += THREADS) {
         if (r0 > 0) {
+            const int r = r0 + threadIdx.x;
             units = r < a.p.rows ? paged_shape(a, paged_row(a.p, r, nullptr)).units : 0;
-            at = cta_prefix<THREADS>(units, n, warp_sums);
+            prefix = run.row_first + cta_prefix<THREADS>(units, n, warp_sums);
+        } else if (a.p.rows > THREADS) {
+            (void)cta_prefix<THREADS>(units, n, warp_sums);
         } else {
-            __syncthreads();
-            n = THREADS < a.p.rows ? 0 : total;
-            if (THREADS < a.p.rows) (void)cta_prefix<THREADS>(units, n, warp_sums);
+            n = run.total;
         }
-        at += before;
-        if (u < u1 && units > 0 && u >= at && u < at + units) *found = {u, u1, r, at};
-        before += n;
+        if (units > 0 && run.u >= prefix && run.u < prefix + units) { found->row = r0 + threadIdx.x; found->row_first = prefix; }
+        if (run.u < run.row_first + n) break;
+        run.row_first += n;
     }
     __syncthreads();
-    return *found;
+    run.row = found->row;
+    run.row_first = found->row_first;
+    return run;
 }
-// A piece of work: tiles [k0, k1) of the item (row, head, q_tile), which has k_tiles of them.
+// A piece of work: units [k0, k1) of the item (row, head, q_tile), which has k_tiles of them.
 struct PagedPiece {
     int row, head, q_tile, k0, k1, k_tiles;
     PagedRow r;
@@ -151,16 +175,63 @@ __device__ __forceinline__ bool paged_next(const PagedPlan &a, PagedRun &run, Pa
         run.row_first += s.units;
         if (++run.row >= a.p.rows) return false;
     }
-    const long long in = run.u - run.row_first;
-    const int item = (int)(in / s.k_tiles);
+    long long in = run.u - run.row_first;
     w.row = run.row;
-    w.k_tiles = s.k_tiles;
-    w.k0 = (int)(in - (long long)item * s.k_tiles);
-    w.k1 = (int)min((long long)s.k_tiles, w.k0 + (run.u1 - run.u));
-    w.head = item / s.q_tiles;
-    w.q_tile = item - w.head * s.q_tiles;
+    w.head = (int)(in / s.per);
+    in -= w.head * s.per;
+    int lo = 0, hi = s.q_tiles - 1;   // the tile that unit `in` is of
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (paged_units(a, s.base, mid) <= in) lo = mid;
+        else hi = mid - 1;
+    }
+    const long long first = paged_units(a, s.base, lo);
+    w.q_tile = lo;
+    w.k_tiles = (int)(paged_units(a, s.base, lo + 1) - first);
+    w.k0 = (int)(in - first);
+    w.k1 = (int)min((long long)w.k_tiles, w.k0 + (run.u1 - run.u));
     run.u += w.k1 - w.k0;
     return true;
 }
+// What a piece covers: its tokens [t0, t0 + ntok) of the row's new ones, and the keys [lo, hi) of it that any of them sees.
+struct PagedSpan {
+    int t0, ntok, base, lo, hi;
+};
+__device__ __forceinline__ PagedSpan paged_span(const PagedPlan &a, const PagedPiece &w) {
+    PagedSpan s;
+    s.t0 = w.q_tile << a.tq_shift;
+    s.ntok = min(1 << a.tq_shift, w.r.count - s.t0);
+    s.base = w.r.len - w.r.count;
+    const int last = s.base + s.t0 + s.ntok;   // behind the last key that a token of the item sees
+    s.lo = a.whole ? 0 : (int)min((long long)w.k0 << a.key_shift, 0x7fffffffll);
+    s.hi = a.whole ? last : (int)min((long long)last, (long long)w.k1 << a.key_shift);
+    return s;
+}
+
+struct PagedAttnArgs {
+    PagedPlan plan;
+    const void *q, *k, *v;
+    void *out;
+    long long q_stride, o_stride;
+    float sl;          // scale in powers of two
+    float *acc, *ml;   // pieces: [2 ctas][rows of a tile][dim] sums, [2 ctas][rows of a tile][2] maximum and sum of weights
+    int ctas, tile_rows;
+    int *status;
+};
+// Bytes that the pieces of a launch take.
+static inline size_t paged_piece_bytes(int ctas, int tile_rows, int hd) { return (size_t)2 * ctas * tile_rows * (hd + 2) * 4; }
+static inline int paged_log2(int n) { return 31 - __builtin_clz(n); }
+// Sets how a launch of `ctas` CTAs, tiles of `tile_rows` query rows and 2^key_shift keys deals its work out, cutting items where the workspace has room.
+static inline void paged_deal(PagedAttnArgs &a, int ctas, int tile_rows, int key_shift, int least, int hd, void *workspace, size_t bytes) {
+    a.ctas = ctas; a.tile_rows = tile_rows;
+    a.plan.tq_shift = paged_log2(tile_rows / a.plan.group);
+    a.plan.key_shift = key_shift;
+    a.plan.whole = !workspace || bytes < paged_piece_bytes(ctas, tile_rows, hd);
+    a.plan.least = a.plan.whole ? 1 : least;
+    a.acc = (float *)workspace;
+    a.ml = a.acc + (size_t)2 * ctas * tile_rows * hd;
+}
+// Finishes the items that the launch before it cut.
+int paged_merge(const PagedAttnArgs &a, int hd, ab2_dtype dtype, cudaStream_t s);
 
 }  // namespace ab2

@@ -220,7 +220,7 @@ int paged_check(const ab2_paged *c, ab2_dtype dtype) {
     AB2_REQUIRE(c->pages > 0 && c->kv_heads > 0 && c->rows > 0 && c->tokens >= 0 && c->table_width > 0, AB2_ERR_BAD_SHAPE,
                 "paged cache of %d pages, %d heads, %d rows of %d pages, %d tokens", c->pages, c->kv_heads, c->rows, c->table_width, c->tokens);
     AB2_REQUIRE(c->table_stride >= c->table_width, AB2_ERR_BAD_SHAPE, "table rows of %d pages lie %lld apart", c->table_width, c->table_stride);
-    AB2_REQUIRE((long long)c->table_width * c->page_size < (1ll << 31) && (long long)c->kv_heads * c->page_size < (1ll << 31), AB2_ERR_BAD_SHAPE, "rows of 2^31 tokens or more");
+    AB2_REQUIRE((long long)c->table_width * c->page_size < (1ll << 31) && (long long)c->kv_heads * c->page_size < (1ll << 31) && (long long)c->kv_heads * c->pages < (1ll << 31), AB2_ERR_BAD_SHAPE, "rows of 2^31 tokens or more");
     AB2_REQUIRE(c->starts || c->tokens == c->rows, AB2_ERR_BAD_SHAPE, "%d tokens for %d rows of one token each", c->tokens, c->rows);
     AB2_REQUIRE((((uintptr_t)c->k_pages | (uintptr_t)c->v_pages) & 15) == 0, AB2_ERR_BAD_ALIGN, "pages must be 16-byte aligned");
     return AB2_OK;

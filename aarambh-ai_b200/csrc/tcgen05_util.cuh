@@ -223,6 +223,9 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};\n" ::AB2_REGS32("r", v), "r"(addr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n" ::AB2_REGS16("r", v), "r"(addr) : "memory");
+}
 // A wait of a whole warp, with one answer for it.  Lanes that left a loop after a wait while others went on would leave those
 // waiting for them in the warp's next collective instruction for good.  So the warps of the GEMMs that execute any do not
 // leave: after a time-out they walk through the rest of their work, whose waits then give up at once, over whatever the

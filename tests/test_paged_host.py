@@ -132,53 +132,78 @@ def bounded(starts, lens, b, tokens, capacity):
     return first, min(max(s1, first), tokens) - first, min(max(lens[b], 0), capacity)
 
 
-def shape(count, length, tq, shift, whole, kv_heads):
-    q, k = -(-count // tq), 1 if whole else max(1, -(-length // (1 << shift)))
-    return q, k, q * k * kv_heads
+def units(base, n, ts, ks, whole):
+    """paged_units: its closed forms."""
+    if whole:
+        return n
+    s = ks - ts
+    if s <= 0:
+        return n * ((base + (1 << ks) - 1) >> ks) + ((n * (n + 1) // 2) << -s)
+    c = ((base + (1 << ts) - 1) >> ts) + (1 << s)
+    floors = lambda y: (((y >> s) * ((y >> s) - 1) // 2) << s) + (y >> s) * (y & ((1 << s) - 1))  # noqa: E731
+    return floors(c + n) - floors(c)
+
+
+def test_units_are_the_keys_that_a_tile_of_queries_sees():
+    rng = random.Random(2)
+    for _ in range(2000):
+        base, n, ts, ks = rng.choice([0, 1, 5, 64, 127, 128, rng.randint(0, 70000)]), rng.randint(0, 60), rng.randint(0, 8), rng.choice([5, 6, 7])
+        assert units(base, n, ts, ks, False) == sum(-(-(base + ((i + 1) << ts)) // (1 << ks)) for i in range(n))
 
 
 @pytest.mark.parametrize("whole", [False, True])
 def test_every_unit_of_work_is_done_once_and_cut_items_are_finished(whole):
     rng = random.Random(3)
-    for trial in range(300):
-        rows, kv_heads, ctas = rng.randint(1, 9), rng.randint(1, 4), rng.choice([2, 7, 296])
-        tq, shift = rng.choice([1, 2, 8, 16]), 6
+    for trial in range(400):
+        rows, kv_heads, most_ctas, group = rng.randint(1, 9), rng.randint(1, 4), rng.choice([2, 7, 296]), rng.choice([1, 3, 4, 8])
+        ts, ks, least = rng.choice([(0, 6, 1), (1, 6, 2), (3, 6, 1), (6, 7, 4), (8, 7, 4)])
+        above, most = rng.choice([(0, 2 ** 31 - 1), (32, 2 ** 31 - 1), (0, 32)])
+        least = 1 if whole else least
         lens = [rng.choice([0, 1, 63, 64, 65, 500, 4000]) for _ in range(rows)]
         new = [rng.choice([0, 1, min(2, n), n // 2, n]) if n else 0 for n in lens]
-        shapes = [shape(c, n, tq, shift, whole, kv_heads) for c, n in zip(new, lens)]
-        total = sum(s[2] for s in shapes)
-        begin = [total * c // ctas for c in range(ctas + 1)]
+        tiles = [-(-c // (1 << ts)) if above < c * group <= most else 0 for c in new]
+        per = [units(n - c, q, ts, ks, whole) for n, c, q in zip(lens, new, tiles)]
+        total = kv_heads * sum(per)
+        ctas = max(1, min(most_ctas, total // least))
+        begin = [total * min(c, ctas) // ctas for c in range(most_ctas + 1)]
         done, slots, merged = {}, {}, []
-        for c in range(ctas):
-            u = begin[c]
-            last = None
+        for c in range(most_ctas):
+            u, last = begin[c], None
             while u < begin[c + 1]:
                 before, row = 0, 0
-                while u >= before + shapes[row][2]:
-                    before += shapes[row][2]
+                while u >= before + per[row] * kv_heads:
+                    before += per[row] * kv_heads
                     row += 1
-                qt, kt, _ = shapes[row]
-                item, k0 = divmod(u - before, kt)
+                head, at = divmod(u - before, per[row])
+                lo, hi = 0, tiles[row] - 1
+                while lo < hi:
+                    mid = (lo + hi + 1) // 2
+                    lo, hi = (mid, hi) if units(lens[row] - new[row], mid, ts, ks, whole) <= at else (lo, mid - 1)
+                first, kt = units(lens[row] - new[row], lo, ts, ks, whole), units(lens[row] - new[row], lo + 1, ts, ks, whole) - units(lens[row] - new[row], lo, ts, ks, whole)
+                k0 = at - first
                 k1 = min(kt, k0 + begin[c + 1] - u)
-                head, tile = divmod(item, qt)
-                assert head < kv_heads and tile * tq < new[row]
+                assert head < kv_heads and lo << ts < new[row] and 0 <= k0 < k1 <= kt
                 for k in range(k0, k1):
-                    assert done.setdefault((row, head, tile, k), c) == c
+                    assert done.setdefault((row, head, lo, k), c) == c
                 if (k0, k1) != (0, kt):
                     assert not whole
                     slot = 2 * c + (k0 == 0)
                     assert slot not in slots
-                    slots[slot] = (row, head, tile)
+                    slots[slot] = (row, head, lo)
                 u += k1 - k0
-                last = (row, head, tile, k0, k1, kt, u + kt - k1)
-            if last and last[3] == 0 and last[4] < last[5] and c < ctas - 1:
+                last = (row, head, lo, k0, k1, kt, u + kt - k1)
+            if last and last[3] == 0 and last[4] < last[5]:
+                assert c < most_ctas - 1
                 to = c + 1
                 while to + 1 < ctas and begin[to + 1] < last[6]:
                     to += 1
-                merged.append((last[:3], [2 * j + (j == c) for j in range(c, to + 1) if begin[j] < begin[j + 1]]))
+                merged.append((last[:3], [2 * j + (j == c) for j in range(c, to + 1)]))
         assert len(done) == total
         assert sorted(s for _, m in merged for s in m) == sorted(slots)
         assert all(slots[s] == item for item, m in merged for s in m)
+        want = {(r, h, i, k) for r in range(rows) for h in range(kv_heads) for i in range(tiles[r])
+                for k in range(1 if whole else -(-(lens[r] - new[r] + ((i + 1) << ts)) // (1 << ks)))}
+        assert want == set(done)
 
 
 def test_no_table_length_or_start_leads_out_of_the_buffers():
