@@ -6,6 +6,7 @@
 // One pass over the keys: each tile of scores moves m, rescales what has been summed, and adds its weights and values.  Scores, weights,
 // their sums and the sums of values are f32.  A query that sees no key answers zeros.
 //
+// This file: f32, on CUDA cores; attention_paged_mma.cu and attention_paged_tc.cu: bf16.
 // A CTA multiplies the queries of a KV head's whole group (tokens x heads of the group, up to QR rows) with a tile of 32 keys on CUDA cores;
 // keys and values come by cp.async, the next tile's while this one's are looked at.
 #include <algorithm>
@@ -17,17 +18,19 @@ using namespace ab2;
 namespace ab2 {
 int paged_check(const ab2_paged *c, ab2_dtype dtype);
 PagedView paged_view(const ab2_paged *c);
+size_t paged_mma_bytes(int hd);
+int paged_mma_attention(const PagedAttnArgs &a, int hd, int max_new, void *workspace, size_t bytes, cudaStream_t s);
 size_t paged_tc_bytes(int hd);
 int paged_tc_attention(const PagedAttnArgs &a, int hd, void *workspace, size_t bytes, cudaStream_t s);
-constexpr int PAGED_FEW_ROWS = 32;   // query rows of a KV head up to which the tensor-memory kernel's tiles of 128 would be nearly empty
+constexpr int PAGED_FEW_ROWS = 16;   // query rows of a KV head up to which the tensor-memory kernel's tiles of 128 would be nearly empty
 namespace {
 
 constexpr int PA_THREADS = 128, PA_KEYS = 32;
 
-template <typename T, int HD, int QR> struct SimtShape {
+template <int HD, int QR> struct SimtShape {
     static constexpr int TX = QR == 32 ? 8 : 16, RPT = QR * TX / PA_THREADS, KPT = PA_KEYS / TX, DPT = HD / TX;
-    static constexpr int KROW = HD + 16 / (int)sizeof(T);                     // a row's bank moves on by 16 bytes
-    static constexpr int BUF = PA_KEYS * KROW * (int)sizeof(T);
+    static constexpr int KROW = HD + 4;                     // a row's bank moves on by 16 bytes
+    static constexpr int BUF = PA_KEYS * KROW * 4;
     static constexpr int SMEM = 4 * BUF + QR * (HD + 4) * 4 + QR * (PA_KEYS + 1) * 4;
 };
 
@@ -35,19 +38,14 @@ __device__ __forceinline__ void cp16(void *dst, const void *src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
-__device__ __forceinline__ float4 load4(const __nv_bfloat16 *p) {
-    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
-}
-
-template <typename T, int HD, int QR>
+template <int HD, int QR>
 __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_constant__ PagedAttnArgs a) {
-    using S = SimtShape<T, HD, QR>;
-    constexpr int TX = S::TX, RPT = S::RPT, KPT = S::KPT, DPT = S::DPT, KROW = S::KROW, CH = 16 / (int)sizeof(T);
+    using S = SimtShape<HD, QR>;
+    constexpr int TX = S::TX, RPT = S::RPT, KPT = S::KPT, DPT = S::DPT, KROW = S::KROW, CH = 4;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ long long warp_sums[PA_THREADS / 32];
     __shared__ PagedRun found;
-    T *kbuf = (T *)smem, *vbuf = kbuf + 2 * PA_KEYS * KROW;
+    float *kbuf = (float *)smem, *vbuf = kbuf + 2 * PA_KEYS * KROW;
     float *qs = (float *)(smem + 4 * S::BUF), *ps = qs + QR * (HD + 4);
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     const PagedView &p = a.plan.p;
@@ -60,7 +58,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
         for (int i = threadIdx.x; i < QR * HD / 4; i += PA_THREADS) {
             const int r = i / (HD / 4), d = i % (HD / 4) * 4, tok = r / group, g = r - tok * group;
             float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (tok < ntok) f = load4((const T *)a.q + (size_t)(w.r.first + t0 + tok) * a.q_stride + (size_t)(w.head * group + g) * HD + d);
+            if (tok < ntok) f = load4((const float *)a.q + (size_t)(w.r.first + t0 + tok) * a.q_stride + (size_t)(w.head * group + g) * HD + d);
             *reinterpret_cast<float4 *>(qs + r * (HD + 4) + d) = make_float4(f.x * a.sl, f.y * a.sl, f.z * a.sl, f.w * a.sl);
         }
         // rows past the last key read as zeros
@@ -70,8 +68,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
                 const bool in = key < hi;
                 const int at = in ? key : lo;
                 const size_t row = (((size_t)paged_page(p, w.row, at, a.status) * p.kv_heads + w.head) << p.page_shift) + (at & ((1 << p.page_shift) - 1));
-                cp16(kbuf + (buf * PA_KEYS + j) * KROW + d, (const T *)a.k + row * HD + d, in);
-                cp16(vbuf + (buf * PA_KEYS + j) * KROW + d, (const T *)a.v + row * HD + d, in);
+                cp16(kbuf + (buf * PA_KEYS + j) * KROW + d, (const float *)a.k + row * HD + d, in);
+                cp16(vbuf + (buf * PA_KEYS + j) * KROW + d, (const float *)a.v + row * HD + d, in);
             }
             asm volatile("cp.async.commit_group;\n" ::: "memory");
         };
@@ -171,11 +169,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
             if (tok >= ntok) continue;
             if (all) {
                 const float f = sum[i] == 0.f ? 0.f : 1.f / sum[i];
-                T *dst = (T *)a.out + (size_t)(w.r.first + t0 + tok) * a.o_stride + (size_t)(w.head * group + g) * HD;
+                float *dst = (float *)a.out + (size_t)(w.r.first + t0 + tok) * a.o_stride + (size_t)(w.head * group + g) * HD;
 #pragma unroll
-                for (int d = 0; d < DPT; d += 4)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) dst[tx * 4 + d * TX + e] = from_f32<T>(o[i][d + e] * f);
+                for (int d = 0; d < DPT; d += 4) *reinterpret_cast<float4 *>(dst + tx * 4 + d * TX) = make_float4(o[i][d] * f, o[i][d + 1] * f, o[i][d + 2] * f, o[i][d + 3] * f);
             } else {
                 float *dst = a.acc + (slot * QR + r) * HD;
 #pragma unroll
@@ -225,28 +221,27 @@ __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const __grid_co
 
 int simt_ctas() { return 2 * device_sm_count(); }
 
-template <typename T, int HD, int QR>
+template <int HD, int QR>
 int launch_simt(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
-    using S = SimtShape<T, HD, QR>;
+    using S = SimtShape<HD, QR>;
     static bool configured[64] = {false};  // the attribute is per device
     int dev = 0;
     AB2_CUDA(cudaGetDevice(&dev));
     AB2_REQUIRE(dev >= 0 && dev < 64, AB2_ERR_BAD_ARG, "device index %d out of range", dev);
     if (!configured[dev]) {
-        AB2_CUDA(cudaFuncSetAttribute(paged_simt_kernel<T, HD, QR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+        AB2_CUDA(cudaFuncSetAttribute(paged_simt_kernel<HD, QR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
         configured[dev] = true;
     }
     paged_deal(a, simt_ctas(), QR, 6, 1, HD, workspace, bytes);
-    paged_simt_kernel<T, HD, QR><<<a.ctas, PA_THREADS, S::SMEM, s>>>(a);
+    paged_simt_kernel<HD, QR><<<a.ctas, PA_THREADS, S::SMEM, s>>>(a);
     AB2_LAUNCH_CHECK();
-    return a.plan.whole ? AB2_OK : paged_merge(a, HD, ActType<T>::value, s);
+    return a.plan.whole ? AB2_OK : paged_merge(a, HD, AB2_F32, s);
 }
 
-template <typename T>
 int simt_attention(const PagedAttnArgs &a, int hd, int max_new, void *workspace, size_t bytes, cudaStream_t s) {
     const bool few = max_new * (long long)a.plan.group <= 8;
-    if (hd == 128) return few ? launch_simt<T, 128, 8>(a, workspace, bytes, s) : launch_simt<T, 128, 32>(a, workspace, bytes, s);
-    return few ? launch_simt<T, 64, 8>(a, workspace, bytes, s) : launch_simt<T, 64, 32>(a, workspace, bytes, s);
+    if (hd == 128) return few ? launch_simt<128, 8>(a, workspace, bytes, s) : launch_simt<128, 32>(a, workspace, bytes, s);
+    return few ? launch_simt<64, 8>(a, workspace, bytes, s) : launch_simt<64, 32>(a, workspace, bytes, s);
 }
 
 }  // namespace
@@ -266,7 +261,7 @@ int paged_merge(const PagedAttnArgs &a, int hd, ab2_dtype dtype, cudaStream_t s)
 AB2_API int ab2_paged_workspace(int head_dim, size_t *bytes) {
     AB2_REQUIRE(bytes, AB2_ERR_BAD_ARG, "null argument");
     AB2_REQUIRE(head_dim == 64 || head_dim == 128, AB2_ERR_UNSUPPORTED, "paged caches have heads of 64 or 128, not %d", head_dim);
-    *bytes = std::max(paged_piece_bytes(simt_ctas(), 32, head_dim), paged_tc_bytes(head_dim));
+    *bytes = std::max(std::max(paged_piece_bytes(simt_ctas(), 32, head_dim), paged_mma_bytes(head_dim)), paged_tc_bytes(head_dim));
     return AB2_OK;
 }
 
@@ -288,12 +283,17 @@ AB2_API int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long 
     a.plan.group = heads / cache->kv_heads; a.plan.above = 0; a.plan.most = 0x7fffffff; a.sl = scale * 1.44269504088896341f;
     rc = device_status_word(&a.status);
     if (rc != AB2_OK) return rc;
-    if (dtype == AB2_F32) return simt_attention<float>(a, cache->head_dim, max_new, workspace_dev, workspace_bytes, (cudaStream_t)stream);
-    const bool chunks = cache->starts && (long long)max_new * a.plan.group > PAGED_FEW_ROWS;   // there may be rows for the tensor-memory kernel
-    if (chunks) a.plan.most = PAGED_FEW_ROWS;
-    rc = simt_attention<__nv_bfloat16>(a, cache->head_dim, max_new, workspace_dev, workspace_bytes, (cudaStream_t)stream);
-    if (rc != AB2_OK || !chunks) return rc;
-    a.plan.above = PAGED_FEW_ROWS;
-    a.plan.most = 0x7fffffff;
+    if (!cache->starts) max_new = 1;
+    if (dtype == AB2_F32) return simt_attention(a, cache->head_dim, max_new, workspace_dev, workspace_bytes, (cudaStream_t)stream);
+    // Rows of up to 16 query rows a KV head go to the warp-level kernel, the others to the tensor-memory kernel; a launch for which there can be no row is
+    // left out.  Rows with more new tokens than they were said to have are served all the same.
+    const bool few = a.plan.group <= PAGED_FEW_ROWS, chunks = (long long)max_new * a.plan.group > PAGED_FEW_ROWS;
+    if (few) {
+        if (chunks) a.plan.most = PAGED_FEW_ROWS;
+        rc = paged_mma_attention(a, cache->head_dim, max_new, workspace_dev, workspace_bytes, (cudaStream_t)stream);
+        if (rc != AB2_OK || !chunks) return rc;
+        a.plan.above = PAGED_FEW_ROWS;
+        a.plan.most = 0x7fffffff;
+    }
     return paged_tc_attention(a, cache->head_dim, workspace_dev, workspace_bytes, (cudaStream_t)stream);
 }

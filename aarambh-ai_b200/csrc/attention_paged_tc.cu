@@ -130,41 +130,6 @@ __device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, flo
     sum += (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// A row of a piece over the keys [lo, to] of it that it sees, by one warp: a lane has every 32nd dimension.
-template <int HD>
-__device__ __forceinline__ void pc_again(const PagedAttnArgs &a, const PcPiece &x, int r, int lane, bool all, size_t slot) {
-    constexpr int N = HD / 32;
-    const int tok = r / a.plan.group, head = x.w.head * a.plan.group + r % a.plan.group;
-    const int to = min(x.s.hi - 1, x.s.base + x.s.t0 + tok);
-    const __nv_bfloat16 *q = (const __nv_bfloat16 *)a.q + (size_t)(x.w.r.first + x.s.t0 + tok) * a.q_stride + (size_t)head * HD;
-    float qv[N], acc[N] = {}, top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) qv[i] = __bfloat162float(q[lane + 32 * i]) * a.sl;
-    for (int key = x.s.lo; key <= to; ++key) {
-        const size_t row = (((size_t)paged_page(a.plan.p, x.w.row, key, a.status) * a.plan.p.kv_heads + x.w.head) << a.plan.p.page_shift) + (key & ((1 << a.plan.p.page_shift) - 1));
-        float s = 0.f, vv[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            s = fmaf(qv[i], __bfloat162float(((const __nv_bfloat16 *)a.k)[row * HD + lane + 32 * i]), s);
-            vv[i] = __bfloat162float(((const __nv_bfloat16 *)a.v)[row * HD + lane + 32 * i]);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        const float best = fmaxf(top, s), m = best == -INFINITY ? 0.f : best, keep = exp2f(top - m), w = exp2f(s - m);
-        sum = sum * keep + w;
-#pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] = fmaf(w, vv[i], acc[i] * keep);
-        top = best;
-    }
-    const float f = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (all) ((__nv_bfloat16 *)a.out)[(size_t)(x.w.r.first + x.s.t0 + tok) * a.o_stride + (size_t)head * HD + lane + 32 * i] = __float2bfloat16_rn(acc[i] * f);
-        else a.acc[(slot + r) * HD + lane + 32 * i] = acc[i];
-    }
-    if (!all && lane == 0) *reinterpret_cast<float2 *>(a.ml + (slot + r) * 2) = make_float2(top, sum);
-}
-
 template <int HD>
 __global__ void __launch_bounds__(PC_THREADS, 1)
 paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PagedAttnArgs a) {
@@ -366,7 +331,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             if (!all && rr < rows) *reinterpret_cast<float2 *>(a.ml + (slot + rr) * 2) = make_float2(top, sum);
             __syncwarp();
             for (uint32_t left = __ballot_sync(0xffffffffu, rr < rows && poison != 0.f); left; left &= left - 1)  // NaN is not 0
-                pc_again<HD>(a, x, g * PC_Q + quad * 32 + __ffs(left) - 1, lane, all, slot);
+                paged_again<HD>(a, x.w, x.s, g * PC_Q + quad * 32 + __ffs(left) - 1, lane, all, slot);
             // the next piece's products may go over what has been read
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
         }

@@ -95,6 +95,7 @@ __device__ __forceinline__ PagedShape paged_shape(const PagedPlan &a, const Page
     return s;
 }
 // Sums over a CTA of THREADS threads: returns the thread's exclusive prefix of v, `total` gets the sum.  Every thread calls it.
+// A warp by itself (THREADS 32) needs no shared memory and no other warp.
 template <int THREADS> __device__ __forceinline__ long long cta_prefix(long long v, long long &total, long long *warp_sums) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     long long x = v;
@@ -102,6 +103,10 @@ template <int THREADS> __device__ __forceinline__ long long cta_prefix(long long
     for (int o = 1; o < 32; o <<= 1) {
         const long long y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
+    }
+    if (THREADS == 32) {
+        total = __shfl_sync(0xffffffffu, x, 31);
+        return x - v;
     }
     __syncthreads();  // the last call's sums have been read
     if (lane == 31) warp_sums[warp] = x;
@@ -124,12 +129,12 @@ struct PagedRun {
 };
 // Where the run of CTA c begins.
 __device__ __forceinline__ long long paged_begin(const PagedRun &run, int c) { return run.total * min(c, run.ctas) / run.ctas; }
-// The run of CTA `c` of `ctas`, found by the whole CTA.  `found` is shared.
+// The run of CTA (or, with THREADS 32, warp) `c` of `ctas`, found by all its threads.  `found` is shared.
 template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const PagedPlan &a, int c, int ctas, long long *warp_sums, PagedRun *found, int *status) {
     PagedRun run = {0, 0, 0, 0, 0, 0};
     long long n, prefix = 0, units = 0;
     for (int r0 = 0; r0 < a.p.rows; r0 += THREADS) {
-        const int r = r0 + threadIdx.x;
+        const int r = r0 + (int)(threadIdx.x % THREADS);
         const long long here = r < a.p.rows ? paged_shape(a, paged_row(a.p, r, c == 0 ? status : nullptr)).units : 0;
         const long long at = cta_prefix<THREADS>(here, n, warp_sums);
         if (r0 == 0) { prefix = at; units = here; }
@@ -142,7 +147,7 @@ template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const Paged
     // the row whose units the run's first is among; found by one thread
     for (int r0 = 0;; r0 += THREADS) {
         if (r0 > 0) {
-            const int r = r0 + threadIdx.x;
+            const int r = r0 + (int)(threadIdx.x % THREADS);
             units = r < a.p.rows ? paged_shape(a, paged_row(a.p, r, nullptr)).units : 0;
             prefix = run.row_first + cta_prefix<THREADS>(units, n, warp_sums);
         } else if (a.p.rows > THREADS) {
@@ -150,11 +155,12 @@ template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const Paged
         } else {
             n = run.total;
         }
-        if (units > 0 && run.u >= prefix && run.u < prefix + units) { found->row = r0 + threadIdx.x; found->row_first = prefix; }
+        if (units > 0 && run.u >= prefix && run.u < prefix + units) { found->row = r0 + (int)(threadIdx.x % THREADS); found->row_first = prefix; }
         if (run.u < run.row_first + n) break;
         run.row_first += n;
     }
-    __syncthreads();
+    if (THREADS == 32) __syncwarp();
+    else __syncthreads();
     run.row = found->row;
     run.row_first = found->row_first;
     return run;
@@ -208,6 +214,7 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedPlan &a, const PagedP
     return s;
 }
 
+// `ctas` counts runs: CTAs, or warps where each has a run of its own.
 struct PagedAttnArgs {
     PagedPlan plan;
     const void *q, *k, *v;
@@ -231,6 +238,42 @@ static inline void paged_deal(PagedAttnArgs &a, int ctas, int tile_rows, int key
     a.acc = (float *)workspace;
     a.ml = a.acc + (size_t)2 * ctas * tile_rows * hd;
 }
+// Row r of a piece of bf16 over the keys [lo, to] of it that it sees, by one warp, a lane every 32nd dimension: where a product with hidden values
+// has left Inf or NaN (a weight of 0 times either), this gives what the keys in sight alone give.
+template <int HD>
+__device__ __forceinline__ void paged_again(const PagedAttnArgs &a, const PagedPiece &w, const PagedSpan &sp, int r, int lane, bool all, size_t slot) {
+    constexpr int N = HD / 32;
+    const int tok = r / a.plan.group, head = w.head * a.plan.group + r % a.plan.group;
+    const int to = min(sp.hi - 1, sp.base + sp.t0 + tok);
+    const __nv_bfloat16 *q = (const __nv_bfloat16 *)a.q + (size_t)(w.r.first + sp.t0 + tok) * a.q_stride + (size_t)head * HD;
+    float qv[N], acc[N] = {}, top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) qv[i] = __bfloat162float(q[lane + 32 * i]) * a.sl;
+    for (int key = sp.lo; key <= to; ++key) {
+        const size_t row = (((size_t)paged_page(a.plan.p, w.row, key, a.status) * a.plan.p.kv_heads + w.head) << a.plan.p.page_shift) + (key & ((1 << a.plan.p.page_shift) - 1));
+        float s = 0.f, vv[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            s = fmaf(qv[i], __bfloat162float(((const __nv_bfloat16 *)a.k)[row * HD + lane + 32 * i]), s);
+            vv[i] = __bfloat162float(((const __nv_bfloat16 *)a.v)[row * HD + lane + 32 * i]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        const float best = fmaxf(top, s), m = best == -INFINITY ? 0.f : best, keep = exp2f(top - m), e = exp2f(s - m);
+        sum = sum * keep + e;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = fmaf(e, vv[i], acc[i] * keep);
+        top = best;
+    }
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (all) ((__nv_bfloat16 *)a.out)[(size_t)(w.r.first + sp.t0 + tok) * a.o_stride + (size_t)head * HD + lane + 32 * i] = __float2bfloat16_rn(acc[i] * f);
+        else a.acc[(slot + r) * HD + lane + 32 * i] = acc[i];
+    }
+    if (!all && lane == 0) *reinterpret_cast<float2 *>(a.ml + (slot + r) * 2) = make_float2(top, sum);
+}
+
 // Finishes the items that the launch before it cut.
 int paged_merge(const PagedAttnArgs &a, int hd, ab2_dtype dtype, cudaStream_t s);
 

@@ -415,7 +415,7 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     starts: torch.Tensor | None = None, max_new: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """q [tokens, heads, dim]: each row's new tokens, whose keys and values have been appended, attend to the row's keys up to their
     own; table, lens and starts as in ``paged_append``.  ``max_new`` bounds the new tokens of a row (None: not known); it picks
-    kernels and changes no result.  Tokens behind the last row are left as ``out`` holds them."""
+    kernels, whose results differ by rounding.  Tokens behind the last row are left as ``out`` holds them."""
     _on_device(q, k_pages, v_pages, table, lens, starts)
     q, qs = _heads(q, "q")
     n, h, d = q.shape

@@ -388,7 +388,8 @@ int ab2_paged_append(const ab2_paged *cache, const void *k_dev, long long k_stri
                      int heads, void *q_out_dev, long long q_out_stride, const double *frequencies_dev, int rot_dims, int layout, float magnitude, ab2_dtype dtype, ab2_stream stream);
 /* Attention of the new tokens, whose keys and values have been appended: a token sees its row's keys up to its own position, query head
  * j reads KV head j / (heads / kv_heads), up to 32 query heads for one KV head; a token that sees no key answers zeros.  Keys and values out of
- * sight may hold anything.  max_new (at least the most new tokens of a row) picks kernels, results do not rest on it.  workspace_dev
+ * sight may hold anything.  max_new (at least the most new tokens of a row) picks kernels; rows that have more are
+ * answered all the same.  workspace_dev
  * (ab2_paged_workspace bytes, 16-byte aligned, nothing in it is kept between calls) lets long rows be cut between CTAs; NULL: they are not. */
 int ab2_paged_workspace(int head_dim, size_t *bytes);
 int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long long q_stride, int heads, void *out_dev, long long out_stride, int max_new, float scale,
