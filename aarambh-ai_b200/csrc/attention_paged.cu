@@ -50,9 +50,11 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     const PagedView &p = a.plan.p;
     PagedRun run = paged_run<PA_THREADS>(a.plan, blockIdx.x, gridDim.x, warp_sums, &found, a.status);
+    if (threadIdx.x == 0) paged_uncut(a, blockIdx.x);
     PagedPiece w;
     while (paged_next(a.plan, run, w)) {
         const PagedSpan sp = paged_span(a.plan, w);
+        if (threadIdx.x == 0) paged_cut(a, run, w, sp, blockIdx.x);
         const int t0 = sp.t0, ntok = sp.ntok, base = sp.base, lo = sp.lo, hi = sp.hi, group = a.plan.group;
         __syncthreads();
         for (int i = threadIdx.x; i < QR * HD / 4; i += PA_THREADS) {
@@ -182,40 +184,57 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
     }
 }
 
-// The pieces of cut items: CTA c finishes the item that CTA c of the launch before began and did not end.
+// The pieces of cut items: CTA (c, y) finishes rows of the item that run c of the launch before began and did not end.
+constexpr int MERGE_ROWS = 16;   // of a CTA
 template <typename T, int HD>
 __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
-    __shared__ long long warp_sums[PA_THREADS / 32];
-    __shared__ PagedRun found;
+    __shared__ float tops[MERGE_ROWS], sums[MERGE_ROWS];
     pdl_wait();
     const int c = blockIdx.x, group = a.plan.group;
-    PagedRun run = paged_run<PA_THREADS>(a.plan, c, a.ctas, warp_sums, &found, nullptr);
-    PagedPiece w;
-    w.k1 = w.k_tiles = w.k0 = 0;
-    while (paged_next(a.plan, run, w)) {}
-    if (w.k0 != 0 || w.k1 >= w.k_tiles) return;   // the CTA's last piece
-    const long long end = run.u + (w.k_tiles - w.k1);   // the unit behind the item
-    int last = c + 1;   // the CTA that ends it
-    while (last + 1 < run.ctas && paged_begin(run, last + 1) < end) ++last;
-    const PagedSpan sp = paged_span(a.plan, w);
-    auto slot = [&](int i) { return (2 * (size_t)i + (i == c)) * a.tile_rows; };
-    for (int i = threadIdx.x + blockIdx.y * PA_THREADS; i < sp.ntok * group * (HD / 4); i += PA_THREADS * gridDim.y) {
-        const int r = i / (HD / 4), d = i % (HD / 4) * 4, tok = r / group, g = r - tok * group;
-        float top = -INFINITY;
-        for (int j = c; j <= last; ++j) top = fmaxf(top, a.ml[(slot(j) + r) * 2]);
-        const float m = top == -INFINITY ? 0.f : top;
-        float sum = 0.f;
+    const int4 cut = a.cut[c];
+    const int rows = cut.y * group - blockIdx.y * MERGE_ROWS, pieces = cut.w - c + 1;
+    if (rows <= 0) return;
+    // run c's piece is its last, the others' is their first: slots 2 c + 1, 2 c + 2, 2 c + 4, ...
+    const size_t row0 = (size_t)blockIdx.y * MERGE_ROWS;
+    auto slot = [&](int j) { return (2 * (size_t)(c + j) + (j == 0)) * a.tile_rows + row0; };
+    // a row's maximum over all pieces, and the sum of its weights relative to it: 8 lanes a row
+    for (int r = threadIdx.x >> 3; r < MERGE_ROWS; r += PA_THREADS / 8) {
+        float top = -INFINITY, sum = 0.f;
+        if (r < rows) {
+#pragma unroll 4
+            for (int j = threadIdx.x & 7; j < pieces; j += 8) {
+                const float2 ml = *reinterpret_cast<const float2 *>(a.ml + (slot(j) + r) * 2);
+                const float best = fmaxf(top, ml.x), m = best == -INFINITY ? 0.f : best;
+                sum = sum * exp2f(top - m) + ml.y * exp2f(ml.x - m);
+                top = best;
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            const float t = __shfl_xor_sync(0xffffffffu, top, o), s = __shfl_xor_sync(0xffffffffu, sum, o), best = fmaxf(top, t), m = best == -INFINITY ? 0.f : best;
+            // in the same order on both sides, so that all lanes have the same bits
+            const float lo = (threadIdx.x & o) ? s * exp2f(t - m) : sum * exp2f(top - m), hi = (threadIdx.x & o) ? sum * exp2f(top - m) : s * exp2f(t - m);
+            sum = lo + hi;
+            top = best;
+        }
+        if ((threadIdx.x & 7) == 0) { tops[r] = top == -INFINITY ? 0.f : top; sums[r] = sum; }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(rows, MERGE_ROWS) * (HD / 4); i += PA_THREADS) {
+        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int j = c; j <= last; ++j) {
-            const float2 ml = *reinterpret_cast<const float2 *>(a.ml + (slot(j) + r) * 2);
-            const float f = exp2f(ml.x - m);
+#pragma unroll 8
+        for (int j = 0; j < pieces; ++j) {
+            const float f = exp2f(a.ml[(slot(j) + r) * 2] - tops[r]);
             const float4 v = *reinterpret_cast<const float4 *>(a.acc + (slot(j) + r) * HD + d);
-            sum = fmaf(f, ml.y, sum);
             o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
         }
-        const float f = sum == 0.f ? 0.f : 1.f / sum;
-        T *dst = (T *)a.out + (size_t)(w.r.first + sp.t0 + tok) * a.o_stride + (size_t)(w.head * group + g) * HD + d;
-        dst[0] = from_f32<T>(o.x * f); dst[1] = from_f32<T>(o.y * f); dst[2] = from_f32<T>(o.z * f); dst[3] = from_f32<T>(o.w * f);
+        const float f = sums[r] == 0.f ? 0.f : 1.f / sums[r];
+        const int row = (int)row0 + r, tok = row / group;
+        T *dst = (T *)a.out + (size_t)(cut.x + tok) * a.o_stride + (size_t)(cut.z * group + row - tok * group) * HD + d;
+        alignas(16) T y[4] = {from_f32<T>(o.x * f), from_f32<T>(o.y * f), from_f32<T>(o.z * f), from_f32<T>(o.w * f)};
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(y);
+        else *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(y);
     }
 }
 
@@ -248,7 +267,7 @@ int simt_attention(const PagedAttnArgs &a, int hd, int max_new, void *workspace,
 
 int paged_merge(const PagedAttnArgs &a, int hd, ab2_dtype dtype, cudaStream_t s) {
     ChainedLaunches chained(true);
-    const dim3 grid(a.ctas - 1, std::max(1, a.tile_rows / 32));
+    const dim3 grid(a.ctas, (a.tile_rows + MERGE_ROWS - 1) / MERGE_ROWS);
     auto kernel = dtype == AB2_F32 ? (hd == 128 ? paged_merge_kernel<float, 128> : paged_merge_kernel<float, 64>)
                                    : (hd == 128 ? paged_merge_kernel<__nv_bfloat16, 128> : paged_merge_kernel<__nv_bfloat16, 64>);
     cudaError_t e = launch_kernel(kernel, grid, dim3(PA_THREADS), 0, s, a);

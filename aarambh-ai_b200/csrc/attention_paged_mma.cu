@@ -65,6 +65,7 @@ __global__ void __launch_bounds__(32 * PM_WARPS, 2) paged_mma_kernel(const __gri
     uint8_t *ring = smem + warp * STAGES * S::BLOCK;
     const int me = warp * gridDim.x + blockIdx.x;   // a little work spreads over all SMs
     PagedRun run = paged_run<32>(a.plan, me, a.ctas, nullptr, &found[warp], a.status);
+    if (lane == 0) paged_uncut(a, me);
 
     // ---- the copies run ahead of the products, over the same pieces
     PagedRun ahead = run;
@@ -109,6 +110,7 @@ __global__ void __launch_bounds__(32 * PM_WARPS, 2) paged_mma_kernel(const __gri
     PagedPiece w;
     while (paged_next(a.plan, run, w)) {
         const PagedSpan sp = paged_span(a.plan, w);
+        if (lane == 0) paged_cut(a, run, w, sp, me);
         const int rows = sp.ntok * group;
         // rows of the tile: 8 t + g as columns of Q^T, 8 t + 2 c and 8 t + 2 c + 1 as columns of scores and sums
         uint32_t q[NT][KS][2];

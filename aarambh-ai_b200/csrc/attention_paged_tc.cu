@@ -1,15 +1,18 @@
 // Attention of chunks over a paged bf16 cache on the 5th-generation tensor cores: rows whose new tokens fill more than a warp-level tile.
 // The mathematics is that of attention_paged.cu.  An item is up to 256 query rows, tokens x heads of one KV head's group, in two tiles of 128:
 //
-//   S_g[128 rows][128 keys] = Q_g . K^T          both K-major in shared memory
-//   O_g[128 rows][dim]     += P_g . V            P in tensor memory, where the scores were; V N-major in shared memory
+//   S_g[128 rows][80 keys] = Q_g . K^T          both K-major in shared memory
+//   O_g[128 rows][dim]    += P_g . V            P in tensor memory, V N-major in shared memory
 //
-//   warp 0       TMA producer: pages to tiles of 128 keys, K and V in turn, in a ring
-//   warp 1       MMA issue
+//   warp 0       TMA producer: pages to tiles of 80 keys, K and V in turn, in a ring
+//   warps 1, 2   MMA issue for tile 0 and tile 1
 //   warps 4-7    softmax of tile 0, a thread per row;   warps 8-11   of tile 1
-// While one tile's scores become weights the other's products run.  The weights enter rounded to bf16, half a step (2^-8) each and
-// independent, which the sum over the keys averages; their sum is that of the f32 weights.  Scores, maxima, sums and O are f32.
-// The weights are relative to a maximum per row that moves only when a score exceeds it by 2^8; then O is rescaled in tensor memory.
+// Tiles are of 80 keys because scores (80 columns) and weights (40) of two tiles of rows then fit beside their sums of 128 dimensions in the 512
+// columns of tensor memory: the scores of the next tile are made while the weights of this one are, and a softmax warp never waits for its own
+// products.  (With 128 keys the weights lay over the scores, and scores - softmax - sums was a chain: 0.98 ms where this takes PCTIME, 4096 tokens
+// behind 12288, 32 / 8 heads of 128.)  The weights enter rounded to bf16, half a step (2^-8) each and independent, which the sum over the keys
+// averages; their sum is that of the f32 weights.  Scores, maxima, sums and O are f32.  The weights are relative to a maximum per row that moves only
+// when a score exceeds it by 2^8; then O is rescaled in tensor memory.
 //
 // An MMA multiplies a hidden value by a weight of 0, so an Inf or a NaN there would reach rows that do not see it.  Rows of a page behind the
 // sequence's end are cleared in shared memory; a row whose sums come out as Inf or NaN (a later token's value may hold them) is computed
@@ -26,17 +29,19 @@ using namespace ab2::tc;
 namespace ab2 {
 namespace {
 
-constexpr int PC_Q = 128, PC_KEYS = 128, PC_THREADS = 384, PC_BOX = 128 * 128;  // a box is 128 rows of 64 elements
+constexpr int PC_Q = 128, PC_KEYS = 80, PC_THREADS = 384;
+constexpr int PC_QBOX = PC_Q * 128, PC_BOX = PC_KEYS * 128;   // boxes of queries, and of keys or values: rows of 64 elements
+constexpr int PC_ROWS = 16;   // that one copy brings: the least that a page holds
 constexpr float PC_SLACK = 8.f;  // powers of two a score may exceed the row's maximum by
 constexpr float PC_NONE = -1e30f;
 
 template <int HD> struct PcShape {
-    static constexpr int BOXES = HD / 64, TILE = BOXES * PC_BOX, SLOTS = HD == 128 ? 5 : 8;
-    static constexpr int SMEM = 1024 + (2 + SLOTS) * TILE;
+    static constexpr int BOXES = HD / 64, QTILE = BOXES * PC_QBOX, TILE = BOXES * PC_BOX, SLOTS = HD == 128 ? 4 : 8;   // a slot holds a tile's keys and its values
+    static constexpr int SMEM = 1024 + 2 * QTILE + SLOTS * 2 * TILE;
 };
 
 struct PcShared {
-    uint64_t full[8], empty[8], qfull[2], sfull[2], pfull[2], odone[2];
+    uint64_t full[8], empty[8], qfull[2], sfull[2], sfree[2], pfull[2], odone[2];
     uint32_t tmem_base;
     int failed;
     PagedRun found;
@@ -54,55 +59,78 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// Two f32 at a time.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ float low(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float high(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t x) { return pair(ex2(low(x)), ex2(high(x))); }
 // What all roles know of a piece.
 struct PcPiece {
     PagedPiece w;
     PagedSpan s;
-    int first;      // tile of keys that it begins with
     int tiles[2];   // of keys that a tile of rows looks at
     int most;
 };
 __device__ __forceinline__ bool pc_next(const PagedPlan &a, PagedRun &run, PcPiece &x) {
     if (!paged_next(a, run, x.w)) return false;
     x.s = paged_span(a, x.w);
-    x.first = x.s.lo / PC_KEYS;
     const int rows = x.s.ntok * a.group;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
         // keys up to those of the last token of the tile of rows
         const int last = min(x.s.hi, x.s.base + x.s.t0 + (min(rows, (g + 1) * PC_Q) - 1) / a.group + 1);
-        x.tiles[g] = rows > g * PC_Q ? max(0, (last + PC_KEYS - 1) / PC_KEYS - x.first) : 0;
+        x.tiles[g] = rows > g * PC_Q ? max(0, (last - x.s.lo + PC_KEYS - 1) / PC_KEYS) : 0;
     }
     x.most = max(x.tiles[0], x.tiles[1]);
     return true;
 }
 
-// One tile of keys for the warp's 32 rows, a lane each: scores to weights in tensor memory.  With EDGE keys past `lim` are out of sight.
-template <int HD, bool EDGE>
-__device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, float sl, int lim, bool has_o, float &top, float &sum) {
-    uint32_t v[4][32];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) tmem_ld32_start(v[c], s_addr + 32 * c);
+// One tile of keys for the warp's 32 rows, a lane each: scores to weights.  With EDGE keys past `lim` are out of sight.  `before` waits until the
+// products with the tile before are done: its weights' place is free then, and the sums stand still.
+template <int HD, bool EDGE, class Before>
+__device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, float sl, int lim, bool has_o, float &top, float &sum, uint64_t *taken, uint64_t *ready, Before before) {
+    uint32_t va[32], vb[32], vc[16];
+    tmem_ld32_start(va, s_addr);
+    tmem_ld32_start(vb, s_addr + 32);
+    tmem_ld16_start(vc, s_addr + 64);
+    tmem_ld16_wait(vc);
+    tmem_ld32_wait(va);
+    tmem_ld32_wait(vb);
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) bar_arrive(taken);
+    auto v = [&](int k) -> uint32_t & { return k < 32 ? va[k] : k < 64 ? vb[k - 32] : vc[k - 64]; };
     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        tmem_ld32_wait(v[c]);
+    for (int k = 0; k < PC_KEYS; ++k)
+        if (EDGE && k > lim) v(k) = 0xff800000u;
 #pragma unroll
-        for (int k = 0; k < 32; ++k)
-            if (EDGE && 32 * c + k > lim) v[c][k] = 0xff800000u;
+    for (int k = 0; k < PC_KEYS; k += 8)
 #pragma unroll
-        for (int k = 0; k < 32; k += 8)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(v[c][k + e]), __uint_as_float(v[c][k + 4 + e]));
-    }
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(v(k + e)), __uint_as_float(v(k + 4 + e)));
     const float best = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sl;  // the scale is not negative
     const float now = best > top + PC_SLACK ? best : top;
+    before();
     if (__any_sync(0xffffffffu, now != top)) {
         const float corr = ex2(top - now);
         sum *= corr;
         top = now;
-        // the scores came after the products of the last tile: the sums stand still
         if (has_o) {
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 #pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {
                 uint32_t o[32];
@@ -113,21 +141,47 @@ __device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, flo
             }
         }
     }
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint64_t sl2 = pair(sl, sl), top2 = pair(-top, -top);
+    uint64_t total[2] = {0ull, 0ull};
+    auto weights = [&](int k) {   // of keys k and k + 1
+        const uint64_t e = ex2_pair(fma2(pair(__uint_as_float(v(k)), __uint_as_float(v(k + 1))), sl2, top2));
+        total[(k >> 1) & 1] = add2(total[(k >> 1) & 1], e);
+        const __nv_bfloat162 b = __floats2bfloat162_rn(low(e), high(e));
+        return *reinterpret_cast<const uint32_t *>(&b);
+    };
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < 2; ++c) {
         uint32_t p[16];
 #pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-            const float e0 = ex2(fmaf(__uint_as_float(v[c][k]), sl, -top)), e1 = ex2(fmaf(__uint_as_float(v[c][k + 1]), sl, -top));
-            part[(k >> 1) & 1] += e0;
-            part[2 + ((k >> 1) & 1)] += e1;
-            const __nv_bfloat162 b = __floats2bfloat162_rn(e0, e1);
-            p[k >> 1] = *reinterpret_cast<const uint32_t *>(&b);
-        }
-        tmem_st16(s_addr + 16 * c, p);
+        for (int k = 0; k < 16; ++k) p[k] = weights(32 * c + 2 * k);
+        tmem_st16(s_addr + PC_KEYS + 16 * c, p);
     }
-    sum += (part[0] + part[1]) + (part[2] + part[3]);
+    {
+        uint32_t p[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) p[k] = weights(64 + 2 * k);
+        tmem_st8(s_addr + PC_KEYS + 32, p);
+    }
+    total[0] = add2(total[0], total[1]);
+    sum += low(total[0]) + high(total[0]);
+    asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) bar_arrive(ready);
+}
+
+// Four lanes with four pieces each: piece k of lane i for piece i of lane k.
+__device__ __forceinline__ void exchange4(uint4 (&o)[4], int lane) {
+    auto swap = [](uint4 &a, uint4 &b, bool odd, int d) {   // the even lane's b for the odd lane's a
+        uint4 s = odd ? a : b;
+        s.x = __shfl_xor_sync(0xffffffffu, s.x, d); s.y = __shfl_xor_sync(0xffffffffu, s.y, d); s.z = __shfl_xor_sync(0xffffffffu, s.z, d); s.w = __shfl_xor_sync(0xffffffffu, s.w, d);
+        if (odd) a = s;
+        else b = s;
+    };
+    swap(o[0], o[1], lane & 1, 1);
+    swap(o[2], o[3], lane & 1, 1);
+    swap(o[0], o[2], lane & 2, 2);
+    swap(o[1], o[3], lane & 2, 2);
 }
 
 template <int HD>
@@ -136,16 +190,17 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     using S = PcShape<HD>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ PcShared sh;
-    uint8_t *qbuf = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023), *ring = qbuf + 2 * S::TILE;
+    uint8_t *qbuf = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023), *ring = qbuf + 2 * S::QTILE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *failed = &sh.failed;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::SLOTS; ++i) { bar_init(&sh.full[i], 1); bar_init(&sh.empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { bar_init(&sh.qfull[i], 4); bar_init(&sh.sfull[i], 1); bar_init(&sh.pfull[i], 4); bar_init(&sh.odone[i], 1); }
+        for (int i = 0; i < S::SLOTS; ++i) { bar_init(&sh.full[i], 1); bar_init(&sh.empty[i], 2); }
+        for (int i = 0; i < 2; ++i) { bar_init(&sh.qfull[i], 4); bar_init(&sh.sfull[i], 1); bar_init(&sh.sfree[i], 4); bar_init(&sh.pfull[i], 4); bar_init(&sh.odone[i], 1); }
         sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     PagedRun run = paged_run<PC_THREADS>(a.plan, blockIdx.x, a.ctas, sh.warp_sums, &sh.found, a.status);
+    if (threadIdx.x == PC_THREADS - 1) paged_uncut(a, blockIdx.x);
     if (run.u >= run.u1) return;   // the whole CTA
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(sptr(&sh.tmem_base)));
@@ -154,7 +209,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-    const uint32_t tmem = sh.tmem_base, tmem_o = tmem + 2 * PC_KEYS;
+    const uint32_t tmem = sh.tmem_base, tmem_o = tmem + 256;   // a tile of rows has 128 columns for scores and weights
     const PagedView &p = a.plan.p;
     PcPiece x;
     // the block's registers: 128 threads of 72 and 256 of 216 are the 384 of 168 that it was launched with
@@ -162,83 +217,73 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
         if (warp == 0) {
             // ---------------------------------------------------------- TMA producer: K, V, K, V, ...
-            const int rows = min(PC_KEYS, 1 << p.page_shift), boxes = PC_KEYS / rows;   // of a page in a tile, pages a tile
             int n = 0;
             while (pc_next(a.plan, run, x)) {
                 for (int j = 0; j < x.most; ++j) {
-                    const int key = (x.first + j) * PC_KEYS + lane * rows;
-                    const bool mine = lane < boxes && key < x.s.hi;   // pages that hold keys of the piece
+                    const int key = x.s.lo + j * PC_KEYS + lane * PC_ROWS;
+                    const bool mine = lane < PC_KEYS / PC_ROWS && key < x.s.hi;
                     const int page = mine ? paged_page(p, x.w.row, key, a.status) : 0;
-                    const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * rows * HD * 2;
-                    for (int kv = 0; kv < 2; ++kv, ++n) {
-                        const int slot = n % S::SLOTS;
-                        warp_wait(&sh.empty[slot], ((n / S::SLOTS) & 1) ^ 1, failed);
-                        if (lane == 0) bar_expect_tx(&sh.full[slot], (uint32_t)bytes);
-                        __syncwarp();
-                        if (mine && !*failed)
+                    const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * PC_ROWS * HD * 2;
+                    const int slot = n % S::SLOTS;
+                    warp_wait(&sh.empty[slot], ((n++ / S::SLOTS) & 1) ^ 1, failed);
+                    if (lane == 0) bar_expect_tx(&sh.full[slot], (uint32_t)(2 * bytes));
+                    __syncwarp();
+                    if (mine && !*failed)
+#pragma unroll
+                        for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
                             for (int b = 0; b < S::BOXES; ++b)
-                                tma_load_3d(ring + slot * S::TILE + b * PC_BOX + lane * rows * 128, kv ? &vmap : &kmap, b * 64, key & ((1 << p.page_shift) - 1), page * p.kv_heads + x.w.head, &sh.full[slot]);
-                    }
+                                tma_load_3d(ring + (2 * slot + kv) * S::TILE + b * PC_BOX + lane * PC_ROWS * 128, kv ? &vmap : &kmap, b * 64, key & ((1 << p.page_shift) - 1), page * p.kv_heads + x.w.head, &sh.full[slot]);
                 }
             }
-        } else if (warp == 1) {
-            // ---------------------------------------------------------- MMA issue
+        } else if (warp < 3) {
+            // ---------------------------------------------------------- MMA issue for a tile of rows
             constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
             constexpr uint32_t S_DESC = IDESC | ((uint32_t)(PC_KEYS >> 3) << 17), O_DESC = IDESC | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
-            int n = 0, summed[2] = {0, 0}, asked[2] = {0, 0};   // slots of the ring taken; of either tile of rows the products with V and the pieces
-            // n0: the slot of the piece's first K
-            auto scores = [&](int n0, int g, int j) {
-                const int slot = (n0 + 2 * j) % S::SLOTS;
+            const int g = warp - 1;
+            const uint32_t s_at = tmem + (uint32_t)(g * 128), p_at = s_at + PC_KEYS, o_at = tmem_o + (uint32_t)(g * HD);
+            int n = 0, scored = 0, done = 0, asked = 0;   // slots of the ring passed; scores, sums and pieces of this tile of rows
+            auto scores = [&](int n) {
+                const int slot = n % S::SLOTS;
+                warp_wait(&sh.full[slot], (n / S::SLOTS) & 1, failed);
+                if (scored > 0) warp_wait(&sh.sfree[g], (scored - 1) & 1, failed);
+                asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                 if (elect_one()) {
 #pragma unroll
                     for (int b = 0; b < S::BOXES; ++b) {
-                        const uint64_t qd = umma_desc(sptr(qbuf + g * S::TILE + b * PC_BOX)), kd = umma_desc(sptr(ring + slot * S::TILE + b * PC_BOX));
+                        const uint64_t qd = umma_desc(sptr(qbuf + g * S::QTILE + b * PC_QBOX)), kd = umma_desc(sptr(ring + 2 * slot * S::TILE + b * PC_BOX));
 #pragma unroll
                         for (int k = 0; k < 4; ++k)  // descriptors count in 16 bytes
-                            umma_bf16(tmem + (uint32_t)(g * PC_KEYS), qd + (uint64_t)(2 * k), kd + (uint64_t)(2 * k), S_DESC, (b | k) != 0);
+                            umma_bf16(s_at, qd + (uint64_t)(2 * k), kd + (uint64_t)(2 * k), S_DESC, (b | k) != 0);
                     }
-                    if (g == 1 || x.tiles[1] <= j) umma_commit(&sh.empty[slot]);
                     umma_commit(&sh.sfull[g]);
                 }
                 __syncwarp();
+                ++scored;
             };
             while (pc_next(a.plan, run, x)) {
-                const int n0 = n;
-                for (int g = 0; g < 2; ++g)
-                    if (x.s.ntok * a.plan.group > g * PC_Q) warp_wait(&sh.qfull[g], asked[g]++ & 1, failed);
-                if (x.most > 0) {
-                    warp_wait(&sh.full[n % S::SLOTS], (n / S::SLOTS) & 1, failed);
-                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                    for (int g = 0; g < 2; ++g)
-                        if (x.tiles[g] > 0) scores(n0, g, 0);
-                }
-                for (int j = 0; j < x.most; ++j, n += 2) {
-                    const int slot = (n + 1) % S::SLOTS;
-                    warp_wait(&sh.full[slot], ((n + 1) / S::SLOTS) & 1, failed);
-                    bool next = false;   // the next tile of keys has come
-                    for (int g = 0; g < 2; ++g) {
-                        if (j >= x.tiles[g]) continue;
-                        warp_wait(&sh.pfull[g], summed[g] & 1, failed);
-                        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                        if (elect_one()) {
-                            const uint64_t vd = umma_desc_mn(sptr(ring + slot * S::TILE), PC_BOX);
-#pragma unroll
-                            for (int k = 0; k < PC_KEYS / 16; ++k)
-                                umma_bf16_ts(tmem_o + (uint32_t)(g * HD), tmem + (uint32_t)(g * PC_KEYS + 8 * k), vd + (uint64_t)(k * (2048 >> 4)), O_DESC, j > 0 || k > 0);
-                            if (g == 1 || x.tiles[1] <= j) umma_commit(&sh.empty[slot]);
-                            umma_commit(&sh.odone[g]);
-                        }
-                        __syncwarp();
-                        ++summed[g];
-                        if (j + 1 < x.tiles[g]) {
-                            if (!next) warp_wait(&sh.full[(n + 2) % S::SLOTS], ((n + 2) / S::SLOTS) & 1, failed);
-                            next = true;
-                            warp_wait(&sh.odone[g], (summed[g] - 1) & 1, failed);   // the weights lie where the scores will
-                            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                            scores(n0, g, j + 1);
-                        }
+                const int tiles = x.tiles[g];
+                if (x.s.ntok * a.plan.group > g * PC_Q) warp_wait(&sh.qfull[g], asked++ & 1, failed);
+                if (tiles > 0) scores(n);
+                for (int j = 0; j < x.most; ++j, ++n) {
+                    const int slot = n % S::SLOTS;
+                    if (j + 1 < tiles) scores(n + 1);
+                    if (j >= tiles) {   // only the other tile of rows looks at this one
+                        warp_wait(&sh.full[slot], (n / S::SLOTS) & 1, failed);
+                        if (lane == 0) bar_arrive(&sh.empty[slot]);
+                        continue;
                     }
+                    warp_wait(&sh.pfull[g], done++ & 1, failed);
+                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                    if (elect_one()) {
+                        const uint64_t vd = umma_desc_mn(sptr(ring + (2 * slot + 1) * S::TILE), PC_BOX);
+#pragma unroll
+                        for (int k = 0; k < PC_KEYS / 16; ++k)
+                            umma_bf16_ts(o_at, p_at + (uint32_t)(8 * k), vd + (uint64_t)(k * (2048 >> 4)), O_DESC, j > 0 || k > 0);
+                        umma_commit(&sh.odone[g]);
+                        umma_commit(&sh.empty[slot]);
+                    }
+                    __syncwarp();
                 }
             }
         }
@@ -246,21 +291,32 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         // ---------------------------------------------------------- softmax
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
         const int g = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, group = a.plan.group;
-        const uint32_t quad_addr = (uint32_t)(quad * 32) << 16, s_addr = tmem + quad_addr + (uint32_t)(g * PC_KEYS), o_addr = tmem_o + quad_addr + (uint32_t)(g * HD);
-        const float sl = fabsf(a.sl);
+        const uint32_t quad_addr = (uint32_t)(quad * 32) << 16, s_addr = tmem + quad_addr + (uint32_t)(g * 128), o_addr = tmem_o + quad_addr + (uint32_t)(g * HD);
+        const float sl = fmaxf(fabsf(a.sl), 1.17549435e-38f);   // above 0, so that hidden scores stay -inf
         const uint32_t flip = a.sl < 0.f ? 0x80008000u : 0u;   // a negative scale's sign goes to the queries
         int n = 0, scored = 0;
         while (pc_next(a.plan, run, x)) {
             const int rows = x.s.ntok * group, n0 = n;
-            n += 2 * x.most;
+            n += x.most;
+            if (threadIdx.x == PC_THREADS - 1) paged_cut(a, run, x.w, x.s, blockIdx.x);
             if (rows <= g * PC_Q) continue;
             // the queries: a quad's warp stores 32 rows of its tile, a row 16 bytes a lane
-            for (int i = threadIdx.x & 127; i < PC_Q * HD / 8; i += 128) {
-                const int row = i / (HD / 8), d = i % (HD / 8), rr = g * PC_Q + row, tok = rr / group;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (rr < rows) v = *reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)a.q + (size_t)(x.w.r.first + x.s.t0 + tok) * a.q_stride + (size_t)(x.w.head * group + rr - tok * group) * HD + d * 8);
-                v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-                *reinterpret_cast<uint4 *>(qbuf + g * S::TILE + (d >> 3) * PC_BOX + row * 128 + (((d & 7) ^ (row & 7)) << 4)) = v;
+            constexpr int Q_LOADS = PC_Q * HD / 8 / 128;   // all in flight
+            {
+                const int i0 = threadIdx.x & 127;
+                uint4 v[Q_LOADS];
+#pragma unroll
+                for (int u = 0; u < Q_LOADS; ++u) {
+                    const int i = i0 + 128 * u, d = i % (HD / 8), rr = g * PC_Q + i / (HD / 8), tok = rr / group;
+                    v[u] = make_uint4(0u, 0u, 0u, 0u);
+                    if (rr < rows) v[u] = *reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)a.q + (size_t)(x.w.r.first + x.s.t0 + tok) * a.q_stride + (size_t)(x.w.head * group + rr - tok * group) * HD + d * 8);
+                }
+#pragma unroll
+                for (int u = 0; u < Q_LOADS; ++u) {
+                    const int i = i0 + 128 * u, d = i % (HD / 8), row = i / (HD / 8);
+                    v[u].x ^= flip; v[u].y ^= flip; v[u].z ^= flip; v[u].w ^= flip;
+                    *reinterpret_cast<uint4 *>(qbuf + g * S::QTILE + (d >> 3) * PC_QBOX + row * 128 + (((d & 7) ^ (row & 7)) << 4)) = v[u];
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
@@ -269,27 +325,24 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const int least = x.s.base + x.s.t0 + (g * PC_Q) / group;   // the first row sees up to here
             float top = PC_NONE, sum = 0.f;
             for (int j = 0; j < x.tiles[g]; ++j, ++scored) {
-                const int at = (x.first + j) * PC_KEYS;
-                warp_wait(&sh.sfull[g], scored & 1, failed);
-                asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                const int lim = min(pos, x.s.hi - 1) - at;
-                if (at + PC_KEYS - 1 > least || at + PC_KEYS > x.s.hi || (g + 1) * PC_Q > rows) pc_softmax<HD, true>(s_addr, o_addr, sl, lim, j > 0, top, sum);
-                else pc_softmax<HD, false>(s_addr, o_addr, sl, lim, j > 0, top, sum);
+                const int at = x.s.lo + j * PC_KEYS;
                 if (at + PC_KEYS > x.s.hi) {   // what lies behind the piece's keys may be anything
-                    const int slot = (n0 + 2 * j + 1) % S::SLOTS;
-                    warp_wait(&sh.full[slot], ((n0 + 2 * j + 1) / S::SLOTS) & 1, failed);
-                    if (at + r >= x.s.hi)
+                    const int slot = (n0 + j) % S::SLOTS;
+                    warp_wait(&sh.full[slot], ((n0 + j) / S::SLOTS) & 1, failed);
+                    if (at + r >= x.s.hi && r < PC_KEYS)
 #pragma unroll
                         for (int b = 0; b < S::BOXES; ++b)
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4 *>(ring + slot * S::TILE + b * PC_BOX + r * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4 *>(ring + (2 * slot + 1) * S::TILE + b * PC_BOX + r * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                    __syncwarp();
+                    __syncwarp();   // and the products wait for all four warps
                 }
-                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-                asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-                __syncwarp();
-                if (lane == 0) bar_arrive(&sh.pfull[g]);
+                warp_wait(&sh.sfull[g], scored & 1, failed);
+                asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                const int lim = min(pos, x.s.hi - 1) - at;
+                auto before = [&] { if (j > 0) warp_wait(&sh.odone[g], (scored - 1) & 1, failed); };
+                if (at + PC_KEYS - 1 > least || at + PC_KEYS > x.s.hi || (g + 1) * PC_Q > rows) pc_softmax<HD, true>(s_addr, o_addr, sl, lim, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
+                else pc_softmax<HD, false>(s_addr, o_addr, sl, lim, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
             }
             if (x.tiles[g] > 0) warp_wait(&sh.odone[g], (scored - 1) & 1, failed);
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -297,7 +350,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const size_t slot = (2 * (size_t)blockIdx.x + (x.w.k0 == 0)) * a.tile_rows;
             const float f = !all ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
             float poison = 0.f;  // stays 0 unless an output is Inf or NaN
-            __nv_bfloat16 *dst = (__nv_bfloat16 *)a.out + (size_t)(x.w.r.first + x.s.t0 + tok) * a.o_stride + (size_t)(x.w.head * group + rr - tok * group) * HD;
+            // A lane has a row, 16 bytes of which at a time would go to 32 places: four lanes exchange pieces and store 64 bytes of a row each time.
+            __nv_bfloat16 *dst[4];
+            bool have[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int row = g * PC_Q + quad * 32 + (lane & ~3) + k, t = row / group;
+                have[k] = row < rows;
+                dst[k] = (__nv_bfloat16 *)a.out + (size_t)(x.w.r.first + x.s.t0 + t) * a.o_stride + (size_t)(x.w.head * group + row - t * group) * HD + 8 * (lane & 3);
+            }
+            float *part = a.acc + (slot + g * PC_Q + quad * 32 + (lane & ~3)) * HD + 4 * (lane & 3);
 #pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {
                 uint32_t v[32];
@@ -312,20 +374,33 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     poison = fmaf(y, 0.f, poison);
                     v[k] = __float_as_uint(y);
                 }
-                if (all && rr < rows) {
+                if (all) {
+                    uint4 o[4];
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
-                        uint32_t o[4];
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t w[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[k + 2 * e]), __uint_as_float(v[k + 2 * e + 1]));
-                            o[e] = *reinterpret_cast<const uint32_t *>(&b);
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[8 * k + 2 * e]), __uint_as_float(v[8 * k + 2 * e + 1]));
+                            w[e] = *reinterpret_cast<const uint32_t *>(&b);
                         }
-                        *reinterpret_cast<uint4 *>(dst + 32 * c + k) = make_uint4(o[0], o[1], o[2], o[3]);
+                        o[k] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                } else if (rr < rows) {
+                    exchange4(o, lane);
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4 *>(a.acc + (slot + rr) * HD + 32 * c + k) = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                    for (int k = 0; k < 4; ++k)
+                        if (have[k]) *reinterpret_cast<uint4 *>(dst[k] + 32 * c) = o[k];
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint4 o[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[k] = make_uint4(v[16 * h + 4 * k], v[16 * h + 4 * k + 1], v[16 * h + 4 * k + 2], v[16 * h + 4 * k + 3]);
+                        exchange4(o, lane);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (have[k]) *reinterpret_cast<uint4 *>(part + k * HD + 32 * c + 16 * h) = o[k];
+                    }
                 }
             }
             if (!all && rr < rows) *reinterpret_cast<float2 *>(a.ml + (slot + rr) * 2) = make_float2(top, sum);
@@ -346,10 +421,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     }
 }
 
-// The pages of a layer: [pages kv_heads][page_size][dim], in boxes of 64 elements of the rows that a page has in a tile.
+// The pages of a layer: [pages kv_heads][page_size][dim], in boxes of 64 elements of 16 rows.
 int pages_map(CUtensorMap *map, const void *pages, const PagedView &p, int hd) {
     const int page = 1 << p.page_shift;
-    return make_mats_map(map, pages, p.pages * p.kv_heads, page, hd, hd, (long long)page * hd, std::min(page, PC_KEYS));
+    return make_mats_map(map, pages, p.pages * p.kv_heads, page, hd, hd, (long long)page * hd, PC_ROWS);
 }
 
 template <int HD>
@@ -367,7 +442,7 @@ int launch_tc(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
     int rc = pages_map(&kmap, a.k, a.plan.p, HD);
     if (rc == AB2_OK) rc = pages_map(&vmap, a.v, a.plan.p, HD);
     if (rc != AB2_OK) return rc;
-    paged_deal(a, device_sm_count(), 2 * PC_Q, paged_log2(PC_KEYS), 4, HD, workspace, bytes);
+    paged_deal(a, device_sm_count(), 2 * PC_Q, 7, 4, HD, workspace, bytes);
     paged_tc_kernel<HD><<<a.ctas, PC_THREADS, S::SMEM, s>>>(kmap, vmap, a);
     AB2_LAUNCH_CHECK();
     return a.plan.whole ? AB2_OK : paged_merge(a, HD, AB2_BF16, s);

@@ -7,7 +7,7 @@
 //
 // in f32, rounded once.  A CTA has a slice of a row's vocabulary: it counts the history's tokens of its slice in shared memory (integer
 // additions, whose order changes nothing), notes which entry of the bias list is each token's last, and then passes over
-// the slice once, 16 bytes a load.  Every CTA of a row reads the row's history, from L2 after the first.  Bound by HBM for large
+// the slice once, 16 bytes a load; a bit for each token says whether there is anything to look up for it.  Every CTA of a row reads the row's history, from L2 after the first.  Bound by HBM for large
 // batches, by the launch, the clearing of the counts and the history's latency for small ones.
 #include <algorithm>
 
@@ -19,7 +19,7 @@ namespace ab2 {
 int device_sm_count();
 namespace {
 
-constexpr int LG_THREADS = 256;
+constexpr int LG_THREADS = 256, LG_SLICE = 4096;   // tokens a CTA at most
 
 struct LogitArgs {
     const void *logits;
@@ -44,55 +44,105 @@ __device__ __forceinline__ float ruled(float z, int count, float rho, float pres
     return z - (presence + frequency * (float)count);
 }
 
+template <typename T> __device__ __forceinline__ uint32_t lowest_bits();   // of -inf
+template <> __device__ __forceinline__ uint32_t lowest_bits<float>() { return 0xff800000u; }
+template <> __device__ __forceinline__ uint32_t lowest_bits<__half>() { return 0xfc00u; }
+template <> __device__ __forceinline__ uint32_t lowest_bits<__nv_bfloat16>() { return 0xff80u; }
+
 template <typename T, int V>  // V elements a load
 __global__ void __launch_bounds__(LG_THREADS) adjust_logits_kernel(const __grid_constant__ LogitArgs a) {
-    extern __shared__ __align__(16) int counts[];  // [slice], then with biases [slice]: the list's entry for the token, + 1
+    // [slice / 32] which tokens the history or the biases touch, [slice] counts, with biases [slice] the list's entry for the token, + 1
+    extern __shared__ __align__(16) uint32_t touched[];
+    int *counts = (int *)touched + a.slice / 32, *entry = counts + (a.history ? a.slice : 0);
     const int row = blockIdx.y, first = blockIdx.x * a.slice, n = min(a.slice, a.vocab - first);
-    int *entry = counts + a.slice;
-    const int tables = (a.history ? a.slice : 0) + (a.biases ? a.slice : 0);
-    int *table = a.history ? counts : entry;
-    for (int i = threadIdx.x * 4; i < tables; i += LG_THREADS * 4) *reinterpret_cast<int4 *>(table + i) = make_int4(0, 0, 0, 0);
+    const T *in = (const T *)a.logits + row * a.stride + first;
+    const uint32_t *mask = a.allowed ? a.allowed + (size_t)row * a.words + (first >> 5) : nullptr;
+    constexpr int LOADS = LG_SLICE / (LG_THREADS * V);   // the slice's logits are on their way while the tables are made
+    alignas(16) T e[LOADS][V];
+    uint32_t bits[LOADS];
+#pragma unroll
+    for (int b = 0; b < LOADS; ++b) {
+        const int i = (threadIdx.x + b * LG_THREADS) * V;
+        if (i >= n) continue;
+        if constexpr (V > 1) *reinterpret_cast<uint4 *>(e[b]) = *reinterpret_cast<const uint4 *>(in + i);
+        else e[b][0] = in[i];
+        bits[b] = mask ? mask[i >> 5] >> (i & 31) : 0xffffffffu;
+    }
+    const int tables = a.slice / 32 + (a.history ? a.slice : 0) + (a.biases ? a.slice : 0);
+    for (int i = threadIdx.x * 4; i < tables; i += LG_THREADS * 4) *reinterpret_cast<uint4 *>(touched + i) = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     float rho = 1.f, presence = 0.f, frequency = 0.f;
     if (a.history) {
         rho = a.rules[3 * row]; presence = a.rules[3 * row + 1]; frequency = a.rules[3 * row + 2];
         const int *h = a.history + row * a.history_stride;
         const int len = min(a.lengths ? a.lengths[row] : a.history_width, a.history_width);
-        for (int i = threadIdx.x; i < len; i += LG_THREADS * 8) {
-            int v[8];
+        auto count = [&](int v) {
+            if ((unsigned)v >= (unsigned)n) return;
+            atomicAdd(counts + v, 1);
+            atomicOr(touched + (v >> 5), 1u << (v & 31));
+        };
+        int done = 0;
+        if (((uintptr_t)h & 15) == 0) {   // four ids a load, four loads in flight
+            done = max(len, 0) & ~3;
+            for (int i = threadIdx.x * 4; i < done; i += LG_THREADS * 16) {
+                int4 v[4];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = i + u * LG_THREADS < len ? h[i + u * LG_THREADS] - first : -1;
+                for (int u = 0; u < 4; ++u) v[u] = i + u * LG_THREADS * 4 < done ? *reinterpret_cast<const int4 *>(h + i + u * LG_THREADS * 4) : make_int4(-1, -1, -1, -1);
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if ((unsigned)v[u] < (unsigned)n) atomicAdd(counts + v[u], 1);
+                for (int u = 0; u < 4; ++u) {
+                    if (i + u * LG_THREADS * 4 >= done) continue;
+                    count(v[u].x - first); count(v[u].y - first); count(v[u].z - first); count(v[u].w - first);
+                }
+            }
         }
+        for (int i = done + threadIdx.x; i < len; i += LG_THREADS) count(h[i] - first);
     }
     for (int i = threadIdx.x; i < a.biases; i += LG_THREADS) {
         const int v = a.bias_ids[(size_t)row * a.biases + i] - first;
-        if ((unsigned)v < (unsigned)n) atomicMax(entry + v, i + 1);
+        if ((unsigned)v >= (unsigned)n) continue;
+        atomicMax(entry + v, i + 1);
+        atomicOr(touched + (v >> 5), 1u << (v & 31));
     }
     __syncthreads();
-    const T *in = (const T *)a.logits + row * a.stride + first;
     T *out = (T *)a.out + (size_t)row * a.vocab + first;
-    const uint32_t *mask = a.allowed ? a.allowed + (size_t)row * a.words + (first >> 5) : nullptr;
     const float *bias = a.bias_values + (size_t)row * a.biases;
-    for (int i = threadIdx.x * V; i < n; i += LG_THREADS * V) {
-        alignas(16) T e[V];
-        if constexpr (V > 1) *reinterpret_cast<uint4 *>(e) = *reinterpret_cast<const uint4 *>(in + i);
-        else e[0] = in[i];
-        const uint32_t bits = mask ? mask[i >> 5] >> (i & 31) : 0xffffffffu;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            float z = to_f32(e[j]);
-            if (a.history) z = ruled(z, counts[i + j], rho, presence, frequency);
-            if (a.biases) {
-                const int b = entry[i + j];
-                if (b) z += bias[b - 1];
+    for (int b = 0; b < LOADS; ++b) {
+        const int i = (threadIdx.x + b * LG_THREADS) * V;
+        if (i >= n) continue;
+        {
+            // most tokens are in no history and no list: they pass, or become -inf, as bits
+            const uint32_t any = touched[i >> 5] >> (i & 31) & ((1u << V) - 1);
+            for (uint32_t left = any & bits[b]; left; left &= left - 1) {
+                const int j = __ffs(left) - 1;
+                float z = to_f32(in[i + j]);
+                if (a.history) z = ruled(z, counts[i + j], rho, presence, frequency);
+                if (a.biases) {
+                    const int k = entry[i + j];
+                    if (k) z += bias[k - 1];
+                }
+                const T r = from_f32<T>(z);
+#pragma unroll
+                for (int m = 0; m < V; ++m)
+                    if (m == j) e[b][m] = r;
             }
-            e[j] = from_f32<T>((bits >> j) & 1 ? z : -INFINITY);
+            if constexpr (V > 1) {
+                uint32_t q[4];
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    q[m] = reinterpret_cast<const uint32_t *>(e[b])[m];
+                    if constexpr (sizeof(T) == 4) {
+                        if (!((bits[b] >> m) & 1)) q[m] = lowest_bits<T>();
+                    } else {
+                        const uint32_t keep = ((bits[b] >> (2 * m)) & 1 ? 0xffffu : 0u) | ((bits[b] >> (2 * m + 1)) & 1 ? 0xffff0000u : 0u);
+                        q[m] = (q[m] & keep) | (lowest_bits<T>() * 0x10001u & ~keep);
+                    }
+                }
+                *reinterpret_cast<uint4 *>(out + i) = make_uint4(q[0], q[1], q[2], q[3]);
+            } else {
+                out[i] = bits[b] & 1 ? e[b][0] : from_f32<T>(-INFINITY);
+            }
         }
-        if constexpr (V > 1) *reinterpret_cast<uint4 *>(out + i) = *reinterpret_cast<const uint4 *>(e);
-        else out[i] = e[0];
     }
 }
 
@@ -101,10 +151,10 @@ int launch_adjust(LogitArgs a, int rows, cudaStream_t s) {
     constexpr int V = 16 / sizeof(T);
     const bool wide = a.vocab % V == 0 && a.stride % V == 0 && (((uintptr_t)a.logits | (uintptr_t)a.out) & 15) == 0;
     // Slices of 4096 tokens, smaller ones where those are fewer than two CTAs an SM; 512 at least, so that a thread has a load of its own.
-    a.slice = 4096;
+    a.slice = LG_SLICE;
     while (a.slice > 512 && (long long)rows * ((a.vocab + a.slice - 1) / a.slice) < 2 * device_sm_count()) a.slice /= 2;
     const dim3 grid((a.vocab + a.slice - 1) / a.slice, rows);
-    const size_t smem = (size_t)a.slice * 4 * (a.biases ? 2 : 1);
+    const size_t smem = (size_t)a.slice * 4 * ((a.history ? 1 : 0) + (a.biases ? 1 : 0)) + a.slice / 8;
     if (wide) adjust_logits_kernel<T, V><<<grid, LG_THREADS, smem, s>>>(a);
     else adjust_logits_kernel<T, 1><<<grid, LG_THREADS, smem, s>>>(a);
     AB2_LAUNCH_CHECK();

@@ -222,11 +222,12 @@ struct PagedAttnArgs {
     long long q_stride, o_stride;
     float sl;          // scale in powers of two
     float *acc, *ml;   // pieces: [2 ctas][rows of a tile][dim] sums, [2 ctas][rows of a tile][2] maximum and sum of weights
+    int4 *cut;         // [ctas] the item that a run began and did not end: its first token, its tokens (0: there is none), its head, the run that ends it
     int ctas, tile_rows;
     int *status;
 };
 // Bytes that the pieces of a launch take.
-static inline size_t paged_piece_bytes(int ctas, int tile_rows, int hd) { return (size_t)2 * ctas * tile_rows * (hd + 2) * 4; }
+static inline size_t paged_piece_bytes(int ctas, int tile_rows, int hd) { return (size_t)2 * ctas * tile_rows * (hd + 2) * 4 + (size_t)ctas * 16; }
 static inline int paged_log2(int n) { return 31 - __builtin_clz(n); }
 // Sets how a launch of `ctas` CTAs, tiles of `tile_rows` query rows and 2^key_shift keys deals its work out, cutting items where the workspace has room.
 static inline void paged_deal(PagedAttnArgs &a, int ctas, int tile_rows, int key_shift, int least, int hd, void *workspace, size_t bytes) {
@@ -237,7 +238,16 @@ static inline void paged_deal(PagedAttnArgs &a, int ctas, int tile_rows, int key
     a.plan.least = a.plan.whole ? 1 : least;
     a.acc = (float *)workspace;
     a.ml = a.acc + (size_t)2 * ctas * tile_rows * hd;
+    a.cut = (int4 *)(a.ml + (size_t)4 * ctas * tile_rows);
 }
+// What run c leaves to the merge, written by one thread: nothing, to begin with, and its last piece if that begins an item and does not end it.
+__device__ __forceinline__ void paged_uncut(const PagedAttnArgs &a, int c) { if (!a.plan.whole) a.cut[c] = make_int4(0, 0, 0, 0); }
+__device__ __forceinline__ void paged_cut(const PagedAttnArgs &a, const PagedRun &run, const PagedPiece &w, const PagedSpan &sp, int c) {
+    if (w.k0 > 0 || w.k1 == w.k_tiles) return;
+    const long long end = run.u + (w.k_tiles - w.k1);   // the unit behind the item: the last run that begins before it ends it
+    a.cut[c] = make_int4(w.r.first + sp.t0, sp.ntok, w.head, (int)min((long long)run.ctas - 1, (end * run.ctas - 1) / run.total));
+}
+
 // Row r of a piece of bf16 over the keys [lo, to] of it that it sees, by one warp, a lane every 32nd dimension: where a product with hidden values
 // has left Inf or NaN (a weight of 0 times either), this gives what the keys in sight alone give.
 template <int HD>

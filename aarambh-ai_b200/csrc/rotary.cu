@@ -4,8 +4,8 @@
 //
 // Pairs are (i, i + n) with the half layout and (2i, 2i + 1) with the interleaved one, n = rot / 2 of them; the dimensions from rot on pass
 // as they are.  One pass over q and k (and v, which is copied into its pages): bound by HBM from some hundred tokens on, by the launch
-// below.  A warp has one token, its lanes (head, P pairs) of it: where a head's chunks of pairs divide 32 a lane keeps its pairs
-// from head to head and turns its P angles once.
+// below.  A warp has one token (or a part of its heads where tokens are few): its lanes turn the token's angles once, into shared memory,
+// and then take items (head, P pairs) of it; where a head's chunks divide 32 a lane keeps its pairs from head to head.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -15,7 +15,7 @@ using namespace ab2;
 namespace ab2 {
 namespace {
 
-constexpr int ROT_WARPS = 4, ROT_BATCH = 4;  // items of a lane in flight
+constexpr int ROT_WARPS = 4, ROT_BATCH = 2;  // items of a lane in flight
 
 struct RotArgs {
     const void *q, *k, *v;
@@ -56,10 +56,20 @@ template <typename T, int E> struct Vec {
     }
 };
 
-template <typename T, int P, bool HALF, bool PAGED>
-__global__ void __launch_bounds__(32 * ROT_WARPS) rotary_kernel(const __grid_constant__ RotArgs a) {
-    const int lane = threadIdx.x & 31;
-    const long long w = (long long)blockIdx.x * ROT_WARPS + (threadIdx.x >> 5);
+// Where an item (a head's chunk) lies: its first P elements, and the others `gap` further.
+template <typename T> struct RotItem {
+    const T *src;
+    T *dst;
+    int gap, chunk;   // from `turned` on: passes as it is
+    bool kept;
+};
+
+// EVEN: a head's chunks divide 32, so that a lane keeps its chunk from head to head.
+template <typename T, int P, bool HALF, bool PAGED, bool EVEN>
+__global__ void __launch_bounds__(32 * ROT_WARPS, 6) rotary_kernel(const __grid_constant__ RotArgs a) {
+    extern __shared__ __align__(16) float2 turns[];   // [warps][pairs] cos and sin, times the magnitude
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long w = (long long)blockIdx.x * ROT_WARPS + warp;
     const int t = (int)(w / a.parts), part = (int)(w % a.parts);
     if (t >= a.tokens) return;
     long long pos = 0;
@@ -86,56 +96,69 @@ __global__ void __launch_bounds__(32 * ROT_WARPS) rotary_kernel(const __grid_con
     } else {
         pos = a.pos64 ? ((const long long *)a.pos)[t] : ((const int *)a.pos)[t];
     }
-    const int lo = part * a.per_warp, vheads = a.heads + a.kv_heads * (PAGED ? 2 : 1), hi = min(lo + a.per_warp, vheads * a.chunks);
     const int turned = a.pairs / P;          // chunks that turn
+    const int lo = part * a.per_warp, vheads = a.heads + a.kv_heads * (PAGED ? 2 : 1), hi = min(lo + a.per_warp, vheads * a.chunks);
+    auto item = [&](int h, int chunk) {
+        RotItem<T> it;
+        const int at = chunk < turned ? (HALF ? chunk * P : chunk * 2 * P) : 2 * a.pairs + (chunk - turned) * 2 * P;
+        it.gap = HALF && chunk < turned ? a.pairs : P;
+        it.chunk = chunk;
+        it.kept = true;
+        if (h < a.heads) {
+            it.src = (const T *)a.q + ((size_t)t * a.q_stride + (size_t)(h * a.dim + at));
+            it.dst = (T *)a.qo + ((size_t)t * a.qo_stride + (size_t)(h * a.dim + at));
+        } else {
+            const int g = h - a.heads;
+            const bool value = PAGED && g >= a.kv_heads;
+            const int of = (value ? g - a.kv_heads : g) * a.dim + at;
+            if (value) it.chunk = turned;
+            it.src = (value ? (const T *)a.v + (size_t)t * a.v_stride : (const T *)a.k + (size_t)t * a.k_stride) + of;
+            if (PAGED) {
+                it.dst = (T *)(value ? a.vp : a.kp) + (slot + ((size_t)(value ? g - a.kv_heads : g) << a.cache.page_shift)) * a.dim + at;
+                it.kept = kept;
+            } else {
+                it.dst = (T *)a.ko + (size_t)t * a.ko_stride + of;
+            }
+        }
+        return it;
+    };
+    const int step = EVEN ? 32 / a.chunks : 0;
+    int head = (lo + lane) / a.chunks;
+    const int chunk0 = (lo + lane) % a.chunks;
+    float2 *cs = turns + warp * a.pairs;
     float c[P], s[P];
     int known = -1;                          // the chunk whose angles c and s are
-    for (int i0 = lo + lane; i0 < hi; i0 += 32 * ROT_BATCH) {
+    bool first = true;
+    for (int i0 = lo + lane; __any_sync(0xffffffffu, i0 < hi); i0 += 32 * ROT_BATCH) {
+        RotItem<T> it[ROT_BATCH];
         Vec<T, P> x[ROT_BATCH], y[ROT_BATCH];
-        // where an item lies: its first P elements, and the others `gap` further
-        auto item = [&](int i, const T *&src, T *&dst, int &gap, int &chunk) {
-            const int h = i / a.chunks;
-            chunk = i % a.chunks;
-            const int at = chunk < turned ? (HALF ? chunk * P : chunk * 2 * P) : 2 * a.pairs + (chunk - turned) * 2 * P;
-            gap = HALF && chunk < turned ? a.pairs : P;
-            if (h < a.heads) {
-                src = (const T *)a.q + (size_t)t * a.q_stride + (size_t)h * a.dim + at;
-                dst = (T *)a.qo + (size_t)t * a.qo_stride + (size_t)h * a.dim + at;
-            } else if (!PAGED || h < a.heads + a.kv_heads) {
-                const int g = h - a.heads;
-                src = (const T *)a.k + (size_t)t * a.k_stride + (size_t)g * a.dim + at;
-                dst = PAGED ? (T *)a.kp + (slot + ((size_t)g << a.cache.page_shift)) * a.dim + at : (T *)a.ko + (size_t)t * a.ko_stride + (size_t)g * a.dim + at;
-            } else {
-                const int g = h - a.heads - a.kv_heads;
-                src = (const T *)a.v + (size_t)t * a.v_stride + (size_t)g * a.dim + at;
-                dst = (T *)a.vp + (slot + ((size_t)g << a.cache.page_shift)) * a.dim + at;
-                chunk = turned;  // a value passes as it is
-            }
-        };
 #pragma unroll
         for (int b = 0; b < ROT_BATCH; ++b) {
             const int i = i0 + 32 * b;
-            if (i >= hi) break;
-            const T *src;
-            T *dst;
-            int gap, chunk;
-            item(i, src, dst, gap, chunk);
-            x[b].load(src);
-            y[b].load(src + gap);
+            it[b] = EVEN ? item(head, chunk0) : item(i / a.chunks, i % a.chunks);
+            head += step;
+            if (i < hi) {
+                x[b].load(it[b].src);
+                y[b].load(it[b].src + it[b].gap);
+            }
+        }
+        if (first) {   // while the first items come, a pair a lane
+            first = false;
+            for (int j = lane; j < a.pairs; j += 32) {
+                float2 v;
+                turn_cos_sin((unsigned long long)pos * turns_per_position(__ldg(a.freq + j)), a.mag, v.x, v.y);
+                cs[j] = v;
+            }
+            __syncwarp();
         }
 #pragma unroll
         for (int b = 0; b < ROT_BATCH; ++b) {
-            const int i = i0 + 32 * b;
-            if (i >= hi) break;
-            const T *src;
-            T *dst;
-            int gap, chunk;
-            item(i, src, dst, gap, chunk);
-            if (chunk < turned) {
-                if (chunk != known) {
-                    known = chunk;
+            if (i0 + 32 * b >= hi) continue;
+            if (it[b].chunk < turned) {
+                if (EVEN ? known < 0 : it[b].chunk != known) {
+                    known = it[b].chunk;
 #pragma unroll
-                    for (int j = 0; j < P; ++j) turn_cos_sin((unsigned long long)pos * turns_per_position(__ldg(a.freq + chunk * P + j)), a.mag, c[j], s[j]);
+                    for (int j = 0; j < P; ++j) { const float2 v = cs[known * P + j]; c[j] = v.x; s[j] = v.y; }
                 }
                 if (HALF) {
 #pragma unroll
@@ -155,29 +178,30 @@ __global__ void __launch_bounds__(32 * ROT_WARPS) rotary_kernel(const __grid_con
                     }
                 }
             }
-            if (PAGED && !kept && i / a.chunks >= a.heads) continue;
-            x[b].store(dst);
-            y[b].store(dst + gap);
+            if (!it[b].kept) continue;
+            x[b].store(it[b].dst);
+            y[b].store(it[b].dst + it[b].gap);
         }
     }
 }
 
-template <typename T, int P>
+template <typename T, int P, bool EVEN>
 int launch_rotary(const RotArgs &a, bool half, bool paged, cudaStream_t s) {
     const dim3 grid((unsigned)(((long long)a.tokens * a.parts + ROT_WARPS - 1) / ROT_WARPS));
-    if (paged) (half ? rotary_kernel<T, P, true, true> : rotary_kernel<T, P, false, true>)<<<grid, 32 * ROT_WARPS, 0, s>>>(a);
-    else (half ? rotary_kernel<T, P, true, false> : rotary_kernel<T, P, false, false>)<<<grid, 32 * ROT_WARPS, 0, s>>>(a);
+    const size_t smem = (size_t)ROT_WARPS * a.pairs * sizeof(float2);
+    if (paged) (half ? rotary_kernel<T, P, true, true, EVEN> : rotary_kernel<T, P, false, true, EVEN>)<<<grid, 32 * ROT_WARPS, smem, s>>>(a);
+    else (half ? rotary_kernel<T, P, true, false, EVEN> : rotary_kernel<T, P, false, false, EVEN>)<<<grid, 32 * ROT_WARPS, smem, s>>>(a);
     AB2_LAUNCH_CHECK();
     return AB2_OK;
 }
 
-// Chunks of 8 pairs (loads of 16 bytes and more) where every piece starts on such a boundary, else of 4, else single pairs.
+// Chunks of P pairs that make loads of 16 bytes where every piece starts on such a boundary, else of 4 pairs, else single pairs.
 int rotary_go(RotArgs a, bool half, bool paged, ab2_dtype dtype, cudaStream_t s) {
     const int rest = a.dim - 2 * a.pairs;
     uintptr_t where = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.qo | (uintptr_t)a.ko | (uintptr_t)a.kp | (uintptr_t)a.vp;
     const size_t esize = dtype_size(dtype);
     const long long steps = a.q_stride | a.k_stride | a.v_stride | a.qo_stride | a.ko_stride | a.dim;
-    int P = 8;
+    int P = dtype == AB2_F32 ? 4 : 8;
     while (P > 1 && (a.pairs % P || rest % (2 * P) || steps % P || where % std::min<size_t>(16, P * esize))) P = P == 8 ? 4 : 1;
     a.chunks = a.dim / (2 * P);
     // A warp's items: all of a token's where there are tokens enough for some warps on every scheduler, else fewer (a lane has one at least).
@@ -186,7 +210,10 @@ int rotary_go(RotArgs a, bool half, bool paged, ab2_dtype dtype, cudaStream_t s)
     a.per_warp = ((items + a.parts - 1) / a.parts + 31) / 32 * 32;
     a.parts = (items + a.per_warp - 1) / a.per_warp;
     AB2_REQUIRE(((long long)a.tokens * a.parts + ROT_WARPS - 1) / ROT_WARPS < (1ll << 31), AB2_ERR_BAD_SHAPE, "%d tokens of %d heads are more than one launch takes", a.tokens, a.heads);
-#define AB2_ROTARY(T) (P == 8 ? launch_rotary<T, 8>(a, half, paged, s) : P == 4 ? launch_rotary<T, 4>(a, half, paged, s) : launch_rotary<T, 1>(a, half, paged, s))
+    const bool even = 32 % a.chunks == 0;
+#define AB2_ROTARY(T)                                                                                                                                   \
+    (sizeof(T) == 2 && P == 8 ? (even ? launch_rotary<T, 16 / sizeof(T), true>(a, half, paged, s) : launch_rotary<T, 16 / sizeof(T), false>(a, half, paged, s))                                     \
+     : P == 4 ? (even ? launch_rotary<T, 4, true>(a, half, paged, s) : launch_rotary<T, 4, false>(a, half, paged, s)) : launch_rotary<T, 1, false>(a, half, paged, s))
     switch (dtype) {
     case AB2_F32: return AB2_ROTARY(float);
     case AB2_F16: return AB2_ROTARY(__half);
@@ -198,6 +225,7 @@ int rotary_go(RotArgs a, bool half, bool paged, ab2_dtype dtype, cudaStream_t s)
 int check_layout(int layout, int dim, int rot, const double *freq) {
     AB2_REQUIRE(layout == AB2_ROTARY_HALF || layout == AB2_ROTARY_INTERLEAVED, AB2_ERR_BAD_ARG, "unknown rotary layout %d", layout);
     AB2_REQUIRE(dim > 0 && dim % 2 == 0 && rot >= 0 && rot % 2 == 0 && rot <= dim, AB2_ERR_BAD_SHAPE, "rotary positions turn an even number of an even head's dimensions, got %d of %d", rot, dim);
+    AB2_REQUIRE(rot <= 2048, AB2_ERR_UNSUPPORTED, "up to 2048 dimensions of a head are rotated, got %d", rot);
     AB2_REQUIRE(rot == 0 || freq, AB2_ERR_BAD_ARG, "null frequencies");
     return AB2_OK;
 }

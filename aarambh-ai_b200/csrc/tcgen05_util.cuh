@@ -196,6 +196,12 @@ __device__ __forceinline__ void tmem_ld16(uint32_t (&v)[16], uint32_t addr) {
         : AB2_REGS16("=r", v) : "r"(addr));
     asm volatile("tcgen05.wait::ld.sync.aligned;\n" : AB2_REGS16("+r", v)::"memory");
 }
+__device__ __forceinline__ void tmem_ld16_start(uint32_t (&v)[16], uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        : AB2_REGS16("=r", v) : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld16_wait(uint32_t (&v)[16]) { asm volatile("tcgen05.wait::ld.sync.aligned;\n" : AB2_REGS16("+r", v)::"memory"); }
 __device__ __forceinline__ void tmem_ld32_start(uint32_t (&v)[32], uint32_t addr) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -222,6 +228,9 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};\n" ::AB2_REGS32("r", v), "r"(addr)
         : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};\n" ::AB2_REGS8("r", v), "r"(addr) : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n" ::AB2_REGS16("r", v), "r"(addr) : "memory");

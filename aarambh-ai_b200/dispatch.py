@@ -277,9 +277,15 @@ def rotary_frequencies(dims: int, base: float = 10000.0, scaling: RotaryScaling 
 
 def _on_device(*tensors) -> None:
     """Kernels run on the current device's stream: every tensor has to be there."""
+    here = None
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.get_device() != torch.cuda.current_device()):
-            raise _lib.Ab2Error(-7, f"tensors must be on the current CUDA device (this library has no CPU path), got one on {t.device}")
+        if t is None:
+            continue
+        at = t.get_device()   # -1 for host memory
+        if at != here:   # the first one, or a wrong one
+            if here is not None or at < 0 or at != torch.cuda.current_device():
+                raise _lib.Ab2Error(-7, f"tensors must be on the current CUDA device (this library has no CPU path), got one on {t.device}")
+            here = at
 
 
 def _typed(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str) -> torch.Tensor:
@@ -287,7 +293,7 @@ def _typed(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str) -> torc
         raise _lib.Ab2Error(-3, f"{what} must be {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise _lib.Ab2Error(-1, f"{what} must have shape {list(shape)}, got {list(t.shape)}")
-    return t if t.is_contiguous() else t.contiguous()
+    return t.contiguous()
 
 
 def _heads(t: torch.Tensor, what: str):
@@ -300,6 +306,11 @@ def _heads(t: torch.Tensor, what: str):
     if (s2 == 1 or d == 1) and (s1 == d or h == 1) and (s0 >= h * d or n < 2):
         return t, (s0 if n > 1 else h * d)
     return t.contiguous(), h * d
+
+
+def _fresh(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor like t."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _rotation(frequencies, layout: str, dim: int):
@@ -332,9 +343,9 @@ def rotary_apply(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     positions = _typed(positions, positions.dtype, (n,), "positions")
     frequencies, rot = _rotation(frequencies, layout, d)
     if out is None:
-        qo, qos, ko, kos = torch.empty((n, h, d), dtype=q.dtype, device=q.device), h * d, None, kv * d
+        qo, qos, ko, kos = _fresh(q), h * d, None, kv * d
         if k is not None:
-            ko = torch.empty((n, kv, d), dtype=q.dtype, device=q.device)
+            ko = _fresh(k)
     else:
         qo, qos = _result(out[0], q, "out[0]")
         ko, kos = _result(out[1], k, "out[1]") if k is not None else (None, 0)
@@ -399,7 +410,7 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, 
         if q.shape[0] != n or q.shape[2] != d or q.dtype != k.dtype:
             raise _lib.Ab2Error(-1, f"q {list(q.shape)} {q.dtype} does not match k {list(k.shape)} {k.dtype}")
         if out is None:
-            qo, qos = torch.empty((n, h, d), dtype=q.dtype, device=q.device), h * d
+            qo, qos = _fresh(q), h * d
         else:
             qo, qos = _result(out, q, "out")
     check(lib.ab2_paged_append(C.byref(c), k.data_ptr(), ks, v.data_ptr(), vs, q.data_ptr() if q is not None else None, qs, h,
@@ -427,7 +438,7 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if (q.data_ptr() | qs * q.element_size()) & 15:
         q, qs = q.clone(memory_format=torch.contiguous_format), h * d
     if out is None:
-        out, os = torch.empty((n, h, d), dtype=q.dtype, device=q.device), h * d
+        out, os = _fresh(q), h * d
     else:
         out, os = _result(out, q, "out")
     if max_new is None:
@@ -498,7 +509,7 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, len
         allowed = _typed(allowed, torch.int32, (rows, (vocab + 31) // 32), "allowed")
         ap = allowed.data_ptr()
     if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        out = _fresh(logits)
     elif out.shape != logits.shape or out.dtype != logits.dtype or not out.is_contiguous():
         raise _lib.Ab2Error(-1, f"out must be contiguous {logits.dtype} {list(logits.shape)}")
     check(lib.ab2_adjust_logits(logits.data_ptr(), stride, rows, vocab, hp, hs, width, lp, rp, bp, vp, biases, ap, out.data_ptr(),

@@ -26,7 +26,8 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 
 def stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream of the current device (its handle alone: building a Stream object took 3 us of every call)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _ptr(a) -> int:

@@ -88,7 +88,7 @@ class Batch:
                 refs.append(torch.zeros_like(q)); tols.append(torch.zeros_like(q))
                 continue
             s = torch.einsum("ihd,jhd->hij", q, k) * self.scale
-            mag = torch.einsum("ihd,jhd->hij", q.abs(), k.abs()) * self.scale
+            mag = torch.einsum("ihd,jhd->hij", q.abs(), k.abs()) * abs(self.scale)
             late = torch.arange(n, device=q.device)[None, :] > torch.arange(n - m, n, device=q.device)[:, None]
             p = torch.exp(s.masked_fill(late, -math.inf) - s.masked_fill(late, -math.inf).amax(-1, keepdim=True).clamp(min=-1e300))
             p = p.masked_fill(late, 0.0)

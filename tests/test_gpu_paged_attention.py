@@ -94,6 +94,15 @@ def test_scores_far_apart(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("new", [1, 4, 70])
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1.0])
+def test_any_scale(dtype, new, scale):
+    b = Batch([300, 95], [new, new], 8, 2, 64, 16, dtype, seed=3, scatter=0.5)
+    b.scale = scale
+    check(b)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("new", [1, 6, 90])
 def test_strides_padding_and_results_in_place(dtype, new):
     p = pkg()
