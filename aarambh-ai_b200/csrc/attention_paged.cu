@@ -184,51 +184,64 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
     }
 }
 
-// The pieces of cut items: CTA (c, y) finishes rows of the item that run c of the launch before began and did not end.
+// The pieces of cut items: CTA (c, y) finishes rows of the item that run c of the launch before began and did not end.  GROUPS times 128 threads share an
+// item's pieces out: there are two or three where a run is a CTA's, and up to as many as there are runs where it is a warp's.
 constexpr int MERGE_ROWS = 16;   // of a CTA
-template <typename T, int HD>
-__global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
+template <typename T, int HD, int GROUPS>
+__global__ void __launch_bounds__(128 * GROUPS) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int LANES = 8 * GROUPS, THREADS = 128 * GROUPS;   // lanes of a row, for its maximum
     __shared__ float tops[MERGE_ROWS], sums[MERGE_ROWS];
+    __shared__ float4 others[GROUPS][128];
     pdl_wait();
     const int c = blockIdx.x, group = a.plan.group;
     const int4 cut = a.cut[c];
-    const int rows = cut.y * group - blockIdx.y * MERGE_ROWS, pieces = cut.w - c + 1;
+    const int rows = min(cut.y * group - (int)blockIdx.y * MERGE_ROWS, MERGE_ROWS), pieces = cut.w - c + 1;
     if (rows <= 0) return;
     // run c's piece is its last, the others' is their first: slots 2 c + 1, 2 c + 2, 2 c + 4, ...
     const size_t row0 = (size_t)blockIdx.y * MERGE_ROWS;
     auto slot = [&](int j) { return (2 * (size_t)(c + j) + (j == 0)) * a.tile_rows + row0; };
-    // a row's maximum over all pieces, and the sum of its weights relative to it: 8 lanes a row
-    for (int r = threadIdx.x >> 3; r < MERGE_ROWS; r += PA_THREADS / 8) {
+    {   // a row's maximum over all pieces, and the sum of its weights relative to it
+        const int r = threadIdx.x / LANES;
         float top = -INFINITY, sum = 0.f;
-        if (r < rows) {
+        if (r < rows)
 #pragma unroll 4
-            for (int j = threadIdx.x & 7; j < pieces; j += 8) {
-                const float2 ml = *reinterpret_cast<const float2 *>(a.ml + (slot(j) + r) * 2);
-                const float best = fmaxf(top, ml.x), m = best == -INFINITY ? 0.f : best;
-                sum = sum * exp2f(top - m) + ml.y * exp2f(ml.x - m);
-                top = best;
-            }
-        }
+            for (int j = threadIdx.x % LANES; j < pieces; j += LANES) top = fmaxf(top, a.ml[(slot(j) + r) * 2]);
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-            const float t = __shfl_xor_sync(0xffffffffu, top, o), s = __shfl_xor_sync(0xffffffffu, sum, o), best = fmaxf(top, t), m = best == -INFINITY ? 0.f : best;
-            // in the same order on both sides, so that all lanes have the same bits
-            const float lo = (threadIdx.x & o) ? s * exp2f(t - m) : sum * exp2f(top - m), hi = (threadIdx.x & o) ? sum * exp2f(top - m) : s * exp2f(t - m);
-            sum = lo + hi;
-            top = best;
-        }
-        if ((threadIdx.x & 7) == 0) { tops[r] = top == -INFINITY ? 0.f : top; sums[r] = sum; }
+        for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float m = top == -INFINITY ? 0.f : top;
+        if (r < rows)
+#pragma unroll 4
+            for (int j = threadIdx.x % LANES; j < pieces; j += LANES) {
+                const float2 ml = *reinterpret_cast<const float2 *>(a.ml + (slot(j) + r) * 2);
+                sum = fmaf(ml.y, exp2f(ml.x - m), sum);
+            }
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (threadIdx.x % LANES == 0) { tops[r] = m; sums[r] = sum; }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < min(rows, MERGE_ROWS) * (HD / 4); i += PA_THREADS) {
-        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+    const int part = threadIdx.x / 128;
+    for (int i0 = 0; i0 < rows * (HD / 4); i0 += 128) {
+        const int i = i0 + threadIdx.x % 128, r = i / (HD / 4), d = i % (HD / 4) * 4;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < rows)
 #pragma unroll 8
-        for (int j = 0; j < pieces; ++j) {
-            const float f = exp2f(a.ml[(slot(j) + r) * 2] - tops[r]);
-            const float4 v = *reinterpret_cast<const float4 *>(a.acc + (slot(j) + r) * HD + d);
-            o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+            for (int j = part; j < pieces; j += GROUPS) {
+                const float f = exp2f(a.ml[(slot(j) + r) * 2] - tops[r]);
+                const float4 v = *reinterpret_cast<const float4 *>(a.acc + (slot(j) + r) * HD + d);
+                o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+            }
+        if (GROUPS > 1) {
+            if (i0 > 0) __syncthreads();   // the sums before have been taken
+            others[part][threadIdx.x % 128] = o;
+            __syncthreads();
+            if (part > 0) continue;
+            for (int g = 1; g < GROUPS; ++g) {
+                const float4 v = others[g][threadIdx.x];
+                o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+            }
         }
+        if (r >= rows) continue;
         const float f = sums[r] == 0.f ? 0.f : 1.f / sums[r];
         const int row = (int)row0 + r, tok = row / group;
         T *dst = (T *)a.out + (size_t)(cut.x + tok) * a.o_stride + (size_t)(cut.z * group + row - tok * group) * HD + d;
@@ -268,9 +281,11 @@ int simt_attention(const PagedAttnArgs &a, int hd, int max_new, void *workspace,
 int paged_merge(const PagedAttnArgs &a, int hd, ab2_dtype dtype, cudaStream_t s) {
     ChainedLaunches chained(true);
     const dim3 grid(a.ctas, (a.tile_rows + MERGE_ROWS - 1) / MERGE_ROWS);
-    auto kernel = dtype == AB2_F32 ? (hd == 128 ? paged_merge_kernel<float, 128> : paged_merge_kernel<float, 64>)
-                                   : (hd == 128 ? paged_merge_kernel<__nv_bfloat16, 128> : paged_merge_kernel<__nv_bfloat16, 64>);
-    cudaError_t e = launch_kernel(kernel, grid, dim3(PA_THREADS), 0, s, a);
+    const bool tall = a.tile_rows > 32;   // a run is a CTA's, and few of them share an item
+    auto kernel = dtype == AB2_F32 ? (hd == 128 ? paged_merge_kernel<float, 128, 4> : paged_merge_kernel<float, 64, 4>)
+                  : tall           ? (hd == 128 ? paged_merge_kernel<__nv_bfloat16, 128, 1> : paged_merge_kernel<__nv_bfloat16, 64, 1>)
+                                   : (hd == 128 ? paged_merge_kernel<__nv_bfloat16, 128, 4> : paged_merge_kernel<__nv_bfloat16, 64, 4>);
+    cudaError_t e = launch_kernel(kernel, grid, dim3(dtype == AB2_BF16 && tall ? 128 : 512), 0, s, a);
     if (e != cudaSuccess) return fail(AB2_ERR_CUDA, "paged attention launch failed: %s", cudaGetErrorString(e));
     return AB2_OK;
 }

@@ -15,14 +15,14 @@ using namespace ab2;
 namespace ab2 {
 namespace {
 
-constexpr int ROT_WARPS = 4, ROT_BATCH = 2;  // items of a lane in flight
+constexpr int ROT_WARPS = 4, ROT_BATCH = 4;  // heads of a lane in flight
 
 struct RotArgs {
     const void *q, *k, *v;
     void *qo, *ko;
     long long q_stride, k_stride, v_stride, qo_stride, ko_stride;  // elements from a token to the next
     int heads, kv_heads, dim, pairs, tokens, chunks;               // chunks of P pairs a head has, the unturned dimensions among them
-    int per_warp, parts;                                           // items (head, chunk) of a warp, warps of a token
+    int per_warp, parts;                                           // heads of q, k and v of a warp, warps of a token
     const void *pos;
     int pos64;
     const double *freq;
@@ -32,37 +32,83 @@ struct RotArgs {
     int *status;
 };
 
-// E elements in one load or store (E * sizeof(T) is 2, 4, 8, 16 or 32 bytes)
+// E elements in loads and stores of up to 16 bytes, held as 32-bit words (one element: as itself).
 template <typename T, int E> struct Vec {
-    static constexpr int BYTES = E * (int)sizeof(T), WORD = BYTES >= 16 ? 16 : BYTES;
-    T e[E];
+    static constexpr int WORDS = E * (int)sizeof(T) / 4;
+    uint32_t w[WORDS];
     __device__ __forceinline__ void load(const T *p) {
+        if constexpr (WORDS % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < BYTES; i += WORD) {
-            if constexpr (WORD == 16) *reinterpret_cast<uint4 *>((char *)e + i) = *reinterpret_cast<const uint4 *>((const char *)p + i);
-            else if constexpr (WORD == 8) *reinterpret_cast<uint2 *>((char *)e + i) = *reinterpret_cast<const uint2 *>((const char *)p + i);
-            else if constexpr (WORD == 4) *reinterpret_cast<uint32_t *>((char *)e + i) = *reinterpret_cast<const uint32_t *>((const char *)p + i);
-            else *reinterpret_cast<uint16_t *>((char *)e + i) = *reinterpret_cast<const uint16_t *>((const char *)p + i);
+            for (int i = 0; i < WORDS; i += 4) { const uint4 v = *reinterpret_cast<const uint4 *>((const uint32_t *)p + i); w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w; }
+        } else {
+            static_assert(WORDS == 2, "chunks of 8 or 16 bytes");
+            const uint2 v = *reinterpret_cast<const uint2 *>(p);
+            w[0] = v.x; w[1] = v.y;
         }
     }
     __device__ __forceinline__ void store(T *p) const {
+        if constexpr (WORDS % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < BYTES; i += WORD) {
-            if constexpr (WORD == 16) *reinterpret_cast<uint4 *>((char *)p + i) = *reinterpret_cast<const uint4 *>((const char *)e + i);
-            else if constexpr (WORD == 8) *reinterpret_cast<uint2 *>((char *)p + i) = *reinterpret_cast<const uint2 *>((const char *)e + i);
-            else if constexpr (WORD == 4) *reinterpret_cast<uint32_t *>((char *)p + i) = *reinterpret_cast<const uint32_t *>((const char *)e + i);
-            else *reinterpret_cast<uint16_t *>((char *)p + i) = *reinterpret_cast<const uint16_t *>((const char *)e + i);
+            for (int i = 0; i < WORDS; i += 4) *reinterpret_cast<uint4 *>((uint32_t *)p + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        } else {
+            *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
         }
     }
 };
-
-// Where an item (a head's chunk) lies: its first P elements, and the others `gap` further.
-template <typename T> struct RotItem {
-    const T *src;
-    T *dst;
-    int gap, chunk;   // from `turned` on: passes as it is
-    bool kept;
+template <typename T> struct Vec<T, 1> {
+    T e;
+    __device__ __forceinline__ void load(const T *p) { e = *p; }
+    __device__ __forceinline__ void store(T *p) const { *p = e; }
 };
+__device__ __forceinline__ float2 two_of(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ float2 two_of(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+__device__ __forceinline__ uint32_t word_of(float lo, float hi, __nv_bfloat16) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&b);
+}
+__device__ __forceinline__ uint32_t word_of(float lo, float hi, __half) {
+    const __half2 b = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&b);
+}
+__device__ __forceinline__ void turn(float &x, float &y, float c, float s) {
+    const float u = x, v = y;
+    x = u * c - v * s;
+    y = u * s + v * c;
+}
+
+// A chunk of P pairs turned: x and y are its first P elements and its others.  (Interleaved: pair j is elements 2 j and 2 j + 1 of the 2 P.)
+template <typename T, int P, bool HALF> __device__ __forceinline__ void rot_turn(Vec<T, P> &x, Vec<T, P> &y, const float (&c)[P], const float (&s)[P]) {
+    if constexpr (P == 1) {
+        float u = to_f32(x.e), v = to_f32(y.e);
+        turn(u, v, c[0], s[0]);
+        x.e = from_f32<T>(u);
+        y.e = from_f32<T>(v);
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            uint32_t &e0 = HALF ? x.w[j] : 2 * j < P ? x.w[(2 * j) % P] : y.w[(2 * j) % P];
+            uint32_t &e1 = HALF ? y.w[j] : 2 * j + 1 < P ? x.w[(2 * j + 1) % P] : y.w[(2 * j + 1) % P];
+            float u = __uint_as_float(e0), v = __uint_as_float(e1);
+            turn(u, v, c[j], s[j]);
+            e0 = __float_as_uint(u);
+            e1 = __float_as_uint(v);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < P / 2; ++j) {
+            float2 u = two_of(x.w[j], T()), v = two_of(y.w[j], T());
+            if (HALF) {
+                turn(u.x, v.x, c[2 * j], s[2 * j]);
+                turn(u.y, v.y, c[2 * j + 1], s[2 * j + 1]);
+            } else {
+                turn(u.x, u.y, c[j], s[j]);
+                turn(v.x, v.y, c[P / 2 + j], s[P / 2 + j]);
+            }
+            x.w[j] = word_of(u.x, u.y, T());
+            y.w[j] = word_of(v.x, v.y, T());
+        }
+    }
+}
 
 // EVEN: a head's chunks divide 32, so that a lane keeps its chunk from head to head.
 template <typename T, int P, bool HALF, bool PAGED, bool EVEN>
@@ -97,92 +143,77 @@ __global__ void __launch_bounds__(32 * ROT_WARPS, 6) rotary_kernel(const __grid_
         pos = a.pos64 ? ((const long long *)a.pos)[t] : ((const int *)a.pos)[t];
     }
     const int turned = a.pairs / P;          // chunks that turn
-    const int lo = part * a.per_warp, vheads = a.heads + a.kv_heads * (PAGED ? 2 : 1), hi = min(lo + a.per_warp, vheads * a.chunks);
-    auto item = [&](int h, int chunk) {
-        RotItem<T> it;
-        const int at = chunk < turned ? (HALF ? chunk * P : chunk * 2 * P) : 2 * a.pairs + (chunk - turned) * 2 * P;
-        it.gap = HALF && chunk < turned ? a.pairs : P;
-        it.chunk = chunk;
-        it.kept = true;
-        if (h < a.heads) {
-            it.src = (const T *)a.q + ((size_t)t * a.q_stride + (size_t)(h * a.dim + at));
-            it.dst = (T *)a.qo + ((size_t)t * a.qo_stride + (size_t)(h * a.dim + at));
-        } else {
-            const int g = h - a.heads;
-            const bool value = PAGED && g >= a.kv_heads;
-            const int of = (value ? g - a.kv_heads : g) * a.dim + at;
-            if (value) it.chunk = turned;
-            it.src = (value ? (const T *)a.v + (size_t)t * a.v_stride : (const T *)a.k + (size_t)t * a.k_stride) + of;
-            if (PAGED) {
-                it.dst = (T *)(value ? a.vp : a.kp) + (slot + ((size_t)(value ? g - a.kv_heads : g) << a.cache.page_shift)) * a.dim + at;
-                it.kept = kept;
-            } else {
-                it.dst = (T *)a.ko + (size_t)t * a.ko_stride + of;
-            }
-        }
-        return it;
-    };
-    const int step = EVEN ? 32 / a.chunks : 0;
-    int head = (lo + lane) / a.chunks;
-    const int chunk0 = (lo + lane) % a.chunks;
     float2 *cs = turns + warp * a.pairs;
+    for (int j = lane; j < a.pairs; j += 32) {   // a pair a lane
+        float2 v;
+        turn_cos_sin((unsigned long long)pos * turns_per_position(__ldg(a.freq + j)), a.mag, v.x, v.y);
+        cs[j] = v;
+    }
+    __syncwarp();
     float c[P], s[P];
     int known = -1;                          // the chunk whose angles c and s are
-    bool first = true;
-    for (int i0 = lo + lane; __any_sync(0xffffffffu, i0 < hi); i0 += 32 * ROT_BATCH) {
-        RotItem<T> it[ROT_BATCH];
-        Vec<T, P> x[ROT_BATCH], y[ROT_BATCH];
+    auto angles = [&](int chunk) {
+        if (chunk == known || chunk >= turned) return;
+        known = chunk;
 #pragma unroll
-        for (int b = 0; b < ROT_BATCH; ++b) {
-            const int i = i0 + 32 * b;
-            it[b] = EVEN ? item(head, chunk0) : item(i / a.chunks, i % a.chunks);
-            head += step;
-            if (i < hi) {
-                x[b].load(it[b].src);
-                y[b].load(it[b].src + it[b].gap);
-            }
-        }
-        if (first) {   // while the first items come, a pair a lane
-            first = false;
-            for (int j = lane; j < a.pairs; j += 32) {
-                float2 v;
-                turn_cos_sin((unsigned long long)pos * turns_per_position(__ldg(a.freq + j)), a.mag, v.x, v.y);
-                cs[j] = v;
-            }
-            __syncwarp();
-        }
+        for (int j = 0; j < P; ++j) { const float2 v = cs[chunk * P + j]; c[j] = v.x; s[j] = v.y; }
+    };
+    auto start = [&](int chunk) { return chunk < turned ? (HALF ? chunk * P : chunk * 2 * P) : 2 * a.pairs + (chunk - turned) * 2 * P; };
+    // Heads [h0, h1) of a tensor whose first lies at src, and goes to dst: `gap` elements from a head to the next there.
+    const int step = EVEN ? 32 / a.chunks : 0, sub = EVEN ? lane / a.chunks : 0, chunk0 = EVEN ? lane % a.chunks : 0;
+    if (EVEN) angles(chunk0);
+    auto heads = [&](const T *src, T *dst, size_t gap, int h0, int h1, bool turns) {
+        if (EVEN) {
+            const bool turn = turns && chunk0 < turned;
+            const int at = start(chunk0), other = HALF && chunk0 < turned ? a.pairs : P;
+            for (int h = h0 + sub; h < h1; h += step * ROT_BATCH) {
+                Vec<T, P> x[ROT_BATCH], y[ROT_BATCH];
+                const T *from = src + (h * a.dim + at);
+                T *to = dst + (size_t)h * gap + at;
 #pragma unroll
-        for (int b = 0; b < ROT_BATCH; ++b) {
-            if (i0 + 32 * b >= hi) continue;
-            if (it[b].chunk < turned) {
-                if (EVEN ? known < 0 : it[b].chunk != known) {
-                    known = it[b].chunk;
-#pragma unroll
-                    for (int j = 0; j < P; ++j) { const float2 v = cs[known * P + j]; c[j] = v.x; s[j] = v.y; }
-                }
-                if (HALF) {
-#pragma unroll
-                    for (int j = 0; j < P; ++j) {
-                        const float u = to_f32(x[b].e[j]), v = to_f32(y[b].e[j]);
-                        x[b].e[j] = from_f32<T>(u * c[j] - v * s[j]);
-                        y[b].e[j] = from_f32<T>(u * s[j] + v * c[j]);
+                for (int b = 0; b < ROT_BATCH; ++b)
+                    if (h + b * step < h1) {
+                        x[b].load(from + b * step * a.dim);
+                        y[b].load(from + b * step * a.dim + other);
                     }
-                } else {
 #pragma unroll
-                    for (int j = 0; j < P; ++j) {  // pair j: elements 2j and 2j + 1 of the 2 P of x and y
-                        T &e0 = 2 * j < P ? x[b].e[(2 * j) % P] : y[b].e[(2 * j) % P];
-                        T &e1 = 2 * j + 1 < P ? x[b].e[(2 * j + 1) % P] : y[b].e[(2 * j + 1) % P];
-                        const float u = to_f32(e0), v = to_f32(e1);
-                        e0 = from_f32<T>(u * c[j] - v * s[j]);
-                        e1 = from_f32<T>(u * s[j] + v * c[j]);
+                for (int b = 0; b < ROT_BATCH; ++b)
+                    if (h + b * step < h1) {
+                        if (turn) rot_turn<T, P, HALF>(x[b], y[b], c, s);
+                        x[b].store(to + (size_t)(b * step) * gap);
+                        y[b].store(to + (size_t)(b * step) * gap + other);
                     }
-                }
             }
-            if (!it[b].kept) continue;
-            x[b].store(it[b].dst);
-            y[b].store(it[b].dst + it[b].gap);
+        } else {
+            for (int i = h0 * a.chunks + lane; i < h1 * a.chunks; i += 32) {
+                const int h = i / a.chunks, chunk = i - h * a.chunks, at = start(chunk), other = HALF && chunk < turned ? a.pairs : P;
+                Vec<T, P> x, y;
+                x.load(src + (h * a.dim + at));
+                y.load(src + (h * a.dim + at + other));
+                if (turns && chunk < turned) {
+                    angles(chunk);
+                    rot_turn<T, P, HALF>(x, y, c, s);
+                }
+                x.store(dst + (size_t)h * gap + at);
+                y.store(dst + (size_t)h * gap + at + other);
+            }
         }
+    };
+    // the warp's share of the heads of q, k and v, one after the other
+    const int h0 = part * a.per_warp, h1 = h0 + a.per_warp, dim = a.dim;
+    auto share = [&](int first, int count, int &lo, int &hi) { lo = min(max(h0 - first, 0), count); hi = min(max(h1 - first, 0), count); };
+    int lo, hi;
+    share(0, a.heads, lo, hi);
+    if (lo < hi) heads((const T *)a.q + (size_t)t * a.q_stride, (T *)a.qo + (size_t)t * a.qo_stride, dim, lo, hi, true);
+    if (!kept) return;
+    share(a.heads, a.kv_heads, lo, hi);
+    if (lo < hi) {
+        if (PAGED) heads((const T *)a.k + (size_t)t * a.k_stride, (T *)a.kp + slot * dim, (size_t)dim << a.cache.page_shift, lo, hi, true);
+        else heads((const T *)a.k + (size_t)t * a.k_stride, (T *)a.ko + (size_t)t * a.ko_stride, dim, lo, hi, true);
     }
+    if (!PAGED) return;
+    share(a.heads + a.kv_heads, a.kv_heads, lo, hi);
+    if (lo < hi) heads((const T *)a.v + (size_t)t * a.v_stride, (T *)a.vp + slot * dim, (size_t)dim << a.cache.page_shift, lo, hi, false);
 }
 
 template <typename T, int P, bool EVEN>
@@ -204,11 +235,10 @@ int rotary_go(RotArgs a, bool half, bool paged, ab2_dtype dtype, cudaStream_t s)
     int P = dtype == AB2_F32 ? 4 : 8;
     while (P > 1 && (a.pairs % P || rest % (2 * P) || steps % P || where % std::min<size_t>(16, P * esize))) P = P == 8 ? 4 : 1;
     a.chunks = a.dim / (2 * P);
-    // A warp's items: all of a token's where there are tokens enough for some warps on every scheduler, else fewer (a lane has one at least).
-    const int items = (a.heads + a.kv_heads * (paged ? 2 : 1)) * a.chunks, want = std::max(1, device_sm_count() * 16 / std::max(1, a.tokens));
-    a.parts = std::max(1, std::min(want, (items + 31) / 32));
-    a.per_warp = ((items + a.parts - 1) / a.parts + 31) / 32 * 32;
-    a.parts = (items + a.per_warp - 1) / a.per_warp;
+    // A warp has all heads of a token where there are tokens enough for some warps on every scheduler, else fewer: a load a lane at least.
+    const int vheads = a.heads + a.kv_heads * (paged ? 2 : 1), want = std::max(1, device_sm_count() * 16 / std::max(1, a.tokens)), least = std::max(1, 32 / a.chunks);
+    a.per_warp = std::max(least, (vheads + want - 1) / want);
+    a.parts = (vheads + a.per_warp - 1) / a.per_warp;
     AB2_REQUIRE(((long long)a.tokens * a.parts + ROT_WARPS - 1) / ROT_WARPS < (1ll << 31), AB2_ERR_BAD_SHAPE, "%d tokens of %d heads are more than one launch takes", a.tokens, a.heads);
     const bool even = 32 % a.chunks == 0;
 #define AB2_ROTARY(T)                                                                                                                                   \
