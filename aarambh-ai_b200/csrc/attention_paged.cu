@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(128 * GROUPS) paged_merge_kernel(const __grid_
     }
 }
 
-int simt_ctas() { return 2 * device_sm_count(); }
+int simt_ctas(int hd) { return (hd == 64 ? 4 : 2) * device_sm_count(); }   // what shared memory holds
 
 template <int HD, int QR>
 int launch_simt(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
@@ -264,7 +264,7 @@ int launch_simt(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) 
         AB2_CUDA(cudaFuncSetAttribute(paged_simt_kernel<HD, QR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
         configured[dev] = true;
     }
-    paged_deal(a, simt_ctas(), QR, 6, 1, HD, workspace, bytes);
+    paged_deal(a, simt_ctas(HD), QR, 5, 1, HD, workspace, bytes);
     paged_simt_kernel<HD, QR><<<a.ctas, PA_THREADS, S::SMEM, s>>>(a);
     AB2_LAUNCH_CHECK();
     return a.plan.whole ? AB2_OK : paged_merge(a, HD, AB2_F32, s);
@@ -295,7 +295,7 @@ int paged_merge(const PagedAttnArgs &a, int hd, ab2_dtype dtype, cudaStream_t s)
 AB2_API int ab2_paged_workspace(int head_dim, size_t *bytes) {
     AB2_REQUIRE(bytes, AB2_ERR_BAD_ARG, "null argument");
     AB2_REQUIRE(head_dim == 64 || head_dim == 128, AB2_ERR_UNSUPPORTED, "paged caches have heads of 64 or 128, not %d", head_dim);
-    *bytes = std::max(std::max(paged_piece_bytes(simt_ctas(), 32, head_dim), paged_mma_bytes(head_dim)), paged_tc_bytes(head_dim));
+    *bytes = std::max(std::max(paged_piece_bytes(simt_ctas(head_dim), 32, head_dim), paged_mma_bytes(head_dim)), paged_tc_bytes(head_dim));
     return AB2_OK;
 }
 

@@ -19,7 +19,10 @@ namespace ab2 {
 int device_sm_count();
 namespace {
 
-constexpr int LG_THREADS = 256, LG_SLICE = 4096;   // tokens a CTA at most
+constexpr int LG_THREADS = 256, LG_CTAS = 5;
+// Tokens a CTA at most: its loads of logits are all in flight, a token at a time fewer, and a table each takes the room of two.
+template <int V, bool PACKED> constexpr int LG_SLICE = (V == 1 ? 2048 : 8192) / (PACKED ? 1 : 2);
+constexpr int LG_COUNT = 20;                       // bits of a table's word for the count, the others are the bias list's entry
 
 struct LogitArgs {
     const void *logits;
@@ -37,27 +40,22 @@ struct LogitArgs {
     int words;
 };
 
-// One token's logit.
-__device__ __forceinline__ float ruled(float z, int count, float rho, float presence, float frequency) {
-    if (count == 0) return z;
-    z = z > 0.f ? z / rho : z * rho;
-    return z - (presence + frequency * (float)count);
-}
-
 template <typename T> __device__ __forceinline__ uint32_t lowest_bits();   // of -inf
 template <> __device__ __forceinline__ uint32_t lowest_bits<float>() { return 0xff800000u; }
 template <> __device__ __forceinline__ uint32_t lowest_bits<__half>() { return 0xfc00u; }
 template <> __device__ __forceinline__ uint32_t lowest_bits<__nv_bfloat16>() { return 0xff80u; }
 
-template <typename T, int V>  // V elements a load
-__global__ void __launch_bounds__(LG_THREADS) adjust_logits_kernel(const __grid_constant__ LogitArgs a) {
-    // [slice / 32] which tokens the history or the biases touch, [slice] counts, with biases [slice] the list's entry for the token, + 1
+// V elements a load.  PACKED: a token's count and its entry of the bias list, + 1, share a word (fewer than 2^20 and 2^12 of them), else a table each.
+template <typename T, int V, bool PACKED>
+__global__ void __launch_bounds__(LG_THREADS, LG_CTAS) adjust_logits_kernel(const __grid_constant__ LogitArgs a) {
+    // [slice / 32] which tokens the history or the biases touch, [slice] counts, not PACKED [slice] entries
     extern __shared__ __align__(16) uint32_t touched[];
-    int *counts = (int *)touched + a.slice / 32, *entry = counts + (a.history ? a.slice : 0);
+    int *counts = (int *)touched + a.slice / 32, *entry = counts + (PACKED ? 0 : a.slice);
+    constexpr int ENTRY = PACKED ? LG_COUNT : 0;   // where a word's entry begins
     const int row = blockIdx.y, first = blockIdx.x * a.slice, n = min(a.slice, a.vocab - first);
     const T *in = (const T *)a.logits + row * a.stride + first;
     const uint32_t *mask = a.allowed ? a.allowed + (size_t)row * a.words + (first >> 5) : nullptr;
-    constexpr int LOADS = LG_SLICE / (LG_THREADS * V);   // the slice's logits are on their way while the tables are made
+    constexpr int LOADS = LG_SLICE<V, PACKED> / (LG_THREADS * V);   // the slice's logits are on their way while the tables are made
     alignas(16) T e[LOADS][V];
     uint32_t bits[LOADS];
 #pragma unroll
@@ -68,9 +66,16 @@ __global__ void __launch_bounds__(LG_THREADS) adjust_logits_kernel(const __grid_
         else e[b][0] = in[i];
         bits[b] = mask ? mask[i >> 5] >> (i & 31) : 0xffffffffu;
     }
-    const int tables = a.slice / 32 + (a.history ? a.slice : 0) + (a.biases ? a.slice : 0);
+    const int tables = a.slice / 32 + (a.history || a.biases ? (PACKED ? 1 : 2) * a.slice : 0);
     for (int i = threadIdx.x * 4; i < tables; i += LG_THREADS * 4) *reinterpret_cast<uint4 *>(touched + i) = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
+    for (int i = threadIdx.x; i < a.biases; i += LG_THREADS) {
+        const int v = a.bias_ids[(size_t)row * a.biases + i] - first;
+        if ((unsigned)v >= (unsigned)n) continue;
+        atomicMax((unsigned *)entry + v, (unsigned)(i + 1) << ENTRY);
+        atomicOr(touched + (v >> 5), 1u << (v & 31));
+    }
+    if (PACKED && a.biases) __syncthreads();   // the counts come below the entries
     float rho = 1.f, presence = 0.f, frequency = 0.f;
     if (a.history) {
         rho = a.rules[3 * row]; presence = a.rules[3 * row + 1]; frequency = a.rules[3 * row + 2];
@@ -97,68 +102,62 @@ __global__ void __launch_bounds__(LG_THREADS) adjust_logits_kernel(const __grid_
         }
         for (int i = done + threadIdx.x; i < len; i += LG_THREADS) count(h[i] - first);
     }
-    for (int i = threadIdx.x; i < a.biases; i += LG_THREADS) {
-        const int v = a.bias_ids[(size_t)row * a.biases + i] - first;
-        if ((unsigned)v >= (unsigned)n) continue;
-        atomicMax(entry + v, i + 1);
-        atomicOr(touched + (v >> 5), 1u << (v & 31));
-    }
-    __syncthreads();
+    // the slice as it is, and -inf where the mask says so: most tokens are in no history and no list
     T *out = (T *)a.out + (size_t)row * a.vocab + first;
-    const float *bias = a.bias_values + (size_t)row * a.biases;
 #pragma unroll
     for (int b = 0; b < LOADS; ++b) {
         const int i = (threadIdx.x + b * LG_THREADS) * V;
         if (i >= n) continue;
-        {
-            // most tokens are in no history and no list: they pass, or become -inf, as bits
-            const uint32_t any = touched[i >> 5] >> (i & 31) & ((1u << V) - 1);
-            for (uint32_t left = any & bits[b]; left; left &= left - 1) {
-                const int j = __ffs(left) - 1;
-                float z = to_f32(in[i + j]);
-                if (a.history) z = ruled(z, counts[i + j], rho, presence, frequency);
-                if (a.biases) {
-                    const int k = entry[i + j];
-                    if (k) z += bias[k - 1];
-                }
-                const T r = from_f32<T>(z);
+        if constexpr (V > 1) {
+            uint32_t q[4];
 #pragma unroll
-                for (int m = 0; m < V; ++m)
-                    if (m == j) e[b][m] = r;
-            }
-            if constexpr (V > 1) {
-                uint32_t q[4];
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    q[m] = reinterpret_cast<const uint32_t *>(e[b])[m];
-                    if constexpr (sizeof(T) == 4) {
-                        if (!((bits[b] >> m) & 1)) q[m] = lowest_bits<T>();
-                    } else {
-                        const uint32_t keep = ((bits[b] >> (2 * m)) & 1 ? 0xffffu : 0u) | ((bits[b] >> (2 * m + 1)) & 1 ? 0xffff0000u : 0u);
-                        q[m] = (q[m] & keep) | (lowest_bits<T>() * 0x10001u & ~keep);
-                    }
+            for (int m = 0; m < 4; ++m) {
+                q[m] = reinterpret_cast<const uint32_t *>(e[b])[m];
+                if constexpr (sizeof(T) == 4) {
+                    if (!((bits[b] >> m) & 1)) q[m] = lowest_bits<T>();
+                } else {
+                    const uint32_t keep = ((bits[b] >> (2 * m)) & 1 ? 0xffffu : 0u) | ((bits[b] >> (2 * m + 1)) & 1 ? 0xffff0000u : 0u);
+                    q[m] = (q[m] & keep) | (lowest_bits<T>() * 0x10001u & ~keep);
                 }
-                *reinterpret_cast<uint4 *>(out + i) = make_uint4(q[0], q[1], q[2], q[3]);
-            } else {
-                out[i] = bits[b] & 1 ? e[b][0] : from_f32<T>(-INFINITY);
             }
+            *reinterpret_cast<uint4 *>(out + i) = make_uint4(q[0], q[1], q[2], q[3]);
+        } else {
+            out[i] = bits[b] & 1 ? e[b][0] : from_f32<T>(-INFINITY);
         }
     }
+    __syncthreads();   // the tables are whole, and the tokens stored
+    // then the tokens that are in one, where the mask allows them (what has been stored is their logit): a word of 32 tokens a thread
+    const float *bias = a.bias_values + (size_t)row * a.biases, inverse = 1.f / rho;
+    for (int w = threadIdx.x; w * 32 < n; w += LG_THREADS)
+        for (uint32_t left = touched[w] & (mask ? mask[w] : 0xffffffffu); left; left &= left - 1) {
+            const int i = w * 32 + __ffs(left) - 1, word = counts[i], count = PACKED ? word & ((1 << LG_COUNT) - 1) : word;
+            const unsigned k = (unsigned)entry[i] >> ENTRY;
+            float z = to_f32(out[i]);
+            if (count > 0) z = (z > 0.f ? z * inverse : z * rho) - (presence + frequency * (float)count);
+            if (k) z += bias[k - 1];
+            out[i] = from_f32<T>(z);
+        }
 }
 
-template <typename T>
+template <typename T, int V>
 int launch_adjust(LogitArgs a, int rows, cudaStream_t s) {
-    constexpr int V = 16 / sizeof(T);
-    const bool wide = a.vocab % V == 0 && a.stride % V == 0 && (((uintptr_t)a.logits | (uintptr_t)a.out) & 15) == 0;
-    // Slices of 4096 tokens, smaller ones where those are fewer than two CTAs an SM; 512 at least, so that a thread has a load of its own.
-    a.slice = LG_SLICE;
+    // Slices of 8192 tokens, smaller ones where those are fewer than two CTAs an SM; 512 at least.  64 x 128256 bf16 behind 4096 tokens take 16.6 us
+    // (33 MB: 5.3 us of HBM); what bounds them is every slice's walk through its row's history and the look-ups of what that touches.
+    const bool packed = a.history_width < (1 << LG_COUNT) && a.biases < (1 << (32 - LG_COUNT)) - 1;
+    a.slice = packed ? LG_SLICE<V, true> : LG_SLICE<V, false>;
     while (a.slice > 512 && (long long)rows * ((a.vocab + a.slice - 1) / a.slice) < 2 * device_sm_count()) a.slice /= 2;
     const dim3 grid((a.vocab + a.slice - 1) / a.slice, rows);
-    const size_t smem = (size_t)a.slice * 4 * ((a.history ? 1 : 0) + (a.biases ? 1 : 0)) + a.slice / 8;
-    if (wide) adjust_logits_kernel<T, V><<<grid, LG_THREADS, smem, s>>>(a);
-    else adjust_logits_kernel<T, 1><<<grid, LG_THREADS, smem, s>>>(a);
+    const size_t smem = (size_t)a.slice * 4 * (a.history || a.biases ? (packed ? 1 : 2) : 0) + a.slice / 8;
+    if (packed) adjust_logits_kernel<T, V, true><<<grid, LG_THREADS, smem, s>>>(a);
+    else adjust_logits_kernel<T, V, false><<<grid, LG_THREADS, smem, s>>>(a);
     AB2_LAUNCH_CHECK();
     return AB2_OK;
+}
+template <typename T>
+int launch_adjust(const LogitArgs &a, int rows, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const bool wide = a.vocab % V == 0 && a.stride % V == 0 && (((uintptr_t)a.logits | (uintptr_t)a.out) & 15) == 0;
+    return wide ? launch_adjust<T, V>(a, rows, s) : launch_adjust<T, 1>(a, rows, s);
 }
 
 }  // namespace

@@ -289,11 +289,11 @@ def _on_device(*tensors) -> None:
 
 
 def _typed(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str) -> torch.Tensor:
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise _lib.Ab2Error(-3, f"{what} must be {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise _lib.Ab2Error(-1, f"{what} must have shape {list(shape)}, got {list(t.shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _heads(t: torch.Tensor, what: str):
@@ -443,13 +443,14 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         out, os = _result(out, q, "out")
     if max_new is None:
         max_new = 1 if starts is None else max(n, 1)
-    key = (d, q.get_device())
-    if key not in _paged_bytes:
-        size = C.c_size_t()
-        check(lib.ab2_paged_workspace(d, C.byref(size)))
-        _paged_bytes[key] = size.value
-    work = torch.empty(_paged_bytes[key], dtype=torch.uint8, device=q.device)
-    check(lib.ab2_paged_attention(C.byref(c), q.data_ptr(), qs, h, out.data_ptr(), os, max_new, scale, work.data_ptr(), work.numel(),
+    # rows that cannot be longer than 256 tokens are not worth cutting: 1 x 256 tokens take PCSMALL
+    size = _paged_bytes.get((d, q.get_device()), -1) if c.table_width * c.page_size > 256 else 0
+    if size < 0:
+        n = C.c_size_t()
+        check(lib.ab2_paged_workspace(d, C.byref(n)))
+        size = _paged_bytes[(d, q.get_device())] = n.value
+    work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    check(lib.ab2_paged_attention(C.byref(c), q.data_ptr(), qs, h, out.data_ptr(), os, max_new, scale, work.data_ptr() if size else None, size,
                                   dtype_code(q.dtype), stream_ptr()))
     return out
 

@@ -108,6 +108,18 @@ def test_rows_apart_and_offsets_off_the_boundary():
     assert torch.equal(p.dispatch.adjust_logits(wide[:, 0], h, None, r), p.dispatch.adjust_logits(wide[:, 0].contiguous(), h.contiguous(), None, r))
 
 
+def test_more_biases_and_history_than_share_a_word():
+    p = pkg()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for n, m in ((1 << 20, 3), (50, 5000), (1 << 20, 5000)):
+        logits = torch.randn(1, 9000, generator=g, device="cuda")
+        h = torch.randint(0, 9000, (1, n), generator=g, device="cuda", dtype=torch.int32)
+        h[:, ::2] = 8191   # more than a few bits of count
+        ids = torch.randint(0, 9000, (1, m), generator=g, device="cuda", dtype=torch.int32)
+        v, r = torch.randn(1, m, generator=g, device="cuda"), torch.tensor([[1.2, 0.3, 0.001]], device="cuda")
+        agree(p.dispatch.adjust_logits(logits, h, None, r, ids, v), *expected(logits, h, None, r, ids, v))
+
+
 def test_recorded_and_replayed():
     p = pkg()
     logits, h = torch.randn(2, 5000, device="cuda"), torch.zeros(2, 40, dtype=torch.int32, device="cuda")
