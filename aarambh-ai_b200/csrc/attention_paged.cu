@@ -44,12 +44,12 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
     constexpr int TX = S::TX, RPT = S::RPT, KPT = S::KPT, DPT = S::DPT, KROW = S::KROW, CH = 4;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ long long warp_sums[PA_THREADS / 32];
-    __shared__ PagedRun found;
+    __shared__ int2 found[2];
     float *kbuf = (float *)smem, *vbuf = kbuf + 2 * PA_KEYS * KROW;
     float *qs = (float *)(smem + 4 * S::BUF), *ps = qs + QR * (HD + 4);
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     const PagedView &p = a.plan.p;
-    PagedRun run = paged_run<PA_THREADS>(a.plan, blockIdx.x, gridDim.x, warp_sums, &found, a.status);
+    PagedRun run = paged_run<PA_THREADS>(a.plan, blockIdx.x, gridDim.x, warp_sums, found, a.status);
     if (threadIdx.x == 0) paged_uncut(a, blockIdx.x);
     PagedPiece w;
     while (paged_next(a.plan, run, w)) {
@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
         const int t0 = sp.t0, ntok = sp.ntok, base = sp.base, lo = sp.lo, hi = sp.hi, group = a.plan.group;
         __syncthreads();
         for (int i = threadIdx.x; i < QR * HD / 4; i += PA_THREADS) {
-            const int r = i / (HD / 4), d = i % (HD / 4) * 4, tok = r / group, g = r - tok * group;
+            const int r = i / (HD / 4), d = i % (HD / 4) * 4, tok = paged_token(a.plan, r), g = r - tok * group;
             float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
             if (tok < ntok) f = load4((const float *)a.q + (size_t)(w.r.first + t0 + tok) * a.q_stride + (size_t)(w.head * group + g) * HD + d);
             *reinterpret_cast<float4 *>(qs + r * (HD + 4) + d) = make_float4(f.x * a.sl, f.y * a.sl, f.z * a.sl, f.w * a.sl);
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
         int lim[RPT];
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
-            const int tok = (ty * RPT + i) / group;
+            const int tok = paged_token(a.plan, ty * RPT + i);
             lim[i] = tok < ntok ? base + t0 + tok : -1;
             top[i] = -INFINITY;
             sum[i] = 0.f;
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
         const size_t slot = 2 * (size_t)blockIdx.x + (w.k0 == 0);
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
-            const int r = ty * RPT + i, tok = r / group, g = r - tok * group;
+            const int r = ty * RPT + i, tok = paged_token(a.plan, r), g = r - tok * group;
 #pragma unroll
             for (int m = TX / 2; m > 0; m >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], m);
             if (tok >= ntok) continue;
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
 constexpr int MERGE_ROWS = 16;   // of a CTA
 template <typename T, int HD, int GROUPS>
 __global__ void __launch_bounds__(128 * GROUPS) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
-    constexpr int LANES = 8 * GROUPS, THREADS = 128 * GROUPS;   // lanes of a row, for its maximum
+    constexpr int LANES = 8 * GROUPS;   // of a row, for its maximum
     __shared__ float tops[MERGE_ROWS], sums[MERGE_ROWS];
     __shared__ float4 others[GROUPS][128];
     pdl_wait();
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(128 * GROUPS) paged_merge_kernel(const __grid_
         }
         if (r >= rows) continue;
         const float f = sums[r] == 0.f ? 0.f : 1.f / sums[r];
-        const int row = (int)row0 + r, tok = row / group;
+        const int row = (int)row0 + r, tok = paged_token(a.plan, row);
         T *dst = (T *)a.out + (size_t)(cut.x + tok) * a.o_stride + (size_t)(cut.z * group + row - tok * group) * HD + d;
         alignas(16) T y[4] = {from_f32<T>(o.x * f), from_f32<T>(o.y * f), from_f32<T>(o.z * f), from_f32<T>(o.w * f)};
         if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(y);

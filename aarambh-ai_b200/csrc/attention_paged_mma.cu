@@ -58,13 +58,13 @@ __global__ void __launch_bounds__(32 * PM_WARPS, 2) paged_mma_kernel(const __gri
     using S = PmShape<HD>;
     constexpr int KS = HD / 16, CH = HD / 8, STAGES = S::STAGES, LOADS = PM_KEYS * CH / 32;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ PagedRun found[PM_WARPS];
+    __shared__ int2 found[PM_WARPS][2];
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, group = a.plan.group;
     const PagedView &p = a.plan.p;
     uint8_t *ring = smem + warp * STAGES * S::BLOCK;
     const int me = warp * gridDim.x + blockIdx.x;   // a little work spreads over all SMs
-    PagedRun run = paged_run<32>(a.plan, me, a.ctas, nullptr, &found[warp], a.status);
+    PagedRun run = paged_run<32>(a.plan, me, a.ctas, nullptr, found[warp], a.status);
     if (lane == 0) paged_uncut(a, me);
 
     // ---- the copies run ahead of the products, over the same pieces
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(32 * PM_WARPS, 2) paged_mma_kernel(const __gri
         float top[NT][2], sum[NT][2], o[KS][NT][4];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const int r = 8 * t + g, tok = r / group;
+            const int r = 8 * t + g, tok = paged_token(a.plan, r);
             const uint32_t *src = (const uint32_t *)((const __nv_bfloat16 *)a.q + (size_t)(w.r.first + sp.t0 + tok) * a.q_stride + (size_t)(w.head * group + r - tok * group) * HD);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(32 * PM_WARPS, 2) paged_mma_kernel(const __gri
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int col = 8 * t + 2 * c + e;
-                lim[t][e] = col < rows ? sp.base + sp.t0 + col / group : 0x7fffffff;   // a column without a row is not looked at
+                lim[t][e] = col < rows ? sp.base + sp.t0 + paged_token(a.plan, col) : 0x7fffffff;   // a column without a row is not looked at
                 top[t][e] = PM_NONE;
                 sum[t][e] = 0.f;
             }
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(32 * PM_WARPS, 2) paged_mma_kernel(const __gri
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t x = transposed(pack_bf16(o[m][t][2 * h], o[m][t][2 * h + 1]));   // row 8 t + g, dimensions 2 c and 2 c + 1 of the 8
-                        const int r = 8 * t + g, tok = r / group;
+                        const int r = 8 * t + g, tok = paged_token(a.plan, r);
                         if (r < rows) *reinterpret_cast<uint32_t *>((__nv_bfloat16 *)a.out + (size_t)(w.r.first + sp.t0 + tok) * a.o_stride + (size_t)(w.head * group + r - tok * group) * HD + 16 * m + 8 * h + 2 * c) = x;
                     }
             } else {

@@ -40,14 +40,6 @@ template <int HD> struct PcShape {
     static constexpr int SMEM = 1024 + 2 * QTILE + SLOTS * 2 * TILE;
 };
 
-struct PcShared {
-    uint64_t full[8], empty[8], qfull[2], sfull[2], sfree[2], pfull[2], odone[2];
-    uint32_t tmem_base;
-    int failed;
-    PagedRun found;
-    long long warp_sums[PC_THREADS / 32];
-};
-
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -82,27 +74,38 @@ __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) { return pair(ex2(low(x
 struct PcPiece {
     PagedPiece w;
     PagedSpan s;
-    int tiles[2];   // of keys that a tile of rows looks at
+    int first, second;   // tiles of keys that either tile of rows looks at
     int most;
 };
 __device__ __forceinline__ bool pc_next(const PagedPlan &a, PagedRun &run, PcPiece &x) {
     if (!paged_next(a, run, x.w)) return false;
     x.s = paged_span(a, x.w);
     const int rows = x.s.ntok * a.group;
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-        // keys up to those of the last token of the tile of rows
-        const int last = min(x.s.hi, x.s.base + x.s.t0 + (min(rows, (g + 1) * PC_Q) - 1) / a.group + 1);
-        x.tiles[g] = rows > g * PC_Q ? max(0, (last - x.s.lo + PC_KEYS - 1) / PC_KEYS) : 0;
-    }
-    x.most = max(x.tiles[0], x.tiles[1]);
+    auto tiles = [&](int first, int end) {   // of rows [first, end) of the item: keys up to those of the last token
+        const int last = min(x.s.hi, x.s.base + x.s.t0 + paged_token(a, end - 1) + 1);
+        return end > first ? max(0, (last - x.s.lo + PC_KEYS - 1) / PC_KEYS) : 0;
+    };
+    x.first = tiles(0, min(rows, PC_Q));
+    x.second = tiles(PC_Q, rows);
+    x.most = max(x.first, x.second);
     return true;
 }
+
+struct PcShared {
+    uint64_t full[8], empty[8], qfull[2], sfull[2], sfree[2], pfull[2], odone[2];
+    uint32_t tmem_base;
+    int failed;
+    int2 found[2];
+    long long warp_sums[PC_THREADS / 32];
+    // of every softmax warp: its run, the piece that it is at and the next one (kept from its registers, which the scores fill)
+    PagedRun run[8];
+    PcPiece piece[8][2];
+};
 
 // One tile of keys for the warp's 32 rows, a lane each: scores to weights.  With EDGE keys past `lim` are out of sight.  `before` waits until the
 // products with the tile before are done: its weights' place is free then, and the sums stand still.
 template <int HD, bool EDGE, class Before>
-__device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, float sl, int lim, bool has_o, float &top, float &sum, uint64_t *taken, uint64_t *ready, Before before) {
+__device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, bool has_o, float &top, float &sum, uint64_t *taken, uint64_t *ready, Before before) {
     uint32_t va[32], vb[32], vc[16];
     tmem_ld32_start(va, s_addr);
     tmem_ld32_start(vb, s_addr + 32);
@@ -114,6 +117,9 @@ __device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, flo
     __syncwarp();
     if ((threadIdx.x & 31) == 0) bar_arrive(taken);
     auto v = [&](int k) -> uint32_t & { return k < 32 ? va[k] : k < 64 ? vb[k - 32] : vc[k - 64]; };
+    if (flip)   // a negative scale
+#pragma unroll
+        for (int k = 0; k < PC_KEYS; ++k) v(k) ^= 0x80000000u;
     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int k = 0; k < PC_KEYS; ++k)
@@ -199,7 +205,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    PagedRun run = paged_run<PC_THREADS>(a.plan, blockIdx.x, a.ctas, sh.warp_sums, &sh.found, a.status);
+    PagedRun run = paged_run<PC_THREADS>(a.plan, blockIdx.x, a.ctas, sh.warp_sums, sh.found, a.status);
     if (threadIdx.x == PC_THREADS - 1) paged_uncut(a, blockIdx.x);
     if (run.u >= run.u1) return;   // the whole CTA
     if (warp == 1) {
@@ -226,6 +232,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * PC_ROWS * HD * 2;
                     const int slot = n % S::SLOTS;
                     warp_wait(&sh.empty[slot], ((n++ / S::SLOTS) & 1) ^ 1, failed);
+                    if (n == 2 && x.first > 0) warp_wait(&sh.qfull[0], 0, failed);   // the first queries come before what is fetched ahead
                     if (lane == 0) bar_expect_tx(&sh.full[slot], (uint32_t)(2 * bytes));
                     __syncwarp();
                     if (mine && !*failed)
@@ -262,9 +269,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 ++scored;
             };
             while (pc_next(a.plan, run, x)) {
-                const int tiles = x.tiles[g];
-                if (x.s.ntok * a.plan.group > g * PC_Q) warp_wait(&sh.qfull[g], asked++ & 1, failed);
-                if (tiles > 0) scores(n);
+                const int tiles = g ? x.second : x.first;
+                if (tiles > 0) {
+                    warp_wait(&sh.qfull[g], asked++ & 1, failed);
+                    scores(n);
+                }
                 for (int j = 0; j < x.most; ++j, ++n) {
                     const int slot = n % S::SLOTS;
                     if (j + 1 < tiles) scores(n + 1);
@@ -293,43 +302,63 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const int g = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, group = a.plan.group;
         const uint32_t quad_addr = (uint32_t)(quad * 32) << 16, s_addr = tmem + quad_addr + (uint32_t)(g * 128), o_addr = tmem_o + quad_addr + (uint32_t)(g * HD);
         const float sl = fmaxf(fabsf(a.sl), 1.17549435e-38f);   // above 0, so that hidden scores stay -inf
-        const uint32_t flip = a.sl < 0.f ? 0x80008000u : 0u;   // a negative scale's sign goes to the queries
+        const bool flip = a.sl < 0.f;
         int n = 0, scored = 0;
-        while (pc_next(a.plan, run, x)) {
-            const int rows = x.s.ntok * group, n0 = n;
-            n += x.most;
-            if (threadIdx.x == PC_THREADS - 1) paged_cut(a, run, x.w, x.s, blockIdx.x);
-            if (rows <= g * PC_Q) continue;
-            // the queries: a quad's warp stores 32 rows of its tile, a row 16 bytes a lane
-            constexpr int Q_LOADS = PC_Q * HD / 8 / 128;   // all in flight
-            {
-                const int i0 = threadIdx.x & 127;
-                uint4 v[Q_LOADS];
-#pragma unroll
-                for (int u = 0; u < Q_LOADS; ++u) {
-                    const int i = i0 + 128 * u, d = i % (HD / 8), rr = g * PC_Q + i / (HD / 8), tok = rr / group;
-                    v[u] = make_uint4(0u, 0u, 0u, 0u);
-                    if (rr < rows) v[u] = *reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)a.q + (size_t)(x.w.r.first + x.s.t0 + tok) * a.q_stride + (size_t)(x.w.head * group + rr - tok * group) * HD + d * 8);
-                }
-#pragma unroll
-                for (int u = 0; u < Q_LOADS; ++u) {
-                    const int i = i0 + 128 * u, d = i % (HD / 8), row = i / (HD / 8);
-                    v[u].x ^= flip; v[u].y ^= flip; v[u].z ^= flip; v[u].w ^= flip;
-                    *reinterpret_cast<uint4 *>(qbuf + g * S::QTILE + (d >> 3) * PC_QBOX + row * 128 + (((d & 7) ^ (row & 7)) << 4)) = v[u];
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        int n0 = 0, here = 0;   // the first of the ring's slots of the next piece; where that is kept
+        if (lane == 0) sh.run[warp - 4] = run;
+        // the next piece in which this tile of rows has any
+        auto next = [&]() {
             __syncwarp();
-            if (lane == 0) bar_arrive(&sh.qfull[g]);
-            const int rr = g * PC_Q + r, tok = rr / group, pos = rr < rows ? x.s.base + x.s.t0 + tok : -1;
-            const int least = x.s.base + x.s.t0 + (g * PC_Q) / group;   // the first row sees up to here
+            PagedRun run = sh.run[warp - 4];
+            PcPiece x;
+            bool more;
+            while ((more = pc_next(a.plan, run, x))) {
+                n0 = n;
+                n += x.most;
+                if (threadIdx.x == PC_THREADS - 1) paged_cut(a, run, x.w, x.s, blockIdx.x);
+                if (x.s.ntok * group > g * PC_Q) break;
+            }
+            here ^= 1;
+            __syncwarp();
+            if (lane == 0) { sh.run[warp - 4] = run; sh.piece[warp - 4][here] = x; }
+            __syncwarp();
+            return more;
+        };
+        // its queries, on their way to shared memory
+        auto fetch_q = [&]() {
+            const PcPiece &x = sh.piece[warp - 4][here];
+            if ((g ? x.second : x.first) == 0) return;   // nothing to ask
+            const PagedSpan s = x.s;
+            const long long first = x.w.r.first + s.t0, head0 = x.w.head * group;
+            const int i0 = threadIdx.x & 127, rows = s.ntok * group;
+#pragma unroll
+            for (int u = 0; u < PC_Q * HD / 8 / 128; ++u) {
+                const int i = i0 + 128 * u, d = i % (HD / 8), row = i / (HD / 8), rr = g * PC_Q + row, in = rr < rows ? 16 : 0, tok = paged_token(a.plan, in ? rr : 0);
+                const __nv_bfloat16 *src = (const __nv_bfloat16 *)a.q + (first + tok) * a.q_stride + (head0 + (in ? rr - tok * group : 0)) * HD + d * 8;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(sptr(qbuf + g * S::QTILE + (d >> 3) * PC_QBOX + row * 128 + (((d & 7) ^ (row & 7)) << 4))), "l"(src), "r"(in) : "memory");
+            }
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        };
+        bool more = next();
+        if (more) fetch_q();
+        while (more) {
+            const PcPiece &x = sh.piece[warp - 4][here];
+            const int rows = x.s.ntok * group, tiles = g ? x.second : x.first, lo = x.s.lo, hi = x.s.hi, slot0 = n0;
+            if (tiles > 0) {
+                asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.qfull[g]);
+            }
+            const int rr = g * PC_Q + r, tok = paged_token(a.plan, rr), pos = rr < rows ? x.s.base + x.s.t0 + tok : -1;
+            const int least = x.s.base + x.s.t0 + paged_token(a.plan, g * PC_Q);   // the first row sees up to here
             float top = PC_NONE, sum = 0.f;
-            for (int j = 0; j < x.tiles[g]; ++j, ++scored) {
-                const int at = x.s.lo + j * PC_KEYS;
-                if (at + PC_KEYS > x.s.hi) {   // what lies behind the piece's keys may be anything
-                    const int slot = (n0 + j) % S::SLOTS;
-                    warp_wait(&sh.full[slot], ((n0 + j) / S::SLOTS) & 1, failed);
-                    if (at + r >= x.s.hi && r < PC_KEYS)
+            for (int j = 0; j < tiles; ++j, ++scored) {
+                const int at = lo + j * PC_KEYS;
+                if (at + PC_KEYS > hi) {   // what lies behind the piece's keys may be anything
+                    const int slot = (slot0 + j) % S::SLOTS;
+                    warp_wait(&sh.full[slot], ((slot0 + j) / S::SLOTS) & 1, failed);
+                    if (at + r >= hi && r < PC_KEYS)
 #pragma unroll
                         for (int b = 0; b < S::BOXES; ++b)
 #pragma unroll
@@ -339,15 +368,20 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
                 warp_wait(&sh.sfull[g], scored & 1, failed);
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                const int lim = min(pos, x.s.hi - 1) - at;
+                const int lim = min(pos, hi - 1) - at;
                 auto before = [&] { if (j > 0) warp_wait(&sh.odone[g], (scored - 1) & 1, failed); };
-                if (at + PC_KEYS - 1 > least || at + PC_KEYS > x.s.hi || (g + 1) * PC_Q > rows) pc_softmax<HD, true>(s_addr, o_addr, sl, lim, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
-                else pc_softmax<HD, false>(s_addr, o_addr, sl, lim, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
+                if (at + PC_KEYS - 1 > least || at + PC_KEYS > hi || (g + 1) * PC_Q > rows) pc_softmax<HD, true>(s_addr, o_addr, sl, flip, lim, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
+                else pc_softmax<HD, false>(s_addr, o_addr, sl, flip, lim, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
             }
-            if (x.tiles[g] > 0) warp_wait(&sh.odone[g], (scored - 1) & 1, failed);
+            // the scores are all made: the next piece's queries may take the place of these, while the sums go out
+            more = next();
+            if (more) fetch_q();
+            const PagedPiece w = x.w;
+            const PagedSpan s = x.s;
+            if (tiles > 0) warp_wait(&sh.odone[g], (scored - 1) & 1, failed);
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            const bool all = x.w.k0 == 0 && x.w.k1 == x.w.k_tiles;
-            const size_t slot = (2 * (size_t)blockIdx.x + (x.w.k0 == 0)) * a.tile_rows;
+            const bool all = w.k0 == 0 && w.k1 == w.k_tiles;
+            const size_t slot = (2 * (size_t)blockIdx.x + (w.k0 == 0)) * a.tile_rows;
             const float f = !all ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
             float poison = 0.f;  // stays 0 unless an output is Inf or NaN
             // A lane has a row, 16 bytes of which at a time would go to 32 places: four lanes exchange pieces and store 64 bytes of a row each time.
@@ -355,9 +389,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             bool have[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int row = g * PC_Q + quad * 32 + (lane & ~3) + k, t = row / group;
+                const int row = g * PC_Q + quad * 32 + (lane & ~3) + k, t = paged_token(a.plan, row);
                 have[k] = row < rows;
-                dst[k] = (__nv_bfloat16 *)a.out + (size_t)(x.w.r.first + x.s.t0 + t) * a.o_stride + (size_t)(x.w.head * group + row - t * group) * HD + 8 * (lane & 3);
+                dst[k] = (__nv_bfloat16 *)a.out + (size_t)(w.r.first + s.t0 + t) * a.o_stride + (size_t)(w.head * group + row - t * group) * HD + 8 * (lane & 3);
             }
             float *part = a.acc + (slot + g * PC_Q + quad * 32 + (lane & ~3)) * HD + 4 * (lane & 3);
 #pragma unroll 1
@@ -365,7 +399,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 uint32_t v[32];
                 __syncwarp();
                 tmem_ld32(v, o_addr + 32 * c);
-                if (x.tiles[g] == 0)
+                if (tiles == 0)
 #pragma unroll
                     for (int k = 0; k < 32; ++k) v[k] = 0u;
 #pragma unroll
@@ -406,7 +440,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             if (!all && rr < rows) *reinterpret_cast<float2 *>(a.ml + (slot + rr) * 2) = make_float2(top, sum);
             __syncwarp();
             for (uint32_t left = __ballot_sync(0xffffffffu, rr < rows && poison != 0.f); left; left &= left - 1)  // NaN is not 0
-                paged_again<HD>(a, x.w, x.s, g * PC_Q + quad * 32 + __ffs(left) - 1, lane, all, slot);
+                paged_again<HD>(a, w, s, g * PC_Q + quad * 32 + __ffs(left) - 1, lane, all, slot);
             // the next piece's products may go over what has been read
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
         }

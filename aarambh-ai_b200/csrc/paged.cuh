@@ -68,7 +68,9 @@ struct PagedPlan {
     PagedView p;
     int tq_shift, key_shift, whole, group, above, most;
     int least;                  // units that are worth a CTA
+    int per_group;              // 2^16 / group, rounded up: r / group is r per_group / 2^16 for rows r of a tile (at most 256) and groups up to 32
 };
+__device__ __forceinline__ int paged_token(const PagedPlan &a, int r) { return (r * a.per_group) >> 16; }
 struct PagedShape {
     int q_tiles, base;          // of the row; keys before its new tokens
     long long per;              // units of a head
@@ -121,18 +123,22 @@ template <int THREADS> __device__ __forceinline__ long long cta_prefix(long long
     return before + x - v;
 }
 struct PagedRun {
-    long long u, u1;       // units left to the CTA
-    int row;               // that u lies in
-    long long row_first;   // the row's first unit
+    long long u, u1;       // units left to the CTA, the first and the one behind them
     long long total;       // units of the launch
     int ctas;              // that have any
+    int row, head, q_tile, k, k_tiles;   // where the run stands: the next unit, and the units of its item
+    PagedRow r;            // that row
+    int q_tiles, base;
 };
 // Where the run of CTA c begins.
 __device__ __forceinline__ long long paged_begin(const PagedRun &run, int c) { return run.total * min(c, run.ctas) / run.ctas; }
+__device__ __forceinline__ int paged_keys(const PagedPlan &a, int base, int q_tile) {   // units of a tile of queries
+    return a.whole ? 1 : (int)(((long long)base + ((long long)(q_tile + 1) << a.tq_shift) + (1 << a.key_shift) - 1) >> a.key_shift);
+}
 // The run of CTA (or, with THREADS 32, warp) `c` of `ctas`, found by all its threads.  `found` is shared.
-template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const PagedPlan &a, int c, int ctas, long long *warp_sums, PagedRun *found, int *status) {
-    PagedRun run = {0, 0, 0, 0, 0, 0};
-    long long n, prefix = 0, units = 0;
+template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const PagedPlan &a, int c, int ctas, long long *warp_sums, int2 *found, int *status) {
+    PagedRun run = {};
+    long long n, prefix = 0, units = 0, row_first = 0;
     for (int r0 = 0; r0 < a.p.rows; r0 += THREADS) {
         const int r = r0 + (int)(threadIdx.x % THREADS);
         const long long here = r < a.p.rows ? paged_shape(a, paged_row(a.p, r, c == 0 ? status : nullptr)).units : 0;
@@ -149,20 +155,37 @@ template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const Paged
         if (r0 > 0) {
             const int r = r0 + (int)(threadIdx.x % THREADS);
             units = r < a.p.rows ? paged_shape(a, paged_row(a.p, r, nullptr)).units : 0;
-            prefix = run.row_first + cta_prefix<THREADS>(units, n, warp_sums);
+            prefix = row_first + cta_prefix<THREADS>(units, n, warp_sums);
         } else if (a.p.rows > THREADS) {
             (void)cta_prefix<THREADS>(units, n, warp_sums);
         } else {
             n = run.total;
         }
-        if (units > 0 && run.u >= prefix && run.u < prefix + units) { found->row = r0 + (int)(threadIdx.x % THREADS); found->row_first = prefix; }
-        if (run.u < run.row_first + n) break;
-        run.row_first += n;
+        if (units > 0 && run.u >= prefix && run.u < prefix + units) {
+            const PagedShape s = paged_shape(a, paged_row(a.p, r0 + (int)(threadIdx.x % THREADS), nullptr));
+            const long long in = run.u - prefix;
+            const int head = (int)(in / s.per);
+            found[0] = make_int2(r0 + (int)(threadIdx.x % THREADS), head);
+            const long long y = in - head * s.per;
+            int lo = 0, hi = s.q_tiles - 1;   // the tile that unit y of the head is of
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (paged_units(a, s.base, mid) <= y) lo = mid;
+                else hi = mid - 1;
+            }
+            found[1] = make_int2(lo, (int)(y - paged_units(a, s.base, lo)));
+        }
+        if (run.u < row_first + n) break;
+        row_first += n;
     }
     if (THREADS == 32) __syncwarp();
     else __syncthreads();
-    run.row = found->row;
-    run.row_first = found->row_first;
+    run.row = found[0].x; run.head = found[0].y; run.q_tile = found[1].x; run.k = found[1].y;
+    run.r = paged_row(a.p, run.row, nullptr);
+    const PagedShape s = paged_shape(a, run.r);
+    run.q_tiles = s.q_tiles;
+    run.base = s.base;
+    run.k_tiles = paged_keys(a, run.base, run.q_tile);
     return run;
 }
 // A piece of work: units [k0, k1) of the item (row, head, q_tile), which has k_tiles of them.
@@ -173,29 +196,27 @@ struct PagedPiece {
 // The next piece of the run; false at its end.  The same for all threads that call it with the same run.
 __device__ __forceinline__ bool paged_next(const PagedPlan &a, PagedRun &run, PagedPiece &w) {
     if (run.u >= run.u1) return false;
-    PagedShape s;
-    for (;;) {
-        w.r = paged_row(a.p, run.row, nullptr);
-        s = paged_shape(a, w.r);
-        if (run.u < run.row_first + s.units) break;
-        run.row_first += s.units;
-        if (++run.row >= a.p.rows) return false;
+    if (run.k == run.k_tiles) {   // the next item: of the head, of the row, of the next row that has any
+        run.k = 0;
+        if (++run.q_tile == run.q_tiles) {
+            run.q_tile = 0;
+            if (++run.head == a.p.kv_heads) {
+                run.head = 0;
+                do {
+                    if (++run.row >= a.p.rows) return false;
+                    run.r = paged_row(a.p, run.row, nullptr);
+                    const PagedShape s = paged_shape(a, run.r);
+                    run.q_tiles = s.q_tiles;
+                    run.base = s.base;
+                } while (run.q_tiles == 0);
+            }
+        }
+        run.k_tiles = paged_keys(a, run.base, run.q_tile);
     }
-    long long in = run.u - run.row_first;
-    w.row = run.row;
-    w.head = (int)(in / s.per);
-    in -= w.head * s.per;
-    int lo = 0, hi = s.q_tiles - 1;   // the tile that unit `in` is of
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (paged_units(a, s.base, mid) <= in) lo = mid;
-        else hi = mid - 1;
-    }
-    const long long first = paged_units(a, s.base, lo);
-    w.q_tile = lo;
-    w.k_tiles = (int)(paged_units(a, s.base, lo + 1) - first);
-    w.k0 = (int)(in - first);
+    w.row = run.row; w.head = run.head; w.q_tile = run.q_tile; w.r = run.r; w.k_tiles = run.k_tiles;
+    w.k0 = run.k;
     w.k1 = (int)min((long long)w.k_tiles, w.k0 + (run.u1 - run.u));
+    run.k = w.k1;
     run.u += w.k1 - w.k0;
     return true;
 }
@@ -234,6 +255,7 @@ static inline void paged_deal(PagedAttnArgs &a, int ctas, int tile_rows, int key
     a.ctas = ctas; a.tile_rows = tile_rows;
     a.plan.tq_shift = paged_log2(tile_rows / a.plan.group);
     a.plan.key_shift = key_shift;
+    a.plan.per_group = (65536 + a.plan.group - 1) / a.plan.group;
     a.plan.whole = !workspace || bytes < paged_piece_bytes(ctas, tile_rows, hd);
     a.plan.least = a.plan.whole ? 1 : least;
     a.acc = (float *)workspace;
@@ -253,7 +275,7 @@ __device__ __forceinline__ void paged_cut(const PagedAttnArgs &a, const PagedRun
 template <int HD>
 __device__ __forceinline__ void paged_again(const PagedAttnArgs &a, const PagedPiece &w, const PagedSpan &sp, int r, int lane, bool all, size_t slot) {
     constexpr int N = HD / 32;
-    const int tok = r / a.plan.group, head = w.head * a.plan.group + r % a.plan.group;
+    const int tok = paged_token(a.plan, r), head = w.head * a.plan.group + r - tok * a.plan.group;
     const int to = min(sp.hi - 1, sp.base + sp.t0 + tok);
     const __nv_bfloat16 *q = (const __nv_bfloat16 *)a.q + (size_t)(w.r.first + sp.t0 + tok) * a.q_stride + (size_t)head * HD;
     float qv[N], acc[N] = {}, top = -INFINITY, sum = 0.f;

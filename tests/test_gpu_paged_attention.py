@@ -56,6 +56,11 @@ def test_rows_without_tokens_and_queries_without_keys(dtype):
     got = b.run(pkg())
     assert pkg().device_status() == 0
     assert (got[:5] == 0).all() and torch.isfinite(got).all() and (got[5:] != 0).any()
+    wide = Batch([300, 70], [300, 70], 8, 2, 64, 16, dtype, seed=1)   # many tiles of queries without keys, one after the other
+    wide.lens_dev.copy_(torch.tensor([0, 4], dtype=torch.int32))
+    for bound in (300, 1):
+        out = wide.run(pkg(), max_new=bound)
+        assert pkg().device_status() == 0 and (out[:366] == 0).all() and (out[366:] != 0).any()
     c = Batch([40], [3], 8, 2, 64, 16, dtype)
     c.q, c.k_pages, c.v_pages, c.table = b.q[5:].contiguous(), b.k_pages, b.v_pages, b.table
     c.lens_dev.fill_(3)

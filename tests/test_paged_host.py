@@ -169,7 +169,7 @@ def test_every_unit_of_work_is_done_once_and_cut_items_are_finished(whole):
         done, slots, merged = {}, {}, []
         for c in range(most_ctas):
             u, last = begin[c], None
-            while u < begin[c + 1]:
+            if u < begin[c + 1]:   # where the run begins
                 before, row = 0, 0
                 while u >= before + per[row] * kv_heads:
                     before += per[row] * kv_heads
@@ -179,24 +179,35 @@ def test_every_unit_of_work_is_done_once_and_cut_items_are_finished(whole):
                 while lo < hi:
                     mid = (lo + hi + 1) // 2
                     lo, hi = (mid, hi) if units(lens[row] - new[row], mid, ts, ks, whole) <= at else (lo, mid - 1)
-                first, kt = units(lens[row] - new[row], lo, ts, ks, whole), units(lens[row] - new[row], lo + 1, ts, ks, whole) - units(lens[row] - new[row], lo, ts, ks, whole)
-                k0 = at - first
-                k1 = min(kt, k0 + begin[c + 1] - u)
+                k = at - units(lens[row] - new[row], lo, ts, ks, whole)
+                keys = lambda: 1 if whole else (lens[row] - new[row] + ((lo + 1) << ts) + (1 << ks) - 1) >> ks  # noqa: E731
+                kt = keys()
+            while u < begin[c + 1]:
+                if k == kt:   # the next item
+                    k, lo = 0, lo + 1
+                    if lo == tiles[row]:
+                        lo, head = 0, head + 1
+                        if head == kv_heads:
+                            head, row = 0, row + 1
+                            while tiles[row] == 0:
+                                row += 1
+                    kt = keys()
+                k0, k1 = k, min(kt, k + begin[c + 1] - u)
                 assert head < kv_heads and lo << ts < new[row] and 0 <= k0 < k1 <= kt
-                for k in range(k0, k1):
-                    assert done.setdefault((row, head, lo, k), c) == c
+                for i in range(k0, k1):
+                    assert done.setdefault((row, head, lo, i), c) == c
                 if (k0, k1) != (0, kt):
                     assert not whole
                     slot = 2 * c + (k0 == 0)
                     assert slot not in slots
                     slots[slot] = (row, head, lo)
                 u += k1 - k0
+                k = k1
                 last = (row, head, lo, k0, k1, kt, u + kt - k1)
             if last and last[3] == 0 and last[4] < last[5]:
                 assert c < most_ctas - 1
-                to = c + 1
-                while to + 1 < ctas and begin[to + 1] < last[6]:
-                    to += 1
+                to = min(ctas - 1, (last[6] * ctas - 1) // total)
+                assert begin[to] < last[6] <= begin[to + 1]
                 merged.append((last[:3], [2 * j + (j == c) for j in range(c, to + 1)]))
         assert len(done) == total
         assert sorted(s for _, m in merged for s in m) == sorted(slots)
