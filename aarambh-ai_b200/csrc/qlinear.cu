@@ -87,7 +87,7 @@ int qlinear_generic(const ab2_qweight *w, const void *x, int M, ab2_dtype dtype,
 
 thread_local bool g_pdl_launch = false;
 
-// Per-device status word written by kernels whose bounded waits ran out.
+// Per-device status word written by kernels whose bounded waits ran out, or that found a table or a length out of bounds.
 static int *g_status_word[64] = {nullptr};
 static int g_sm_count[64] = {0};
 
@@ -96,9 +96,21 @@ int device_status_word(int **out) {
     AB2_CUDA(cudaGetDevice(&dev));
     AB2_REQUIRE(dev >= 0 && dev < 64, AB2_ERR_BAD_ARG, "device index %d out of range", dev);
     if (!g_status_word[dev]) {
-        AB2_CUDA(cudaMalloc((void **)&g_status_word[dev], sizeof(int)));
-        AB2_CUDA(cudaMemset(g_status_word[dev], 0, sizeof(int)));
+        // A first call may be one that is recorded: neither the allocation nor a stream of the word's own belongs to the recording.
+        int *word = nullptr;
+        cudaStream_t own = nullptr;
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        AB2_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        cudaError_t e = cudaMalloc((void **)&word, sizeof(int));
+        if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+        if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof(int), own);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+        if (own) cudaStreamDestroy(own);
+        AB2_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        if (e != cudaSuccess && word) cudaFree(word);
+        AB2_CUDA(e);
         AB2_CUDA(cudaDeviceGetAttribute(&g_sm_count[dev], cudaDevAttrMultiProcessorCount, dev));
+        g_status_word[dev] = word;
     }
     *out = g_status_word[dev];
     return AB2_OK;
@@ -465,6 +477,6 @@ AB2_API int ab2_device_status(int *status_host) {
     AB2_CUDA(cudaDeviceSynchronize());
     AB2_CUDA(cudaMemcpy(status_host, word, sizeof(int), cudaMemcpyDeviceToHost));
     AB2_CUDA(cudaMemset(word, 0, sizeof(int)));
-    if (*status_host != 0) ++g_recovery_epoch;
+    if (*status_host == AB2_ERR_TIMEOUT) ++g_recovery_epoch;
     return AB2_OK;
 }

@@ -61,7 +61,8 @@ typedef struct ab2_tp ab2_tp;
 int ab2_version(void);
 const char *ab2_last_error(void);
 /* Synchronises the current device and returns (then clears) its status word:
- * AB2_OK, or AB2_ERR_TIMEOUT when a kernel's bounded wait ran out.  No
+ * AB2_OK, AB2_ERR_TIMEOUT when a kernel's bounded wait ran out, or AB2_ERR_BAD_ARG when a
+ * table, length or start that a call reads on the device (ab2_paged) was out of bounds.  No
  * counterpart in the reference, whose kernels never wait on one another. */
 int ab2_device_status(int *status_host);
 
