@@ -155,6 +155,9 @@ class LayerSpec(C.Structure):
                 ("limit", _f), ("kv_rank", _i), ("head_gate", _i), ("glu", _i), ("routing", _i), ("shared_ff", _i), ("poly", _f * 4)]
 
 
+PAGED_UNCUT = 256   # AB2_PAGED_UNCUT
+
+
 class Paged(C.Structure):
     """ab2_paged."""
     _fields_ = [("k_pages", _p), ("v_pages", _p), ("table", _p), ("lens", _p), ("starts", _p), ("pages", _i), ("page_size", _i),

@@ -65,7 +65,35 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("link of libaarambh_b200.so failed")
+    build_fast(force, verbose)
     return LIB
+
+
+FAST = os.path.join(HERE, "_fast.so")
+
+
+def build_fast(force: bool = False, verbose: bool = False) -> str:
+    """csrc/fast.cpp, the Python module of the serving step's plain calls, against the torch and the Python that run this."""
+    import importlib.util
+    import sysconfig
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise RuntimeError("torch is needed to build _fast.so")
+    torch_dir, source, header = os.path.dirname(spec.origin), os.path.join(CSRC, "fast.cpp"), os.path.join(ROOT, "include", "aarambh_b200.h")
+    if not force and os.path.exists(FAST) and os.path.getmtime(FAST) >= _newest([source, header, os.path.join(torch_dir, "version.py")]):
+        return FAST
+    cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", source, "-o", FAST + ".new", "-I" + os.path.join(ROOT, "include"),
+           "-I" + os.path.join(torch_dir, "include"), "-I" + os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"), "-I" + cuda,
+           "-I" + sysconfig.get_path("include"), "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-L" + HERE, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or res.returncode != 0:
+        sys.stderr.write(" ".join(cmd) + "\n" + res.stdout + res.stderr)
+    if res.returncode != 0:
+        raise RuntimeError("g++ failed for fast.cpp")
+    os.replace(FAST + ".new", FAST)
+    return FAST
 
 
 def build_locked() -> str:

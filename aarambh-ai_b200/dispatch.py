@@ -232,6 +232,13 @@ class MoeExperts:
 
 
 # -- a serving step over a paged cache (``kvcache.PagedKVCache`` keeps the pages) ---------------------
+# Plain calls (contiguous tensors that match) are made by csrc/fast.cpp, which answers None to all others; they are looked at here.  The same
+# kernels either way: where that module does not load (it is built for one Python and one torch) a call takes some 8 us more of host time.
+try:
+    from . import _fast
+except ImportError:
+    _fast = None
+
 
 @dataclass
 class RotaryScaling:
@@ -329,6 +336,10 @@ def rotary_apply(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     """q [tokens, heads, dim] and k [tokens, kv_heads, dim] (or None), each token rotated by its position (``positions`` [tokens],
     int32 or int64); pairs ``half`` (i, i + n) or ``interleaved`` (2i, 2i + 1), n the count of ``frequencies`` (``rotary_frequencies``).
     ``out``: a pair of tensors for the results, which may be q and k."""
+    if out is None and _fast is not None:
+        got = _fast.rotary(q, k, positions, frequencies, layout, magnitude)
+        if got is not None:
+            return got if type(got) is tuple else check(got)
     _on_device(q, k, positions, frequencies)
     q, qs = _heads(q, "q")
     n, h, d = q.shape
@@ -392,6 +403,10 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, 
     """Writes the new tokens' k (rotated at their positions in their rows, as they are without ``frequencies``) and v
     [tokens, kv_heads, dim] to the pages that ``table`` [rows, pages] names; ``lens`` [rows] are the rows' tokens with the new ones,
     ``starts`` [rows + 1] where a row's new tokens begin (None: one a row).  Returns the rotated q [tokens, heads, dim], if any."""
+    if out is None and _fast is not None:
+        got = _fast.append(k_pages, v_pages, k, v, table, lens, starts, q, frequencies, layout, magnitude)
+        if got is not None:
+            return check(got) if type(got) is int else got if got is not True else None
     _on_device(k_pages, v_pages, k, v, table, lens, starts, q, frequencies)
     k, ks = _heads(k, "k")
     v, vs = _heads(v, "v")
@@ -419,14 +434,15 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, 
     return qo
 
 
-_paged_bytes = {}   # head_dim, device -> bytes of a workspace
-
-
 def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float,
                     starts: torch.Tensor | None = None, max_new: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """q [tokens, heads, dim]: each row's new tokens, whose keys and values have been appended, attend to the row's keys up to their
     own; table, lens and starts as in ``paged_append``.  ``max_new`` bounds the new tokens of a row (None: not known); it picks
     kernels, whose results differ by rounding.  Tokens behind the last row are left as ``out`` holds them."""
+    if out is None and _fast is not None:
+        got = _fast.attention(q, k_pages, v_pages, table, lens, scale, starts, max_new)
+        if got is not None:
+            return check(got) if type(got) is int else got
     _on_device(q, k_pages, v_pages, table, lens, starts)
     q, qs = _heads(q, "q")
     n, h, d = q.shape
@@ -443,12 +459,10 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         out, os = _result(out, q, "out")
     if max_new is None:
         max_new = 1 if starts is None else max(n, 1)
-    # rows that cannot be longer than 256 tokens are not worth cutting: 1 x 256 tokens take PCSMALL
-    size = _paged_bytes.get((d, q.get_device()), -1) if c.table_width * c.page_size > 256 else 0
-    if size < 0:
-        n = C.c_size_t()
-        check(lib.ab2_paged_workspace(d, C.byref(n)))
-        size = _paged_bytes[(d, q.get_device())] = n.value
+    size = C.c_size_t()
+    if c.table_width * c.page_size > _lib.PAGED_UNCUT:
+        check(lib.ab2_paged_workspace(d, C.byref(size)))
+    size = size.value
     work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     check(lib.ab2_paged_attention(C.byref(c), q.data_ptr(), qs, h, out.data_ptr(), os, max_new, scale, work.data_ptr() if size else None, size,
                                   dtype_code(q.dtype), stream_ptr()))
@@ -474,6 +488,10 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, len
     by the repetition where it is positive, else multiplied, then lowered by presence + frequency c.  Then ``bias_values`` [rows, m] f32 are
     added at ``bias_ids`` [rows, m] int32 (of an id named twice the last counts), and tokens whose bit in ``allowed``
     [rows, ceil(vocab / 32)] int32 (``allowed_words``) is 0 become -inf.  ``out`` may be the logits."""
+    if out is None and _fast is not None:
+        got = _fast.logits(logits, history, lengths, rules, bias_ids, bias_values, allowed)
+        if got is not None:
+            return check(got) if type(got) is int else got
     _on_device(logits, history, lengths, rules, bias_ids, bias_values, allowed, out)
     if logits.dim() != 2:
         raise _lib.Ab2Error(-1, f"logits must be [rows, vocab], got {list(logits.shape)}")

@@ -392,6 +392,7 @@ int ab2_paged_append(const ab2_paged *cache, const void *k_dev, long long k_stri
  * sight may hold anything.  max_new (at least the most new tokens of a row) picks kernels; rows that have more are
  * answered all the same.  workspace_dev
  * (ab2_paged_workspace bytes, 16-byte aligned, nothing in it is kept between calls) lets long rows be cut between CTAs; NULL: they are not. */
+#define AB2_PAGED_UNCUT 256 /* tokens of a row up to which it is not worth a workspace: cutting takes a second launch */
 int ab2_paged_workspace(int head_dim, size_t *bytes);
 int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long long q_stride, int heads, void *out_dev, long long out_stride, int max_new, float scale,
                         void *workspace_dev, size_t workspace_bytes, ab2_dtype dtype, ab2_stream stream);
