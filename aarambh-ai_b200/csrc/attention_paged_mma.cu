@@ -146,25 +146,25 @@ __global__ void __launch_bounds__(32 * PM_WARPS, 2) paged_mma_kernel(const __gri
             const uint32_t at = smem_at(ring + stage * S::BLOCK);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             // ---- scores: rows of K are keys
-            float s[NT][4];
+            float s[NT][4], s2[NT][4];   // two sums, so that a product waits for every other one only
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
+                for (int e = 0; e < 4; ++e) s[t][e] = s2[t][e] = 0.f;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 uint32_t f[4];
                 const int r = lane & 15, ch = 2 * k + (lane >> 4);
                 ldsm4(f, at + r * (HD * 2) + ((ch ^ (r & 7)) << 4));
 #pragma unroll
-                for (int t = 0; t < NT; ++t) mma_bf16(s[t], f, q[t][k][0], q[t][k][1]);
+                for (int t = 0; t < NT; ++t) mma_bf16(k & 1 ? s2[t] : s[t], f, q[t][k][0], q[t][k][1]);
             }
             // ---- weights
             uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[t][e] *= a.sl;
+                for (int e = 0; e < 4; ++e) s[t][e] = (s[t][e] + s2[t][e]) * a.sl;
                 if (key + PM_KEYS > sure)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)

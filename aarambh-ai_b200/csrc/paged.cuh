@@ -130,8 +130,12 @@ struct PagedRun {
     PagedRow r;            // that row
     int q_tiles, base;
 };
+// a / b of numbers that are not negative: in 32 bits, a fifth of the time, where they fit.
+__device__ __forceinline__ long long paged_div(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
 // Where the run of CTA c begins.
-__device__ __forceinline__ long long paged_begin(const PagedRun &run, int c) { return run.total * min(c, run.ctas) / run.ctas; }
+__device__ __forceinline__ long long paged_begin(const PagedRun &run, int c) { return paged_div(run.total * min(c, run.ctas), run.ctas); }
 __device__ __forceinline__ int paged_keys(const PagedPlan &a, int base, int q_tile) {   // units of a tile of queries
     return a.whole ? 1 : (int)(((long long)base + ((long long)(q_tile + 1) << a.tq_shift) + (1 << a.key_shift) - 1) >> a.key_shift);
 }
@@ -146,7 +150,7 @@ template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const Paged
         if (r0 == 0) { prefix = at; units = here; }
         run.total += n;
     }
-    run.ctas = (int)max(1ll, min((long long)ctas, run.total / a.least));
+    run.ctas = (int)max(1ll, min((long long)ctas, paged_div(run.total, a.least)));
     run.u = paged_begin(run, c);
     run.u1 = paged_begin(run, c + 1);
     if (run.u >= run.u1) return run;
@@ -164,7 +168,7 @@ template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const Paged
         if (units > 0 && run.u >= prefix && run.u < prefix + units) {
             const PagedShape s = paged_shape(a, paged_row(a.p, r0 + (int)(threadIdx.x % THREADS), nullptr));
             const long long in = run.u - prefix;
-            const int head = (int)(in / s.per);
+            const int head = (int)paged_div(in, s.per);
             found[0] = make_int2(r0 + (int)(threadIdx.x % THREADS), head);
             const long long y = in - head * s.per;
             int lo = 0, hi = s.q_tiles - 1;   // the tile that unit y of the head is of
@@ -267,7 +271,7 @@ __device__ __forceinline__ void paged_uncut(const PagedAttnArgs &a, int c) { if 
 __device__ __forceinline__ void paged_cut(const PagedAttnArgs &a, const PagedRun &run, const PagedPiece &w, const PagedSpan &sp, int c) {
     if (w.k0 > 0 || w.k1 == w.k_tiles) return;
     const long long end = run.u + (w.k_tiles - w.k1);   // the unit behind the item: the last run that begins before it ends it
-    a.cut[c] = make_int4(w.r.first + sp.t0, sp.ntok, w.head, (int)min((long long)run.ctas - 1, (end * run.ctas - 1) / run.total));
+    a.cut[c] = make_int4(w.r.first + sp.t0, sp.ntok, w.head, (int)min((long long)run.ctas - 1, paged_div(end * run.ctas - 1, run.total)));
 }
 
 // Row r of a piece of bf16 over the keys [lo, to] of it that it sees, by one warp, a lane every 32nd dimension: where a product with hidden values
