@@ -8,11 +8,19 @@
 //   warps 1, 2   MMA issue for tile 0 and tile 1
 //   warps 4-7    softmax of tile 0, a thread per row;   warps 8-11   of tile 1
 // Tiles are of 80 keys because scores (80 columns) and weights (40) of two tiles of rows then fit beside their sums of 128 dimensions in the 512
-// columns of tensor memory: the scores of the next tile are made while the weights of this one are, and a softmax warp never waits for its own
-// products.  (With 128 keys the weights lay over the scores, and scores - softmax - sums was a chain: 0.98 ms where this takes PCTIME, 4096 tokens
-// behind 12288, 32 / 8 heads of 128.)  The weights enter rounded to bf16, half a step (2^-8) each and independent, which the sum over the keys
-// averages; their sum is that of the f32 weights.  Scores, maxima, sums and O are f32.  The weights are relative to a maximum per row that moves only
-// when a score exceeds it by 2^8; then O is rescaled in tensor memory.
+// columns of tensor memory: the scores of the next tile are made while the weights of this one are.  An MMA of 80 keys reads shared memory as fast as
+// it goes (419 clocks for 128 rows, 512 for 128 keys: 1.3 of the time a key; with the sums 716 a tile of 80, 1.12).
+// The weights enter rounded to bf16, half a step (2^-8) each and independent, which the sum over the keys averages; their sum is that of the f32
+// weights.  Scores, maxima, sums and O are f32.  The weights are relative to a maximum per row that moves only when a score exceeds it by 2^8; then O is
+// rescaled in tensor memory.
+//
+// 4096 tokens behind 12288, 32 / 8 heads of 128: 0.92 ms, 1.05 PFLOP/s, 0.63 of cuBLAS in a burst and 0.75 of it sustained; 2048 behind 2048 126 us;
+// six rows of 1 to 512 tokens behind up to 5000 128 us.  Bound by the two softmax warps of a scheduler: of the 2300 clocks of a tile of 80 keys they
+// need 1250 for the exponentials, which both make at the same time (2 x 128 x 80 at 16 a clock are 1280), and the rest for scores from tensor memory,
+// the maximum, and waits on one another of some 150 clocks each; the products take 1432.  Measured and not kept: tiles of 128 keys with the
+// weights over the scores (a chain of scores, softmax and sums; 0.98 ms), of 64 with two places for weights (1.17), a
+// warp's loads of the next scores between its exponentials (1.17), the tiles' exponentials in turns by a barrier (0.98), polynomials for some of
+// them (an eighth: no change; more: slower), weights handed over in four parts (1.11).
 //
 // An MMA multiplies a hidden value by a weight of 0, so an Inf or a NaN there would reach rows that do not see it.  Rows of a page behind the
 // sequence's end are cleared in shared memory; a row whose sums come out as Inf or NaN (a later token's value may hold them) is computed

@@ -4,8 +4,10 @@
 //
 // Pairs are (i, i + n) with the half layout and (2i, 2i + 1) with the interleaved one, n = rot / 2 of them; the dimensions from rot on pass
 // as they are.  One pass over q and k (and v, which is copied into its pages): bound by HBM from some hundred tokens on, by the launch
-// below.  A warp has one token (or a part of its heads where tokens are few): its lanes turn the token's angles once, into shared memory,
-// and then take items (head, P pairs) of it; where a head's chunks divide 32 a lane keeps its pairs from head to head.
+// below: 8192 tokens of 32 / 8 heads of 128 in bf16 31 us, 5.3 TB/s (0.82 of a copy's); 5891 tokens of 16 / 4 appended 19 us; 8 tokens 4 us.
+// A warp has one token (or a part of its heads where tokens are few): its lanes turn the token's angles once, into shared memory, and then take
+// (head, P pairs) of q, k and v one tensor after the other; where a head's chunks divide 32 a lane keeps its pairs from head to head.  Angles made by every
+// lane for itself, and elements of 16 bits held as such, took 35 and 42 us.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -278,7 +280,7 @@ int paged_check(const ab2_paged *c, ab2_dtype dtype) {
     AB2_REQUIRE(c->pages > 0 && c->kv_heads > 0 && c->rows > 0 && c->tokens >= 0 && c->table_width > 0, AB2_ERR_BAD_SHAPE,
                 "paged cache of %d pages, %d heads, %d rows of %d pages, %d tokens", c->pages, c->kv_heads, c->rows, c->table_width, c->tokens);
     AB2_REQUIRE(c->table_stride >= c->table_width, AB2_ERR_BAD_SHAPE, "table rows of %d pages lie %lld apart", c->table_width, c->table_stride);
-    AB2_REQUIRE((long long)c->table_width * c->page_size < (1ll << 31) && (long long)c->kv_heads * c->page_size < (1ll << 31) && (long long)c->kv_heads * c->pages < (1ll << 31), AB2_ERR_BAD_SHAPE, "rows of 2^31 tokens or more");
+    AB2_REQUIRE((long long)c->table_width * c->page_size <= (1ll << 30) && (long long)c->kv_heads * c->page_size < (1ll << 31) && (long long)c->kv_heads * c->pages < (1ll << 31), AB2_ERR_BAD_SHAPE, "rows of more than 2^30 tokens, or 2^31 pages and heads");
     AB2_REQUIRE(c->starts || c->tokens == c->rows, AB2_ERR_BAD_SHAPE, "%d tokens for %d rows of one token each", c->tokens, c->rows);
     AB2_REQUIRE((((uintptr_t)c->k_pages | (uintptr_t)c->v_pages) & 15) == 0, AB2_ERR_BAD_ALIGN, "pages must be 16-byte aligned");
     return AB2_OK;

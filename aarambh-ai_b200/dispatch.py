@@ -438,7 +438,7 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     starts: torch.Tensor | None = None, max_new: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """q [tokens, heads, dim]: each row's new tokens, whose keys and values have been appended, attend to the row's keys up to their
     own; table, lens and starts as in ``paged_append``.  ``max_new`` bounds the new tokens of a row (None: not known); it picks
-    kernels, whose results differ by rounding.  Tokens behind the last row are left as ``out`` holds them."""
+    kernels, whose results differ by rounding.  Tokens behind the last row are left as ``out`` (not q) holds them."""
     if out is None and _fast is not None:
         got = _fast.attention(q, k_pages, v_pages, table, lens, scale, starts, max_new)
         if got is not None:
@@ -457,8 +457,7 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         out, os = _fresh(q), h * d
     else:
         out, os = _result(out, q, "out")
-    if max_new is None:
-        max_new = 1 if starts is None else max(n, 1)
+    max_new = (1 if starts is None else max(n, 1)) if max_new is None else min(max_new, 2 ** 31 - 1)
     size = C.c_size_t()
     if c.table_width * c.page_size > _lib.PAGED_UNCUT:
         check(lib.ab2_paged_workspace(d, C.byref(size)))

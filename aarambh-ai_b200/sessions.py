@@ -57,6 +57,8 @@ class LogitRules:
                 if may.numel() and (int(may.min()) < 0 or int(may.max()) >= vocab):
                     raise _lib.Ab2Error(-1, "an allowed token outside the vocabulary")
                 may = torch.zeros(vocab, dtype=torch.bool, device=logits.device).index_fill_(0, may.long().view(-1), True)
+            if not bool(may.any()):
+                raise _lib.Ab2Error(-7, "the session's rules allow no token")
             args["allowed"] = allowed_words(may.view(1, vocab))
         return adjust_logits(logits, **args) if args else logits
 

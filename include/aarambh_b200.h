@@ -376,7 +376,7 @@ int ab2_rotary_apply(const void *q_dev, long long q_stride, int heads, const voi
  * behind the last row are left as they are.  Table, lens and starts are device memory, read when the kernels run: a recorded call
  * serves what they hold then.  Values out of bounds (a page outside the pool, a row longer than its table, starts that fall or pass
  * `tokens`) are brought within them, nothing outside the buffers is touched, and ab2_device_status reports AB2_ERR_BAD_ARG; the
- * outputs are void then.  Rows that write a page must not share it. */
+ * outputs are void then.  A row's table has room for 2^30 tokens at most.  Rows that write a page must not share it. */
 typedef struct {
     void *k_pages, *v_pages;
     const int *table, *lens, *starts;
@@ -384,11 +384,13 @@ typedef struct {
     long long table_stride;   /* entries from a row of the table to the next, table_width or more */
 } ab2_paged;
 /* Writes k (rotated at its position in the row; rot_dims 0: as it is) and v of the new tokens to their pages, and with heads > 0 the
- * rotated q to q_out_dev, in one launch. */
+ * rotated q to q_out_dev, in one launch; q_out_dev may be q_dev.  A token without a place (a row with more new tokens than tokens, a page
+ * outside the pool) is not written, and reported as above. */
 int ab2_paged_append(const ab2_paged *cache, const void *k_dev, long long k_stride, const void *v_dev, long long v_stride, const void *q_dev, long long q_stride,
                      int heads, void *q_out_dev, long long q_out_stride, const double *frequencies_dev, int rot_dims, int layout, float magnitude, ab2_dtype dtype, ab2_stream stream);
 /* Attention of the new tokens, whose keys and values have been appended: a token sees its row's keys up to its own position, query head
- * j reads KV head j / (heads / kv_heads), up to 32 query heads for one KV head; a token that sees no key answers zeros.  Keys and values out of
+ * j reads KV head j / (heads / kv_heads), up to 32 query heads for one KV head; a token that sees no key answers zeros.  out_dev
+ * must not overlap q_dev.  Keys and values out of
  * sight may hold anything.  max_new (at least the most new tokens of a row) picks kernels; rows that have more are
  * answered all the same.  workspace_dev
  * (ab2_paged_workspace bytes, 16-byte aligned, nothing in it is kept between calls) lets long rows be cut between CTAs; NULL: they are not. */

@@ -139,7 +139,7 @@ def test_without_a_workspace_and_with_any_bound_on_new_tokens(dtype):
     for new, lens in (([1, 1], [900, 40]), ([30, 1], [2000, 70]), ([200, 3], [1200, 333])):
         b = Batch(lens, new, 8, 2, 128, 32, dtype, seed=5)
         ref, tol = b.expected()
-        for bound in (1, max(new), 10 ** 6):
+        for bound in (1, max(new), 10 ** 6, 2 ** 40):
             held(b.run(p, max_new=bound), ref, tol)
         c, keep = p.dispatch._paged(b.k_pages, b.v_pages, b.table, b.lens_dev, b.starts, b.T)
         out = torch.empty_like(b.q)
@@ -252,7 +252,7 @@ def test_refusals():
            dict(k_pages=b.k_pages[:, :, :8], v_pages=b.v_pages[:, :, :8]), dict(v_pages=b.v_pages[:1]), dict(lens=b.lens_dev.long()), dict(lens=b.lens_dev[:1]),
            dict(starts=b.starts[:2]), dict(table=b.table.long()), dict(starts=None), dict(max_new=0), dict(out=b.q.float()), dict(out=b.q[:1]),
            dict(k_pages=b.k_pages.transpose(1, 2), v_pages=b.v_pages.transpose(1, 2)), dict(q=b.q.half(), k_pages=b.k_pages.half(), v_pages=b.v_pages.half()),
-           dict(q=b.q.repeat(1, 9, 1))]
+           dict(q=b.q.repeat(1, 9, 1)), dict(out=b.q)]
     for change in bad:
         with pytest.raises(p.Ab2Error):
             p.dispatch.attention_paged(**{**ok, **change})

@@ -138,3 +138,7 @@ def test_sessions_with_rules():
         R(repetition=0.0)
     with pytest.raises(p.Ab2Error):
         run(R(allowed=lambda ids: [10 ** 6]))
+    for nothing in ([], [False] * SMALL["vocab"]):
+        with pytest.raises(p.Ab2Error):
+            run(R(allowed=lambda ids: nothing))
+    assert run(R(allowed=lambda ids: None))[0] == plain

@@ -88,10 +88,10 @@ def test_entry_points_refuse_before_any_device_work():
     assert attention(None) == -7
     for kw, code in ((dict(k_pages=None), -7), (dict(v_pages=None), -7), (dict(table=None), -7), (dict(lens=None), -7), (dict(page_size=24), -8), (dict(page_size=8), -8), (dict(page_size=512), -8),
                      (dict(head_dim=96), -8), (dict(pages=0), -1), (dict(rows=0), -1), (dict(tokens=-1), -1), (dict(table_width=0), -1), (dict(table_stride=2), -1), (dict(kv_heads=0), -1),
-                     (dict(starts=None), -1), (dict(k_pages=(1 << 20) + 8), -2), (dict(table_width=1 << 28, table_stride=1 << 28), -1)):
+                     (dict(starts=None), -1), (dict(k_pages=(1 << 20) + 8), -2), (dict(table_width=(1 << 26) + 1, table_stride=1 << 28), -1)):
         assert attention(paged(**kw)) == code, kw
         assert lib.ab2_paged_append(C.byref(paged(**kw)), 1 << 25, 128, 1 << 26, 128, None, 0, 0, None, 0, None, 0, 0, 1.0, 2, None) == code, kw
-    for kw, code in ((dict(q=None), -7), (dict(out=None), -7), (dict(heads=7), -1), (dict(heads=0), -1), (dict(heads=66), -1), (dict(max_new=0), -1), (dict(qs=511), -1), (dict(os=100), -1),
+    for kw, code in ((dict(q=None), -7), (dict(out=None), -7), (dict(heads=7), -1), (dict(heads=0), -1), (dict(heads=66), -1), (dict(out=1 << 25), -7), (dict(max_new=0), -1), (dict(qs=511), -1), (dict(os=100), -1),
                      (dict(qs=513), -2), (dict(q=(1 << 25) + 2), -2), (dict(dtype=1), -3), (dict(dtype=9), -3), (dict(work=(1 << 25) + 8), -2)):
         assert attention(paged(), **kw) == code, kw
     assert attention(paged(tokens=0)) == 0
