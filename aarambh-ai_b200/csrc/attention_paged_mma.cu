@@ -11,8 +11,8 @@
 // Weights enter as two bf16 terms, the rounded weight and what rounding left: the tensor pipe has time for both, and no rounding but the
 // output's is left.  A row's maximum moves only when a score exceeds it by 2^8.
 //
-// 48 rows of up to 8192 tokens, 32 / 8 heads of 128 (1.02 GB): 170 us, 0.92 of a copy's rate; 2 x 100000 129 us (0.88); 1 x 700 12.6 us, of which the launch,
-// lengths and first copies are 4, four blocks of 16 keys one after the other 2, the merge's launch and its loads 4.  On CUDA cores: 672 us and 35.
+// 48 rows of up to 8192 tokens, 32 / 8 heads of 128 (1.02 GB): 172 us with the merge, 0.91 of a copy's rate (on CUDA cores 672); 2 x 100000 127 us
+// (0.89).  1 x 700: 12.7 us, by one kernel of 8 and a merge of 4.3 that reads little: latency.
 #include <algorithm>
 
 #include "paged.cuh"

@@ -16,11 +16,12 @@
 //
 // 4096 tokens behind 12288, 32 / 8 heads of 128: 0.92 ms, 1.05 PFLOP/s, 0.63 of cuBLAS in a burst and 0.75 of it sustained; 2048 behind 2048 126 us;
 // six rows of 1 to 512 tokens behind up to 5000 128 us.  Bound by the two softmax warps of a scheduler: of the 2300 clocks of a tile of 80 keys they
-// need 1250 for the exponentials, which both make at the same time (2 x 128 x 80 at 16 a clock are 1280), and the rest for scores from tensor memory,
-// the maximum, and waits on one another of some 150 clocks each; the products take 1432.  Measured and not kept: tiles of 128 keys with the
-// weights over the scores (a chain of scores, softmax and sums; 0.98 ms), of 64 with two places for weights (1.17), a
-// warp's loads of the next scores between its exponentials (1.17), the tiles' exponentials in turns by a barrier (0.98), polynomials for some of
-// them (an eighth: no change; more: slower), weights handed over in four parts (1.11).
+// need 1250 for the exponentials (read by clocks in the kernel; both tiles' are 2 x 128 x 80, at 16 a clock 1280), and the rest for scores from
+// tensor memory, the maximum, and the waits for scores and for the last tile's products, some 150 clocks each; the products take 1432.
+//
+// Measured and not kept, each against the kernel of its day: the tiles' exponentials in turns by a barrier 0.98 ms for 0.91; polynomials for a quarter of
+// them 0.96 for 0.91.  Forms before this one: tiles of 128 keys with the weights over the scores (a chain of scores, softmax and sums) 0.98 to 1.02;
+// an MMA warp a tile there, weights handed over in two or four parts, 1.08 and 1.11; tiles of 64 with two places for weights 1.17, with registers spilled.
 //
 // An MMA multiplies a hidden value by a weight of 0, so an Inf or a NaN there would reach rows that do not see it.  Rows of a page behind the
 // sequence's end are cleared in shared memory; a row whose sums come out as Inf or NaN (a later token's value may hold them) is computed

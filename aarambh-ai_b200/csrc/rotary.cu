@@ -6,8 +6,8 @@
 // as they are.  One pass over q and k (and v, which is copied into its pages): bound by HBM from some hundred tokens on, by the launch
 // below: 8192 tokens of 32 / 8 heads of 128 in bf16 31 us, 5.3 TB/s (0.82 of a copy's); 5891 tokens of 16 / 4 appended 19 us; 8 tokens 4 us.
 // A warp has one token (or a part of its heads where tokens are few): its lanes turn the token's angles once, into shared memory, and then take
-// (head, P pairs) of q, k and v one tensor after the other; where a head's chunks divide 32 a lane keeps its pairs from head to head.  Angles made by every
-// lane for itself, and elements of 16 bits held as such, took 35 and 42 us.
+// (head, P pairs) of q, k and v one tensor after the other; where a head's chunks divide 32 a lane keeps its pairs from head to head.  The first
+// form, whose lanes made every angle for themselves, took 35 us; this one with elements of 16 bits held as such, not in words, 39.
 #include <algorithm>
 
 #include "paged.cuh"
