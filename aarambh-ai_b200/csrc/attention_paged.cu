@@ -43,8 +43,9 @@ __device__ __forceinline__ void cp16(void *dst, const void *src, bool in) {
 }
 __device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 template <int HD, int QR>
-__global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(PA_THREADS, HD == 64 ? 4 : 2) paged_simt_kernel(const __grid_constant__ PagedAttnArgs a) {
     using S = SimtShape<HD, QR>;
+    pdl_wait();
     constexpr int TX = S::TX, RPT = S::RPT, KPT = S::KPT, DPT = S::DPT, KROW = S::KROW, CH = 4;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ long long warp_sums[PA_THREADS / 32];
@@ -99,11 +100,11 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
                 asm volatile("cp.async.wait_group 0;\n" ::: "memory");
             }
             __syncthreads();
-            float s[RPT][KPT];
+            float4 s4[RPT][KPT];   // a score as four sums: shorter chains, for time and for rounding
 #pragma unroll
             for (int i = 0; i < RPT; ++i)
 #pragma unroll
-                for (int j = 0; j < KPT; ++j) s[i][j] = 0.f;
+                for (int j = 0; j < KPT; ++j) s4[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
             for (int d = 0; d < HD; d += 4) {
                 float4 qv[RPT], kv[KPT];
@@ -114,31 +115,39 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
 #pragma unroll
                 for (int i = 0; i < RPT; ++i)
 #pragma unroll
-                    for (int j = 0; j < KPT; ++j) s[i][j] = fmaf(qv[i].x, kv[j].x, fmaf(qv[i].y, kv[j].y, fmaf(qv[i].z, kv[j].z, fmaf(qv[i].w, kv[j].w, s[i][j]))));
+                    for (int j = 0; j < KPT; ++j) {
+                        s4[i][j].x = fmaf(qv[i].x, kv[j].x, s4[i][j].x); s4[i][j].y = fmaf(qv[i].y, kv[j].y, s4[i][j].y);
+                        s4[i][j].z = fmaf(qv[i].z, kv[j].z, s4[i][j].z); s4[i][j].w = fmaf(qv[i].w, kv[j].w, s4[i][j].w);
+                    }
             }
+            // the sums of this tile's values alone, joined to the others' at its end: one chain over all keys would round once a key and not once a tile
+            float s[RPT][KPT], keep[RPT], here[RPT][DPT];
 #pragma unroll
             for (int i = 0; i < RPT; ++i) {
                 float best = top[i];
 #pragma unroll
                 for (int j = 0; j < KPT; ++j) {
                     const int key = key0 + tx + TX * j;
+                    s[i][j] = (s4[i][j].x + s4[i][j].y) + (s4[i][j].z + s4[i][j].w);
                     if (key > lim[i] || key >= hi) s[i][j] = -INFINITY;   // out of sight, whatever it holds
                     best = fmaxf(best, s[i][j]);
                 }
 #pragma unroll
                 for (int m = TX / 2; m > 0; m >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, m));
-                const float m = best == -INFINITY ? 0.f : best, keep = exp2f(top[i] - m);
+                const float m = best == -INFINITY ? 0.f : best;
+                keep[i] = exp2f(top[i] - m);
                 top[i] = best;
-                sum[i] *= keep;
+                float weights = 0.f;
 #pragma unroll
-                for (int d = 0; d < DPT; ++d) o[i][d] *= keep;
+                for (int d = 0; d < DPT; ++d) here[i][d] = 0.f;
 #pragma unroll
                 for (int j = 0; j < KPT; ++j) {
                     const int key = key0 + tx + TX * j;
                     const float e = key > lim[i] || key >= hi ? 0.f : exp2f(s[i][j] - m);
-                    sum[i] += e;
+                    weights += e;
                     ps[(ty * RPT + i) * (PA_KEYS + 1) + tx + TX * j] = e;
                 }
+                sum[i] = fmaf(sum[i], keep[i], weights);
             }
             __syncwarp();  // a row's weights come from lanes of one warp
             // keys that no row of the thread sees may hold anything: their weight is 0, and 0 times Inf is not
@@ -156,13 +165,17 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
 #pragma unroll
                     for (int i = 0; i < RPT; ++i) {
                         if (RPT > 1 && key0 + j > lim[i]) continue;
-                        o[i][d] = fmaf(e[i], v.x, o[i][d]);
-                        o[i][d + 1] = fmaf(e[i], v.y, o[i][d + 1]);
-                        o[i][d + 2] = fmaf(e[i], v.z, o[i][d + 2]);
-                        o[i][d + 3] = fmaf(e[i], v.w, o[i][d + 3]);
+                        here[i][d] = fmaf(e[i], v.x, here[i][d]);
+                        here[i][d + 1] = fmaf(e[i], v.y, here[i][d + 1]);
+                        here[i][d + 2] = fmaf(e[i], v.z, here[i][d + 2]);
+                        here[i][d + 3] = fmaf(e[i], v.w, here[i][d + 3]);
                     }
                 }
             }
+#pragma unroll
+            for (int i = 0; i < RPT; ++i)
+#pragma unroll
+                for (int d = 0; d < DPT; ++d) o[i][d] = fmaf(o[i][d], keep[i], here[i][d]);
             __syncthreads();
         }
         const bool all = w.k0 == 0 && w.k1 == w.k_tiles;
@@ -189,21 +202,35 @@ __global__ void __launch_bounds__(PA_THREADS) paged_simt_kernel(const __grid_con
 }
 
 // The pieces of cut items: CTA (c, y) finishes rows of the item that run c of the launch before began and did not end.  GROUPS times 128 threads share an
-// item's pieces out: there are two or three where a run is a CTA's, and up to as many as there are runs where it is a warp's.
+// item's pieces out: there are two or three where a run is a CTA's, and up to as many as there are runs where it is a warp's.  With one group a
+// thread's first pieces are asked for before the rows' maxima, on which their factors wait (64 tokens behind 4000, 18 pieces an item: 33 us for 35).
 constexpr int MERGE_ROWS = 16;   // of a CTA
 template <typename T, int HD, int GROUPS>
 __global__ void __launch_bounds__(128 * GROUPS) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
     constexpr int LANES = 8 * GROUPS;   // of a row, for its maximum
+    constexpr int POS = GROUPS == 1 ? MERGE_ROWS * HD / 512 : 1, BATCH = 2;   // places of a thread and, with one group, pieces that it holds at once
     __shared__ float tops[MERGE_ROWS], sums[MERGE_ROWS];
     __shared__ float4 others[GROUPS][128];
     pdl_wait();
-    const int c = blockIdx.x, group = a.plan.group;
+    pdl_launch_dependents();   // behind the wait, so that no more than one launch waits at a time
+    const int c = blockIdx.x, group = a.plan.group, part = threadIdx.x / 128, me = threadIdx.x % 128;
+    const size_t row0 = (size_t)blockIdx.y * MERGE_ROWS;
     const int4 cut = a.cut[c];
-    const int rows = min(cut.y * group - (int)blockIdx.y * MERGE_ROWS, MERGE_ROWS), pieces = cut.w - c + 1;
+    const int rows = min(cut.y * group - (int)row0, MERGE_ROWS), pieces = cut.w - c + 1;
     if (rows <= 0) return;
     // run c's piece is its last, the others' is their first: slots 2 c + 1, 2 c + 2, 2 c + 4, ...
-    const size_t row0 = (size_t)blockIdx.y * MERGE_ROWS;
     auto slot = [&](int j) { return (2 * (size_t)(c + j) + (j == 0)) * a.tile_rows + row0; };
+    float4 v[BATCH][POS];
+    auto fetch = [&](int i0, int j0) {
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+            for (int k = 0; k < POS; ++k) {
+                const int j = j0 + b * GROUPS, i = i0 + 128 * k + me, r = i / (HD / 4);
+                v[b][k] = j < pieces && r < rows ? *reinterpret_cast<const float4 *>(a.acc + (slot(j) + r) * HD + i % (HD / 4) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+    };
+    if (GROUPS == 1) fetch(0, part);
     {   // a row's maximum over all pieces, and the sum of its weights relative to it
         const int r = threadIdx.x / LANES;
         float top = -INFINITY, sum = 0.f;
@@ -224,34 +251,53 @@ __global__ void __launch_bounds__(128 * GROUPS) paged_merge_kernel(const __grid_
         if (threadIdx.x % LANES == 0) { tops[r] = m; sums[r] = sum; }
     }
     __syncthreads();
-    const int part = threadIdx.x / 128;
-    for (int i0 = 0; i0 < rows * (HD / 4); i0 += 128) {
-        const int i = i0 + threadIdx.x % 128, r = i / (HD / 4), d = i % (HD / 4) * 4;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < rows)
+    for (int i0 = 0; i0 < rows * (HD / 4); i0 += 128 * POS) {
+        float4 o[POS];
+#pragma unroll
+        for (int k = 0; k < POS; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (GROUPS > 1) {
+            const int i = i0 + me, r = i / (HD / 4), d = i % (HD / 4) * 4;
+            if (r < rows)
 #pragma unroll 8
-            for (int j = part; j < pieces; j += GROUPS) {
-                const float f = exp2f(a.ml[(slot(j) + r) * 2] - tops[r]);
-                const float4 v = *reinterpret_cast<const float4 *>(a.acc + (slot(j) + r) * HD + d);
-                o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
-            }
+                for (int j = part; j < pieces; j += GROUPS) {
+                    const float f = exp2f(a.ml[(slot(j) + r) * 2] - tops[r]);
+                    const float4 x = *reinterpret_cast<const float4 *>(a.acc + (slot(j) + r) * HD + d);
+                    o[0].x = fmaf(f, x.x, o[0].x); o[0].y = fmaf(f, x.y, o[0].y); o[0].z = fmaf(f, x.z, o[0].z); o[0].w = fmaf(f, x.w, o[0].w);
+                }
+        }
+        for (int j0 = part; GROUPS == 1 && j0 < pieces; j0 += BATCH) {
+            if (i0 > 0 || j0 > part) fetch(i0, j0);
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+                for (int k = 0; k < POS; ++k) {
+                    const int j = j0 + b * GROUPS, r = (i0 + 128 * k + me) / (HD / 4);
+                    const float f = j < pieces && r < rows ? exp2f(a.ml[(slot(j) + r) * 2] - tops[r]) : 0.f;
+                    o[k].x = fmaf(f, v[b][k].x, o[k].x); o[k].y = fmaf(f, v[b][k].y, o[k].y);
+                    o[k].z = fmaf(f, v[b][k].z, o[k].z); o[k].w = fmaf(f, v[b][k].w, o[k].w);
+                }
+        }
         if (GROUPS > 1) {
             if (i0 > 0) __syncthreads();   // the sums before have been taken
-            others[part][threadIdx.x % 128] = o;
+            others[part][me] = o[0];
             __syncthreads();
             if (part > 0) continue;
             for (int g = 1; g < GROUPS; ++g) {
-                const float4 v = others[g][threadIdx.x];
-                o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+                const float4 x = others[g][me];
+                o[0].x += x.x; o[0].y += x.y; o[0].z += x.z; o[0].w += x.w;
             }
         }
-        if (r >= rows) continue;
-        const float f = sums[r] == 0.f ? 0.f : 1.f / sums[r];
-        const int row = (int)row0 + r, tok = paged_token(a.plan, row);
-        T *dst = (T *)a.out + (size_t)(cut.x + tok) * a.o_stride + (size_t)(cut.z * group + row - tok * group) * HD + d;
-        alignas(16) T y[4] = {from_f32<T>(o.x * f), from_f32<T>(o.y * f), from_f32<T>(o.z * f), from_f32<T>(o.w * f)};
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(y);
-        else *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(y);
+#pragma unroll
+        for (int k = 0; k < POS; ++k) {
+            const int i = i0 + 128 * k + me, r = i / (HD / 4), d = i % (HD / 4) * 4;
+            if (r >= rows) continue;
+            const float f = sums[r] == 0.f ? 0.f : 1.f / sums[r];
+            const int row = (int)row0 + r, tok = paged_token(a.plan, row);
+            T *dst = (T *)a.out + (size_t)(cut.x + tok) * a.o_stride + (size_t)(cut.z * group + row - tok * group) * HD + d;
+            alignas(16) T y[4] = {from_f32<T>(o[k].x * f), from_f32<T>(o[k].y * f), from_f32<T>(o[k].z * f), from_f32<T>(o[k].w * f)};
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(y);
+            else *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(y);
+        }
     }
 }
 
@@ -269,8 +315,8 @@ int launch_simt(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) 
         configured[dev] = true;
     }
     paged_deal(a, simt_ctas(HD), QR, 5, 1, HD, workspace, bytes);
-    paged_simt_kernel<HD, QR><<<a.ctas, PA_THREADS, S::SMEM, s>>>(a);
-    AB2_LAUNCH_CHECK();
+    ChainedLaunches chained(true);   // the launch before it, an append or a merge, need not have ended when this one is set up: it waits in the kernel
+    AB2_CUDA(launch_kernel(paged_simt_kernel<HD, QR>, dim3(a.ctas), dim3(PA_THREADS), S::SMEM, s, a));
     return a.plan.whole ? AB2_OK : paged_merge(a, HD, AB2_F32, s);
 }
 

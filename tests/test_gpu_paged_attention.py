@@ -257,3 +257,54 @@ def test_refusals():
         with pytest.raises(p.Ab2Error):
             p.dispatch.attention_paged(**{**ok, **change})
     assert p.dispatch.attention_paged(**{**ok, "q": b.q[:0], "starts": torch.zeros(3, dtype=torch.int32, device="cuda")}).shape == (0, 8, 64)
+
+
+@pytest.mark.parametrize("new", [1, 4, 90])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_recorded_behind_copies_and_other_streams(new, dtype):
+    """A call that is recorded behind a copy, a clear and another stream's work reads what they left: its launch may be set up before they have ended."""
+    b = Batch([300, 95, 7], [new] * 3, 8, 2, 64, 16, dtype, seed=11, scatter=0.5)
+    want = b.run(pkg())
+    q = torch.zeros_like(b.q)
+    run = lambda: pkg().dispatch.attention_paged(q, b.k_pages, b.v_pages, b.table, b.lens_dev, b.scale, b.starts)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        q.zero_()
+        with torch.cuda.stream(side):
+            half = torch.empty_like(b.q).copy_(b.q)
+            for _ in range(20):
+                half.mul_(2).mul_(0.5)   # exact, and slower than what the main stream does
+        torch.cuda.current_stream().wait_stream(side)
+        q.copy_(half)
+        first, second = run(), run()
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(first, want) and torch.equal(second, want)
+    for _ in range(20):   # eager: behind kernels that have not ended
+        q.zero_()
+        q.copy_(b.q.mul(2)).mul_(0.5)
+        got = run()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 20])
+def test_a_long_f32_row_rounds_once_a_tile(new, dim):
+    """Equal scores and equal values, all keys by one CTA (there is no workspace to cut the row by): the mean is the value itself, and every rounding of a
+    sum goes the same way.  The weights are 1 and their sum is exact.  Values are summed over 32 keys, and those sums over n / 32 tiles: at most
+    n / 32 + 32 roundings of 2^-24 each, and 4 more for the reciprocal, the product and the tile's last part.  One chain over the 20000 keys would be off by
+    1.8e-4 (0.7 added to itself in f32), where 3.9e-5 is allowed."""
+    n = 20000
+    b = Batch([n], [new], 4, 2, dim, 256, F32, seed=1)
+    b.q.zero_()
+    b.v_pages.copy_(torch.where(torch.isnan(b.v_pages), b.v_pages, torch.full_like(b.v_pages, 0.7)))
+    out = torch.empty_like(b.q)
+    p = pkg()
+    c, keep = p.dispatch._paged(b.k_pages, b.v_pages, b.table, b.lens_dev, b.starts, b.T)
+    p.check(p.lib.ab2_paged_attention(C.byref(c), b.q.data_ptr(), 4 * dim, 4, out.data_ptr(), 4 * dim, new, b.scale, None, 0, p.dispatch.dtype_code(F32), torch.cuda.current_stream().cuda_stream))
+    value = b.v_pages[~torch.isnan(b.v_pages)][0].double()
+    assert ((out.double() / value - 1).abs() <= (n / 32 + 32 + 4) * 2.0 ** -24).all()
