@@ -62,6 +62,7 @@ __global__ void __launch_bounds__(32 * PM_WARPS, 2) paged_mma_kernel(const __gri
     constexpr int KS = HD / 16, CH = HD / 8, STAGES = S::STAGES, LOADS = PM_KEYS * CH / 32;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int2 found[PM_WARPS][2];
+    pdl_wait();
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, group = a.plan.group;
     const PagedView &p = a.plan.p;
@@ -296,8 +297,8 @@ int launch_mma(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
         configured[dev] = true;
     }
     paged_deal(a, mma_runs(), 8 * NT, 6, 1, HD, workspace, bytes);
-    paged_mma_kernel<HD, NT><<<a.ctas / PM_WARPS, 32 * PM_WARPS, S::SMEM, s>>>(a);
-    AB2_LAUNCH_CHECK();
+    ChainedLaunches chained(true);   // set up while the launch before it ends
+    AB2_CUDA(launch_kernel(paged_mma_kernel<HD, NT>, dim3(a.ctas / PM_WARPS), dim3(32 * PM_WARPS), S::SMEM, s, a));
     return a.plan.whole ? AB2_OK : paged_merge(a, HD, AB2_BF16, s);
 }
 

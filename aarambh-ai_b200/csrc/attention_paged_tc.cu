@@ -208,6 +208,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     uint8_t *qbuf = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023), *ring = qbuf + 2 * S::QTILE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *failed = &sh.failed;
+    pdl_wait();   // ahead of tensor memory too, which the launch before may hold
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::SLOTS; ++i) { bar_init(&sh.full[i], 1); bar_init(&sh.empty[i], 2); }
         for (int i = 0; i < 2; ++i) { bar_init(&sh.qfull[i], 4); bar_init(&sh.sfull[i], 1); bar_init(&sh.sfree[i], 4); bar_init(&sh.pfull[i], 4); bar_init(&sh.odone[i], 1); }
@@ -486,8 +487,8 @@ int launch_tc(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
     if (rc == AB2_OK) rc = pages_map(&vmap, a.v, a.plan.p, HD);
     if (rc != AB2_OK) return rc;
     paged_deal(a, device_sm_count(), 2 * PC_Q, 7, 4, HD, workspace, bytes);
-    paged_tc_kernel<HD><<<a.ctas, PC_THREADS, S::SMEM, s>>>(kmap, vmap, a);
-    AB2_LAUNCH_CHECK();
+    ChainedLaunches chained(true);   // set up while the launch before it ends
+    AB2_CUDA(launch_kernel(paged_tc_kernel<HD>, dim3(a.ctas), dim3(PC_THREADS), S::SMEM, s, kmap, vmap, a));
     return a.plan.whole ? AB2_OK : paged_merge(a, HD, AB2_BF16, s);
 }
 
