@@ -14,8 +14,8 @@
 // weights.  Scores, maxima, sums and O are f32.  The weights are relative to a maximum per row that moves only when a score exceeds it by 2^8; then O is
 // rescaled in tensor memory.
 //
-// 4096 tokens behind 12288, 32 / 8 heads of 128: 0.92 ms, 1.05 PFLOP/s, 0.63 of cuBLAS in a burst and 0.75 of it sustained; 2048 behind 2048 126 us;
-// six rows of 1 to 512 tokens behind up to 5000 128 us.  Bound by the two softmax warps of a scheduler: of the 2300 clocks of a tile of 80 keys they
+// 4096 tokens behind 12288, 32 / 8 heads of 128: 0.92 ms, 1.05 PFLOP/s, 0.63 of cuBLAS in a burst and 0.75 of it sustained; 2048 behind 2048 120 us;
+// six rows of 1 to 512 tokens behind up to 5000 126 us.  Bound by the two softmax warps of a scheduler: of the 2300 clocks of a tile of 80 keys they
 // need 1250 for the exponentials (read by clocks in the kernel; both tiles' are 2 x 128 x 80, at 16 a clock 1280), and the rest for scores from
 // tensor memory, the maximum, and the waits for scores and for the last tile's products, some 150 clocks each; the products take 1432.
 //
@@ -208,13 +208,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     uint8_t *qbuf = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023), *ring = qbuf + 2 * S::QTILE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *failed = &sh.failed;
-    pdl_wait();   // ahead of tensor memory too, which the launch before may hold
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::SLOTS; ++i) { bar_init(&sh.full[i], 1); bar_init(&sh.empty[i], 2); }
         for (int i = 0; i < 2; ++i) { bar_init(&sh.qfull[i], 4); bar_init(&sh.sfull[i], 1); bar_init(&sh.sfree[i], 4); bar_init(&sh.pfull[i], 4); bar_init(&sh.odone[i], 1); }
         sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
+    pdl_wait();   // ahead of tensor memory too, which the launch before may hold
     PagedRun run = paged_run<PC_THREADS>(a.plan, blockIdx.x, a.ctas, sh.warp_sums, sh.found, a.status);
     if (threadIdx.x == PC_THREADS - 1) paged_uncut(a, blockIdx.x);
     if (run.u >= run.u1) return;   // the whole CTA
@@ -487,7 +487,8 @@ int launch_tc(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
     if (rc == AB2_OK) rc = pages_map(&vmap, a.v, a.plan.p, HD);
     if (rc != AB2_OK) return rc;
     paged_deal(a, device_sm_count(), 2 * PC_Q, 7, 4, HD, workspace, bytes);
-    ChainedLaunches chained(true);   // set up while the launch before it ends
+    // Set up while the launch before it ends: 8 x 300 tokens 36.6 us for 39.3, 2048 behind 2048 120 for 121.5; 4096 behind 12288 lose 0.6 %, 922 for 916.
+    ChainedLaunches chained(true);
     AB2_CUDA(launch_kernel(paged_tc_kernel<HD>, dim3(a.ctas), dim3(PC_THREADS), S::SMEM, s, kmap, vmap, a));
     return a.plan.whole ? AB2_OK : paged_merge(a, HD, AB2_BF16, s);
 }
