@@ -8,8 +8,10 @@
 //
 // This file: f32, on CUDA cores; attention_paged_mma.cu and attention_paged_tc.cu: bf16.
 // A CTA multiplies the queries of a KV head's whole group (tokens x heads of the group, up to QR rows) with a tile of 32 keys on CUDA cores;
-// keys and values come by cp.async, the next tile's while this one's are looked at.  Three rows of up to 130 tokens behind 380, 6 / 2 heads of 64: 22.8 us,
-// with kernels of 18 and 7 by themselves.  Its scores load 16 bytes from shared memory six times for 32 multiplications (4 x 4 results a thread would: eight for 64).
+// keys and values come by cp.async, the next tile's while this one's are looked at.  Values are summed over a tile and
+// then joined to the others', which rounds once a tile.  500 tokens behind 1000, 16 / 4 heads of 128: 170 us, 30 TFLOP/s, by tiles of 64 rows, whose scores
+// load 16 bytes from shared memory eight times for 64 multiplications; by tiles of 32, six times for 32, 229.  Three rows of up to 130 tokens behind 380,
+// 6 / 2 heads of 64: 22.4 us, of which launches, lengths, first copies and the merge are most.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -30,12 +32,16 @@ constexpr int PAGED_FEW_ROWS = 16;   // query rows of a KV head up to which the 
 namespace {
 
 constexpr int PA_THREADS = 128, PA_KEYS = 32;
+constexpr int TALL_ROWS = 512, TALL_ALL = 2560;
 
 template <int HD, int QR> struct SimtShape {
-    static constexpr int TX = QR == 32 ? 8 : 16, RPT = QR * TX / PA_THREADS, KPT = PA_KEYS / TX, DPT = HD / TX;
-    static constexpr int KROW = HD + 4;                     // a row's bank moves on by 16 bytes
+    static constexpr int TX = QR == 8 ? 16 : 8, TY = PA_THREADS / TX, RPT = QR / TY, KPT = PA_KEYS / TX, DPT = HD / TX;
+    // Row i of a thread: two are neighbours, which see much the same keys; four lie TY apart, or those of a warp would meet in the same banks.
+    static constexpr int STEP = RPT == 4 ? TY : 1, FIRST = RPT == 4 ? 1 : RPT;
+    static constexpr int KROW = HD + 4, PROW = PA_KEYS + 4;   // a row's bank moves on by 16 bytes
     static constexpr int BUF = PA_KEYS * KROW * 4;
-    static constexpr int SMEM = 4 * BUF + QR * (HD + 4) * 4 + QR * (PA_KEYS + 1) * 4;
+    static constexpr int SMEM = 4 * BUF + QR * KROW * 4 + QR * PROW * 4;
+    static constexpr int CTAS = HD == 128 ? 2 : QR == 64 ? 3 : 4;   // of an SM: what shared memory holds
 };
 
 __device__ __forceinline__ void cp16(void *dst, const void *src, bool in) {
@@ -43,16 +49,16 @@ __device__ __forceinline__ void cp16(void *dst, const void *src, bool in) {
 }
 __device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 template <int HD, int QR>
-__global__ void __launch_bounds__(PA_THREADS, HD == 64 ? 4 : 2) paged_simt_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_simt_kernel(const __grid_constant__ PagedAttnArgs a) {
     using S = SimtShape<HD, QR>;
     pdl_wait();
-    constexpr int TX = S::TX, RPT = S::RPT, KPT = S::KPT, DPT = S::DPT, KROW = S::KROW, CH = 4;
+    constexpr int TX = S::TX, RPT = S::RPT, KPT = S::KPT, DPT = S::DPT, KROW = S::KROW, PROW = S::PROW, STEP = S::STEP, CH = 4;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ long long warp_sums[PA_THREADS / 32];
     __shared__ int2 found[2];
     float *kbuf = (float *)smem, *vbuf = kbuf + 2 * PA_KEYS * KROW;
-    float *qs = (float *)(smem + 4 * S::BUF), *ps = qs + QR * (HD + 4);
-    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+    float *qs = (float *)(smem + 4 * S::BUF), *ps = qs + QR * KROW;
+    const int tx = threadIdx.x % TX, row0 = threadIdx.x / TX * S::FIRST;
     const PagedView &p = a.plan.p;
     PagedRun run = paged_run<PA_THREADS>(a.plan, blockIdx.x, gridDim.x, warp_sums, found, a.status);
     if (threadIdx.x == 0) paged_uncut(a, blockIdx.x);
@@ -66,7 +72,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 64 ? 4 : 2) paged_simt_kerne
             const int r = i / (HD / 4), d = i % (HD / 4) * 4, tok = paged_token(a.plan, r), g = r - tok * group;
             float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
             if (tok < ntok) f = load4((const float *)a.q + (size_t)(w.r.first + t0 + tok) * a.q_stride + (size_t)(w.head * group + g) * HD + d);
-            *reinterpret_cast<float4 *>(qs + r * (HD + 4) + d) = make_float4(f.x * a.sl, f.y * a.sl, f.z * a.sl, f.w * a.sl);
+            *reinterpret_cast<float4 *>(qs + r * KROW + d) = make_float4(f.x * a.sl, f.y * a.sl, f.z * a.sl, f.w * a.sl);
         }
         // rows past the last key read as zeros
         auto fetch = [&](int key0, int buf) {
@@ -81,11 +87,13 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 64 ? 4 : 2) paged_simt_kerne
             asm volatile("cp.async.commit_group;\n" ::: "memory");
         };
         float top[RPT], sum[RPT], o[RPT][DPT];
-        int lim[RPT];
+        int lim[RPT], seen = -1, sure = hi - 1;   // the last key that any row of the thread sees, and the last that all do
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
-            const int tok = paged_token(a.plan, ty * RPT + i);
-            lim[i] = tok < ntok ? base + t0 + tok : -1;
+            const int tok = paged_token(a.plan, row0 + STEP * i);
+            lim[i] = tok < ntok ? base + t0 + tok : 0x7fffffff;   // a row without a token is not looked at, and keeps no other from what all see
+            if (tok < ntok) seen = lim[i];                        // rows go by tokens
+            sure = min(sure, lim[i]);
             top[i] = -INFINITY;
             sum[i] = 0.f;
 #pragma unroll
@@ -109,7 +117,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 64 ? 4 : 2) paged_simt_kerne
             for (int d = 0; d < HD; d += 4) {
                 float4 qv[RPT], kv[KPT];
 #pragma unroll
-                for (int i = 0; i < RPT; ++i) qv[i] = *reinterpret_cast<const float4 *>(qs + (ty * RPT + i) * (HD + 4) + d);
+                for (int i = 0; i < RPT; ++i) qv[i] = *reinterpret_cast<const float4 *>(qs + (row0 + STEP * i) * KROW + d);
 #pragma unroll
                 for (int j = 0; j < KPT; ++j) kv[j] = load4(kbuf + (buf * PA_KEYS + tx + TX * j) * KROW + d);
 #pragma unroll
@@ -145,20 +153,40 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 64 ? 4 : 2) paged_simt_kerne
                     const int key = key0 + tx + TX * j;
                     const float e = key > lim[i] || key >= hi ? 0.f : exp2f(s[i][j] - m);
                     weights += e;
-                    ps[(ty * RPT + i) * (PA_KEYS + 1) + tx + TX * j] = e;
+                    ps[(row0 + STEP * i) * PROW + tx + TX * j] = e;
                 }
                 sum[i] = fmaf(sum[i], keep[i], weights);
             }
             __syncwarp();  // a row's weights come from lanes of one warp
             // keys that no row of the thread sees may hold anything: their weight is 0, and 0 times Inf is not
-            int seen = -1;
+            const bool every = RPT > 1 && seen >= 0 && key0 + PA_KEYS - 1 <= sure;   // of the tile's keys is seen by every row of the thread
+            if (every) {
+#pragma unroll 2
+                for (int j = 0; j < PA_KEYS; j += 4) {
+                    float4 e[RPT];
 #pragma unroll
-            for (int i = 0; i < RPT; ++i) seen = max(seen, lim[i]);
-            const int n = min(PA_KEYS, min(hi, seen + 1) - key0);
+                    for (int i = 0; i < RPT; ++i) e[i] = load4(ps + (row0 + STEP * i) * PROW + j);
+#pragma unroll
+                    for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+                        for (int d = 0; d < DPT; d += 4) {
+                            const float4 v = load4(vbuf + (buf * PA_KEYS + j + jj) * KROW + tx * 4 + d * TX);
+#pragma unroll
+                            for (int i = 0; i < RPT; ++i) {
+                                const float f = jj == 0 ? e[i].x : jj == 1 ? e[i].y : jj == 2 ? e[i].z : e[i].w;
+                                here[i][d] = fmaf(f, v.x, here[i][d]);
+                                here[i][d + 1] = fmaf(f, v.y, here[i][d + 1]);
+                                here[i][d + 2] = fmaf(f, v.z, here[i][d + 2]);
+                                here[i][d + 3] = fmaf(f, v.w, here[i][d + 3]);
+                            }
+                        }
+                }
+            }
+            const int n = every ? 0 : min(PA_KEYS, min(hi - key0, seen + 1 - key0));
             for (int j = 0; j < n; ++j) {
                 float e[RPT];
 #pragma unroll
-                for (int i = 0; i < RPT; ++i) e[i] = ps[(ty * RPT + i) * (PA_KEYS + 1) + j];
+                for (int i = 0; i < RPT; ++i) e[i] = ps[(row0 + STEP * i) * PROW + j];
 #pragma unroll
                 for (int d = 0; d < DPT; d += 4) {
                     const float4 v = load4(vbuf + (buf * PA_KEYS + j) * KROW + tx * 4 + d * TX);
@@ -182,7 +210,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 64 ? 4 : 2) paged_simt_kerne
         const size_t slot = 2 * (size_t)blockIdx.x + (w.k0 == 0);
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
-            const int r = ty * RPT + i, tok = paged_token(a.plan, r), g = r - tok * group;
+            const int r = row0 + STEP * i, tok = paged_token(a.plan, r), g = r - tok * group;
 #pragma unroll
             for (int m = TX / 2; m > 0; m >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], m);
             if (tok >= ntok) continue;
@@ -301,7 +329,7 @@ __global__ void __launch_bounds__(128 * GROUPS) paged_merge_kernel(const __grid_
     }
 }
 
-int simt_ctas(int hd) { return (hd == 64 ? 4 : 2) * device_sm_count(); }   // what shared memory holds
+template <int HD, int QR> size_t simt_bytes() { return paged_piece_bytes(SimtShape<HD, QR>::CTAS * device_sm_count(), QR, HD); }
 
 template <int HD, int QR>
 int launch_simt(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
@@ -314,16 +342,20 @@ int launch_simt(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) 
         AB2_CUDA(cudaFuncSetAttribute(paged_simt_kernel<HD, QR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
         configured[dev] = true;
     }
-    paged_deal(a, simt_ctas(HD), QR, 5, 1, HD, workspace, bytes);
+    paged_deal(a, S::CTAS * device_sm_count(), QR, 5, 1, HD, workspace, bytes);
     ChainedLaunches chained(true);   // the launch before it, an append or a merge, need not have ended when this one is set up: it waits in the kernel
     AB2_CUDA(launch_kernel(paged_simt_kernel<HD, QR>, dim3(a.ctas), dim3(PA_THREADS), S::SMEM, s, a));
     return a.plan.whole ? AB2_OK : paged_merge(a, HD, AB2_F32, s);
 }
 
 int simt_attention(const PagedAttnArgs &a, int hd, int max_new, void *workspace, size_t bytes, cudaStream_t s) {
-    const bool few = max_new * (long long)a.plan.group <= 8;
-    if (hd == 128) return few ? launch_simt<128, 8>(a, workspace, bytes, s) : launch_simt<128, 32>(a, workspace, bytes, s);
-    return few ? launch_simt<64, 8>(a, workspace, bytes, s) : launch_simt<64, 32>(a, workspace, bytes, s);
+    // Tiles of 64 rows load a third less from shared memory but are half as many, with more rows that no token fills.  They pay for long chunks: from 512 query
+    // rows a KV head of a sequence, where the batch has 2560 of all heads to share out (us by tiles of 32 and of
+    // 64: 500 tokens behind 1000, 16 heads of 128, 229 and 170; 200 behind 1000 88 and 78; 5 x 60 behind 500 41 and 43; 100 behind 1000, 6 heads of 64, 26 and 33).
+    const long long rows = max_new * (long long)a.plan.group, all = (long long)a.plan.p.tokens * a.plan.group * a.plan.p.kv_heads;
+    const bool tall = rows >= TALL_ROWS && all >= TALL_ALL;
+    if (hd == 128) return rows <= 8 ? launch_simt<128, 8>(a, workspace, bytes, s) : tall ? launch_simt<128, 64>(a, workspace, bytes, s) : launch_simt<128, 32>(a, workspace, bytes, s);
+    return rows <= 8 ? launch_simt<64, 8>(a, workspace, bytes, s) : tall ? launch_simt<64, 64>(a, workspace, bytes, s) : launch_simt<64, 32>(a, workspace, bytes, s);
 }
 
 }  // namespace
@@ -332,10 +364,11 @@ int paged_merge(const PagedAttnArgs &a, int hd, ab2_dtype dtype, cudaStream_t s)
     ChainedLaunches chained(true);
     const dim3 grid(a.ctas, (a.tile_rows + MERGE_ROWS - 1) / MERGE_ROWS);
     const bool tall = a.tile_rows > 32;   // a run is a CTA's, and few of them share an item
-    auto kernel = dtype == AB2_F32 ? (hd == 128 ? paged_merge_kernel<float, 128, 4> : paged_merge_kernel<float, 64, 4>)
+    auto kernel = dtype == AB2_F32 ? (tall ? (hd == 128 ? paged_merge_kernel<float, 128, 1> : paged_merge_kernel<float, 64, 1>)
+                                           : (hd == 128 ? paged_merge_kernel<float, 128, 4> : paged_merge_kernel<float, 64, 4>))
                   : tall           ? (hd == 128 ? paged_merge_kernel<__nv_bfloat16, 128, 1> : paged_merge_kernel<__nv_bfloat16, 64, 1>)
                                    : (hd == 128 ? paged_merge_kernel<__nv_bfloat16, 128, 4> : paged_merge_kernel<__nv_bfloat16, 64, 4>);
-    cudaError_t e = launch_kernel(kernel, grid, dim3(dtype == AB2_BF16 && tall ? 128 : 512), 0, s, a);
+    cudaError_t e = launch_kernel(kernel, grid, dim3(tall ? 128 : 512), 0, s, a);
     if (e != cudaSuccess) return fail(AB2_ERR_CUDA, "paged attention launch failed: %s", cudaGetErrorString(e));
     return AB2_OK;
 }
@@ -345,7 +378,8 @@ int paged_merge(const PagedAttnArgs &a, int hd, ab2_dtype dtype, cudaStream_t s)
 AB2_API int ab2_paged_workspace(int head_dim, size_t *bytes) {
     AB2_REQUIRE(bytes, AB2_ERR_BAD_ARG, "null argument");
     AB2_REQUIRE(head_dim == 64 || head_dim == 128, AB2_ERR_UNSUPPORTED, "paged caches have heads of 64 or 128, not %d", head_dim);
-    *bytes = std::max(std::max(paged_piece_bytes(simt_ctas(head_dim), 32, head_dim), paged_mma_bytes(head_dim)), paged_tc_bytes(head_dim));
+    const size_t simt = head_dim == 128 ? std::max(simt_bytes<128, 32>(), simt_bytes<128, 64>()) : std::max(simt_bytes<64, 32>(), simt_bytes<64, 64>());
+    *bytes = std::max(simt, std::max(paged_mma_bytes(head_dim), paged_tc_bytes(head_dim)));
     return AB2_OK;
 }
 

@@ -308,3 +308,28 @@ def test_a_long_f32_row_rounds_once_a_tile(new, dim):
     p.check(p.lib.ab2_paged_attention(C.byref(c), b.q.data_ptr(), 4 * dim, 4, out.data_ptr(), 4 * dim, new, b.scale, None, 0, p.dispatch.dtype_code(F32), torch.cuda.current_stream().cuda_stream))
     value = b.v_pages[~torch.isnan(b.v_pages)][0].double()
     assert ((out.double() / value - 1).abs() <= (n / 32 + 32 + 4) * 2.0 ** -24).all()
+
+
+TALL = [(520, 8, 1, 128, 16), (300, 12, 4, 64, 64), (531, 5, 5, 128, 128), (180, 32, 2, 64, 32), (171, 30, 10, 128, 32), (90, 32, 1, 64, 256)]
+
+
+@pytest.mark.parametrize("new,heads,kv_heads,dim,page", TALL)
+def test_long_f32_chunks(new, heads, kv_heads, dim, page):
+    """Rows of the tallest tiles: groups of 1 to 32 heads, with rows of no tokens, of no keys before them, and of a tile's last few tokens."""
+    check(Batch([new, 0, new + 333, new + 1, 40], [new, 0, new, 1, 33], heads, kv_heads, dim, page, F32, seed=new))
+
+
+@pytest.mark.parametrize("new,heads,kv_heads,dim,page", TALL)
+def test_long_f32_chunks_out_of_sight(new, heads, kv_heads, dim, page):
+    """Whatever the last 45 tokens hold, those before them answer the same bits."""
+    b = Batch([new + 70], [new], heads, kv_heads, dim, page, F32, seed=7)
+    want = b.run(pkg()).clone()
+    seen = new - 45
+    for bad_k, bad_v in ((math.nan, math.nan), (1.0, math.inf), (math.inf, 1.0), (torch.finfo(F32).min, -math.inf)):
+        for pos in range(new + 70 - 45, new + 70):
+            at = b.table[0, pos // page].item()
+            b.k_pages[at, :, pos % page] = bad_k
+            b.v_pages[at, :, pos % page] = bad_v
+        got = b.run(pkg())
+        assert torch.equal(got[:seen], want[:seen])
+    assert pkg().device_status() == 0
