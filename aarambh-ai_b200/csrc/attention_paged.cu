@@ -11,7 +11,8 @@
 // keys and values come by cp.async, the next tile's while this one's are looked at.  Values are summed over a tile and
 // then joined to the others', which rounds once a tile.  500 tokens behind 1000, 16 / 4 heads of 128: 170 us, 30 TFLOP/s, by tiles of 64 rows, whose scores
 // load 16 bytes from shared memory eight times for 64 multiplications; by tiles of 32, six times for 32, 229.  Three rows of up to 130 tokens behind 380,
-// 6 / 2 heads of 64: 22.4 us, of which launches, lengths, first copies and the merge are most.
+// 6 / 2 heads of 64: 22.4 us (a kernel of 18 and a merge of 7 by
+// themselves, before a launch was set up while the one before it ended).
 #include <algorithm>
 
 #include "paged.cuh"

@@ -487,8 +487,10 @@ int launch_tc(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
     if (rc == AB2_OK) rc = pages_map(&vmap, a.v, a.plan.p, HD);
     if (rc != AB2_OK) return rc;
     paged_deal(a, device_sm_count(), 2 * PC_Q, 7, 4, HD, workspace, bytes);
-    // Set up while the launch before it ends: 8 x 300 tokens 36.6 us for 39.3, 2048 behind 2048 120 for 121.5; 4096 behind 12288 lose 0.6 %, 922 for 916.
-    ChainedLaunches chained(true);
+    // Set up while the launch before it ends, which saves some 1.7 us of any call and costs long ones up to 2 %.  How long a call is lies with the context,
+    // which the host does not know; by its query rows (us not set up early and early, 32 heads of 128): 300 tokens behind 300 34.1 and 32.5, 1024 behind
+    // 1024 52.6 and 50.4, 2048 alone 79.7 and 77.9, behind 12288 442 and 445; 3000 behind 3000 238 and 241, 4096 alone 197 and 195, behind 12288 924 and 943.
+    ChainedLaunches chained((long long)a.plan.p.tokens * a.plan.group * a.plan.p.kv_heads <= 65536);
     AB2_CUDA(launch_kernel(paged_tc_kernel<HD>, dim3(a.ctas), dim3(PC_THREADS), S::SMEM, s, kmap, vmap, a));
     return a.plan.whole ? AB2_OK : paged_merge(a, HD, AB2_BF16, s);
 }
