@@ -242,7 +242,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * PC_ROWS * HD * 2;
                     const int slot = n % S::SLOTS;
                     warp_wait(&sh.empty[slot], ((n++ / S::SLOTS) & 1) ^ 1, failed);
-                    if (n == 2 && x.first > 0) warp_wait(&sh.qfull[0], 0, failed);   // the first queries come before what is fetched ahead
+                    // The first queries come before what is fetched ahead.  Only at the second slot of the run's first piece with keys, and only where the first
+                    // tile of rows looks at it: its warps cannot announce their next queries without that slot, so the barrier is in its first phase or just
+                    // behind it.  A later phase would have this parity again, and might wait for what is not yet fetched.
+                    if (n == 2 && j == 1 && x.first > 1) warp_wait(&sh.qfull[0], 0, failed);
                     if (lane == 0) bar_expect_tx(&sh.full[slot], (uint32_t)(2 * bytes));
                     __syncwarp();
                     if (mine && !*failed)
