@@ -368,7 +368,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             float top = PC_NONE, sum = 0.f;
             for (int j = 0; j < tiles; ++j, ++scored) {
                 const int at = lo + j * PC_KEYS;
+                warp_wait(&sh.sfull[g], scored & 1, failed);
                 if (at + PC_KEYS > hi) {   // what lies behind the piece's keys may be anything
+                    // Behind the wait for the scores, never ahead of it: these warps pass over pieces without rows of theirs, and the slot's barrier may still be phases
+                    // away from the one meant, with the same parity.
                     const int slot = (slot0 + j) % S::SLOTS;
                     warp_wait(&sh.full[slot], ((slot0 + j) / S::SLOTS) & 1, failed);
                     if (at + r >= hi && r < PC_KEYS)
@@ -379,7 +382,6 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                     __syncwarp();   // and the products wait for all four warps
                 }
-                warp_wait(&sh.sfull[g], scored & 1, failed);
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                 const int lim = min(pos, hi - 1) - at;
                 auto before = [&] { if (j > 0) warp_wait(&sh.odone[g], (scored - 1) & 1, failed); };
