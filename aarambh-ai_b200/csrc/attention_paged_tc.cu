@@ -25,7 +25,7 @@
 //
 // An MMA multiplies a hidden value by a weight of 0, so an Inf or a NaN there would reach rows that do not see it.  Rows of a page behind the
 // sequence's end are cleared in shared memory; a row whose sums come out as Inf or NaN (a later token's value may hold them) is computed
-// again on CUDA cores over the keys in its sight.  Every wait on an mbarrier is bounded; on a time-out the CTA records AB2_ERR_TIMEOUT and
+// again on CUDA cores over the keys in its sight, behind all pieces of the CTA, so that no bounded wait lasts as long as that.  Every wait on an mbarrier is bounded; on a time-out the CTA records AB2_ERR_TIMEOUT and
 // walks through the rest of its work without waiting.
 #include <algorithm>
 
@@ -105,7 +105,10 @@ struct PcShared {
     uint32_t tmem_base;
     int failed;
     int2 found[2];
-    long long warp_sums[PC_THREADS / 32];
+    union {
+        long long warp_sums[PC_THREADS / 32];   // while the CTA looks for its run
+        PagedRun start;                         // that run, from then on
+    };
     // of every softmax warp: its run, the piece that it is at and the next one (kept from its registers, which the scores fill)
     PagedRun run[8];
     PcPiece piece[8][2];
@@ -205,6 +208,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     using S = PcShape<HD>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ PcShared sh;
+    static_assert(S::SMEM + sizeof(PcShared) <= 227 * 1024, "shared memory of a CTA");
     uint8_t *qbuf = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023), *ring = qbuf + 2 * S::QTILE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *failed = &sh.failed;
@@ -218,6 +222,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     PagedRun run = paged_run<PC_THREADS>(a.plan, blockIdx.x, a.ctas, sh.warp_sums, sh.found, a.status);
     if (threadIdx.x == PC_THREADS - 1) paged_uncut(a, blockIdx.x);
     if (run.u >= run.u1) return;   // the whole CTA
+    if (threadIdx.x == 0) sh.start = run;
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(sptr(&sh.tmem_base)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
@@ -352,7 +357,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
             asm volatile("cp.async.commit_group;\n" ::: "memory");
         };
-        bool more = next();
+        bool more = next(), again = false;   // again: a row's sums came out as Inf or NaN
         if (more) fetch_q();
         while (more) {
             const PcPiece &x = sh.piece[warp - 4][here];
@@ -453,11 +458,34 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
             }
             if (!all && rr < rows) *reinterpret_cast<float2 *>(a.ml + (slot + rr) * 2) = make_float2(top, sum);
-            __syncwarp();
-            for (uint32_t left = __ballot_sync(0xffffffffu, rr < rows && poison != 0.f); left; left &= left - 1)  // NaN is not 0
-                paged_again<HD>(a, w, s, g * PC_Q + quad * 32 + __ffs(left) - 1, lane, all, slot);
+            again |= __any_sync(0xffffffffu, rr < rows && poison != 0.f);   // NaN is not 0
             // the next piece's products may go over what has been read
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+        }
+        // Rows to compute again, found by what has been stored of them.  Behind the last piece: it may take long, and until then other roles would wait for these
+        // warps at barriers whose waits are bounded.
+        if (again) {
+            PagedRun walk = sh.start;
+            PcPiece x;
+            while (pc_next(a.plan, walk, x)) {
+                const int rr = g * PC_Q + r, rows = x.s.ntok * group;
+                if (rows <= g * PC_Q) continue;
+                const bool all = x.w.k0 == 0 && x.w.k1 == x.w.k_tiles;
+                const size_t slot = (2 * (size_t)blockIdx.x + (x.w.k0 == 0)) * a.tile_rows;
+                uint32_t worst = 0;   // of the exponents
+                if (rr < rows) {
+                    const int tok = paged_token(a.plan, rr);
+                    const uint32_t *o = all ? (const uint32_t *)((const __nv_bfloat16 *)a.out + (size_t)(x.w.r.first + x.s.t0 + tok) * a.o_stride + (size_t)(x.w.head * group + rr - tok * group) * HD)
+                                            : (const uint32_t *)(a.acc + (slot + rr) * HD);
+                    for (int i = 0; i < (all ? HD / 2 : HD); ++i) {
+                        worst = max(worst, o[i] & 0x7f800000u);
+                        if (all) worst = max(worst, (o[i] & 0x7f80u) << 16);
+                    }
+                }
+                for (uint32_t left = __ballot_sync(0xffffffffu, worst == 0x7f800000u); left; left &= left - 1)
+                    paged_again<HD>(a, x.w, x.s, g * PC_Q + quad * 32 + __ffs(left) - 1, lane, all, slot);
+                __syncwarp();
+            }
         }
     }
     // ---- teardown: every warp arrives here (all waits are bounded)

@@ -274,32 +274,54 @@ __device__ __forceinline__ void paged_cut(const PagedAttnArgs &a, const PagedRun
     a.cut[c] = make_int4(w.r.first + sp.t0, sp.ntok, w.head, (int)min((long long)run.ctas - 1, paged_div(end * run.ctas - 1, run.total)));
 }
 
-// Row r of a piece of bf16 over the keys [lo, to] of it that it sees, by one warp, a lane every 32nd dimension: where a product with hidden values
-// has left Inf or NaN (a weight of 0 times either), this gives what the keys in sight alone give.
+// Row r of a piece of bf16 over the keys [lo, to] of it that it sees, by one warp: where a product with hidden values has left Inf or NaN (a weight of 0
+// times either), this gives what the keys in sight alone give.  32 keys at a time: a lane has one for the scores, and every 32nd dimension for the sums, so
+// that loads of 32 keys are in flight where one key after the other waited for its page, its shuffles and its exponential.
 template <int HD>
 __device__ __forceinline__ void paged_again(const PagedAttnArgs &a, const PagedPiece &w, const PagedSpan &sp, int r, int lane, bool all, size_t slot) {
     constexpr int N = HD / 32;
     const int tok = paged_token(a.plan, r), head = w.head * a.plan.group + r - tok * a.plan.group;
     const int to = min(sp.hi - 1, sp.base + sp.t0 + tok);
     const __nv_bfloat16 *q = (const __nv_bfloat16 *)a.q + (size_t)(w.r.first + sp.t0 + tok) * a.q_stride + (size_t)head * HD;
-    float qv[N], acc[N] = {}, top = -INFINITY, sum = 0.f;
+    float acc[N] = {}, top = -INFINITY, sum = 0.f;
+    for (int key0 = sp.lo; key0 <= to; key0 += 32) {
+        const int key = key0 + lane, n = min(32, to - key0 + 1);
+        long long row = 0;
+        float s = -INFINITY;
+        if (lane < n) {
+            row = (((long long)paged_page(a.plan.p, w.row, key, a.status) * a.plan.p.kv_heads + w.head) << a.plan.p.page_shift) + (key & ((1 << a.plan.p.page_shift) - 1));
+            const __nv_bfloat16 *k = (const __nv_bfloat16 *)a.k + row * HD;
+            s = 0.f;
+#pragma unroll 4
+            for (int d = 0; d < HD; d += 8) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(q + d), y = *reinterpret_cast<const uint4 *>(k + d);
+                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-    for (int i = 0; i < N; ++i) qv[i] = __bfloat162float(q[lane + 32 * i]) * a.sl;
-    for (int key = sp.lo; key <= to; ++key) {
-        const size_t row = (((size_t)paged_page(a.plan.p, w.row, key, a.status) * a.plan.p.kv_heads + w.head) << a.plan.p.page_shift) + (key & ((1 << a.plan.p.page_shift) - 1));
-        float s = 0.f, vv[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            s = fmaf(qv[i], __bfloat162float(((const __nv_bfloat16 *)a.k)[row * HD + lane + 32 * i]), s);
-            vv[i] = __bfloat162float(((const __nv_bfloat16 *)a.v)[row * HD + lane + 32 * i]);
+                for (int i = 0; i < 4; ++i) {
+                    s = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ys[i] << 16), s);
+                    s = fmaf(__uint_as_float(xs[i] & 0xffff0000u), __uint_as_float(ys[i] & 0xffff0000u), s);
+                }
+            }
+            s *= a.sl;
         }
+        float best = fmaxf(top, s);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        const float best = fmaxf(top, s), m = best == -INFINITY ? 0.f : best, keep = exp2f(top - m), e = exp2f(s - m);
-        sum = sum * keep + e;
+        for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+        const float m = best == -INFINITY ? 0.f : best, keep = exp2f(top - m), e = lane < n ? exp2f(s - m) : 0.f;
+        float here = e;
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] = fmaf(e, vv[i], acc[i] * keep);
+        for (int o = 16; o > 0; o >>= 1) here += __shfl_xor_sync(0xffffffffu, here, o);
+        sum = sum * keep + here;
         top = best;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] *= keep;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+            const float f = __shfl_sync(0xffffffffu, e, j);
+            const __nv_bfloat16 *v = (const __nv_bfloat16 *)a.v + __shfl_sync(0xffffffffu, row, j) * HD + lane;
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] = fmaf(f, __bfloat162float(v[32 * i]), acc[i]);
+        }
     }
     const float f = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll

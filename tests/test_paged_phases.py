@@ -33,9 +33,13 @@ def at_any_piece(n, j, first):
     return n == 2 and first > 0
 
 
-def roles(pieces, slots, waits, cleared="behind scores"):
+LONG = "a row is computed again"
+
+
+def roles(pieces, slots, waits, cleared="behind scores", again=None):
     """Generators that yield the (barrier, phase) they wait for.  A piece: tiles of keys that either tile of rows looks at, the last of them partial.  The
-    softmax clears what lies behind a partial tile's keys in its slot of the ring, `cleared` "behind scores" or "ahead of scores"."""
+    softmax clears what lies behind a partial tile's keys in its slot of the ring, `cleared` "behind scores" or "ahead of scores".  `again`: where the first
+    tile's softmax stays for as long as it takes, "in its piece" (the first) or "behind all"."""
     full, empty = [Barrier(1) for _ in range(slots)], [Barrier(2) for _ in range(slots)]
     qfull, sfull, sfree, pfull, odone = ([Barrier(1), Barrier(1)] for _ in range(5))
 
@@ -98,6 +102,10 @@ def roles(pieces, slots, waits, cleared="behind scores"):
             if piece[g]:
                 yield odone[g], scored - 1
             n += max(piece)
+            if g == 0 and again == "in its piece":
+                yield LONG
+        if g == 0 and again == "behind all":
+            yield LONG
 
     return [producer(), products(0), products(1), softmax(0), softmax(1)]
 
@@ -119,6 +127,9 @@ def comes_to_an_end(pieces, slots, waits, pick, **kw):
         try:
             live[i] = live[i][0], next(live[i][0])
         except StopIteration:
+            del live[i]
+            continue
+        if live[i][1] == LONG:   # for good, as far as the others' bounded waits go
             del live[i]
     return True
 
@@ -156,3 +167,9 @@ def test_a_slot_cleared_ahead_of_its_scores_would_be_another():
         with pytest.raises(WrongPhase):
             comes_to_an_end(pieces, 4, as_it_is, ahead, cleared="ahead of scores")
         assert comes_to_an_end(pieces, 4, as_it_is, ahead)
+
+
+def test_no_role_waits_for_a_row_that_is_computed_again():
+    for pieces in LISTS:
+        assert comes_to_an_end(pieces, 4, as_it_is, max, again="behind all")
+    assert not comes_to_an_end([(2, 2)] * 4, 4, as_it_is, max, again="in its piece")
