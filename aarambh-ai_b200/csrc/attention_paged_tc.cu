@@ -10,7 +10,11 @@
 // Tiles are of 80 keys because scores (80 columns) and weights (40) of two tiles of rows then fit beside their sums of 128 dimensions in the 512
 // columns of tensor memory: the scores of the next tile are made while the weights of this one are.  An MMA of 80 keys reads shared memory as fast as
 // it goes (419 clocks for 128 rows, 512 for 128 keys: 1.3 of the time a key; with the sums 716 a tile of 80, 1.12).
-// The weights enter rounded to bf16, half a step (2^-8) each and independent, which the sum over the keys averages; their sum is that of the f32
+// The weights of chunks enter rounded to bf16, half a step (2^-8) each and independent, which the sum over the keys averages: 2.3e-3 of the norm, where the
+// output's own rounding is 1.66e-3.  A second term of what rounding left would take a second product with V, and tiles of 64 keys, so that both terms fit
+// tensor memory: 4096 tokens behind 12288 took 1140 to 1170 us so for 915, six mixed rows 156 for 130, with the sums' error gone.  Items of up to 16 query rows, which
+// alone would go to the warp-level kernel and its two terms, have both here too, at no product more: their rows lie twice among the 128 of a tile, the second
+// time with the second term, and the two rows of sums are added (the six mixed rows 133.5 us for 130.5).  So a token's precision does not hang on who shares its batch.  The sum of the weights is that of the f32
 // weights.  Scores, maxima, sums and O are f32.  The weights are relative to a maximum per row that moves only when a score exceeds it by 2^8; then O is
 // rescaled in tensor memory.
 //
@@ -41,6 +45,7 @@ namespace {
 constexpr int PC_Q = 128, PC_KEYS = 80, PC_THREADS = 384;
 constexpr int PC_QBOX = PC_Q * 128, PC_BOX = PC_KEYS * 128;   // boxes of queries, and of keys or values: rows of 64 elements
 constexpr int PC_ROWS = 16;   // that one copy brings: the least that a page holds
+constexpr int PC_TWICE = 16;  // query rows of an item up to which it has each of them twice, for both terms of its weights
 constexpr float PC_SLACK = 8.f;  // powers of two a score may exceed the row's maximum by
 constexpr float PC_NONE = -1e30f;
 
@@ -114,10 +119,11 @@ struct PcShared {
     PcPiece piece[8][2];
 };
 
-// One tile of keys for the warp's 32 rows, a lane each: scores to weights.  With EDGE keys past `lim` are out of sight.  `before` waits until the
+// One tile of keys for the warp's 32 rows, a lane each: scores to weights.  With EDGE keys past `lim` are out of sight, and a lane that is `second` hands on what
+// rounding left of each weight (a kind of its own for that cost the loops around it 5 %).  `before` waits until the
 // products with the tile before are done: its weights' place is free then, and the sums stand still.
 template <int HD, bool EDGE, class Before>
-__device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, bool has_o, float &top, float &sum, uint64_t *taken, uint64_t *ready, Before before) {
+__device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, bool second, bool has_o, float &top, float &sum, uint64_t *taken, uint64_t *ready, Before before) {
     uint32_t va[32], vb[32], vc[16];
     tmem_ld32_start(va, s_addr);
     tmem_ld32_start(vb, s_addr + 32);
@@ -165,7 +171,12 @@ __device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, flo
         const uint64_t e = ex2_pair(fma2(pair(__uint_as_float(v(k)), __uint_as_float(v(k + 1))), sl2, top2));
         total[(k >> 1) & 1] = add2(total[(k >> 1) & 1], e);
         const __nv_bfloat162 b = __floats2bfloat162_rn(low(e), high(e));
-        return *reinterpret_cast<const uint32_t *>(&b);
+        uint32_t word = *reinterpret_cast<const uint32_t *>(&b);
+        if (EDGE) {
+            const __nv_bfloat162 left = __floats2bfloat162_rn(low(e) - __uint_as_float(word << 16), high(e) - __uint_as_float(word & 0xffff0000u));
+            if (second) word = *reinterpret_cast<const uint32_t *>(&left);
+        }
+        return word;
     };
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -349,9 +360,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const PagedSpan s = x.s;
             const long long first = x.w.r.first + s.t0, head0 = x.w.head * group;
             const int i0 = threadIdx.x & 127, rows = s.ntok * group;
+            const bool twice = rows <= PC_TWICE;
 #pragma unroll
             for (int u = 0; u < PC_Q * HD / 8 / 128; ++u) {
-                const int i = i0 + 128 * u, d = i % (HD / 8), row = i / (HD / 8), rr = g * PC_Q + row, in = rr < rows ? 16 : 0, tok = paged_token(a.plan, in ? rr : 0);
+                const int i = i0 + 128 * u, d = i % (HD / 8), row = i / (HD / 8), rr = twice && row < 2 * PC_TWICE ? row % PC_TWICE : g * PC_Q + row, in = rr < rows ? 16 : 0, tok = paged_token(a.plan, in ? rr : 0);
                 const __nv_bfloat16 *src = (const __nv_bfloat16 *)a.q + (first + tok) * a.q_stride + (head0 + (in ? rr - tok * group : 0)) * HD + d * 8;
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(sptr(qbuf + g * S::QTILE + (d >> 3) * PC_QBOX + row * 128 + (((d & 7) ^ (row & 7)) << 4))), "l"(src), "r"(in) : "memory");
             }
@@ -368,7 +380,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.qfull[g]);
             }
-            const int rr = g * PC_Q + r, tok = paged_token(a.plan, rr), pos = rr < rows ? x.s.base + x.s.t0 + tok : -1;
+            const bool twice = rows <= PC_TWICE;   // and this the first tile of rows
+            const bool second = twice && (lane & PC_TWICE);
+            const int rr = g * PC_Q + r, asks = twice && r < 2 * PC_TWICE ? r % PC_TWICE : rr, pos = asks < rows ? x.s.base + x.s.t0 + paged_token(a.plan, asks) : -1;
             const int least = x.s.base + x.s.t0 + paged_token(a.plan, g * PC_Q);   // the first row sees up to here
             float top = PC_NONE, sum = 0.f;
             for (int j = 0; j < tiles; ++j, ++scored) {
@@ -390,8 +404,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                 const int lim = min(pos, hi - 1) - at;
                 auto before = [&] { if (j > 0) warp_wait(&sh.odone[g], (scored - 1) & 1, failed); };
-                if (at + PC_KEYS - 1 > least || at + PC_KEYS > hi || (g + 1) * PC_Q > rows) pc_softmax<HD, true>(s_addr, o_addr, sl, flip, lim, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
-                else pc_softmax<HD, false>(s_addr, o_addr, sl, flip, lim, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
+                if (at + PC_KEYS - 1 > least || at + PC_KEYS > hi || (g + 1) * PC_Q > rows) pc_softmax<HD, true>(s_addr, o_addr, sl, flip, lim, second, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
+                else pc_softmax<HD, false>(s_addr, o_addr, sl, flip, lim, false, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
             }
             // the scores are all made: the next piece's queries may take the place of these, while the sums go out
             more = next();
@@ -422,6 +436,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 if (tiles == 0)
 #pragma unroll
                     for (int k = 0; k < 32; ++k) v[k] = 0u;
+                if (twice)   // both terms' sums
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) + __shfl_xor_sync(0xffffffffu, __uint_as_float(v[k]), PC_TWICE));
 #pragma unroll
                 for (int k = 0; k < 32; ++k) {
                     const float y = __uint_as_float(v[k]) * f;
