@@ -5,10 +5,11 @@
 //   z <- z + bias_v                        where v is biased
 //   z <- -inf                              where the row's mask has v's bit 0
 //
-// in f32, rounded once.  A CTA has a slice of a row's vocabulary: it counts the history's tokens of its slice in shared memory (integer
-// additions, whose order changes nothing), notes which entry of the bias list is each token's last, and then passes over
-// the slice once, 16 bytes a load; a bit for each token says whether there is anything to look up for it.  Every CTA of a row reads the row's history, from L2 after the first.  Bound by HBM for large
-// batches, by the launch, the clearing of the counts and the history's latency for small ones.
+// each step in f32, the result rounded to the logits' type.  A CTA has a slice of a row's vocabulary: it counts the history's tokens of its slice in shared memory
+// (integer additions, whose order changes nothing) and notes which entry of the bias list is each token's last, with a bit for each token that says whether there is
+// anything to look up for it.  Then it passes over the slice twice: 16 bytes a load, storing logits as they are and -inf where the mask says so; and again over the
+// words of those bits, changing the few tokens that the history or the biases touch.  Every CTA of a row reads the row's history, from L2 after the first.  Bound
+// by HBM for large batches, by the launch, the clearing of the counts and the history's latency for small ones.
 #include <algorithm>
 
 #include "common.cuh"
@@ -76,9 +77,18 @@ __global__ void __launch_bounds__(LG_THREADS, LG_CTAS) adjust_logits_kernel(cons
         atomicOr(touched + (v >> 5), 1u << (v & 31));
     }
     if (PACKED && a.biases) __syncthreads();   // the counts come below the entries
-    float rho = 1.f, presence = 0.f, frequency = 0.f;
+    float rho = 1.f, presence = 0.f, frequency = 0.f, inverse = 1.f, half0 = 1.f, half1 = 1.f;
     if (a.history) {
         rho = a.rules[3 * row]; presence = a.rules[3 * row + 1]; frequency = a.rules[3 * row + 2];
+        // A quotient of f32 logits is rounded once.  Logits of 16 bits are multiplied by the reciprocal of the penalty's significand and by its power of two in halves,
+        // which no penalty takes out of range; the second rounding (2^-24) is nothing beside theirs.  Made here, while the history is on its way (64 x 128256 in bf16 16.7 us;
+        // behind it 18.2, with a division 18.4).
+        if constexpr (sizeof(T) == 2) {
+            int power;
+            inverse = 1.f / frexpf(rho, &power);
+            half0 = ldexpf(1.f, -power >> 1);
+            half1 = ldexpf(1.f, -power - (-power >> 1));
+        }
         const int *h = a.history + row * a.history_stride;
         const int len = min(a.lengths ? a.lengths[row] : a.history_width, a.history_width);
         auto count = [&](int v) {
@@ -127,13 +137,14 @@ __global__ void __launch_bounds__(LG_THREADS, LG_CTAS) adjust_logits_kernel(cons
     }
     __syncthreads();   // the tables are whole, and the tokens stored
     // then the tokens that are in one, where the mask allows them (what has been stored is their logit): a word of 32 tokens a thread
-    const float *bias = a.bias_values + (size_t)row * a.biases, inverse = 1.f / rho;
+    const float *bias = a.bias_values + (size_t)row * a.biases;
+    auto divided = [&](float z) { return sizeof(T) == 4 ? z / rho : z * half0 * inverse * half1; };
     for (int w = threadIdx.x; w * 32 < n; w += LG_THREADS)
         for (uint32_t left = touched[w] & (mask ? mask[w] : 0xffffffffu); left; left &= left - 1) {
             const int i = w * 32 + __ffs(left) - 1, word = counts[i], count = PACKED ? word & ((1 << LG_COUNT) - 1) : word;
             const unsigned k = (unsigned)entry[i] >> ENTRY;
             float z = to_f32(out[i]);
-            if (count > 0) z = (z > 0.f ? z * inverse : z * rho) - (presence + frequency * (float)count);
+            if (count > 0) z = (z > 0.f ? divided(z) : z * rho) - (presence + frequency * (float)count);
             if (k) z += bias[k - 1];
             out[i] = from_f32<T>(z);
         }

@@ -403,7 +403,7 @@ int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long long q_s
  * ids outside the vocabulary are passed over) and rules_dev [rows][3] = {repetition > 0, presence, frequency}: where c > 0, z = z > 0 ? z /
  * repetition : z * repetition, then z -= presence + frequency c.  Then z += bias_values[row][i] at bias_ids[row][i] ([rows][biases]; of an id
  * named twice the last counts, ids outside the vocabulary are passed over), and z = -inf where bit v % 32 of allowed_dev [rows][ceil(vocab / 32)]
- * word v / 32 is 0 (NULL: all are allowed).  In f32, rounded once. */
+ * word v / 32 is 0 (NULL: all are allowed).  Each step in f32, the result rounded to the logits' type. */
 int ab2_adjust_logits(const void *logits_dev, long long stride, int rows, int vocab, const int *history_dev, long long history_stride, int history_width,
                       const int *lengths_dev, const float *rules_dev, const int *bias_ids_dev, const float *bias_values_dev, int biases, const uint32_t *allowed_dev,
                       void *out_dev, ab2_dtype dtype, ab2_stream stream);
