@@ -46,7 +46,8 @@ __device__ __forceinline__ unsigned long long turns_per_position(double f) {
     return __double2ull_rn((t - floor(t)) * 18446744073709551616.0);
 }
 // cos and sin of `a` 2^-64 turns, times m.  The nearest quarter turn goes by the top bits; what is left, an eighth of a turn at most either way,
-// keeps 29 bits as a float.
+// is a whole number of up to 2^29 units of 2^-31 half turns, and keeps 24 bits as a float: off by 2^4 units at most there, 2^-25.3 radians (cutting the bits below a
+// unit off takes 2^-29.3 more).
 __device__ __forceinline__ void turn_cos_sin(unsigned long long a, float m, float &c, float &s) {
     const unsigned q = (unsigned)((a + (1ull << 61)) >> 62);
     const int left = (int)((long long)(a - ((unsigned long long)q << 62)) >> 32);
