@@ -392,11 +392,15 @@ AB2_API int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long 
     AB2_REQUIRE(max_new > 0, AB2_ERR_BAD_SHAPE, "rows of at most %d new tokens", max_new);
     if (cache->tokens == 0) return AB2_OK;
     AB2_REQUIRE(q_dev && out_dev, AB2_ERR_BAD_ARG, "null argument");
-    AB2_REQUIRE(q_dev != out_dev, AB2_ERR_BAD_ARG, "the outputs may not take the queries' place");   // a query may be read after outputs have been written
     const long long row = (long long)heads * cache->head_dim;
     AB2_REQUIRE(q_stride >= row && out_stride >= row, AB2_ERR_BAD_SHAPE, "a token's heads lie one after the other, and tokens do not overlap");
     const size_t esize = dtype_size(dtype);
     AB2_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev | (uintptr_t)workspace_dev) & 15) == 0 && ((q_stride | out_stride) * esize & 15) == 0, AB2_ERR_BAD_ALIGN, "queries, outputs and their rows must be 16-byte aligned");
+    // a query, key or value may be read after outputs have been written
+    const long long es = (long long)esize, pool = (long long)cache->pages * cache->page_size * cache->kv_heads * cache->head_dim * es;
+    const RowsAt o_at = {out_dev, row * es, out_stride * es, cache->tokens};
+    AB2_REQUIRE(!rows_meet(o_at, {q_dev, row * es, q_stride * es, cache->tokens}) && !rows_meet(o_at, {cache->k_pages, pool, pool, 1}) && !rows_meet(o_at, {cache->v_pages, pool, pool, 1}), AB2_ERR_BAD_ARG,
+                "the outputs may not take the place of queries or pages");
     PagedAttnArgs a = {};
     a.plan.p = paged_view(cache);
     a.q = q_dev; a.k = cache->k_pages; a.v = cache->v_pages; a.out = out_dev; a.q_stride = q_stride; a.o_stride = out_stride;

@@ -116,6 +116,32 @@ __device__ __forceinline__ float f16_bits_to_f32(uint16_t b) {
 
 static inline size_t dtype_size(ab2_dtype d) { return d == AB2_F32 ? 4 : 2; }
 
+// Rows of `row` bytes, `step` bytes from one to the next (row or more), as a call's arguments name them.
+struct RowsAt {
+    const void *p;
+    long long row, step, n;
+    uintptr_t begin(long long i) const { return (uintptr_t)p + (uintptr_t)(i * step); }
+    uintptr_t end() const { return begin(n - 1) + (uintptr_t)row; }
+};
+// Whether any byte is of both: parts of one buffer may lie between each other and not meet (q and k of a fused projection).
+static inline bool rows_meet(const RowsAt &a, const RowsAt &b) {
+    if (!a.p || !b.p || a.n <= 0 || b.n <= 0 || a.row <= 0 || b.row <= 0 || a.end() <= b.begin(0) || b.end() <= a.begin(0)) return false;
+    if (a.step == b.step) {   // row j of b begins d bytes behind row j + q of a
+        const long long delta = (long long)((uintptr_t)b.p - (uintptr_t)a.p), q = delta >= 0 ? delta / a.step : -((-delta + a.step - 1) / a.step), d = delta - q * a.step;
+        return (d < a.row && q < a.n && q > -b.n) || (d + b.row > a.step && q + 1 < a.n && q + 1 > -b.n);
+    }
+    for (long long i = 0, j = 0; i < a.n && j < b.n;) {
+        if (a.begin(i) + (uintptr_t)a.row <= b.begin(j)) ++i;
+        else if (b.begin(j) + (uintptr_t)b.row <= a.begin(i)) ++j;
+        else return true;
+    }
+    return false;
+}
+// A result that takes its input's place exactly, or lies apart from it.
+static inline bool in_place_or_apart(const RowsAt &out, const RowsAt &in) {
+    return (out.p == in.p && out.row == in.row && (out.step == in.step || out.n == 1)) || !rows_meet(out, in);
+}
+
 // ---- programmatic dependent launch ------------------------------------------
 // Kernels of the decoder step are launched so that a kernel may start while its
 // predecessor is still draining: everything that does not depend on the

@@ -187,6 +187,8 @@ AB2_API int ab2_adjust_logits(const void *logits_dev, long long stride, int rows
     AB2_REQUIRE(history_width >= 0 && biases >= 0, AB2_ERR_BAD_SHAPE, "history of %d, %d biases", history_width, biases);
     AB2_REQUIRE(history_width == 0 || (history_dev && rules_dev && history_stride >= history_width), AB2_ERR_BAD_ARG, "a history needs its tokens, rows that do not overlap, and rules");
     AB2_REQUIRE(biases == 0 || (bias_ids_dev && bias_values_dev), AB2_ERR_BAD_ARG, "null bias list");
+    const long long es = (long long)dtype_size(dtype);
+    AB2_REQUIRE(in_place_or_apart({out_dev, vocab * es, vocab * es, rows}, {logits_dev, vocab * es, stride * es, rows}), AB2_ERR_BAD_ARG, "the result takes the logits' place, or lies apart from them");
     LogitArgs a = {};
     a.logits = logits_dev; a.out = out_dev; a.stride = stride; a.vocab = vocab;
     if (history_width > 0) { a.history = history_dev; a.history_stride = history_stride; a.history_width = history_width; a.lengths = lengths_dev; a.rules = rules_dev; }

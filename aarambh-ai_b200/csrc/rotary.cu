@@ -308,6 +308,11 @@ AB2_API int ab2_rotary_apply(const void *q_dev, long long q_stride, int heads, c
     const long long row = (long long)heads * head_dim, krow = (long long)kv_heads * head_dim;
     AB2_REQUIRE((long long)(heads + kv_heads) * head_dim < (1ll << 30), AB2_ERR_BAD_SHAPE, "%d and %d heads of %d are too many", heads, kv_heads, head_dim);
     AB2_REQUIRE((heads == 0 || (q_stride >= row && q_out_stride >= row)) && (kv_heads == 0 || (k_stride >= krow && k_out_stride >= krow)), AB2_ERR_BAD_SHAPE, "a token's heads lie one after the other, and tokens do not overlap");
+    const long long es = (long long)dtype_size(dtype);
+    const RowsAt q_at = {heads ? q_dev : nullptr, row * es, q_stride * es, tokens}, k_at = {kv_heads ? k_dev : nullptr, krow * es, k_stride * es, tokens};
+    const RowsAt qo_at = {heads ? q_out_dev : nullptr, row * es, q_out_stride * es, tokens}, ko_at = {kv_heads ? k_out_dev : nullptr, krow * es, k_out_stride * es, tokens};
+    AB2_REQUIRE(in_place_or_apart(qo_at, q_at) && in_place_or_apart(ko_at, k_at) && !rows_meet(qo_at, k_at) && !rows_meet(ko_at, q_at) && !rows_meet(qo_at, ko_at), AB2_ERR_BAD_ARG,
+                "an output takes its input's place, or lies apart from both inputs and the other output");
     RotArgs a = {};
     if (heads) { a.q = q_dev; a.qo = q_out_dev; a.q_stride = q_stride; a.qo_stride = q_out_stride; }
     if (kv_heads) { a.k = k_dev; a.ko = k_out_dev; a.k_stride = k_stride; a.ko_stride = k_out_stride; }
@@ -329,6 +334,12 @@ AB2_API int ab2_paged_append(const ab2_paged *cache, const void *k_dev, long lon
     const long long row = (long long)heads * cache->head_dim, krow = (long long)cache->kv_heads * cache->head_dim;
     AB2_REQUIRE((heads + 2ll * cache->kv_heads) * cache->head_dim < (1ll << 30), AB2_ERR_BAD_SHAPE, "%d and %d heads of %d are too many", heads, cache->kv_heads, cache->head_dim);
     AB2_REQUIRE(k_stride >= krow && v_stride >= krow && (heads == 0 || (q_stride >= row && q_out_stride >= row)), AB2_ERR_BAD_SHAPE, "a token's heads lie one after the other, and tokens do not overlap");
+    const long long es = (long long)dtype_size(dtype), pool = (long long)cache->pages * cache->page_size * krow * es;
+    const RowsAt qo_at = {heads ? q_out_dev : nullptr, row * es, q_out_stride * es, cache->tokens}, kp_at = {cache->k_pages, pool, pool, 1}, vp_at = {cache->v_pages, pool, pool, 1};
+    AB2_REQUIRE(in_place_or_apart(qo_at, {heads ? q_dev : nullptr, row * es, q_stride * es, cache->tokens}) && !rows_meet(qo_at, {k_dev, krow * es, k_stride * es, cache->tokens}) &&
+                    !rows_meet(qo_at, {v_dev, krow * es, v_stride * es, cache->tokens}),
+                AB2_ERR_BAD_ARG, "the rotated queries take the queries' place, or lie apart from queries, keys and values");
+    AB2_REQUIRE(!rows_meet(kp_at, vp_at) && !rows_meet(qo_at, kp_at) && !rows_meet(qo_at, vp_at), AB2_ERR_BAD_ARG, "pages of keys, pages of values and the rotated queries lie apart");
     RotArgs a = {};
     a.k = k_dev; a.v = v_dev; a.k_stride = k_stride; a.v_stride = v_stride;
     if (heads) { a.q = q_dev; a.qo = q_out_dev; a.q_stride = q_stride; a.qo_stride = q_out_stride; }

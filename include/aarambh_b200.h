@@ -365,7 +365,7 @@ typedef enum {
     AB2_ROTARY_INTERLEAVED = 1 /* pairs (2 i, 2 i + 1) */
 } ab2_rotary_layout;
 /* q [tokens][heads][head_dim] and k [tokens][kv_heads][head_dim] of element type `dtype` (either may have 0 heads), tokens
- * `*_stride` elements apart, to the same shapes; an output may be its input.  positions_dev [tokens], i32 or (positions_64) i64. */
+ * `*_stride` elements apart, to the same shapes; an output takes its input's place, or lies apart from all of them.  positions_dev [tokens], i32 or (positions_64) i64. */
 int ab2_rotary_apply(const void *q_dev, long long q_stride, int heads, const void *k_dev, long long k_stride, int kv_heads, int head_dim,
                      const void *positions_dev, int positions_64, int tokens, const double *frequencies_dev, int rot_dims, int layout, float magnitude,
                      void *q_out_dev, long long q_out_stride, void *k_out_dev, long long k_out_stride, ab2_dtype dtype, ab2_stream stream);
@@ -384,13 +384,13 @@ typedef struct {
     long long table_stride;   /* entries from a row of the table to the next, table_width or more */
 } ab2_paged;
 /* Writes k (rotated at its position in the row; rot_dims 0: as it is) and v of the new tokens to their pages, and with heads > 0 the
- * rotated q to q_out_dev, in one launch; q_out_dev may be q_dev.  A token without a place (a row with more new tokens than tokens, a page
+ * rotated q to q_out_dev, in one launch; q_out_dev may be q_dev, and lies apart from all else.  Pages of keys and of values do not overlap.  A token without a place (a row with more new tokens than tokens, a page
  * outside the pool) is not written, and reported as above. */
 int ab2_paged_append(const ab2_paged *cache, const void *k_dev, long long k_stride, const void *v_dev, long long v_stride, const void *q_dev, long long q_stride,
                      int heads, void *q_out_dev, long long q_out_stride, const double *frequencies_dev, int rot_dims, int layout, float magnitude, ab2_dtype dtype, ab2_stream stream);
 /* Attention of the new tokens, whose keys and values have been appended: a token sees its row's keys up to its own position, query head
  * j reads KV head j / (heads / kv_heads), up to 32 query heads for one KV head; a token that sees no key answers zeros.  out_dev
- * must not overlap q_dev.  Keys and values out of
+ * must not overlap q_dev or the pages.  Keys and values out of
  * sight may hold anything.  max_new (at least the most new tokens of a row) picks kernels; rows that have more are
  * answered all the same.  workspace_dev
  * (ab2_paged_workspace bytes, 16-byte aligned, nothing in it is kept between calls) lets long rows be cut between CTAs; NULL: they are not. */
@@ -399,7 +399,7 @@ int ab2_paged_workspace(int head_dim, size_t *bytes);
 int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long long q_stride, int heads, void *out_dev, long long out_stride, int max_new, float scale,
                         void *workspace_dev, size_t workspace_bytes, ab2_dtype dtype, ab2_stream stream);
 /* Rules of a sampler on logits [rows][vocab] (`stride` elements from row to row) to out_dev [rows][vocab], which may be the logits where
- * stride = vocab.  With c the times a token occurs in history_dev [rows][history_width] (i32, the first lengths_dev[row] of a row or, NULL, all;
+ * stride = vocab, and lies apart from them otherwise.  With c the times a token occurs in history_dev [rows][history_width] (i32, the first lengths_dev[row] of a row or, NULL, all;
  * ids outside the vocabulary are passed over) and rules_dev [rows][3] = {repetition > 0, presence, frequency}: where c > 0, z = z > 0 ? z /
  * repetition : z * repetition, then z -= presence + frequency c.  Then z += bias_values[row][i] at bias_ids[row][i] ([rows][biases]; of an id
  * named twice the last counts, ids outside the vocabulary are passed over), and z = -inf where bit v % 32 of allowed_dev [rows][ceil(vocab / 32)]
