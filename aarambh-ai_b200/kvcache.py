@@ -9,7 +9,7 @@ layers, snapshot / restore).  Storage is f32, bf16 or per-token-per-head INT8.
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -132,12 +132,16 @@ class PagedStep:
     tokens: int                   # that q, k and v have room for
     max_new: int
     packed: torch.Tensor          # the three above
+    before: list = field(default_factory=list)   # tokens of each row without the new ones
+    cuts: list = field(default_factory=list)     # how often each row had been cut back, and all rows together
+    all_cuts: int = 0
 
 
 class PagedKVCache:
     """Keys and values in pages of one pool that the sequences share: a sequence holds as many as its tokens need, in any order, where
     ``KVCache`` gives each the same capacity for good.  ``k`` and ``v`` are [layers, pages, kv_heads, page_size, head_dim] (f32 or bf16).
-    A pass over some rows: ``step`` takes the pages it needs, then for every layer ``append`` and ``attention``, at its end ``commit``.
+    A pass over some rows: ``step`` takes the pages it needs, then for every layer ``append`` and ``attention``, at its end ``commit``.  A step whose rows
+    have been cut back or have moved on since is refused: its pages may be another row's.
     Calls on a cache go on one stream, or are ordered by the caller."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, batch: int = 1, n_layers: int = 1, dtype: str = "bf16", device="cuda"):
@@ -153,6 +157,7 @@ class PagedKVCache:
         self._free = list(range(pages - 1, -1, -1))
         self._pages = [[] for _ in range(batch)]
         self._lens = [0] * batch
+        self._cuts, self._all_cuts = [0] * batch, 0
 
     def _row(self, row: int) -> int:
         if not 0 <= row < self.batch:
@@ -205,28 +210,33 @@ class PagedKVCache:
             flat += self._pages[r] + [0] * (width - len(self._pages[r]))
         into.packed.copy_(torch.tensor(flat, dtype=torch.int32))
         into.rows, into.new = rows, new
+        into.before, into.cuts, into.all_cuts = [self._lens[r] for r in rows], [self._cuts[r] for r in rows], self._all_cuts
         return into
 
     def append(self, step: PagedStep, k: torch.Tensor, v: torch.Tensor, layer: int = 0, q: torch.Tensor | None = None, frequencies=None, layout: str = "half",
                magnitude: float = 1.0, out: torch.Tensor | None = None):
         """``dispatch.paged_append`` on a layer: k, v (and q) [step.tokens, heads, dim]."""
         from .dispatch import paged_append
-        self._fits(step, k)
+        self._holds(step, k)
         return paged_append(self.k[layer], self.v[layer], k, v, step.table, step.lens, step.starts, q, frequencies, layout, magnitude, out)
 
     def attention(self, step: PagedStep, q: torch.Tensor, scale: float, layer: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
         """``dispatch.attention_paged`` on a layer: q [step.tokens, heads, dim]."""
         from .dispatch import attention_paged
-        self._fits(step, q)
+        self._holds(step, q)
         return attention_paged(q, self.k[layer], self.v[layer], step.table, step.lens, scale, step.starts, step.max_new, out)
 
-    @staticmethod
-    def _fits(step, t):
-        if t.shape[0] < step.tokens:
+    def _holds(self, step, t=None):
+        if t is not None and t.shape[0] < step.tokens:
             raise _lib.Ab2Error(-1, f"a step of {step.tokens} tokens over a tensor of {t.shape[0]}")
+        if step.all_cuts != self._all_cuts and step.cuts != [self._cuts[r] for r in step.rows]:
+            raise _lib.Ab2Error(-7, f"rows {[r for r, c in zip(step.rows, step.cuts) if c != self._cuts[r]]} were cut back behind the step's making: it needs to be made anew")
 
     def commit(self, step: PagedStep) -> None:
-        """The rows' lengths move on by the step's new tokens."""
+        """The rows' lengths move on by the step's new tokens, once."""
+        self._holds(step)
+        if step.before != [self._lens[r] for r in step.rows]:
+            raise _lib.Ab2Error(-7, f"rows {[r for r, n in zip(step.rows, step.before) if n != self._lens[r]]} have moved on since the step was made")
         for r, n in zip(step.rows, step.new):
             self._lens[r] += n
 
@@ -235,6 +245,8 @@ class PagedKVCache:
         if not 0 <= new_len <= self.seq_len(row):
             raise _lib.Ab2Error(-4, f"row {row} holds {self.seq_len(row)} tokens and cannot be cut to {new_len}")
         self._lens[row] = new_len
+        self._cuts[row] += 1
+        self._all_cuts += 1
         keep = -(-new_len // self.page_size)
         self._free += self._pages[row][:keep - 1 if keep else None:-1]
         del self._pages[row][keep:]
