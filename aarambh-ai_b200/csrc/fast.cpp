@@ -46,6 +46,7 @@ int dtype_of(const at::Tensor &t) {
 }
 int layout_of(PyObject *o) {
     const char *s = PyUnicode_Check(o) ? PyUnicode_AsUTF8(o) : nullptr;
+    if (!s) PyErr_Clear();   // of a text that has no UTF-8
     return s && !strcmp(s, "half") ? AB2_ROTARY_HALF : s && !strcmp(s, "interleaved") ? AB2_ROTARY_INTERLEAVED : -1;
 }
 bool is(const at::Tensor *t, at::ScalarType type, std::initializer_list<int64_t> shape) { return t->scalar_type() == type && t->sizes().equals(shape); }
@@ -68,6 +69,9 @@ template <class F> PyObject *guarded(F f) {
         return f();
     } catch (const std::exception &e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    } catch (...) {
+        PyErr_SetString(PyExc_RuntimeError, "an exception of unknown type");
         return nullptr;
     }
 }
