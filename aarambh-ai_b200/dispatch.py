@@ -470,9 +470,11 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
 def allowed_words(mask: torch.Tensor) -> torch.Tensor:
     """A truth value for every token [rows, vocab] as the words that ``adjust_logits`` takes: int32 [rows, ceil(vocab / 32)]."""
+    if mask.dim() != 2:
+        raise _lib.Ab2Error(-1, f"a mask must be [rows, vocab], got {list(mask.shape)}")
     rows, vocab = mask.shape
     bits = torch.zeros((rows, (vocab + 31) // 32 * 32), dtype=torch.int64, device=mask.device)
-    bits[:, :vocab] = mask
+    bits[:, :vocab] = mask != 0
     words = (bits.view(rows, -1, 32) << torch.arange(32, device=mask.device)).sum(-1)
     return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
 
