@@ -14,6 +14,7 @@ sampler.rs:217-224); text, tools and stochastic samplers stay with the caller.
 """
 from __future__ import annotations
 
+import math
 from collections.abc import Callable
 from dataclasses import dataclass, field
 
@@ -167,6 +168,8 @@ class SessionEngine:
         if session.rules is not None:
             logits = session.rules.apply(logits, session.prompt_ids, session.generated_ids)
         token = int(argmax(logits)[0])
+        if session.rules is not None and session.rules.allowed is not None and float(logits[0, token]) == -math.inf:
+            raise _lib.Ab2Error(-7, "no token that the session's rules allow has a logit above -inf")
         session.generated_ids.append(token)
         if len(session.generated_ids) >= session.max_new_tokens or token == session.eos_token_id:
             session.finished = True
