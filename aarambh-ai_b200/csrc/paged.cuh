@@ -8,6 +8,8 @@ namespace ab2 {
 int device_status_word(int **out);
 int device_sm_count();
 
+// What deals work out is compiled for the host too, where tests/test_paged_plan.py runs it over batches of all kinds.
+
 // What a ragged batch of new tokens says of a row, with everything that device memory could hold brought within bounds: row b's new tokens
 // are [first, first + count) of q, k and v, and its last one is at position len - 1.
 struct PagedRow {
@@ -18,8 +20,14 @@ struct PagedView {
     long long table_stride;
     int rows, tokens, width, pages, page_shift, kv_heads;
 };
-__device__ __forceinline__ void paged_bad(int *status) { atomicCAS(status, 0, (int)AB2_ERR_BAD_ARG); }
-__device__ __forceinline__ PagedRow paged_row(const PagedView &p, int b, int *status) {
+__host__ __device__ __forceinline__ void paged_bad(int *status) {
+#ifdef __CUDA_ARCH__
+    atomicCAS(status, 0, (int)AB2_ERR_BAD_ARG);
+#else
+    *status = (int)AB2_ERR_BAD_ARG;
+#endif
+}
+__host__ __device__ __forceinline__ PagedRow paged_row(const PagedView &p, int b, int *status) {
     PagedRow r;
     const int s0 = p.starts ? p.starts[b] : b, s1 = p.starts ? p.starts[b + 1] : b + 1, len = p.lens[b];
     r.first = min(max(s0, 0), p.tokens);
@@ -71,14 +79,14 @@ struct PagedPlan {
     int least;                  // units that are worth a CTA
     int per_group;              // 2^16 / group, rounded up: r / group is r per_group / 2^16 for rows r of a tile (at most 256) and groups up to 32
 };
-__device__ __forceinline__ int paged_token(const PagedPlan &a, int r) { return (r * a.per_group) >> 16; }
+__host__ __device__ __forceinline__ int paged_token(const PagedPlan &a, int r) { return (r * a.per_group) >> 16; }
 struct PagedShape {
     int q_tiles, base;          // of the row; keys before its new tokens
     long long per;              // units of a head
     long long units;
 };
 // Units of the first n tiles of a row's queries: the sum over i < n of ceil((base + (i + 1) tq) / keys), both powers of two.
-__device__ __forceinline__ long long paged_units(const PagedPlan &a, int base, long long n) {
+__host__ __device__ __forceinline__ long long paged_units(const PagedPlan &a, int base, long long n) {
     if (a.whole) return n;
     const int s = a.key_shift - a.tq_shift;
     if (s <= 0) return n * (((long long)base + (1 << a.key_shift) - 1) >> a.key_shift) + ((n * (n + 1) / 2) << -s);
@@ -87,7 +95,7 @@ __device__ __forceinline__ long long paged_units(const PagedPlan &a, int base, l
     auto floors = [&](long long y) { const long long q = y >> s; return (q * (q - 1) / 2 << s) + q * (y & ((1ll << s) - 1)); };
     return floors(c + n) - floors(c);
 }
-__device__ __forceinline__ PagedShape paged_shape(const PagedPlan &a, const PagedRow &r) {
+__host__ __device__ __forceinline__ PagedShape paged_shape(const PagedPlan &a, const PagedRow &r) {
     PagedShape s = {0, 0, 0, 0};
     const long long rows = (long long)r.count * a.group;
     if (rows <= a.above || rows > a.most) return s;
@@ -132,13 +140,41 @@ struct PagedRun {
     int q_tiles, base;
 };
 // a / b of numbers that are not negative: in 32 bits, a fifth of the time, where they fit.
-__device__ __forceinline__ long long paged_div(long long a, long long b) {
+__host__ __device__ __forceinline__ long long paged_div(long long a, long long b) {
     return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
 }
 // Where the run of CTA c begins.
-__device__ __forceinline__ long long paged_begin(const PagedRun &run, int c) { return paged_div(run.total * min(c, run.ctas), run.ctas); }
-__device__ __forceinline__ int paged_keys(const PagedPlan &a, int base, int q_tile) {   // units of a tile of queries
+__host__ __device__ __forceinline__ long long paged_begin(const PagedRun &run, int c) { return paged_div(run.total * min(c, run.ctas), run.ctas); }
+__host__ __device__ __forceinline__ int paged_keys(const PagedPlan &a, int base, int q_tile) {   // units of a tile of queries
     return a.whole ? 1 : (int)(((long long)base + ((long long)(q_tile + 1) << a.tq_shift) + (1 << a.key_shift) - 1) >> a.key_shift);
+}
+// Unit `in` of a row: its head, the tile of queries it is of, and which of that tile's.
+struct PagedUnit {
+    int head, q_tile, k;
+};
+__host__ __device__ __forceinline__ PagedUnit paged_find(const PagedPlan &a, const PagedShape &s, long long in) {
+    const int head = (int)paged_div(in, s.per);
+    const long long y = in - head * s.per;
+    int lo = 0, hi = s.q_tiles - 1;   // the tile that unit y of the head is of
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (paged_units(a, s.base, mid) <= y) lo = mid;
+        else hi = mid - 1;
+    }
+    return {head, lo, (int)(y - paged_units(a, s.base, lo))};
+}
+// Puts the run at that unit.
+__host__ __device__ __forceinline__ void paged_at(const PagedPlan &a, PagedRun &run, int row, const PagedUnit &u) {
+    run.row = row; run.head = u.head; run.q_tile = u.q_tile; run.k = u.k;
+    run.r = paged_row(a.p, row, nullptr);
+    const PagedShape s = paged_shape(a, run.r);
+    run.q_tiles = s.q_tiles;
+    run.base = s.base;
+    run.k_tiles = paged_keys(a, run.base, run.q_tile);
+}
+__host__ __device__ __forceinline__ int paged_ctas(const PagedPlan &a, long long total, int ctas) {   // that have any of `total` units
+    const long long n = paged_div(total, a.least);
+    return n < 1 ? 1 : n < ctas ? (int)n : ctas;
 }
 // The run of CTA (or, with THREADS 32, warp) `c` of `ctas`, found by all its threads.  `found` is shared.
 template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const PagedPlan &a, int c, int ctas, long long *warp_sums, int2 *found, int *status) {
@@ -151,7 +187,7 @@ template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const Paged
         if (r0 == 0) { prefix = at; units = here; }
         run.total += n;
     }
-    run.ctas = (int)max(1ll, min((long long)ctas, paged_div(run.total, a.least)));
+    run.ctas = paged_ctas(a, run.total, ctas);
     run.u = paged_begin(run, c);
     run.u1 = paged_begin(run, c + 1);
     if (run.u >= run.u1) return run;
@@ -167,30 +203,17 @@ template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const Paged
             n = run.total;
         }
         if (units > 0 && run.u >= prefix && run.u < prefix + units) {
-            const PagedShape s = paged_shape(a, paged_row(a.p, r0 + (int)(threadIdx.x % THREADS), nullptr));
-            const long long in = run.u - prefix;
-            const int head = (int)paged_div(in, s.per);
-            found[0] = make_int2(r0 + (int)(threadIdx.x % THREADS), head);
-            const long long y = in - head * s.per;
-            int lo = 0, hi = s.q_tiles - 1;   // the tile that unit y of the head is of
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (paged_units(a, s.base, mid) <= y) lo = mid;
-                else hi = mid - 1;
-            }
-            found[1] = make_int2(lo, (int)(y - paged_units(a, s.base, lo)));
+            const int row = r0 + (int)(threadIdx.x % THREADS);
+            const PagedUnit u = paged_find(a, paged_shape(a, paged_row(a.p, row, nullptr)), run.u - prefix);
+            found[0] = make_int2(row, u.head);
+            found[1] = make_int2(u.q_tile, u.k);
         }
         if (run.u < row_first + n) break;
         row_first += n;
     }
     if (THREADS == 32) __syncwarp();
     else __syncthreads();
-    run.row = found[0].x; run.head = found[0].y; run.q_tile = found[1].x; run.k = found[1].y;
-    run.r = paged_row(a.p, run.row, nullptr);
-    const PagedShape s = paged_shape(a, run.r);
-    run.q_tiles = s.q_tiles;
-    run.base = s.base;
-    run.k_tiles = paged_keys(a, run.base, run.q_tile);
+    paged_at(a, run, found[0].x, {found[0].y, found[1].x, found[1].y});
     return run;
 }
 // A piece of work: units [k0, k1) of the item (row, head, q_tile), which has k_tiles of them.
@@ -199,7 +222,7 @@ struct PagedPiece {
     PagedRow r;
 };
 // The next piece of the run; false at its end.  The same for all threads that call it with the same run.
-__device__ __forceinline__ bool paged_next(const PagedPlan &a, PagedRun &run, PagedPiece &w) {
+__host__ __device__ __forceinline__ bool paged_next(const PagedPlan &a, PagedRun &run, PagedPiece &w) {
     if (run.u >= run.u1) return false;
     if (run.k == run.k_tiles) {   // the next item: of the head, of the row, of the next row that has any
         run.k = 0;
@@ -229,7 +252,7 @@ __device__ __forceinline__ bool paged_next(const PagedPlan &a, PagedRun &run, Pa
 struct PagedSpan {
     int t0, ntok, base, lo, hi;
 };
-__device__ __forceinline__ PagedSpan paged_span(const PagedPlan &a, const PagedPiece &w) {
+__host__ __device__ __forceinline__ PagedSpan paged_span(const PagedPlan &a, const PagedPiece &w) {
     PagedSpan s;
     s.t0 = w.q_tile << a.tq_shift;
     s.ntok = min(1 << a.tq_shift, w.r.count - s.t0);
@@ -269,7 +292,7 @@ static inline void paged_deal(PagedAttnArgs &a, int ctas, int tile_rows, int key
 }
 // What run c leaves to the merge, written by one thread: nothing, to begin with, and its last piece if that begins an item and does not end it.
 __device__ __forceinline__ void paged_uncut(const PagedAttnArgs &a, int c) { if (!a.plan.whole) a.cut[c] = make_int4(0, 0, 0, 0); }
-__device__ __forceinline__ void paged_cut(const PagedAttnArgs &a, const PagedRun &run, const PagedPiece &w, const PagedSpan &sp, int c) {
+__host__ __device__ __forceinline__ void paged_cut(const PagedAttnArgs &a, const PagedRun &run, const PagedPiece &w, const PagedSpan &sp, int c) {
     if (w.k0 > 0 || w.k1 == w.k_tiles) return;
     const long long end = run.u + (w.k_tiles - w.k1);   // the unit behind the item: the last run that begins before it ends it
     a.cut[c] = make_int4(w.r.first + sp.t0, sp.ntok, w.head, (int)min((long long)run.ctas - 1, paged_div(end * run.ctas - 1, run.total)));
