@@ -26,9 +26,12 @@ size_t paged_mma_bytes(int hd);
 int paged_mma_attention(const PagedAttnArgs &a, int hd, int max_new, void *workspace, size_t bytes, cudaStream_t s);
 size_t paged_tc_bytes(int hd);
 int paged_tc_attention(const PagedAttnArgs &a, int hd, void *workspace, size_t bytes, cudaStream_t s);
-// A batch of chunks and single tokens: one launch for both up to this many rows, since a launch for the single tokens and its merge cost more than
-// they save (a chunk of 512 among single tokens behind 4000: 8 rows 103 us by two launches, 82 by one; 32 rows 168, 167; 64 rows behind 2000 157, 163).
-constexpr int PAGED_FEW_SEQUENCES = 32;
+// A batch of chunks and single tokens: one launch for both up to this many rows times KV heads, since a launch for the single tokens and its merge cost more than
+// they save; but in the kernel of chunks each of them takes a tile of 128 rows, and loses by its context, which the host does not know.  A chunk of 512 among
+// single tokens, us by two launches and by one: 32 / 8 heads of 128, 32 rows behind 500 65 and 56, behind 4000 168 and 163, behind 16000 487 and 559; 64 rows 82 and 80,
+// 247 and 274; 16 / 1 heads of 128, 128 rows behind 500 57 and 40, behind 4000 118 and 98; 16 / 4 heads of 64, 16 rows behind 500 43 and 29, behind 4000 61 and 62, behind 16000
+// 141 and 178, 32 rows 42 and 33, 80 and 90, 180 and 284.
+constexpr int paged_few_items(int hd) { return hd == 128 ? 256 : 64; }
 constexpr int PAGED_FEW_ROWS = 16;   // query rows of a KV head up to which the tensor-memory kernel's tiles of 128 would be nearly empty
 namespace {
 
@@ -411,7 +414,7 @@ AB2_API int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long 
     if (dtype == AB2_F32) return simt_attention(a, cache->head_dim, max_new, workspace_dev, workspace_bytes, (cudaStream_t)stream);
     // Rows of up to 16 query rows a KV head go to the warp-level kernel, the others to the tensor-memory kernel; a launch for which there can be no row is
     // left out.  Rows with more new tokens than they were said to have are served all the same.
-    const bool chunks = (long long)max_new * a.plan.group > PAGED_FEW_ROWS, few = a.plan.group <= PAGED_FEW_ROWS && !(chunks && cache->rows <= PAGED_FEW_SEQUENCES);
+    const bool chunks = (long long)max_new * a.plan.group > PAGED_FEW_ROWS, few = a.plan.group <= PAGED_FEW_ROWS && !(chunks && (long long)cache->rows * cache->kv_heads <= paged_few_items(cache->head_dim));
     if (few) {
         if (chunks) a.plan.most = PAGED_FEW_ROWS;
         rc = paged_mma_attention(a, cache->head_dim, max_new, workspace_dev, workspace_bytes, (cudaStream_t)stream);

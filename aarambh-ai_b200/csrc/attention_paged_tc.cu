@@ -537,9 +537,9 @@ int launch_tc(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
     if (rc == AB2_OK) rc = pages_map(&vmap, a.v, a.plan.p, HD);
     if (rc != AB2_OK) return rc;
     paged_deal(a, device_sm_count(), 2 * PC_Q, 7, 4, HD, workspace, bytes);
-    // Set up while the launch before it ends, which saves some 1.7 us of any call and costs long ones up to 2 %.  How long a call is lies with the context,
-    // which the host does not know; by its query rows (us not set up early and early, 32 heads of 128): 300 tokens behind 300 34.1 and 32.5, 1024 behind
-    // 1024 52.6 and 50.4, 2048 alone 79.7 and 77.9, behind 12288 442 and 445; 3000 behind 3000 238 and 241, 4096 alone 197 and 195, behind 12288 924 and 943.
+    // Set up while the launch before it ends, up to 65536 query rows: all that were tried gain there, and beyond it none does and the longest loses.  32 heads of 128, us
+    // not set up early and early: 300 tokens behind 300 35.0 and 32.6, behind 16000 103 and 101.4, 1024 behind 1024 53.7 and 51.9, 2048 alone 82.0 and 80.9, behind
+    // 12288 383.8 and 382.6; 3000 behind 3000 231 to 240 and 233 to 237, 4096 alone 207 and 207 to 210, behind 4096 372 and 371, behind 12288 860 to 872 and 876 to 884, 8192 alone 617 and 613 to 621.
     ChainedLaunches chained((long long)a.plan.p.tokens * a.plan.group * a.plan.p.kv_heads <= 65536);
     AB2_CUDA(launch_kernel(paged_tc_kernel<HD>, dim3(a.ctas), dim3(PC_THREADS), S::SMEM, s, kmap, vmap, a));
     return a.plan.whole ? AB2_OK : paged_merge(a, HD, AB2_BF16, s);

@@ -31,9 +31,10 @@ def mixed(rows, heads, kv_heads, dim, page, dtype=BF, ctx=300, chunk=70):
 
 
 @pytest.mark.parametrize("heads,kv_heads,dim,page", [(8, 2, 128, 16), (16, 1, 64, 32), (6, 2, 64, 16), (20, 1, 128, 64)])
-@pytest.mark.parametrize("rows", [31, 32, 33, 34, 64, 425])
+@pytest.mark.parametrize("rows", [31, 32, 33, 34, 64, 65, 128, 129, 425])
 def test_single_tokens_and_chunks_of_many_rows(rows, heads, kv_heads, dim, page):
-    """Up to 32 rows one launch serves all; of more, the few-token rows and the chunks have a launch each, which leave out the other's."""
+    """One launch serves all up to a number of rows (128, 64 and 32 of the first three kinds of heads); of more, the few-token rows and the chunks have a launch each, which
+    leave out the other's."""
     p, b = pkg(), mixed(rows, heads, kv_heads, dim, page)
     n = b.starts_list[-1]
     ref, tol = b.expected()
