@@ -184,6 +184,8 @@ class PagedKVCache:
         rows, new = [int(r) for r in rows], [int(n) for n in new]
         if not rows or len(rows) != len(new) or min(new) < 0 or len(set(rows)) != len(rows):
             raise _lib.Ab2Error(-1, f"a step takes distinct rows and new tokens of each, got rows {rows}, new {new}")
+        if room < 0:
+            raise _lib.Ab2Error(-1, f"room for {room} more tokens")
         for r in rows:
             self._row(r)
         lens = [self._lens[r] + n for r, n in zip(rows, new)]

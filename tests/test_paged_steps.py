@@ -56,3 +56,11 @@ def test_other_rows_may_be_cut():
     c.truncate(3, 2)
     c.commit(s)
     assert [c.seq_len(r) for r in range(3)] == [11, 21, 3]
+
+
+def test_a_table_is_never_narrower_than_its_rows():
+    c = cache()
+    c.commit(c.step([0], [40]))
+    with pytest.raises(pkg().Ab2Error):
+        c.step([0], [30], room=-60)
+    assert c.free_pages() == 8 - 3 and len(c._pages[0]) == 3
