@@ -11,8 +11,8 @@
 // Weights enter as two bf16 terms, the rounded weight and what rounding left: the tensor pipe has time for both, and no rounding but the
 // output's is left.  A row's maximum moves only when a score exceeds it by 2^8.
 //
-// 48 rows of up to 8192 tokens, 32 / 8 heads of 128 (1.02 GB): 170 us with the merge, 0.92 of a copy's rate (on CUDA cores 672); 2 x 100000 128 us
-// (0.89).  1 x 700: 10.3 to 10.9 us (12.3 to 12.7 before a launch was set up while the one before it ended), a kernel of 8 and a merge of 4.3 by themselves:
+// 48 rows of up to 8192 tokens, 32 / 8 heads of 128 (1.02 GB): 170 us with the merge, 0.92 of a copy's rate (on CUDA cores 672); 2 x 100000 128 to 138 us
+// (0.89 to 0.83 by the card).  1 x 700: 10.3 to 10.9 us (12.3 to 12.7 before a launch was set up while the one before it ended), a kernel of 8 and a merge of 4.3 by themselves:
 // latency.  A merge by fewer CTAs, each for the cuts of several runs, took 80 us for 41 at 1 x 32000: cuts lie evenly apart, and met in the same CTAs.
 #include <algorithm>
 

@@ -19,9 +19,9 @@
 // rescaled in tensor memory.
 //
 // 4096 tokens behind 12288, 32 / 8 heads of 128: 0.92 ms, 1.05 PFLOP/s, 0.63 of cuBLAS in a burst and 0.75 of it sustained; 2048 behind 2048 120 us;
-// six rows of 1 to 512 tokens behind up to 5000 126 us.  Bound by the two softmax warps of a scheduler: of the 2300 clocks of a tile of 80 keys they
-// need 1250 for the exponentials (read by clocks in the kernel; both tiles' are 2 x 128 x 80, at 16 a clock 1280), and the rest for scores from
-// tensor memory, the maximum, and the waits for scores and for the last tile's products, some 150 clocks each; the products take 1432.
+// six rows of 1 to 512 tokens behind up to 5000 134 us; 4096 behind 12288, 16 / 4 heads of 64, 0.41 ms.  A tile of 80 keys takes some 2300 clocks, of which both tiles'
+// exponentials (2 x 128 x 80, at 16 a clock) need 1280 and the products 1432; no pipe is full (1024 behind 3072 by counters: exponentials 42 %, tensor pipe 41 %, issue
+// slots 36 %).  What bounds it is the chain of a softmax warp: scores from tensor memory, the maximum, the last tile's products, exponentials, weights back.
 //
 // Measured and not kept, each against the kernel of its day: the tiles' exponentials in turns by a barrier 0.98 ms for 0.91; polynomials for a quarter of
 // them 0.96 for 0.91.  Forms before this one: tiles of 128 keys with the weights over the scores (a chain of scores, softmax and sums) 0.98 to 1.02;
