@@ -20,7 +20,7 @@
 //
 // 4096 tokens behind 12288, 32 / 8 heads of 128: 0.92 ms, 1.05 PFLOP/s, 0.63 of cuBLAS in a burst and 0.75 of it sustained; 2048 behind 2048 120 us;
 // six rows of 1 to 512 tokens behind up to 5000 134 us; 4096 behind 12288, 16 / 4 heads of 64, 0.41 ms.  A tile of 80 keys takes some 2300 clocks, of which both tiles'
-// exponentials (2 x 128 x 80, at 16 a clock) need 1280 and the products 1432; no pipe is full (1024 behind 3072 by counters: exponentials 42 %, tensor pipe 41 %, issue
+// exponentials (2 x 128 x 80, at 16 a clock) need 1280 and the products 1432; no pipe is full (1024 behind 3000 by counters: exponentials 42 %, tensor pipe 42 %, issue
 // slots 36 %).  What bounds it is the chain of a softmax warp: scores from tensor memory, the maximum, the last tile's products, exponentials, weights back.
 //
 // Measured and not kept, each against the kernel of its day: the tiles' exponentials in turns by a barrier 0.98 ms for 0.91; polynomials for a quarter of
