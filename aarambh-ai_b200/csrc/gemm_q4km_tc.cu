@@ -21,7 +21,7 @@
 // With fewer tiles than SMs the blocks of a tile are divided over several CTAs; their f32 sums meet in a reduce pass.
 // What bounds it is the unpack and the per-block epilogue (about 450 cycles a stage against the MMA's 257 at 128
 // tokens).  14336 x 4096 at 300 tokens: 3329 us on CUDA cores,
-// 73 us here (482 TFLOP/s); 3072 x 2048: 421 -> 20 us, at 9 tokens 17 -> 11.
+// 73 us here (482 TFLOP/s).
 // Every wait on an mbarrier is bounded; on a time-out the CTA records AB2_ERR_TIMEOUT, walks through the rest
 // of its work, frees its tensor memory and returns.
 #include <cuda.h>
