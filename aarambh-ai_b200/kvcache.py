@@ -132,7 +132,7 @@ class PagedStep:
     tokens: int                   # that q, k and v have room for
     max_new: int
     packed: torch.Tensor          # the three above
-    before: list = field(default_factory=list)   # tokens of each row without the new ones
+    before: list = field(default_factory=list)   # tokens of each row without the new ones (empty in a step that a caller put together: it is not looked at)
     cuts: list = field(default_factory=list)     # how often each row had been cut back, and all rows together
     all_cuts: int = 0
 
@@ -231,13 +231,13 @@ class PagedKVCache:
     def _holds(self, step, t=None):
         if t is not None and t.shape[0] < step.tokens:
             raise _lib.Ab2Error(-1, f"a step of {step.tokens} tokens over a tensor of {t.shape[0]}")
-        if step.all_cuts != self._all_cuts and step.cuts != [self._cuts[r] for r in step.rows]:
+        if step.all_cuts != self._all_cuts and step.cuts and step.cuts != [self._cuts[r] for r in step.rows]:
             raise _lib.Ab2Error(-7, f"rows {[r for r, c in zip(step.rows, step.cuts) if c != self._cuts[r]]} were cut back behind the step's making: it needs to be made anew")
 
     def commit(self, step: PagedStep) -> None:
         """The rows' lengths move on by the step's new tokens, once."""
         self._holds(step)
-        if step.before != [self._lens[r] for r in step.rows]:
+        if step.before and step.before != [self._lens[r] for r in step.rows]:
             raise _lib.Ab2Error(-7, f"rows {[r for r, n in zip(step.rows, step.before) if n != self._lens[r]]} have moved on since the step was made")
         for r, n in zip(step.rows, step.new):
             self._lens[r] += n

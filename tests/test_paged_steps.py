@@ -64,3 +64,12 @@ def test_a_table_is_never_narrower_than_its_rows():
     with pytest.raises(pkg().Ab2Error):
         c.step([0], [30], room=-60)
     assert c.free_pages() == 8 - 3 and len(c._pages[0]) == 3
+
+
+def test_a_step_that_a_caller_put_together():
+    c = cache()
+    made = c.step([0], [5])
+    own = pkg().PagedStep(made.rows, made.new, made.table, made.lens, made.starts, made.tokens, made.max_new, made.packed)
+    c.truncate(0, 1)
+    c.commit(own)
+    assert c.seq_len(0) == 5
