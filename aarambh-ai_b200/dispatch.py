@@ -438,7 +438,8 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     starts: torch.Tensor | None = None, max_new: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """q [tokens, heads, dim]: each row's new tokens, whose keys and values have been appended, attend to the row's keys up to their
     own; table, lens and starts as in ``paged_append``.  ``max_new`` bounds the new tokens of a row (None: not known); it picks
-    kernels, whose results differ by rounding.  Tokens behind the last row are left as ``out`` (not q) holds them."""
+    kernels, whose results differ by rounding.  Over bf16 a softmax weight keeps 16 bits where a row's new tokens times the query heads of a KV head are
+    at most 16, and 8 where they are more.  Tokens behind the last row are left as ``out`` (not q) holds them."""
     if out is None and _fast is not None:
         got = _fast.attention(q, k_pages, v_pages, table, lens, scale, starts, max_new)
         if got is not None:

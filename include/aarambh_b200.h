@@ -391,7 +391,8 @@ int ab2_paged_append(const ab2_paged *cache, const void *k_dev, long long k_stri
 /* Attention of the new tokens, whose keys and values have been appended: a token sees its row's keys up to its own position, query head
  * j reads KV head j / (heads / kv_heads), up to 32 query heads for one KV head; a token that sees no key answers zeros.  out_dev
  * must not overlap q_dev or the pages.  Keys and values out of
- * sight may hold anything.  max_new (at least the most new tokens of a row) picks kernels; rows that have more are
+ * sight may hold anything.  Scores, sums and the softmax are f32; over bf16 the weights enter the product with the values in two bf16 terms (2^-16 each) where a row's
+ * new tokens times the query heads of a KV head are at most 16, rounded to bf16 (2^-8 each) where they are more.  max_new (at least the most new tokens of a row) picks kernels; rows that have more are
  * answered all the same.  workspace_dev
  * (ab2_paged_workspace bytes, 16-byte aligned, nothing in it is kept between calls) lets long rows be cut between CTAs; NULL: they are not. */
 #define AB2_PAGED_UNCUT 256 /* tokens of a row up to which it is not worth a workspace: cutting takes a second launch */
