@@ -101,6 +101,9 @@ SIGNATURES = {
     "ab2_paged_append": ([_p, _p, _ll, _p, _ll, _p, _ll, _i, _p, _ll, _p, _i, _i, _f, _i, _p], _i),
     "ab2_paged_workspace": ([_i, C.POINTER(C.c_size_t)], _i),
     "ab2_paged_attention": ([_p, _p, _ll, _i, _p, _ll, _i, _f, _p, C.c_size_t, _i, _p], _i),
+    "ab2_paged_attention_window": ([_p, _i, _i, _p, _ll, _i, _p, _ll, _i, _f, _p, C.c_size_t, _i, _p], _i),
+    "ab2_paged_append_e4m3": ([_p, _p, _p, _p, _ll, _p, _ll, _p, _ll, _i, _p, _ll, _p, _i, _i, _f, _i, _p], _i),
+    "ab2_paged_attention_e4m3": ([_p, _p, _p, _i, _i, _p, _ll, _i, _p, _ll, _i, _f, _p, C.c_size_t, _i, _p], _i),
     "ab2_adjust_logits": ([_p, _ll, _i, _i, _p, _ll, _i, _p, _p, _p, _p, _i, _p, _p, _i, _p], _i),
     "ab2_model_create": ([_pp, _p, _i, _i], _i),
     "ab2_model_create_stack": ([_pp, _p, _p, _i, _i], _i),
@@ -156,6 +159,7 @@ class LayerSpec(C.Structure):
 
 
 PAGED_UNCUT = 256   # AB2_PAGED_UNCUT
+PAGED_BLOCK = 16    # tokens of a head that share a scale in pages of 8 bits
 
 
 class Paged(C.Structure):

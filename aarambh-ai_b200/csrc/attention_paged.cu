@@ -20,8 +20,6 @@
 using namespace ab2;
 
 namespace ab2 {
-int paged_check(const ab2_paged *c, ab2_dtype dtype);
-PagedView paged_view(const ab2_paged *c);
 size_t paged_mma_bytes(int hd);
 int paged_mma_attention(const PagedAttnArgs &a, int hd, int max_new, void *workspace, size_t bytes, cudaStream_t s);
 size_t paged_tc_bytes(int hd);
@@ -38,13 +36,14 @@ namespace {
 constexpr int PA_THREADS = 128, PA_KEYS = 32;
 constexpr int TALL_ROWS = 512, TALL_ALL = 2560;
 
-template <int HD, int QR> struct SimtShape {
+template <int HD, int QR, bool E8 = false> struct SimtShape {
     static constexpr int TX = QR == 8 ? 16 : 8, TY = PA_THREADS / TX, RPT = QR / TY, KPT = PA_KEYS / TX, DPT = HD / TX;
     // Row i of a thread: two are neighbours, which see much the same keys; four lie TY apart, or those of a warp would meet in the same banks.
     static constexpr int STEP = RPT == 4 ? TY : 1, FIRST = RPT == 4 ? 1 : RPT;
     static constexpr int KROW = HD + 4, PROW = PA_KEYS + 4;   // a row's bank moves on by 16 bytes
     static constexpr int BUF = PA_KEYS * KROW * 4;
-    static constexpr int SMEM = 4 * BUF + QR * KROW * 4 + QR * PROW * 4;
+    static constexpr int RAW = PA_KEYS * HD;   // e4m3: codes come two tiles ahead, and are made floats a tile at a time
+    static constexpr int SMEM = (E8 ? 2 * BUF + 4 * RAW : 4 * BUF) + QR * KROW * 4 + QR * PROW * 4;
     static constexpr int CTAS = HD == 128 ? 2 : QR == 64 ? 3 : 4;   // of an SM: what shared memory holds
 };
 
@@ -52,16 +51,19 @@ __device__ __forceinline__ void cp16(void *dst, const void *src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
-template <int HD, int QR>
+template <int HD, int QR, bool E8, bool WIN>   // pages of e4m3; a window
 __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_simt_kernel(const __grid_constant__ PagedAttnArgs a) {
-    using S = SimtShape<HD, QR>;
+    using S = SimtShape<HD, QR, E8>;
     pdl_wait();
     constexpr int TX = S::TX, RPT = S::RPT, KPT = S::KPT, DPT = S::DPT, KROW = S::KROW, PROW = S::PROW, STEP = S::STEP, CH = 4;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ long long warp_sums[PA_THREADS / 32];
     __shared__ int2 found[2];
-    float *kbuf = (float *)smem, *vbuf = kbuf + 2 * PA_KEYS * KROW;
-    float *qs = (float *)(smem + 4 * S::BUF), *ps = qs + QR * KROW;
+    __shared__ float scales[E8 ? 2 : 1][2][PA_KEYS / PAGED_BLOCK];
+    constexpr int BUFS = E8 ? 1 : 2;
+    float *kbuf = (float *)smem, *vbuf = kbuf + BUFS * PA_KEYS * KROW;
+    uint8_t *raw = smem + 2 * S::BUF;
+    float *qs = (float *)(smem + (E8 ? 2 * S::BUF + 4 * S::RAW : 4 * S::BUF)), *ps = qs + QR * KROW;
     const int tx = threadIdx.x % TX, row0 = threadIdx.x / TX * S::FIRST;
     const PagedView &p = a.plan.p;
     PagedRun run = paged_run<PA_THREADS>(a.plan, blockIdx.x, gridDim.x, warp_sums, found, a.status);
@@ -69,6 +71,7 @@ __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_sim
     PagedPiece w;
     while (paged_next(a.plan, run, w)) {
         const PagedSpan sp = paged_span(a.plan, w);
+        const PagedHole hole = WIN ? paged_hole(a.plan, sp.base, w.q_tile) : PagedHole{0, 0};
         if (threadIdx.x == 0) paged_cut(a, run, w, sp, blockIdx.x);
         const int t0 = sp.t0, ntok = sp.ntok, base = sp.base, lo = sp.lo, hi = sp.hi, group = a.plan.group;
         __syncthreads();
@@ -80,13 +83,27 @@ __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_sim
         }
         // rows past the last key read as zeros
         auto fetch = [&](int key0, int buf) {
-            for (int i = threadIdx.x; i < PA_KEYS * HD / CH; i += PA_THREADS) {
-                const int j = i / (HD / CH), d = i % (HD / CH) * CH, key = key0 + j;
-                const bool in = key < hi;
-                const int at = in ? key : lo;
-                const size_t row = (((size_t)paged_page(p, w.row, at, a.status) * p.kv_heads + w.head) << p.page_shift) + (at & ((1 << p.page_shift) - 1));
-                cp16(kbuf + (buf * PA_KEYS + j) * KROW + d, (const float *)a.k + row * HD + d, in);
-                cp16(vbuf + (buf * PA_KEYS + j) * KROW + d, (const float *)a.v + row * HD + d, in);
+            if constexpr (E8) {   // a block of PAGED_BLOCK keys lies in one page
+                constexpr int CODES = HD / 16;
+                for (int i = threadIdx.x; i < PA_KEYS * CODES; i += PA_THREADS) {
+                    const int j = i / CODES, ch = i % CODES, v = key0 + j, key = WIN ? paged_key(hole, v) : v;
+                    const bool in = v < hi && !(WIN && paged_hidden(a.plan, sp, key & ~(PAGED_BLOCK - 1), PAGED_BLOCK));
+                    const size_t row = in ? (((size_t)paged_page(p, w.row, key, a.status) * p.kv_heads + w.head) << p.page_shift) + (key & ((1 << p.page_shift) - 1)) : 0;
+                    cp16(raw + (2 * buf * PA_KEYS + j) * HD + ch * 16, (const uint8_t *)a.k + row * HD + ch * 16, in);
+                    cp16(raw + ((2 * buf + 1) * PA_KEYS + j) * HD + ch * 16, (const uint8_t *)a.v + row * HD + ch * 16, in);
+                    if (j % PAGED_BLOCK == 0 && ch < 2)
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"((uint32_t)__cvta_generic_to_shared(&scales[buf][ch][j / PAGED_BLOCK])), "l"((ch ? a.v_scales : a.k_scales) + row / PAGED_BLOCK), "r"(in ? 4 : 0) : "memory");
+                }
+            } else {
+                for (int i = threadIdx.x; i < PA_KEYS * HD / CH; i += PA_THREADS) {
+                    const int j = i / (HD / CH), d = i % (HD / CH) * CH, key = WIN ? paged_key(hole, key0 + j) : key0 + j;
+                    const bool hidden = WIN && (key0 + j >= hi || paged_hidden(a.plan, sp, key & ~(PAGED_BLOCK - 1), PAGED_BLOCK));
+                    const bool in = WIN ? !hidden : key < hi;
+                    const int at = in ? key : lo;
+                    const size_t row = hidden ? 0 : (((size_t)paged_page(p, w.row, at, a.status) * p.kv_heads + w.head) << p.page_shift) + (at & ((1 << p.page_shift) - 1));
+                    cp16(kbuf + (buf * PA_KEYS + j) * KROW + d, (const float *)a.k + row * HD + d, in);
+                    cp16(vbuf + (buf * PA_KEYS + j) * KROW + d, (const float *)a.v + row * HD + d, in);
+                }
             }
             asm volatile("cp.async.commit_group;\n" ::: "memory");
         };
@@ -95,7 +112,7 @@ __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_sim
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
             const int tok = paged_token(a.plan, row0 + STEP * i);
-            lim[i] = tok < ntok ? base + t0 + tok : 0x7fffffff;   // a row without a token is not looked at, and keeps no other from what all see
+            lim[i] = tok < ntok ? base + t0 + tok - hole.gap : 0x7fffffff;   // a row without a token is not looked at, and keeps no other from what all see
             if (tok < ntok) seen = lim[i];                        // rows go by tokens
             sure = min(sure, lim[i]);
             top[i] = -INFINITY;
@@ -103,6 +120,9 @@ __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_sim
 #pragma unroll
             for (int d = 0; d < DPT; ++d) o[i][d] = 0.f;
         }
+        // of a row, which keys it sees; and from which on every row sees those behind the sinks
+        auto sees = [&](int i, int key) { return key <= lim[i] && (!WIN || key < a.plan.sinks || key > lim[i] - a.plan.window); };
+        const int late = WIN ? base + t0 + ntok - a.plan.window - hole.gap : 0;
         if (lo < hi) fetch(lo, 0);
         for (int key0 = lo, buf = 0; key0 < hi; key0 += PA_KEYS, buf ^= 1) {
             if (key0 + PA_KEYS < hi) {
@@ -112,6 +132,17 @@ __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_sim
                 asm volatile("cp.async.wait_group 0;\n" ::: "memory");
             }
             __syncthreads();
+            if constexpr (E8) {
+                for (int i = threadIdx.x; i < 2 * PA_KEYS * HD / 4; i += PA_THREADS) {
+                    const int kv = i / (PA_KEYS * HD / 4), j = i / (HD / 4) % PA_KEYS, d = i % (HD / 4) * 4;
+                    const uint32_t x = *reinterpret_cast<const uint32_t *>(raw + ((2 * buf + kv) * PA_KEYS + j) * HD + d);
+                    const float f = scales[buf][kv][j / PAGED_BLOCK];
+                    const float2 lo2 = floats_of_codes(x), hi2 = floats_of_codes(x >> 16);
+                    *reinterpret_cast<float4 *>((kv ? vbuf : kbuf) + j * KROW + d) = make_float4(lo2.x * f, lo2.y * f, hi2.x * f, hi2.y * f);
+                }
+                __syncthreads();
+            }
+            const int place = E8 ? 0 : buf * PA_KEYS;   // of the tile among kbuf's and vbuf's rows
             float4 s4[RPT][KPT];   // a score as four sums: shorter chains, for time and for rounding
 #pragma unroll
             for (int i = 0; i < RPT; ++i)
@@ -123,7 +154,7 @@ __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_sim
 #pragma unroll
                 for (int i = 0; i < RPT; ++i) qv[i] = *reinterpret_cast<const float4 *>(qs + (row0 + STEP * i) * KROW + d);
 #pragma unroll
-                for (int j = 0; j < KPT; ++j) kv[j] = load4(kbuf + (buf * PA_KEYS + tx + TX * j) * KROW + d);
+                for (int j = 0; j < KPT; ++j) kv[j] = load4(kbuf + (place + tx + TX * j) * KROW + d);
 #pragma unroll
                 for (int i = 0; i < RPT; ++i)
 #pragma unroll
@@ -141,7 +172,7 @@ __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_sim
                 for (int j = 0; j < KPT; ++j) {
                     const int key = key0 + tx + TX * j;
                     s[i][j] = (s4[i][j].x + s4[i][j].y) + (s4[i][j].z + s4[i][j].w);
-                    if (key > lim[i] || key >= hi) s[i][j] = -INFINITY;   // out of sight, whatever it holds
+                    if (!sees(i, key) || key >= hi) s[i][j] = -INFINITY;   // out of sight, whatever it holds
                     best = fmaxf(best, s[i][j]);
                 }
 #pragma unroll
@@ -155,7 +186,7 @@ __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_sim
 #pragma unroll
                 for (int j = 0; j < KPT; ++j) {
                     const int key = key0 + tx + TX * j;
-                    const float e = key > lim[i] || key >= hi ? 0.f : exp2f(s[i][j] - m);
+                    const float e = !sees(i, key) || key >= hi ? 0.f : exp2f(s[i][j] - m);
                     weights += e;
                     ps[(row0 + STEP * i) * PROW + tx + TX * j] = e;
                 }
@@ -163,7 +194,7 @@ __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_sim
             }
             __syncwarp();  // a row's weights come from lanes of one warp
             // keys that no row of the thread sees may hold anything: their weight is 0, and 0 times Inf is not
-            const bool every = RPT > 1 && seen >= 0 && key0 + PA_KEYS - 1 <= sure;   // of the tile's keys is seen by every row of the thread
+            const bool every = RPT > 1 && seen >= 0 && key0 + PA_KEYS - 1 <= sure && (!WIN || key0 >= late || key0 + PA_KEYS <= a.plan.sinks);   // of the tile's keys is seen by every row of the thread
             if (every) {
 #pragma unroll 2
                 for (int j = 0; j < PA_KEYS; j += 4) {
@@ -174,7 +205,7 @@ __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_sim
                     for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
                         for (int d = 0; d < DPT; d += 4) {
-                            const float4 v = load4(vbuf + (buf * PA_KEYS + j + jj) * KROW + tx * 4 + d * TX);
+                            const float4 v = load4(vbuf + (place + j + jj) * KROW + tx * 4 + d * TX);
 #pragma unroll
                             for (int i = 0; i < RPT; ++i) {
                                 const float f = jj == 0 ? e[i].x : jj == 1 ? e[i].y : jj == 2 ? e[i].z : e[i].w;
@@ -193,10 +224,10 @@ __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_sim
                 for (int i = 0; i < RPT; ++i) e[i] = ps[(row0 + STEP * i) * PROW + j];
 #pragma unroll
                 for (int d = 0; d < DPT; d += 4) {
-                    const float4 v = load4(vbuf + (buf * PA_KEYS + j) * KROW + tx * 4 + d * TX);
+                    const float4 v = load4(vbuf + (place + j) * KROW + tx * 4 + d * TX);
 #pragma unroll
                     for (int i = 0; i < RPT; ++i) {
-                        if (RPT > 1 && key0 + j > lim[i]) continue;
+                        if ((RPT > 1 || WIN) && !sees(i, key0 + j)) continue;
                         here[i][d] = fmaf(e[i], v.x, here[i][d]);
                         here[i][d + 1] = fmaf(e[i], v.y, here[i][d + 1]);
                         here[i][d + 2] = fmaf(e[i], v.z, here[i][d + 2]);
@@ -335,21 +366,27 @@ __global__ void __launch_bounds__(128 * GROUPS) paged_merge_kernel(const __grid_
 
 template <int HD, int QR> size_t simt_bytes() { return paged_piece_bytes(SimtShape<HD, QR>::CTAS * device_sm_count(), QR, HD); }
 
-template <int HD, int QR>
+template <int HD, int QR, bool E8, bool WIN>
 int launch_simt(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
-    using S = SimtShape<HD, QR>;
+    using S = SimtShape<HD, QR, E8>;
     static bool configured[64] = {false};  // the attribute is per device
     int dev = 0;
     AB2_CUDA(cudaGetDevice(&dev));
     AB2_REQUIRE(dev >= 0 && dev < 64, AB2_ERR_BAD_ARG, "device index %d out of range", dev);
     if (!configured[dev]) {
-        AB2_CUDA(cudaFuncSetAttribute(paged_simt_kernel<HD, QR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+        AB2_CUDA(cudaFuncSetAttribute(paged_simt_kernel<HD, QR, E8, WIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
         configured[dev] = true;
     }
     paged_deal(a, S::CTAS * device_sm_count(), QR, 5, 1, HD, workspace, bytes);
     ChainedLaunches chained(true);   // the launch before it, an append or a merge, need not have ended when this one is set up: it waits in the kernel
-    AB2_CUDA(launch_kernel(paged_simt_kernel<HD, QR>, dim3(a.ctas), dim3(PA_THREADS), S::SMEM, s, a));
+    AB2_CUDA(launch_kernel(paged_simt_kernel<HD, QR, E8, WIN>, dim3(a.ctas), dim3(PA_THREADS), S::SMEM, s, a));
     return a.plan.whole ? AB2_OK : paged_merge(a, HD, AB2_F32, s);
+}
+
+template <int HD, int QR>
+int launch_simt(const PagedAttnArgs &a, void *workspace, size_t bytes, cudaStream_t s) {
+    if (a.plan.window) return a.k_scales ? launch_simt<HD, QR, true, true>(a, workspace, bytes, s) : launch_simt<HD, QR, false, true>(a, workspace, bytes, s);
+    return a.k_scales ? launch_simt<HD, QR, true, false>(a, workspace, bytes, s) : launch_simt<HD, QR, false, false>(a, workspace, bytes, s);
 }
 
 int simt_attention(const PagedAttnArgs &a, int hd, int max_new, void *workspace, size_t bytes, cudaStream_t s) {
@@ -387,10 +424,14 @@ AB2_API int ab2_paged_workspace(int head_dim, size_t *bytes) {
     return AB2_OK;
 }
 
-AB2_API int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long long q_stride, int heads, void *out_dev, long long out_stride, int max_new, float scale,
-                                void *workspace_dev, size_t workspace_bytes, ab2_dtype dtype, ab2_stream stream) {
+// The pages' scales, with them pages hold e4m3 and not `dtype`; a window, 0: none.
+static int paged_attend(const ab2_paged *cache, const float *k_scales_dev, const float *v_scales_dev, int window, int sinks, const void *q_dev, long long q_stride, int heads, void *out_dev, long long out_stride,
+                        int max_new, float scale, void *workspace_dev, size_t workspace_bytes, ab2_dtype dtype, ab2_stream stream) {
     int rc = paged_check(cache, dtype);
     if (rc != AB2_OK) return rc;
+    AB2_REQUIRE(!k_scales_dev == !v_scales_dev, AB2_ERR_BAD_ARG, "pages of e4m3 have scales of keys and of values");
+    AB2_REQUIRE(window >= 0 && sinks >= 0 && window <= (1 << 30) && sinks <= (1 << 30) && (window > 0 || sinks == 0), AB2_ERR_BAD_SHAPE,
+                "a window of %d keys and %d first ones: up to 2^30 of each are served, and first ones beside a window", window, sinks);
     AB2_REQUIRE(heads > 0 && heads % cache->kv_heads == 0 && heads / cache->kv_heads <= 32, AB2_ERR_BAD_SHAPE, "%d query heads over %d KV heads: a multiple of them up to 32 is served", heads, cache->kv_heads);
     AB2_REQUIRE(max_new > 0, AB2_ERR_BAD_SHAPE, "rows of at most %d new tokens", max_new);
     if (cache->tokens == 0) return AB2_OK;
@@ -398,15 +439,18 @@ AB2_API int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long 
     const long long row = (long long)heads * cache->head_dim;
     AB2_REQUIRE(q_stride >= row && out_stride >= row, AB2_ERR_BAD_SHAPE, "a token's heads lie one after the other, and tokens do not overlap");
     const size_t esize = dtype_size(dtype);
-    AB2_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev | (uintptr_t)workspace_dev) & 15) == 0 && ((q_stride | out_stride) * esize & 15) == 0, AB2_ERR_BAD_ALIGN, "queries, outputs and their rows must be 16-byte aligned");
+    AB2_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev | (uintptr_t)workspace_dev) & 15) == 0 && (((uintptr_t)k_scales_dev | (uintptr_t)v_scales_dev) & 3) == 0 && ((q_stride | out_stride) * esize & 15) == 0, AB2_ERR_BAD_ALIGN, "queries, outputs and their rows must be 16-byte aligned");
     // a query, key or value may be read after outputs have been written
-    const long long es = (long long)esize, pool = (long long)cache->pages * cache->page_size * cache->kv_heads * cache->head_dim * es;
+    const long long es = (long long)esize, pool = (long long)cache->pages * cache->page_size * cache->kv_heads * cache->head_dim * (k_scales_dev ? 1 : es);
+    const long long blocks = (long long)cache->pages * cache->kv_heads * (cache->page_size / PAGED_BLOCK) * 4;
     const RowsAt o_at = {out_dev, row * es, out_stride * es, cache->tokens};
+    AB2_REQUIRE(!rows_meet(o_at, {k_scales_dev, blocks, blocks, 1}) && !rows_meet(o_at, {v_scales_dev, blocks, blocks, 1}), AB2_ERR_BAD_ARG, "the outputs may not take the place of scales");
     AB2_REQUIRE(!rows_meet(o_at, {q_dev, row * es, q_stride * es, cache->tokens}) && !rows_meet(o_at, {cache->k_pages, pool, pool, 1}) && !rows_meet(o_at, {cache->v_pages, pool, pool, 1}), AB2_ERR_BAD_ARG,
                 "the outputs may not take the place of queries or pages");
     PagedAttnArgs a = {};
     a.plan.p = paged_view(cache);
     a.q = q_dev; a.k = cache->k_pages; a.v = cache->v_pages; a.out = out_dev; a.q_stride = q_stride; a.o_stride = out_stride;
+    a.k_scales = k_scales_dev; a.v_scales = v_scales_dev; a.plan.window = window; a.plan.sinks = sinks;
     a.plan.group = heads / cache->kv_heads; a.plan.above = 0; a.plan.most = 0x7fffffff; a.sl = scale * 1.44269504088896341f;
     rc = device_status_word(&a.status);
     if (rc != AB2_OK) return rc;
@@ -423,4 +467,20 @@ AB2_API int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long 
         a.plan.most = 0x7fffffff;
     }
     return paged_tc_attention(a, cache->head_dim, workspace_dev, workspace_bytes, (cudaStream_t)stream);
+}
+
+AB2_API int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long long q_stride, int heads, void *out_dev, long long out_stride, int max_new, float scale,
+                                void *workspace_dev, size_t workspace_bytes, ab2_dtype dtype, ab2_stream stream) {
+    return paged_attend(cache, nullptr, nullptr, 0, 0, q_dev, q_stride, heads, out_dev, out_stride, max_new, scale, workspace_dev, workspace_bytes, dtype, stream);
+}
+
+AB2_API int ab2_paged_attention_window(const ab2_paged *cache, int window, int sinks, const void *q_dev, long long q_stride, int heads, void *out_dev, long long out_stride, int max_new, float scale,
+                                       void *workspace_dev, size_t workspace_bytes, ab2_dtype dtype, ab2_stream stream) {
+    return paged_attend(cache, nullptr, nullptr, window, sinks, q_dev, q_stride, heads, out_dev, out_stride, max_new, scale, workspace_dev, workspace_bytes, dtype, stream);
+}
+
+AB2_API int ab2_paged_attention_e4m3(const ab2_paged *cache, const float *k_scales_dev, const float *v_scales_dev, int window, int sinks, const void *q_dev, long long q_stride, int heads, void *out_dev,
+                                     long long out_stride, int max_new, float scale, void *workspace_dev, size_t workspace_bytes, ab2_dtype dtype, ab2_stream stream) {
+    AB2_REQUIRE(k_scales_dev && v_scales_dev, AB2_ERR_BAD_ARG, "null scales");
+    return paged_attend(cache, k_scales_dev, v_scales_dev, window, sinks, q_dev, q_stride, heads, out_dev, out_stride, max_new, scale, workspace_dev, workspace_bytes, dtype, stream);
 }

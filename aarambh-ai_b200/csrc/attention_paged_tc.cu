@@ -32,6 +32,7 @@
 // again on CUDA cores over the keys in its sight, behind all pieces of the CTA, so that no bounded wait lasts as long as that.  Every wait on an mbarrier is bounded; on a time-out the CTA records AB2_ERR_TIMEOUT and
 // walks through the rest of its work without waiting.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 #include "tcgen05_util.cuh"
@@ -42,16 +43,19 @@ using namespace ab2::tc;
 namespace ab2 {
 namespace {
 
-constexpr int PC_Q = 128, PC_KEYS = 80, PC_THREADS = 384;
+constexpr int PC_Q = 128, PC_KEYS = 80, PC_THREADS = 384, PC_EXPAND = 128;
 constexpr int PC_QBOX = PC_Q * 128, PC_BOX = PC_KEYS * 128;   // boxes of queries, and of keys or values: rows of 64 elements
 constexpr int PC_ROWS = 16;   // that one copy brings: the least that a page holds
 constexpr int PC_TWICE = 16;  // query rows of an item up to which it has each of them twice, for both terms of its weights
+constexpr int PC_FEW_REGS = 56, PC_MANY_REGS = 200;   // E8: of a thread of other roles, and of softmax
 constexpr float PC_SLACK = 8.f;  // powers of two a score may exceed the row's maximum by
 constexpr float PC_NONE = -1e30f;
 
-template <int HD> struct PcShape {
-    static constexpr int BOXES = HD / 64, QTILE = BOXES * PC_QBOX, TILE = BOXES * PC_BOX, SLOTS = HD == 128 ? 4 : 8;   // a slot holds a tile's keys and its values
-    static constexpr int SMEM = 1024 + 2 * QTILE + SLOTS * 2 * TILE;
+template <int HD, bool E8 = false> struct PcShape {
+    static constexpr int THREADS = PC_THREADS + (E8 ? PC_EXPAND : 0);
+    static constexpr int BOXES = HD / 64, QTILE = BOXES * PC_QBOX, TILE = BOXES * PC_BOX, SLOTS = (E8 ? 3 : 4) * (HD == 128 ? 1 : 2);   // a slot holds a tile's keys and its values
+    static constexpr int RAW = E8 ? 2 * PC_KEYS * HD : 0, RAWS = E8 ? (HD == 128 ? 2 : 4) : 0;   // codes of a tile's keys and values, and tiles of them
+    static constexpr int SMEM = 1024 + 2 * QTILE + SLOTS * 2 * TILE + RAWS * RAW;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -91,12 +95,13 @@ struct PcPiece {
     int first, second;   // tiles of keys that either tile of rows looks at
     int most;
 };
-__device__ __forceinline__ bool pc_next(const PagedPlan &a, PagedRun &run, PcPiece &x) {
+template <bool WIN> __device__ __forceinline__ bool pc_next(const PagedPlan &a, PagedRun &run, PcPiece &x) {
     if (!paged_next(a, run, x.w)) return false;
     x.s = paged_span(a, x.w);
     const int rows = x.s.ntok * a.group;
+    const int gap = WIN ? paged_hole(a, x.s.base, x.w.q_tile).gap : 0;
     auto tiles = [&](int first, int end) {   // of rows [first, end) of the item: keys up to those of the last token
-        const int last = min(x.s.hi, x.s.base + x.s.t0 + paged_token(a, end - 1) + 1);
+        const int last = min(x.s.hi, x.s.base + x.s.t0 + paged_token(a, end - 1) + 1 - gap);
         return end > first ? max(0, (last - x.s.lo + PC_KEYS - 1) / PC_KEYS) : 0;
     };
     x.first = tiles(0, min(rows, PC_Q));
@@ -105,14 +110,20 @@ __device__ __forceinline__ bool pc_next(const PagedPlan &a, PagedRun &run, PcPie
     return true;
 }
 
-struct PcShared {
-    uint64_t full[8], empty[8], qfull[2], sfull[2], sfree[2], pfull[2], odone[2];
+template <int SLOTS, int RAWS> struct PcShared {
+    uint64_t full[SLOTS], empty[SLOTS], qfull[2], sfull[2], sfree[2], pfull[2], odone[2];
+    uint64_t rfull[RAWS > 0 ? RAWS : 1], rempty[RAWS > 0 ? RAWS : 1];
     uint32_t tmem_base;
     int failed;
-    int2 found[2];
     union {
-        long long warp_sums[PC_THREADS / 32];   // while the CTA looks for its run
-        PagedRun start;                         // that run, from then on
+        struct {                                // while the CTA looks for its run
+            long long warp_sums[(PC_THREADS + (RAWS > 0 ? PC_EXPAND : 0)) / 32];
+            int2 found[2];
+        };
+        struct {
+            PagedRun start;                     // that run, over the sums alone: other threads may still read what was found
+            float scales[RAWS > 0 ? RAWS : 1][2][PC_KEYS / PC_ROWS];   // of a tile of codes, keys and values; behind a barrier of all
+        };
     };
     // of every softmax warp: its run, the piece that it is at and the next one (kept from its registers, which the scores fill)
     PagedRun run[8];
@@ -121,9 +132,10 @@ struct PcShared {
 
 // One tile of keys for the warp's 32 rows, a lane each: scores to weights.  With EDGE keys past `lim` are out of sight, and a lane that is `second` hands on what
 // rounding left of each weight (a kind of its own for that cost the loops around it 5 %).  `before` waits until the
-// products with the tile before are done: its weights' place is free then, and the sums stand still.
-template <int HD, bool EDGE, class Before>
-__device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, bool second, bool has_o, float &top, float &sum, uint64_t *taken, uint64_t *ready, Before before) {
+// products with the tile before are done: its weights' place is free then, and the sums stand still.  WIN: of the tile's keys those from `sinks` up to `since` are
+// hidden too.
+template <int HD, bool EDGE, bool WIN, class Before>
+__device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, int sinks, int since, bool second, bool has_o, float &top, float &sum, uint64_t *taken, uint64_t *ready, Before before) {
     uint32_t va[32], vb[32], vc[16];
     tmem_ld32_start(va, s_addr);
     tmem_ld32_start(vb, s_addr + 32);
@@ -139,9 +151,21 @@ __device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, flo
 #pragma unroll
         for (int k = 0; k < PC_KEYS; ++k) v(k) ^= 0x80000000u;
     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if constexpr (EDGE && WIN) {
+        // a bit for each key in sight, 32 at a time
+        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };   // bits of the keys below n
 #pragma unroll
-    for (int k = 0; k < PC_KEYS; ++k)
-        if (EDGE && k > lim) v(k) = 0xff800000u;
+        for (int w = 0; w < PC_KEYS; w += 32) {
+            const uint32_t seen = below(lim + 1 - w) & (below(sinks - w) | ~below(since - w));
+#pragma unroll
+            for (int k = w; k < w + 32 && k < PC_KEYS; ++k)
+                if (!((seen >> (k - w)) & 1)) v(k) = 0xff800000u;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < PC_KEYS; ++k)
+            if (EDGE && k > lim) v(k) = 0xff800000u;
+    }
 #pragma unroll
     for (int k = 0; k < PC_KEYS; k += 8)
 #pragma unroll
@@ -213,24 +237,39 @@ __device__ __forceinline__ void exchange4(uint4 (&o)[4], int lane) {
     swap(o[1], o[3], lane & 2, 2);
 }
 
-template <int HD>
-__global__ void __launch_bounds__(PC_THREADS, 1)
+// Eight codes as eight bf16 values: exact where the scale is a power of two (and the value no smaller than bf16's least).
+__device__ __forceinline__ uint4 pc_values(uint32_t x, uint32_t y, float scale) {
+    auto two = [&](uint32_t codes) {
+        const float2 f = floats_of_codes(codes);
+        const __nv_bfloat162 b = __floats2bfloat162_rn(f.x * scale, f.y * scale);
+        return *reinterpret_cast<const uint32_t *>(&b);
+    };
+    return make_uint4(two(x), two(x >> 16), two(y), two(y >> 16));
+}
+
+// E8: pages of e4m3.  Four more warps make a tile's codes, which come by bulk copies, bf16 values in the ring's slots; all other roles are the same.
+// WIN: a window.
+template <int HD, bool E8, bool WIN>
+__global__ void __launch_bounds__(PcShape<HD, E8>::THREADS, 1)
 paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PagedAttnArgs a) {
-    using S = PcShape<HD>;
+    using S = PcShape<HD, E8>;
+    using Page = std::conditional_t<E8, uint8_t, __nv_bfloat16>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ PcShared sh;
-    static_assert(S::SMEM + sizeof(PcShared) <= 227 * 1024, "shared memory of a CTA");
-    uint8_t *qbuf = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023), *ring = qbuf + 2 * S::QTILE;
+    __shared__ PcShared<S::SLOTS, S::RAWS> sh;
+    static_assert(S::SMEM + sizeof(sh) <= 227 * 1024, "shared memory of a CTA");
+    static_assert(sizeof(PagedRun) <= S::THREADS / 32 * sizeof(long long), "the run lies over the sums");
+    uint8_t *qbuf = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023), *ring = qbuf + 2 * S::QTILE, *codes = ring + S::SLOTS * 2 * S::TILE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *failed = &sh.failed;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::SLOTS; ++i) { bar_init(&sh.full[i], 1); bar_init(&sh.empty[i], 2); }
+        for (int i = 0; i < S::SLOTS; ++i) { bar_init(&sh.full[i], E8 ? PC_EXPAND / 32 : 1); bar_init(&sh.empty[i], 2); }
+        for (int i = 0; i < S::RAWS; ++i) { bar_init(&sh.rfull[i], 1); bar_init(&sh.rempty[i], PC_EXPAND / 32); }
         for (int i = 0; i < 2; ++i) { bar_init(&sh.qfull[i], 4); bar_init(&sh.sfull[i], 1); bar_init(&sh.sfree[i], 4); bar_init(&sh.pfull[i], 4); bar_init(&sh.odone[i], 1); }
         sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     pdl_wait();   // ahead of tensor memory too, which the launch before may hold
-    PagedRun run = paged_run<PC_THREADS>(a.plan, blockIdx.x, a.ctas, sh.warp_sums, sh.found, a.status);
+    PagedRun run = paged_run<S::THREADS>(a.plan, blockIdx.x, a.ctas, sh.warp_sums, sh.found, a.status);
     if (threadIdx.x == PC_THREADS - 1) paged_uncut(a, blockIdx.x);
     if (run.u >= run.u1) return;   // the whole CTA
     if (threadIdx.x == 0) sh.start = run;
@@ -245,16 +284,80 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const PagedView &p = a.plan.p;
     PcPiece x;
     // the block's registers: 128 threads of 72 and 256 of 216 are the 384 of 168 that it was launched with
-    if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
-        if (warp == 0) {
+    // (E8: 256 of 56 and 256 of 200 are the 512 of 128)
+    if (E8 && warp >= PC_THREADS / 32) {
+        // ---------------------------------------------------------- codes to values
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PC_FEW_REGS));
+        constexpr int CH = HD / 16, ALL = PC_KEYS * CH;   // pieces of 16 codes of a row, and of a tile
+        const int me = threadIdx.x - PC_THREADS;
+        int n = 0;
+        while (pc_next<WIN>(a.plan, run, x)) {
+            const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
+            for (int j = 0; j < x.most; ++j, ++n) {
+                const int slot = n % S::SLOTS, raw = n % (S::RAWS > 0 ? S::RAWS : 1), key0 = x.s.lo + j * PC_KEYS;
+                warp_wait(&sh.rfull[raw], (n / (S::RAWS > 0 ? S::RAWS : 1)) & 1, failed);
+                warp_wait(&sh.empty[slot], ((n / S::SLOTS) & 1) ^ 1, failed);
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+                    for (int i = me; i < ALL; i += PC_EXPAND) {
+                        const int r = i / CH, ch = i % CH, key = key0 + r;
+                        // behind the piece's keys, and where no token sees a block, zeros
+                        const bool in = key < x.s.hi && !(WIN && paged_hidden(a.plan, x.s, paged_key(hole, key & ~(PAGED_BLOCK - 1)), PAGED_BLOCK));
+                        uint4 c = make_uint4(0u, 0u, 0u, 0u);
+                        if (in) c = *reinterpret_cast<const uint4 *>(codes + raw * S::RAW + (kv * PC_KEYS + r) * HD + ch * 16);
+                        const float scale = sh.scales[raw][kv][r / PAGED_BLOCK];
+                        const uint4 lo = pc_values(c.x, c.y, in ? scale : 0.f), hi = pc_values(c.z, c.w, in ? scale : 0.f);
+                        // 16 codes are two chunks of the row in its box of 64 elements; those of the second box go in the other order, so that eight lanes meet in no bank
+                        uint8_t *row = ring + (2 * slot + kv) * S::TILE + (ch >> 2) * PC_BOX + r * 128;
+                        const int c0 = 2 * (ch & 3), odd = (ch >> 2) & 1;
+                        *reinterpret_cast<uint4 *>(row + (((c0 + odd) ^ (r & 7)) << 4)) = odd ? hi : lo;
+                        *reinterpret_cast<uint4 *>(row + (((c0 + 1 - odd) ^ (r & 7)) << 4)) = odd ? lo : hi;
+                    }
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                __syncwarp();   // every lane's codes have been read, as what it stored is made of them
+                if (lane == 0) {
+                    bar_arrive(&sh.full[slot]);
+                    bar_arrive(&sh.rempty[raw]);
+                }
+            }
+        }
+    } else if (warp < 4) {
+        if (E8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PC_FEW_REGS));
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        if (E8 && warp == 0) {
+            // ---------------------------------------------------------- producer of codes
+            int n = 0;
+            while (pc_next<WIN>(a.plan, run, x)) {
+                const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
+                for (int j = 0; j < x.most; ++j, ++n) {
+                    const int v = x.s.lo + j * PC_KEYS + lane * PC_ROWS, key = WIN ? paged_key(hole, v) : v;
+                    const bool mine = lane < PC_KEYS / PC_ROWS && v < x.s.hi && !(WIN && paged_hidden(a.plan, x.s, key, PC_ROWS));
+                    const size_t row = mine ? (((size_t)paged_page(p, x.w.row, key, a.status) * p.kv_heads + x.w.head) << p.page_shift) + (key & ((1 << p.page_shift) - 1)) : 0;
+                    const float ks = mine ? __ldg(a.k_scales + row / PAGED_BLOCK) : 0.f, vs = mine ? __ldg(a.v_scales + row / PAGED_BLOCK) : 0.f;
+                    const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * PC_ROWS * HD;
+                    const int raw = n % (S::RAWS > 0 ? S::RAWS : 1);
+                    warp_wait(&sh.rempty[raw], ((n / (S::RAWS > 0 ? S::RAWS : 1)) & 1) ^ 1, failed);
+                    if (mine) { sh.scales[raw][0][lane] = ks; sh.scales[raw][1][lane] = vs; }
+                    __syncwarp();
+                    if (lane == 0) bar_expect_tx(&sh.rfull[raw], (uint32_t)(2 * bytes));
+                    __syncwarp();
+                    if (mine && !*failed) {
+                        bulk_copy(codes + raw * S::RAW + lane * PC_ROWS * HD, (const uint8_t *)a.k + row * HD, PC_ROWS * HD, &sh.rfull[raw]);
+                        bulk_copy(codes + raw * S::RAW + (PC_KEYS + lane * PC_ROWS) * HD, (const uint8_t *)a.v + row * HD, PC_ROWS * HD, &sh.rfull[raw]);
+                    }
+                }
+            }
+        } else if (warp == 0) {
             // ---------------------------------------------------------- TMA producer: K, V, K, V, ...
             int n = 0;
-            while (pc_next(a.plan, run, x)) {
+            while (pc_next<WIN>(a.plan, run, x)) {
+                const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
                 for (int j = 0; j < x.most; ++j) {
-                    const int key = x.s.lo + j * PC_KEYS + lane * PC_ROWS;
-                    const bool mine = lane < PC_KEYS / PC_ROWS && key < x.s.hi;
-                    const int page = mine ? paged_page(p, x.w.row, key, a.status) : 0;
+                    const int v = x.s.lo + j * PC_KEYS + lane * PC_ROWS, key = WIN ? paged_key(hole, v) : v;
+                    const bool mine = lane < PC_KEYS / PC_ROWS && v < x.s.hi;
+                    // a block that no token sees comes from behind the pool, as zeros
+                    const int page = !mine ? 0 : WIN && paged_hidden(a.plan, x.s, key, PC_ROWS) ? p.pages : paged_page(p, x.w.row, key, a.status);
                     const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * PC_ROWS * HD * 2;
                     const int slot = n % S::SLOTS;
                     warp_wait(&sh.empty[slot], ((n++ / S::SLOTS) & 1) ^ 1, failed);
@@ -297,7 +400,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 __syncwarp();
                 ++scored;
             };
-            while (pc_next(a.plan, run, x)) {
+            while (pc_next<WIN>(a.plan, run, x)) {
                 const int tiles = g ? x.second : x.first;
                 if (tiles > 0) {
                     warp_wait(&sh.qfull[g], asked++ & 1, failed);
@@ -327,7 +430,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         }
     } else {
         // ---------------------------------------------------------- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
+        if (E8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(PC_MANY_REGS));
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
         const int g = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, group = a.plan.group;
         const uint32_t quad_addr = (uint32_t)(quad * 32) << 16, s_addr = tmem + quad_addr + (uint32_t)(g * 128), o_addr = tmem_o + quad_addr + (uint32_t)(g * HD);
         const float sl = fmaxf(fabsf(a.sl), 1.17549435e-38f);   // above 0, so that hidden scores stay -inf
@@ -341,7 +445,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             PagedRun run = sh.run[warp - 4];
             PcPiece x;
             bool more;
-            while ((more = pc_next(a.plan, run, x))) {
+            while ((more = pc_next<WIN>(a.plan, run, x))) {
                 n0 = n;
                 n += x.most;
                 if (threadIdx.x == PC_THREADS - 1) paged_cut(a, run, x.w, x.s, blockIdx.x);
@@ -382,13 +486,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
             const bool twice = rows <= PC_TWICE;   // and this the first tile of rows
             const bool second = twice && (lane & PC_TWICE);
-            const int rr = g * PC_Q + r, asks = twice && r < 2 * PC_TWICE ? r % PC_TWICE : rr, pos = asks < rows ? x.s.base + x.s.t0 + paged_token(a.plan, asks) : -1;
-            const int least = x.s.base + x.s.t0 + paged_token(a.plan, g * PC_Q);   // the first row sees up to here
+            const int rr = g * PC_Q + r, asks = twice && r < 2 * PC_TWICE ? r % PC_TWICE : rr;
+            const int gap = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile).gap : 0, first = x.s.base + x.s.t0 - gap;   // all in virtual keys
+            const int pos = asks < rows ? first + paged_token(a.plan, asks) : -1;
+            const int least = first + paged_token(a.plan, g * PC_Q);   // the first row sees up to here
+            const int late = WIN ? first + paged_token(a.plan, min(rows, (g + 1) * PC_Q) - 1) + 1 - a.plan.window : 0;   // the last row sees from here on, and the sinks
             float top = PC_NONE, sum = 0.f;
             for (int j = 0; j < tiles; ++j, ++scored) {
                 const int at = lo + j * PC_KEYS;
                 warp_wait(&sh.sfull[g], scored & 1, failed);
-                if (at + PC_KEYS > hi) {   // what lies behind the piece's keys may be anything
+                if (!E8 && at + PC_KEYS > hi) {   // what lies behind the piece's keys may be anything
                     // Behind the wait for the scores, never ahead of it: these warps pass over pieces without rows of theirs, and the slot's barrier may still be phases
                     // away from the one meant, with the same parity.
                     const int slot = (slot0 + j) % S::SLOTS;
@@ -402,10 +509,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     __syncwarp();   // and the products wait for all four warps
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                const int lim = min(pos, hi - 1) - at;
+                const int lim = min(pos, hi - 1) - at, low = WIN ? pos + 1 - a.plan.window - at : 0;
                 auto before = [&] { if (j > 0) warp_wait(&sh.odone[g], (scored - 1) & 1, failed); };
-                if (at + PC_KEYS - 1 > least || at + PC_KEYS > hi || (g + 1) * PC_Q > rows) pc_softmax<HD, true>(s_addr, o_addr, sl, flip, lim, second, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
-                else pc_softmax<HD, false>(s_addr, o_addr, sl, flip, lim, false, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
+                if (at + PC_KEYS - 1 > least || at + PC_KEYS > hi || (g + 1) * PC_Q > rows || (WIN && at < late && at + PC_KEYS > a.plan.sinks))
+                    pc_softmax<HD, true, WIN>(s_addr, o_addr, sl, flip, lim, WIN ? a.plan.sinks - at : 0, low, second, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
+                else pc_softmax<HD, false, WIN>(s_addr, o_addr, sl, flip, lim, 0, 0, false, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
             }
             // the scores are all made: the next piece's queries may take the place of these, while the sums go out
             more = next();
@@ -484,7 +592,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         if (again) {
             PagedRun walk = sh.start;
             PcPiece x;
-            while (pc_next(a.plan, walk, x)) {
+            while (pc_next<WIN>(a.plan, walk, x)) {
                 const int rr = g * PC_Q + r, rows = x.s.ntok * group;
                 if (rows <= g * PC_Q) continue;
                 const bool all = x.w.k0 == 0 && x.w.k1 == x.w.k_tiles;
@@ -500,7 +608,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     }
                 }
                 for (uint32_t left = __ballot_sync(0xffffffffu, worst == 0x7f800000u); left; left &= left - 1)
-                    paged_again<HD>(a, x.w, x.s, g * PC_Q + quad * 32 + __ffs(left) - 1, lane, all, slot);
+                    paged_again<HD, Page>(a, x.w, x.s, g * PC_Q + quad * 32 + __ffs(left) - 1, lane, all, slot);
                 __syncwarp();
             }
         }
@@ -521,28 +629,36 @@ int pages_map(CUtensorMap *map, const void *pages, const PagedView &p, int hd) {
     return make_mats_map(map, pages, p.pages * p.kv_heads, page, hd, hd, (long long)page * hd, PC_ROWS);
 }
 
-template <int HD>
+template <int HD, bool E8, bool WIN>
 int launch_tc(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
-    using S = PcShape<HD>;
+    using S = PcShape<HD, E8>;
     static bool configured[64] = {false};  // the attribute is per device
     int dev = 0;
     AB2_CUDA(cudaGetDevice(&dev));
     AB2_REQUIRE(dev >= 0 && dev < 64, AB2_ERR_BAD_ARG, "device index %d out of range", dev);
     if (!configured[dev]) {
-        AB2_CUDA(cudaFuncSetAttribute(paged_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+        AB2_CUDA(cudaFuncSetAttribute(paged_tc_kernel<HD, E8, WIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
         configured[dev] = true;
     }
-    CUtensorMap kmap, vmap;
-    int rc = pages_map(&kmap, a.k, a.plan.p, HD);
-    if (rc == AB2_OK) rc = pages_map(&vmap, a.v, a.plan.p, HD);
-    if (rc != AB2_OK) return rc;
+    CUtensorMap kmap = {}, vmap = {};
+    if (!E8) {
+        int rc = pages_map(&kmap, a.k, a.plan.p, HD);
+        if (rc == AB2_OK) rc = pages_map(&vmap, a.v, a.plan.p, HD);
+        if (rc != AB2_OK) return rc;
+    }
     paged_deal(a, device_sm_count(), 2 * PC_Q, 7, 4, HD, workspace, bytes);
     // Set up while the launch before it ends, up to 65536 query rows: all that were tried gain there, and beyond it none does and the longest loses.  32 heads of 128, us
     // not set up early and early: 300 tokens behind 300 35.0 and 32.6, behind 16000 103 and 101.4, 1024 behind 1024 53.7 and 51.9, 2048 alone 82.0 and 80.9, behind
     // 12288 383.8 and 382.6; 3000 behind 3000 231 to 240 and 233 to 237, 4096 alone 207 and 207 to 210, behind 4096 372 and 371, behind 12288 860 to 872 and 876 to 884, 8192 alone 617 and 613 to 621.
     ChainedLaunches chained((long long)a.plan.p.tokens * a.plan.group * a.plan.p.kv_heads <= 65536);
-    AB2_CUDA(launch_kernel(paged_tc_kernel<HD>, dim3(a.ctas), dim3(PC_THREADS), S::SMEM, s, kmap, vmap, a));
+    AB2_CUDA(launch_kernel(paged_tc_kernel<HD, E8, WIN>, dim3(a.ctas), dim3(S::THREADS), S::SMEM, s, kmap, vmap, a));
     return a.plan.whole ? AB2_OK : paged_merge(a, HD, AB2_BF16, s);
+}
+
+template <int HD>
+int launch_tc(const PagedAttnArgs &a, void *workspace, size_t bytes, cudaStream_t s) {
+    if (a.plan.window) return a.k_scales ? launch_tc<HD, true, true>(a, workspace, bytes, s) : launch_tc<HD, false, true>(a, workspace, bytes, s);
+    return a.k_scales ? launch_tc<HD, true, false>(a, workspace, bytes, s) : launch_tc<HD, false, false>(a, workspace, bytes, s);
 }
 
 }  // namespace

@@ -7,6 +7,9 @@ namespace ab2 {
 
 int device_status_word(int **out);
 int device_sm_count();
+int paged_check(const ab2_paged *c, ab2_dtype dtype);
+int append_check(const ab2_paged *cache, long long page_es, const void *k_dev, long long k_stride, const void *v_dev, long long v_stride, const void *q_dev, long long q_stride, int heads, void *q_out_dev,
+                 long long q_out_stride, const double *frequencies_dev, int rot_dims, int layout, ab2_dtype dtype);
 
 // What deals work out is compiled for the host too, where tests/test_paged_plan.py runs it over batches of all kinds.
 
@@ -20,6 +23,7 @@ struct PagedView {
     long long table_stride;
     int rows, tokens, width, pages, page_shift, kv_heads;
 };
+PagedView paged_view(const ab2_paged *c);
 __host__ __device__ __forceinline__ void paged_bad(int *status) {
 #ifdef __CUDA_ARCH__
     atomicCAS(status, 0, (int)AB2_ERR_BAD_ARG);
@@ -43,6 +47,38 @@ __device__ __forceinline__ int paged_page(const PagedView &p, int b, int pos, in
     paged_bad(status);
     return 0;
 }
+
+// ---- pages of 8 bits: e4m3 codes, and a scale for every PAGED_BLOCK tokens of a head ([pages][kv_heads][page_size / PAGED_BLOCK] f32); a value is its code times
+// its scale.
+constexpr int PAGED_BLOCK = 16;
+__device__ __forceinline__ uint32_t f16x2_of_codes(uint32_t two) {   // of the lower 16 bits, exactly
+    uint32_t d;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(d) : "h"((uint16_t)two));
+    return d;
+}
+__device__ __forceinline__ float2 floats_of_codes(uint32_t two) {
+    const uint32_t h = f16x2_of_codes(two);
+    return __half22float2(*reinterpret_cast<const __half2 *>(&h));
+}
+// 16 bytes of a row of keys or values as floats, to be scaled where they are codes.
+template <typename P> struct PagedChunk {   // bf16: 8 elements
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void floats(uint4 x, float (&y)[N]) {
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { y[2 * i] = __uint_as_float(w[i] << 16); y[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+    static __device__ __forceinline__ float one(P x) { return to_f32(x); }
+};
+template <> struct PagedChunk<uint8_t> {
+    static constexpr int N = 16;
+    static __device__ __forceinline__ void floats(uint4 x, float (&y)[N]) {
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { const float2 f = floats_of_codes(w[i >> 1] >> (16 * (i & 1))); y[2 * i] = f.x; y[2 * i + 1] = f.y; }
+    }
+    static __device__ __forceinline__ float one(uint8_t x) { return floats_of_codes(x).x; }
+};
 
 // ---- rotary positions
 // A pair (x, y) at position p turns by the angle p f: (x cos - y sin, x sin + y cos), times a magnitude.  Only the fraction of a turn
@@ -78,6 +114,7 @@ struct PagedPlan {
     int tq_shift, key_shift, whole, group, above, most;
     int least;                  // units that are worth a CTA
     int per_group;              // 2^16 / group, rounded up: r / group is r per_group / 2^16 for rows r of a tile (at most 256) and groups up to 32
+    int window, sinks;          // a token sees its row's last `window` keys (0: all) and the first `sinks`
 };
 __host__ __device__ __forceinline__ int paged_token(const PagedPlan &a, int r) { return (r * a.per_group) >> 16; }
 struct PagedShape {
@@ -85,15 +122,37 @@ struct PagedShape {
     long long per;              // units of a head
     long long units;
 };
-// Units of the first n tiles of a row's queries: the sum over i < n of ceil((base + (i + 1) tq) / keys), both powers of two.
+// The sum over x < y of floor(x / 2^s).
+__host__ __device__ __forceinline__ long long paged_floors(long long y, int s) {
+    const long long q = y >> s;
+    return (q * (q - 1) / 2 << s) + q * (y & ((1ll << s) - 1));
+}
+// Through a window a tile of queries sees two runs of units: those of the sinks, and those from its first token's window on.  The units between are left
+// out, and the tile's units are numbered as if there were none ("virtual" keys: those behind the sinks' units, less what is left out).
+__host__ __device__ __forceinline__ long long paged_sink_units(const PagedPlan &a) { return ((long long)a.sinks + (1 << a.key_shift) - 1) >> a.key_shift; }
+__host__ __device__ __forceinline__ int paged_gap(const PagedPlan &a, int base, int q_tile) {   // units between
+    if (!a.window) return 0;
+    const long long y = (long long)base + ((long long)q_tile << a.tq_shift) - a.window + 1, gap = (y >> a.key_shift) - paged_sink_units(a);
+    return gap > 0 ? (int)gap : 0;
+}
+__host__ __device__ __forceinline__ long long paged_gaps(const PagedPlan &a, int base, long long n) {   // their sum over the first n tiles
+    if (!a.window) return 0;
+    const long long sinks = paged_sink_units(a), y = (long long)base - a.window + 1, from = ((sinks + 1) << a.key_shift) - y;   // tile i has some where i tq >= from
+    const long long first = from > 0 ? (from + (1 << a.tq_shift) - 1) >> a.tq_shift : 0, m = n - first, y0 = y + (first << a.tq_shift);
+    if (m <= 0) return 0;
+    const int s = a.key_shift - a.tq_shift;
+    if (s <= 0) return m * ((y0 >> a.key_shift) - sinks) + ((m * (m - 1) / 2) << -s);
+    const long long c = y0 >> a.tq_shift;
+    return paged_floors(c + m, s) - paged_floors(c, s) - m * sinks;
+}
+// Units of the first n tiles of a row's queries: the sum over i < n of ceil((base + (i + 1) tq) / keys), both powers of two, less what a window leaves out.
 __host__ __device__ __forceinline__ long long paged_units(const PagedPlan &a, int base, long long n) {
     if (a.whole) return n;
     const int s = a.key_shift - a.tq_shift;
-    if (s <= 0) return n * (((long long)base + (1 << a.key_shift) - 1) >> a.key_shift) + ((n * (n + 1) / 2) << -s);
+    if (s <= 0) return n * (((long long)base + (1 << a.key_shift) - 1) >> a.key_shift) + ((n * (n + 1) / 2) << -s) - paged_gaps(a, base, n);
     // ceil((b + i + 1) / 2^s) with b = ceil(base / tq): floors of c + i over 2^s, summed up to c + n and without those up to c
     const long long c = (((long long)base + (1 << a.tq_shift) - 1) >> a.tq_shift) + (1ll << s);
-    auto floors = [&](long long y) { const long long q = y >> s; return (q * (q - 1) / 2 << s) + q * (y & ((1ll << s) - 1)); };
-    return floors(c + n) - floors(c);
+    return paged_floors(c + n, s) - paged_floors(c, s) - paged_gaps(a, base, n);
 }
 __host__ __device__ __forceinline__ PagedShape paged_shape(const PagedPlan &a, const PagedRow &r) {
     PagedShape s = {0, 0, 0, 0};
@@ -146,7 +205,7 @@ __host__ __device__ __forceinline__ long long paged_div(long long a, long long b
 // Where the run of CTA c begins.
 __host__ __device__ __forceinline__ long long paged_begin(const PagedRun &run, int c) { return paged_div(run.total * min(c, run.ctas), run.ctas); }
 __host__ __device__ __forceinline__ int paged_keys(const PagedPlan &a, int base, int q_tile) {   // units of a tile of queries
-    return a.whole ? 1 : (int)(((long long)base + ((long long)(q_tile + 1) << a.tq_shift) + (1 << a.key_shift) - 1) >> a.key_shift);
+    return a.whole ? 1 : (int)(((long long)base + ((long long)(q_tile + 1) << a.tq_shift) + (1 << a.key_shift) - 1) >> a.key_shift) - paged_gap(a, base, q_tile);
 }
 // Unit `in` of a row: its head, the tile of queries it is of, and which of that tile's.
 struct PagedUnit {
@@ -248,19 +307,35 @@ __host__ __device__ __forceinline__ bool paged_next(const PagedPlan &a, PagedRun
     run.u += w.k1 - w.k0;
     return true;
 }
-// What a piece covers: its tokens [t0, t0 + ntok) of the row's new ones, and the keys [lo, hi) of it that any of them sees.
+// What a piece covers: its tokens [t0, t0 + ntok) of the row's new ones, and the (virtual) keys [lo, hi) of it that any of them sees, or may see: hidden ones lie
+// at the ends of the units of the sinks and of the window.
 struct PagedSpan {
     int t0, ntok, base, lo, hi;
 };
+// What a window leaves out of a tile of queries: `gap` keys ahead of virtual key `jump`.
+struct PagedHole {
+    int gap, jump;
+};
+__host__ __device__ __forceinline__ PagedHole paged_hole(const PagedPlan &a, int base, int q_tile) {
+    PagedHole h;
+    h.gap = paged_gap(a, base, q_tile) << a.key_shift;
+    h.jump = h.gap ? (int)(paged_sink_units(a) << a.key_shift) : 0;
+    return h;
+}
 __host__ __device__ __forceinline__ PagedSpan paged_span(const PagedPlan &a, const PagedPiece &w) {
     PagedSpan s;
     s.t0 = w.q_tile << a.tq_shift;
     s.ntok = min(1 << a.tq_shift, w.r.count - s.t0);
     s.base = w.r.len - w.r.count;
-    const int last = s.base + s.t0 + s.ntok;   // behind the last key that a token of the item sees
+    const int last = s.base + s.t0 + s.ntok - paged_hole(a, s.base, w.q_tile).gap;   // behind the last key that a token of the item sees
     s.lo = a.whole ? 0 : (int)min((long long)w.k0 << a.key_shift, 0x7fffffffll);
     s.hi = a.whole ? last : (int)min((long long)last, (long long)w.k1 << a.key_shift);
     return s;
+}
+__host__ __device__ __forceinline__ int paged_key(const PagedHole &h, int key) { return key >= h.jump ? key + h.gap : key; }
+// Whether no token of the item sees any of the n keys from `key` (of the row) on: their page may be gone.
+__host__ __device__ __forceinline__ bool paged_hidden(const PagedPlan &a, const PagedSpan &s, int key, int n) {
+    return a.window && key >= a.sinks && key + n <= s.base + s.t0 - a.window + 1;
 }
 
 // `ctas` counts runs: CTAs, or warps where each has a run of its own.
@@ -274,6 +349,7 @@ struct PagedAttnArgs {
     int4 *cut;         // [ctas] the item that a run began and did not end: its first token, its tokens (0: there is none), its head, the run that ends it
     int ctas, tile_rows;
     int *status;
+    const float *k_scales, *v_scales;   // of e4m3 pages: one for PAGED_BLOCK tokens of a head
 };
 // Bytes that the pieces of a launch take.
 static inline size_t paged_piece_bytes(int ctas, int tile_rows, int hd) { return (size_t)2 * ctas * tile_rows * (hd + 2) * 4 + (size_t)ctas * 16; }
@@ -298,40 +374,46 @@ __host__ __device__ __forceinline__ void paged_cut(const PagedAttnArgs &a, const
     a.cut[c] = make_int4(w.r.first + sp.t0, sp.ntok, w.head, (int)min((long long)run.ctas - 1, paged_div(end * run.ctas - 1, run.total)));
 }
 
-// Row r of a piece of bf16 over the keys [lo, to] of it that it sees, by one warp: where a product with hidden values has left Inf or NaN (a weight of 0
-// times either), this gives what the keys in sight alone give.  32 keys at a time: a lane has one for the scores, and every 32nd dimension for the sums, so
-// that loads of 32 keys are in flight where one key after the other waited for its page, its shuffles and its exponential.
-template <int HD>
+// Row r of a piece (queries of bf16, pages of P: bf16, or e4m3 codes) over the keys of it that it sees, by one warp: where a product with hidden values has left Inf or
+// NaN (a weight of 0 times either), this gives what the keys in sight alone give.  32 keys at a time: a lane has one for the scores, and every 32nd dimension for the
+// sums, so that loads of 32 keys are in flight where one key after the other waited for its page, its shuffles and its exponential.
+template <int HD, typename P = __nv_bfloat16>
 __device__ __forceinline__ void paged_again(const PagedAttnArgs &a, const PagedPiece &w, const PagedSpan &sp, int r, int lane, bool all, size_t slot) {
     constexpr int N = HD / 32;
+    constexpr bool CODES = sizeof(P) == 1;
+    using Chunk = PagedChunk<P>;
     const int tok = paged_token(a.plan, r), head = w.head * a.plan.group + r - tok * a.plan.group;
-    const int to = min(sp.hi - 1, sp.base + sp.t0 + tok);
+    const PagedHole hole = paged_hole(a.plan, sp.base, w.q_tile);
+    const int pos = sp.base + sp.t0 + tok, to = min(sp.hi - 1, pos - hole.gap);
     const __nv_bfloat16 *q = (const __nv_bfloat16 *)a.q + (size_t)(w.r.first + sp.t0 + tok) * a.q_stride + (size_t)head * HD;
     float acc[N] = {}, top = -INFINITY, sum = 0.f;
     for (int key0 = sp.lo; key0 <= to; key0 += 32) {
-        const int key = key0 + lane, n = min(32, to - key0 + 1);
-        long long row = 0;
-        float s = -INFINITY;
-        if (lane < n) {
+        const int key = paged_key(hole, key0 + lane), n = min(32, to - key0 + 1);
+        long long row = -1;   // of a key out of sight
+        float s = -INFINITY, vs = 1.f;
+        if (lane < n && (!a.plan.window || key < a.plan.sinks || key > pos - a.plan.window)) {
             row = (((long long)paged_page(a.plan.p, w.row, key, a.status) * a.plan.p.kv_heads + w.head) << a.plan.p.page_shift) + (key & ((1 << a.plan.p.page_shift) - 1));
-            const __nv_bfloat16 *k = (const __nv_bfloat16 *)a.k + row * HD;
+            const P *k = (const P *)a.k + row * HD;
             s = 0.f;
 #pragma unroll 4
-            for (int d = 0; d < HD; d += 8) {
-                const uint4 x = *reinterpret_cast<const uint4 *>(q + d), y = *reinterpret_cast<const uint4 *>(k + d);
-                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+            for (int d = 0; d < HD; d += Chunk::N) {
+                float x[Chunk::N], y[Chunk::N];
+                Chunk::floats(*reinterpret_cast<const uint4 *>(k + d), y);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ys[i] << 16), s);
-                    s = fmaf(__uint_as_float(xs[i] & 0xffff0000u), __uint_as_float(ys[i] & 0xffff0000u), s);
-                }
+                for (int i = 0; i < Chunk::N; i += 8) PagedChunk<__nv_bfloat16>::floats(*reinterpret_cast<const uint4 *>(q + d + i), *reinterpret_cast<float (*)[8]>(x + i));
+#pragma unroll
+                for (int i = 0; i < Chunk::N; ++i) s = fmaf(x[i], y[i], s);
             }
             s *= a.sl;
+            if (CODES) {
+                s *= a.k_scales[row / PAGED_BLOCK];
+                vs = a.v_scales[row / PAGED_BLOCK];
+            }
         }
         float best = fmaxf(top, s);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-        const float m = best == -INFINITY ? 0.f : best, keep = exp2f(top - m), e = lane < n ? exp2f(s - m) : 0.f;
+        const float m = best == -INFINITY ? 0.f : best, keep = exp2f(top - m), e = row >= 0 ? exp2f(s - m) : 0.f;
         float here = e;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) here += __shfl_xor_sync(0xffffffffu, here, o);
@@ -341,10 +423,12 @@ __device__ __forceinline__ void paged_again(const PagedAttnArgs &a, const PagedP
         for (int i = 0; i < N; ++i) acc[i] *= keep;
 #pragma unroll 4
         for (int j = 0; j < n; ++j) {
-            const float f = __shfl_sync(0xffffffffu, e, j);
-            const __nv_bfloat16 *v = (const __nv_bfloat16 *)a.v + __shfl_sync(0xffffffffu, row, j) * HD + lane;
+            const float f = __shfl_sync(0xffffffffu, CODES ? e * vs : e, j);
+            const long long from = __shfl_sync(0xffffffffu, row, j);
+            if (from < 0) continue;
+            const P *v = (const P *)a.v + from * HD + lane;
 #pragma unroll
-            for (int i = 0; i < N; ++i) acc[i] = fmaf(f, __bfloat162float(v[32 * i]), acc[i]);
+            for (int i = 0; i < N; ++i) acc[i] = fmaf(f, Chunk::one(v[32 * i]), acc[i]);
         }
     }
     const float f = sum == 0.f ? 0.f : 1.f / sum;

@@ -293,6 +293,29 @@ PagedView paged_view(const ab2_paged *c) {
     return v;
 }
 
+// What the appends look their arguments over for; `page_es`: bytes of an element of the pages.
+int append_check(const ab2_paged *cache, long long page_es, const void *k_dev, long long k_stride, const void *v_dev, long long v_stride, const void *q_dev, long long q_stride, int heads, void *q_out_dev,
+                 long long q_out_stride, const double *frequencies_dev, int rot_dims, int layout, ab2_dtype dtype) {
+    int rc = paged_check(cache, dtype);
+    if (rc != AB2_OK) return rc;
+    rc = check_layout(layout, cache->head_dim, rot_dims, frequencies_dev);
+    if (rc != AB2_OK) return rc;
+    AB2_REQUIRE(heads >= 0, AB2_ERR_BAD_SHAPE, "%d heads", heads);
+    if (cache->tokens == 0) return AB2_OK;
+    AB2_REQUIRE(k_dev && v_dev && (heads == 0 || (q_dev && q_out_dev)), AB2_ERR_BAD_ARG, "null argument");
+    AB2_REQUIRE(on_elements({k_dev, v_dev, heads ? q_dev : nullptr, heads ? q_out_dev : nullptr}, dtype), AB2_ERR_BAD_ALIGN, "tensors must lie on their elements");
+    const long long row = (long long)heads * cache->head_dim, krow = (long long)cache->kv_heads * cache->head_dim;
+    AB2_REQUIRE((heads + 2ll * cache->kv_heads) * cache->head_dim < (1ll << 30), AB2_ERR_BAD_SHAPE, "%d and %d heads of %d are too many", heads, cache->kv_heads, cache->head_dim);
+    AB2_REQUIRE(k_stride >= krow && v_stride >= krow && (heads == 0 || (q_stride >= row && q_out_stride >= row)), AB2_ERR_BAD_SHAPE, "a token's heads lie one after the other, and tokens do not overlap");
+    const long long es = (long long)dtype_size(dtype), pool = (long long)cache->pages * cache->page_size * krow * page_es;
+    const RowsAt qo_at = {heads ? q_out_dev : nullptr, row * es, q_out_stride * es, cache->tokens}, kp_at = {cache->k_pages, pool, pool, 1}, vp_at = {cache->v_pages, pool, pool, 1};
+    AB2_REQUIRE(in_place_or_apart(qo_at, {heads ? q_dev : nullptr, row * es, q_stride * es, cache->tokens}) && !rows_meet(qo_at, {k_dev, krow * es, k_stride * es, cache->tokens}) &&
+                    !rows_meet(qo_at, {v_dev, krow * es, v_stride * es, cache->tokens}),
+                AB2_ERR_BAD_ARG, "the rotated queries take the queries' place, or lie apart from queries, keys and values");
+    AB2_REQUIRE(!rows_meet(kp_at, vp_at) && !rows_meet(qo_at, kp_at) && !rows_meet(qo_at, vp_at), AB2_ERR_BAD_ARG, "pages of keys, pages of values and the rotated queries lie apart");
+    return AB2_OK;
+}
+
 }  // namespace ab2
 
 AB2_API int ab2_rotary_apply(const void *q_dev, long long q_stride, int heads, const void *k_dev, long long k_stride, int kv_heads, int head_dim,
@@ -323,23 +346,8 @@ AB2_API int ab2_rotary_apply(const void *q_dev, long long q_stride, int heads, c
 
 AB2_API int ab2_paged_append(const ab2_paged *cache, const void *k_dev, long long k_stride, const void *v_dev, long long v_stride, const void *q_dev, long long q_stride,
                              int heads, void *q_out_dev, long long q_out_stride, const double *frequencies_dev, int rot_dims, int layout, float magnitude, ab2_dtype dtype, ab2_stream stream) {
-    int rc = paged_check(cache, dtype);
-    if (rc != AB2_OK) return rc;
-    rc = check_layout(layout, cache->head_dim, rot_dims, frequencies_dev);
-    if (rc != AB2_OK) return rc;
-    AB2_REQUIRE(heads >= 0, AB2_ERR_BAD_SHAPE, "%d heads", heads);
-    if (cache->tokens == 0) return AB2_OK;
-    AB2_REQUIRE(k_dev && v_dev && (heads == 0 || (q_dev && q_out_dev)), AB2_ERR_BAD_ARG, "null argument");
-    AB2_REQUIRE(on_elements({k_dev, v_dev, heads ? q_dev : nullptr, heads ? q_out_dev : nullptr}, dtype), AB2_ERR_BAD_ALIGN, "tensors must lie on their elements");
-    const long long row = (long long)heads * cache->head_dim, krow = (long long)cache->kv_heads * cache->head_dim;
-    AB2_REQUIRE((heads + 2ll * cache->kv_heads) * cache->head_dim < (1ll << 30), AB2_ERR_BAD_SHAPE, "%d and %d heads of %d are too many", heads, cache->kv_heads, cache->head_dim);
-    AB2_REQUIRE(k_stride >= krow && v_stride >= krow && (heads == 0 || (q_stride >= row && q_out_stride >= row)), AB2_ERR_BAD_SHAPE, "a token's heads lie one after the other, and tokens do not overlap");
-    const long long es = (long long)dtype_size(dtype), pool = (long long)cache->pages * cache->page_size * krow * es;
-    const RowsAt qo_at = {heads ? q_out_dev : nullptr, row * es, q_out_stride * es, cache->tokens}, kp_at = {cache->k_pages, pool, pool, 1}, vp_at = {cache->v_pages, pool, pool, 1};
-    AB2_REQUIRE(in_place_or_apart(qo_at, {heads ? q_dev : nullptr, row * es, q_stride * es, cache->tokens}) && !rows_meet(qo_at, {k_dev, krow * es, k_stride * es, cache->tokens}) &&
-                    !rows_meet(qo_at, {v_dev, krow * es, v_stride * es, cache->tokens}),
-                AB2_ERR_BAD_ARG, "the rotated queries take the queries' place, or lie apart from queries, keys and values");
-    AB2_REQUIRE(!rows_meet(kp_at, vp_at) && !rows_meet(qo_at, kp_at) && !rows_meet(qo_at, vp_at), AB2_ERR_BAD_ARG, "pages of keys, pages of values and the rotated queries lie apart");
+    int rc = append_check(cache, (long long)dtype_size(dtype), k_dev, k_stride, v_dev, v_stride, q_dev, q_stride, heads, q_out_dev, q_out_stride, frequencies_dev, rot_dims, layout, dtype);
+    if (rc != AB2_OK || cache->tokens == 0) return rc;
     RotArgs a = {};
     a.k = k_dev; a.v = v_dev; a.k_stride = k_stride; a.v_stride = v_stride;
     if (heads) { a.q = q_dev; a.qo = q_out_dev; a.q_stride = q_stride; a.qo_stride = q_out_stride; }

@@ -397,21 +397,43 @@ def _paged(k_pages, v_pages, table, lens, starts, tokens: int):
     return c, (table, lens, starts)
 
 
+def _scales(scales, k_pages, v_pages):
+    """The scales of keys and of values where pages hold 8 bits; (None, None) where they do not."""
+    codes = k_pages.dtype is torch.float8_e4m3fn
+    if scales is not None and (not isinstance(scales, (tuple, list)) or len(scales) != 2):
+        raise _lib.Ab2Error(-7, "scales are a pair, those of keys and those of values")
+    if codes != (scales is not None):
+        raise _lib.Ab2Error(-7, "pages of float8_e4m3fn need scales" if codes else f"pages of {k_pages.dtype} have no scales")
+    if not codes:
+        return None, None
+    if k_pages.dim() != 4:
+        raise _lib.Ab2Error(-1, f"pages must be [pages, kv_heads, page_size, head_dim], got {list(k_pages.shape)}")
+    shape = (k_pages.shape[0], k_pages.shape[1], k_pages.shape[2] // _lib.PAGED_BLOCK)
+    for t in scales:
+        if not t.is_contiguous():
+            raise _lib.Ab2Error(-1, "scales must be contiguous")
+    return tuple(_typed(t, torch.float32, shape, f"scales of {w}") for t, w in zip(scales, ("keys", "values")))
+
+
 def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
                  starts: torch.Tensor | None = None, q: torch.Tensor | None = None, frequencies: torch.Tensor | None = None, layout: str = "half",
-                 magnitude: float = 1.0, out: torch.Tensor | None = None):
+                 magnitude: float = 1.0, out: torch.Tensor | None = None, scales=None):
     """Writes the new tokens' k (rotated at their positions in their rows, as they are without ``frequencies``) and v
     [tokens, kv_heads, dim] to the pages that ``table`` [rows, pages] names; ``lens`` [rows] are the rows' tokens with the new ones,
-    ``starts`` [rows + 1] where a row's new tokens begin (None: one a row).  Returns the rotated q [tokens, heads, dim], if any."""
-    if out is None and _fast is not None:
+    ``starts`` [rows + 1] where a row's new tokens begin (None: one a row).  Returns the rotated q [tokens, heads, dim], if any.
+
+    Pages of 8 bits (float8_e4m3fn) have ``scales``, those of keys and those of values, each [pages, kv_heads, page_size / 16] f32: a value is its code times the
+    scale of its 16 tokens, a power of two that grows with the tokens that come (earlier ones' codes are made anew then)."""
+    if out is None and scales is None and _fast is not None:
         got = _fast.append(k_pages, v_pages, k, v, table, lens, starts, q, frequencies, layout, magnitude)
         if got is not None:
             return check(got) if type(got) is int else got if got is not True else None
-    _on_device(k_pages, v_pages, k, v, table, lens, starts, q, frequencies)
+    k_scales, v_scales = _scales(scales, k_pages, v_pages)
+    _on_device(k_pages, v_pages, k, v, table, lens, starts, q, frequencies, k_scales, v_scales)
     k, ks = _heads(k, "k")
     v, vs = _heads(v, "v")
     n, kv, d = k.shape
-    if v.shape != k.shape or v.dtype != k.dtype or k.dtype != k_pages.dtype:
+    if v.shape != k.shape or v.dtype != k.dtype or scales is None and k.dtype != k_pages.dtype:
         raise _lib.Ab2Error(-1, f"k {list(k.shape)} {k.dtype} and v {list(v.shape)} {v.dtype} do not match each other and pages of {k_pages.dtype}")
     c, _keep = _paged(k_pages, v_pages, table, lens, starts, n)
     if (kv, d) != (c.kv_heads, c.head_dim):
@@ -428,6 +450,11 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, 
             qo, qos = _fresh(q), h * d
         else:
             qo, qos = _result(out, q, "out")
+    if k_scales is not None:
+        check(lib.ab2_paged_append_e4m3(C.byref(c), k_scales.data_ptr(), v_scales.data_ptr(), k.data_ptr(), ks, v.data_ptr(), vs, q.data_ptr() if q is not None else None, qs, h,
+                                        qo.data_ptr() if qo is not None else None, qos, frequencies.data_ptr() if frequencies is not None else None, rot,
+                                        _lib.ROTARY[layout], magnitude, dtype_code(k.dtype), stream_ptr()))
+        return qo
     check(lib.ab2_paged_append(C.byref(c), k.data_ptr(), ks, v.data_ptr(), vs, q.data_ptr() if q is not None else None, qs, h,
                                qo.data_ptr() if qo is not None else None, qos, frequencies.data_ptr() if frequencies is not None else None, rot,
                                _lib.ROTARY[layout], magnitude, dtype_code(k.dtype), stream_ptr()))
@@ -435,20 +462,27 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, 
 
 
 def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float,
-                    starts: torch.Tensor | None = None, max_new: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                    starts: torch.Tensor | None = None, max_new: int | None = None, out: torch.Tensor | None = None, scales=None, window: int = 0,
+                    sinks: int = 0) -> torch.Tensor:
     """q [tokens, heads, dim]: each row's new tokens, whose keys and values have been appended, attend to the row's keys up to their
     own; table, lens and starts as in ``paged_append``.  ``max_new`` bounds the new tokens of a row (None: not known); it picks
     kernels, whose results differ by rounding.  Over bf16 a softmax weight keeps 16 bits where a row's new tokens times the query heads of a KV head are
-    at most 16, and 8 where they are more.  Tokens behind the last row are left as ``out`` (not q) holds them."""
-    if out is None and _fast is not None:
+    at most 16, and 8 where they are more.  Tokens behind the last row are left as ``out`` (not q) holds them.
+
+    ``scales``: of pages of 8 bits, as in ``paged_append``; a weight keeps 11 bits there, or 8.  With a ``window`` a token sees its row's last so many keys, its own
+    among them, and the first ``sinks`` of the row; pages that hold no key in sight of a row's new tokens are not looked at."""
+    if out is None and scales is None and not window and not sinks and _fast is not None:
         got = _fast.attention(q, k_pages, v_pages, table, lens, scale, starts, max_new)
         if got is not None:
             return check(got) if type(got) is int else got
-    _on_device(q, k_pages, v_pages, table, lens, starts)
+    k_scales, v_scales = _scales(scales, k_pages, v_pages)
+    _on_device(q, k_pages, v_pages, table, lens, starts, k_scales, v_scales)
     q, qs = _heads(q, "q")
     n, h, d = q.shape
-    if q.dtype != k_pages.dtype:
+    if q.dtype != k_pages.dtype and scales is None:
         raise _lib.Ab2Error(-3, f"queries of {q.dtype} over pages of {k_pages.dtype}")
+    if not 0 <= window <= 2 ** 30 or not 0 <= sinks <= 2 ** 30 or sinks and not window:
+        raise _lib.Ab2Error(-1, f"a window of {window} keys and {sinks} first ones: up to 2^30 of each are served, and first ones beside a window")
     c, _keep = _paged(k_pages, v_pages, table, lens, starts, n)
     if d != c.head_dim:
         raise _lib.Ab2Error(-1, f"queries have heads of {d}, the pages of {c.head_dim}")
@@ -464,8 +498,13 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         check(lib.ab2_paged_workspace(d, C.byref(size)))
     size = size.value
     work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    check(lib.ab2_paged_attention(C.byref(c), q.data_ptr(), qs, h, out.data_ptr(), os, max_new, scale, work.data_ptr() if size else None, size,
-                                  dtype_code(q.dtype), stream_ptr()))
+    rest = (q.data_ptr(), qs, h, out.data_ptr(), os, max_new, scale, work.data_ptr() if size else None, size, dtype_code(q.dtype), stream_ptr())
+    if k_scales is not None:
+        check(lib.ab2_paged_attention_e4m3(C.byref(c), k_scales.data_ptr(), v_scales.data_ptr(), window, sinks, *rest))
+    elif window:
+        check(lib.ab2_paged_attention_window(C.byref(c), window, sinks, *rest))
+    else:
+        check(lib.ab2_paged_attention(C.byref(c), *rest))
     return out
 
 

@@ -139,21 +139,25 @@ class PagedStep:
 
 class PagedKVCache:
     """Keys and values in pages of one pool that the sequences share: a sequence holds as many as its tokens need, in any order, where
-    ``KVCache`` gives each the same capacity for good.  ``k`` and ``v`` are [layers, pages, kv_heads, page_size, head_dim] (f32 or bf16).
+    ``KVCache`` gives each the same capacity for good.  ``k`` and ``v`` are [layers, pages, kv_heads, page_size, head_dim] (f32, bf16, or e4m3 with
+    ``k_scales`` and ``v_scales`` [layers, pages, kv_heads, page_size / 16] f32: half the room of bf16, for queries, keys and values of bf16 or f32).
     A pass over some rows: ``step`` takes the pages it needs, then for every layer ``append`` and ``attention``, at its end ``commit``.  A step whose rows
     have been cut back or have moved on since is refused: its pages may be another row's.
     Calls on a cache go on one stream, or are ordered by the caller."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, batch: int = 1, n_layers: int = 1, dtype: str = "bf16", device="cuda"):
-        if dtype not in ("f32", "bf16"):
-            raise _lib.Ab2Error(-3, f"paged caches hold f32 or bf16, not {dtype}")
+        if dtype not in ("f32", "bf16", "e4m3"):
+            raise _lib.Ab2Error(-3, f"paged caches hold f32, bf16 or e4m3, not {dtype}")
         if page_size not in (16, 32, 64, 128, 256) or head_dim not in (64, 128):
             raise _lib.Ab2Error(-8, f"pages of {page_size} tokens, heads of {head_dim}: 16, 32, 64, 128 or 256 tokens and heads of 64 or 128 are served")
         if min(pages, kv_heads, batch, n_layers) <= 0:
             raise _lib.Ab2Error(-1, f"paged cache of {pages} pages, {kv_heads} heads, {batch} rows, {n_layers} layers")
         self.page_size, self.kv_heads, self.head_dim, self.batch, self.n_layers, self.dtype = page_size, kv_heads, head_dim, batch, n_layers, dtype
-        self.k, self.v = (torch.zeros((n_layers, pages, kv_heads, page_size, head_dim), dtype=torch.float32 if dtype == "f32" else torch.bfloat16, device=device)
-                          for _ in range(2))
+        kind = {"f32": torch.float32, "bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn}[dtype]
+        self.k, self.v = (torch.zeros((n_layers, pages, kv_heads, page_size, head_dim), dtype=kind, device=device) for _ in range(2))
+        self.k_scales = self.v_scales = None
+        if dtype == "e4m3":
+            self.k_scales, self.v_scales = (torch.zeros((n_layers, pages, kv_heads, page_size // _lib.PAGED_BLOCK), dtype=torch.float32, device=device) for _ in range(2))
         self._free = list(range(pages - 1, -1, -1))
         self._pages = [[] for _ in range(batch)]
         self._lens = [0] * batch
@@ -220,13 +224,16 @@ class PagedKVCache:
         """``dispatch.paged_append`` on a layer: k, v (and q) [step.tokens, heads, dim]."""
         from .dispatch import paged_append
         self._holds(step, k)
-        return paged_append(self.k[layer], self.v[layer], k, v, step.table, step.lens, step.starts, q, frequencies, layout, magnitude, out)
+        return paged_append(self.k[layer], self.v[layer], k, v, step.table, step.lens, step.starts, q, frequencies, layout, magnitude, out, self._scales(layer))
 
-    def attention(self, step: PagedStep, q: torch.Tensor, scale: float, layer: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
-        """``dispatch.attention_paged`` on a layer: q [step.tokens, heads, dim]."""
+    def attention(self, step: PagedStep, q: torch.Tensor, scale: float, layer: int = 0, out: torch.Tensor | None = None, window: int = 0, sinks: int = 0) -> torch.Tensor:
+        """``dispatch.attention_paged`` on a layer: q [step.tokens, heads, dim]; with a ``window`` a token sees its last so many keys and the first ``sinks``."""
         from .dispatch import attention_paged
         self._holds(step, q)
-        return attention_paged(q, self.k[layer], self.v[layer], step.table, step.lens, scale, step.starts, step.max_new, out)
+        return attention_paged(q, self.k[layer], self.v[layer], step.table, step.lens, scale, step.starts, step.max_new, out, self._scales(layer), window, sinks)
+
+    def _scales(self, layer: int):
+        return None if self.k_scales is None else (self.k_scales[layer], self.v_scales[layer])
 
     def _holds(self, step, t=None):
         if t is not None and t.shape[0] < step.tokens:
@@ -261,4 +268,11 @@ class PagedKVCache:
         """The row's keys and values [len, kv_heads, head_dim] in f32."""
         n = self.seq_len(row)
         at = torch.tensor(self._pages[row], dtype=torch.int64, device=self.k.device)
-        return tuple(p[layer][at].transpose(1, 2).reshape(-1, self.kv_heads, self.head_dim)[:n].float() for p in (self.k, self.v))
+        both = []
+        for p, scales in ((self.k, self.k_scales), (self.v, self.v_scales)):
+            if scales is None:
+                x = p[layer][at]
+            else:
+                x = p[layer].view(torch.uint8)[at].view(torch.float8_e4m3fn).float() * scales[layer][at].repeat_interleave(_lib.PAGED_BLOCK, dim=-1)[..., None]
+            both.append(x.transpose(1, 2).reshape(-1, self.kv_heads, self.head_dim)[:n].float())
+        return tuple(both)

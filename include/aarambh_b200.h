@@ -399,6 +399,25 @@ int ab2_paged_append(const ab2_paged *cache, const void *k_dev, long long k_stri
 int ab2_paged_workspace(int head_dim, size_t *bytes);
 int ab2_paged_attention(const ab2_paged *cache, const void *q_dev, long long q_stride, int heads, void *out_dev, long long out_stride, int max_new, float scale,
                         void *workspace_dev, size_t workspace_bytes, ab2_dtype dtype, ab2_stream stream);
+/* The same through a window: a token at position i sees the keys j <= i with i - j < window (0: all of them) or j < sinks, up to 2^30 of each, sinks only
+ * beside a window.  Table entries of pages that hold no key which any new token of the row sees are not read: such pages may be another row's. */
+int ab2_paged_attention_window(const ab2_paged *cache, int window, int sinks, const void *q_dev, long long q_stride, int heads, void *out_dev, long long out_stride,
+                               int max_new, float scale, void *workspace_dev, size_t workspace_bytes, ab2_dtype dtype, ab2_stream stream);
+/* Pages of 8 bits: k_pages and v_pages [pages][kv_heads][page_size][head_dim] hold e4m3 codes, k_scales_dev and v_scales_dev
+ * [pages][kv_heads][page_size / 16] f32 a scale for every 16 tokens of a head; a value is its code times its scale.  `dtype` is that of q, k and v.
+ *
+ * The append gives a block the least power of two (2^-118 at least) with which its new values (k rotated and rounded to `dtype`), divided by it, are at
+ * most 448, or the scale that it has where it holds earlier tokens and that is larger; where it grows, earlier tokens' codes are made anew from their values.
+ * Codes are rounded to nearest, Inf and NaN become NaN.  Codes of slots that hold no token are left as they are.  Pages, scales and all else lie apart.
+ *
+ * The attention takes scales that are powers of two as they are; of other scales a chunk's values (code times scale) are rounded to bf16.  Over bf16 queries the
+ * weights of rows of up to 16 query rows are rounded to f16 (2^-11 each), of more to bf16 (2^-8 each). */
+int ab2_paged_append_e4m3(const ab2_paged *cache, float *k_scales_dev, float *v_scales_dev, const void *k_dev, long long k_stride, const void *v_dev,
+                          long long v_stride, const void *q_dev, long long q_stride, int heads, void *q_out_dev, long long q_out_stride,
+                          const double *frequencies_dev, int rot_dims, int layout, float magnitude, ab2_dtype dtype, ab2_stream stream);
+int ab2_paged_attention_e4m3(const ab2_paged *cache, const float *k_scales_dev, const float *v_scales_dev, int window, int sinks, const void *q_dev,
+                             long long q_stride, int heads, void *out_dev, long long out_stride, int max_new, float scale, void *workspace_dev,
+                             size_t workspace_bytes, ab2_dtype dtype, ab2_stream stream);
 /* Rules of a sampler on logits [rows][vocab] (`stride` elements from row to row) to out_dev [rows][vocab], which may be the logits where
  * stride = vocab, and lies apart from them otherwise.  With c the times a token occurs in history_dev [rows][history_width] (i32, the first lengths_dev[row] of a row or, NULL, all;
  * ids outside the vocabulary are passed over) and rules_dev [rows][3] = {repetition > 0, presence, frequency}: where c > 0, z = z > 0 ? z /
