@@ -104,6 +104,7 @@ SIGNATURES = {
     "ab2_paged_attention_window": ([_p, _i, _i, _p, _ll, _i, _p, _ll, _i, _f, _p, C.c_size_t, _i, _p], _i),
     "ab2_paged_append_e4m3": ([_p, _p, _p, _p, _ll, _p, _ll, _p, _ll, _i, _p, _ll, _p, _i, _i, _f, _i, _p], _i),
     "ab2_paged_attention_e4m3": ([_p, _p, _p, _i, _i, _p, _ll, _i, _p, _ll, _i, _f, _p, C.c_size_t, _i, _p], _i),
+    "ab2_sample": ([_p, _ll, _i, _i, _p, _i, _p, _p, _p, _p, _p, _i, _p], _i),
     "ab2_adjust_logits": ([_p, _ll, _i, _i, _p, _ll, _i, _p, _p, _p, _p, _i, _p, _p, _i, _p], _i),
     "ab2_model_create": ([_pp, _p, _i, _i], _i),
     "ab2_model_create_stack": ([_pp, _p, _p, _i, _i], _i),

@@ -575,3 +575,32 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, len
     check(lib.ab2_adjust_logits(logits.data_ptr(), stride, rows, vocab, hp, hs, width, lp, rp, bp, vp, biases, ap, out.data_ptr(),
                                 dtype_code(logits.dtype), stream_ptr()))
     return out
+
+
+def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
+           min_p: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """A token of each row of logits [rows, vocab] by the given ``uniforms`` [rows] (f32 or f64, 0 <= u < 1): int32 [rows].
+
+    Tokens go by falling logit / temperature, of equal ones the lower index first: the first ``top_k`` stay (0: all), of these the shortest prefix that holds
+    ``top_p`` of their mass (1: all), of these the ones with ``min_p`` of the likeliest one's probability or more (0: all).  The token is the first that stayed, in
+    order of index, whose cumulative mass exceeds u times all of theirs.  All four are [rows], f32 (top_k int32), or None.  A temperature that is not positive gives
+    the likeliest token; NaN and -inf are never drawn, and a row with nothing else answers -1."""
+    _on_device(logits, uniforms, temperature, top_k, top_p, min_p, out)
+    if logits.dim() != 2:
+        raise _lib.Ab2Error(-1, f"logits must be [rows, vocab], got {list(logits.shape)}")
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < vocab:
+        logits = logits.contiguous()
+    if uniforms.dtype not in (torch.float32, torch.float64):
+        raise _lib.Ab2Error(-3, f"uniforms must be f32 or f64, got {uniforms.dtype}")
+    uniforms = _typed(uniforms, uniforms.dtype, (rows,), "uniforms")
+    rules = []
+    for t, dtype, what in ((temperature, torch.float32, "temperature"), (top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p")):
+        rules.append(None if t is None else _typed(t, dtype, (rows,), what))
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    elif out.dtype != torch.int32 or out.shape != (rows,) or not out.is_contiguous():
+        raise _lib.Ab2Error(-1, f"out must be contiguous int32 [{rows}]")
+    check(lib.ab2_sample(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, uniforms.data_ptr(), uniforms.dtype == torch.float64,
+                         *(t.data_ptr() if t is not None else None for t in rules), out.data_ptr(), dtype_code(logits.dtype), stream_ptr()))
+    return out

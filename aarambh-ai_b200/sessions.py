@@ -10,18 +10,19 @@ Sessions live in the rows of ONE batched KV cache; a decode pass over sessions
 with different lengths is ONE forward over the list of their rows, whatever rows
 they occupy (per-row lengths, one attention launch for all of them), where the
 reference loops over rows.  Sampling here is greedy (last maximum, as ``argmax`` in
-sampler.rs:217-224); text, tools and stochastic samplers stay with the caller.
+sampler.rs:217-224) or, for sessions with a ``Sampling``, by temperature, top-k, top-p and min-p; text and tools stay with the caller.
 """
 from __future__ import annotations
 
 import math
+import random
 from collections.abc import Callable
 from dataclasses import dataclass, field
 
 import torch
 
 from . import _lib
-from .dispatch import adjust_logits, allowed_words, argmax
+from .dispatch import adjust_logits, allowed_words, argmax, sample
 from .model import DecoderModel
 
 
@@ -65,6 +66,29 @@ class LogitRules:
 
 
 @dataclass
+class Sampling:
+    """How a session's next token is drawn (``dispatch.sample``), by a generator of its own: sessions with equal seeds and logits draw equal tokens, whoever shares
+    their batch."""
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    seed: int = 0
+
+    def __post_init__(self):
+        if not (self.temperature >= 0 and math.isfinite(self.temperature)) or self.top_k < 0 or not 0 <= self.top_p <= 1 or not 0 <= self.min_p <= 1:
+            raise _lib.Ab2Error(-7, f"a temperature of 0 or more, top-k of 0 or more, top-p and min-p from 0 to 1, got {self}")
+        self._random = random.Random(self.seed)
+
+    def draw(self, logits: torch.Tensor) -> torch.Tensor:
+        """logits [1, vocab] -> the token [1]."""
+        numbers = torch.tensor([self.temperature, self.top_p, self.min_p], dtype=torch.float32).to(logits.device)
+        u = torch.tensor([self._random.random()], dtype=torch.float64).to(logits.device)
+        top_k = torch.tensor([min(self.top_k, logits.shape[-1])], dtype=torch.int32).to(logits.device)
+        return sample(logits, u, numbers[0:1], top_k, numbers[1:2], numbers[2:3])
+
+
+@dataclass
 class GenerationSession:
     row: int
     prompt_len: int
@@ -76,6 +100,7 @@ class GenerationSession:
     finished: bool = False
     rules: LogitRules | None = None
     prompt_ids: list = field(default_factory=list)
+    sampling: Sampling | None = None
 
     def is_finished(self) -> bool:
         return self.finished
@@ -141,7 +166,7 @@ class SessionEngine:
 
     # -- engine.rs:271-318 ---------------------------------------------------
     def prepare_session_with_chunk_size(self, prompt_ids, max_new_tokens: int, chunk_size: int = 128,
-                                        eos_token_id: int | None = None, rules: LogitRules | None = None) -> GenerationSession:
+                                        eos_token_id: int | None = None, rules: LogitRules | None = None, sampling: Sampling | None = None) -> GenerationSession:
         if chunk_size <= 0:
             raise _lib.Ab2Error(-1, "prefill chunk size must be greater than zero")
         ids = [int(t) for t in prompt_ids]
@@ -156,9 +181,9 @@ class SessionEngine:
             chunk = torch.tensor([ids[off:off + chunk_size]])
             logits = self.model.forward_with_cache(chunk, off, self.cache, row=row, last_only=True)
         return GenerationSession(row, len(ids), min(max_new_tokens, max_seq - len(ids)), logits.view(-1),
-                                 eos_token_id=eos_token_id, rules=rules, prompt_ids=ids if rules is not None else [])
+                                 eos_token_id=eos_token_id, rules=rules, prompt_ids=ids if rules is not None else [], sampling=sampling)
 
-    # -- GenerationSession::advance, greedy (engine.rs:822-976) ---------------
+    # -- GenerationSession::advance (engine.rs:822-976) ------------------------
     def advance(self, session: GenerationSession) -> int | None:
         """Samples the next token from ``next_logits``, under the session's rules if it has any; it becomes the
         pending token of the next decode pass.  Returns it, or None once finished."""
@@ -167,7 +192,9 @@ class SessionEngine:
         logits = session.next_logits.view(1, -1)
         if session.rules is not None:
             logits = session.rules.apply(logits, session.prompt_ids, session.generated_ids)
-        token = int(argmax(logits)[0])
+        token = int((argmax(logits) if session.sampling is None else session.sampling.draw(logits))[0])
+        if token < 0:
+            raise _lib.Ab2Error(-7, "no token of the session has a logit above -inf")
         if session.rules is not None and session.rules.allowed is not None and float(logits[0, token]) == -math.inf:
             raise _lib.Ab2Error(-7, "no token that the session's rules allow has a logit above -inf")
         session.generated_ids.append(token)
