@@ -25,7 +25,8 @@ int device_sm_count();
 namespace {
 
 typedef unsigned long long u64;
-constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32, SP_BINS = 2048, SP_PER = 32, SP_LIST = 4096, SP_MINE = SP_LIST / SP_THREADS, SP_CTAS = 8, SP_TABLE = 256;
+constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32, SP_BINS = 4096, SP_PER = 64, SP_LIST = 1024, SP_MINE = SP_LIST / SP_THREADS, SP_CTAS = 8;
+constexpr float SP_MAGIC = 12582912.f;   // 1.5 2^23: added to a float, its low bits are the nearest whole number's
 
 struct SampleArgs {
     const void *logits, *uniforms;
@@ -49,10 +50,12 @@ struct alignas(16) SampleShared {
     };
     u64 list[SP_LIST];            // tokens: key and, below it, what is larger for lower indices
     u64 weights[SP_LIST];
-    double powers[SP_TABLE];      // 2^(-j / SP_TABLE)
     u64 red[2][SP_WARPS], slot[2], part[SP_WARPS];
     float scan[3][SP_WARPS];
-    int top_bits, listed, found[4];
+    uint32_t powers[256];         // 2^(j / 256), times 2^31
+    float tops[2];                // the slice's largest logit, and one that so many of its tokens reach; read by the cluster's others
+    int listed, found[4], index;
+    uint32_t key_range[2];        // read by the cluster's others
     u64 cut;
 };
 
@@ -66,47 +69,58 @@ __device__ __forceinline__ float logit_of(uint32_t key) { return key == 0u ? -IN
 __device__ __forceinline__ u64 token_of(uint32_t key, int index) { return (u64)key << 32 | (0xffffffffu - (uint32_t)index); }
 __device__ __forceinline__ int index_of(u64 token) { return (int)(0xffffffffu - (uint32_t)token); }
 
-// Sorts list[0, n) by falling values; what lies behind n, up to the next power of two or SP_THREADS, becomes 0.  Bitonic: a thread an element, exchanged by shuffles
-// where the partner is in the warp; longer lists in shared memory throughout.
+// 2^F 2^-x as a whole number, x = (top - z) c: for logits, temperatures and powers of two out of the ordinary.
+__device__ __noinline__ u64 weight_of(float z, float top, double c, int shift) {
+    if (z == top) return 1ull << shift;
+    const double x = ((double)top - (double)z) * c;
+    return x < (double)shift + 2.0 ? __double2ull_rn(exp2((double)shift - x)) : 0ull;   // NaN and -inf: 0
+}
+
+// Sorts E values of each thread, value e of thread t being e SP_THREADS + t, to fall.  Bitonic: partners are exchanged by shuffles where they are in the warp.
+template <int E, typename X> __device__ __forceinline__ void sort_threads(X (&v)[E], X *buffer) {
+    const int tid = threadIdx.x;
+    for (int k = 2; k <= E * SP_THREADS; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            if (E == 2 && j == SP_THREADS) {
+                const X a = v[0], b = v[E - 1];
+                v[0] = a > b ? a : b;
+                v[E - 1] = a > b ? b : a;
+                continue;
+            }
+            X o[E];
+            if (j >= 32) {
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < E; ++e) buffer[e * SP_THREADS + tid] = v[e];
+                __syncthreads();
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = j >= 32 ? buffer[(e * SP_THREADS + tid) ^ j] : __shfl_xor_sync(0xffffffffu, v[e], j & 31);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const bool falls = ((e * SP_THREADS + tid) & k) == 0, larger = ((tid & j) == 0) == falls;   // of the two this thread keeps the larger one
+                v[e] = (o[e] > v[e]) == larger ? o[e] : v[e];
+            }
+        }
+}
+// Sorts list[0, n), up to 2 SP_THREADS, to fall; what lies behind becomes 0.
 __device__ __forceinline__ void sort_list(u64 *list, int n) {
     const int tid = threadIdx.x;
     if (n <= SP_THREADS) {
-        u64 v = tid < n ? list[tid] : 0ull;
-        for (int k = 2; k <= SP_THREADS; k <<= 1) {
-            const bool falls = (tid & k) == 0;
-            for (int j = k >> 1; j > 0; j >>= 1) {
-                u64 o;
-                if (j >= 32) {
-                    __syncthreads();
-                    list[tid] = v;
-                    __syncthreads();
-                    o = list[tid ^ j];
-                } else {
-                    o = __shfl_xor_sync(0xffffffffu, v, j);
-                }
-                const bool larger = ((tid & j) == 0) == falls;   // of the two this thread keeps the larger one
-                v = (o > v) == larger ? o : v;
-            }
-        }
+        u64 v[1] = {tid < n ? list[tid] : 0ull};
+        sort_threads<1>(v, list);
         __syncthreads();
-        list[tid] = v;
+        list[tid] = v[0];
+    } else {
+        u64 v[2] = {list[tid], tid + SP_THREADS < n ? list[tid + SP_THREADS] : 0ull};
+        sort_threads<2>(v, list);
         __syncthreads();
-        return;
+        list[tid] = v[0];
+        list[tid + SP_THREADS] = v[1];
     }
-    int all = SP_THREADS;
-    while (all < n) all <<= 1;
-    for (int i = n + tid; i < all; i += SP_THREADS) list[i] = 0ull;
-    for (int k = 2; k <= all; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            __syncthreads();
-            for (int t = tid; t < all / 2; t += SP_THREADS) {
-                const int i = 2 * t - (t & (j - 1));
-                const u64 x = list[i], y = list[i + j];
-                if ((x < y) == ((i & k) == 0)) { list[i] = y; list[i + j] = x; }
-            }
-        }
     __syncthreads();
 }
+static_assert(SP_LIST == 2 * SP_THREADS, "what a sort takes");
 
 template <typename T, bool CACHED>
 __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_constant__ SampleArgs a) {
@@ -118,11 +132,22 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
     const int first = rank * a.slice, n = max(0, min(a.slice, a.vocab - first));
     const T *in = (const T *)a.logits + row * a.stride + first;
 
+    const float temperature = a.temperature ? a.temperature[row] : 1.f;
+    const bool warm = temperature > 0.f;   // else the likeliest token
+    const double c = warm ? 1.4426950408889634 / (double)temperature : INFINITY;
+    const float top_p = a.top_p ? a.top_p[row] : 1.f;
+    float min_p = a.min_p ? a.min_p[row] : 0.f;
+    int k = a.top_k ? a.top_k[row] : 0;
+    if (!warm || min_p > 1.f) k = 1;
+    min_p = fminf(min_p, 1.f);   // NaN: 1, the likeliest and what is as likely
+    const bool by_p = top_p < 1.f;
+
     // ---- the slice, and the row's largest logit
     float top = -INFINITY;
     constexpr int V = 16 / sizeof(T);
     const bool wide = ((uintptr_t)in & 15) == 0;
     if (wide) {
+#pragma unroll 4
         for (int i = tid * V; i < n; i += SP_THREADS * V) {
             alignas(16) T e[V];
             if (i + V <= n) {
@@ -136,25 +161,30 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
             for (int j = 0; j < V; ++j) top = fmaxf(top, to_f32(e[j]));
         }
     } else {
+#pragma unroll 4
         for (int i = tid; i < n; i += SP_THREADS) {
-            if (CACHED) cache[i] = in[i];
-            top = fmaxf(top, to_f32(in[i]));
+            const T e = in[i];
+            if (CACHED) cache[i] = e;
+            top = fmaxf(top, to_f32(e));
         }
         if (CACHED)   // whole pieces of V are read
             for (int i = n + tid; i < (n + V - 1) / V * V; i += SP_THREADS) cache[i] = from_f32<T>(-INFINITY);
     }
-    for (int b = tid; b < SP_BINS; b += SP_THREADS) sh.counts[b] = 0;
-    for (int j = tid; j < SP_TABLE; j += SP_THREADS) sh.powers[j] = exp2(-(double)j / SP_TABLE);
+    if (tid < 256) sh.powers[tid] = (uint32_t)__double2ull_rn(exp2((double)tid / 256) * 2147483648.0);
+    // With top-k: of the threads' largest logits the nth, n chosen so that k of the row's tokens at least reach the smallest of those of all CTAs, and not many more.
+    const int nth = k > 0 && k <= 600 ? (k + C - 1) / C : 0;
+    const bool few = nth > 0 && nth <= SP_THREADS;
+    float reached = -INFINITY;
+    if (few) {
+        float v[1] = {top}, *buffer = (float *)sh.list;
+        sort_threads<1>(v, buffer);
+        __syncthreads();
+        buffer[tid] = v[0];
+        __syncthreads();
+        reached = buffer[nth - 1];
+        __syncthreads();   // the list may be written from here on
+    }
     if (tid == 0) sh.listed = 0;
-    const float temperature = a.temperature ? a.temperature[row] : 1.f;
-    const bool warm = temperature > 0.f;   // else the likeliest token
-    const double c = warm ? 1.4426950408889634 / (double)temperature : INFINITY;
-    const float top_p = a.top_p ? a.top_p[row] : 1.f;
-    float min_p = a.min_p ? a.min_p[row] : 0.f;
-    int k = a.top_k ? a.top_k[row] : 0;
-    if (!warm || min_p > 1.f) k = 1;
-    min_p = fminf(min_p, 1.f);   // NaN: 1, the likeliest and what is as likely
-    const bool by_p = top_p < 1.f;
 
     int phase = 0;
     auto block_sum = [&](u64 v) {   // of all threads, for all threads
@@ -200,138 +230,150 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
 #pragma unroll
     for (int w = 0; w < SP_WARPS; ++w) top = fmaxf(top, sh.scan[0][w]);
     if (C > 1) {
-        if (tid == 0) sh.top_bits = __float_as_int(top);
+        if (tid == 0) { sh.tops[0] = top; sh.tops[1] = reached; }
         cluster.sync();
-        for (int r = 0; r < C; ++r) top = fmaxf(top, __int_as_float(*cluster.map_shared_rank(&sh.top_bits, r)));
+        for (int r = 0; r < C; ++r) {
+            const float2 v = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(sh.tops, r));
+            top = fmaxf(top, v.x);
+            reached = fminf(reached, v.y);
+        }
     }
     if (!(top > -INFINITY)) {   // no token can be drawn
         if (rank == 0 && tid == 0) a.out[row] = -1;
         if (C > 1) cluster.sync();   // the others may still read this CTA's maximum
         return;
     }
-    const float cf = (float)c;
-    const double c_table = c * SP_TABLE, full = (double)(1ull << a.shift), top_d = (double)top;
-    const float far = (float)(a.shift + 2);
-    // 2^F 2^-x as a whole number: x in units of 1 / SP_TABLE is a whole number k and a rest of a half at most, 2^-x the table's entry times a cubic polynomial of the rest
-    // (2^-42 of it off).  Adding 2^52 to a double rounds it to a whole number, which its low bits then are.
+    // A token's weight.  z log2(e) / temperature = k / 256 + r + l: k a whole number, |r| a 512th at most, l what the product's rounding left.  The weight is, in units of
+    // 2^-F of a power of two just above the largest, 2^((k - k0) / 256) e^v with v = (r + l) ln 2: the power from a table, e^v - 1 = v + v^2 / 2 + v^3 / 6 as a whole
+    // number of 2^-31.  Some 2^-31 of the weight off, either way, one logit's apart from another's.  (In f64 it took four times as long: this GPU's f64 is slow.)
+    const float ch = (float)c, cl = (float)(c - (double)ch);
+    const double top_c = (double)top * c;
+    const bool quick = c > 1e-30 && c < 1e30 && top_c > -1000.0 && top_c < 1000.0;
+    const int k0 = quick ? (int)ceil(top_c * 256.0) : 0, up = a.shift + 1;   // F + 1
+    const float lowest = quick ? top - (float)((a.shift + 3) / c) : 0.f;   // weighs nothing
     auto weight = [&](float z) -> u64 {
-        if (z == top) return 1ull << a.shift;
-        if (!((top - z) * cf < far)) return 0ull;   // NaN and -inf too
-        const uint32_t b = __float_as_uint(z);      // as f64: exact but for 0 and subnormals, which come out below 2^-126
-        const double d = __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
-        const double t = (top_d - d) * c_table, whole = t + 6755399441055744.0;   // 1.5 2^52
-        const int k = __double2loint(whole);
-        const double r = t - (whole - 6755399441055744.0), u = r * -(0.6931471805599453 / SP_TABLE);
-        const double p = sh.powers[k & (SP_TABLE - 1)] * fma(u, fma(u, fma(u, 1.0 / 6, 0.5), 1.0), 1.0);
-        const double w = __hiloint2double(__double2hiint(p) + ((a.shift - (k >> 8)) << 20), __double2loint(p)) + 4503599627370496.0;   // 2^52
-        return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
+        if (!quick) return weight_of(z, top, c, a.shift);
+        z = fmaxf(z, lowest);   // NaN and -inf too
+        const float zc = z * ch, l = fmaf(z, cl, fmaf(z, ch, -zc));
+        const float m = fmaf(z, ch * 256.f, SP_MAGIC), r = fmaf(m - SP_MAGIC, -0.00390625f, zc);
+        const int q = __float_as_int(m) - 0x4b400000 - k0;
+        const float v = fmaf(l, 0.693147182f, r * 0.693147182f), e = fmaf(v * v, fmaf(v, 1.6666667e-1f, 0.5f), v) + 5.859375e-3f;   // 1.5 2^(23 - 31)
+        const int d = __float_as_int(e) - 0x3bc00000;
+        const uint32_t p = sh.powers[q & 255];
+        const uint32_t mantissa = p + (uint32_t)((long long)d * (int)(p >> 1) >> 30);   // 2^31 2^((q mod 256) / 256) e^v, up to 2^32: e^v is at most half a step of the table
+        const int n = up + (q >> 8);   // 2^(n - 32) times it, rounded
+        const u64 w = (u64)mantissa << (n & 31);
+        return n >= 32 ? w : n < 0 ? 0ull : (w + 0x80000000ull) >> 32;
     };
-    static_assert(SP_TABLE == 256, "k >> 8");
-    const float c_bin = cf * SP_PER;
-    auto bin_of = [&](float z) { return z == top ? 0 : (int)fminf((top - z) * c_bin, (float)(SP_BINS - 1)); };   // rises where z falls
-    const double wmin = (double)min_p * full;
+    const float c_bin = fminf(ch, 1e30f) * SP_PER;
+    const bool infinite = top == INFINITY;
+    auto bin_of = [&](float z) {   // rises where z falls
+        if (infinite) return z == top ? 0 : SP_BINS - 1;
+        return __float_as_int(fminf(fmaf(top - z, c_bin, SP_MAGIC), SP_MAGIC + (SP_BINS - 1))) - 0x4b400000;
+    };
+    const double full = (double)weight(top), wmin = (double)min_p * full;
     auto likely = [&](u64 w) { return !(min_p > 0.f) || (double)w >= wmin; };
-    // f(logit, index in the slice) of all tokens of the slice that can be drawn; those of a thread are V neighbours at a time
-    auto for_slice = [&](auto f) {
-        if (CACHED || wide) {
-            for (int i = tid * V; i < n; i += SP_THREADS * V) {
-                alignas(16) T e[V];
-                if (CACHED) *reinterpret_cast<uint4 *>(e) = *reinterpret_cast<const uint4 *>(cache + i);
-                else if (i + V <= n) *reinterpret_cast<uint4 *>(e) = *reinterpret_cast<const uint4 *>(in + i);
-                else
-                    for (int j = 0; j < V; ++j) e[j] = i + j < n ? in[i + j] : from_f32<T>(-INFINITY);
+    auto load = [&](int i, T (&e)[V]) {   // V tokens from i on, a multiple of V; -inf behind the slice
+        if (CACHED) {
+            *reinterpret_cast<uint4 *>(e) = *reinterpret_cast<const uint4 *>(cache + i);
+        } else if (wide && i + V <= n) {
+            *reinterpret_cast<uint4 *>(e) = *reinterpret_cast<const uint4 *>(in + i);
+        } else {
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float z = to_f32(e[j]);
-                    if (z > -INFINITY) f(z, i + j);
+            for (int j = 0; j < V; ++j) e[j] = i + j < n ? in[i + j] : from_f32<T>(-INFINITY);
+        }
+    };
+    // f(logit, index in the slice) of all tokens of the slice that can be drawn
+    auto for_slice = [&](auto f) {
+        for (int i = tid * V; i < n; i += SP_THREADS * V) {
+            alignas(16) T e[V];
+            load(i, e);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float z = to_f32(e[j]);
+                if (z > -INFINITY) f(z, i + j);
+            }
+        }
+    };
+    // found(index): of the token whose cumulative value(logit, index in the slice), in order of index, reaches target(the sum of all), called by one thread of the cluster.
+    // Every warp sums a run of the slice; the one that the target falls into looks again.
+    auto locate = [&](auto value, auto target_of, auto found) {
+        const int run = ((n + SP_WARPS - 1) / SP_WARPS + 32 * V - 1) / (32 * V) * (32 * V), i0 = warp * run, i1 = min(n, i0 + run);
+        u64 part = 0;
+        for (int i = i0 + lane * V; i < i1; i += 32 * V) {
+            alignas(16) T e[V];
+            load(i, e);
+#pragma unroll
+            for (int j = 0; j < V; ++j) part += value(to_f32(e[j]), i + j);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+        if (lane == 0) sh.part[warp] = part;
+        const u64 slice = block_sum(lane == 0 ? part : 0ull);
+        if (tid == 0) sh.slot[cphase] = slice;
+        cluster.sync();
+        u64 before = 0, mass = 0;
+        for (int r = 0; r < C; ++r) {
+            const u64 s = *cluster.map_shared_rank(&sh.slot[cphase], r);
+            if (r < rank) before += s;
+            mass += s;
+        }
+        cphase ^= 1;
+        const u64 target = target_of(mass);
+        if (before < target && target <= before + slice) {
+            for (int w = 0; w < warp; ++w) before += sh.part[w];
+            if (before < target && target <= before + part) {   // in this warp's run
+                for (int i = i0; i < i1; i += 32 * V) {
+                    alignas(16) T e[V];
+                    u64 here = 0;
+                    const int at = i + lane * V;
+                    if (at < i1) load(at, e);
+                    else
+                        for (int j = 0; j < V; ++j) e[j] = from_f32<T>(-INFINITY);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) here += value(to_f32(e[j]), at + j);
+                    u64 up = here;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const u64 v = __shfl_up_sync(0xffffffffu, up, o);
+                        if (lane >= o) up += v;
+                    }
+                    const unsigned there = __ballot_sync(0xffffffffu, before + up >= target);
+                    if (there) {
+                        if (lane == __ffs(there) - 1) {
+                            u64 sum = before + up - here;
+                            for (int j = 0; j < V; ++j) {
+                                sum += value(to_f32(e[j]), at + j);
+                                if (sum >= target) {
+                                    found(first + at + j);
+                                    break;
+                                }
+                            }
+                        }
+                        break;
+                    }
+                    before += __shfl_sync(0xffffffffu, up, 31);
                 }
             }
-        } else {
-            for (int i = tid; i < n; i += SP_THREADS) {
-                const float z = to_f32(in[i]);
-                if (z > -INFINITY) f(z, i);
-            }
         }
+        cluster.sync();   // the others may still read this CTA's sum
     };
-
-    // ---- counts by bins; all of the mass, where top-k does not cut it
-    u64 all = 0;
-    if (k <= 0 && by_p) for_slice([&](float z, int) { atomicAdd(&sh.counts[bin_of(z)], 1); all += weight(z); });
-    else for_slice([&](float z, int) { atomicAdd(&sh.counts[bin_of(z)], 1); });
-    all = cluster_sum(all);   // and the counts are whole
-    {
-        constexpr int B = SP_BINS / SP_THREADS;
-        int count[B] = {}, sum = 0;
-        float lo = 0.f, hi = 0.f, los[B], his[B];
-        for (int r = 0; r < C; ++r) {
-            const int4 v = *reinterpret_cast<const int4 *>(cluster.map_shared_rank(sh.counts, r) + tid * B);
-            count[0] += v.x; count[1] += v.y; count[2] += v.z; count[3] += v.w;
-        }
-        static_assert(B == 4, "bins of a thread");
-#pragma unroll
-        for (int j = 0; j < B; ++j) {   // in units of the likeliest token's
-            const float edge = exp2f(-(float)(tid * B + j) / SP_PER);
-            count[j] = sum += count[j];
-            const int here = count[j] - (j ? count[j - 1] : 0);
-            hi += (float)here * edge;
-            lo += tid * B + j == SP_BINS - 1 ? 0.f : (float)here * edge * 0.97857206f;   // 2^(-1 / SP_PER)
-            his[j] = hi;
-            los[j] = lo;
-        }
-        int s = sum;
-        float l = lo, h = hi;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int ps = __shfl_up_sync(0xffffffffu, s, o);
-            const float pl = __shfl_up_sync(0xffffffffu, l, o), ph = __shfl_up_sync(0xffffffffu, h, o);
-            if (lane >= o) { s += ps; l += pl; h += ph; }
-        }
-        if (lane == 31) { sh.scan[0][warp] = __int_as_float(s); sh.scan[1][warp] = l; sh.scan[2][warp] = h; }
-        if (tid < 4) sh.found[tid] = SP_BINS - 1;
-        __syncthreads();
-        s -= sum; l -= lo; h -= hi;
-        for (int w = 0; w < warp; ++w) { s += __float_as_int(sh.scan[0][w]); l += sh.scan[1][w]; h += sh.scan[2][w]; }
-#pragma unroll
-        for (int j = 0; j < B; ++j) { sh.cum[tid * B + j] = s + count[j]; sh.least[tid * B + j] = l + los[j]; sh.most[tid * B + j] = h + his[j]; }
-        __syncthreads();
-    }
-    const int valid = sh.cum[SP_BINS - 1];
-    const bool by_k = k > 0 && k < valid;
-    // the first bin whose cumulative value is `least` or more
-    auto first_bin = [&](auto cumulative, auto least, int which) {
-        for (int b = tid; b < SP_BINS; b += SP_THREADS)
-            if (cumulative[b] >= least && (b == 0 || !(cumulative[b - 1] >= least))) atomicMin(&sh.found[which], b);
-        __syncthreads();
-        return sh.found[which];
-    };
-    const int k_bin = by_k ? first_bin(sh.cum, k, 0) : SP_BINS - 1;
-    if (by_p && k > 0 && !by_k) {   // more than there are: its mass has not been summed
-        u64 s = 0;
-        for_slice([&](float z, int) { s += weight(z); });
-        all = cluster_sum(s);
-    }
     const double share = (double)fmaxf(top_p, 0.f);
-    int last = k_bin;   // the last bin that the list needs; top-p takes its share of all that top-k left, those that min-p drops among them
-    if (!by_k && by_p) last = first_bin(sh.least, (float)(share * ((double)all / full)) * 1.001f, 1);
-    if (min_p > 0.f && !(by_k && by_p)) last = min(last, (int)fminf(fmaxf(-log2f(min_p), 0.f) * SP_PER + 1.f, (float)(SP_BINS - 1)));
-    const bool filters = by_k || by_p || min_p > 0.f;
-
     auto draw_target = [&](u64 mass) {   // the token's cumulative mass reaches this
         const double u = a.uniforms_64 ? ((const double *)a.uniforms)[row] : (double)((const float *)a.uniforms)[row];
         return (u > 0.0 ? min((u64)fmin(u * (double)mass, 9.0e18), mass - 1) : 0ull) + 1;
     };
     auto whole = [&](double x) { return max((u64)ceil(fmin(x, 9.0e18)), 1ull); };   // a mass reaches x where it reaches this
 
-    // Tokens of bins [b0, b1] to the first CTA's list; false, and no list, where it does not hold them.
-    auto gather = [&](int b0, int b1) {
-        if (sh.cum[b1] - (b0 > 0 ? sh.cum[b0 - 1] : 0) > SP_LIST) return false;
+    // Tokens of which wanted(logit) to the first CTA's list, as many as it holds.
+    auto gather = [&](auto wanted) {
         SampleShared *there = cluster.map_shared_rank(&sh, 0);
         for_slice([&](float z, int i) {
-            const int b = bin_of(z);
-            if (b >= b0 && b <= b1) there->list[atomicAdd(&there->listed, 1)] = token_of(key_of(z), first + i);
+            if (!wanted(z)) return;
+            const int at = atomicAdd(&there->listed, 1);
+            if (at < SP_LIST) there->list[at] = token_of(key_of(z), first + i);
         });
         cluster.sync();
-        return true;
     };
     // A thread's tokens of the sorted list, neighbours, and their weights (0: of those behind `count`, or below `least`); the mass ahead of the first.
     u64 mine[SP_MINE], w[SP_MINE], ahead = 0;
@@ -352,16 +394,12 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
         ahead = block_before(sum);
         return sum;
     };
-
-    if (filters && sh.cum[last] <= SP_LIST) {
-        // ---- all that can stay is in the list
-        gather(0, last);
-        if (rank != 0) return;   // nobody reads this CTA's memory any more
-        const int listed = sh.listed;
-        sort_list(sh.list, listed);
-        const u64 sum = weigh(by_k ? min(k, listed) : listed, 1ull);
+    // The token, where all that can stay is in the list: by the first CTA.  most: of top-k; mass: of all tokens, where top-p takes its share of that.
+    auto from_list = [&](int most, bool cut_by_k, u64 mass) {
+        sort_list(sh.list, sh.listed);
+        const u64 sum = weigh(min(most, sh.listed), 1ull);
         if (by_p) {
-            const u64 target = whole(share * (double)(by_k ? block_sum(sum) : all));
+            const u64 target = whole(share * (double)(cut_by_k ? block_sum(sum) : mass));
             u64 at = ahead;
 #pragma unroll
             for (int j = 0; j < SP_MINE; ++j) {
@@ -406,155 +444,239 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
             if (at < target && target <= next) a.out[row] = index_of(token >> 32);
             at = next;
         }
-        return;
+    };
+
+    // ---- a logit that all which can stay reach: by top-k, or by min-p (whose share top-p does not take)
+    if (few || (min_p > 0.f && !by_p)) {
+        float from = reached;
+        if (min_p > 0.f && !by_p) from = fmaxf(from, infinite ? top : (float)((double)top - (-log2((double)min_p) * 1.001 + 0.01) / c));
+        gather([&](float z) { return z >= from; });
+        if (*cluster.map_shared_rank(&sh.listed, 0) <= SP_LIST) {
+            if (rank != 0) return;   // nobody reads this CTA's memory any more
+            from_list(k > 0 ? k : SP_LIST, k > 0, 0ull);
+            if (C > 1) cluster.sync();   // the others have read the list's length: those that have left count as arrived
+            return;
+        }
+        cluster.sync();
+        if (tid == 0) sh.listed = 0;   // of the first CTA; behind another barrier of all it is written again
     }
 
-    // ---- slices
     u64 cut = 0ull;   // the last token that stays
-    auto share_cut = [&]() {   // what the first CTA found, for all
-        if (rank == 0 && tid == 0) { sh.cut = cut; sh.listed = 0; }
-        cluster.sync();
-        cut = *cluster.map_shared_rank(&sh.cut, 0);
-        cluster.sync();
-    };
-    // Where no list holds a bin: of its tokens that stay so far, those of which the sum of value(logit) reaches `target`, by halving keys and then indices.
-    auto halve = [&](int bin, u64 target, auto value) {
-        auto total = [&](auto counts) {
-            u64 s = 0;
-            for_slice([&](float z, int i) {
-                const u64 token = token_of(key_of(z), first + i);
-                if (bin_of(z) == bin && token >= cut && counts(token)) s += value(z);
-            });
-            return cluster_sum(s);
-        };
-        u64 lo = max(cut, 1ull), hi = token_of(key_of(top), 0);   // the largest token at which the sum from it on reaches the target
-        if (total([&](u64 t) { return t >= lo; }) < target) return cut;
-        while (lo < hi) {
-            const u64 mid = lo + (hi - lo) / 2 + 1;
-            if (total([&](u64 t) { return t >= mid; }) >= target) lo = mid;
-            else hi = mid - 1;
-        }
-        return lo;
-    };
-    if (by_k) {
-        const int before = k_bin > 0 ? sh.cum[k_bin - 1] : 0;
-        if (gather(k_bin, k_bin)) {
-            if (rank == 0) {
-                sort_list(sh.list, sh.listed);
-                cut = sh.list[k - before - 1];
+    if (k > 0 || by_p || min_p > 0.f) {
+        // ---- counts by bins; all of the mass, where top-k does not cut it
+        for (int b = tid; b < SP_BINS; b += SP_THREADS) sh.counts[b] = 0;
+        __syncthreads();
+        u64 all = 0;
+        if (k <= 0 && by_p) for_slice([&](float z, int) { atomicAdd(&sh.counts[bin_of(z)], 1); all += weight(z); });
+        else for_slice([&](float z, int) { atomicAdd(&sh.counts[bin_of(z)], 1); });
+        all = cluster_sum(all);   // and the counts are whole
+        {
+            constexpr int B = SP_BINS / SP_THREADS;
+            int count[B] = {}, sum = 0;
+            float lo = 0.f, hi = 0.f, los[B], his[B];
+            for (int r = 0; r < C; ++r) {
+                const int4 *from = reinterpret_cast<const int4 *>(cluster.map_shared_rank(sh.counts, r) + tid * B), v = from[0], w = from[1];
+                count[0] += v.x; count[1] += v.y; count[2] += v.z; count[3] += v.w;
+                count[4] += w.x; count[5] += w.y; count[6] += w.z; count[7] += w.w;
             }
-            __syncthreads();   // before listed is cleared
-            share_cut();
-        } else {
-            cut = halve(k_bin, (u64)(k - before), [](float) { return 1ull; });
+            static_assert(B == 8, "bins of a thread");
+#pragma unroll
+            for (int j = 0; j < B; ++j) {   // in units of the likeliest token's; bin b is of x from (b - 1/2) / SP_PER to (b + 1/2) / SP_PER
+                const float edge = exp2f(-((float)(tid * B + j) - 0.5f) / SP_PER);
+                count[j] = sum += count[j];
+                const int here = count[j] - (j ? count[j - 1] : 0);
+                hi += (float)here * edge;
+                lo += tid * B + j == SP_BINS - 1 ? 0.f : (float)here * edge * 0.98922801f;   // 2^(-1 / SP_PER)
+                his[j] = hi;
+                los[j] = lo;
+            }
+            int s = sum;
+            float l = lo, h = hi;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int ps = __shfl_up_sync(0xffffffffu, s, o);
+                const float pl = __shfl_up_sync(0xffffffffu, l, o), ph = __shfl_up_sync(0xffffffffu, h, o);
+                if (lane >= o) { s += ps; l += pl; h += ph; }
+            }
+            if (lane == 31) { sh.scan[0][warp] = __int_as_float(s); sh.scan[1][warp] = l; sh.scan[2][warp] = h; }
+            if (tid < 4) sh.found[tid] = SP_BINS - 1;
+            __syncthreads();
+            s -= sum; l -= lo; h -= hi;
+            for (int w = 0; w < warp; ++w) { s += __float_as_int(sh.scan[0][w]); l += sh.scan[1][w]; h += sh.scan[2][w]; }
+#pragma unroll
+            for (int j = 0; j < B; ++j) { sh.cum[tid * B + j] = s + count[j]; sh.least[tid * B + j] = l + los[j]; sh.most[tid * B + j] = h + his[j]; }
+            __syncthreads();
         }
-        if (by_p) {
+        const bool by_k = k > 0 && k < sh.cum[SP_BINS - 1];
+        // the first bin whose cumulative value is `least` or more
+        auto first_bin = [&](auto cumulative, auto least, int which) {
+            for (int b = tid; b < SP_BINS; b += SP_THREADS)
+                if (cumulative[b] >= least && (b == 0 || !(cumulative[b - 1] >= least))) atomicMin(&sh.found[which], b);
+            __syncthreads();
+            return sh.found[which];
+        };
+        auto within = [&](int b0, int b1) { return sh.cum[b1] - (b0 > 0 ? sh.cum[b0 - 1] : 0) <= SP_LIST; };   // whether the list holds those bins
+        const int k_bin = by_k ? first_bin(sh.cum, k, 0) : SP_BINS - 1;
+        if (by_p && k > 0 && !by_k) {   // more than there are: its mass has not been summed
             u64 s = 0;
-            for_slice([&](float z, int i) { if (token_of(key_of(z), first + i) >= cut) s += weight(z); });
+            for_slice([&](float z, int) { s += weight(z); });
             all = cluster_sum(s);
         }
-    }
-    if (by_p) {
-        u64 target = whole(share * (double)all);
-        const float near = (float)((double)target / full);
-        int b0 = first_bin(sh.most, near * 0.999f, 2), b1 = min(max(first_bin(sh.least, near * 1.001f, 3), b0), k_bin);
-        b0 = min(b0, b1);
-        __syncthreads();   // the bounds have been read; the masses of bins b0 .. b1, exactly, take their place
-        for (int b = b0 + tid; b <= b1; b += SP_THREADS) sh.low[b] = sh.high[b] = 0u;
-        __syncthreads();
-        u64 s = 0;
-        for_slice([&](float z, int i) {
-            const int b = bin_of(z);
-            if (b > b1 || token_of(key_of(z), first + i) < cut) return;
-            const u64 w = weight(z);
-            if (b < b0) {
-                s += w;
-            } else {
-                const uint32_t w0 = (uint32_t)w, carry = atomicAdd(&sh.low[b], w0) > ~w0 ? 1u : 0u, w1 = (uint32_t)(w >> 32) + carry;
-                if (w1) atomicAdd(&sh.high[b], w1);
+        int last = k_bin;   // the last bin that the list needs; top-p takes its share of all that top-k left, those that min-p drops among them
+        if (!by_k && by_p) last = first_bin(sh.least, (float)(share * ((double)all / full)) * 1.001f, 1);
+        if (min_p > 0.f && !(by_k && by_p)) last = min(last, (int)fminf(fmaxf(-log2f(min_p), 0.f) * SP_PER + 2.f, (float)(SP_BINS - 1)));
+        if ((by_k || by_p || min_p > 0.f) && within(0, last)) {
+            gather([&](float z) { return bin_of(z) <= last; });
+            if (rank == 0) from_list(by_k ? k : SP_LIST, by_k, all);
+            return;
+        }
+
+        // ---- slices
+        auto share_cut = [&]() {   // what the first CTA found, for all
+            if (rank == 0 && tid == 0) { sh.cut = cut; sh.listed = 0; }
+            cluster.sync();
+            cut = *cluster.map_shared_rank(&sh.cut, 0);
+            cluster.sync();
+        };
+        // Where no list holds a bin: of its tokens that stay so far, the last one of the shortest prefix of which the sum of value(logit) reaches `target`, by halving keys;
+        // of equal ones, by their count.
+        auto halve = [&](int bin, u64 target, auto value) {
+            if (tid == 0) { sh.key_range[0] = 0xffffffffu; sh.key_range[1] = 0u; }
+            __syncthreads();
+            uint32_t lo = 0xffffffffu, hi = 0u;
+            for_slice([&](float z, int i) {
+                if (bin_of(z) != bin || token_of(key_of(z), first + i) < cut) return;
+                lo = min(lo, key_of(z));
+                hi = max(hi, key_of(z));
+            });
+            lo = __reduce_min_sync(0xffffffffu, lo);
+            hi = __reduce_max_sync(0xffffffffu, hi);
+            if (lane == 0) { atomicMin(&sh.key_range[0], lo); atomicMax(&sh.key_range[1], hi); }
+            __syncthreads();
+            cluster.sync();
+            for (int r = 0; r < C; ++r) {
+                lo = min(lo, *cluster.map_shared_rank(&sh.key_range[0], r));
+                hi = max(hi, *cluster.map_shared_rank(&sh.key_range[1], r));
             }
-        });
-        s = cluster_sum(s);
-        for (int b = b0 + tid; b <= b1; b += SP_THREADS) {
-            u64 here = 0;
-            for (int r = 0; r < C; ++r) here += ((u64)*cluster.map_shared_rank(&sh.high[b], r) << 32) + *cluster.map_shared_rank(&sh.low[b], r);
-            sh.weights[b - b0] = here;
-        }
-        __syncthreads();
-        int bin = b1;   // of the border
-        for (int b = b0; b < b1; ++b) {
-            const u64 here = sh.weights[b - b0];
-            if (s + here >= target) { bin = b; break; }
-            s += here;
-        }
-        target = target > s ? target - s : 1ull;
-        if (gather(bin, bin)) {
-            if (rank == 0) {
-                sort_list(sh.list, sh.listed);
-                weigh(sh.listed, max(cut, 1ull));
-                // the last token whose mass ahead is below the target
-                if (tid == 0) sh.cut = ~0ull;
-                __syncthreads();
-                u64 at = ahead, lowest = ~0ull;
-#pragma unroll
-                for (int j = 0; j < SP_MINE; ++j) {
-                    if (mine[j] >= max(cut, 1ull) && at < target) lowest = mine[j];
-                    at += w[j];
+            auto total = [&](uint32_t from, bool one) {   // of keys from `from` on, or of that one
+                u64 s = 0;
+                for_slice([&](float z, int i) {
+                    const uint32_t key = key_of(z);
+                    if (bin_of(z) == bin && (one ? key == from : key >= from) && token_of(key, first + i) >= cut) s += value(z);
+                });
+                return cluster_sum(s);
+            };
+            while (lo < hi) {   // the largest key at which the sum from it on reaches the target
+                const uint32_t mid = lo + (hi - lo) / 2 + 1;
+                if (total(mid, false) >= target) lo = mid;
+                else hi = mid - 1;
+            }
+            const uint32_t key = lo;
+            const u64 ties = total(key, true), each = value(logit_of(key)), before = total(key, false) - ties;
+            if (each == 0 || before + ties <= target) return max(cut, token_of(key, 0x7fffffff));   // all of them
+            const u64 need = target > before ? (target - before + each - 1) / each : 1ull;
+            locate([&](float z, int i) -> u64 { return key_of(z) == key && token_of(key, first + i) >= cut; }, [&](u64) { return need; },
+                   [&](int i) { *cluster.map_shared_rank(&sh.index, 0) = i; });
+            const int index = *cluster.map_shared_rank(&sh.index, 0);   // behind locate's barrier
+            cluster.sync();
+            return token_of(key, index);
+        };
+        if (by_k) {
+            const int before = k_bin > 0 ? sh.cum[k_bin - 1] : 0;
+            if (within(k_bin, k_bin)) {
+                gather([&](float z) { return bin_of(z) == k_bin; });
+                if (rank == 0) {
+                    sort_list(sh.list, sh.listed);
+                    cut = sh.list[k - before - 1];
                 }
-                if (lowest != ~0ull) atomicMin(&sh.cut, lowest);
-                __syncthreads();
-                cut = sh.cut;
+                __syncthreads();   // before listed is cleared
+                share_cut();
+            } else {
+                cut = halve(k_bin, (u64)(k - before), [](float) { return 1ull; });
+            }
+            if (by_p) {
+                u64 s = 0;
+                for_slice([&](float z, int i) { if (token_of(key_of(z), first + i) >= cut) s += weight(z); });
+                all = cluster_sum(s);
+            }
+        }
+        if (by_p) {
+            u64 target = whole(share * (double)all);
+            const float near = (float)((double)target / full);
+            const int b1 = min(first_bin(sh.least, near * 1.001f, 3), k_bin), b0 = min(first_bin(sh.most, near * 0.999f, 2), b1);
+            __syncthreads();   // the bounds have been read; the masses of bins b0 .. b1, exactly, take their place
+            for (int b = b0 + tid; b <= b1; b += SP_THREADS) sh.low[b] = sh.high[b] = 0u;
+            __syncthreads();
+            u64 s = 0;
+            for_slice([&](float z, int i) {
+                const int b = bin_of(z);
+                if (b > b1 || token_of(key_of(z), first + i) < cut) return;
+                const u64 w = weight(z);
+                if (b < b0) {
+                    s += w;
+                } else {
+                    const uint32_t w0 = (uint32_t)w, carry = atomicAdd(&sh.low[b], w0) > ~w0 ? 1u : 0u, w1 = (uint32_t)(w >> 32) + carry;
+                    if (w1) atomicAdd(&sh.high[b], w1);
+                }
+            });
+            s = cluster_sum(s);
+            u64 masses[SP_BINS / SP_THREADS];
+#pragma unroll
+            for (int i = 0; i < SP_BINS / SP_THREADS; ++i) {
+                const int b = b0 + tid + i * SP_THREADS;
+                masses[i] = 0ull;
+                if (b <= b1)
+                    for (int r = 0; r < C; ++r) masses[i] += ((u64)*cluster.map_shared_rank(&sh.high[b], r) << 32) + *cluster.map_shared_rank(&sh.low[b], r);
+            }
+            cluster.sync();   // all have read the slices' masses: the row's take their place
+#pragma unroll
+            for (int i = 0; i < SP_BINS / SP_THREADS; ++i) {
+                const int b = b0 + tid + i * SP_THREADS;
+                if (b <= b1) { sh.low[b] = (uint32_t)masses[i]; sh.high[b] = (uint32_t)(masses[i] >> 32); }
             }
             __syncthreads();
-            share_cut();
-        } else {
-            cut = halve(bin, target, weight);
+            int bin = b1;   // of the border
+            for (int b = b0; b < b1; ++b) {
+                const u64 here = (u64)sh.high[b] << 32 | sh.low[b];
+                if (s + here >= target) { bin = b; break; }
+                s += here;
+            }
+            target = target > s ? target - s : 1ull;
+            if (within(bin, bin)) {
+                gather([&](float z) { return bin_of(z) == bin; });
+                if (rank == 0) {
+                    sort_list(sh.list, sh.listed);
+                    weigh(sh.listed, max(cut, 1ull));
+                    // the last token whose mass ahead is below the target
+                    if (tid == 0) sh.cut = ~0ull;
+                    __syncthreads();
+                    u64 at = ahead, lowest = ~0ull;
+#pragma unroll
+                    for (int j = 0; j < SP_MINE; ++j) {
+                        if (mine[j] >= max(cut, 1ull) && at < target) lowest = mine[j];
+                        at += w[j];
+                    }
+                    if (lowest != ~0ull) atomicMin(&sh.cut, lowest);
+                    __syncthreads();
+                    cut = sh.cut;
+                }
+                __syncthreads();
+                share_cut();
+            } else {
+                cut = halve(bin, target, weight);
+            }
         }
     }
-    // every warp's run of the slice, the CTAs', and the token
-    auto logit = [&](int i) { return to_f32(CACHED ? cache[i] : in[i]); };
-    const int run = ((n + SP_WARPS - 1) / SP_WARPS + 31) / 32 * 32, i0 = warp * run, i1 = min(n, i0 + run);
-    auto kept = [&](int i) -> u64 {
-        const float z = logit(i);
+
+    // ---- what stays of every warp's run of the slice, of the CTAs', and the token
+    const bool everything = cut == 0ull && !(min_p > 0.f);
+    auto kept = [&](float z, int i) -> u64 {
+        if (everything) return weight(z);   // nothing for those that cannot be drawn
         if (!(z > -INFINITY) || token_of(key_of(z), first + i) < cut) return 0ull;
         const u64 w = weight(z);
         return likely(w) ? w : 0ull;
     };
-    u64 part = 0;
-    for (int i = i0 + lane; i < i1; i += 32) part += kept(i);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-    if (lane == 0) sh.part[warp] = part;
-    const u64 slice = block_sum(lane == 0 ? part : 0ull);
-    if (tid == 0) sh.slot[cphase] = slice;
-    cluster.sync();
-    u64 before = 0, mass = 0;
-    for (int r = 0; r < C; ++r) {
-        const u64 s = *cluster.map_shared_rank(&sh.slot[cphase], r);
-        if (r < rank) before += s;
-        mass += s;
-    }
-    const u64 target = draw_target(mass);
-    if (before < target && target <= before + slice) {
-        for (int w = 0; w < warp; ++w) before += sh.part[w];
-        if (before < target && target <= before + part) {   // in this warp's run
-            for (int i = i0; i < i1; i += 32) {
-                u64 up = i + lane < i1 ? kept(i + lane) : 0ull;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const u64 v = __shfl_up_sync(0xffffffffu, up, o);
-                    if (lane >= o) up += v;
-                }
-                const unsigned there = __ballot_sync(0xffffffffu, before + up >= target);
-                if (there) {
-                    if (lane == 0) a.out[row] = first + i + __ffs(there) - 1;
-                    break;
-                }
-                before += __shfl_sync(0xffffffffu, up, 31);
-            }
-        }
-    }
-    cluster.sync();   // the others may still read this CTA's sum
+    locate(kept, draw_target, [&](int i) { a.out[row] = i; });
 }
 
 template <typename T, bool CACHED>

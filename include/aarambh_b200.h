@@ -433,7 +433,8 @@ int ab2_adjust_logits(const void *logits_dev, long long stride, int rows, int vo
  * more (1: all; the first token always stays), of these the ones with p >= min_p times the largest p (0: all).  The answer is the first that stayed, in order of index,
  * whose cumulative mass exceeds u times the mass of all that stayed, u the row's number of uniforms_dev (f32, or with uniforms_64 f64; 0 <= u < 1).  A temperature
  * that is not positive gives the likeliest token.  NaN and -inf are never drawn; a row without another logit answers -1.  temperature_dev, top_k_dev, top_p_dev and
- * min_p_dev are [rows], or NULL for 1, 0, 1 and 0.  The mass is summed exactly (whole numbers of 2^-44 of the largest p): equal inputs give equal tokens.  Up to 2^24 tokens. */
+ * min_p_dev are [rows], or NULL for 1, 0, 1 and 0.  Each p is off by
+ * 2^-30 of itself and 2^-45 of the largest at most and they are summed exactly, as whole numbers: equal inputs give equal tokens.  Up to 2^24 tokens. */
 int ab2_sample(const void *logits_dev, long long stride, int rows, int vocab, const void *uniforms_dev, int uniforms_64, const float *temperature_dev,
                const int *top_k_dev, const float *top_p_dev, const float *min_p_dev, int *out_dev, ab2_dtype dtype, ab2_stream stream);
 

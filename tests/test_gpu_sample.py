@@ -12,8 +12,9 @@ BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
 def allowed(z, u, T=1.0, k=0, p=1.0, least=0.0):
-    """The tokens that may be the answer for one row: one, but where u or p falls on a border between two by less than what weights are off: whole numbers of 2^-44 of the
-    largest (half of one for each token, 2^-52 of it by f64's exponential), and f64 sums."""
+    """The tokens that may be the answer for one row: one, but where u or p falls on a border between two by less than what weights are off.  A weight is a table's power of two
+    (rounded to 31 bits: 2^-32) times e^v as a whole number of 2^-31 (2^-32, and its float 2^-33), their product cut to 31 bits (2^-31): 2^-30.4 of it together, less than 2^-30; then
+    it is rounded to a whole number of 2^-44 of the largest, half of one for each token.  f64 sums of up to 2^20 terms: 2^-33."""
     z = z.double().cpu().numpy()
     valid = np.nonzero(z > -np.inf)[0]
     if len(valid) == 0:
@@ -27,7 +28,7 @@ def allowed(z, u, T=1.0, k=0, p=1.0, least=0.0):
         k = 1
     if 0 < k < len(order):
         order = order[:k]
-    off = len(z) * 2.0 ** -44
+    off = len(z) * 2.0 ** -44 + w.sum() * 2.0 ** -30
     answers = set()
     ws = w[order]
     up = np.cumsum(ws)
