@@ -251,8 +251,7 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
     const bool quick = c > 1e-30 && c < 1e30 && top_c > -1000.0 && top_c < 1000.0;
     const int k0 = quick ? (int)ceil(top_c * 256.0) : 0, up = a.shift + 1;   // F + 1
     const float lowest = quick ? top - (float)((a.shift + 3) / c) : 0.f;   // weighs nothing
-    auto weight = [&](float z) -> u64 {
-        if (!quick) return weight_of(z, top, c, a.shift);
+    auto quick_weight = [&](float z) -> u64 {
         z = fmaxf(z, lowest);   // NaN and -inf too
         const float zc = z * ch, l = fmaf(z, cl, fmaf(z, ch, -zc));
         const float m = fmaf(z, ch * 256.f, SP_MAGIC), r = fmaf(m - SP_MAGIC, -0.00390625f, zc);
@@ -264,6 +263,13 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
         const int n = up + (q >> 8);   // 2^(n - 32) times it, rounded
         const u64 w = (u64)mantissa << (n & 31);
         return n >= 32 ? w : n < 0 ? 0ull : (w + 0x80000000ull) >> 32;
+    };
+    auto slow_weight = [&](float z) { return weight_of(z, top, c, a.shift); };
+    auto weight = [&](float z) { return quick ? quick_weight(z) : slow_weight(z); };
+    // f(weight) for a pass: decided once, so that the products of a thread's tokens run side by side
+    auto by_weight = [&](auto f) {
+        if (quick) f(quick_weight);
+        else f(slow_weight);
     };
     const float c_bin = fminf(ch, 1e30f) * SP_PER;
     const bool infinite = top == INFINITY;
@@ -293,6 +299,15 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
                 const float z = to_f32(e[j]);
                 if (z > -INFINITY) f(z, i + j);
             }
+        }
+    };
+    // f of all of them, whether they can be drawn or not
+    auto for_all = [&](auto f) {
+        for (int i = tid * V; i < n; i += SP_THREADS * V) {
+            alignas(16) T e[V];
+            load(i, e);
+#pragma unroll
+            for (int j = 0; j < V; ++j) f(to_f32(e[j]), i + j);
         }
     };
     // found(index): of the token whose cumulative value(logit, index in the slice), in order of index, reaches target(the sum of all), called by one thread of the cluster.
@@ -467,7 +482,13 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
         for (int b = tid; b < SP_BINS; b += SP_THREADS) sh.counts[b] = 0;
         __syncthreads();
         u64 all = 0;
-        if (k <= 0 && by_p) for_slice([&](float z, int) { atomicAdd(&sh.counts[bin_of(z)], 1); all += weight(z); });
+        if (k <= 0 && by_p)
+            by_weight([&](auto weight) {
+                for_all([&](float z, int) {
+                    if (z > -INFINITY) atomicAdd(&sh.counts[bin_of(z)], 1);
+                    all += weight(z);
+                });
+            });
         else for_slice([&](float z, int) { atomicAdd(&sh.counts[bin_of(z)], 1); });
         all = cluster_sum(all);   // and the counts are whole
         {
@@ -608,16 +629,16 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
             for (int b = b0 + tid; b <= b1; b += SP_THREADS) sh.low[b] = sh.high[b] = 0u;
             __syncthreads();
             u64 s = 0;
-            for_slice([&](float z, int i) {
-                const int b = bin_of(z);
-                if (b > b1 || token_of(key_of(z), first + i) < cut) return;
-                const u64 w = weight(z);
-                if (b < b0) {
-                    s += w;
-                } else {
-                    const uint32_t w0 = (uint32_t)w, carry = atomicAdd(&sh.low[b], w0) > ~w0 ? 1u : 0u, w1 = (uint32_t)(w >> 32) + carry;
-                    if (w1) atomicAdd(&sh.high[b], w1);
-                }
+            by_weight([&](auto weight) {
+                for_all([&](float z, int i) {
+                    const int b = z > -INFINITY ? bin_of(z) : SP_BINS;
+                    const u64 w = weight(z);
+                    if (b < b0) s += w;   // ahead of the bins of the border: top-k left them
+                    if (b >= b0 && b <= b1 && token_of(key_of(z), first + i) >= cut) {
+                        const uint32_t w0 = (uint32_t)w, carry = atomicAdd(&sh.low[b], w0) > ~w0 ? 1u : 0u, w1 = (uint32_t)(w >> 32) + carry;
+                        if (w1) atomicAdd(&sh.high[b], w1);
+                    }
+                });
             });
             s = cluster_sum(s);
             u64 masses[SP_BINS / SP_THREADS];
@@ -669,14 +690,17 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
     }
 
     // ---- what stays of every warp's run of the slice, of the CTAs', and the token
-    const bool everything = cut == 0ull && !(min_p > 0.f);
-    auto kept = [&](float z, int i) -> u64 {
-        if (everything) return weight(z);   // nothing for those that cannot be drawn
-        if (!(z > -INFINITY) || token_of(key_of(z), first + i) < cut) return 0ull;
-        const u64 w = weight(z);
-        return likely(w) ? w : 0ull;
-    };
-    locate(kept, draw_target, [&](int i) { a.out[row] = i; });
+    const auto found = [&](int i) { a.out[row] = i; };
+    if (cut == 0ull && !(min_p > 0.f)) {   // all: nothing weighs what cannot be drawn
+        by_weight([&](auto weight) { locate([&](float z, int) { return weight(z); }, draw_target, found); });
+    } else {
+        by_weight([&](auto weight) {
+            locate([&](float z, int i) {
+                const u64 w = weight(z);
+                return token_of(key_of(z), first + i) >= cut && likely(w) ? w : 0ull;
+            }, draw_target, found);
+        });
+    }
 }
 
 template <typename T, bool CACHED>
