@@ -117,10 +117,28 @@ bool paged_of(Args &a, int kp, int tab, int len, int st, int64_t tokens, ab2_pag
     return true;
 }
 
-// append(k_pages, v_pages, k, v, table, lens, starts, q, frequencies, layout, magnitude)
+// The scales of pages of 8 bits, a pair (or None: neither); false where they and the pages do not belong together.
+bool scales_of(Args &a, PyObject *pair, const at::Tensor &pages, const float *&ks, const float *&vs) {
+    ks = vs = nullptr;
+    const bool codes = pages.scalar_type() == at::kFloat8_e4m3fn;
+    if (pair == Py_None) return !codes;
+    if (!codes || !PyTuple_CheckExact(pair) || PyTuple_GET_SIZE(pair) != 2) return false;
+    PyObject *both[2] = {PyTuple_GET_ITEM(pair, 0), PyTuple_GET_ITEM(pair, 1)};
+    Args s{both, a.device};
+    const at::Tensor *k = s(0), *v = s(1);
+    if (!s.plain) return false;
+    for (const at::Tensor *t : {k, v})
+        if (!is(t, at::kFloat, {pages.size(0), pages.size(1), pages.size(2) / 16})) return false;
+    ks = (const float *)ptr(k);
+    vs = (const float *)ptr(v);
+    return true;
+}
+
+// append(k_pages, v_pages, k, v, table, lens, starts, q, frequencies, layout, magnitude[, scales])
 PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
-        if (n != 11) return none();
+        if (n != 11 && n != 12) return none();
+        PyObject *scales = n > 11 ? args[11] : Py_None;
         Args a{args};
         const at::Tensor *k = a(2), *v = a(3), *q = a(7, true), *f = a(8, true), *pages;
         const int layout = layout_of(args[9]);
@@ -128,11 +146,19 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t n) {
         if (!a.plain || layout < 0 || !number(args[10], magnitude) || k->dim() != 3 || v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type()) return none();
         const int64_t tokens = k->size(0), kv = k->size(1), dim = k->size(2), heads = q && q->dim() == 3 ? q->size(1) : 0;
         ab2_paged c;
-        if (!paged_of(a, 0, 4, 5, 6, tokens, c, pages) || pages->scalar_type() != k->scalar_type() || kv != c.kv_heads || dim != c.head_dim || dtype_of(*k) < 0 || !fits(heads)) return none();
+        if (!paged_of(a, 0, 4, 5, 6, tokens, c, pages) || (scales == Py_None && pages->scalar_type() != k->scalar_type()) || kv != c.kv_heads || dim != c.head_dim || dtype_of(*k) < 0 || !fits(heads)) return none();
         if (q && (q->dim() != 3 || q->scalar_type() != k->scalar_type() || q->size(0) != tokens || q->size(2) != dim)) return none();
         if (f && (f->dim() != 1 || f->scalar_type() != at::kDouble || 2 * f->size(0) > dim)) return none();
+        const float *ks, *vs;
+        if (!a.plain || !scales_of(a, scales, *pages, ks, vs)) return none();
         at::Tensor out;
         if (q) out = at::empty_like(*q);
+        if (ks) {
+            const int rc = ab2_paged_append_e4m3(&c, (float *)ks, (float *)vs, ptr(k), kv * dim, ptr(v), kv * dim, ptr(q), heads * dim, (int)heads, q ? out.data_ptr() : nullptr, heads * dim,
+                                                 (const double *)ptr(f), f ? (int)(2 * f->size(0)) : 0, layout, (float)magnitude, (ab2_dtype)dtype_of(*k), c10::cuda::getCurrentCUDAStream().stream());
+            if (rc != AB2_OK) return PyLong_FromLong(rc);
+            return q ? THPVariable_Wrap(out) : Py_NewRef(Py_True);
+        }
         const int rc = ab2_paged_append(&c, ptr(k), kv * dim, ptr(v), kv * dim, ptr(q), heads * dim, (int)heads, q ? out.data_ptr() : nullptr, heads * dim, (const double *)ptr(f),
                                         f ? (int)(2 * f->size(0)) : 0, layout, (float)magnitude, (ab2_dtype)dtype_of(*k), c10::cuda::getCurrentCUDAStream().stream());
         if (rc != AB2_OK) return PyLong_FromLong(rc);
@@ -140,25 +166,35 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
-// attention(q, k_pages, v_pages, table, lens, scale, starts, max_new)
+// attention(q, k_pages, v_pages, table, lens, scale, starts, max_new[, scales, window, sinks])
 PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
-        if (n != 8) return none();
+        if (n != 8 && n != 11) return none();
+        PyObject *scales = n > 8 ? args[8] : Py_None;
         Args a{args};
         const at::Tensor *q = a(0), *pages;
-        double scale, most = -1;
-        if (!a.plain || q->dim() != 3 || !number(args[5], scale) || (args[7] != Py_None && (!PyLong_CheckExact(args[7]) || !number(args[7], most) || most > 0x7fffffff))) return none();
+        double scale, most = -1, window = 0, sinks = 0;
+        if (!a.plain || q->dim() != 3 || !number(args[5], scale) || (args[7] != Py_None && (!PyLong_CheckExact(args[7]) || !number(args[7], most) || most > 0x7fffffff)) ||
+            (n > 8 && (!PyLong_CheckExact(args[9]) || !number(args[9], window) || !PyLong_CheckExact(args[10]) || !number(args[10], sinks))) || window < 0 || window > 0x7fffffff || sinks < 0 || sinks > 0x7fffffff)
+            return none();
         const int64_t tokens = q->size(0), heads = q->size(1), dim = q->size(2);
         ab2_paged c;
-        if (!paged_of(a, 1, 3, 4, 6, tokens, c, pages) || pages->scalar_type() != q->scalar_type() || dim != c.head_dim || dtype_of(*q) < 0 || !fits(heads)) return none();
+        if (!paged_of(a, 1, 3, 4, 6, tokens, c, pages) || (scales == Py_None && pages->scalar_type() != q->scalar_type()) || dim != c.head_dim || dtype_of(*q) < 0 || !fits(heads)) return none();
+        const float *ks, *vs;
+        if (!a.plain || !scales_of(a, scales, *pages, ks, vs)) return none();
         if (((uintptr_t)q->data_ptr() | (uintptr_t)(heads * dim * q->element_size())) & 15) return none();
         if (args[7] == Py_None) most = c.starts ? (double)std::max<int64_t>(tokens, 1) : 1;
         size_t bytes = 0;
         if (c.table_width * (int64_t)c.page_size > AB2_PAGED_UNCUT && ab2_paged_workspace(c.head_dim, &bytes) != AB2_OK) return none();
         at::Tensor out = at::empty_like(*q), work;
         if (bytes > 0) work = at::empty({(int64_t)bytes}, q->options().dtype(at::kByte));
-        const int rc = ab2_paged_attention(&c, q->data_ptr(), heads * dim, (int)heads, out.data_ptr(), heads * dim, (int)most, (float)scale, bytes > 0 ? work.data_ptr() : nullptr, bytes,
-                                           (ab2_dtype)dtype_of(*q), c10::cuda::getCurrentCUDAStream().stream());
+        void *room = bytes > 0 ? work.data_ptr() : nullptr;
+        ab2_stream stream = c10::cuda::getCurrentCUDAStream().stream();
+        const ab2_dtype type = (ab2_dtype)dtype_of(*q);
+        const long long row = heads * dim;
+        const int rc = ks       ? ab2_paged_attention_e4m3(&c, ks, vs, (int)window, (int)sinks, q->data_ptr(), row, (int)heads, out.data_ptr(), row, (int)most, (float)scale, room, bytes, type, stream)
+                       : window || sinks ? ab2_paged_attention_window(&c, (int)window, (int)sinks, q->data_ptr(), row, (int)heads, out.data_ptr(), row, (int)most, (float)scale, room, bytes, type, stream)
+                                : ab2_paged_attention(&c, q->data_ptr(), row, (int)heads, out.data_ptr(), row, (int)most, (float)scale, room, bytes, type, stream);
         return rc == AB2_OK ? THPVariable_Wrap(out) : PyLong_FromLong(rc);
     });
 }
@@ -193,10 +229,31 @@ PyObject *logits(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// sample(logits, uniforms, temperature, top_k, top_p, min_p)
+PyObject *sample(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        if (n != 6) return none();
+        Args a{args};
+        const at::Tensor *z = a(0), *u = a(1), *temperature = a(2, true), *top_k = a(3, true), *top_p = a(4, true), *min_p = a(5, true);
+        if (!a.plain || z->dim() != 2 || dtype_of(*z) < 0) return none();
+        const int64_t rows = z->size(0), vocab = z->size(1);
+        const bool wide = u->scalar_type() == at::kDouble;
+        if (!fits(rows) || !fits(vocab) || !is(u, wide ? at::kDouble : at::kFloat, {rows})) return none();
+        for (const at::Tensor *t : {temperature, top_p, min_p})
+            if (t && !is(t, at::kFloat, {rows})) return none();
+        if (top_k && !is(top_k, at::kInt, {rows})) return none();
+        at::Tensor out = at::empty({rows}, z->options().dtype(at::kInt));
+        const int rc = ab2_sample(z->data_ptr(), vocab, (int)rows, (int)vocab, u->data_ptr(), wide, (const float *)ptr(temperature), (const int *)ptr(top_k), (const float *)ptr(top_p),
+                                  (const float *)ptr(min_p), out.data_ptr<int>(), (ab2_dtype)dtype_of(*z), c10::cuda::getCurrentCUDAStream().stream());
+        return rc == AB2_OK ? THPVariable_Wrap(out) : PyLong_FromLong(rc);
+    });
+}
+
 PyMethodDef methods[] = {{"rotary", (PyCFunction)(void (*)(void))rotary, METH_FASTCALL, nullptr},
                          {"append", (PyCFunction)(void (*)(void))append, METH_FASTCALL, nullptr},
                          {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL, nullptr},
                          {"logits", (PyCFunction)(void (*)(void))logits, METH_FASTCALL, nullptr},
+                         {"sample", (PyCFunction)(void (*)(void))sample, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

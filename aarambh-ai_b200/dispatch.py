@@ -424,8 +424,8 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, 
 
     Pages of 8 bits (float8_e4m3fn) have ``scales``, those of keys and those of values, each [pages, kv_heads, page_size / 16] f32: a value is its code times the
     scale of its 16 tokens, a power of two that grows with the tokens that come (earlier ones' codes are made anew then)."""
-    if out is None and scales is None and _fast is not None:
-        got = _fast.append(k_pages, v_pages, k, v, table, lens, starts, q, frequencies, layout, magnitude)
+    if out is None and _fast is not None:
+        got = _fast.append(k_pages, v_pages, k, v, table, lens, starts, q, frequencies, layout, magnitude, scales)
         if got is not None:
             return check(got) if type(got) is int else got if got is not True else None
     k_scales, v_scales = _scales(scales, k_pages, v_pages)
@@ -471,8 +471,8 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     ``scales``: of pages of 8 bits, as in ``paged_append``; a weight keeps 11 bits there, or 8.  With a ``window`` a token sees its row's last so many keys, its own
     among them, and the first ``sinks`` of the row; pages that hold no key in sight of a row's new tokens are not looked at."""
-    if out is None and scales is None and not window and not sinks and _fast is not None:
-        got = _fast.attention(q, k_pages, v_pages, table, lens, scale, starts, max_new)
+    if out is None and _fast is not None:
+        got = _fast.attention(q, k_pages, v_pages, table, lens, scale, starts, max_new, scales, window, sinks)
         if got is not None:
             return check(got) if type(got) is int else got
     k_scales, v_scales = _scales(scales, k_pages, v_pages)
@@ -585,6 +585,10 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: torch.Tens
     ``top_p`` of their mass (1: all), of these the ones with ``min_p`` of the likeliest one's probability or more (0: all).  The token is the first that stayed, in
     order of index, whose cumulative mass exceeds u times all of theirs.  All four are [rows], f32 (top_k int32), or None.  A temperature that is not positive gives
     the likeliest token; NaN and -inf are never drawn, and a row with nothing else answers -1."""
+    if out is None and _fast is not None:
+        got = _fast.sample(logits, uniforms, temperature, top_k, top_p, min_p)
+        if got is not None:
+            return check(got) if type(got) is int else got
     _on_device(logits, uniforms, temperature, top_k, top_p, min_p, out)
     if logits.dim() != 2:
         raise _lib.Ab2Error(-1, f"logits must be [rows, vocab], got {list(logits.shape)}")
