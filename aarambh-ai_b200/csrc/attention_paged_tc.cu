@@ -87,13 +87,18 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) { return pair(ex2(low(x)), ex2(high(x))); }
 // What all roles know of a piece.
 struct PcPiece {
     PagedPiece w;
     PagedSpan s;
     int first, second;   // tiles of keys that either tile of rows looks at
-    int most;
+    __device__ __forceinline__ int most() const { return max(first, second); }
 };
 template <bool WIN> __device__ __forceinline__ bool pc_next(const PagedPlan &a, PagedRun &run, PcPiece &x) {
     if (!paged_next(a, run, x.w)) return false;
@@ -106,7 +111,6 @@ template <bool WIN> __device__ __forceinline__ bool pc_next(const PagedPlan &a, 
     };
     x.first = tiles(0, min(rows, PC_Q));
     x.second = tiles(PC_Q, rows);
-    x.most = max(x.first, x.second);
     return true;
 }
 
@@ -122,7 +126,7 @@ template <int SLOTS, int RAWS> struct PcShared {
         };
         struct {
             PagedRun start;                     // that run, over the sums alone: other threads may still read what was found
-            float scales[RAWS > 0 ? RAWS : 1][2][PC_KEYS / PC_ROWS];   // of a tile of codes, keys and values; behind a barrier of all
+            float scales[RAWS > 0 ? SLOTS + RAWS : 1][2][PC_KEYS / PC_ROWS];   // of tiles of codes, keys and values, as many as are on their way or in use; behind a barrier of all
         };
     };
     // of every softmax warp: its run, the piece that it is at and the next one (kept from its registers, which the scores fill)
@@ -237,17 +241,117 @@ __device__ __forceinline__ void exchange4(uint4 (&o)[4], int lane) {
     swap(o[1], o[3], lane & 2, 2);
 }
 
-// Eight codes as eight bf16 values: exact where the scale is a power of two (and the value no smaller than bf16's least).
-__device__ __forceinline__ uint4 pc_values(uint32_t x, uint32_t y, float scale) {
-    auto two = [&](uint32_t codes) {
-        const float2 f = floats_of_codes(codes);
-        const __nv_bfloat162 b = __floats2bfloat162_rn(f.x * scale, f.y * scale);
-        return *reinterpret_cast<const uint32_t *>(&b);
+// Over codes the operands are f16: codes as they are, queries in units of a power of two of their row's, weights times their block's scale.  So nothing is multiplied but
+// scores (a block's scale beside the softmax's) and weights.  A tile's weights are in units of `vref`, a scale of values that moves as the maximum does: up to any larger one, down where
+// f16 would lose bits of them.  Where scales of a tile are too far apart for that, the row's sum becomes NaN, and it is computed again in f32 like those that meet NaN.
+constexpr float PC_UP = 128.f, PC_LESS = 9.765625e-4f, PC_APART = 9.5367432e-7f, PC_NOTHING = 8.6736174e-19f, PC_ZEROS = 7.8886091e-31f;   // 2^7, 2^-10, 2^-20, 2^-60, 2^-100
+template <int HD, bool EDGE, bool WIN, class Before>
+__device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, int sinks, int since, const float (*scales)[PC_KEYS / PC_ROWS], bool has_o, float &top, float &sum,
+                                                 float &vref, uint64_t *taken, uint64_t *ready, Before before) {
+    constexpr int BLOCKS = PC_KEYS / PC_ROWS;
+    uint32_t va[32], vb[32], vc[16];
+    tmem_ld32_start(va, s_addr);
+    tmem_ld32_start(vb, s_addr + 32);
+    tmem_ld16_start(vc, s_addr + 64);
+    float vm = 0.f, apart = INFINITY, scale[BLOCKS], weigh[BLOCKS];   // of a block: what its scores are multiplied by; its weights
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+        scale[b] = fmaxf(sl * scales[0][b], 1.17549435e-38f);   // above 0, so that hidden scores stay -inf
+        weigh[b] = scales[1][b];
+        vm = fmaxf(vm, weigh[b]);
+        apart = fminf(apart, weigh[b] > PC_ZEROS ? weigh[b] : INFINITY);
+    }
+    tmem_ld16_wait(vc);
+    tmem_ld32_wait(va);
+    tmem_ld32_wait(vb);
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) bar_arrive(taken);
+    auto v = [&](int k) -> uint32_t & { return k < 32 ? va[k] : k < 64 ? vb[k - 32] : vc[k - 64]; };
+    if (flip)   // a negative scale
+#pragma unroll
+        for (int k = 0; k < PC_KEYS; ++k) v(k) ^= 0x80000000u;
+    if constexpr (EDGE && WIN) {
+        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };   // bits of the keys below n
+#pragma unroll
+        for (int w = 0; w < PC_KEYS; w += 32) {
+            const uint32_t seen = below(lim + 1 - w) & (below(sinks - w) | ~below(since - w));
+#pragma unroll
+            for (int k = w; k < w + 32 && k < PC_KEYS; ++k)
+                if (!((seen >> (k - w)) & 1)) v(k) = 0xff800000u;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < PC_KEYS; ++k)
+            if (EDGE && k > lim) v(k) = 0xff800000u;
+    }
+    float best = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+        float m0 = max3(__uint_as_float(v(16 * b)), __uint_as_float(v(16 * b + 1)), __uint_as_float(v(16 * b + 2))), m1 = max3(__uint_as_float(v(16 * b + 3)), __uint_as_float(v(16 * b + 4)), __uint_as_float(v(16 * b + 5)));
+#pragma unroll
+        for (int k = 6; k < 14; k += 4) {
+            m0 = max3(m0, __uint_as_float(v(16 * b + k)), __uint_as_float(v(16 * b + k + 1)));
+            m1 = max3(m1, __uint_as_float(v(16 * b + k + 2)), __uint_as_float(v(16 * b + k + 3)));
+        }
+        m0 = max3(m0, __uint_as_float(v(16 * b + 14)), __uint_as_float(v(16 * b + 15)));
+        best = fmaxf(best, fmaxf(m0, m1) * scale[b]);
+    }
+    const float now = best > top + PC_SLACK ? best : top;
+    float unit = vref;
+    if (vm > vref || (vm < vref * PC_LESS && vm > vref * PC_NOTHING)) unit = fmaxf(vm, 3.0092655e-36f);
+    if (apart < vm * PC_APART || (vm > PC_ZEROS && vm <= vref * PC_NOTHING)) sum = __uint_as_float(0x7fc00000u);
+    before();
+    if (__any_sync(0xffffffffu, now != top || unit != vref)) {
+        const float keep = ex2(top - now), corr = unit == vref ? keep : keep * (vref / unit);
+        sum *= keep;
+        top = now;
+        vref = unit;
+        if (has_o) {
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(o, o_addr + 32 * c);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
+                tmem_st32(o_addr + 32 * c, o);
+            }
+        }
+    }
+    const float inverse = vref > 0.f ? PC_UP / vref : 0.f;
+    const uint64_t top2 = pair(-top, -top);
+    uint64_t total[2] = {0ull, 0ull};
+    auto weights = [&](int k) {   // of keys k and k + 1
+        const float m = scale[k >> 4], f = weigh[k >> 4] * inverse;
+        const uint64_t e = ex2_pair(fma2(pair(__uint_as_float(v(k)), __uint_as_float(v(k + 1))), pair(m, m), top2));
+        total[(k >> 1) & 1] = add2(total[(k >> 1) & 1], e);
+        const uint64_t w = mul2(e, pair(f, f));
+        const __half2 h = __floats2half2_rn(low(w), high(w));
+        return *reinterpret_cast<const uint32_t *>(&h);
     };
-    return make_uint4(two(x), two(x >> 16), two(y), two(y >> 16));
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        uint32_t p[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) p[k] = weights(32 * c + 2 * k);
+        tmem_st16(s_addr + PC_KEYS + 16 * c, p);
+    }
+    {
+        uint32_t p[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) p[k] = weights(64 + 2 * k);
+        tmem_st8(s_addr + PC_KEYS + 32, p);
+    }
+    total[0] = add2(total[0], total[1]);
+    sum += low(total[0]) + high(total[0]);
+    asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) bar_arrive(ready);
 }
 
-// E8: pages of e4m3.  Four more warps make a tile's codes, which come by bulk copies, bf16 values in the ring's slots; all other roles are the same.
+// E8: pages of e4m3.  Four more warps make a tile's codes, which come by bulk copies, f16 in the ring's slots; issue is the same but for the type.
 // WIN: a window.
 template <int HD, bool E8, bool WIN>
 __global__ void __launch_bounds__(PcShape<HD, E8>::THREADS, 1)
@@ -286,14 +390,14 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     // the block's registers: 128 threads of 72 and 256 of 216 are the 384 of 168 that it was launched with
     // (E8: 256 of 56 and 256 of 200 are the 512 of 128)
     if (E8 && warp >= PC_THREADS / 32) {
-        // ---------------------------------------------------------- codes to values
+        // ---------------------------------------------------------- codes to f16
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PC_FEW_REGS));
         constexpr int CH = HD / 16, ALL = PC_KEYS * CH;   // pieces of 16 codes of a row, and of a tile
         const int me = threadIdx.x - PC_THREADS;
         int n = 0;
         while (pc_next<WIN>(a.plan, run, x)) {
             const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
-            for (int j = 0; j < x.most; ++j, ++n) {
+            for (int j = 0; j < x.most(); ++j, ++n) {
                 const int slot = n % S::SLOTS, raw = n % (S::RAWS > 0 ? S::RAWS : 1), key0 = x.s.lo + j * PC_KEYS;
                 warp_wait(&sh.rfull[raw], (n / (S::RAWS > 0 ? S::RAWS : 1)) & 1, failed);
                 warp_wait(&sh.empty[slot], ((n / S::SLOTS) & 1) ^ 1, failed);
@@ -306,8 +410,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         const bool in = key < x.s.hi && !(WIN && paged_hidden(a.plan, x.s, paged_key(hole, key & ~(PAGED_BLOCK - 1)), PAGED_BLOCK));
                         uint4 c = make_uint4(0u, 0u, 0u, 0u);
                         if (in) c = *reinterpret_cast<const uint4 *>(codes + raw * S::RAW + (kv * PC_KEYS + r) * HD + ch * 16);
-                        const float scale = sh.scales[raw][kv][r / PAGED_BLOCK];
-                        const uint4 lo = pc_values(c.x, c.y, in ? scale : 0.f), hi = pc_values(c.z, c.w, in ? scale : 0.f);
+                        const uint4 lo = make_uint4(f16x2_of_codes(c.x), f16x2_of_codes(c.x >> 16), f16x2_of_codes(c.y), f16x2_of_codes(c.y >> 16));
+                        const uint4 hi = make_uint4(f16x2_of_codes(c.z), f16x2_of_codes(c.z >> 16), f16x2_of_codes(c.w), f16x2_of_codes(c.w >> 16));
                         // 16 codes are two chunks of the row in its box of 64 elements; those of the second box go in the other order, so that eight lanes meet in no bank
                         uint8_t *row = ring + (2 * slot + kv) * S::TILE + (ch >> 2) * PC_BOX + r * 128;
                         const int c0 = 2 * (ch & 3), odd = (ch >> 2) & 1;
@@ -330,7 +434,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             int n = 0;
             while (pc_next<WIN>(a.plan, run, x)) {
                 const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
-                for (int j = 0; j < x.most; ++j, ++n) {
+                for (int j = 0; j < x.most(); ++j, ++n) {
                     const int v = x.s.lo + j * PC_KEYS + lane * PC_ROWS, key = WIN ? paged_key(hole, v) : v;
                     const bool mine = lane < PC_KEYS / PC_ROWS && v < x.s.hi && !(WIN && paged_hidden(a.plan, x.s, key, PC_ROWS));
                     const size_t row = mine ? (((size_t)paged_page(p, x.w.row, key, a.status) * p.kv_heads + x.w.head) << p.page_shift) + (key & ((1 << p.page_shift) - 1)) : 0;
@@ -338,7 +442,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * PC_ROWS * HD;
                     const int raw = n % (S::RAWS > 0 ? S::RAWS : 1);
                     warp_wait(&sh.rempty[raw], ((n / (S::RAWS > 0 ? S::RAWS : 1)) & 1) ^ 1, failed);
-                    if (mine) { sh.scales[raw][0][lane] = ks; sh.scales[raw][1][lane] = vs; }
+                    if (lane < PC_KEYS / PC_ROWS) { sh.scales[n % (S::SLOTS + S::RAWS)][0][lane] = ks; sh.scales[n % (S::SLOTS + S::RAWS)][1][lane] = vs; }
                     __syncwarp();
                     if (lane == 0) bar_expect_tx(&sh.rfull[raw], (uint32_t)(2 * bytes));
                     __syncwarp();
@@ -353,7 +457,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             int n = 0;
             while (pc_next<WIN>(a.plan, run, x)) {
                 const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
-                for (int j = 0; j < x.most; ++j) {
+                for (int j = 0; j < x.most(); ++j) {
                     const int v = x.s.lo + j * PC_KEYS + lane * PC_ROWS, key = WIN ? paged_key(hole, v) : v;
                     const bool mine = lane < PC_KEYS / PC_ROWS && v < x.s.hi;
                     // a block that no token sees comes from behind the pool, as zeros
@@ -377,7 +481,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
         } else if (warp < 3) {
             // ---------------------------------------------------------- MMA issue for a tile of rows
-            constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
+            constexpr uint32_t IDESC = (1u << 4) | (E8 ? 0u : (1u << 7) | (1u << 10)) | ((128u >> 4) << 24);   // both operands f16, or bf16
             constexpr uint32_t S_DESC = IDESC | ((uint32_t)(PC_KEYS >> 3) << 17), O_DESC = IDESC | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
             const int g = warp - 1;
             const uint32_t s_at = tmem + (uint32_t)(g * 128), p_at = s_at + PC_KEYS, o_at = tmem_o + (uint32_t)(g * HD);
@@ -406,7 +510,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     warp_wait(&sh.qfull[g], asked++ & 1, failed);
                     scores(n);
                 }
-                for (int j = 0; j < x.most; ++j, ++n) {
+                for (int j = 0; j < x.most(); ++j, ++n) {
                     const int slot = n % S::SLOTS;
                     if (j + 1 < tiles) scores(n + 1);
                     if (j >= tiles) {   // only the other tile of rows looks at this one
@@ -447,7 +551,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             bool more;
             while ((more = pc_next<WIN>(a.plan, run, x))) {
                 n0 = n;
-                n += x.most;
+                n += x.most();
                 if (threadIdx.x == PC_THREADS - 1) paged_cut(a, run, x.w, x.s, blockIdx.x);
                 if (x.s.ntok * group > g * PC_Q) break;
             }
@@ -458,11 +562,36 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             return more;
         };
         // its queries, on their way to shared memory
+        float back = 1.f, vref = 0.f;   // E8: what the row's queries are to be multiplied by; the unit of its weights
         auto fetch_q = [&]() {
             const PcPiece &x = sh.piece[warp - 4][here];
             if ((g ? x.second : x.first) == 0) return;   // nothing to ask
             const PagedSpan s = x.s;
             const long long first = x.w.r.first + s.t0, head0 = x.w.head * group;
+            if constexpr (E8) {   // a thread its row: as f16 with the largest between 2^14 and 2^15, exact for all that are not 2^-28 of it or less
+                const int rr = g * PC_Q + r, tok = paged_token(a.plan, rr);
+                const bool in = rr < s.ntok * group;
+                const uint4 *src = (const uint4 *)((const __nv_bfloat16 *)a.q + (first + (in ? tok : 0)) * a.q_stride + (head0 + (in ? rr - tok * group : 0)) * HD);
+                uint4 q[HD / 8];
+                float most = 0.f;
+#pragma unroll
+                for (int i = 0; i < HD / 8; ++i) q[i] = in ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                for (int i = 0; i < HD / 8; ++i)
+                    for (uint32_t w : {q[i].x, q[i].y, q[i].z, q[i].w}) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u))));
+                const int up = min(max(268 - (int)(__float_as_uint(most) >> 23), 1), 253);
+                const float f = __uint_as_float((uint32_t)up << 23);
+                back = __uint_as_float((uint32_t)(254 - up) << 23);
+#pragma unroll
+                for (int i = 0; i < HD / 8; ++i) {
+                    auto two = [&](uint32_t w) {
+                        const __half2 h = __floats2half2_rn(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xffff0000u) * f);
+                        return *reinterpret_cast<const uint32_t *>(&h);
+                    };
+                    *reinterpret_cast<uint4 *>(qbuf + g * S::QTILE + (i >> 3) * PC_QBOX + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(two(q[i].x), two(q[i].y), two(q[i].z), two(q[i].w));
+                }
+                return;
+            }
             const int i0 = threadIdx.x & 127, rows = s.ntok * group;
             const bool twice = rows <= PC_TWICE;
 #pragma unroll
@@ -484,7 +613,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.qfull[g]);
             }
-            const bool twice = rows <= PC_TWICE;   // and this the first tile of rows
+            const bool twice = !E8 && rows <= PC_TWICE;   // and this the first tile of rows
+            const float row_sl = E8 ? sl * back : sl;
+            vref = 0.f;
             const bool second = twice && (lane & PC_TWICE);
             const int rr = g * PC_Q + r, asks = twice && r < 2 * PC_TWICE ? r % PC_TWICE : rr;
             const int gap = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile).gap : 0, first = x.s.base + x.s.t0 - gap;   // all in virtual keys
@@ -511,10 +642,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                 const int lim = min(pos, hi - 1) - at, low = WIN ? pos + 1 - a.plan.window - at : 0;
                 auto before = [&] { if (j > 0) warp_wait(&sh.odone[g], (scored - 1) & 1, failed); };
-                if (at + PC_KEYS - 1 > least || at + PC_KEYS > hi || (g + 1) * PC_Q > rows || (WIN && at < late && at + PC_KEYS > a.plan.sinks))
+                const bool edge = at + PC_KEYS - 1 > least || at + PC_KEYS > hi || (g + 1) * PC_Q > rows || (WIN && at < late && at + PC_KEYS > a.plan.sinks);
+                if constexpr (E8) {
+                    const float (*scales)[PC_KEYS / PC_ROWS] = sh.scales[(slot0 + j) % (S::SLOTS + S::RAWS)];
+                    if (edge) pc_softmax_codes<HD, true, WIN>(s_addr, o_addr, row_sl, flip, lim, WIN ? a.plan.sinks - at : 0, low, scales, j > 0, top, sum, vref, &sh.sfree[g], &sh.pfull[g], before);
+                    else pc_softmax_codes<HD, false, WIN>(s_addr, o_addr, row_sl, flip, lim, 0, 0, scales, j > 0, top, sum, vref, &sh.sfree[g], &sh.pfull[g], before);
+                } else if (edge)
                     pc_softmax<HD, true, WIN>(s_addr, o_addr, sl, flip, lim, WIN ? a.plan.sinks - at : 0, low, second, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
                 else pc_softmax<HD, false, WIN>(s_addr, o_addr, sl, flip, lim, 0, 0, false, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
             }
+            const float unit = E8 ? vref * (1.f / PC_UP) : 1.f;
             // the scores are all made: the next piece's queries may take the place of these, while the sums go out
             more = next();
             if (more) fetch_q();
@@ -524,7 +661,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             const bool all = w.k0 == 0 && w.k1 == w.k_tiles;
             const size_t slot = (2 * (size_t)blockIdx.x + (w.k0 == 0)) * a.tile_rows;
-            const float f = !all ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+            const float f = !all ? (E8 && sum != sum ? sum : unit) : sum == 0.f ? 0.f : unit / sum;
             float poison = 0.f;  // stays 0 unless an output is Inf or NaN
             // A lane has a row, 16 bytes of which at a time would go to 32 places: four lanes exchange pieces and store 64 bytes of a row each time.
             __nv_bfloat16 *dst[4];
