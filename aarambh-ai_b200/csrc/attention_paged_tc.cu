@@ -43,19 +43,19 @@ using namespace ab2::tc;
 namespace ab2 {
 namespace {
 
-constexpr int PC_Q = 128, PC_KEYS = 80, PC_THREADS = 384, PC_EXPAND = 128;
+constexpr int PC_Q = 128, PC_KEYS = 80, PC_THREADS = 384, PC_LOAD = 128;   // threads; those that load codes
 constexpr int PC_QBOX = PC_Q * 128, PC_BOX = PC_KEYS * 128;   // boxes of queries, and of keys or values: rows of 64 elements
 constexpr int PC_ROWS = 16;   // that one copy brings: the least that a page holds
 constexpr int PC_TWICE = 16;  // query rows of an item up to which it has each of them twice, for both terms of its weights
-constexpr int PC_FEW_REGS = 56, PC_MANY_REGS = 200;   // E8: of a thread of other roles, and of softmax
+constexpr int PC_FEW_REGS = 72, PC_LOAD_REGS = 104, PC_MANY_REGS = 168;   // over codes, of a thread of copies and issue, of loads, and of softmax: 128 of either of the first, and 256, are the 512 of 128 of the launch
 constexpr float PC_SLACK = 8.f;  // powers of two a score may exceed the row's maximum by
 constexpr float PC_NONE = -1e30f;
 
 template <int HD, bool E8 = false> struct PcShape {
-    static constexpr int THREADS = PC_THREADS + (E8 ? PC_EXPAND : 0);
-    static constexpr int BOXES = HD / 64, QTILE = BOXES * PC_QBOX, TILE = BOXES * PC_BOX, SLOTS = (E8 ? 3 : 4) * (HD == 128 ? 1 : 2);   // a slot holds a tile's keys and its values
-    static constexpr int RAW = E8 ? 2 * PC_KEYS * HD : 0, RAWS = E8 ? (HD == 128 ? 2 : 4) : 0;   // codes of a tile's keys and values, and tiles of them
-    static constexpr int SMEM = 1024 + 2 * QTILE + SLOTS * 2 * TILE + RAWS * RAW;
+    static constexpr int THREADS = PC_THREADS + (E8 ? PC_LOAD : 0);
+    static constexpr int BOXES = HD / 64, QTILE = BOXES * PC_QBOX, VTILE = BOXES * PC_BOX, KTILE = E8 ? PC_KEYS * HD : VTILE;   // bytes of a tile: queries (over codes two terms of 8 bits), values, keys
+    static constexpr int SLOTS = HD == 128 ? (E8 ? 5 : 4) : 8, SLOT = KTILE + VTILE;   // a slot holds a tile's keys and its values
+    static constexpr int SMEM = 1024 + 2 * QTILE + SLOTS * SLOT;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -87,11 +87,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
 __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) { return pair(ex2(low(x)), ex2(high(x))); }
 // What all roles know of a piece.
 struct PcPiece {
@@ -114,19 +109,21 @@ template <bool WIN> __device__ __forceinline__ bool pc_next(const PagedPlan &a, 
     return true;
 }
 
-template <int SLOTS, int RAWS> struct PcShared {
+struct PcScales {
+    float k[PC_KEYS / PC_ROWS], v;   // of the blocks of keys, and the unit of the values
+};
+template <int SLOTS, int THREADS> struct PcShared {
     uint64_t full[SLOTS], empty[SLOTS], qfull[2], sfull[2], sfree[2], pfull[2], odone[2];
-    uint64_t rfull[RAWS > 0 ? RAWS : 1], rempty[RAWS > 0 ? RAWS : 1];
     uint32_t tmem_base;
     int failed;
     union {
         struct {                                // while the CTA looks for its run
-            long long warp_sums[(PC_THREADS + (RAWS > 0 ? PC_EXPAND : 0)) / 32];
+            long long warp_sums[THREADS / 32];
             int2 found[2];
         };
         struct {
             PagedRun start;                     // that run, over the sums alone: other threads may still read what was found
-            float scales[RAWS > 0 ? SLOTS + RAWS : 1][2][PC_KEYS / PC_ROWS];   // of tiles of codes, keys and values, as many as are on their way or in use; behind a barrier of all
+            PcScales scales[THREADS > PC_THREADS ? SLOTS : 1];   // of a slot's codes; behind a barrier of all
         };
     };
     // of every softmax warp: its run, the piece that it is at and the next one (kept from its registers, which the scores fill)
@@ -241,26 +238,25 @@ __device__ __forceinline__ void exchange4(uint4 (&o)[4], int lane) {
     swap(o[1], o[3], lane & 2, 2);
 }
 
-// Over codes the operands are f16: codes as they are, queries in units of a power of two of their row's, weights times their block's scale.  So nothing is multiplied but
-// scores (a block's scale beside the softmax's) and weights.  A tile's weights are in units of `vref`, a scale of values that moves as the maximum does: up to any larger one, down where
-// f16 would lose bits of them.  Where scales of a tile are too far apart for that, the row's sum becomes NaN, and it is computed again in f32 like those that meet NaN.
-constexpr float PC_UP = 128.f, PC_LESS = 9.765625e-4f, PC_APART = 9.5367432e-7f, PC_NOTHING = 8.6736174e-19f, PC_ZEROS = 7.8886091e-31f;   // 2^7, 2^-10, 2^-20, 2^-60, 2^-100
+// Over codes keys are multiplied as they are, with queries in two e4m3 terms: a bf16 number has 8 significant bits, and is the sum of two of 4 (in units of a power of two of
+// its row's that puts the largest at 224 to 448; below 2^-2 the second term has fewer: 2^-18 of the row's largest element off at most).  A block's scale multiplies its scores beside the
+// softmax's factor.  Values are f16, in units of the tile's largest scale (a block's other scale is a power of two below it, and exact down to 2^-15); their weights are f16 in units of `vref`, a
+// scale of values that moves as the maximum does: up to any larger one, down where f16 would lose bits of them.  A tile whose scales of values lie too far apart has NaN for its unit:
+// the sums of all its rows become NaN, and they are computed again in f32 like those that meet NaN.
+constexpr float PC_UP = 128.f, PC_LESS = 9.765625e-4f, PC_APART = 3.0517578e-5f, PC_NOTHING = 8.6736174e-19f, PC_ZEROS = 7.8886091e-31f;   // 2^7, 2^-10, 2^-15, 2^-60, 2^-100
 template <int HD, bool EDGE, bool WIN, class Before>
-__device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, int sinks, int since, const float (*scales)[PC_KEYS / PC_ROWS], bool has_o, float &top, float &sum,
-                                                 float &vref, uint64_t *taken, uint64_t *ready, Before before) {
+__device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, int sinks, int since, const PcScales &of, bool has_o, float &top, float &sum, float &vref,
+                                                 uint64_t *taken, uint64_t *ready, Before before) {
     constexpr int BLOCKS = PC_KEYS / PC_ROWS;
     uint32_t va[32], vb[32], vc[16];
     tmem_ld32_start(va, s_addr);
     tmem_ld32_start(vb, s_addr + 32);
     tmem_ld16_start(vc, s_addr + 64);
-    float vm = 0.f, apart = INFINITY, scale[BLOCKS], weigh[BLOCKS];   // of a block: what its scores are multiplied by; its weights
+    float scale[BLOCKS], unit = vref;
 #pragma unroll
-    for (int b = 0; b < BLOCKS; ++b) {
-        scale[b] = fmaxf(sl * scales[0][b], 1.17549435e-38f);   // above 0, so that hidden scores stay -inf
-        weigh[b] = scales[1][b];
-        vm = fmaxf(vm, weigh[b]);
-        apart = fminf(apart, weigh[b] > PC_ZEROS ? weigh[b] : INFINITY);
-    }
+    for (int b = 0; b < BLOCKS; ++b) scale[b] = fmaxf(sl * of.k[b], 1.17549435e-38f);   // above 0, so that hidden scores stay -inf
+    const float values = of.v;
+    if (values > vref || (values < vref * PC_LESS && values > vref * PC_NOTHING)) unit = fmaxf(values, 3.0092655e-36f);
     tmem_ld16_wait(vc);
     tmem_ld32_wait(va);
     tmem_ld32_wait(vb);
@@ -288,19 +284,16 @@ __device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_add
     float best = -INFINITY;
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) {
-        float m0 = max3(__uint_as_float(v(16 * b)), __uint_as_float(v(16 * b + 1)), __uint_as_float(v(16 * b + 2))), m1 = max3(__uint_as_float(v(16 * b + 3)), __uint_as_float(v(16 * b + 4)), __uint_as_float(v(16 * b + 5)));
+        auto s = [&](int k) { return __uint_as_float(v(16 * b + k)); };
+        float m0 = max3(s(0), s(1), s(2)), m1 = max3(s(3), s(4), s(5));
 #pragma unroll
         for (int k = 6; k < 14; k += 4) {
-            m0 = max3(m0, __uint_as_float(v(16 * b + k)), __uint_as_float(v(16 * b + k + 1)));
-            m1 = max3(m1, __uint_as_float(v(16 * b + k + 2)), __uint_as_float(v(16 * b + k + 3)));
+            m0 = max3(m0, s(k), s(k + 1));
+            m1 = max3(m1, s(k + 2), s(k + 3));
         }
-        m0 = max3(m0, __uint_as_float(v(16 * b + 14)), __uint_as_float(v(16 * b + 15)));
-        best = fmaxf(best, fmaxf(m0, m1) * scale[b]);
+        best = max3(best, max3(m0, s(14), s(15)) * scale[b], m1 * scale[b]);
     }
     const float now = best > top + PC_SLACK ? best : top;
-    float unit = vref;
-    if (vm > vref || (vm < vref * PC_LESS && vm > vref * PC_NOTHING)) unit = fmaxf(vm, 3.0092655e-36f);
-    if (apart < vm * PC_APART || (vm > PC_ZEROS && vm <= vref * PC_NOTHING)) sum = __uint_as_float(0x7fc00000u);
     before();
     if (__any_sync(0xffffffffu, now != top || unit != vref)) {
         const float keep = ex2(top - now), corr = unit == vref ? keep : keep * (vref / unit);
@@ -319,15 +312,14 @@ __device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_add
             }
         }
     }
-    const float inverse = vref > 0.f ? PC_UP / vref : 0.f;
-    const uint64_t top2 = pair(-top, -top);
+    // the tile's values in units of vref, 2^7 larger; 2^-40 and less makes weights of nothing (and their sum is still theirs)
+    const float f = vref > 0.f ? fmaxf(values / vref * PC_UP, 9.0949470e-13f) : PC_UP, shifted = __log2f(f) - top;
+    const uint64_t top2 = pair(shifted, shifted);
     uint64_t total[2] = {0ull, 0ull};
     auto weights = [&](int k) {   // of keys k and k + 1
-        const float m = scale[k >> 4], f = weigh[k >> 4] * inverse;
-        const uint64_t e = ex2_pair(fma2(pair(__uint_as_float(v(k)), __uint_as_float(v(k + 1))), pair(m, m), top2));
+        const uint64_t e = ex2_pair(fma2(pair(__uint_as_float(v(k)), __uint_as_float(v(k + 1))), pair(scale[k >> 4], scale[k >> 4]), top2));
         total[(k >> 1) & 1] = add2(total[(k >> 1) & 1], e);
-        const uint64_t w = mul2(e, pair(f, f));
-        const __half2 h = __floats2half2_rn(low(w), high(w));
+        const __half2 h = __floats2half2_rn(low(e), high(e));
         return *reinterpret_cast<const uint32_t *>(&h);
     };
 #pragma unroll
@@ -344,14 +336,15 @@ __device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_add
         tmem_st8(s_addr + PC_KEYS + 32, p);
     }
     total[0] = add2(total[0], total[1]);
-    sum += low(total[0]) + high(total[0]);
+    sum = fmaf(low(total[0]) + high(total[0]), 1.f / f, sum);
+    if (values != values) sum = values;
     asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncwarp();
     if ((threadIdx.x & 31) == 0) bar_arrive(ready);
 }
 
-// E8: pages of e4m3.  Four more warps make a tile's codes, which come by bulk copies, f16 in the ring's slots; issue is the same but for the type.
+// E8: pages of e4m3.  Keys come by the same copies; four more warps load values, a tile ahead, and make them f16 in the ring's slots.
 // WIN: a window.
 template <int HD, bool E8, bool WIN>
 __global__ void __launch_bounds__(PcShape<HD, E8>::THREADS, 1)
@@ -359,15 +352,14 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     using S = PcShape<HD, E8>;
     using Page = std::conditional_t<E8, uint8_t, __nv_bfloat16>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ PcShared<S::SLOTS, S::RAWS> sh;
+    __shared__ PcShared<S::SLOTS, S::THREADS> sh;
     static_assert(S::SMEM + sizeof(sh) <= 227 * 1024, "shared memory of a CTA");
     static_assert(sizeof(PagedRun) <= S::THREADS / 32 * sizeof(long long), "the run lies over the sums");
-    uint8_t *qbuf = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023), *ring = qbuf + 2 * S::QTILE, *codes = ring + S::SLOTS * 2 * S::TILE;
+    uint8_t *qbuf = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023), *ring = qbuf + 2 * S::QTILE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *failed = &sh.failed;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::SLOTS; ++i) { bar_init(&sh.full[i], E8 ? PC_EXPAND / 32 : 1); bar_init(&sh.empty[i], 2); }
-        for (int i = 0; i < S::RAWS; ++i) { bar_init(&sh.rfull[i], 1); bar_init(&sh.rempty[i], PC_EXPAND / 32); }
+        for (int i = 0; i < S::SLOTS; ++i) { bar_init(&sh.full[i], 1 + (E8 ? PC_LOAD / 64 : 0)); bar_init(&sh.empty[i], 2); }
         for (int i = 0; i < 2; ++i) { bar_init(&sh.qfull[i], 4); bar_init(&sh.sfull[i], 1); bar_init(&sh.sfree[i], 4); bar_init(&sh.pfull[i], 4); bar_init(&sh.odone[i], 1); }
         sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -388,72 +380,89 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const PagedView &p = a.plan.p;
     PcPiece x;
     // the block's registers: 128 threads of 72 and 256 of 216 are the 384 of 168 that it was launched with
-    // (E8: 256 of 56 and 256 of 200 are the 512 of 128)
     if (E8 && warp >= PC_THREADS / 32) {
-        // ---------------------------------------------------------- codes to f16
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PC_FEW_REGS));
-        constexpr int CH = HD / 16, ALL = PC_KEYS * CH;   // pieces of 16 codes of a row, and of a tile
-        const int me = threadIdx.x - PC_THREADS;
-        int n = 0;
-        while (pc_next<WIN>(a.plan, run, x)) {
+        // ---------------------------------------------------------- values from codes
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PC_LOAD_REGS));
+        // Either half of these warps has every other tile, so that two tiles' loads are on their way.  Piece i of a tile is 16 codes of row i / CH; a thread has pieces me, me + 64, ...
+        constexpr int CH = HD / 16, HALF = PC_LOAD / 2, MINE = PC_KEYS * CH / HALF, BLOCKS = PC_KEYS / PC_ROWS;
+        static_assert(PC_KEYS * CH % HALF == 0, "a tile's pieces");
+        const int half = (warp - PC_THREADS / 32) / (HALF / 32), me = (threadIdx.x - PC_THREADS) % HALF, row0 = me / CH, ch = me % CH;
+        constexpr int ROWS = HALF / CH;   // from a piece to the next
+        uint4 vc[MINE];
+        long long at = -1;            // lane b: where block b of the tile to load begins, in rows of a head; -1: nothing of it is in sight
+        float ks = 0.f, vs = 0.f;     // its scales
+        int j = -1, n = -1, hi = 0, key0 = 0;   // n: the tile to load, of all
+        bool more;
+        auto seek = [&]() {   // this half's next tile, and its blocks
+            more = true;
+            do {
+                ++n;
+                for (++j; j >= x.most(); j = 0)
+                    if (!pc_next<WIN>(a.plan, run, x)) { more = false; return; }
+            } while ((n & 1) != half);
             const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
-            for (int j = 0; j < x.most(); ++j, ++n) {
-                const int slot = n % S::SLOTS, raw = n % (S::RAWS > 0 ? S::RAWS : 1), key0 = x.s.lo + j * PC_KEYS;
-                warp_wait(&sh.rfull[raw], (n / (S::RAWS > 0 ? S::RAWS : 1)) & 1, failed);
-                warp_wait(&sh.empty[slot], ((n / S::SLOTS) & 1) ^ 1, failed);
+            key0 = x.s.lo + j * PC_KEYS;
+            hi = x.s.hi;
+            const int v = key0 + lane * PC_ROWS, key = WIN ? paged_key(hole, v) : v;
+            const bool in = lane < BLOCKS && v < hi && !(WIN && paged_hidden(a.plan, x.s, key, PC_ROWS));
+            at = in ? (((long long)paged_page(p, x.w.row, key, a.status) * p.kv_heads + x.w.head) << p.page_shift) + (key & ((1 << p.page_shift) - 1)) : -1;
+        };
+        auto load = [&]() {
+            ks = at >= 0 ? __ldg(a.k_scales + at / PAGED_BLOCK) : 0.f;
+            vs = at >= 0 ? __ldg(a.v_scales + at / PAGED_BLOCK) : 0.f;
 #pragma unroll
-                for (int kv = 0; kv < 2; ++kv)
-#pragma unroll
-                    for (int i = me; i < ALL; i += PC_EXPAND) {
-                        const int r = i / CH, ch = i % CH, key = key0 + r;
-                        // behind the piece's keys, and where no token sees a block, zeros
-                        const bool in = key < x.s.hi && !(WIN && paged_hidden(a.plan, x.s, paged_key(hole, key & ~(PAGED_BLOCK - 1)), PAGED_BLOCK));
-                        uint4 c = make_uint4(0u, 0u, 0u, 0u);
-                        if (in) c = *reinterpret_cast<const uint4 *>(codes + raw * S::RAW + (kv * PC_KEYS + r) * HD + ch * 16);
-                        const uint4 lo = make_uint4(f16x2_of_codes(c.x), f16x2_of_codes(c.x >> 16), f16x2_of_codes(c.y), f16x2_of_codes(c.y >> 16));
-                        const uint4 hi = make_uint4(f16x2_of_codes(c.z), f16x2_of_codes(c.z >> 16), f16x2_of_codes(c.w), f16x2_of_codes(c.w >> 16));
-                        // 16 codes are two chunks of the row in its box of 64 elements; those of the second box go in the other order, so that eight lanes meet in no bank
-                        uint8_t *row = ring + (2 * slot + kv) * S::TILE + (ch >> 2) * PC_BOX + r * 128;
-                        const int c0 = 2 * (ch & 3), odd = (ch >> 2) & 1;
-                        *reinterpret_cast<uint4 *>(row + (((c0 + odd) ^ (r & 7)) << 4)) = odd ? hi : lo;
-                        *reinterpret_cast<uint4 *>(row + (((c0 + 1 - odd) ^ (r & 7)) << 4)) = odd ? lo : hi;
-                    }
-                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                __syncwarp();   // every lane's codes have been read, as what it stored is made of them
-                if (lane == 0) {
-                    bar_arrive(&sh.full[slot]);
-                    bar_arrive(&sh.rempty[raw]);
-                }
+            for (int u = 0; u < MINE; ++u) {
+                const int r = row0 + u * ROWS;
+                const long long from = __shfl_sync(0xffffffffu, at, r / PC_ROWS);
+                vc[u] = make_uint4(0u, 0u, 0u, 0u);
+                if (from < 0 || key0 + r >= hi) continue;   // zeros, behind the keys too
+                vc[u] = __ldg(reinterpret_cast<const uint4 *>((const uint8_t *)a.v + (size_t)(from + r % PC_ROWS) * HD + ch * 16));
             }
+        };
+        x.first = x.second = 0;
+        seek();
+        if (more) load();
+        while (more) {
+            // the unit of the tile's values, and its blocks' scales in it
+            float unit = vs;
+#pragma unroll
+            for (int m = 1; m < 8; m <<= 1) unit = fmaxf(unit, __shfl_xor_sync(0xffffffffu, unit, m));
+            const __half2 f = __float2half2_rn(unit > 0.f ? vs / unit : 0.f);
+            if (__any_sync(0xffffffffu, lane < BLOCKS && vs < unit * PC_APART && vs > PC_ZEROS)) unit = __uint_as_float(0x7fc00000u);
+            const float kscale = ks;
+            const int slot = n % S::SLOTS, phase = ((n / S::SLOTS) & 1) ^ 1;
+            seek();   // the table's entries are on their way
+            warp_wait(&sh.empty[slot], phase, failed);
+            if (me < 32) {
+                if (lane < BLOCKS) sh.scales[slot].k[lane] = kscale;
+                if (lane == 0) sh.scales[slot].v = unit;
+            }
+#pragma unroll
+            for (int u = 0; u < MINE; ++u) {
+                const int r = row0 + u * ROWS;
+                const uint32_t fb = __shfl_sync(0xffffffffu, *reinterpret_cast<const uint32_t *>(&f), r / PC_ROWS);
+                auto two = [&](uint32_t codes) {
+                    const uint32_t h = f16x2_of_codes(codes);
+                    const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&h), *reinterpret_cast<const __half2 *>(&fb));
+                    return *reinterpret_cast<const uint32_t *>(&y);
+                };
+                const uint4 c = vc[u], low8 = make_uint4(two(c.x), two(c.x >> 16), two(c.y), two(c.y >> 16)), high8 = make_uint4(two(c.z), two(c.z >> 16), two(c.w), two(c.w >> 16));
+                // 16 codes are two chunks of the row in its box of 64 elements; those of the second box go in the other order, so that eight lanes meet in no bank
+                uint8_t *row = ring + slot * S::SLOT + S::KTILE + (ch >> 2) * PC_BOX + r * 128;
+                const int c0 = 2 * (ch & 3), odd = (ch >> 2) & 1;
+                *reinterpret_cast<uint4 *>(row + (((c0 + odd) ^ (r & 7)) << 4)) = odd ? high8 : low8;
+                *reinterpret_cast<uint4 *>(row + (((c0 + 1 - odd) ^ (r & 7)) << 4)) = odd ? low8 : high8;
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.full[slot]);
+            if (more) load();
         }
     } else if (warp < 4) {
         if (E8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PC_FEW_REGS));
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
-        if (E8 && warp == 0) {
-            // ---------------------------------------------------------- producer of codes
-            int n = 0;
-            while (pc_next<WIN>(a.plan, run, x)) {
-                const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
-                for (int j = 0; j < x.most(); ++j, ++n) {
-                    const int v = x.s.lo + j * PC_KEYS + lane * PC_ROWS, key = WIN ? paged_key(hole, v) : v;
-                    const bool mine = lane < PC_KEYS / PC_ROWS && v < x.s.hi && !(WIN && paged_hidden(a.plan, x.s, key, PC_ROWS));
-                    const size_t row = mine ? (((size_t)paged_page(p, x.w.row, key, a.status) * p.kv_heads + x.w.head) << p.page_shift) + (key & ((1 << p.page_shift) - 1)) : 0;
-                    const float ks = mine ? __ldg(a.k_scales + row / PAGED_BLOCK) : 0.f, vs = mine ? __ldg(a.v_scales + row / PAGED_BLOCK) : 0.f;
-                    const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * PC_ROWS * HD;
-                    const int raw = n % (S::RAWS > 0 ? S::RAWS : 1);
-                    warp_wait(&sh.rempty[raw], ((n / (S::RAWS > 0 ? S::RAWS : 1)) & 1) ^ 1, failed);
-                    if (lane < PC_KEYS / PC_ROWS) { sh.scales[n % (S::SLOTS + S::RAWS)][0][lane] = ks; sh.scales[n % (S::SLOTS + S::RAWS)][1][lane] = vs; }
-                    __syncwarp();
-                    if (lane == 0) bar_expect_tx(&sh.rfull[raw], (uint32_t)(2 * bytes));
-                    __syncwarp();
-                    if (mine && !*failed) {
-                        bulk_copy(codes + raw * S::RAW + lane * PC_ROWS * HD, (const uint8_t *)a.k + row * HD, PC_ROWS * HD, &sh.rfull[raw]);
-                        bulk_copy(codes + raw * S::RAW + (PC_KEYS + lane * PC_ROWS) * HD, (const uint8_t *)a.v + row * HD, PC_ROWS * HD, &sh.rfull[raw]);
-                    }
-                }
-            }
-        } else if (warp == 0) {
-            // ---------------------------------------------------------- TMA producer: K, V, K, V, ...
+        if (warp == 0) {
+            // ---------------------------------------------------------- TMA producer: K, V, K, V, ...; over codes K alone
             int n = 0;
             while (pc_next<WIN>(a.plan, run, x)) {
                 const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
@@ -462,26 +471,27 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     const bool mine = lane < PC_KEYS / PC_ROWS && v < x.s.hi;
                     // a block that no token sees comes from behind the pool, as zeros
                     const int page = !mine ? 0 : WIN && paged_hidden(a.plan, x.s, key, PC_ROWS) ? p.pages : paged_page(p, x.w.row, key, a.status);
-                    const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * PC_ROWS * HD * 2;
+                    const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * PC_ROWS * HD * (E8 ? 1 : 4);
                     const int slot = n % S::SLOTS;
                     warp_wait(&sh.empty[slot], ((n++ / S::SLOTS) & 1) ^ 1, failed);
                     // The first queries come before what is fetched ahead.  Only at the second slot of the run's first piece with keys, and only where the first
                     // tile of rows looks at it: its warps cannot announce their next queries without that slot, so the barrier is in its first phase or just
                     // behind it.  A later phase would have this parity again, and might wait for what is not yet fetched.
-                    if (n == 2 && j == 1 && x.first > 1) warp_wait(&sh.qfull[0], 0, failed);
-                    if (lane == 0) bar_expect_tx(&sh.full[slot], (uint32_t)(2 * bytes));
+                    if (!E8 && n == 2 && j == 1 && x.first > 1) warp_wait(&sh.qfull[0], 0, failed);
+                    if (lane == 0) bar_expect_tx(&sh.full[slot], (uint32_t)bytes);
                     __syncwarp();
-                    if (mine && !*failed)
+                    if (E8 && mine && !*failed) tma_load_3d(ring + slot * S::SLOT + lane * PC_ROWS * HD, &kmap, 0, key & ((1 << p.page_shift) - 1), page * p.kv_heads + x.w.head, &sh.full[slot]);
+                    if (!E8 && mine && !*failed)
 #pragma unroll
                         for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
                             for (int b = 0; b < S::BOXES; ++b)
-                                tma_load_3d(ring + (2 * slot + kv) * S::TILE + b * PC_BOX + lane * PC_ROWS * 128, kv ? &vmap : &kmap, b * 64, key & ((1 << p.page_shift) - 1), page * p.kv_heads + x.w.head, &sh.full[slot]);
+                                tma_load_3d(ring + slot * S::SLOT + kv * S::KTILE + b * PC_BOX + lane * PC_ROWS * 128, kv ? &vmap : &kmap, b * 64, key & ((1 << p.page_shift) - 1), page * p.kv_heads + x.w.head, &sh.full[slot]);
                 }
             }
         } else if (warp < 3) {
             // ---------------------------------------------------------- MMA issue for a tile of rows
-            constexpr uint32_t IDESC = (1u << 4) | (E8 ? 0u : (1u << 7) | (1u << 10)) | ((128u >> 4) << 24);   // both operands f16, or bf16
+            constexpr uint32_t IDESC = (1u << 4) | (E8 ? 0u : (1u << 7) | (1u << 10)) | ((128u >> 4) << 24);   // both operands e4m3 (of scores) or f16, or bf16
             constexpr uint32_t S_DESC = IDESC | ((uint32_t)(PC_KEYS >> 3) << 17), O_DESC = IDESC | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
             const int g = warp - 1;
             const uint32_t s_at = tmem + (uint32_t)(g * 128), p_at = s_at + PC_KEYS, o_at = tmem_o + (uint32_t)(g * HD);
@@ -492,12 +502,22 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 if (scored > 0) warp_wait(&sh.sfree[g], (scored - 1) & 1, failed);
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                 if (elect_one()) {
+                    if constexpr (E8) {   // both terms of the queries: of 128 dimensions two boxes, of 64 the halves of a row
+                        const uint64_t kd = HD == 128 ? umma_desc(sptr(ring + slot * S::SLOT)) : umma_desc_64(sptr(ring + slot * S::SLOT));
 #pragma unroll
-                    for (int b = 0; b < S::BOXES; ++b) {
-                        const uint64_t qd = umma_desc(sptr(qbuf + g * S::QTILE + b * PC_QBOX)), kd = umma_desc(sptr(ring + 2 * slot * S::TILE + b * PC_BOX));
+                        for (int b = 0; b < 2; ++b) {
+                            const uint64_t qd = umma_desc(sptr(qbuf + g * S::QTILE + (HD == 128 ? b * PC_QBOX : 0))) + (uint64_t)(HD == 128 ? 0 : 4 * b);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)  // descriptors count in 16 bytes
-                            umma_bf16(s_at, qd + (uint64_t)(2 * k), kd + (uint64_t)(2 * k), S_DESC, (b | k) != 0);
+                            for (int k = 0; k < HD / 32; ++k) umma_f8(s_at, qd + (uint64_t)(2 * k), kd + (uint64_t)(2 * k), S_DESC, (b | k) != 0);
+                        }
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < S::BOXES; ++b) {
+                            const uint64_t qd = umma_desc(sptr(qbuf + g * S::QTILE + b * PC_QBOX)), kd = umma_desc(sptr(ring + slot * S::SLOT + b * PC_BOX));
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)  // descriptors count in 16 bytes
+                                umma_bf16(s_at, qd + (uint64_t)(2 * k), kd + (uint64_t)(2 * k), S_DESC, (b | k) != 0);
+                        }
                     }
                     umma_commit(&sh.sfull[g]);
                 }
@@ -521,7 +541,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     warp_wait(&sh.pfull[g], done++ & 1, failed);
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                     if (elect_one()) {
-                        const uint64_t vd = umma_desc_mn(sptr(ring + (2 * slot + 1) * S::TILE), PC_BOX);
+                        const uint64_t vd = umma_desc_mn(sptr(ring + slot * S::SLOT + S::KTILE), PC_BOX);
 #pragma unroll
                         for (int k = 0; k < PC_KEYS / 16; ++k)
                             umma_bf16_ts(o_at, p_at + (uint32_t)(8 * k), vd + (uint64_t)(k * (2048 >> 4)), O_DESC, j > 0 || k > 0);
@@ -568,7 +588,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             if ((g ? x.second : x.first) == 0) return;   // nothing to ask
             const PagedSpan s = x.s;
             const long long first = x.w.r.first + s.t0, head0 = x.w.head * group;
-            if constexpr (E8) {   // a thread its row: as f16 with the largest between 2^14 and 2^15, exact for all that are not 2^-28 of it or less
+            if constexpr (E8) {   // a thread its row
                 const int rr = g * PC_Q + r, tok = paged_token(a.plan, rr);
                 const bool in = rr < s.ntok * group;
                 const uint4 *src = (const uint4 *)((const __nv_bfloat16 *)a.q + (first + (in ? tok : 0)) * a.q_stride + (head0 + (in ? rr - tok * group : 0)) * HD);
@@ -579,16 +599,33 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 #pragma unroll
                 for (int i = 0; i < HD / 8; ++i)
                     for (uint32_t w : {q[i].x, q[i].y, q[i].z, q[i].w}) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u))));
-                const int up = min(max(268 - (int)(__float_as_uint(most) >> 23), 1), 253);
-                const float f = __uint_as_float((uint32_t)up << 23);
-                back = __uint_as_float((uint32_t)(254 - up) << 23);
+                // times 2^(127 - down) the largest is between 224 and 448 = 1.75 2^8
+                const uint32_t bits = __float_as_uint(most);
+                const int down = min(max((int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u), 1), 253);
+                const float f = most < INFINITY ? __uint_as_float((uint32_t)(254 - down) << 23) : __uint_as_float(0x7fc00000u);   // Inf has no code
+                back = __uint_as_float((uint32_t)down << 23);
 #pragma unroll
-                for (int i = 0; i < HD / 8; ++i) {
-                    auto two = [&](uint32_t w) {
-                        const __half2 h = __floats2half2_rn(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xffff0000u) * f);
-                        return *reinterpret_cast<const uint32_t *>(&h);
-                    };
-                    *reinterpret_cast<uint4 *>(qbuf + g * S::QTILE + (i >> 3) * PC_QBOX + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(two(q[i].x), two(q[i].y), two(q[i].z), two(q[i].w));
+                for (int i = 0; i < HD / 16; ++i) {
+                    uint32_t high[4], rest[4];
+                    const uint32_t words[8] = {q[2 * i].x, q[2 * i].y, q[2 * i].z, q[2 * i].w, q[2 * i + 1].x, q[2 * i + 1].y, q[2 * i + 1].z, q[2 * i + 1].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t h[2], l[2];
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            const uint32_t w = words[2 * e + d];
+                            const float x = __uint_as_float(w << 16) * f, y = __uint_as_float(w & 0xffff0000u) * f;
+                            h[d] = codes_of(x, y);
+                            const float2 hf = floats_of_codes(h[d]);
+                            l[d] = codes_of(x - hf.x, y - hf.y);
+                        }
+                        high[e] = h[0] | h[1] << 16;
+                        rest[e] = l[0] | l[1] << 16;
+                    }
+                    uint8_t *row = qbuf + g * S::QTILE + r * 128;
+                    *reinterpret_cast<uint4 *>(row + ((i ^ (r & 7)) << 4)) = make_uint4(high[0], high[1], high[2], high[3]);
+                    if (HD == 128) *reinterpret_cast<uint4 *>(row + PC_QBOX + ((i ^ (r & 7)) << 4)) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+                    else *reinterpret_cast<uint4 *>(row + (((i + 4) ^ (r & 7)) << 4)) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
                 }
                 return;
             }
@@ -635,7 +672,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 #pragma unroll
                         for (int b = 0; b < S::BOXES; ++b)
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4 *>(ring + (2 * slot + 1) * S::TILE + b * PC_BOX + r * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4 *>(ring + slot * S::SLOT + S::KTILE + b * PC_BOX + r * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                     __syncwarp();   // and the products wait for all four warps
                 }
@@ -644,7 +681,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 auto before = [&] { if (j > 0) warp_wait(&sh.odone[g], (scored - 1) & 1, failed); };
                 const bool edge = at + PC_KEYS - 1 > least || at + PC_KEYS > hi || (g + 1) * PC_Q > rows || (WIN && at < late && at + PC_KEYS > a.plan.sinks);
                 if constexpr (E8) {
-                    const float (*scales)[PC_KEYS / PC_ROWS] = sh.scales[(slot0 + j) % (S::SLOTS + S::RAWS)];
+                    const PcScales &scales = sh.scales[(slot0 + j) % S::SLOTS];
                     if (edge) pc_softmax_codes<HD, true, WIN>(s_addr, o_addr, row_sl, flip, lim, WIN ? a.plan.sinks - at : 0, low, scales, j > 0, top, sum, vref, &sh.sfree[g], &sh.pfull[g], before);
                     else pc_softmax_codes<HD, false, WIN>(s_addr, o_addr, row_sl, flip, lim, 0, 0, scales, j > 0, top, sum, vref, &sh.sfree[g], &sh.pfull[g], before);
                 } else if (edge)
@@ -778,7 +815,10 @@ int launch_tc(PagedAttnArgs a, void *workspace, size_t bytes, cudaStream_t s) {
         configured[dev] = true;
     }
     CUtensorMap kmap = {}, vmap = {};
-    if (!E8) {
+    if (E8) {
+        const int rc = make_byte_mats_map(&kmap, a.k, a.plan.p.pages * a.plan.p.kv_heads, 1 << a.plan.p.page_shift, HD, PC_ROWS);
+        if (rc != AB2_OK) return rc;
+    } else {
         int rc = pages_map(&kmap, a.k, a.plan.p, HD);
         if (rc == AB2_OK) rc = pages_map(&vmap, a.v, a.plan.p, HD);
         if (rc != AB2_OK) return rc;

@@ -60,6 +60,11 @@ __device__ __forceinline__ float2 floats_of_codes(uint32_t two) {
     const uint32_t h = f16x2_of_codes(two);
     return __half22float2(*reinterpret_cast<const __half2 *>(&h));
 }
+__device__ __forceinline__ uint32_t codes_of(float lo, float hi) {   // the nearest, up to 448
+    uint16_t d;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(d) : "f"(hi), "f"(lo));
+    return d;
+}
 // 16 bytes of a row of keys or values as floats, to be scaled where they are codes.
 template <typename P> struct PagedChunk {   // bf16: 8 elements
     static constexpr int N = 8;

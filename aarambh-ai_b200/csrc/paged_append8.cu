@@ -57,11 +57,6 @@ template <> struct Two<float> {
     __device__ __forceinline__ void store(float *p) const { *reinterpret_cast<float2 *>(p) = f; }
     __device__ __forceinline__ void store(float *p, float *r) const { *p = f.x; *r = f.y; }
 };
-__device__ __forceinline__ uint32_t codes_of(float lo, float hi) {
-    uint16_t d;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(d) : "f"(hi), "f"(lo));
-    return d;
-}
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 // HALF: pairs (i, i + n); WIDE: two elements of a lane lie side by side on their boundary, else they are taken one by one.

@@ -60,7 +60,8 @@ class LongBatch(Batch):
 
     def expected(self):
         """As ``Batch.expected``, but for what hides keys.  Over codes a score is multiplied by three factors more (2^-24 each, beside a product of dim terms), and queries of bf16 as f16
-        of a power of two of the row's own lose 2^-39 of its largest element at most."""
+        of a power of two of the row's own lose 2^-39 of its largest element at most; those of chunks, in two e4m3 terms of which the largest
+        is at least 224 and the least step 2^-9, lose 2^-10 / 224 < 2^-17.8 of it in each product, twice in a weight and twice in a quotient.  A weight as f16 (2^-11) is within bf16's 2^-8."""
         group = self.heads // self.kv_heads
         refs, tols = [], []
         for r, (n, m) in enumerate(zip(self.lens, self.new)):
@@ -83,6 +84,9 @@ class LongBatch(Batch):
             off = 2 * (2 * (self.dim + 8) * 2.0 ** -24 * mag.masked_fill(hidden, 0.0).amax(-1) + 2.0 ** -20 + (n + 8) * 2.0 ** -24)
             if self.dtype == torch.bfloat16:
                 off = off + 2.0 ** -8
+                if self.scales is not None:
+                    lost = 2.0 ** -17.8 * abs(self.scale) * q.abs().amax(-1).T[:, :, None] * kz.abs().sum(-1).T[:, None, :]
+                    off = off + 4 * lost.masked_fill(hidden, 0.0).amax(-1)
             refs.append(ref)
             tols.append(off.transpose(0, 1)[..., None] * spread + ref.abs() * STEP[self.dtype] * 1.01 + 1e-30)
         return torch.cat(refs), torch.cat(tols)
