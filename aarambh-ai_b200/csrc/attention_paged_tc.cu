@@ -43,19 +43,20 @@ using namespace ab2::tc;
 namespace ab2 {
 namespace {
 
-constexpr int PC_Q = 128, PC_KEYS = 80, PC_THREADS = 384, PC_LOAD = 128;   // threads; those that load codes
+constexpr int PC_Q = 128, PC_KEYS = 80, PC_THREADS = 384, PC_LOAD = 128;   // threads; those that make codes values
 constexpr int PC_QBOX = PC_Q * 128, PC_BOX = PC_KEYS * 128;   // boxes of queries, and of keys or values: rows of 64 elements
 constexpr int PC_ROWS = 16;   // that one copy brings: the least that a page holds
 constexpr int PC_TWICE = 16;  // query rows of an item up to which it has each of them twice, for both terms of its weights
-constexpr int PC_FEW_REGS = 72, PC_LOAD_REGS = 104, PC_MANY_REGS = 168;   // over codes, of a thread of copies and issue, of loads, and of softmax: 128 of either of the first, and 256, are the 512 of 128 of the launch
+constexpr int PC_FEW_REGS = 80, PC_LOAD_REGS = 48, PC_MANY_REGS = 192;   // over codes, of a thread of copies and issue, of those that make values, and of softmax: 128 of either of the first, and 256, are the 512 of 128 of the launch
 constexpr float PC_SLACK = 8.f;  // powers of two a score may exceed the row's maximum by
 constexpr float PC_NONE = -1e30f;
 
 template <int HD, bool E8 = false> struct PcShape {
     static constexpr int THREADS = PC_THREADS + (E8 ? PC_LOAD : 0);
     static constexpr int BOXES = HD / 64, QTILE = BOXES * PC_QBOX, VTILE = BOXES * PC_BOX, KTILE = E8 ? PC_KEYS * HD : VTILE;   // bytes of a tile: queries (over codes two terms of 8 bits), values, keys
-    static constexpr int SLOTS = HD == 128 ? (E8 ? 5 : 4) : 8, SLOT = KTILE + VTILE;   // a slot holds a tile's keys and its values
-    static constexpr int SMEM = 1024 + 2 * QTILE + SLOTS * SLOT;
+    static constexpr int SLOTS = HD == 128 ? 4 : 8, SLOT = KTILE + VTILE;   // a slot holds a tile's keys and its values
+    static constexpr int RAWS = E8 ? 2 : 0, RAW = E8 ? PC_KEYS * HD : 0;             // codes of values as they come
+    static constexpr int SMEM = 1024 + 2 * QTILE + SLOTS * SLOT + RAWS * RAW;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -109,11 +110,15 @@ template <bool WIN> __device__ __forceinline__ bool pc_next(const PagedPlan &a, 
     return true;
 }
 
-struct PcScales {
-    float k[PC_KEYS / PC_ROWS], v;   // of the blocks of keys, and the unit of the values
+struct PcTile {   // of codes
+    float k[PC_KEYS / PC_ROWS], v;    // scales of the blocks of keys, and the unit of the values
+    __half2 f[PC_KEYS / PC_ROWS];     // scales of the blocks of values in that unit
+    int rows;                         // that the piece has of it; negative: there is no more tile
+    uint32_t blocks;                  // a bit for each that a token sees
 };
-template <int SLOTS, int THREADS> struct PcShared {
-    uint64_t full[SLOTS], empty[SLOTS], qfull[2], sfull[2], sfree[2], pfull[2], odone[2];
+template <int SLOTS, int RAWS, int THREADS> struct PcShared {
+    static constexpr int TILES = RAWS ? SLOTS + RAWS : 1;   // on their way or in use
+    uint64_t full[SLOTS], empty[SLOTS], qfull[2], sfull[2], sfree[2], pfull[2], odone[2], rfull[RAWS ? RAWS : 1], rempty[RAWS ? RAWS : 1];
     uint32_t tmem_base;
     int failed;
     union {
@@ -123,7 +128,7 @@ template <int SLOTS, int THREADS> struct PcShared {
         };
         struct {
             PagedRun start;                     // that run, over the sums alone: other threads may still read what was found
-            PcScales scales[THREADS > PC_THREADS ? SLOTS : 1];   // of a slot's codes; behind a barrier of all
+            PcTile tiles[TILES];                // behind a barrier of all
         };
     };
     // of every softmax warp: its run, the piece that it is at and the next one (kept from its registers, which the scores fill)
@@ -245,7 +250,7 @@ __device__ __forceinline__ void exchange4(uint4 (&o)[4], int lane) {
 // the sums of all its rows become NaN, and they are computed again in f32 like those that meet NaN.
 constexpr float PC_UP = 128.f, PC_LESS = 9.765625e-4f, PC_APART = 3.0517578e-5f, PC_NOTHING = 8.6736174e-19f, PC_ZEROS = 7.8886091e-31f;   // 2^7, 2^-10, 2^-15, 2^-60, 2^-100
 template <int HD, bool EDGE, bool WIN, class Before>
-__device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, int sinks, int since, const PcScales &of, bool has_o, float &top, float &sum, float &vref,
+__device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, int sinks, int since, const PcTile &of, bool has_o, float &top, float &sum, float &vref,
                                                  uint64_t *taken, uint64_t *ready, Before before) {
     constexpr int BLOCKS = PC_KEYS / PC_ROWS;
     uint32_t va[32], vb[32], vc[16];
@@ -344,7 +349,7 @@ __device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_add
     if ((threadIdx.x & 31) == 0) bar_arrive(ready);
 }
 
-// E8: pages of e4m3.  Keys come by the same copies; four more warps load values, a tile ahead, and make them f16 in the ring's slots.
+// E8: pages of e4m3.  Keys come by the same copies; four more warps make values, which come as codes, f16 in the ring's slots.
 // WIN: a window.
 template <int HD, bool E8, bool WIN>
 __global__ void __launch_bounds__(PcShape<HD, E8>::THREADS, 1)
@@ -352,14 +357,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     using S = PcShape<HD, E8>;
     using Page = std::conditional_t<E8, uint8_t, __nv_bfloat16>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ PcShared<S::SLOTS, S::THREADS> sh;
+    __shared__ PcShared<S::SLOTS, S::RAWS, S::THREADS> sh;
+    constexpr int RAWS = S::RAWS ? S::RAWS : 1, TILES = sh.TILES;
     static_assert(S::SMEM + sizeof(sh) <= 227 * 1024, "shared memory of a CTA");
     static_assert(sizeof(PagedRun) <= S::THREADS / 32 * sizeof(long long), "the run lies over the sums");
-    uint8_t *qbuf = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023), *ring = qbuf + 2 * S::QTILE;
+    uint8_t *qbuf = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023), *ring = qbuf + 2 * S::QTILE, *codes = ring + S::SLOTS * S::SLOT;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *failed = &sh.failed;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::SLOTS; ++i) { bar_init(&sh.full[i], 1 + (E8 ? PC_LOAD / 64 : 0)); bar_init(&sh.empty[i], 2); }
+        for (int i = 0; i < S::SLOTS; ++i) { bar_init(&sh.full[i], 1 + (E8 ? PC_LOAD / 32 : 0)); bar_init(&sh.empty[i], 2); }
+        for (int i = 0; i < S::RAWS; ++i) { bar_init(&sh.rfull[i], 1); bar_init(&sh.rempty[i], PC_LOAD / 32); }
         for (int i = 0; i < 2; ++i) { bar_init(&sh.qfull[i], 4); bar_init(&sh.sfull[i], 1); bar_init(&sh.sfree[i], 4); bar_init(&sh.pfull[i], 4); bar_init(&sh.odone[i], 1); }
         sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -383,70 +390,28 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     if (E8 && warp >= PC_THREADS / 32) {
         // ---------------------------------------------------------- values from codes
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PC_LOAD_REGS));
-        // Either half of these warps has every other tile, so that two tiles' loads are on their way.  Piece i of a tile is 16 codes of row i / CH; a thread has pieces me, me + 64, ...
-        constexpr int CH = HD / 16, HALF = PC_LOAD / 2, MINE = PC_KEYS * CH / HALF, BLOCKS = PC_KEYS / PC_ROWS;
-        static_assert(PC_KEYS * CH % HALF == 0, "a tile's pieces");
-        const int half = (warp - PC_THREADS / 32) / (HALF / 32), me = (threadIdx.x - PC_THREADS) % HALF, row0 = me / CH, ch = me % CH;
-        constexpr int ROWS = HALF / CH;   // from a piece to the next
-        uint4 vc[MINE];
-        long long at = -1;            // lane b: where block b of the tile to load begins, in rows of a head; -1: nothing of it is in sight
-        float ks = 0.f, vs = 0.f;     // its scales
-        int j = -1, n = -1, hi = 0, key0 = 0;   // n: the tile to load, of all
-        bool more;
-        auto seek = [&]() {   // this half's next tile, and its blocks
-            more = true;
-            do {
-                ++n;
-                for (++j; j >= x.most(); j = 0)
-                    if (!pc_next<WIN>(a.plan, run, x)) { more = false; return; }
-            } while ((n & 1) != half);
-            const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
-            key0 = x.s.lo + j * PC_KEYS;
-            hi = x.s.hi;
-            const int v = key0 + lane * PC_ROWS, key = WIN ? paged_key(hole, v) : v;
-            const bool in = lane < BLOCKS && v < hi && !(WIN && paged_hidden(a.plan, x.s, key, PC_ROWS));
-            at = in ? (((long long)paged_page(p, x.w.row, key, a.status) * p.kv_heads + x.w.head) << p.page_shift) + (key & ((1 << p.page_shift) - 1)) : -1;
-        };
-        auto load = [&]() {
-            ks = at >= 0 ? __ldg(a.k_scales + at / PAGED_BLOCK) : 0.f;
-            vs = at >= 0 ? __ldg(a.v_scales + at / PAGED_BLOCK) : 0.f;
-#pragma unroll
-            for (int u = 0; u < MINE; ++u) {
-                const int r = row0 + u * ROWS;
-                const long long from = __shfl_sync(0xffffffffu, at, r / PC_ROWS);
-                vc[u] = make_uint4(0u, 0u, 0u, 0u);
-                if (from < 0 || key0 + r >= hi) continue;   // zeros, behind the keys too
-                vc[u] = __ldg(reinterpret_cast<const uint4 *>((const uint8_t *)a.v + (size_t)(from + r % PC_ROWS) * HD + ch * 16));
-            }
-        };
-        x.first = x.second = 0;
-        seek();
-        if (more) load();
-        while (more) {
-            // the unit of the tile's values, and its blocks' scales in it
-            float unit = vs;
-#pragma unroll
-            for (int m = 1; m < 8; m <<= 1) unit = fmaxf(unit, __shfl_xor_sync(0xffffffffu, unit, m));
-            const __half2 f = __float2half2_rn(unit > 0.f ? vs / unit : 0.f);
-            if (__any_sync(0xffffffffu, lane < BLOCKS && vs < unit * PC_APART && vs > PC_ZEROS)) unit = __uint_as_float(0x7fc00000u);
-            const float kscale = ks;
-            const int slot = n % S::SLOTS, phase = ((n / S::SLOTS) & 1) ^ 1;
-            seek();   // the table's entries are on their way
-            warp_wait(&sh.empty[slot], phase, failed);
-            if (me < 32) {
-                if (lane < BLOCKS) sh.scales[slot].k[lane] = kscale;
-                if (lane == 0) sh.scales[slot].v = unit;
-            }
-#pragma unroll
-            for (int u = 0; u < MINE; ++u) {
-                const int r = row0 + u * ROWS;
-                const uint32_t fb = __shfl_sync(0xffffffffu, *reinterpret_cast<const uint32_t *>(&f), r / PC_ROWS);
+        // A short loop: unrolled, its text drives that of the softmax out of the instruction cache (4096 behind 12288, values by registers a tile ahead, 1150 us).
+        constexpr int CH = HD / 16;   // pieces of 16 codes of a row
+        for (int n = 0;; ++n) {
+            const int slot = n % S::SLOTS, raw = n % RAWS;
+            warp_wait(&sh.rfull[raw], (n / RAWS) & 1, failed);
+            const PcTile &tile = sh.tiles[n % TILES];
+            const int rows = tile.rows;
+            if (rows < 0 || *failed) break;
+            const uint32_t blocks = tile.blocks;
+            warp_wait(&sh.empty[slot], ((n / S::SLOTS) & 1) ^ 1, failed);
+#pragma unroll 1
+            for (int i = threadIdx.x - PC_THREADS; i < PC_KEYS * CH; i += PC_LOAD) {
+                const int r = i / CH, ch = i % CH;
+                const __half2 f = tile.f[r / PC_ROWS];
+                uint4 c = make_uint4(0u, 0u, 0u, 0u);   // behind the piece's keys, and where no token sees a block
+                if (r < rows && ((blocks >> (r / PC_ROWS)) & 1)) c = *reinterpret_cast<const uint4 *>(codes + raw * S::RAW + i * 16);
                 auto two = [&](uint32_t codes) {
                     const uint32_t h = f16x2_of_codes(codes);
-                    const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&h), *reinterpret_cast<const __half2 *>(&fb));
+                    const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&h), f);
                     return *reinterpret_cast<const uint32_t *>(&y);
                 };
-                const uint4 c = vc[u], low8 = make_uint4(two(c.x), two(c.x >> 16), two(c.y), two(c.y >> 16)), high8 = make_uint4(two(c.z), two(c.z >> 16), two(c.w), two(c.w >> 16));
+                const uint4 low8 = make_uint4(two(c.x), two(c.x >> 16), two(c.y), two(c.y >> 16)), high8 = make_uint4(two(c.z), two(c.z >> 16), two(c.w), two(c.w >> 16));
                 // 16 codes are two chunks of the row in its box of 64 elements; those of the second box go in the other order, so that eight lanes meet in no bank
                 uint8_t *row = ring + slot * S::SLOT + S::KTILE + (ch >> 2) * PC_BOX + r * 128;
                 const int c0 = 2 * (ch & 3), odd = (ch >> 2) & 1;
@@ -454,15 +419,55 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 *reinterpret_cast<uint4 *>(row + (((c0 + 1 - odd) ^ (r & 7)) << 4)) = odd ? low8 : high8;
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            __syncwarp();
-            if (lane == 0) bar_arrive(&sh.full[slot]);
-            if (more) load();
+            __syncwarp();   // every lane's codes have been read, as what it stored is made of them
+            if (lane == 0) {
+                bar_arrive(&sh.full[slot]);
+                bar_arrive(&sh.rempty[raw]);
+            }
         }
     } else if (warp < 4) {
         if (E8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PC_FEW_REGS));
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
-        if (warp == 0) {
-            // ---------------------------------------------------------- TMA producer: K, V, K, V, ...; over codes K alone
+        if (E8 && warp == 0) {
+            // ---------------------------------------------------------- producer over codes: V, as codes, then K
+            int n = 0;
+            while (pc_next<WIN>(a.plan, run, x)) {
+                const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
+                for (int j = 0; j < x.most(); ++j, ++n) {
+                    const int v = x.s.lo + j * PC_KEYS + lane * PC_ROWS, key = WIN ? paged_key(hole, v) : v, raw = n % RAWS, slot = n % S::SLOTS;
+                    const bool mine = lane < PC_KEYS / PC_ROWS && v < x.s.hi && !(WIN && paged_hidden(a.plan, x.s, key, PC_ROWS));
+                    const int page = mine ? paged_page(p, x.w.row, key, a.status) : 0, at = key & ((1 << p.page_shift) - 1);
+                    const size_t row = mine ? (((size_t)page * p.kv_heads + x.w.head) << p.page_shift) + at : 0;
+                    const float ks = mine ? __ldg(a.k_scales + row / PAGED_BLOCK) : 0.f, vs = mine ? __ldg(a.v_scales + row / PAGED_BLOCK) : 0.f;
+                    const uint32_t blocks = __ballot_sync(0xffffffffu, mine);
+                    const int bytes = __popc(blocks) * PC_ROWS * HD;
+                    float unit = vs;
+#pragma unroll
+                    for (int m = 1; m < 8; m <<= 1) unit = fmaxf(unit, __shfl_xor_sync(0xffffffffu, unit, m));
+                    const __half2 f = __float2half2_rn(unit > 0.f ? vs / unit : 0.f);
+                    if (__any_sync(0xffffffffu, lane < 8 && vs < unit * PC_APART && vs > PC_ZEROS)) unit = __uint_as_float(0x7fc00000u);
+                    warp_wait(&sh.rempty[raw], ((n / RAWS) & 1) ^ 1, failed);
+                    PcTile &tile = sh.tiles[n % TILES];
+                    if (lane < PC_KEYS / PC_ROWS) { tile.k[lane] = ks; tile.f[lane] = f; }
+                    if (lane == 0) { tile.v = unit; tile.rows = x.s.hi - (x.s.lo + j * PC_KEYS); tile.blocks = blocks; }
+                    __syncwarp();
+                    if (lane == 0) bar_expect_tx(&sh.rfull[raw], (uint32_t)bytes);
+                    __syncwarp();
+                    if (mine && !*failed) bulk_copy(codes + raw * S::RAW + lane * PC_ROWS * HD, (const uint8_t *)a.v + row * HD, PC_ROWS * HD, &sh.rfull[raw]);
+                    warp_wait(&sh.empty[slot], ((n / S::SLOTS) & 1) ^ 1, failed);
+                    if (lane == 0) bar_expect_tx(&sh.full[slot], (uint32_t)bytes);
+                    __syncwarp();
+                    // (of blocks that are not copied the slot holds what it held: their scores are hidden, whatever they are)
+                    if (mine && !*failed) tma_load_3d(ring + slot * S::SLOT + lane * PC_ROWS * HD, &kmap, 0, at, page * p.kv_heads + x.w.head, &sh.full[slot]);
+                }
+            }
+            warp_wait(&sh.rempty[n % RAWS], ((n / RAWS) & 1) ^ 1, failed);
+            if (lane == 0) {
+                sh.tiles[n % TILES].rows = -1;
+                bar_arrive(&sh.rfull[n % RAWS]);
+            }
+        } else if (warp == 0) {
+            // ---------------------------------------------------------- TMA producer: K, V, K, V, ...
             int n = 0;
             while (pc_next<WIN>(a.plan, run, x)) {
                 const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
@@ -471,17 +476,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     const bool mine = lane < PC_KEYS / PC_ROWS && v < x.s.hi;
                     // a block that no token sees comes from behind the pool, as zeros
                     const int page = !mine ? 0 : WIN && paged_hidden(a.plan, x.s, key, PC_ROWS) ? p.pages : paged_page(p, x.w.row, key, a.status);
-                    const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * PC_ROWS * HD * (E8 ? 1 : 4);
+                    const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * PC_ROWS * HD * 4;
                     const int slot = n % S::SLOTS;
                     warp_wait(&sh.empty[slot], ((n++ / S::SLOTS) & 1) ^ 1, failed);
                     // The first queries come before what is fetched ahead.  Only at the second slot of the run's first piece with keys, and only where the first
                     // tile of rows looks at it: its warps cannot announce their next queries without that slot, so the barrier is in its first phase or just
                     // behind it.  A later phase would have this parity again, and might wait for what is not yet fetched.
-                    if (!E8 && n == 2 && j == 1 && x.first > 1) warp_wait(&sh.qfull[0], 0, failed);
+                    if (n == 2 && j == 1 && x.first > 1) warp_wait(&sh.qfull[0], 0, failed);
                     if (lane == 0) bar_expect_tx(&sh.full[slot], (uint32_t)bytes);
                     __syncwarp();
-                    if (E8 && mine && !*failed) tma_load_3d(ring + slot * S::SLOT + lane * PC_ROWS * HD, &kmap, 0, key & ((1 << p.page_shift) - 1), page * p.kv_heads + x.w.head, &sh.full[slot]);
-                    if (!E8 && mine && !*failed)
+                    if (mine && !*failed)
 #pragma unroll
                         for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
@@ -681,9 +685,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 auto before = [&] { if (j > 0) warp_wait(&sh.odone[g], (scored - 1) & 1, failed); };
                 const bool edge = at + PC_KEYS - 1 > least || at + PC_KEYS > hi || (g + 1) * PC_Q > rows || (WIN && at < late && at + PC_KEYS > a.plan.sinks);
                 if constexpr (E8) {
-                    const PcScales &scales = sh.scales[(slot0 + j) % S::SLOTS];
-                    if (edge) pc_softmax_codes<HD, true, WIN>(s_addr, o_addr, row_sl, flip, lim, WIN ? a.plan.sinks - at : 0, low, scales, j > 0, top, sum, vref, &sh.sfree[g], &sh.pfull[g], before);
-                    else pc_softmax_codes<HD, false, WIN>(s_addr, o_addr, row_sl, flip, lim, 0, 0, scales, j > 0, top, sum, vref, &sh.sfree[g], &sh.pfull[g], before);
+                    const PcTile &tile = sh.tiles[(slot0 + j) % TILES];
+                    if (edge) pc_softmax_codes<HD, true, WIN>(s_addr, o_addr, row_sl, flip, lim, WIN ? a.plan.sinks - at : 0, low, tile, j > 0, top, sum, vref, &sh.sfree[g], &sh.pfull[g], before);
+                    else pc_softmax_codes<HD, false, WIN>(s_addr, o_addr, row_sl, flip, lim, 0, 0, tile, j > 0, top, sum, vref, &sh.sfree[g], &sh.pfull[g], before);
                 } else if (edge)
                     pc_softmax<HD, true, WIN>(s_addr, o_addr, sl, flip, lim, WIN ? a.plan.sinks - at : 0, low, second, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
                 else pc_softmax<HD, false, WIN>(s_addr, o_addr, sl, flip, lim, 0, 0, false, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);

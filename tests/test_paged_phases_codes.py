@@ -1,5 +1,5 @@
-"""The barriers of the tensor-memory kernel over pages of 8 bits, restated: the warps that load codes and make them f16 in the ring's slots, and the issue of the
-products and the softmax of two tiles of rows as over bf16 (``test_paged_phases``)."""
+"""The barriers of the tensor-memory kernel over pages of 8 bits, restated: a producer of codes (values, then keys), the warps that make values f16 in the ring's slots, and
+the issue of the products and the softmax of two tiles of rows as over bf16 (``test_paged_phases``)."""
 import itertools
 import random
 
@@ -7,18 +7,30 @@ import pytest
 
 from test_paged_phases import LISTS, Barrier, WrongPhase
 
-WARPS = 2   # of a tile: two have every other one
+WARPS = 4
 
 
-def roles(pieces, slots):
+def roles(pieces, slots, raws):
     full, empty = [Barrier(1 + WARPS) for _ in range(slots)], [Barrier(2) for _ in range(slots)]
+    rfull, rempty = [Barrier(1) for _ in range(raws)], [Barrier(WARPS) for _ in range(raws)]
     qfull, sfull, sfree, pfull, odone = ([Barrier(1), Barrier(1)] for _ in range(5))
     tiles = sum(max(p) for p in pieces)
 
-    def loads(first, step):   # of keys: all tiles; of values: every other one
-        for n in range(first, tiles, step):
-            yield empty[n % slots], n // slots - 1
-            full[n % slots].arrive()
+    def producer():
+        for n in range(tiles + 1):   # the last is the end
+            yield rempty[n % raws], n // raws - 1
+            rfull[n % raws].arrive()
+            if n < tiles:
+                yield empty[n % slots], n // slots - 1
+                full[n % slots].arrive()
+
+    def values():
+        for n in range(tiles + 1):
+            yield rfull[n % raws], n // raws
+            if n < tiles:
+                yield empty[n % slots], n // slots - 1
+                full[n % slots].arrive()
+                rempty[n % raws].arrive()
 
     def products(g):
         n = scored = done = asked = 0
@@ -62,11 +74,11 @@ def roles(pieces, slots):
             if piece[g]:
                 yield odone[g], scored - 1
 
-    return [loads(0, 1), *(loads(i // WARPS, 2) for i in range(2 * WARPS)), products(0), products(1), softmax(0), softmax(1)]
+    return [producer(), *(values() for _ in range(WARPS)), products(0), products(1), softmax(0), softmax(1)]
 
 
-def comes_to_an_end(pieces, slots, pick):
-    live = {i: (r, None) for i, r in enumerate(roles(pieces, slots))}
+def comes_to_an_end(pieces, slots, raws, pick):
+    live = {i: (r, None) for i, r in enumerate(roles(pieces, slots, raws))}
     while live:
         ready = [i for i, (_, w) in live.items() if w is None or w[0].passed(w[1])]
         if not ready:
@@ -81,16 +93,16 @@ def comes_to_an_end(pieces, slots, pick):
     return True
 
 
-@pytest.mark.parametrize("slots", [4, 5, 8])
-def test_every_order_of_the_roles_ends(slots):
+@pytest.mark.parametrize("slots,raws", [(4, 2), (8, 2), (3, 3)])
+def test_every_order_of_the_roles_ends(slots, raws):
     rng = random.Random(7)
     orders = list(itertools.permutations(range(9)))
     for pieces in LISTS:
         for order in rng.sample(orders, 40):   # each role as far as it can go before the next one
-            assert comes_to_an_end(pieces, slots, lambda ready: min(ready, key=order.index)), (pieces, order)
+            assert comes_to_an_end(pieces, slots, raws, lambda ready: min(ready, key=order.index)), (pieces, order)
     for _ in range(300):
         pieces = []
         for _ in range(rng.randint(1, 9)):
             second = rng.choice([0, 1, 1, 2, 3, 9])
             pieces.append((max(0, second - rng.choice([0, 0, 1])) if second else rng.choice([0, 1, 1, 2, 6]), second))
-        assert comes_to_an_end(pieces, slots, rng.choice)
+        assert comes_to_an_end(pieces, slots, raws, rng.choice)
