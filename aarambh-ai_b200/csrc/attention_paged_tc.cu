@@ -246,22 +246,26 @@ __device__ __forceinline__ void exchange4(uint4 (&o)[4], int lane) {
 // Over codes keys are multiplied as they are, with queries in two e4m3 terms: a bf16 number has 8 significant bits, and is the sum of two of 4 (in units of a power of two of
 // its row's that puts the largest at 224 to 448; below 2^-2 the second term has fewer: 2^-18 of the row's largest element off at most).  A block's scale multiplies its scores beside the
 // softmax's factor.  Values are f16, in units of the tile's largest scale (a block's other scale is a power of two below it, and exact down to 2^-15); their weights are f16 in units of `vref`, a
-// scale of values that moves as the maximum does: up to any larger one, down where f16 would lose bits of them.  A tile whose scales of values lie too far apart has NaN for its unit:
+// scale of values that moves as the maximum does: up to one over 4 times it (2^8 of a weight, 4 and PC_UP make 2^15), down where f16 would lose bits of them.  A tile whose scales of values lie too far apart has NaN for its unit:
 // the sums of all its rows become NaN, and they are computed again in f32 like those that meet NaN.
-constexpr float PC_UP = 128.f, PC_LESS = 9.765625e-4f, PC_APART = 3.0517578e-5f, PC_NOTHING = 8.6736174e-19f, PC_ZEROS = 7.8886091e-31f;   // 2^7, 2^-10, 2^-15, 2^-60, 2^-100
+constexpr float PC_UP = 32.f, PC_MORE = 4.f, PC_LESS = 9.765625e-4f, PC_APART = 3.0517578e-5f, PC_NOTHING = 8.6736174e-19f, PC_ZEROS = 7.8886091e-31f;   // 2^-10, 2^-15, 2^-60, 2^-100
+// What a row's warp keeps of the values' scales: the unit of the sums, and of the tile before its scale, what that adds to a weight's exponent, and its inverse as a factor.
+struct PcUnit {
+    float vref, last, more, less;
+};
 template <int HD, bool EDGE, bool WIN, class Before>
-__device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, int sinks, int since, const PcTile &of, bool has_o, float &top, float &sum, float &vref,
+__device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, int sinks, int since, const PcTile &of, bool has_o, float &top, float &sum, PcUnit &unit,
                                                  uint64_t *taken, uint64_t *ready, Before before) {
     constexpr int BLOCKS = PC_KEYS / PC_ROWS;
     uint32_t va[32], vb[32], vc[16];
     tmem_ld32_start(va, s_addr);
     tmem_ld32_start(vb, s_addr + 32);
     tmem_ld16_start(vc, s_addr + 64);
-    float scale[BLOCKS], unit = vref;
+    float scale[BLOCKS], vref = unit.vref;
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) scale[b] = fmaxf(sl * of.k[b], 1.17549435e-38f);   // above 0, so that hidden scores stay -inf
     const float values = of.v;
-    if (values > vref || (values < vref * PC_LESS && values > vref * PC_NOTHING)) unit = fmaxf(values, 3.0092655e-36f);
+    if (values > vref * PC_MORE || (values < vref * PC_LESS && values > vref * PC_NOTHING)) vref = fmaxf(values, 3.0092655e-36f);
     tmem_ld16_wait(vc);
     tmem_ld32_wait(va);
     tmem_ld32_wait(vb);
@@ -300,11 +304,10 @@ __device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_add
     }
     const float now = best > top + PC_SLACK ? best : top;
     before();
-    if (__any_sync(0xffffffffu, now != top || unit != vref)) {
-        const float keep = ex2(top - now), corr = unit == vref ? keep : keep * (vref / unit);
+    if (__any_sync(0xffffffffu, now != top || vref != unit.vref)) {
+        const float keep = ex2(top - now), corr = vref == unit.vref ? keep : keep * (unit.vref / vref);
         sum *= keep;
         top = now;
-        vref = unit;
         if (has_o) {
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 #pragma unroll 1
@@ -317,8 +320,15 @@ __device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_add
             }
         }
     }
-    // the tile's values in units of vref, 2^7 larger; 2^-40 and less makes weights of nothing (and their sum is still theirs)
-    const float f = vref > 0.f ? fmaxf(values / vref * PC_UP, 9.0949470e-13f) : PC_UP, shifted = __log2f(f) - top;
+    // The tile's values in units of vref, PC_UP times as large; 2^-40 and less makes weights of nothing (and their sum is still theirs).
+    if (values != unit.last || vref != unit.vref) {   // the same for all lanes
+        const float f = vref > 0.f ? fmaxf(values / vref * PC_UP, 9.0949470e-13f) : PC_UP;
+        unit.last = values;
+        unit.vref = vref;
+        unit.more = __log2f(f);
+        unit.less = 1.f / f;
+    }
+    const float shifted = unit.more - top;
     const uint64_t top2 = pair(shifted, shifted);
     uint64_t total[2] = {0ull, 0ull};
     auto weights = [&](int k) {   // of keys k and k + 1
@@ -341,7 +351,7 @@ __device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_add
         tmem_st8(s_addr + PC_KEYS + 32, p);
     }
     total[0] = add2(total[0], total[1]);
-    sum = fmaf(low(total[0]) + high(total[0]), 1.f / f, sum);
+    sum = fmaf(low(total[0]) + high(total[0]), unit.less, sum);
     if (values != values) sum = values;
     asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -391,7 +401,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         // ---------------------------------------------------------- values from codes
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PC_LOAD_REGS));
         // A short loop: unrolled, its text drives that of the softmax out of the instruction cache (4096 behind 12288, values by registers a tile ahead, 1150 us).
-        constexpr int CH = HD / 16;   // pieces of 16 codes of a row
+        // A thread has 16 codes of every ROWS-th row: two chunks of the row in its box of 64 elements; those of the second box go in the other order, so that eight lanes
+        // meet in no bank.
+        constexpr int CH = HD / 16, ROWS = PC_LOAD / CH;
+        const int me = threadIdx.x - PC_THREADS, row0 = me / CH, ch = me % CH, odd = (ch >> 2) & 1, c0 = 2 * (ch & 3) + odd;
+        const uint8_t *from = codes + row0 * HD + ch * 16;
+        uint8_t *to0 = ring + S::KTILE + (ch >> 2) * PC_BOX + row0 * 128 + ((c0 ^ (row0 & 7)) << 4), *to1 = to0 + ((((c0 ^ 1) ^ (row0 & 7)) << 4) - ((c0 ^ (row0 & 7)) << 4));
         for (int n = 0;; ++n) {
             const int slot = n % S::SLOTS, raw = n % RAWS;
             warp_wait(&sh.rfull[raw], (n / RAWS) & 1, failed);
@@ -401,22 +416,18 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const uint32_t blocks = tile.blocks;
             warp_wait(&sh.empty[slot], ((n / S::SLOTS) & 1) ^ 1, failed);
 #pragma unroll 1
-            for (int i = threadIdx.x - PC_THREADS; i < PC_KEYS * CH; i += PC_LOAD) {
-                const int r = i / CH, ch = i % CH;
+            for (int r = row0; r < PC_KEYS; r += ROWS) {
                 const __half2 f = tile.f[r / PC_ROWS];
                 uint4 c = make_uint4(0u, 0u, 0u, 0u);   // behind the piece's keys, and where no token sees a block
-                if (r < rows && ((blocks >> (r / PC_ROWS)) & 1)) c = *reinterpret_cast<const uint4 *>(codes + raw * S::RAW + i * 16);
+                if (r < rows && ((blocks >> (r / PC_ROWS)) & 1)) c = *reinterpret_cast<const uint4 *>(from + raw * S::RAW + (r - row0) * HD);
                 auto two = [&](uint32_t codes) {
                     const uint32_t h = f16x2_of_codes(codes);
                     const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&h), f);
                     return *reinterpret_cast<const uint32_t *>(&y);
                 };
                 const uint4 low8 = make_uint4(two(c.x), two(c.x >> 16), two(c.y), two(c.y >> 16)), high8 = make_uint4(two(c.z), two(c.z >> 16), two(c.w), two(c.w >> 16));
-                // 16 codes are two chunks of the row in its box of 64 elements; those of the second box go in the other order, so that eight lanes meet in no bank
-                uint8_t *row = ring + slot * S::SLOT + S::KTILE + (ch >> 2) * PC_BOX + r * 128;
-                const int c0 = 2 * (ch & 3), odd = (ch >> 2) & 1;
-                *reinterpret_cast<uint4 *>(row + (((c0 + odd) ^ (r & 7)) << 4)) = odd ? high8 : low8;
-                *reinterpret_cast<uint4 *>(row + (((c0 + 1 - odd) ^ (r & 7)) << 4)) = odd ? low8 : high8;
+                *reinterpret_cast<uint4 *>(to0 + slot * S::SLOT + (r - row0) * 128) = odd ? high8 : low8;
+                *reinterpret_cast<uint4 *>(to1 + slot * S::SLOT + (r - row0) * 128) = odd ? low8 : high8;
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();   // every lane's codes have been read, as what it stored is made of them
@@ -586,7 +597,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             return more;
         };
         // its queries, on their way to shared memory
-        float back = 1.f, vref = 0.f;   // E8: what the row's queries are to be multiplied by; the unit of its weights
+        float back = 1.f;   // E8: what the row's queries are to be multiplied by
+        PcUnit unit;
         auto fetch_q = [&]() {
             const PcPiece &x = sh.piece[warp - 4][here];
             if ((g ? x.second : x.first) == 0) return;   // nothing to ask
@@ -656,7 +668,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
             const bool twice = !E8 && rows <= PC_TWICE;   // and this the first tile of rows
             const float row_sl = E8 ? sl * back : sl;
-            vref = 0.f;
+            unit = {0.f, -1.f, 0.f, 1.f};
             const bool second = twice && (lane & PC_TWICE);
             const int rr = g * PC_Q + r, asks = twice && r < 2 * PC_TWICE ? r % PC_TWICE : rr;
             const int gap = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile).gap : 0, first = x.s.base + x.s.t0 - gap;   // all in virtual keys
@@ -686,13 +698,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 const bool edge = at + PC_KEYS - 1 > least || at + PC_KEYS > hi || (g + 1) * PC_Q > rows || (WIN && at < late && at + PC_KEYS > a.plan.sinks);
                 if constexpr (E8) {
                     const PcTile &tile = sh.tiles[(slot0 + j) % TILES];
-                    if (edge) pc_softmax_codes<HD, true, WIN>(s_addr, o_addr, row_sl, flip, lim, WIN ? a.plan.sinks - at : 0, low, tile, j > 0, top, sum, vref, &sh.sfree[g], &sh.pfull[g], before);
-                    else pc_softmax_codes<HD, false, WIN>(s_addr, o_addr, row_sl, flip, lim, 0, 0, tile, j > 0, top, sum, vref, &sh.sfree[g], &sh.pfull[g], before);
+                    if (edge) pc_softmax_codes<HD, true, WIN>(s_addr, o_addr, row_sl, flip, lim, WIN ? a.plan.sinks - at : 0, low, tile, j > 0, top, sum, unit, &sh.sfree[g], &sh.pfull[g], before);
+                    else pc_softmax_codes<HD, false, WIN>(s_addr, o_addr, row_sl, flip, lim, 0, 0, tile, j > 0, top, sum, unit, &sh.sfree[g], &sh.pfull[g], before);
                 } else if (edge)
                     pc_softmax<HD, true, WIN>(s_addr, o_addr, sl, flip, lim, WIN ? a.plan.sinks - at : 0, low, second, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
                 else pc_softmax<HD, false, WIN>(s_addr, o_addr, sl, flip, lim, 0, 0, false, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
             }
-            const float unit = E8 ? vref * (1.f / PC_UP) : 1.f;
+            const float of_sums = E8 ? unit.vref * (1.f / PC_UP) : 1.f;
             // the scores are all made: the next piece's queries may take the place of these, while the sums go out
             more = next();
             if (more) fetch_q();
@@ -702,7 +714,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             const bool all = w.k0 == 0 && w.k1 == w.k_tiles;
             const size_t slot = (2 * (size_t)blockIdx.x + (w.k0 == 0)) * a.tile_rows;
-            const float f = !all ? (E8 && sum != sum ? sum : unit) : sum == 0.f ? 0.f : unit / sum;
+            const float f = !all ? (E8 && sum != sum ? sum : of_sums) : sum == 0.f ? 0.f : of_sums / sum;
             float poison = 0.f;  // stays 0 unless an output is Inf or NaN
             // A lane has a row, 16 bytes of which at a time would go to 32 places: four lanes exchange pieces and store 64 bytes of a row each time.
             __nv_bfloat16 *dst[4];
