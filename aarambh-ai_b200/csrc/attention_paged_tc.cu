@@ -604,45 +604,14 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             if ((g ? x.second : x.first) == 0) return;   // nothing to ask
             const PagedSpan s = x.s;
             const long long first = x.w.r.first + s.t0, head0 = x.w.head * group;
-            if constexpr (E8) {   // a thread its row
-                const int rr = g * PC_Q + r, tok = paged_token(a.plan, rr);
-                const bool in = rr < s.ntok * group;
-                const uint4 *src = (const uint4 *)((const __nv_bfloat16 *)a.q + (first + (in ? tok : 0)) * a.q_stride + (head0 + (in ? rr - tok * group : 0)) * HD);
-                uint4 q[HD / 8];
-                float most = 0.f;
+            if constexpr (E8) {   // every warp its own rows, which it makes codes where they come to lie
 #pragma unroll
-                for (int i = 0; i < HD / 8; ++i) q[i] = in ? src[i] : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                for (int i = 0; i < HD / 8; ++i)
-                    for (uint32_t w : {q[i].x, q[i].y, q[i].z, q[i].w}) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u))));
-                // times 2^(127 - down) the largest is between 224 and 448 = 1.75 2^8
-                const uint32_t bits = __float_as_uint(most);
-                const int down = min(max((int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u), 1), 253);
-                const float f = most < INFINITY ? __uint_as_float((uint32_t)(254 - down) << 23) : __uint_as_float(0x7fc00000u);   // Inf has no code
-                back = __uint_as_float((uint32_t)down << 23);
-#pragma unroll
-                for (int i = 0; i < HD / 16; ++i) {
-                    uint32_t high[4], rest[4];
-                    const uint32_t words[8] = {q[2 * i].x, q[2 * i].y, q[2 * i].z, q[2 * i].w, q[2 * i + 1].x, q[2 * i + 1].y, q[2 * i + 1].z, q[2 * i + 1].w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t h[2], l[2];
-#pragma unroll
-                        for (int d = 0; d < 2; ++d) {
-                            const uint32_t w = words[2 * e + d];
-                            const float x = __uint_as_float(w << 16) * f, y = __uint_as_float(w & 0xffff0000u) * f;
-                            h[d] = codes_of(x, y);
-                            const float2 hf = floats_of_codes(h[d]);
-                            l[d] = codes_of(x - hf.x, y - hf.y);
-                        }
-                        high[e] = h[0] | h[1] << 16;
-                        rest[e] = l[0] | l[1] << 16;
-                    }
-                    uint8_t *row = qbuf + g * S::QTILE + r * 128;
-                    *reinterpret_cast<uint4 *>(row + ((i ^ (r & 7)) << 4)) = make_uint4(high[0], high[1], high[2], high[3]);
-                    if (HD == 128) *reinterpret_cast<uint4 *>(row + PC_QBOX + ((i ^ (r & 7)) << 4)) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
-                    else *reinterpret_cast<uint4 *>(row + (((i + 4) ^ (r & 7)) << 4)) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+                for (int u = 0; u < HD / 8; ++u) {
+                    const int i = lane + 32 * u, d = i % (HD / 8), row = quad * 32 + i / (HD / 8), rr = g * PC_Q + row, in = rr < s.ntok * group ? 16 : 0, tok = paged_token(a.plan, in ? rr : 0);
+                    const __nv_bfloat16 *src = (const __nv_bfloat16 *)a.q + (first + tok) * a.q_stride + (head0 + (in ? rr - tok * group : 0)) * HD + d * 8;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(sptr(qbuf + g * S::QTILE + (d >> 3) * PC_QBOX + row * 128 + (((d & 7) ^ (row & 7)) << 4))), "l"(src), "r"(in) : "memory");
                 }
+                asm volatile("cp.async.commit_group;\n" ::: "memory");
                 return;
             }
             const int i0 = threadIdx.x & 127, rows = s.ntok * group;
@@ -655,6 +624,43 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
             asm volatile("cp.async.commit_group;\n" ::: "memory");
         };
+        // E8: a thread's row of queries, from bf16 to two terms of codes in its place
+        auto terms_of_q = [&]() {
+            auto at = [&](int c) { return reinterpret_cast<uint4 *>(qbuf + g * S::QTILE + (c >> 3) * PC_QBOX + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };   // 16 bytes c of it
+            uint4 q[HD / 8];
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) q[i] = *at(i);
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i)
+                for (uint32_t w : {q[i].x, q[i].y, q[i].z, q[i].w}) most = max3(most, fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u)));
+            // times 2^(127 - down) the largest is between 224 and 448 = 1.75 2^8
+            const uint32_t bits = __float_as_uint(most);
+            const int down = min(max((int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u), 1), 253);
+            const float f = most < INFINITY ? __uint_as_float((uint32_t)(254 - down) << 23) : __uint_as_float(0x7fc00000u);   // Inf has no code
+            back = __uint_as_float((uint32_t)down << 23);
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i) {
+                uint32_t high[4], rest[4];
+                const uint32_t words[8] = {q[2 * i].x, q[2 * i].y, q[2 * i].z, q[2 * i].w, q[2 * i + 1].x, q[2 * i + 1].y, q[2 * i + 1].z, q[2 * i + 1].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t h[2], l[2];
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) {
+                        const uint32_t w = words[2 * e + d];
+                        const __half2 x = __floats2half2_rn(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xffff0000u) * f);   // exact down to 2^-14
+                        h[d] = codes_of(x);
+                        const uint32_t y = f16x2_of_codes(h[d]);
+                        l[d] = codes_of(__hsub2(x, *reinterpret_cast<const __half2 *>(&y)));
+                    }
+                    high[e] = h[0] | h[1] << 16;
+                    rest[e] = l[0] | l[1] << 16;
+                }
+                *at(i) = make_uint4(high[0], high[1], high[2], high[3]);
+                *at(HD / 16 + i) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+            }
+        };
         bool more = next(), again = false;   // again: a row's sums came out as Inf or NaN
         if (more) fetch_q();
         while (more) {
@@ -662,6 +668,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const int rows = x.s.ntok * group, tiles = g ? x.second : x.first, lo = x.s.lo, hi = x.s.hi, slot0 = n0;
             if (tiles > 0) {
                 asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+                if constexpr (E8) {
+                    __syncwarp();   // the warp's rows have come
+                    terms_of_q();
+                }
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.qfull[g]);

@@ -65,6 +65,11 @@ __device__ __forceinline__ uint32_t codes_of(float lo, float hi) {   // the near
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(d) : "f"(hi), "f"(lo));
     return d;
 }
+__device__ __forceinline__ uint32_t codes_of(__half2 x) {
+    uint16_t d;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;\n" : "=h"(d) : "r"(*reinterpret_cast<const uint32_t *>(&x)));
+    return d;
+}
 // 16 bytes of a row of keys or values as floats, to be scaled where they are codes.
 template <typename P> struct PagedChunk {   // bf16: 8 elements
     static constexpr int N = 8;
