@@ -155,9 +155,13 @@ __host__ __device__ __forceinline__ long long paged_gaps(const PagedPlan &a, int
     const long long c = y0 >> a.tq_shift;
     return paged_floors(c + m, s) - paged_floors(c, s) - m * sinks;
 }
+__host__ __device__ __forceinline__ int paged_keys(const PagedPlan &a, int base, int q_tile) {   // units of a tile of queries
+    return a.whole ? 1 : (int)(((long long)base + ((long long)(q_tile + 1) << a.tq_shift) + (1 << a.key_shift) - 1) >> a.key_shift) - paged_gap(a, base, q_tile);
+}
 // Units of the first n tiles of a row's queries: the sum over i < n of ceil((base + (i + 1) tq) / keys), both powers of two, less what a window leaves out.
 __host__ __device__ __forceinline__ long long paged_units(const PagedPlan &a, int base, long long n) {
     if (a.whole) return n;
+    if (n <= 1) return n == 1 ? paged_keys(a, base, 0) : 0;   // single tokens
     const int s = a.key_shift - a.tq_shift;
     if (s <= 0) return n * (((long long)base + (1 << a.key_shift) - 1) >> a.key_shift) + ((n * (n + 1) / 2) << -s) - paged_gaps(a, base, n);
     // ceil((b + i + 1) / 2^s) with b = ceil(base / tq): floors of c + i over 2^s, summed up to c + n and without those up to c
@@ -214,9 +218,6 @@ __host__ __device__ __forceinline__ long long paged_div(long long a, long long b
 }
 // Where the run of CTA c begins.
 __host__ __device__ __forceinline__ long long paged_begin(const PagedRun &run, int c) { return paged_div(run.total * min(c, run.ctas), run.ctas); }
-__host__ __device__ __forceinline__ int paged_keys(const PagedPlan &a, int base, int q_tile) {   // units of a tile of queries
-    return a.whole ? 1 : (int)(((long long)base + ((long long)(q_tile + 1) << a.tq_shift) + (1 << a.key_shift) - 1) >> a.key_shift) - paged_gap(a, base, q_tile);
-}
 // Unit `in` of a row: its head, the tile of queries it is of, and which of that tile's.
 struct PagedUnit {
     int head, q_tile, k;
