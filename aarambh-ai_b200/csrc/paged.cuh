@@ -128,7 +128,7 @@ struct PagedPlan {
 };
 __host__ __device__ __forceinline__ int paged_token(const PagedPlan &a, int r) { return (r * a.per_group) >> 16; }
 struct PagedShape {
-    int q_tiles, base;          // of the row; keys before its new tokens
+    int q_tiles, base;          // of the row; keys before its new tokens, negative where those are more than its keys
     long long per;              // units of a head
     long long units;
 };
@@ -156,16 +156,18 @@ __host__ __device__ __forceinline__ long long paged_gaps(const PagedPlan &a, int
     return paged_floors(c + m, s) - paged_floors(c, s) - m * sinks;
 }
 __host__ __device__ __forceinline__ int paged_keys(const PagedPlan &a, int base, int q_tile) {   // units of a tile of queries
-    return a.whole ? 1 : (int)(((long long)base + ((long long)(q_tile + 1) << a.tq_shift) + (1 << a.key_shift) - 1) >> a.key_shift) - paged_gap(a, base, q_tile);
+    return a.whole ? 1 : (int)((max(base, 0) + ((long long)(q_tile + 1) << a.tq_shift) + (1 << a.key_shift) - 1) >> a.key_shift) - paged_gap(a, base, q_tile);
 }
-// Units of the first n tiles of a row's queries: the sum over i < n of ceil((base + (i + 1) tq) / keys), both powers of two, less what a window leaves out.
+// Units of the first n tiles of a row's queries: the sum over i < n of ceil((base + (i + 1) tq) / keys), both powers of two, less what a window leaves out.  A base
+// below none counts as none there; only the window knows where such a row's tokens stand, so that its gap is the one that their keys are read by.
 __host__ __device__ __forceinline__ long long paged_units(const PagedPlan &a, int base, long long n) {
     if (a.whole) return n;
     if (n <= 1) return n == 1 ? paged_keys(a, base, 0) : 0;   // single tokens
     const int s = a.key_shift - a.tq_shift;
-    if (s <= 0) return n * (((long long)base + (1 << a.key_shift) - 1) >> a.key_shift) + ((n * (n + 1) / 2) << -s) - paged_gaps(a, base, n);
+    const long long ahead = max(base, 0);
+    if (s <= 0) return n * ((ahead + (1 << a.key_shift) - 1) >> a.key_shift) + ((n * (n + 1) / 2) << -s) - paged_gaps(a, base, n);
     // ceil((b + i + 1) / 2^s) with b = ceil(base / tq): floors of c + i over 2^s, summed up to c + n and without those up to c
-    const long long c = (((long long)base + (1 << a.tq_shift) - 1) >> a.tq_shift) + (1ll << s);
+    const long long c = ((ahead + (1 << a.tq_shift) - 1) >> a.tq_shift) + (1ll << s);
     return paged_floors(c + n, s) - paged_floors(c, s) - paged_gaps(a, base, n);
 }
 __host__ __device__ __forceinline__ PagedShape paged_shape(const PagedPlan &a, const PagedRow &r) {
@@ -173,7 +175,7 @@ __host__ __device__ __forceinline__ PagedShape paged_shape(const PagedPlan &a, c
     const long long rows = (long long)r.count * a.group;
     if (rows <= a.above || rows > a.most) return s;
     s.q_tiles = (int)(((long long)r.count + (1 << a.tq_shift) - 1) >> a.tq_shift);
-    s.base = max(r.len - r.count, 0);
+    s.base = r.len - r.count;
     s.per = paged_units(a, s.base, s.q_tiles);
     s.units = s.per * a.p.kv_heads;
     return s;
