@@ -66,12 +66,12 @@ __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_sim
     float *qs = (float *)(smem + (E8 ? 2 * S::BUF + 4 * S::RAW : 4 * S::BUF)), *ps = qs + QR * KROW;
     const int tx = threadIdx.x % TX, row0 = threadIdx.x / TX * S::FIRST;
     const PagedView &p = a.plan.p;
-    PagedRun run = paged_run<PA_THREADS>(a.plan, blockIdx.x, gridDim.x, warp_sums, found, a.status);
+    PagedRun run = paged_run<PA_THREADS, WIN>(a.plan, blockIdx.x, gridDim.x, warp_sums, found, a.status);
     if (threadIdx.x == 0) paged_uncut(a, blockIdx.x);
     PagedPiece w;
-    while (paged_next(a.plan, run, w)) {
-        const PagedSpan sp = paged_span(a.plan, w);
-        const PagedHole hole = WIN ? paged_hole(a.plan, sp.base, w.q_tile) : PagedHole{0, 0};
+    while (paged_next<WIN>(a.plan, run, w)) {
+        const PagedSpan sp = paged_span<WIN>(a.plan, w);
+        const PagedHole hole = paged_hole<WIN>(a.plan, sp.base, w.q_tile);
         if (threadIdx.x == 0) paged_cut(a, run, w, sp, blockIdx.x);
         const int t0 = sp.t0, ntok = sp.ntok, base = sp.base, lo = sp.lo, hi = sp.hi, group = a.plan.group;
         __syncthreads();

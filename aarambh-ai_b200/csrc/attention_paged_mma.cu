@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(32 * PM_WARPS, 2) paged_mma_kernel(const __gri
     const PagedView &p = a.plan.p;
     uint8_t *ring = smem + warp * STAGES * S::BLOCK;
     const int me = warp * gridDim.x + blockIdx.x;   // a little work spreads over all SMs
-    PagedRun run = paged_run<32>(a.plan, me, a.ctas, nullptr, found[warp], a.status);
+    PagedRun run = paged_run<32, WIN>(a.plan, me, a.ctas, nullptr, found[warp], a.status);
     if (lane == 0) paged_uncut(a, me);
 
     // ---- the copies run ahead of the products, over the same pieces
@@ -100,8 +100,8 @@ __global__ void __launch_bounds__(32 * PM_WARPS, 2) paged_mma_kernel(const __gri
     };
     auto seek = [&]() {        // the first block of the next piece that has keys
         for (;;) {
-            if (!paged_next(a.plan, ahead, aw)) { more = false; return; }
-            as = paged_span(a.plan, aw);
+            if (!paged_next<WIN>(a.plan, ahead, aw)) { more = false; return; }
+            as = paged_span<WIN>(a.plan, aw);
             if (WIN) ah = paged_hole(a.plan, as.base, aw.q_tile);
             akey = as.lo;
             if (akey < as.hi) break;
@@ -138,9 +138,9 @@ __global__ void __launch_bounds__(32 * PM_WARPS, 2) paged_mma_kernel(const __gri
 
     int stage = 0;
     PagedPiece w;
-    while (paged_next(a.plan, run, w)) {
-        const PagedSpan sp = paged_span(a.plan, w);
-        const int gap = WIN ? paged_hole(a.plan, sp.base, w.q_tile).gap : 0;
+    while (paged_next<WIN>(a.plan, run, w)) {
+        const PagedSpan sp = paged_span<WIN>(a.plan, w);
+        const int gap = paged_hole<WIN>(a.plan, sp.base, w.q_tile).gap;
         if (lane == 0) paged_cut(a, run, w, sp, me);
         const int rows = sp.ntok * group;
         // rows of the tile: 8 t + g as columns of Q^T, 8 t + 2 c and 8 t + 2 c + 1 as columns of scores and sums
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(32 * PM_WARPS, 2) paged_mma_kernel(const __gri
             }
         }
         __syncwarp();
-        for (poisoned &= rows >= 32 ? 0xffffffffu : (1u << rows) - 1; poisoned; poisoned &= poisoned - 1) paged_again<HD, Page>(a, w, sp, __ffs(poisoned) - 1, lane, all, slot);
+        for (poisoned &= rows >= 32 ? 0xffffffffu : (1u << rows) - 1; poisoned; poisoned &= poisoned - 1) paged_again<HD, Page, WIN>(a, w, sp, __ffs(poisoned) - 1, lane, all, slot);
         __syncwarp();
     }
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");

@@ -97,10 +97,10 @@ struct PcPiece {
     __device__ __forceinline__ int most() const { return max(first, second); }
 };
 template <bool WIN> __device__ __forceinline__ bool pc_next(const PagedPlan &a, PagedRun &run, PcPiece &x) {
-    if (!paged_next(a, run, x.w)) return false;
-    x.s = paged_span(a, x.w);
+    if (!paged_next<WIN>(a, run, x.w)) return false;
+    x.s = paged_span<WIN>(a, x.w);
     const int rows = x.s.ntok * a.group;
-    const int gap = WIN ? paged_hole(a, x.s.base, x.w.q_tile).gap : 0;
+    const int gap = paged_hole<WIN>(a, x.s.base, x.w.q_tile).gap;
     auto tiles = [&](int first, int end) {   // of rows [first, end) of the item: keys up to those of the last token
         const int last = min(x.s.hi, x.s.base + x.s.t0 + paged_token(a, end - 1) + 1 - gap);
         return end > first ? max(0, (last - x.s.lo + PC_KEYS - 1) / PC_KEYS) : 0;
@@ -382,7 +382,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     pdl_wait();   // ahead of tensor memory too, which the launch before may hold
-    PagedRun run = paged_run<S::THREADS>(a.plan, blockIdx.x, a.ctas, sh.warp_sums, sh.found, a.status);
+    PagedRun run = paged_run<S::THREADS, WIN>(a.plan, blockIdx.x, a.ctas, sh.warp_sums, sh.found, a.status);
     if (threadIdx.x == PC_THREADS - 1) paged_uncut(a, blockIdx.x);
     if (run.u >= run.u1) return;   // the whole CTA
     if (threadIdx.x == 0) sh.start = run;
@@ -443,7 +443,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             // ---------------------------------------------------------- producer over codes: V, as codes, then K
             int n = 0;
             while (pc_next<WIN>(a.plan, run, x)) {
-                const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
+                const PagedHole hole = paged_hole<WIN>(a.plan, x.s.base, x.w.q_tile);
                 for (int j = 0; j < x.most(); ++j, ++n) {
                     const int v = x.s.lo + j * PC_KEYS + lane * PC_ROWS, key = WIN ? paged_key(hole, v) : v, raw = n % RAWS, slot = n % S::SLOTS;
                     const bool mine = lane < PC_KEYS / PC_ROWS && v < x.s.hi && !(WIN && paged_hidden(a.plan, x.s, key, PC_ROWS));
@@ -481,7 +481,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             // ---------------------------------------------------------- TMA producer: K, V, K, V, ...
             int n = 0;
             while (pc_next<WIN>(a.plan, run, x)) {
-                const PagedHole hole = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile) : PagedHole{0, 0};
+                const PagedHole hole = paged_hole<WIN>(a.plan, x.s.base, x.w.q_tile);
                 for (int j = 0; j < x.most(); ++j) {
                     const int v = x.s.lo + j * PC_KEYS + lane * PC_ROWS, key = WIN ? paged_key(hole, v) : v;
                     const bool mine = lane < PC_KEYS / PC_ROWS && v < x.s.hi;
@@ -681,7 +681,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             unit = {0.f, -1.f, 0.f, 1.f};
             const bool second = twice && (lane & PC_TWICE);
             const int rr = g * PC_Q + r, asks = twice && r < 2 * PC_TWICE ? r % PC_TWICE : rr;
-            const int gap = WIN ? paged_hole(a.plan, x.s.base, x.w.q_tile).gap : 0, first = x.s.base + x.s.t0 - gap;   // all in virtual keys
+            const int gap = paged_hole<WIN>(a.plan, x.s.base, x.w.q_tile).gap, first = x.s.base + x.s.t0 - gap;   // all in virtual keys
             const int pos = asks < rows ? first + paged_token(a.plan, asks) : -1;
             const int least = first + paged_token(a.plan, g * PC_Q);   // the first row sees up to here
             const int late = WIN ? first + paged_token(a.plan, min(rows, (g + 1) * PC_Q) - 1) + 1 - a.plan.window : 0;   // the last row sees from here on, and the sinks
@@ -808,7 +808,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     }
                 }
                 for (uint32_t left = __ballot_sync(0xffffffffu, worst == 0x7f800000u); left; left &= left - 1)
-                    paged_again<HD, Page>(a, x.w, x.s, g * PC_Q + quad * 32 + __ffs(left) - 1, lane, all, slot);
+                    paged_again<HD, Page, WIN>(a, x.w, x.s, g * PC_Q + quad * 32 + __ffs(left) - 1, lane, all, slot);
                 __syncwarp();
             }
         }

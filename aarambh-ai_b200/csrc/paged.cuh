@@ -137,16 +137,16 @@ __host__ __device__ __forceinline__ long long paged_floors(long long y, int s) {
     const long long q = y >> s;
     return (q * (q - 1) / 2 << s) + q * (y & ((1ll << s) - 1));
 }
-// Through a window a tile of queries sees two runs of units: those of the sinks, and those from its first token's window on.  The units between are left
+// WIN: for kernels that are compiled without windows.  Through a window a tile of queries sees two runs of units: those of the sinks, and those from its first token's window on.  The units between are left
 // out, and the tile's units are numbered as if there were none ("virtual" keys: those behind the sinks' units, less what is left out).
 __host__ __device__ __forceinline__ long long paged_sink_units(const PagedPlan &a) { return ((long long)a.sinks + (1 << a.key_shift) - 1) >> a.key_shift; }
-__host__ __device__ __forceinline__ int paged_gap(const PagedPlan &a, int base, int q_tile) {   // units between
-    if (!a.window) return 0;
+template <bool WIN = true> __host__ __device__ __forceinline__ int paged_gap(const PagedPlan &a, int base, int q_tile) {   // units between
+    if (!WIN || !a.window) return 0;
     const long long y = (long long)base + ((long long)q_tile << a.tq_shift) - a.window + 1, gap = (y >> a.key_shift) - paged_sink_units(a);
     return gap > 0 ? (int)gap : 0;
 }
-__host__ __device__ __forceinline__ long long paged_gaps(const PagedPlan &a, int base, long long n) {   // their sum over the first n tiles
-    if (!a.window) return 0;
+template <bool WIN = true> __host__ __device__ __forceinline__ long long paged_gaps(const PagedPlan &a, int base, long long n) {   // their sum over the first n tiles
+    if (!WIN || !a.window) return 0;
     const long long sinks = paged_sink_units(a), y = (long long)base - a.window + 1, from = ((sinks + 1) << a.key_shift) - y;   // tile i has some where i tq >= from
     const long long first = from > 0 ? (from + (1 << a.tq_shift) - 1) >> a.tq_shift : 0, m = n - first, y0 = y + (first << a.tq_shift);
     if (m <= 0) return 0;
@@ -155,28 +155,28 @@ __host__ __device__ __forceinline__ long long paged_gaps(const PagedPlan &a, int
     const long long c = y0 >> a.tq_shift;
     return paged_floors(c + m, s) - paged_floors(c, s) - m * sinks;
 }
-__host__ __device__ __forceinline__ int paged_keys(const PagedPlan &a, int base, int q_tile) {   // units of a tile of queries
-    return a.whole ? 1 : (int)((max(base, 0) + ((long long)(q_tile + 1) << a.tq_shift) + (1 << a.key_shift) - 1) >> a.key_shift) - paged_gap(a, base, q_tile);
+template <bool WIN = true> __host__ __device__ __forceinline__ int paged_keys(const PagedPlan &a, int base, int q_tile) {   // units of a tile of queries
+    return a.whole ? 1 : (int)((max(base, 0) + ((long long)(q_tile + 1) << a.tq_shift) + (1 << a.key_shift) - 1) >> a.key_shift) - paged_gap<WIN>(a, base, q_tile);
 }
 // Units of the first n tiles of a row's queries: the sum over i < n of ceil((base + (i + 1) tq) / keys), both powers of two, less what a window leaves out.  A base
 // below none counts as none there; only the window knows where such a row's tokens stand, so that its gap is the one that their keys are read by.
-__host__ __device__ __forceinline__ long long paged_units(const PagedPlan &a, int base, long long n) {
+template <bool WIN = true> __host__ __device__ __forceinline__ long long paged_units(const PagedPlan &a, int base, long long n) {
     if (a.whole) return n;
-    if (n <= 1) return n == 1 ? paged_keys(a, base, 0) : 0;   // single tokens
+    if (n <= 1) return n == 1 ? paged_keys<WIN>(a, base, 0) : 0;   // single tokens
     const int s = a.key_shift - a.tq_shift;
     const long long ahead = max(base, 0);
-    if (s <= 0) return n * ((ahead + (1 << a.key_shift) - 1) >> a.key_shift) + ((n * (n + 1) / 2) << -s) - paged_gaps(a, base, n);
+    if (s <= 0) return n * ((ahead + (1 << a.key_shift) - 1) >> a.key_shift) + ((n * (n + 1) / 2) << -s) - paged_gaps<WIN>(a, base, n);
     // ceil((b + i + 1) / 2^s) with b = ceil(base / tq): floors of c + i over 2^s, summed up to c + n and without those up to c
     const long long c = ((ahead + (1 << a.tq_shift) - 1) >> a.tq_shift) + (1ll << s);
-    return paged_floors(c + n, s) - paged_floors(c, s) - paged_gaps(a, base, n);
+    return paged_floors(c + n, s) - paged_floors(c, s) - paged_gaps<WIN>(a, base, n);
 }
-__host__ __device__ __forceinline__ PagedShape paged_shape(const PagedPlan &a, const PagedRow &r) {
+template <bool WIN = true> __host__ __device__ __forceinline__ PagedShape paged_shape(const PagedPlan &a, const PagedRow &r) {
     PagedShape s = {0, 0, 0, 0};
     const long long rows = (long long)r.count * a.group;
     if (rows <= a.above || rows > a.most) return s;
     s.q_tiles = (int)(((long long)r.count + (1 << a.tq_shift) - 1) >> a.tq_shift);
     s.base = r.len - r.count;
-    s.per = paged_units(a, s.base, s.q_tiles);
+    s.per = paged_units<WIN>(a, s.base, s.q_tiles);
     s.units = s.per * a.p.kv_heads;
     return s;
 }
@@ -224,37 +224,37 @@ __host__ __device__ __forceinline__ long long paged_begin(const PagedRun &run, i
 struct PagedUnit {
     int head, q_tile, k;
 };
-__host__ __device__ __forceinline__ PagedUnit paged_find(const PagedPlan &a, const PagedShape &s, long long in) {
+template <bool WIN = true> __host__ __device__ __forceinline__ PagedUnit paged_find(const PagedPlan &a, const PagedShape &s, long long in) {
     const int head = (int)paged_div(in, s.per);
     const long long y = in - head * s.per;
     int lo = 0, hi = s.q_tiles - 1;   // the tile that unit y of the head is of
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (paged_units(a, s.base, mid) <= y) lo = mid;
+        if (paged_units<WIN>(a, s.base, mid) <= y) lo = mid;
         else hi = mid - 1;
     }
-    return {head, lo, (int)(y - paged_units(a, s.base, lo))};
+    return {head, lo, (int)(y - paged_units<WIN>(a, s.base, lo))};
 }
 // Puts the run at that unit.
-__host__ __device__ __forceinline__ void paged_at(const PagedPlan &a, PagedRun &run, int row, const PagedUnit &u) {
+template <bool WIN = true> __host__ __device__ __forceinline__ void paged_at(const PagedPlan &a, PagedRun &run, int row, const PagedUnit &u) {
     run.row = row; run.head = u.head; run.q_tile = u.q_tile; run.k = u.k;
     run.r = paged_row(a.p, row, nullptr);
-    const PagedShape s = paged_shape(a, run.r);
+    const PagedShape s = paged_shape<WIN>(a, run.r);
     run.q_tiles = s.q_tiles;
     run.base = s.base;
-    run.k_tiles = paged_keys(a, run.base, run.q_tile);
+    run.k_tiles = paged_keys<WIN>(a, run.base, run.q_tile);
 }
 __host__ __device__ __forceinline__ int paged_ctas(const PagedPlan &a, long long total, int ctas) {   // that have any of `total` units
     const long long n = paged_div(total, a.least);
     return n < 1 ? 1 : n < ctas ? (int)n : ctas;
 }
 // The run of CTA (or, with THREADS 32, warp) `c` of `ctas`, found by all its threads.  `found` is shared.
-template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const PagedPlan &a, int c, int ctas, long long *warp_sums, int2 *found, int *status) {
+template <int THREADS, bool WIN = true> __device__ __forceinline__ PagedRun paged_run(const PagedPlan &a, int c, int ctas, long long *warp_sums, int2 *found, int *status) {
     PagedRun run = {};
     long long n, prefix = 0, units = 0, row_first = 0;
     for (int r0 = 0; r0 < a.p.rows; r0 += THREADS) {
         const int r = r0 + (int)(threadIdx.x % THREADS);
-        const long long here = r < a.p.rows ? paged_shape(a, paged_row(a.p, r, c == 0 ? status : nullptr)).units : 0;
+        const long long here = r < a.p.rows ? paged_shape<WIN>(a, paged_row(a.p, r, c == 0 ? status : nullptr)).units : 0;
         const long long at = cta_prefix<THREADS>(here, n, warp_sums);
         if (r0 == 0) { prefix = at; units = here; }
         run.total += n;
@@ -267,7 +267,7 @@ template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const Paged
     for (int r0 = 0;; r0 += THREADS) {
         if (r0 > 0) {
             const int r = r0 + (int)(threadIdx.x % THREADS);
-            units = r < a.p.rows ? paged_shape(a, paged_row(a.p, r, nullptr)).units : 0;
+            units = r < a.p.rows ? paged_shape<WIN>(a, paged_row(a.p, r, nullptr)).units : 0;
             prefix = row_first + cta_prefix<THREADS>(units, n, warp_sums);
         } else if (a.p.rows > THREADS) {
             (void)cta_prefix<THREADS>(units, n, warp_sums);
@@ -276,7 +276,7 @@ template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const Paged
         }
         if (units > 0 && run.u >= prefix && run.u < prefix + units) {
             const int row = r0 + (int)(threadIdx.x % THREADS);
-            const PagedUnit u = paged_find(a, paged_shape(a, paged_row(a.p, row, nullptr)), run.u - prefix);
+            const PagedUnit u = paged_find<WIN>(a, paged_shape<WIN>(a, paged_row(a.p, row, nullptr)), run.u - prefix);
             found[0] = make_int2(row, u.head);
             found[1] = make_int2(u.q_tile, u.k);
         }
@@ -285,7 +285,7 @@ template <int THREADS> __device__ __forceinline__ PagedRun paged_run(const Paged
     }
     if (THREADS == 32) __syncwarp();
     else __syncthreads();
-    paged_at(a, run, found[0].x, {found[0].y, found[1].x, found[1].y});
+    paged_at<WIN>(a, run, found[0].x, {found[0].y, found[1].x, found[1].y});
     return run;
 }
 // A piece of work: units [k0, k1) of the item (row, head, q_tile), which has k_tiles of them.
@@ -294,7 +294,7 @@ struct PagedPiece {
     PagedRow r;
 };
 // The next piece of the run; false at its end.  The same for all threads that call it with the same run.
-__host__ __device__ __forceinline__ bool paged_next(const PagedPlan &a, PagedRun &run, PagedPiece &w) {
+template <bool WIN = true> __host__ __device__ __forceinline__ bool paged_next(const PagedPlan &a, PagedRun &run, PagedPiece &w) {
     if (run.u >= run.u1) return false;
     if (run.k == run.k_tiles) {   // the next item: of the head, of the row, of the next row that has any
         run.k = 0;
@@ -305,13 +305,13 @@ __host__ __device__ __forceinline__ bool paged_next(const PagedPlan &a, PagedRun
                 do {
                     if (++run.row >= a.p.rows) return false;
                     run.r = paged_row(a.p, run.row, nullptr);
-                    const PagedShape s = paged_shape(a, run.r);
+                    const PagedShape s = paged_shape<WIN>(a, run.r);
                     run.q_tiles = s.q_tiles;
                     run.base = s.base;
                 } while (run.q_tiles == 0);
             }
         }
-        run.k_tiles = paged_keys(a, run.base, run.q_tile);
+        run.k_tiles = paged_keys<WIN>(a, run.base, run.q_tile);
     }
     w.row = run.row; w.head = run.head; w.q_tile = run.q_tile; w.r = run.r; w.k_tiles = run.k_tiles;
     w.k0 = run.k;
@@ -329,18 +329,18 @@ struct PagedSpan {
 struct PagedHole {
     int gap, jump;
 };
-__host__ __device__ __forceinline__ PagedHole paged_hole(const PagedPlan &a, int base, int q_tile) {
+template <bool WIN = true> __host__ __device__ __forceinline__ PagedHole paged_hole(const PagedPlan &a, int base, int q_tile) {
     PagedHole h;
-    h.gap = paged_gap(a, base, q_tile) << a.key_shift;
+    h.gap = paged_gap<WIN>(a, base, q_tile) << a.key_shift;
     h.jump = h.gap ? (int)(paged_sink_units(a) << a.key_shift) : 0;
     return h;
 }
-__host__ __device__ __forceinline__ PagedSpan paged_span(const PagedPlan &a, const PagedPiece &w) {
+template <bool WIN = true> __host__ __device__ __forceinline__ PagedSpan paged_span(const PagedPlan &a, const PagedPiece &w) {
     PagedSpan s;
     s.t0 = w.q_tile << a.tq_shift;
     s.ntok = min(1 << a.tq_shift, w.r.count - s.t0);
     s.base = w.r.len - w.r.count;
-    const int last = s.base + s.t0 + s.ntok - paged_hole(a, s.base, w.q_tile).gap;   // behind the last key that a token of the item sees
+    const int last = s.base + s.t0 + s.ntok - paged_hole<WIN>(a, s.base, w.q_tile).gap;   // behind the last key that a token of the item sees
     s.lo = a.whole ? 0 : (int)min((long long)w.k0 << a.key_shift, 0x7fffffffll);
     s.hi = a.whole ? last : (int)min((long long)last, (long long)w.k1 << a.key_shift);
     return s;
@@ -390,13 +390,13 @@ __host__ __device__ __forceinline__ void paged_cut(const PagedAttnArgs &a, const
 // Row r of a piece (queries of bf16, pages of P: bf16, or e4m3 codes) over the keys of it that it sees, by one warp: where a product with hidden values has left Inf or
 // NaN (a weight of 0 times either), this gives what the keys in sight alone give.  32 keys at a time: a lane has one for the scores, and every 32nd dimension for the
 // sums, so that loads of 32 keys are in flight where one key after the other waited for its page, its shuffles and its exponential.
-template <int HD, typename P = __nv_bfloat16>
+template <int HD, typename P, bool WIN>
 __device__ __forceinline__ void paged_again(const PagedAttnArgs &a, const PagedPiece &w, const PagedSpan &sp, int r, int lane, bool all, size_t slot) {
     constexpr int N = HD / 32;
     constexpr bool CODES = sizeof(P) == 1;
     using Chunk = PagedChunk<P>;
     const int tok = paged_token(a.plan, r), head = w.head * a.plan.group + r - tok * a.plan.group;
-    const PagedHole hole = paged_hole(a.plan, sp.base, w.q_tile);
+    const PagedHole hole = paged_hole<WIN>(a.plan, sp.base, w.q_tile);
     const int pos = sp.base + sp.t0 + tok, to = min(sp.hi - 1, pos - hole.gap);
     const __nv_bfloat16 *q = (const __nv_bfloat16 *)a.q + (size_t)(w.r.first + sp.t0 + tok) * a.q_stride + (size_t)head * HD;
     float acc[N] = {}, top = -INFINITY, sum = 0.f;
@@ -404,7 +404,7 @@ __device__ __forceinline__ void paged_again(const PagedAttnArgs &a, const PagedP
         const int key = paged_key(hole, key0 + lane), n = min(32, to - key0 + 1);
         long long row = -1;   // of a key out of sight
         float s = -INFINITY, vs = 1.f;
-        if (lane < n && (!a.plan.window || key < a.plan.sinks || key > pos - a.plan.window)) {
+        if (lane < n && (!WIN || key < a.plan.sinks || key > pos - a.plan.window)) {
             row = (((long long)paged_page(a.plan.p, w.row, key, a.status) * a.plan.p.kv_heads + w.head) << a.plan.p.page_shift) + (key & ((1 << a.plan.p.page_shift) - 1));
             const P *k = (const P *)a.k + row * HD;
             s = 0.f;
