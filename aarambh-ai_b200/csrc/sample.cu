@@ -13,6 +13,7 @@
 // up to there go to the first CTA's list, which finds both borders by halving keys, exactly.  Where a list does not hold them (a nucleus of thousands of tokens,
 // thousands of equal logits), or all tokens stay, the CTAs work on their slices instead, and join their sums.
 #include <algorithm>
+#include <type_traits>
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -51,6 +52,8 @@ struct alignas(16) SampleShared {
     u64 list[SP_LIST];            // tokens: key and, below it, what is larger for lower indices
     u64 weights[SP_LIST];
     u64 red[2][SP_WARPS], slot[2], part[SP_WARPS];
+    u64 sums[2];                  // of the slice: mass ahead of top-p's border, and tokens on it; read by the cluster's others
+    int ties[SP_WARPS];
     float scan[3][SP_WARPS];
     uint32_t powers[256];         // 2^(j / 256), times 2^31
     float tops[2];                // the slice's largest logit, and one that so many of its tokens reach; read by the cluster's others
@@ -277,8 +280,9 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
         if (infinite) return z == top ? 0 : SP_BINS - 1;
         return __float_as_int(fminf(fmaf(top - z, c_bin, SP_MAGIC), SP_MAGIC + (SP_BINS - 1))) - 0x4b400000;
     };
-    const double full = (double)weight(top), wmin = (double)min_p * full;
-    auto likely = [&](u64 w) { return !(min_p > 0.f) || (double)w >= wmin; };
+    const double full = (double)weight(top);
+    const u64 wmin = min_p > 0.f ? (u64)ceil((double)min_p * full) : 0ull;
+    auto likely = [&](u64 w) { return w >= wmin; };
     auto load = [&](int i, T (&e)[V]) {   // V tokens from i on, a multiple of V; -inf behind the slice
         if (CACHED) {
             *reinterpret_cast<uint4 *>(e) = *reinterpret_cast<const uint4 *>(cache + i);
@@ -474,6 +478,160 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
         }
         cluster.sync();
         if (tid == 0) sh.listed = 0;   // of the first CTA; behind another barrier of all it is written again
+    }
+
+    // ---- bf16, top-p without top-k: a row has few logits that differ, so that counts of them and a weight for each give top-p's border exactly, ties and all, and one pass
+    // over the weights gives the token.  A slot is a logit, in falling order, from the largest down to the last that weighs anything; those near zero, whose binades go
+    // on down to 2^-126, share one (the band), are weighed token by token, and leave a border among them to what follows.
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const int kt = (int)(key_of(top) >> 16), kl = (int)(key_of(lowest) >> 16);   // the upper half of a key: all of a bf16's
+        int bits = max(128, (kt - kl + 1 - SP_BINS + 255) / 256 * 128), positive, negative, slots;   // the band is of those below the power of two with these bits
+        for (;; bits += 128) {
+            positive = 0x8000 + bits;       // the least key above the band
+            negative = 0x7fff - bits;       // the largest below it
+            slots = kt - kl + 1;
+            if (kl <= negative) slots -= positive - negative - 2;
+            else if (kl < positive) slots = kt - positive + 2;
+            if (slots <= SP_BINS || positive > kt) break;
+        }
+        if (quick && k <= 0 && by_p && slots <= SP_BINS && positive <= kt) {
+            const int shut = positive - negative - 2;   // keys that the band closes up
+            const int band = kt - positive + 1;         // its slot
+            auto slot_of = [&](T z) -> int {            // less than 0, or `slots` and more: of those that weigh nothing (NaN, -inf)
+                const int r = (int)__bfloat16_as_ushort(z), key = r ^ (r & 0x8000 ? 0xffff : 0x8000), d = kt - key;
+                return key >= positive ? d : key > negative ? band : d - shut;
+            };
+            auto logit_at = [&](int slot) {             // not of the band
+                const int key = kt - (slot < band ? slot : slot + shut);
+                return __uint_as_float((uint32_t)(key ^ (key & 0x8000 ? 0x8000 : 0xffff)) << 16);
+            };
+            constexpr int B = SP_BINS / SP_THREADS;
+            for (int b = tid; b < SP_BINS; b += SP_THREADS) sh.counts[b] = 0;
+            __syncthreads();
+            u64 in_band = 0;
+            for (int i = tid * V; i < n; i += SP_THREADS * V) {
+                alignas(16) T e[V];
+                load(i, e);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const int s = slot_of(e[j]);
+                    if ((unsigned)s >= (unsigned)slots) continue;
+                    if (s == band) in_band += quick_weight(to_f32(e[j]));
+                    else atomicAdd(&sh.counts[s], 1);
+                }
+            }
+            in_band = cluster_sum(in_band);
+            if (C == 1) __syncthreads();
+            int count[B] = {};
+            for (int r = 0; r < C; ++r) {
+                const int4 *from = reinterpret_cast<const int4 *>(cluster.map_shared_rank(sh.counts, r) + tid * B), v = from[0], w = from[1];
+                count[0] += v.x; count[1] += v.y; count[2] += v.z; count[3] += v.w;
+                count[4] += w.x; count[5] += w.y; count[6] += w.z; count[7] += w.w;
+            }
+            u64 weights[B], sum = 0;
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+                const int s = tid * B + j;
+                weights[j] = s < slots && s != band ? quick_weight(logit_at(s)) : 0ull;
+                sum += s == band ? in_band : weights[j] * (u64)count[j];
+            }
+            const u64 target = whole(share * (double)block_sum(sum));
+            u64 at = block_before(sum);
+            if (at < target && target <= at + sum) {
+#pragma unroll
+                for (int j = 0; j < B; ++j) {
+                    const u64 here = tid * B + j == band ? in_band : weights[j] * (u64)count[j];
+                    if (at < target && target <= at + here) {
+                        sh.found[0] = tid * B + j;
+                        sh.cut = weights[j] ? (target - at + weights[j] - 1) / weights[j] : 0ull;
+                    }
+                    at += here;
+                }
+            }
+            __syncthreads();
+            const int border = sh.found[0];   // the slot in which top-p ends
+            const u64 need = sh.cut;          // tokens of it that stay
+            if (border != band) {
+                const float edge = logit_at(border);
+                const u64 weighed = quick_weight(edge), each = likely(weighed) ? weighed : 0ull;
+                // of a token: its mass where it is ahead of the border, and whether it is on it
+                auto add = [&](T e, u64 &mass, int &ties) {
+                    const float z = to_f32(e);
+                    const u64 w = quick_weight(z);
+                    if (z > edge && likely(w)) mass += w;
+                    ties += z == edge;
+                };
+                auto kept = [&](u64 mass, u64 ties) { return mass + each * min(ties, need); };   // of equal logits the first ones stay
+                const int run = ((n + SP_WARPS - 1) / SP_WARPS + 32 * V - 1) / (32 * V) * (32 * V), i0 = warp * run, i1 = min(n, i0 + run);
+                u64 mass = 0;
+                int ties = 0;
+                for (int i = i0 + lane * V; i < i1; i += 32 * V) {
+                    alignas(16) T e[V];
+                    load(i, e);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) add(e[j], mass, ties);
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+                ties = __reduce_add_sync(0xffffffffu, ties);
+                if (lane == 0) { sh.part[warp] = mass; sh.ties[warp] = ties; }
+                const u64 slice_mass = block_sum(lane == 0 ? mass : 0ull), slice_ties = block_sum(lane == 0 ? (u64)ties : 0ull);
+                if (tid == 0) { sh.sums[0] = slice_mass; sh.sums[1] = slice_ties; }
+                cluster.sync();
+                u64 m = 0, t = 0, all_mass = 0, all_ties = 0;
+                for (int r = 0; r < C; ++r) {
+                    const ulonglong2 s = *reinterpret_cast<const ulonglong2 *>(cluster.map_shared_rank(sh.sums, r));
+                    if (r < rank) { m += s.x; t += s.y; }
+                    all_mass += s.x;
+                    all_ties += s.y;
+                }
+                const u64 target = draw_target(kept(all_mass, all_ties));
+                if (kept(m, t) < target && target <= kept(m + slice_mass, t + slice_ties)) {
+                    for (int w = 0; w < warp; ++w) { m += sh.part[w]; t += sh.ties[w]; }
+                    if (kept(m, t) < target && target <= kept(m + mass, t + ties)) {   // in this warp's run
+                        for (int i = i0; i < i1; i += 32 * V) {
+                            alignas(16) T e[V];
+                            u64 up = 0;
+                            int level = 0;
+                            const int at = i + lane * V;
+                            if (at < i1) load(at, e);
+                            else
+                                for (int j = 0; j < V; ++j) e[j] = from_f32<T>(-INFINITY);
+#pragma unroll
+                            for (int j = 0; j < V; ++j) add(e[j], up, level);
+                            const u64 here = up;
+                            const int tied = level;
+#pragma unroll
+                            for (int o = 1; o < 32; o <<= 1) {
+                                const u64 v = __shfl_up_sync(0xffffffffu, up, o);
+                                const int l = __shfl_up_sync(0xffffffffu, level, o);
+                                if (lane >= o) { up += v; level += l; }
+                            }
+                            const unsigned there = __ballot_sync(0xffffffffu, kept(m + up, t + level) >= target);
+                            if (there) {
+                                if (lane == __ffs(there) - 1) {
+                                    u64 sum = m + up - here;
+                                    int seen = level - tied;
+                                    for (int j = 0; j < V; ++j) {
+                                        add(e[j], sum, seen);
+                                        if (kept(sum, t + seen) >= target) {
+                                            a.out[row] = first + at + j;
+                                            break;
+                                        }
+                                    }
+                                }
+                                break;
+                            }
+                            m += __shfl_sync(0xffffffffu, up, 31);
+                            t += __shfl_sync(0xffffffffu, level, 31);
+                        }
+                    }
+                }
+                cluster.sync();   // the others may still read this CTA's sums
+                return;
+            }
+            cluster.sync();   // the others may still read this CTA's counts
+        }
     }
 
     u64 cut = 0ull;   // the last token that stays
