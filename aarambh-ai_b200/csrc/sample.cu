@@ -4,14 +4,20 @@
 //   top-k: the first k stay;  top-p: of these the shortest prefix whose mass is p of theirs or more;  min-p: of these the ones with p_v >= min_p
 //   the token: the first one that stayed, in order of index, whose cumulative mass exceeds u times all of theirs
 //
-// Weights are whole numbers, round(2^F p_v) with F up to 44, from f64: their sums are exact whatever the order, so that every run and every way of dealing the
-// row out draws the same token, and a border between two tokens lies within 2^-45 a token of where real numbers have it (f32 sums would move it by more than a
-// token's width in large vocabularies).
+// Weights are whole numbers, round(2^F p_v) with F up to 44, off by 2^-30.4 of themselves (quick_weight): their sums are exact whatever the order, so that every run and
+// every way of dealing the row out draws the same token, and a border between two tokens lies within that and 2^-45 a token of where real numbers have it (f32 sums would
+// move it by more than a token's width in large vocabularies).
 //
-// A cluster of CTAs has a row, each a slice of it, which it keeps in shared memory.  Nothing is sorted: tokens are counted by x in bins of 1/32; the bin in which
-// the k-th token lies, or a bracket of bins around the border of top-p, follows from the counts (a bin's weights differ by 2^(1/32) at most), and the few tokens
-// up to there go to the first CTA's list, which finds both borders by halving keys, exactly.  Where a list does not hold them (a nucleus of thousands of tokens,
-// thousands of equal logits), or all tokens stay, the CTAs work on their slices instead, and join their sums.
+// A cluster of CTAs has a row, each a slice of it, which it keeps in shared memory.  Most rows are decided by a few tokens: with top-k or min-p a logit is found that all
+// which can stay reach (of the threads' largest ones, sorted, the one of which k reach it), what reaches it goes to the first CTA's list, which is sorted, cut and
+// sorted again by index.  Otherwise tokens are counted by x in bins of 1/64 (of bf16 by logit); the bins up to the border go to the list where it holds them, or else the
+// border's bin is found by the bins' exact masses, and the token by one more pass, in which the CTAs join their sums.  Where a bin has more tokens than the list takes
+// (thousands of equal logits) its border is found by halving keys.
+//
+// Bound by its passes over the slice: instructions, not HBM, which a row crosses once.  64 rows of 128256 bf16 logits (16.4 MB, 2.5 us at a copy's rate), us: top-k of 50 or min-p 18,
+// unfiltered 28 (a weight a token, some 25 instructions), top-p of 0.9 50, of which counts of logits and the pass that weighs are two (bins of x, weighed twice and masses joined by carries: 103),
+// all kinds of rules in a batch 50; 4 rows of 32000 f32: 7, 10 to 12, 34, 23.  Weights looked up in a table by their logit instead of computed: 49 for 50, and unfiltered 36 for 28 (its reads of 8
+// bytes meet in banks).
 #include <algorithm>
 #include <type_traits>
 #include <cooperative_groups.h>
@@ -486,7 +492,11 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
         const int kt = (int)(key_of(top) >> 16), kl = (int)(key_of(lowest) >> 16);   // the upper half of a key: all of a bf16's
         int bits = max(128, (kt - kl + 1 - SP_BINS + 255) / 256 * 128), positive, negative, slots;   // the band is of those below the power of two with these bits
-        for (;; bits += 128) {
+        if (top < 0.f) {   // no band: its slot and the border's are never the same
+            positive = 0x10000;
+            negative = 0xfffe;
+            slots = kt - kl + 1;
+        } else for (;; bits += 128) {
             positive = 0x8000 + bits;       // the least key above the band
             negative = 0x7fff - bits;       // the largest below it
             slots = kt - kl + 1;
@@ -494,7 +504,7 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
             else if (kl < positive) slots = kt - positive + 2;
             if (slots <= SP_BINS || positive > kt) break;
         }
-        if (quick && k <= 0 && by_p && slots <= SP_BINS && positive <= kt) {
+        if (quick && k <= 0 && by_p && slots <= SP_BINS && (positive <= kt || top < 0.f)) {
             const int shut = positive - negative - 2;   // keys that the band closes up
             const int band = kt - positive + 1;         // its slot
             auto slot_of = [&](T z) -> int {            // less than 0, or `slots` and more: of those that weigh nothing (NaN, -inf)

@@ -240,3 +240,17 @@ def test_sessions_draw():
     greedy, cold, one, hot = run(None, S(temperature=0.0), S(temperature=5.0, top_k=1), S(temperature=3.0, seed=1))
     assert greedy == cold == one and hot != greedy
     assert run(S(temperature=3.0, seed=1))[0] == hot and run(S(temperature=3.0, seed=2))[0] != hot
+
+
+@pytest.mark.parametrize("vocab", [700, 20000, 128256])
+@pytest.mark.parametrize("least", [0.0, 0.03])
+def test_top_p_over_logits_of_all_kinds(vocab, least):
+    """Log-probabilities, logits next to zero and about it, far from it, few that differ: what top-p keeps ends on ties, near zero, or anywhere."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    n = lambda: torch.randn(vocab, generator=g, device="cuda")  # noqa: E731
+    few = torch.zeros(vocab, device="cuda")
+    few[:5] = torch.tensor([4.0, 3.0, 2.0, 1.0, -1.0])
+    z = torch.stack([torch.log_softmax(3 * n(), 0), n() * 1e-6, n() * 1e-3, few + n() * 1e-30, few - 1e-5, (3 * n()).round(), 300 * n(), 1000 + n(), -1000 - n().abs(), -n().abs() * 1e-20, n() - 7.0, few * 20]).to(BF)
+    rows = z.shape[0]
+    for p, T in ((0.9, 1.0), (0.5, 0.7), (0.99, 3.0), (0.2, 1.0), (0.9999, 1.0)):
+        check(z, torch.rand(rows, generator=torch.Generator().manual_seed(vocab + int(100 * p))).tolist(), [T] * rows, None, [p] * rows, [least] * rows)
