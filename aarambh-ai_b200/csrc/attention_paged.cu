@@ -12,7 +12,8 @@
 // then joined to the others', which rounds once a tile.  500 tokens behind 1000, 16 / 4 heads of 128: 170 us, 30 TFLOP/s, by tiles of 64 rows, whose scores
 // load 16 bytes from shared memory eight times for 64 multiplications; by tiles of 32, six times for 32, 229.  Three rows of up to 130 tokens behind 380,
 // 6 / 2 heads of 64: 22.4 us (a kernel of 18 and a merge of 7 by
-// themselves, before a launch was set up while the one before it ended).
+// themselves, before a launch was set up while the one before it ended); through a window of 100 with 5 first tokens 18.1.  Codes (e4m3) come two tiles ahead and are made floats, times
+// their scales, a tile at a time: 500 behind 1000 185 us for 170; 48 rows of up to 8191, 16 / 4 heads of 64, 161 us, bound like f32 pages by loads from shared memory.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -29,7 +30,9 @@ int paged_tc_attention(const PagedAttnArgs &a, int hd, void *workspace, size_t b
 // single tokens, us by two launches and by one: 32 / 8 heads of 128, 32 rows behind 500 65 and 56, behind 4000 168 and 163, behind 16000 487 and 559; 64 rows 82 and 80,
 // 247 and 274; 16 / 1 heads of 128, 128 rows behind 500 57 and 40, behind 4000 118 and 98; 16 / 4 heads of 64, 16 rows behind 500 43 and 29, behind 4000 61 and 62, behind 16000
 // 141 and 178, 32 rows 42 and 33, 80 and 90, 180 and 284.
-constexpr int paged_few_items(int hd) { return hd == 128 ? 256 : 64; }
+// Over codes a single token's own kernel reads half, and a tile costs more: 32 / 8 heads of 128, 4 rows behind 500 55 and 42, behind 4000 93 and 89, behind 16000 224 and 244; 8 rows
+// 56 and 48, 107 and 114, 247 and 329; 16 rows 56 and 57, 123 and 155, 291 and 485; 16 / 4 heads of 64, 8 rows 47 and 35, 63 and 63, 121 and 167, 16 rows 48 and 36, 67 and 85, 149 and 255.
+constexpr int paged_few_items(int hd, bool codes) { return (hd == 128 ? 256 : 64) / (codes ? hd == 128 ? 4 : 2 : 1); }
 constexpr int PAGED_FEW_ROWS = 16;   // query rows of a KV head up to which the tensor-memory kernel's tiles of 128 would be nearly empty
 namespace {
 
@@ -458,7 +461,7 @@ static int paged_attend(const ab2_paged *cache, const float *k_scales_dev, const
     if (dtype == AB2_F32) return simt_attention(a, cache->head_dim, max_new, workspace_dev, workspace_bytes, (cudaStream_t)stream);
     // Rows of up to 16 query rows a KV head go to the warp-level kernel, the others to the tensor-memory kernel; a launch for which there can be no row is
     // left out.  Rows with more new tokens than they were said to have are served all the same.
-    const bool chunks = (long long)max_new * a.plan.group > PAGED_FEW_ROWS, few = a.plan.group <= PAGED_FEW_ROWS && !(chunks && (long long)cache->rows * cache->kv_heads <= paged_few_items(cache->head_dim));
+    const bool chunks = (long long)max_new * a.plan.group > PAGED_FEW_ROWS, few = a.plan.group <= PAGED_FEW_ROWS && !(chunks && (long long)cache->rows * cache->kv_heads <= paged_few_items(cache->head_dim, k_scales_dev));
     if (few) {
         if (chunks) a.plan.most = PAGED_FEW_ROWS;
         rc = paged_mma_attention(a, cache->head_dim, max_new, workspace_dev, workspace_bytes, (cudaStream_t)stream);

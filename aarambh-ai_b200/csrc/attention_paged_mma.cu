@@ -13,7 +13,13 @@
 //
 // 48 rows of up to 8192 tokens, 32 / 8 heads of 128 (1.02 GB): 170 us with the merge, 0.92 of a copy's rate (on CUDA cores 672); 2 x 100000 128 to 138 us
 // (0.89 to 0.83 by the card).  1 x 700: 10.3 to 10.9 us (12.3 to 12.7 before a launch was set up while the one before it ended), a kernel of 8 and a merge of 4.3 by themselves:
-// latency.  A merge by fewer CTAs, each for the cuts of several runs, took 80 us for 41 at 1 x 32000: cuts lie evenly apart, and met in the same CTAs.
+// latency.  Through a window of 2048 with 4 first tokens, 32 rows of 30000: 55 us, 0.75 of a copy's rate.
+//
+// Over codes (e4m3) a code is an f16 number as it is, and products are of f16: queries times a power of two of their row's that brings the largest to 2^14 to 2^15 (exact but for
+// elements below 2^-28 of it), a block's scale of keys on its scores, its scale of values on its weights, relative to `vref`, a scale that moves as the maximum does.
+// Weights have one f16 term (2^-11): the output's rounding is 2^-8, and the conversions leave the pipes no time for a second.  48 rows of up to 8192: 94 us,
+// 0.83 of a copy's rate for half the bytes (bf16 pages 164); 2 x 100000 73; 64 rows of 12000 through a window of 1024, 16 / 4 heads, 26.5; 1 x 700: 10.7.
+// A merge by fewer CTAs, each for the cuts of several runs, took 80 us for 41 at 1 x 32000: cuts lie evenly apart, and met in the same CTAs.
 #include <algorithm>
 #include <type_traits>
 

@@ -27,6 +27,15 @@
 // them 0.96 for 0.91.  Forms before this one: tiles of 128 keys with the weights over the scores (a chain of scores, softmax and sums) 0.98 to 1.02;
 // an MMA warp a tile there, weights handed over in two or four parts, 1.08 and 1.11; tiles of 64 with two places for weights 1.17, with registers spilled.
 //
+// Over codes (e4m3 pages, 512 threads; see PcUnit for the numbers):
+//   warp 0       producer: values as codes by bulk copies to a ring of their own, keys by TMA as the operand of an e4m3 product, with queries in two terms
+//   warps 4-11   softmax, with the scales of keys on the scores and of values on the weights (f16)
+//   warps 12-15  values from codes to f16, in the ring's slots
+// 4096 behind 12288 1.00 ms (bf16 pages 0.81 to 0.87), six mixed rows 177 to 200 us (124 to 147), 1024 behind 1024 64 (51); through a window of 1024 8000 tokens of 16 / 4 heads behind 5000 230 (158).
+// What it costs more, by copies that leave a part out: making values f16 45 us of 4096 behind 12288, the scales in the softmax 30 or so; the rest is not taken apart.
+// Measured and not kept there: queries in one term (no faster, 2^-4), keys and values both made f16 by warps (1465 us; 1153 with the scales beside the softmax's), values loaded to
+// registers a tile ahead and converted by unrolled code (1150: its text drives the softmax's out of the instruction cache), the next tile's table and scales asked for ahead (no change).
+//
 // An MMA multiplies a hidden value by a weight of 0, so an Inf or a NaN there would reach rows that do not see it.  Rows of a page behind the
 // sequence's end are cleared in shared memory; a row whose sums come out as Inf or NaN (a later token's value may hold them) is computed
 // again on CUDA cores over the keys in its sight, behind all pieces of the CTA, so that no bounded wait lasts as long as that.  Every wait on an mbarrier is bounded; on a time-out the CTA records AB2_ERR_TIMEOUT and
@@ -396,7 +405,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const uint32_t tmem = sh.tmem_base, tmem_o = tmem + 256;   // a tile of rows has 128 columns for scores and weights
     const PagedView &p = a.plan.p;
     PcPiece x;
-    // the block's registers: 128 threads of 72 and 256 of 216 are the 384 of 168 that it was launched with
+    // the block's registers: 128 threads of 72 and 256 of 216 are the 384 of 168 that it was launched with (over codes PC_FEW_REGS and the others of 128)
     if (E8 && warp >= PC_THREADS / 32) {
         // ---------------------------------------------------------- values from codes
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PC_LOAD_REGS));

@@ -469,7 +469,7 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     kernels, whose results differ by rounding.  Over bf16 a softmax weight keeps 16 bits where a row's new tokens times the query heads of a KV head are
     at most 16, and 8 where they are more.  Tokens behind the last row are left as ``out`` (not q) holds them.
 
-    ``scales``: of pages of 8 bits, as in ``paged_append``; a weight keeps 11 bits there, or 8.  With a ``window`` a token sees its row's last so many keys, its own
+    ``scales``: of pages of 8 bits, as in ``paged_append`` (finite, not negative); a weight keeps 11 bits there.  With a ``window`` a token sees its row's last so many keys, its own
     among them, and the first ``sinks`` of the row; pages that hold no key in sight of a row's new tokens are not looked at."""
     if out is None and _fast is not None:
         got = _fast.attention(q, k_pages, v_pages, table, lens, scale, starts, max_new, scales, window, sinks)

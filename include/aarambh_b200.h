@@ -410,8 +410,11 @@ int ab2_paged_attention_window(const ab2_paged *cache, int window, int sinks, co
  * most 448, or the scale that it has where it holds earlier tokens and that is larger; where it grows, earlier tokens' codes are made anew from their values.
  * Codes are rounded to nearest, Inf and NaN become NaN.  Codes of slots that hold no token are left as they are.  Pages, scales and all else lie apart.
  *
- * The attention takes scales that are powers of two as they are; of other scales a chunk's values (code times scale) are rounded to bf16.  Over bf16 queries the
- * weights of rows of up to 16 query rows are rounded to f16 (2^-11 each), of more to bf16 (2^-8 each). */
+ * Tokens that are cut off a row leave its last block's scale as they made it, and what their coming rounded off the others' codes.
+ *
+ * The attention reads the scales of blocks that hold keys in sight, finite ones and not negative; those that the append writes are taken as they are, of scales that are not powers of two a
+ * chunk's values are rounded to f16 (2^-11) in units of the largest of some 80 keys.  Over bf16 queries weights are rounded to f16 (2^-11 each); the
+ * queries of chunks (new tokens times query heads of a KV head above 16) enter in two e4m3 terms, off by 2^-17.8 of the row's largest element at most. */
 int ab2_paged_append_e4m3(const ab2_paged *cache, float *k_scales_dev, float *v_scales_dev, const void *k_dev, long long k_stride, const void *v_dev,
                           long long v_stride, const void *q_dev, long long q_stride, int heads, void *q_out_dev, long long q_out_stride,
                           const double *frequencies_dev, int rot_dims, int layout, float magnitude, ab2_dtype dtype, ab2_stream stream);
