@@ -31,7 +31,7 @@
 //   warp 0       producer: values as codes by bulk copies to a ring of their own, keys by TMA as the operand of an e4m3 product, with queries in two terms
 //   warps 4-11   softmax, with the scales of keys on the scores and of values on the weights (f16)
 //   warps 12-15  values from codes to f16, in the ring's slots
-// 4096 behind 12288 1.00 ms (bf16 pages 0.81 to 0.87), six mixed rows 177 to 200 us (124 to 147), 1024 behind 1024 64 (51); through a window of 1024 8000 tokens of 16 / 4 heads behind 5000 230 (158).
+// 4096 behind 12288 0.99 ms (bf16 pages 0.81 to 0.87), six mixed rows 150 us (123), 1024 behind 1024 60 (51); through a window of 1024 8000 tokens of 16 / 4 heads behind 5000 172 (134).
 // What it costs more, by copies that leave a part out: making values f16 45 us of 4096 behind 12288, the scales in the softmax 30 or so; the rest is not taken apart.
 // Measured and not kept there: queries in one term (no faster, 2^-4), keys and values both made f16 by warps (1465 us; 1153 with the scales beside the softmax's), values loaded to
 // registers a tile ahead and converted by unrolled code (1150: its text drives the softmax's out of the instruction cache), the next tile's table and scales asked for ahead (no change).
@@ -145,12 +145,32 @@ template <int SLOTS, int RAWS, int THREADS> struct PcShared {
     PcPiece piece[8][2];
 };
 
-// One tile of keys for the warp's 32 rows, a lane each: scores to weights.  With EDGE keys past `lim` are out of sight, and a lane that is `second` hands on what
-// rounding left of each weight (a kind of its own for that cost the loops around it 5 %).  `before` waits until the
-// products with the tile before are done: its weights' place is free then, and the sums stand still.  WIN: of the tile's keys those from `sinks` up to `since` are
-// hidden too.
-template <int HD, bool EDGE, bool WIN, class Before>
-__device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, int sinks, int since, bool second, bool has_o, float &top, float &sum, uint64_t *taken, uint64_t *ready, Before before) {
+// Of a tile's scores v(0) .. v(PC_KEYS - 1), those out of sight become -inf: past `lim` and, WIN, from `sinks` up to `since`.
+template <bool WIN, class Scores> __device__ __forceinline__ void pc_hide(Scores v, int lim, int sinks, int since) {
+    if constexpr (WIN) {
+        // a bit for each key in sight, 32 at a time
+        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };   // bits of the keys below n
+#pragma unroll
+        for (int w = 0; w < PC_KEYS; w += 32) {
+            const uint32_t seen = below(lim + 1 - w) & (below(sinks - w) | ~below(since - w));
+#pragma unroll
+            for (int k = w; k < w + 32 && k < PC_KEYS; ++k)
+                if (!((seen >> (k - w)) & 1)) v(k) = 0xff800000u;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < PC_KEYS; ++k)
+            if (k > lim) v(k) = 0xff800000u;
+    }
+}
+
+// One tile of keys for the warp's 32 rows, a lane each: scores to weights.  With `edge` some may be out of sight (pc_hide); with `twice` a lane that is `second` hands on
+// what rounding left of each weight.  `before` waits until the products with the tile before are done: its weights' place is free then, and the sums stand still.
+// KIND: 0 of a tile with neither, 1 of one with an edge, 2 of either.  Over codes and through windows one text serves all tiles, with branches around what some need: two
+// drove each other, and all that runs between pieces, out of the instruction cache (six mixed rows over codes 179 us, in one text 150; 8000 tokens through a window of 1024 149 and 134).  Else
+// tiles with an edge have their own: a prompt has few of them, and its long runs of others go by 3.5 % faster (4096 behind 4096 370 for 383).
+template <int HD, bool WIN, int KIND, class Before>
+__device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, bool edge, int lim, int sinks, int since, bool twice, bool second, bool has_o, float &top, float &sum, uint64_t *taken, uint64_t *ready, Before before) {
     uint32_t va[32], vb[32], vc[16];
     tmem_ld32_start(va, s_addr);
     tmem_ld32_start(vb, s_addr + 32);
@@ -166,21 +186,9 @@ __device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, flo
 #pragma unroll
         for (int k = 0; k < PC_KEYS; ++k) v(k) ^= 0x80000000u;
     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    if constexpr (EDGE && WIN) {
-        // a bit for each key in sight, 32 at a time
-        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };   // bits of the keys below n
-#pragma unroll
-        for (int w = 0; w < PC_KEYS; w += 32) {
-            const uint32_t seen = below(lim + 1 - w) & (below(sinks - w) | ~below(since - w));
-#pragma unroll
-            for (int k = w; k < w + 32 && k < PC_KEYS; ++k)
-                if (!((seen >> (k - w)) & 1)) v(k) = 0xff800000u;
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < PC_KEYS; ++k)
-            if (EDGE && k > lim) v(k) = 0xff800000u;
-    }
+    edge = KIND == 2 ? edge : KIND == 1;
+    twice &= KIND != 0;
+    if (edge) pc_hide<WIN>(v, lim, sinks, since);
 #pragma unroll
     for (int k = 0; k < PC_KEYS; k += 8)
 #pragma unroll
@@ -210,24 +218,30 @@ __device__ __forceinline__ void pc_softmax(uint32_t s_addr, uint32_t o_addr, flo
         const uint64_t e = ex2_pair(fma2(pair(__uint_as_float(v(k)), __uint_as_float(v(k + 1))), sl2, top2));
         total[(k >> 1) & 1] = add2(total[(k >> 1) & 1], e);
         const __nv_bfloat162 b = __floats2bfloat162_rn(low(e), high(e));
-        uint32_t word = *reinterpret_cast<const uint32_t *>(&b);
-        if (EDGE) {
-            const __nv_bfloat162 left = __floats2bfloat162_rn(low(e) - __uint_as_float(word << 16), high(e) - __uint_as_float(word & 0xffff0000u));
-            if (second) word = *reinterpret_cast<const uint32_t *>(&left);
-        }
-        return word;
+        return *reinterpret_cast<const uint32_t *>(&b);
+    };
+    auto rest = [&](int k, uint32_t word) {
+        const uint64_t e = ex2_pair(fma2(pair(__uint_as_float(v(k)), __uint_as_float(v(k + 1))), sl2, top2));
+        const __nv_bfloat162 left = __floats2bfloat162_rn(low(e) - __uint_as_float(word << 16), high(e) - __uint_as_float(word & 0xffff0000u));
+        return second ? *reinterpret_cast<const uint32_t *>(&left) : word;
     };
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         uint32_t p[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) p[k] = weights(32 * c + 2 * k);
+        if (twice)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) p[k] = rest(32 * c + 2 * k, p[k]);
         tmem_st16(s_addr + PC_KEYS + 16 * c, p);
     }
     {
         uint32_t p[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) p[k] = weights(64 + 2 * k);
+        if (twice)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) p[k] = rest(64 + 2 * k, p[k]);
         tmem_st8(s_addr + PC_KEYS + 32, p);
     }
     total[0] = add2(total[0], total[1]);
@@ -262,8 +276,8 @@ constexpr float PC_UP = 32.f, PC_MORE = 4.f, PC_LESS = 9.765625e-4f, PC_APART = 
 struct PcUnit {
     float vref, last, more, less;
 };
-template <int HD, bool EDGE, bool WIN, class Before>
-__device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_addr, float sl, bool flip, int lim, int sinks, int since, const PcTile &of, bool has_o, float &top, float &sum, PcUnit &unit,
+template <int HD, bool WIN, class Before>
+__device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_addr, float sl, bool edge, int lim, int sinks, int since, const PcTile &of, bool has_o, float &top, float &sum, PcUnit &unit,
                                                  uint64_t *taken, uint64_t *ready, Before before) {
     constexpr int BLOCKS = PC_KEYS / PC_ROWS;
     uint32_t va[32], vb[32], vc[16];
@@ -282,23 +296,7 @@ __device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_add
     __syncwarp();
     if ((threadIdx.x & 31) == 0) bar_arrive(taken);
     auto v = [&](int k) -> uint32_t & { return k < 32 ? va[k] : k < 64 ? vb[k - 32] : vc[k - 64]; };
-    if (flip)   // a negative scale
-#pragma unroll
-        for (int k = 0; k < PC_KEYS; ++k) v(k) ^= 0x80000000u;
-    if constexpr (EDGE && WIN) {
-        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };   // bits of the keys below n
-#pragma unroll
-        for (int w = 0; w < PC_KEYS; w += 32) {
-            const uint32_t seen = below(lim + 1 - w) & (below(sinks - w) | ~below(since - w));
-#pragma unroll
-            for (int k = w; k < w + 32 && k < PC_KEYS; ++k)
-                if (!((seen >> (k - w)) & 1)) v(k) = 0xff800000u;
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < PC_KEYS; ++k)
-            if (EDGE && k > lim) v(k) = 0xff800000u;
-    }
+    if (edge) pc_hide<WIN>(v, lim, sinks, since);
     float best = -INFINITY;
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) {
@@ -614,7 +612,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const PagedSpan s = x.s;
             const long long first = x.w.r.first + s.t0, head0 = x.w.head * group;
             if constexpr (E8) {   // every warp its own rows, which it makes codes where they come to lie
-#pragma unroll
+#pragma unroll 2   // short text: the instruction cache has all of a piece to hold (through a window of 128 unrolled 81 us, by 4 73, so 71)
                 for (int u = 0; u < HD / 8; ++u) {
                     const int i = lane + 32 * u, d = i % (HD / 8), row = quad * 32 + i / (HD / 8), rr = g * PC_Q + row, in = rr < s.ntok * group ? 16 : 0, tok = paged_token(a.plan, in ? rr : 0);
                     const __nv_bfloat16 *src = (const __nv_bfloat16 *)a.q + (first + tok) * a.q_stride + (head0 + (in ? rr - tok * group : 0)) * HD + d * 8;
@@ -625,7 +623,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
             const int i0 = threadIdx.x & 127, rows = s.ntok * group;
             const bool twice = rows <= PC_TWICE;
-#pragma unroll
+#pragma unroll 2   // short text: the instruction cache has all of a piece to hold (through a window of 128 unrolled 81 us, by 4 73, so 71)
             for (int u = 0; u < PC_Q * HD / 8 / 128; ++u) {
                 const int i = i0 + 128 * u, d = i % (HD / 8), row = i / (HD / 8), rr = twice && row < 2 * PC_TWICE ? row % PC_TWICE : g * PC_Q + row, in = rr < rows ? 16 : 0, tok = paged_token(a.plan, in ? rr : 0);
                 const __nv_bfloat16 *src = (const __nv_bfloat16 *)a.q + (first + tok) * a.q_stride + (head0 + (in ? rr - tok * group : 0)) * HD + d * 8;
@@ -646,7 +644,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             // times 2^(127 - down) the largest is between 224 and 448 = 1.75 2^8
             const uint32_t bits = __float_as_uint(most);
             const int down = min(max((int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u), 1), 253);
-            const float f = most < INFINITY ? __uint_as_float((uint32_t)(254 - down) << 23) : __uint_as_float(0x7fc00000u);   // Inf has no code
+            const float f = most < INFINITY ? __uint_as_float((uint32_t)(254 - down) << 23 | (flip ? 0x80000000u : 0u)) : __uint_as_float(0x7fc00000u);   // Inf has no code
             back = __uint_as_float((uint32_t)down << 23);
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i) {
@@ -715,13 +713,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 const int lim = min(pos, hi - 1) - at, low = WIN ? pos + 1 - a.plan.window - at : 0;
                 auto before = [&] { if (j > 0) warp_wait(&sh.odone[g], (scored - 1) & 1, failed); };
                 const bool edge = at + PC_KEYS - 1 > least || at + PC_KEYS > hi || (g + 1) * PC_Q > rows || (WIN && at < late && at + PC_KEYS > a.plan.sinks);
-                if constexpr (E8) {
-                    const PcTile &tile = sh.tiles[(slot0 + j) % TILES];
-                    if (edge) pc_softmax_codes<HD, true, WIN>(s_addr, o_addr, row_sl, flip, lim, WIN ? a.plan.sinks - at : 0, low, tile, j > 0, top, sum, unit, &sh.sfree[g], &sh.pfull[g], before);
-                    else pc_softmax_codes<HD, false, WIN>(s_addr, o_addr, row_sl, flip, lim, 0, 0, tile, j > 0, top, sum, unit, &sh.sfree[g], &sh.pfull[g], before);
-                } else if (edge)
-                    pc_softmax<HD, true, WIN>(s_addr, o_addr, sl, flip, lim, WIN ? a.plan.sinks - at : 0, low, second, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
-                else pc_softmax<HD, false, WIN>(s_addr, o_addr, sl, flip, lim, 0, 0, false, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
+                const int sinks = WIN ? a.plan.sinks - at : 0;
+                if constexpr (E8) pc_softmax_codes<HD, WIN>(s_addr, o_addr, row_sl, edge, lim, sinks, low, sh.tiles[(slot0 + j) % TILES], j > 0, top, sum, unit, &sh.sfree[g], &sh.pfull[g], before);
+                else if constexpr (WIN) pc_softmax<HD, true, 2>(s_addr, o_addr, sl, flip, edge, lim, sinks, low, twice, second, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
+                else if (edge) pc_softmax<HD, false, 1>(s_addr, o_addr, sl, flip, true, lim, 0, 0, twice, second, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
+                else pc_softmax<HD, false, 0>(s_addr, o_addr, sl, flip, false, lim, 0, 0, false, false, j > 0, top, sum, &sh.sfree[g], &sh.pfull[g], before);
             }
             const float of_sums = E8 ? unit.vref * (1.f / PC_UP) : 1.f;
             // the scores are all made: the next piece's queries may take the place of these, while the sums go out
