@@ -10,8 +10,10 @@
 // A CTA has a block's new tokens (or, where blocks are few, a part of their heads): it turns their angles once into shared memory, and each warp takes heads of q,
 // k and v one after the other.  A block's scale is its warp's alone: no atomics, no order.  Heads of keys and values stay in registers from the load to the codes.
 //
-// Bound by HBM for prompts: five prompts of up to 2001 tokens, 16 / 4 heads of 128 (66 MB), 18 us, 3.7 TB/s; one of 8192, 32 / 8 heads, 55, 3.4 (a launch of nothing is 4 of it; the rest was not taken apart).  Single tokens by latency: 64 of 32 / 8 heads 7.8 us, one 4.8.
+// Bound by HBM for prompts, and by the instructions of a block: five of up to 2001 tokens, 16 / 4 heads of 128 (66 MB), 20 us, 3.3 TB/s; one of 8192, 32 / 8 heads, 55, 3.4; issue
+// slots are 44 % busy, and shared memory and registers hold four CTAs on an SM.  Single tokens by latency: 64 of 32 / 8 heads 4.8 us, one 3.4.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -64,7 +66,7 @@ __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) 
 // HALF: pairs (i, i + n); WIDE: two elements of a lane lie side by side on their boundary, else they are taken one by one.
 template <typename T, int HD, bool HALF, bool WIDE>
 __global__ void __launch_bounds__(32 * A8_WARPS, 4) append8_kernel(const __grid_constant__ Append8Args a) {
-    constexpr int LANES = HD / 4, AT_ONCE = 32 / LANES, STEPS = PAGED_BLOCK / AT_ONCE;   // lanes of a token's head, tokens a warp has at once
+    constexpr int LANES = HD / 4, AT_ONCE = 32 / LANES;   // lanes of a token's head, tokens a warp has at once
     __shared__ float2 turns[PAGED_BLOCK][HD / 2];
     __shared__ unsigned long long per_position[HD / 2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -103,115 +105,123 @@ __global__ void __launch_bounds__(32 * A8_WARPS, 4) append8_kernel(const __grid_
     auto first_of = [&](int pair, bool turned) { return HALF && turned && pair < a.pairs ? pair : 2 * pair; };
     auto second_of = [&](int pair, bool turned) { return HALF && turned && pair < a.pairs ? pair + a.pairs : 2 * pair + 1; };
     const int tasks = a.heads + 2 * p.kv_heads;
-    for (int task = blockIdx.y * A8_WARPS + warp; task < tasks; task += a.parts * A8_WARPS) {
-        const bool is_q = task < a.heads, is_v = task >= a.heads + p.kv_heads, turned = !is_v;
-        const int head = is_q ? task : (task - a.heads) % p.kv_heads;
-        if (!is_q && !kept) continue;
-        const long long stride = is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride;
-        const T *src = (const T *)(is_q ? a.q : is_v ? a.v : a.k) + t0 * stride + head * HD;
-        const int x0 = first_of(p0, turned), y0 = second_of(p0, turned), x1 = first_of(p0 + 1, turned), y1 = second_of(p0 + 1, turned);
-        // with WIDE the two pairs are of one kind: (x0 x1 | y0 y1) of halves, (x0 y0 | x1 y1) otherwise
-        const bool halves = HALF && turned && p0 < a.pairs;
-        const int o0 = x0, o1 = halves ? x1 : y0, o2 = halves ? y0 : x1, o3 = y1;
-        Two<T> u[STEPS], w[STEPS];
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const int t = i * AT_ONCE + sub;
-            u[i].set(0.f, 0.f);
-            w[i].set(0.f, 0.f);
-            if (t >= n) continue;
-            const T *from = src + t * stride;
-            if (WIDE) {
-                u[i].load(from + o0);
-                w[i].load(from + o2);
-            } else {
-                u[i].load(from + o0, from + o1);
-                w[i].load(from + o2, from + o3);
-            }
-        }
-        if (turned) {
+    // The heads of this warp, with room for `steps` tokens a lane.
+    auto heads = [&](auto steps) {
+        constexpr int STEPS = decltype(steps)::value;
+        for (int task = blockIdx.y * A8_WARPS + warp; task < tasks; task += a.parts * A8_WARPS) {
+            const bool is_q = task < a.heads, is_v = task >= a.heads + p.kv_heads, turned = !is_v;
+            const int head = is_q ? task : (task - a.heads) % p.kv_heads;
+            if (!is_q && !kept) continue;
+            const long long stride = is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride;
+            const T *src = (const T *)(is_q ? a.q : is_v ? a.v : a.k) + t0 * stride + head * HD;
+            const int x0 = first_of(p0, turned), y0 = second_of(p0, turned), x1 = first_of(p0 + 1, turned), y1 = second_of(p0 + 1, turned);
+            // with WIDE the two pairs are of one kind: (x0 x1 | y0 y1) of halves, (x0 y0 | x1 y1) otherwise
+            const bool halves = HALF && turned && p0 < a.pairs;
+            const int o0 = x0, o1 = halves ? x1 : y0, o2 = halves ? y0 : x1, o3 = y1;
+            Two<T> u[STEPS], w[STEPS];
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) {
                 const int t = i * AT_ONCE + sub;
+                u[i].set(0.f, 0.f);
+                w[i].set(0.f, 0.f);
                 if (t >= n) continue;
-                float2 e = u[i].floats(), f = w[i].floats();
-                auto turn = [&](float &x, float &y, int pair) {
-                    if (pair >= a.pairs) return;
-                    const float2 cs = turns[t][pair];
-                    const float s = x, v = y;
-                    x = s * cs.x - v * cs.y;
-                    y = s * cs.y + v * cs.x;
-                };
-                if (halves) {
-                    turn(e.x, f.x, p0);
-                    turn(e.y, f.y, p0 + 1);
-                } else {
-                    turn(e.x, e.y, p0);
-                    turn(f.x, f.y, p0 + 1);
-                }
-                u[i].set(e.x, e.y);
-                w[i].set(f.x, f.y);
-            }
-        }
-        if (is_q) {
-            T *dst = (T *)a.qo + t0 * a.qo_stride + head * HD;
-#pragma unroll
-            for (int i = 0; i < STEPS; ++i) {
-                const int t = i * AT_ONCE + sub;
-                if (t >= n) continue;
-                T *to = dst + t * a.qo_stride;
+                const T *from = src + t * stride;
                 if (WIDE) {
-                    u[i].store(to + o0);
-                    w[i].store(to + o2);
+                    u[i].load(from + o0);
+                    w[i].load(from + o2);
                 } else {
-                    u[i].store(to + o0, to + o1);
-                    w[i].store(to + o2, to + o3);
+                    u[i].load(from + o0, from + o1);
+                    w[i].load(from + o2, from + o3);
                 }
             }
-            continue;
-        }
-        float most = 0.f;
+            if (turned) {
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const float2 e = u[i].floats(), f = w[i].floats();
-            for (float x : {e.x, e.y, f.x, f.y}) most = is_finite(x) ? fmaxf(most, fabsf(x)) : most;
-        }
+                for (int i = 0; i < STEPS; ++i) {
+                    const int t = i * AT_ONCE + sub;
+                    if (t >= n) continue;
+                    float2 e = u[i].floats(), f = w[i].floats();
+                    auto turn = [&](float &x, float &y, int pair) {
+                        if (pair >= a.pairs) return;
+                        const float2 cs = turns[t][pair];
+                        const float s = x, v = y;
+                        x = s * cs.x - v * cs.y;
+                        y = s * cs.y + v * cs.x;
+                    };
+                    if (halves) {
+                        turn(e.x, f.x, p0);
+                        turn(e.y, f.y, p0 + 1);
+                    } else {
+                        turn(e.x, e.y, p0);
+                        turn(f.x, f.y, p0 + 1);
+                    }
+                    u[i].set(e.x, e.y);
+                    w[i].set(f.x, f.y);
+                }
+            }
+            if (is_q) {
+                T *dst = (T *)a.qo + t0 * a.qo_stride + head * HD;
 #pragma unroll
-        for (int m = 16; m > 0; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
-        const uint32_t bits = __float_as_uint(most);
-        const int e = max((int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u), A8_LEAST);   // 448 = 1.75 2^8
-        const size_t slot0 = ((((size_t)id * p.kv_heads + head) << p.page_shift) + (size_t)(pos0 & ((1 << p.page_shift) - 1))) - skip;   // the block's first token
-        float *scales = (is_v ? a.vs : a.ks) + slot0 / PAGED_BLOCK;
-        uint8_t *codes = (is_v ? a.vp : a.kp) + slot0 * HD;
-        const float need = __uint_as_float((uint32_t)(e + 127) << 23), old = skip ? *scales : 0.f, scale = fmaxf(need, old), inverse = 1.f / scale;
-        __syncwarp();
-        if (lane == 0) *scales = scale;
-        if (skip && old < scale) {   // earlier tokens' codes in units of the new scale
-            const float f = old * inverse;
-            for (int t = sub; t < skip; t += AT_ONCE) {
-                uint32_t *at = reinterpret_cast<uint32_t *>(codes + t * HD + 2 * p0);
-                const float2 lo = floats_of_codes(*at), hi = floats_of_codes(*at >> 16);
-                *at = codes_of(lo.x * f, lo.y * f) | codes_of(hi.x * f, hi.y * f) << 16;
+                for (int i = 0; i < STEPS; ++i) {
+                    const int t = i * AT_ONCE + sub;
+                    if (t >= n) continue;
+                    T *to = dst + t * a.qo_stride;
+                    if (WIDE) {
+                        u[i].store(to + o0);
+                        w[i].store(to + o2);
+                    } else {
+                        u[i].store(to + o0, to + o1);
+                        w[i].store(to + o2, to + o3);
+                    }
+                }
+                continue;
+            }
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) {
+                const float2 e = u[i].floats(), f = w[i].floats();
+                for (float x : {e.x, e.y, f.x, f.y}) most = is_finite(x) ? fmaxf(most, fabsf(x)) : most;
+            }
+#pragma unroll
+            for (int m = 16; m > 0; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
+            const uint32_t bits = __float_as_uint(most);
+            const int e = max((int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u), A8_LEAST);   // 448 = 1.75 2^8
+            const size_t slot0 = ((((size_t)id * p.kv_heads + head) << p.page_shift) + (size_t)(pos0 & ((1 << p.page_shift) - 1))) - skip;   // the block's first token
+            float *scales = (is_v ? a.vs : a.ks) + slot0 / PAGED_BLOCK;
+            uint8_t *codes = (is_v ? a.vp : a.kp) + slot0 * HD;
+            const float need = __uint_as_float((uint32_t)(e + 127) << 23), old = skip ? *scales : 0.f, scale = fmaxf(need, old), inverse = 1.f / scale;
+            __syncwarp();
+            if (lane == 0) *scales = scale;
+            if (skip && old < scale) {   // earlier tokens' codes in units of the new scale
+                const float f = old * inverse;
+                for (int t = sub; t < skip; t += AT_ONCE) {
+                    uint32_t *at = reinterpret_cast<uint32_t *>(codes + t * HD + 2 * p0);
+                    const float2 lo = floats_of_codes(*at), hi = floats_of_codes(*at >> 16);
+                    *at = codes_of(lo.x * f, lo.y * f) | codes_of(hi.x * f, hi.y * f) << 16;
+                }
+            }
+            codes += skip * HD;
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) {
+                const int t = i * AT_ONCE + sub;
+                if (t >= n) continue;
+                auto code = [&](float x) { return is_finite(x) ? x * inverse : __uint_as_float(0x7fc00000u); };
+                const float2 e = u[i].floats(), f = w[i].floats();
+                const uint32_t c0 = codes_of(code(e.x), code(e.y)), c1 = codes_of(code(f.x), code(f.y));
+                uint8_t *to = codes + t * HD;
+                if (WIDE) {
+                    *reinterpret_cast<uint16_t *>(to + o0) = (uint16_t)c0;
+                    *reinterpret_cast<uint16_t *>(to + o2) = (uint16_t)c1;
+                } else {
+                    to[o0] = (uint8_t)c0; to[o1] = (uint8_t)(c0 >> 8);
+                    to[o2] = (uint8_t)c1; to[o3] = (uint8_t)(c1 >> 8);
+                }
             }
         }
-        codes += skip * HD;
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const int t = i * AT_ONCE + sub;
-            if (t >= n) continue;
-            auto code = [&](float x) { return is_finite(x) ? x * inverse : __uint_as_float(0x7fc00000u); };
-            const float2 e = u[i].floats(), f = w[i].floats();
-            const uint32_t c0 = codes_of(code(e.x), code(e.y)), c1 = codes_of(code(f.x), code(f.y));
-            uint8_t *to = codes + t * HD;
-            if (WIDE) {
-                *reinterpret_cast<uint16_t *>(to + o0) = (uint16_t)c0;
-                *reinterpret_cast<uint16_t *>(to + o2) = (uint16_t)c1;
-            } else {
-                to[o0] = (uint8_t)c0; to[o1] = (uint8_t)(c0 >> 8);
-                to[o2] = (uint8_t)c1; to[o3] = (uint8_t)(c1 >> 8);
-            }
-        }
-    }
+    };
+    // Single tokens have a text of their own: the block's unrolled one has to come to the instruction cache first, and took 7.8 us for 4.8 (64 rows, 32 / 8 heads; 512 rows
+    // 28 for 10.8; five prompts 18.4 for 20.0).
+    if (n <= AT_ONCE) heads(std::integral_constant<int, 1>{});
+    else heads(std::integral_constant<int, PAGED_BLOCK / AT_ONCE>{});
 }
 
 template <typename T, int HD>
@@ -253,7 +263,7 @@ AB2_API int ab2_paged_append_e4m3(const ab2_paged *cache, float *k_scales_dev, f
     AB2_REQUIRE(slots < (1ll << 31), AB2_ERR_BAD_SHAPE, "%d tokens of %d rows are more than one launch takes", cache->tokens, cache->rows);
     a.slots = (int)slots;
     // A CTA has all heads of a block where there are blocks enough for four CTAs on every SM, else fewer: a head a warp at least.  Sharing a block out makes its angles
-    // anew in every CTA: for 4, 8 and 16 CTAs on an SM, us, five prompts of 5984 tokens 18.5, 17.7, 19.9, one of 8192 55, 56, 60, 512 single tokens 28.4, 28.9, 30.2.
+    // anew in every CTA: for 4 and 8 CTAs on an SM, us, five prompts of up to 2001 tokens 20.0 and 19.0, one of 8192 54.6 and 55.9.
     const int tasks = heads + 2 * cache->kv_heads, most = (tasks + A8_WARPS - 1) / A8_WARPS;
     const long long filled = std::max(1ll, cache->starts ? std::min<long long>(slots, cache->tokens / PAGED_BLOCK + cache->rows) : slots);
     a.parts = (int)std::min<long long>(std::min(most, 65535), std::max(1ll, (4ll * device_sm_count() + filled - 1) / filled));
