@@ -155,3 +155,37 @@ def test_two_recorded_calls_have_workspaces_of_their_own():
     for (g, out), w in zip(graphs, want):
         assert torch.equal(out, w)
     assert pkg().device_status() == 0
+
+
+def test_pages_behind_four_gigabytes():
+    """Pages whose codes lie 2^32 bytes and more behind the pool's beginning, for the append and for every kernel of attention."""
+    p, page, kv, dim = pkg(), 256, 8, 128
+    pages = (2 ** 32 + 2 ** 29) // (page * kv * dim)
+    pools, scales = [[torch.empty((pages, kv, page, dim), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2)], [torch.empty((pages, kv, page // 16), device="cuda") for _ in range(2)]]
+    for dtype, new, window in ((BF, [1, 1], 0), (BF, [90, 1], 0), (BF, [90, 1], 300), (F32, [1, 40], 0)):
+        b = LongBatch([700, 400], new, 32, kv, dim, page, dtype, True, window, 4 if window else 0, hide=False)
+        ref, tol = b.expected()
+        for big, small in zip(pools, (b.k_pages, b.v_pages)):
+            big.view(torch.uint8)[-small.shape[0]:] = small.view(torch.uint8)
+        for big, small in zip(scales, b.scales):
+            big[-small.shape[0]:] = small
+        shift = pages - b.k_pages.shape[0]
+        b.table += shift
+        b.k_pages, b.v_pages = pools
+        b.scales = tuple(scales)
+        held(b.run(p), ref, tol)
+        assert p.device_status() == 0
+        k = torch.randn(sum(new), kv, dim, device="cuda").to(dtype)
+        low = [torch.zeros(b.k_pages.shape[0] - shift, kv, page, dim, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2)]
+        low_scales = [torch.zeros(low[0].shape[0], kv, page // 16, device="cuda") for _ in range(2)]
+        for big in pools:
+            big.view(torch.uint8)[shift:] = 0
+        for big in scales:
+            big[shift:] = 0
+        p.dispatch.paged_append(*low, k, 2 * k, b.table - shift, b.lens_dev, b.starts, scales=tuple(low_scales))
+        p.dispatch.paged_append(*pools, k, 2 * k, b.table, b.lens_dev, b.starts, scales=tuple(scales))
+        assert p.device_status() == 0
+        for big, small in zip(pools, low):
+            assert torch.equal(big.view(torch.uint8)[shift:], small.view(torch.uint8))
+        for big, small in zip(scales, low_scales):
+            assert torch.equal(big[shift:], small)
