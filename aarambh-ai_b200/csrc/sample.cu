@@ -16,7 +16,7 @@
 //
 // Bound by its passes over the slice: instructions, not HBM, which a row crosses once.  64 rows of 128256 bf16 logits (16.4 MB, 2.5 us at a copy's rate), us: top-k of 50 or min-p 18,
 // unfiltered 28 (a weight a token, some 25 instructions), top-p of 0.9 50, of which counts of logits and the pass that weighs are two (bins of x, weighed twice and masses joined by carries: 103),
-// all kinds of rules in a batch 50; 4 rows of 32000 f32: 7, 10 to 12, 34, 23.  Weights looked up in a table by their logit instead of computed: 49 for 50, and unfiltered 36 for 28 (its reads of 8
+// all kinds of rules in a batch 50; 4 rows of 32000 f32: 7, 10 to 12, 27, 16.  Weights looked up in a table by their logit instead of computed: 49 for 50, and unfiltered 36 for 28 (its reads of 8
 // bytes meet in banks).
 #include <algorithm>
 #include <type_traits>
@@ -299,6 +299,34 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
             for (int j = 0; j < V; ++j) e[j] = i + j < n ? in[i + j] : from_f32<T>(-INFINITY);
         }
     };
+    // The row's counts of the thread's bins, behind a barrier of all.  With 4 CTAs or 8 each adds up its share of the bins first:
+    // all bins read by all CTAs took 35 us for 27.5 (top-p alone, 4 rows of 32000 f32).
+    auto counts_of_row = [&](int (&count)[SP_BINS / SP_THREADS]) {
+        constexpr int B = SP_BINS / SP_THREADS;
+        static_assert(B == 8 && SP_CTAS == 8 && SP_BINS / 4 == 2 * SP_THREADS, "bins of a thread");
+        auto add = [&](int r) {
+            const int4 *from = reinterpret_cast<const int4 *>(cluster.map_shared_rank(sh.counts, r) + tid * B), v = from[0], w = from[1];
+            count[0] += v.x; count[1] += v.y; count[2] += v.z; count[3] += v.w;
+            count[4] += w.x; count[5] += w.y; count[6] += w.z; count[7] += w.w;
+        };
+        if (C >= 4) {
+            const int share = SP_BINS / C, mine = rank * share + tid;
+            int sum[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (i * SP_THREADS < share)
+#pragma unroll 4
+                    for (int r = 0; r < C; ++r) sum[i] += cluster.map_shared_rank(sh.counts, r)[mine + i * SP_THREADS];
+            cluster.sync();   // all have read their shares of the slices' counts: the row's take their place
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (i * SP_THREADS < share) sh.counts[mine + i * SP_THREADS] = sum[i];
+            cluster.sync();
+            add(tid * B / share);
+        } else {
+            for (int r = 0; r < C; ++r) add(r);
+        }
+    };
     // f(logit, index in the slice) of all tokens of the slice that can be drawn
     auto for_slice = [&](auto f) {
         for (int i = tid * V; i < n; i += SP_THREADS * V) {
@@ -533,11 +561,7 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
             in_band = cluster_sum(in_band);
             if (C == 1) __syncthreads();
             int count[B] = {};
-            for (int r = 0; r < C; ++r) {
-                const int4 *from = reinterpret_cast<const int4 *>(cluster.map_shared_rank(sh.counts, r) + tid * B), v = from[0], w = from[1];
-                count[0] += v.x; count[1] += v.y; count[2] += v.z; count[3] += v.w;
-                count[4] += w.x; count[5] += w.y; count[6] += w.z; count[7] += w.w;
-            }
+            counts_of_row(count);
             u64 weights[B], sum = 0;
 #pragma unroll
             for (int j = 0; j < B; ++j) {
@@ -663,11 +687,7 @@ __global__ void __launch_bounds__(SP_THREADS, 1) sample_kernel(const __grid_cons
             constexpr int B = SP_BINS / SP_THREADS;
             int count[B] = {}, sum = 0;
             float lo = 0.f, hi = 0.f, los[B], his[B];
-            for (int r = 0; r < C; ++r) {
-                const int4 *from = reinterpret_cast<const int4 *>(cluster.map_shared_rank(sh.counts, r) + tid * B), v = from[0], w = from[1];
-                count[0] += v.x; count[1] += v.y; count[2] += v.z; count[3] += v.w;
-                count[4] += w.x; count[5] += w.y; count[6] += w.z; count[7] += w.w;
-            }
+            counts_of_row(count);
             static_assert(B == 8, "bins of a thread");
 #pragma unroll
             for (int j = 0; j < B; ++j) {   // in units of the likeliest token's; bin b is of x from (b - 1/2) / SP_PER to (b + 1/2) / SP_PER

@@ -189,3 +189,24 @@ def test_pages_behind_four_gigabytes():
             assert torch.equal(big.view(torch.uint8)[shift:], small.view(torch.uint8))
         for big, small in zip(scales, low_scales):
             assert torch.equal(big[shift:], small)
+
+
+@pytest.mark.parametrize("codes,window", [(True, 0), (True, 90), (False, 90)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("scale", [-0.11, 0.0])
+def test_scales_of_scores_that_are_not_positive(dtype, codes, window, scale):
+    for new in ([1, 1, 1], [90, 3, 260]):
+        b = LongBatch([400, 90, 700], new, 8, 2, 128, 32, dtype, codes, window, 5 if window else 0, seed=9)
+        b.scale = scale
+        ref, tol = b.expected()
+        held(b.run(pkg()), ref, tol)
+
+
+def test_many_rows_draw():
+    """More rows than CTAs at once, a cluster of one CTA each."""
+    z = (2 * torch.randn(3000, 1200, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")).to(BF)
+    u = torch.rand(3000, generator=torch.Generator().manual_seed(4))
+    p = torch.full((3000,), 0.7, device="cuda")
+    got = pkg().dispatch.sample(z, u.cuda(), top_p=p).tolist()
+    for i in range(0, 3000, 37):
+        assert got[i] in allowed(z[i], u[i].double().item(), p=p[i].double().item())
