@@ -10,7 +10,7 @@
 // A CTA has a block's new tokens (or, where blocks are few, a part of their heads): it turns their angles once into shared memory, and each warp takes heads of q,
 // k and v one after the other.  A block's scale is its warp's alone: no atomics, no order.  Heads of keys and values stay in registers from the load to the codes.
 //
-// Bound by HBM for prompts, and by the instructions of a block: five of up to 2001 tokens, 16 / 4 heads of 128 (66 MB), 20 us, 3.3 TB/s; one of 8192, 32 / 8 heads, 55, 3.4; issue
+// Bound by HBM for prompts, and by the instructions of a block: five of up to 2001 tokens, 16 / 4 heads of 128 (66 MB), 18.4 us, 3.6 TB/s; one of 8192, 32 / 8 heads, 55, 3.4; issue
 // slots are 44 % busy, and shared memory and registers hold four CTAs on an SM.  Single tokens by latency: 64 of 32 / 8 heads 4.8 us, one 3.4.
 #include <algorithm>
 #include <type_traits>
@@ -63,8 +63,8 @@ template <> struct Two<float> {
 };
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// HALF: pairs (i, i + n); WIDE: two elements of a lane lie side by side on their boundary, else they are taken one by one.
-template <typename T, int HD, bool HALF, bool WIDE>
+// HALF: pairs (i, i + n); WIDE: two elements of a lane lie side by side on their boundary, else they are taken one by one; STEP: most rows have a new token each.
+template <typename T, int HD, bool HALF, bool WIDE, bool STEP>
 __global__ void __launch_bounds__(32 * A8_WARPS, 4) append8_kernel(const __grid_constant__ Append8Args a) {
     constexpr int LANES = HD / 4, AT_ONCE = 32 / LANES;   // lanes of a token's head, tokens a warp has at once
     __shared__ float2 turns[PAGED_BLOCK][HD / 2];
@@ -218,19 +218,25 @@ __global__ void __launch_bounds__(32 * A8_WARPS, 4) append8_kernel(const __grid_
             }
         }
     };
-    // Single tokens have a text of their own: the block's unrolled one has to come to the instruction cache first, and took 7.8 us for 4.8 (64 rows, 32 / 8 heads; 512 rows
-    // 28 for 10.8; five prompts 18.4 for 20.0).
-    if (n <= AT_ONCE) heads(std::integral_constant<int, 1>{});
+    // Single tokens have a text of their own in steps: the block's unrolled one has to come to the instruction cache first, and took 7.8 us for 4.8 (64 rows, 32 / 8 heads; 512
+    // rows 28 for 10.8).  Other batches go without it: five prompts took 20.0 us with both for 18.4.
+    if (STEP && n <= AT_ONCE) heads(std::integral_constant<int, 1>{});
     else heads(std::integral_constant<int, PAGED_BLOCK / AT_ONCE>{});
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool STEP>
 int launch_append8(const Append8Args &a, bool half, bool wide, cudaStream_t s) {
     const dim3 grid(a.slots, a.parts);
-    auto kernel = half ? (wide ? append8_kernel<T, HD, true, true> : append8_kernel<T, HD, true, false>) : (wide ? append8_kernel<T, HD, false, true> : append8_kernel<T, HD, false, false>);
+    auto kernel = half ? (wide ? append8_kernel<T, HD, true, true, STEP> : append8_kernel<T, HD, true, false, STEP>)
+                       : (wide ? append8_kernel<T, HD, false, true, STEP> : append8_kernel<T, HD, false, false, STEP>);
     kernel<<<grid, 32 * A8_WARPS, 0, s>>>(a);
     AB2_LAUNCH_CHECK();
     return AB2_OK;
+}
+template <typename T>
+int launch_append8(const Append8Args &a, int head_dim, bool half, bool wide, cudaStream_t s) {
+    if (a.cache.tokens <= a.cache.rows) return head_dim == 128 ? launch_append8<T, 128, true>(a, half, wide, s) : launch_append8<T, 64, true>(a, half, wide, s);
+    return head_dim == 128 ? launch_append8<T, 128, false>(a, half, wide, s) : launch_append8<T, 64, false>(a, half, wide, s);
 }
 
 }  // namespace
@@ -263,13 +269,12 @@ AB2_API int ab2_paged_append_e4m3(const ab2_paged *cache, float *k_scales_dev, f
     AB2_REQUIRE(slots < (1ll << 31), AB2_ERR_BAD_SHAPE, "%d tokens of %d rows are more than one launch takes", cache->tokens, cache->rows);
     a.slots = (int)slots;
     // A CTA has all heads of a block where there are blocks enough for four CTAs on every SM, else fewer: a head a warp at least.  Sharing a block out makes its angles
-    // anew in every CTA: for 4 and 8 CTAs on an SM, us, five prompts of up to 2001 tokens 20.0 and 19.0, one of 8192 54.6 and 55.9.
+    // anew in every CTA: for 4 and 8 CTAs on an SM, us, five prompts of up to 2001 tokens 18.5 and 17.7, one of 8192 55 and 56.
     const int tasks = heads + 2 * cache->kv_heads, most = (tasks + A8_WARPS - 1) / A8_WARPS;
     const long long filled = std::max(1ll, cache->starts ? std::min<long long>(slots, cache->tokens / PAGED_BLOCK + cache->rows) : slots);
     a.parts = (int)std::min<long long>(std::min(most, 65535), std::max(1ll, (4ll * device_sm_count() + filled - 1) / filled));
     uintptr_t where = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.qo;
     const bool wide = a.pairs % 2 == 0 && where % (2 * es) == 0 && (a.q_stride | a.k_stride | a.v_stride | a.qo_stride) % 2 == 0, half = layout == AB2_ROTARY_HALF;
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == AB2_F32) return cache->head_dim == 128 ? launch_append8<float, 128>(a, half, wide, s) : launch_append8<float, 64>(a, half, wide, s);
-    return cache->head_dim == 128 ? launch_append8<__nv_bfloat16, 128>(a, half, wide, s) : launch_append8<__nv_bfloat16, 64>(a, half, wide, s);
+    return dtype == AB2_F32 ? launch_append8<float>(a, cache->head_dim, half, wide, s) : launch_append8<__nv_bfloat16>(a, cache->head_dim, half, wide, s);
 }
