@@ -282,8 +282,8 @@ __global__ void __launch_bounds__(32 * PM_WARPS, 2) paged_mma_kernel(const __gri
                 // The unit moves to a block's scale that is larger, or so much smaller that f16 would lose bits of its weights (but not to one whose values are
                 // nothing beside the others, as of a block of zeros).  The same for all lanes.
                 if (bs.y > vref || (bs.y < vref * PM_LESS && bs.y > vref * PM_NOTHING)) {
-                    const float f = vref / bs.y;
-                    vref = fmaxf(bs.y, 3.0092655e-36f);
+                    const float to = fmaxf(bs.y, 3.0092655e-36f), f = vref / to;   // 2^-118 at least, and the sums move by what the unit does
+                    vref = to;
                     vinv = PM_UP / vref;
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
