@@ -67,8 +67,8 @@ class LogitRules:
 
 @dataclass
 class Sampling:
-    """How a session's next token is drawn (``dispatch.sample``), by a generator of its own: sessions with equal seeds and logits draw equal tokens, whoever shares
-    their batch."""
+    """How a session's next token is drawn (``dispatch.sample``).  Settings alone, which sessions may share: a session draws by a generator of its own, which begins with
+    ``seed``, so that sessions with equal seeds and logits draw equal tokens, whoever shares their batch or these settings."""
     temperature: float = 1.0
     top_k: int = 0
     top_p: float = 1.0
@@ -80,12 +80,12 @@ class Sampling:
             raise _lib.Ab2Error(-7, f"a temperature of 0 or more, top-k of 0 or more, top-p and min-p from 0 to 1, got {self}")
         self._random = random.Random(self.seed)
 
-    def draw(self, logits: torch.Tensor) -> torch.Tensor:
-        """logits [1, vocab] -> the token [1]."""
-        numbers = torch.tensor([self.temperature, self.top_p, self.min_p], dtype=torch.float32).to(logits.device)
-        u = torch.tensor([self._random.random()], dtype=torch.float64).to(logits.device)
+    def draw(self, logits: torch.Tensor, numbers: random.Random | None = None) -> torch.Tensor:
+        """logits [1, vocab] -> the token [1], by the next of ``numbers`` (None: of a generator for calls that bring none)."""
+        rules = torch.tensor([self.temperature, self.top_p, self.min_p], dtype=torch.float32).to(logits.device)
+        u = torch.tensor([(numbers or self._random).random()], dtype=torch.float64).to(logits.device)
         top_k = torch.tensor([min(self.top_k, logits.shape[-1])], dtype=torch.int32).to(logits.device)
-        return sample(logits, u, numbers[0:1], top_k, numbers[1:2], numbers[2:3])
+        return sample(logits, u, rules[0:1], top_k, rules[1:2], rules[2:3])
 
 
 @dataclass
@@ -101,6 +101,7 @@ class GenerationSession:
     rules: LogitRules | None = None
     prompt_ids: list = field(default_factory=list)
     sampling: Sampling | None = None
+    numbers: random.Random | None = None      # what its tokens are drawn by, from the first draw on
 
     def is_finished(self) -> bool:
         return self.finished
@@ -192,7 +193,9 @@ class SessionEngine:
         logits = session.next_logits.view(1, -1)
         if session.rules is not None:
             logits = session.rules.apply(logits, session.prompt_ids, session.generated_ids)
-        token = int((argmax(logits) if session.sampling is None else session.sampling.draw(logits))[0])
+        if session.sampling is not None and session.numbers is None:
+            session.numbers = random.Random(session.sampling.seed)
+        token = int((argmax(logits) if session.sampling is None else session.sampling.draw(logits, session.numbers))[0])
         if token < 0:
             raise _lib.Ab2Error(-7, "no token of the session has a logit above -inf")
         if session.rules is not None and session.rules.allowed is not None and float(logits[0, token]) == -math.inf:
