@@ -68,7 +68,8 @@ class LogitRules:
 @dataclass
 class Sampling:
     """How a session's next token is drawn (``dispatch.sample``).  Settings alone, which sessions may share: a session draws by a generator of its own, which begins with
-    ``seed``, so that sessions with equal seeds and logits draw equal tokens, whoever shares their batch or these settings."""
+    ``seed``, so that sessions with equal seeds and logits draw equal tokens, whoever shares their batch or these settings.
+    A temperature of 0 gives what a greedy session takes, the last of equal maxima; with any other, tokens of equal logits go by index, the lower one first."""
     temperature: float = 1.0
     top_k: int = 0
     top_p: float = 1.0
@@ -81,8 +82,12 @@ class Sampling:
         self._random = random.Random(self.seed)
 
     def draw(self, logits: torch.Tensor, numbers: random.Random | None = None) -> torch.Tensor:
-        """logits [1, vocab] -> the token [1], by the next of ``numbers`` (None: of a generator for calls that bring none)."""
-        rules = torch.tensor([self.temperature, self.top_p, self.min_p], dtype=torch.float32).to(logits.device)
+        """logits [1, vocab] -> the token [1] (-1 where none is above -inf), by the next of ``numbers`` (None: of a generator for calls that bring none)."""
+        rules = torch.tensor([self.temperature, self.top_p, self.min_p], dtype=torch.float32)
+        if rules[0] == 0:   # in the sampler's 32 bits
+            seen = torch.where(logits > -math.inf, logits, -math.inf)   # NaN is never drawn
+            return torch.where(seen.amax(-1) > -math.inf, argmax(seen), -1)
+        rules = rules.to(logits.device)
         u = torch.tensor([(numbers or self._random).random()], dtype=torch.float64).to(logits.device)
         top_k = torch.tensor([min(self.top_k, logits.shape[-1])], dtype=torch.int32).to(logits.device)
         return sample(logits, u, rules[0:1], top_k, rules[1:2], rules[2:3])
