@@ -400,8 +400,8 @@ def _paged(k_pages, v_pages, table, lens, starts, tokens: int):
 def _scales(scales, k_pages, v_pages):
     """The scales of keys and of values where pages hold 8 bits; (None, None) where they do not."""
     codes = k_pages.dtype is torch.float8_e4m3fn
-    if scales is not None and (not isinstance(scales, (tuple, list)) or len(scales) != 2):
-        raise _lib.Ab2Error(-7, "scales are a pair, those of keys and those of values")
+    if scales is not None and (not isinstance(scales, (tuple, list)) or len(scales) != 2 or not all(isinstance(t, torch.Tensor) for t in scales)):
+        raise _lib.Ab2Error(-7, "scales are a pair of tensors, those of keys and those of values")
     if codes != (scales is not None):
         raise _lib.Ab2Error(-7, "pages of float8_e4m3fn need scales" if codes else f"pages of {k_pages.dtype} have no scales")
     if not codes:
