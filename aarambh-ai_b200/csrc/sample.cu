@@ -946,7 +946,7 @@ AB2_API int ab2_sample(const void *logits_dev, long long stride, int rows, int v
     a.logits = logits_dev; a.stride = stride; a.vocab = vocab; a.uniforms = uniforms_dev; a.uniforms_64 = uniforms_64;
     a.temperature = temperature_dev; a.top_k = top_k_dev; a.top_p = top_p_dev; a.min_p = min_p_dev; a.out = out_dev;
     a.shift = 44;
-    while (((long long)vocab << a.shift) > (1ll << 61)) --a.shift;
+    while (vocab > (1ll << 61 >> a.shift)) --a.shift;   // a row's weights add up to 2^61 at most
     switch (dtype) {
     case AB2_F32: return launch_sample<float>(a, rows, (cudaStream_t)stream);
     case AB2_F16: return launch_sample<__half>(a, rows, (cudaStream_t)stream);
