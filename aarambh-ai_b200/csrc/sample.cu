@@ -4,9 +4,9 @@
 //   top-k: the first k stay;  top-p: of these the shortest prefix whose mass is p of theirs or more;  min-p: of these the ones with p_v >= min_p
 //   the token: the first one that stayed, in order of index, whose cumulative mass exceeds u times all of theirs
 //
-// Weights are whole numbers, round(2^F p_v) with F up to 44, off by 2^-30.4 of themselves (quick_weight): their sums are exact whatever the order, so that every run and
-// every way of dealing the row out draws the same token, and a border between two tokens lies within that and 2^-45 a token of where real numbers have it (f32 sums would
-// move it by more than a token's width in large vocabularies).
+// Weights are whole numbers, round(2^F p_v), off by 2^-30.4 of themselves (quick_weight) and half of one: their sums are exact whatever the order, so that every run and
+// every way of dealing the row out draws the same token, and a border between two tokens lies within that and 2^-(F + 1) a token of where real numbers have it (f32 sums would
+// move it by more than a token's width in large vocabularies).  F is 44 up to 2^17 tokens and one less for every doubling beyond: a row's sum stays below 2^61.
 //
 // A cluster of CTAs has a row, each a slice of it, which it keeps in shared memory.  Most rows are decided by a few tokens: with top-k or min-p a logit is found that all
 // which can stay reach (of the threads' largest ones, sorted, the one of which k reach it), what reaches it goes to the first CTA's list, which is sorted, cut and

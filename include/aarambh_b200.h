@@ -413,8 +413,10 @@ int ab2_paged_attention_window(const ab2_paged *cache, int window, int sinks, co
  * Tokens that are cut off a row leave its last block's scale as they made it, and what their coming rounded off the others' codes.
  *
  * The attention reads the scales of blocks that hold keys in sight, finite ones and not negative; those that the append writes are taken as they are, of scales that are not powers of two a
- * chunk's values are rounded to f16 (2^-11) in units of the largest of some 80 keys.  Over bf16 queries weights are rounded to f16 (2^-11 each); the
- * queries of chunks (new tokens times query heads of a KV head above 16) enter in two e4m3 terms, off by 2^-17.8 of the row's largest element at most. */
+ * chunk's values are rounded to f16 (2^-11) in units of the largest of some 80 keys.  A block whose scale of values is 2^-60 of one before it or less, or 2^-100 or less beside larger
+ * ones, may count as zeros.  Over bf16 queries weights are rounded to f16 (2^-11 each).  The queries that the kernel of chunks answers enter in two e4m3 terms, off by 2^-17.8 of the
+ * row's largest element at most: those of rows with new tokens times query heads of a KV head above 16 and, in a call that may have such rows (by max_new) and up to 64 rows times KV
+ * heads (heads of 64: 32), all others of the call.  Single tokens by themselves enter exactly, but for what is 2^-39 of the row's largest element. */
 int ab2_paged_append_e4m3(const ab2_paged *cache, float *k_scales_dev, float *v_scales_dev, const void *k_dev, long long k_stride, const void *v_dev,
                           long long v_stride, const void *q_dev, long long q_stride, int heads, void *q_out_dev, long long q_out_stride,
                           const double *frequencies_dev, int rot_dims, int layout, float magnitude, ab2_dtype dtype, ab2_stream stream);
@@ -437,7 +439,8 @@ int ab2_adjust_logits(const void *logits_dev, long long stride, int rows, int vo
  * whose cumulative mass exceeds u times the mass of all that stayed, u the row's number of uniforms_dev (f32, or with uniforms_64 f64; 0 <= u < 1).  A temperature
  * that is not positive gives the likeliest token.  NaN and -inf are never drawn; a row without another logit answers -1.  temperature_dev, top_k_dev, top_p_dev and
  * min_p_dev are [rows], or NULL for 1, 0, 1 and 0.  Each p is off by
- * 2^-30 of itself and 2^-45 of the largest at most and they are summed exactly, as whole numbers: equal inputs give equal tokens.  Up to 2^24 tokens. */
+ * 2^-30 of itself and 2^-(F + 1) of the largest at most, F = 44 up to 2^17 tokens and one less for every doubling beyond (37 at 2^24, where tokens 2^-38 of the largest and less
+ * are never drawn); they are summed exactly, as whole numbers: equal inputs give equal tokens.  Up to 2^24 tokens. */
 int ab2_sample(const void *logits_dev, long long stride, int rows, int vocab, const void *uniforms_dev, int uniforms_64, const float *temperature_dev,
                const int *top_k_dev, const float *top_p_dev, const float *min_p_dev, int *out_dev, ab2_dtype dtype, ab2_stream stream);
 
