@@ -121,7 +121,7 @@ template <bool WIN> __device__ __forceinline__ bool pc_next(const PagedPlan &a, 
 
 struct PcTile {   // of codes
     float k[PC_KEYS / PC_ROWS], v;    // scales of the blocks of keys, and the unit of the values
-    __half2 f[PC_KEYS / PC_ROWS];     // scales of the blocks of values in that unit
+    __half2 f[PC_KEYS / PC_ROWS];     // scales of the blocks of values in that unit; those far below it times -PC_FAR
     int rows;                         // that the piece has of it; negative: there is no more tile
     uint32_t blocks;                  // a bit for each that a token sees
 };
@@ -130,6 +130,7 @@ template <int SLOTS, int RAWS, int THREADS> struct PcShared {
     uint64_t full[SLOTS], empty[SLOTS], qfull[2], sfull[2], sfree[2], pfull[2], odone[2], rfull[RAWS ? RAWS : 1], rempty[RAWS ? RAWS : 1];
     uint32_t tmem_base;
     int failed;
+    float lost;   // of codes: how far a value may be off at most, of blocks far below their tile's unit
     union {
         struct {                                // while the CTA looks for its run
             long long warp_sums[THREADS / 32];
@@ -269,9 +270,11 @@ __device__ __forceinline__ void exchange4(uint4 (&o)[4], int lane) {
 // Over codes keys are multiplied as they are, with queries in two e4m3 terms: a bf16 number has 8 significant bits, and is the sum of two of 4 (in units of a power of two of
 // its row's that puts the largest at 224 to 448; below 2^-2 the second term has fewer: 2^-18 of the row's largest element off at most).  A block's scale multiplies its scores beside the
 // softmax's factor.  Values are f16, in units of the tile's largest scale (a block's other scale is a power of two below it, and exact down to 2^-15); their weights are f16 in units of `vref`, a
-// scale of values that moves as the maximum does: up to one over 4 times it (2^8 of a weight, 4 and PC_UP make 2^15), down where f16 would lose bits of them.  A tile whose scales of values lie too far apart has NaN for its unit:
-// the sums of all its rows become NaN, and they are computed again in f32 like those that meet NaN.
-constexpr float PC_UP = 32.f, PC_MORE = 4.f, PC_LESS = 9.765625e-4f, PC_APART = 3.0517578e-5f, PC_NOTHING = 8.6736174e-19f, PC_ZEROS = 7.8886091e-31f;   // 2^-10, 2^-15, 2^-60, 2^-100
+// scale of values that moves as the maximum does: up to one over 4 times it (2^8 of a weight, 4 and PC_UP make 2^15), down where f16 would lose bits of them.  Values of a block further
+// below its tile's largest than 2^-15 are rounded to 2^-24 of the unit, and the producer notes by how much they may be off: rows whose largest output is not 2^20 times that, as of those that see hardly anything else, are computed
+// again in f32 like those that meet NaN.  (With all rows of such a tile computed again one block of 2^-20 among 1000 took 4096 behind 12288 from 1.0 ms to 475; with bf16 for both operands of such a tile
+// all others took 2 to 8 % longer.  This takes 1.12 ms of it, and of 4096 behind 12288 without such blocks nothing, with heads of 64 4 %.)
+constexpr float PC_UP = 32.f, PC_MORE = 4.f, PC_LESS = 9.765625e-4f, PC_APART = 3.0517578e-5f, PC_NOTHING = 8.6736174e-19f, PC_ZEROS = 7.8886091e-31f, PC_FAR = 4096.f, PC_ENOUGH = 1048576.f;   // 2^-10, 2^-15, 2^-60, 2^-100, 2^20
 // What a row's warp keeps of the values' scales: the unit of the sums, and of the tile before its scale, what that adds to a weight's exponent, and its inverse as a factor.
 struct PcUnit {
     float vref, last, more, less;
@@ -359,7 +362,6 @@ __device__ __forceinline__ void pc_softmax_codes(uint32_t s_addr, uint32_t o_add
     }
     total[0] = add2(total[0], total[1]);
     sum = fmaf(low(total[0]) + high(total[0]), unit.less, sum);
-    if (values != values) sum = values;
     asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncwarp();
@@ -386,6 +388,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         for (int i = 0; i < S::RAWS; ++i) { bar_init(&sh.rfull[i], 1); bar_init(&sh.rempty[i], PC_LOAD / 32); }
         for (int i = 0; i < 2; ++i) { bar_init(&sh.qfull[i], 4); bar_init(&sh.sfull[i], 1); bar_init(&sh.sfree[i], 4); bar_init(&sh.pfull[i], 4); bar_init(&sh.odone[i], 1); }
         sh.failed = 0;
+        sh.lost = 0.f;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     pdl_wait();   // ahead of tensor memory too, which the launch before may hold
@@ -425,11 +428,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 #pragma unroll 1
             for (int r = row0; r < PC_KEYS; r += ROWS) {
                 const __half2 f = tile.f[r / PC_ROWS];
+                const bool far = *reinterpret_cast<const int *>(&f) < 0;   // the same for all lanes
                 uint4 c = make_uint4(0u, 0u, 0u, 0u);   // behind the piece's keys, and where no token sees a block
                 if (r < rows && ((blocks >> (r / PC_ROWS)) & 1)) c = *reinterpret_cast<const uint4 *>(from + raw * S::RAW + (r - row0) * HD);
                 auto two = [&](uint32_t codes) {
                     const uint32_t h = f16x2_of_codes(codes);
-                    const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&h), f);
+                    __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&h), f);
+                    if (far) y = __hmul2(y, __float2half2_rn(-1.f / PC_FAR));
                     return *reinterpret_cast<const uint32_t *>(&y);
                 };
                 const uint4 low8 = make_uint4(two(c.x), two(c.x >> 16), two(c.y), two(c.y >> 16)), high8 = make_uint4(two(c.z), two(c.z >> 16), two(c.w), two(c.w >> 16));
@@ -449,6 +454,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         if (E8 && warp == 0) {
             // ---------------------------------------------------------- producer over codes: V, as codes, then K
             int n = 0;
+            float lost = 0.f;
             while (pc_next<WIN>(a.plan, run, x)) {
                 const PagedHole hole = paged_hole<WIN>(a.plan, x.s.base, x.w.q_tile);
                 for (int j = 0; j < x.most(); ++j, ++n) {
@@ -462,8 +468,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     float unit = vs;
 #pragma unroll
                     for (int m = 1; m < 8; m <<= 1) unit = fmaxf(unit, __shfl_xor_sync(0xffffffffu, unit, m));
-                    const __half2 f = __float2half2_rn(unit > 0.f ? vs / unit : 0.f);
-                    if (__any_sync(0xffffffffu, lane < 8 && vs < unit * PC_APART && vs > PC_ZEROS)) unit = __uint_as_float(0x7fc00000u);
+                    const float part = unit > 0.f ? vs / unit : 0.f;
+                    const bool far = part < PC_APART && vs > PC_ZEROS;
+                    const __half2 f = __float2half2_rn(far ? part * -PC_FAR : part);
                     warp_wait(&sh.rempty[raw], ((n / RAWS) & 1) ^ 1, failed);
                     PcTile &tile = sh.tiles[n % TILES];
                     if (lane < PC_KEYS / PC_ROWS) { tile.k[lane] = ks; tile.f[lane] = f; }
@@ -472,6 +479,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     if (lane == 0) bar_expect_tx(&sh.rfull[raw], (uint32_t)bytes);
                     __syncwarp();
                     if (mine && !*failed) bulk_copy(codes + raw * S::RAW + lane * PC_ROWS * HD, (const uint8_t *)a.v + row * HD, PC_ROWS * HD, &sh.rfull[raw]);
+                    if (__any_sync(0xffffffffu, far)) {   // behind the values' copies; the keys' barrier hands it on to those that read it
+                        float off = far ? unit * fminf(2.9802322e-8f, 448.f * part) : 0.f;   // half of f16's least step, or all of the value
+#pragma unroll
+                        for (int m = 1; m < 8; m <<= 1) off = fmaxf(off, __shfl_xor_sync(0xffffffffu, off, m));
+                        if (lane == 0 && off > lost) sh.lost = lost = off;
+                    }
                     warp_wait(&sh.empty[slot], ((n / S::SLOTS) & 1) ^ 1, failed);
                     if (lane == 0) bar_expect_tx(&sh.full[slot], (uint32_t)bytes);
                     __syncwarp();
@@ -729,7 +742,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             const bool all = w.k0 == 0 && w.k1 == w.k_tiles;
             const size_t slot = (2 * (size_t)blockIdx.x + (w.k0 == 0)) * a.tile_rows;
-            const float f = !all ? (E8 && sum != sum ? sum : of_sums) : sum == 0.f ? 0.f : of_sums / sum;
+            const float f = !all ? of_sums : sum == 0.f ? 0.f : of_sums / sum;
             float poison = 0.f;  // stays 0 unless an output is Inf or NaN
             // A lane has a row, 16 bytes of which at a time would go to 32 places: four lanes exchange pieces and store 64 bytes of a row each time.
             __nv_bfloat16 *dst[4];
@@ -794,7 +807,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         }
         // Rows to compute again, found by what has been stored of them.  Behind the last piece: it may take long, and until then other roles would wait for these
         // warps at barriers whose waits are bounded.
-        if (again) {
+        const float lost = E8 ? __shfl_sync(0xffffffffu, *(const volatile float *)&sh.lost, 0) : 0.f;   // of the tiles that these warps' rows have seen, and it may be others
+        if (again || lost > 0.f) {
             PagedRun walk = sh.start;
             PcPiece x;
             while (pc_next<WIN>(a.plan, walk, x)) {
@@ -803,7 +817,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 const bool all = x.w.k0 == 0 && x.w.k1 == x.w.k_tiles;
                 const size_t slot = (2 * (size_t)blockIdx.x + (x.w.k0 == 0)) * a.tile_rows;
                 uint32_t worst = 0;   // of the exponents
+                float least = 0.f;    // that the largest element has to reach
                 if (rr < rows) {
+                    if (E8) least = lost * PC_ENOUGH * (all ? 1.f : a.ml[(slot + rr) * 2 + 1]);
                     const int tok = paged_token(a.plan, rr);
                     const uint32_t *o = all ? (const uint32_t *)((const __nv_bfloat16 *)a.out + (size_t)(x.w.r.first + x.s.t0 + tok) * a.o_stride + (size_t)(x.w.head * group + rr - tok * group) * HD)
                                             : (const uint32_t *)(a.acc + (slot + rr) * HD);
@@ -812,7 +828,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         if (all) worst = max(worst, (o[i] & 0x7f80u) << 16);
                     }
                 }
-                for (uint32_t left = __ballot_sync(0xffffffffu, worst == 0x7f800000u); left; left &= left - 1)
+                for (uint32_t left = __ballot_sync(0xffffffffu, worst == 0x7f800000u || (E8 && __uint_as_float(worst) < least)); left; left &= left - 1)
                     paged_again<HD, Page, WIN>(a, x.w, x.s, g * PC_Q + quad * 32 + __ffs(left) - 1, lane, all, slot);
                 __syncwarp();
             }

@@ -414,7 +414,8 @@ int ab2_paged_attention_window(const ab2_paged *cache, int window, int sinks, co
  *
  * The attention reads the scales of blocks that hold keys in sight, finite ones and not negative; those that the append writes are taken as they are, of scales that are not powers of two a
  * chunk's values are rounded to f16 (2^-11) in units of the largest of some 80 keys.  A block whose scale of values is 2^-60 of one before it or less, or 2^-100 or less beside larger
- * ones, may count as zeros.  Over bf16 queries weights are rounded to f16 (2^-11 each).  The queries that the kernel of chunks answers enter in two e4m3 terms, off by 2^-17.8 of the
+ * ones, may count as zeros.  A chunk's values of blocks 2^-16 and less below the largest scale of those keys are rounded to 2^-24 of that, and a row's answer is off by 2^-20 of its largest element by it at
+ * most: rows for which that would not hold, which see hardly any other block, are computed again in f32, at some hundred times the cost.  Over bf16 queries weights are rounded to f16 (2^-11 each).  The queries that the kernel of chunks answers enter in two e4m3 terms, off by 2^-17.8 of the
  * row's largest element at most: those of rows with new tokens times query heads of a KV head above 16 and, in a call that may have such rows (by max_new) and up to 64 rows times KV
  * heads (heads of 64: 32), all others of the call.  Single tokens by themselves enter exactly, but for what is 2^-39 of the row's largest element. */
 int ab2_paged_append_e4m3(const ab2_paged *cache, float *k_scales_dev, float *v_scales_dev, const void *k_dev, long long k_stride, const void *v_dev,
