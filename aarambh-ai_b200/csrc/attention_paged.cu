@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(PA_THREADS, SimtShape<HD, QR>::CTAS) paged_sim
     float *qs = (float *)(smem + (E8 ? 2 * S::BUF + 4 * S::RAW : 4 * S::BUF)), *ps = qs + QR * KROW;
     const int tx = threadIdx.x % TX, row0 = threadIdx.x / TX * S::FIRST;
     const PagedView &p = a.plan.p;
-    PagedRun run = paged_run<PA_THREADS, WIN>(a.plan, blockIdx.x, gridDim.x, warp_sums, found, a.status);
+    PagedRun run = paged_run<PA_THREADS, WIN, QR == 8>(a.plan, blockIdx.x, gridDim.x, warp_sums, found, a.status);
     if (threadIdx.x == 0) paged_uncut(a, blockIdx.x);
     PagedPiece w;
     while (paged_next<WIN>(a.plan, run, w)) {
