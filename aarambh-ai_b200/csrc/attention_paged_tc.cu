@@ -18,8 +18,8 @@
 // weights.  Scores, maxima, sums and O are f32.  The weights are relative to a maximum per row that moves only when a score exceeds it by 2^8; then O is
 // rescaled in tensor memory.
 //
-// 4096 tokens behind 12288, 32 / 8 heads of 128: 0.92 ms, 1.05 PFLOP/s, 0.63 of cuBLAS in a burst and 0.75 of it sustained; 2048 behind 2048 120 us;
-// six rows of 1 to 512 tokens behind up to 5000 134 us; 4096 behind 12288, 16 / 4 heads of 64, 0.41 ms.  A tile of 80 keys takes some 2300 clocks, of which both tiles'
+// 4096 tokens behind 12288, 32 / 8 heads of 128: 0.78 to 0.92 ms, by the card and for how long it runs (the power cap): 1.05 PFLOP/s and more, 0.63 of cuBLAS in a burst and 0.75 of it sustained; 2048 behind
+// 2048 116 us; six rows of 1 to 512 tokens behind up to 5000 122 to 134 us; 4096 behind 12288, 16 / 4 heads of 64, 0.39 ms.  A tile of 80 keys takes some 2300 clocks, of which both tiles'
 // exponentials (2 x 128 x 80, at 16 a clock) need 1280 and the products 1432; no pipe is full (1024 behind 3000 by counters: exponentials 42 %, tensor pipe 42 %, issue
 // slots 36 %).  What bounds it is the chain of a softmax warp: scores from tensor memory, the maximum, the last tile's products, exponentials, weights back.
 //
@@ -31,7 +31,8 @@
 //   warp 0       producer: values as codes by bulk copies to a ring of their own, keys by TMA as the operand of an e4m3 product, with queries in two terms
 //   warps 4-11   softmax, with the scales of keys on the scores and of values on the weights (f16)
 //   warps 12-15  values from codes to f16, in the ring's slots
-// 4096 behind 12288 0.99 ms (bf16 pages 0.81 to 0.87), six mixed rows 150 us (123), 1024 behind 1024 60 (51); through a window of 1024 8000 tokens of 16 / 4 heads behind 5000 172 (134).
+// In one run, bf16 pages in brackets: 4096 behind 12288 1.00 to 1.04 ms (0.78 to 0.88), six mixed rows 151 us (122), 1024 behind 1024 60 (51), 4096 behind 12288 of 16 / 4 heads of 64 0.52 ms (0.39);
+// through a window of 1024 8000 tokens of 16 / 4 heads behind 5000 174 us (135).
 // What it costs more, by copies that leave a part out: making values f16 45 us of 4096 behind 12288, the scales in the softmax 30 or so; the rest is not taken apart.
 // Measured and not kept there: queries in one term (no faster, 2^-4), keys and values both made f16 by warps (1465 us; 1153 with the scales beside the softmax's), values loaded to
 // registers a tile ahead and converted by unrolled code (1150: its text drives the softmax's out of the instruction cache), the next tile's table and scales asked for ahead (no change).

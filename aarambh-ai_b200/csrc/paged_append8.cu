@@ -10,8 +10,9 @@
 // A CTA has a block's new tokens (or, where blocks are few, a part of their heads): it turns their angles once into shared memory, and each warp takes heads of q,
 // k and v one after the other.  A block's scale is its warp's alone: no atomics, no order.  Heads of keys and values stay in registers from the load to the codes.
 //
-// Bound by HBM for prompts, and by the instructions of a block: five of up to 2001 tokens, 16 / 4 heads of 128 (66 MB), 18.4 us, 3.6 TB/s; one of 8192, 32 / 8 heads, 55, 3.4; issue
-// slots are 44 % busy, and shared memory and registers hold four CTAs on an SM.  Single tokens by latency: 64 of 32 / 8 heads 4.8 us, one 3.4.
+// Bound by the instructions of a block for prompts, ahead of HBM: issue slots are 44 % busy, and shared memory and registers hold four CTAs on an SM.  Five of up to 2001 tokens, 16 / 4 heads of
+// 128 (66 MB), take 24.4 us among other calls, 2.7 TB/s, and 18.4 back to back, where L2 still holds half of it; one of 8192, 32 / 8 heads (185 MB), 48, 3.8 TB/s.  Single tokens by latency: 64 of
+// 32 / 8 heads 4.8 us, one 3.4.
 #include <algorithm>
 #include <type_traits>
 
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(32 * A8_WARPS, 4) append8_kernel(const __grid_
         }
     };
     // Single tokens have a text of their own in steps: the block's unrolled one has to come to the instruction cache first, and took 7.8 us for 4.8 (64 rows, 32 / 8 heads; 512
-    // rows 28 for 10.8).  Other batches go without it: five prompts took 20.0 us with both for 18.4.
+    // rows 28 for 10.8).  Other batches go without it: five prompts took 20.0 us with both for 18.4, back to back.
     if (STEP && n <= AT_ONCE) heads(std::integral_constant<int, 1>{});
     else heads(std::integral_constant<int, PAGED_BLOCK / AT_ONCE>{});
 }

@@ -14,9 +14,9 @@
 // border's bin is found by the bins' exact masses, and the token by one more pass, in which the CTAs join their sums.  Where a bin has more tokens than the list takes
 // (thousands of equal logits) its border is found by halving keys.
 //
-// Bound by its passes over the slice: instructions, not HBM, which a row crosses once.  64 rows of 128256 bf16 logits (16.4 MB, 2.5 us at a copy's rate), us: top-k of 50 or min-p 18,
-// unfiltered 28 (a weight a token, some 25 instructions), top-p of 0.9 50, of which counts of logits and the pass that weighs are two (bins of x, weighed twice and masses joined by carries: 103),
-// all kinds of rules in a batch 50; 4 rows of 32000 f32: 7, 10 to 12, 27, 16.  Weights looked up in a table by their logit instead of computed: 49 for 50, and unfiltered 36 for 28 (its reads of 8
+// Bound by its passes over the slice: instructions, not HBM, which a row crosses once.  64 rows of 128256 bf16 logits (16.4 MB, 2.5 us at a copy's rate), us: top-k of 50 or min-p 20,
+// unfiltered 31 (a weight a token, some 25 instructions), top-p of 0.9 51, of which counts of logits and the pass that weighs are two (bins of x, weighed twice and masses joined by carries: 103),
+// all kinds of rules in a batch 51; 4 rows of 32000 f32: 8, 12 to 13, 29, 18.  Weights looked up in a table by their logit instead of computed: 49 for 50, and unfiltered 36 for 28 (its reads of 8
 // bytes meet in banks).
 #include <algorithm>
 #include <type_traits>
